@@ -478,6 +478,51 @@ int pimhip_rnnt_greedy_decode(PimHipRnntPlan* plan, const void* enc, int64_t n_f
 int pimhip_rnnt_plan_fallbacks(PimHipRnntPlan* plan, uint64_t* events, int* exchanging);
 int pimhip_rnnt_plan_set_spin_limit(PimHipRnntPlan* plan, unsigned int spin_limit);
 
+/* ---- microscaled 4-bit matrices ----------------------------------------------------------------- */
+
+/* No counterpart in the reference, whose weights are fp16: 4-bit floating point (E2M1: +-{0, 0.5, 1, 1.5, 2, 3, 4, 6}) in blocks of 32
+ * values of a row that share an 8-bit scale 2^(code - 127), the OCP microscaling format MXFP4.  Less than a third of fp16's bytes, which
+ * is what a product for one token is made of. */
+
+/* Element types of the entry points below. */
+typedef enum PimHipDataType { PIMHIP_F16 = 0, PIMHIP_BF16 = 1, PIMHIP_F32 = 2 } PimHipDataType;
+
+/* A [rows, cols] matrix in that format, in the caller's device memory (this struct itself lies on the host):
+ *   packed  rows of ceil(cols / 32) * 16 bytes, densely packed, 16-byte aligned: two values a byte, the first in the low half; the last
+ *           block of a row is filled up with zeros
+ *   scales  rows of ceil(cols / 32) codes with a pitch of ld_scales bytes (a multiple of 16), 16-byte aligned; code 255 is "not a
+ *           number" and makes its block's values NaN; bytes behind a row's last block may hold anything
+ *   tops    [rows]: the largest scale code of each row, codes 255 apart (pimhip_mx4_quantize and pimhip_mx4_find_tops write it) */
+typedef struct PimHipMx4Matrix {
+    const void* packed;
+    const void* scales;
+    const void* tops;
+    int64_t rows, cols, ld_scales;
+} PimHipMx4Matrix;
+
+/* Quantises x [out->rows, out->cols] (dtype: any PimHipDataType; pitch ld_x elements) into the memory `out` names.  A block's scale is the
+ * largest power of two not above its largest magnitude, divided by 4 (2^-127 at least); its values are rounded to the nearest
+ * element, ties to the one with an even code, and saturate at 6.  A block that holds an infinity or a NaN gets scale code 255.
+ * Equal inputs give equal bytes. */
+int pimhip_mx4_quantize(const PimHipMx4Matrix* out, const void* x, int dtype, int64_t ld_x, void* stream);
+
+/* Writes m->tops from m->scales: for a matrix whose bytes come from elsewhere. */
+int pimhip_mx4_find_tops(const PimHipMx4Matrix* m, void* stream);
+
+/* out [rows, cols] (dtype, pitch ld_out elements) = the values m stands for, each rounded once to dtype. */
+int pimhip_mx4_dequantize(void* out, int dtype, int64_t ld_out, const PimHipMx4Matrix* m, void* stream);
+
+/* out[t, n] = act(sum_k x[t, k] * weight[n, k] + bias[n]) for `tokens` rows of x (dtype PIMHIP_F16 or PIMHIP_BF16, pitch ld_x; out and
+ * bias are of the same type, bias may be NULL, act a PimHipActFunc).  Weights are converted to dtype on the way to the matrix cores:
+ * exactly in bfloat16; in fp16 relative to the row's largest scale, where values below 2^-38 of the row's largest lose bits.
+ * Sums in fp32, one rounding at the store.  Any sizes, pitches and element-aligned addresses. */
+int pimhip_mx4_linear(void* out, int64_t ld_out, const void* x, int64_t ld_x, int dtype, int64_t tokens, const PimHipMx4Matrix* weight,
+                      const void* bias, int act, void* stream);
+
+/* out[m, n] = sum_k a[m, k] * b[n, k], both operands in 4 bits (dtype: any PimHipDataType, pitch ld_out).  Products are exact, sums
+ * fp32, one rounding at the store. */
+int pimhip_mx4_matmul(void* out, int64_t ld_out, int dtype, const PimHipMx4Matrix* a, const PimHipMx4Matrix* b, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

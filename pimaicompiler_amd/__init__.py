@@ -36,3 +36,4 @@ from .ops import (  # noqa: F401
     synchronize_and_check,
     set_gemv_spin_limit,
 )
+from .mx4 import Mx4Tensor, mx4_dequantize, mx4_linear, mx4_matmul, mx4_quantize  # noqa: F401

@@ -13,6 +13,15 @@ c_void_pp = ctypes.POINTER(ctypes.c_void_p)
 c_int64_p = ctypes.POINTER(ctypes.c_int64)
 c_int_p = ctypes.POINTER(ctypes.c_int)
 
+
+class Mx4Matrix(ctypes.Structure):
+    """PimHipMx4Matrix."""
+    _fields_ = [("packed", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("tops", ctypes.c_void_p), ("rows", ctypes.c_int64),
+                ("cols", ctypes.c_int64), ("ld_scales", ctypes.c_int64)]
+
+
+c_mx4_p = ctypes.POINTER(Mx4Matrix)
+
 # name -> (restype, argtypes); must list every function include/pimhip.h declares.
 SIGNATURES = {
     "pimhip_initialize": (ctypes.c_int, [ctypes.c_int]),
@@ -97,6 +106,12 @@ SIGNATURES = {
                                                      ctypes.c_void_p]),
     "pimhip_input_projection_packed": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                                       ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p]),
+    "pimhip_mx4_quantize": (ctypes.c_int, [c_mx4_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p]),
+    "pimhip_mx4_find_tops": (ctypes.c_int, [c_mx4_p, ctypes.c_void_p]),
+    "pimhip_mx4_dequantize": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, c_mx4_p, ctypes.c_void_p]),
+    "pimhip_mx4_linear": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int64,
+                                         c_mx4_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
+    "pimhip_mx4_matmul": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, c_mx4_p, c_mx4_p, ctypes.c_void_p]),
 }
 
 # Status codes and enums of include/pimhip.h.
@@ -110,6 +125,7 @@ PIMHIP_ACT_NONE = 0
 PIMHIP_ACT_RELU = 1
 PIMHIP_I_X_W = 0
 PIMHIP_W_X_I = 1
+PIMHIP_F16, PIMHIP_BF16, PIMHIP_F32 = 0, 1, 2
 GEMM_UNKNOWN, GEMM_VV, GEMM_MV, GEMM_VM, GEMM_MM = 0, 1, 2, 3, 4
 
 _lib = None

@@ -1,0 +1,176 @@
+// Microscaled 4-bit matrices of the C ABI (include/pimhip.h): quantisation, reading back, and the products with one or both operands in 4 bits.
+#include "api_common.h"
+#include "mx4_kernels.h"
+
+using namespace pimhip;
+
+namespace
+{
+constexpr int64_t kMaxCols = 1 << 30;
+
+int check_matrix(const char* name, const PimHipMx4Matrix* m, Mx4View* v)
+{
+    if (!m) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "%s is null", name);
+    if (m->rows < 0 || m->cols < 1 || m->cols > kMaxCols)
+        return fail(PIMHIP_ERR_INVALID_ARGUMENT, "%s: rows=%lld, cols=%lld (cols in [1, %lld])", name, (long long)m->rows, (long long)m->cols, (long long)kMaxCols);
+    const int64_t blocks = (m->cols + kMxBlock - 1) / kMxBlock;
+    if (m->ld_scales < blocks || (m->ld_scales & 15))
+        return fail(PIMHIP_ERR_INVALID_ARGUMENT, "%s: ld_scales=%lld must be a multiple of 16 and at least %lld", name, (long long)m->ld_scales, (long long)blocks);
+    if (m->rows && (!m->packed || !m->scales || !m->tops)) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "%s: packed, scales and tops must be non-null", name);
+    if (!aligned16(m->packed) || !aligned16(m->scales)) return fail(PIMHIP_ERR_UNSUPPORTED, "%s: packed and scales must be 16-byte aligned", name);
+    *v = Mx4View{(const uint8_t*)m->packed, (const uint8_t*)m->scales, (const uint8_t*)m->tops, m->rows, m->cols, m->ld_scales};
+    return PIMHIP_OK;
+}
+
+int check_element(const char* name, const void* p, int dtype, bool fp32_too)
+{
+    if (dtype != PIMHIP_F16 && dtype != PIMHIP_BF16 && !(fp32_too && dtype == PIMHIP_F32)) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "dtype=%d", dtype);
+    if (!p) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "%s is null", name);
+    if (reinterpret_cast<uintptr_t>(p) & (dtype == PIMHIP_F32 ? 3u : 1u)) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "%s is not aligned to its elements", name);
+    return PIMHIP_OK;
+}
+
+// The two-dimensional grid of a product: row groups by token groups.
+int check_grid(int64_t x, int64_t y)
+{
+    if (x > INT32_MAX || y > 65535) return fail(PIMHIP_ERR_UNSUPPORTED, "the product is too large for one launch (%lld x %lld workgroups)", (long long)x, (long long)y);
+    return PIMHIP_OK;
+}
+
+template <class T, int RT, int TT, int U, int WK>
+int linear_skinny(void* out, int64_t ld_out, const void* x, int64_t ld_x, int64_t M, const Mx4View& w, const void* bias, int relu, hipStream_t s)
+{
+    const int64_t gx = (w.rows + 16 * RT - 1) / (16 * RT), gy = (M + 16 * TT - 1) / (16 * TT);
+    const int rc = check_grid(gx, gy);
+    if (rc != PIMHIP_OK) return rc;
+    mx4_linear_skinny_kernel<T, RT, TT, U, WK><<<dim3((unsigned)gx, (unsigned)gy), 64 * WK, 0, s>>>(
+        (const typename T::elem*)x, w, (const typename T::elem*)bias, (typename T::elem*)out, ld_x, ld_out, M, relu);
+    return PIMHIP_OK;
+}
+
+template <class T>
+int linear(void* out, int64_t ld_out, const void* x, int64_t ld_x, int64_t M, const Mx4View& w, const void* bias, int relu, hipStream_t s)
+{
+    if (M <= 16) return linear_skinny<T, 1, 1, 2, 4>(out, ld_out, x, ld_x, M, w, bias, relu, s);
+    if (M <= 32) return linear_skinny<T, 1, 2, 1, 4>(out, ld_out, x, ld_x, M, w, bias, relu, s);
+    return linear_skinny<T, 1, 4, 1, 4>(out, ld_out, x, ld_x, M, w, bias, relu, s);
+}
+
+template <class O>
+int matmul(void* out, int64_t ld_out, const Mx4View& a, const Mx4View& b, hipStream_t s)
+{
+    auto run = [&](auto kernel, int RT, int TT, int WK) {
+        const int64_t gx = (b.rows + 16 * RT - 1) / (16 * RT), gy = (a.rows + 16 * TT - 1) / (16 * TT);
+        const int rc = check_grid(gx, gy);
+        if (rc != PIMHIP_OK) return rc;
+        kernel<<<dim3((unsigned)gx, (unsigned)gy), 64 * WK, 0, s>>>(a, b, (typename O::elem*)out, ld_out);
+        return (int)PIMHIP_OK;
+    };
+    if (a.rows <= 16) return run(mx4_matmul_skinny_kernel<O, 1, 1, 4>, 1, 1, 4);
+    return run(mx4_matmul_skinny_kernel<O, 2, 4, 4>, 2, 4, 4);
+}
+}  // namespace
+
+extern "C" int pimhip_mx4_quantize(const PimHipMx4Matrix* out, const void* x, int dtype, int64_t ld_x, void* stream)
+{
+    DeviceState* st = nullptr;
+    int rc = current_device_state(&st);
+    if (rc != PIMHIP_OK) return rc;
+    Mx4View v;
+    if ((rc = check_matrix("out", out, &v)) != PIMHIP_OK) return rc;
+    if (v.rows == 0) return PIMHIP_OK;
+    if ((rc = check_element("x", x, dtype, true)) != PIMHIP_OK) return rc;
+    if (v.rows > 1 && ld_x < v.cols) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "ld_x=%lld is less than cols=%lld", (long long)ld_x, (long long)v.cols);
+    // A row of up to 1024 values is one wavefront's (at most two rounds of 512), a longer one a block's.
+    const bool short_rows = v.cols <= 1024;
+    const int64_t grid = short_rows ? (v.rows + 3) / 4 : v.rows;
+    if ((rc = check_grid(grid, 1)) != PIMHIP_OK) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    auto run = [&](auto type) {
+        typedef decltype(type) T;
+        auto kernel = short_rows ? mx4_quantize_kernel<T, 1> : mx4_quantize_kernel<T, 4>;
+        kernel<<<dim3((unsigned)grid), 256, 0, s>>>((const typename T::elem*)x, v.rows, v.cols, ld_x, (uint8_t*)out->packed, (uint8_t*)out->scales, v.ld_scales,
+                                                    (uint8_t*)out->tops);
+    };
+    dtype == PIMHIP_F16 ? run(F16{}) : dtype == PIMHIP_BF16 ? run(BF16{}) : run(F32{});
+    PIMHIP_HIP_CHECK(hipGetLastError());
+    return PIMHIP_OK;
+}
+
+extern "C" int pimhip_mx4_find_tops(const PimHipMx4Matrix* m, void* stream)
+{
+    DeviceState* st = nullptr;
+    int rc = current_device_state(&st);
+    if (rc != PIMHIP_OK) return rc;
+    Mx4View v;
+    if ((rc = check_matrix("matrix", m, &v)) != PIMHIP_OK) return rc;
+    if (v.rows == 0) return PIMHIP_OK;
+    if ((rc = check_grid((v.rows + 3) / 4, 1)) != PIMHIP_OK) return rc;
+    mx4_tops_kernel<<<dim3((unsigned)((v.rows + 3) / 4)), 256, 0, static_cast<hipStream_t>(stream)>>>(v.scales, v.ld_scales, v.rows, (v.cols + kMxBlock - 1) / kMxBlock,
+                                                                                                     (uint8_t*)m->tops);
+    PIMHIP_HIP_CHECK(hipGetLastError());
+    return PIMHIP_OK;
+}
+
+extern "C" int pimhip_mx4_dequantize(void* out, int dtype, int64_t ld_out, const PimHipMx4Matrix* m, void* stream)
+{
+    DeviceState* st = nullptr;
+    int rc = current_device_state(&st);
+    if (rc != PIMHIP_OK) return rc;
+    Mx4View v;
+    if ((rc = check_matrix("matrix", m, &v)) != PIMHIP_OK) return rc;
+    if (v.rows == 0) return PIMHIP_OK;
+    if ((rc = check_element("out", out, dtype, true)) != PIMHIP_OK) return rc;
+    if (v.rows > 1 && ld_out < v.cols) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "ld_out=%lld is less than cols=%lld", (long long)ld_out, (long long)v.cols);
+    const dim3 grid((unsigned)((v.cols + 2047) / 2048), (unsigned)(v.rows < 65535 ? v.rows : 65535));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    auto run = [&](auto type) {
+        typedef decltype(type) T;
+        mx4_dequantize_kernel<T><<<grid, 256, 0, s>>>(v.packed, v.scales, v.rows, v.cols, v.ld_scales, (typename T::elem*)out, ld_out);
+    };
+    dtype == PIMHIP_F16 ? run(F16{}) : dtype == PIMHIP_BF16 ? run(BF16{}) : run(F32{});
+    PIMHIP_HIP_CHECK(hipGetLastError());
+    return PIMHIP_OK;
+}
+
+extern "C" int pimhip_mx4_linear(void* out, int64_t ld_out, const void* x, int64_t ld_x, int dtype, int64_t tokens, const PimHipMx4Matrix* weight,
+                                 const void* bias, int act, void* stream)
+{
+    DeviceState* st = nullptr;
+    int rc = current_device_state(&st);
+    if (rc != PIMHIP_OK) return rc;
+    Mx4View w;
+    if ((rc = check_matrix("weight", weight, &w)) != PIMHIP_OK) return rc;
+    if (tokens < 0) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "tokens=%lld", (long long)tokens);
+    if (act != PIMHIP_ACT_NONE && act != PIMHIP_ACT_RELU) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "act=%d", act);
+    if (tokens == 0 || w.rows == 0) return PIMHIP_OK;
+    if ((rc = check_element("x", x, dtype, false)) != PIMHIP_OK || (rc = check_element("out", out, dtype, false)) != PIMHIP_OK) return rc;
+    if (bias && (rc = check_element("bias", bias, dtype, false)) != PIMHIP_OK) return rc;
+    if (tokens > 1 && (ld_x < w.cols || ld_out < w.rows))
+        return fail(PIMHIP_ERR_INVALID_ARGUMENT, "ld_x=%lld is less than cols=%lld, or ld_out=%lld less than rows=%lld", (long long)ld_x, (long long)w.cols,
+                    (long long)ld_out, (long long)w.rows);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int relu = act == PIMHIP_ACT_RELU;
+    rc = dtype == PIMHIP_F16 ? linear<F16>(out, ld_out, x, ld_x, tokens, w, bias, relu, s) : linear<BF16>(out, ld_out, x, ld_x, tokens, w, bias, relu, s);
+    if (rc != PIMHIP_OK) return rc;
+    PIMHIP_HIP_CHECK(hipGetLastError());
+    return PIMHIP_OK;
+}
+
+extern "C" int pimhip_mx4_matmul(void* out, int64_t ld_out, int dtype, const PimHipMx4Matrix* a, const PimHipMx4Matrix* b, void* stream)
+{
+    DeviceState* st = nullptr;
+    int rc = current_device_state(&st);
+    if (rc != PIMHIP_OK) return rc;
+    Mx4View va, vb;
+    if ((rc = check_matrix("a", a, &va)) != PIMHIP_OK || (rc = check_matrix("b", b, &vb)) != PIMHIP_OK) return rc;
+    if (va.cols != vb.cols) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "a has %lld columns, b %lld", (long long)va.cols, (long long)vb.cols);
+    if (va.rows == 0 || vb.rows == 0) return PIMHIP_OK;
+    if ((rc = check_element("out", out, dtype, true)) != PIMHIP_OK) return rc;
+    if (va.rows > 1 && ld_out < vb.rows) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "ld_out=%lld is less than the %lld rows of b", (long long)ld_out, (long long)vb.rows);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    rc = dtype == PIMHIP_F16 ? matmul<F16>(out, ld_out, va, vb, s) : dtype == PIMHIP_BF16 ? matmul<BF16>(out, ld_out, va, vb, s) : matmul<F32>(out, ld_out, va, vb, s);
+    if (rc != PIMHIP_OK) return rc;
+    PIMHIP_HIP_CHECK(hipGetLastError());
+    return PIMHIP_OK;
+}

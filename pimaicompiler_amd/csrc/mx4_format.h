@@ -1,0 +1,117 @@
+// Microscaled 4-bit floating point on gfx950: the format's constants, the 16-bit types its products run on, and conversions.
+//
+// A row of K values lies in blocks of 32.  A value is one of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} (sign, two exponent bits, one mantissa
+// bit), two to a byte, the first in the low half; a block has one scale 2^(code - 127) in a byte, code 255 meaning "not a
+// number".  The last block of a row is filled up with zeros.
+#pragma once
+
+#include "device_common.h"
+
+namespace pimhip
+{
+typedef __bf16 bf16_t;
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef unsigned int uint4_t __attribute__((ext_vector_type(4)));
+typedef unsigned int uint2_t __attribute__((ext_vector_type(2)));
+typedef uint4_t uint4_any_t __attribute__((aligned(2)));  // sixteen bytes at any address a 16-bit value may have
+typedef uint2_t uint2_any_t __attribute__((aligned(2)));
+typedef float float2_t __attribute__((ext_vector_type(2)));
+typedef int int8v_t __attribute__((ext_vector_type(8)));
+
+static constexpr int kMxBlock = 32;        // values that share a scale
+static constexpr int kMxBlockBytes = 16;   // their packed bytes
+static constexpr unsigned int kMxNan = 255u;
+
+// 2^(code - 127) as a float: code 0 is the subnormal 2^-127, code 255 a NaN.
+__device__ __forceinline__ float mx_scale_f32(unsigned int code)
+{
+    const unsigned int bits = code == kMxNan ? 0x7fc00000u : code << 23;
+    return __builtin_bit_cast(float, bits > 0x00400000u ? bits : 0x00400000u);
+}
+
+// The 16-bit types of activations.  `scale` of a row of 4-bit weights that meets them on the matrix cores:
+//   bfloat16 has the range of every scale: elements are converted with their block's own scale, exactly.
+//   fp16 has not.  Elements are converted relative to the row's largest scale code `top` (the largest element is below 2^15 then),
+//   and the sum is multiplied by 2^(top - 127 - 12) at the end.  Exact for blocks down to 2^-35 of the row's largest scale; what is
+//   further below loses bits that are under 2^-38 of the row's largest value.
+struct F16 {
+    typedef half_t elem;
+    typedef half8_t frag;
+    static constexpr int kLift = 12;
+    static __device__ __forceinline__ float4_t mfma(const frag a, const frag b, const float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ float scale(unsigned int code, int top)
+    {
+        const int e = (int)code - top + 127 + kLift;
+        return __builtin_bit_cast(float, code == kMxNan ? 0x7fc00000u : (unsigned int)(e > 0 ? e : 0) << 23);
+    }
+    static __device__ __forceinline__ float unscale(float v, int top) { return __builtin_amdgcn_ldexpf(v, top - 127 - kLift); }
+    static __device__ __forceinline__ frag from_mx4(unsigned int d, float s)
+    {
+        const half2_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, s, 1);
+        const half2_t c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, s, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, s, 3);
+        return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], e[0], e[1]};
+    }
+    static __device__ __forceinline__ elem round(float v) { return round_f16(v); }
+};
+
+struct BF16 {
+    typedef bf16_t elem;
+    typedef bf16x8_t frag;
+    static __device__ __forceinline__ float4_t mfma(const frag a, const frag b, const float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ float scale(unsigned int code, int) { return mx_scale_f32(code); }
+    static __device__ __forceinline__ float unscale(float v, int) { return v; }
+    static __device__ __forceinline__ frag from_mx4(unsigned int d, float s)
+    {
+        const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 1);
+        const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 2), e = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 3);
+        return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], e[0], e[1]};
+    }
+    static __device__ __forceinline__ elem round(float v) { return (bf16_t)v; }
+};
+
+// fp32, as the type of what is quantised, read back, or written by a product; never an operand of the matrix cores here.
+struct F32 {
+    typedef float elem;
+    static __device__ __forceinline__ elem round(float v) { return v; }
+};
+
+// Eight 16-bit values at any address.
+template <class T>
+__device__ __forceinline__ typename T::frag load8_any(const typename T::elem* p)
+{
+    return __builtin_bit_cast(typename T::frag, (uint4_t)*reinterpret_cast<const uint4_any_t*>(p));
+}
+
+// Values k .. k + 7 of a row of K, zeros behind its end.
+template <class T>
+__device__ __forceinline__ typename T::frag load8_guarded(const typename T::elem* row, int64_t k, int64_t K)
+{
+    if (k + 8 <= K) return load8_any<T>(row + k);
+    typename T::frag v = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (k + i < K) v[i] = row[k + i];
+    return v;
+}
+
+// Four results of one row, next to each other from p on, of which `count` exist.
+template <class O>
+__device__ __forceinline__ void store4(typename O::elem* p, const float4_t v, int count)
+{
+    if constexpr (sizeof(typename O::elem) == 2) {
+        const typename O::elem r[4] = {O::round(v[0]), O::round(v[1]), O::round(v[2]), O::round(v[3])};
+        if (count >= 4) {
+            *reinterpret_cast<uint2_any_t*>(p) = __builtin_bit_cast(uint2_t, r);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < count) p[i] = r[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < count) p[i] = v[i];
+    }
+}
+}  // namespace pimhip

@@ -151,6 +151,43 @@ def _stream_arg(stream):
     return None if stream is None else _stream_handle(stream)
 
 
+class _Launch:
+    """`with _Launch(device, stream) as handle`: the device is the current one inside, `stream` (None, a torch stream or an integer
+    handle) torch's current stream, and `handle` its hipStream_t.  What a call allocates inside belongs to the stream it
+    launches on, also where that is not the caller's current one."""
+
+    def __init__(self, device, stream):
+        self._device = device
+        if stream is None:
+            self._stream = None
+        elif isinstance(stream, torch.cuda.Stream):
+            self._stream = stream
+        else:
+            self._stream = torch.cuda.ExternalStream(int(stream), device=device) if int(stream) else torch.cuda.default_stream(device)
+        self._entered = None
+
+    def __enter__(self):
+        if self._stream is None and self._device.index == torch.cuda.current_device():
+            return torch.cuda.current_stream().cuda_stream
+        if self._stream is not None and self._stream.device != self._device:
+            raise NNRuntimeException(f"the stream is one of {self._stream.device}, the tensors are on {self._device}")
+        self._entered = contextlib.ExitStack()
+        self._entered.enter_context(torch.cuda.device(self._device))
+        if self._stream is not None:
+            self._entered.enter_context(torch.cuda.stream(self._stream))
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self._entered is not None:
+            self._entered.close()
+
+
+def _require_no_gradient(*tensors):
+    """For operators without a backward pass: a tensor that would need one is refused rather than cut off silently."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NNRuntimeException("this operator has no backward pass: call it under torch.no_grad() or on detached tensors")
+
+
 def gemv_status(stream=None):
     """After the caller has synchronised `stream`: has a reducing block of a sliced I_X_W product given up waiting for
     partial sums since the workspace was last put in order?  Returns (on_this_stream, static_entry_point).  Such a product

@@ -1,0 +1,29 @@
+"""What the 4-bit operators refuse before anything reaches a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+import pimaicompiler_amd as P
+from pimaicompiler_amd import _lib as L
+
+
+def test_tensors_off_the_gpu_are_refused():
+    x = torch.zeros(2, 64, dtype=torch.float16)
+    u = torch.zeros(2, 32, dtype=torch.uint8)
+    for call in (lambda: P.mx4_quantize(x), lambda: P.mx4_quantize([1.0]), lambda: P.Mx4Tensor(u, u[:, :2], 64), lambda: P.mx4_linear(x, None),
+                 lambda: P.mx4_dequantize(x), lambda: P.mx4_matmul(x, x)):
+        with pytest.raises(P.NNRuntimeException):
+            call()
+
+
+def test_the_c_interface_needs_an_initialised_device():
+    m = L.Mx4Matrix(None, None, None, 1, 32, 16)
+    lib = L.load()
+    for rc in (lib.pimhip_mx4_quantize(m, None, 0, 32, None), lib.pimhip_mx4_find_tops(m, None), lib.pimhip_mx4_dequantize(None, 0, 32, m, None),
+               lib.pimhip_mx4_linear(None, 1, None, 32, 0, 1, m, None, 0, None), lib.pimhip_mx4_matmul(None, 1, 0, m, m, None)):
+        assert rc in (L.PIMHIP_ERR_HIP, L.PIMHIP_ERR_NOT_INITIALIZED)
+
+
+def test_the_struct_of_the_binding_is_the_header_s():
+    assert ctypes.sizeof(L.Mx4Matrix) == 48 and [n for n, _ in L.Mx4Matrix._fields_] == ["packed", "scales", "tops", "rows", "cols", "ld_scales"]
