@@ -523,6 +523,62 @@ int pimhip_mx4_linear(void* out, int64_t ld_out, const void* x, int64_t ld_x, in
  * fp32, one rounding at the store. */
 int pimhip_mx4_matmul(void* out, int64_t ld_out, int dtype, const PimHipMx4Matrix* a, const PimHipMx4Matrix* b, void* stream);
 
+/* ---- mixture-of-experts layer for a few tokens ----------------------------------------------------- */
+
+/* Activation of an expert's first product. */
+typedef enum PimHipExpertAct { PIMHIP_EXPERT_NONE = 0, PIMHIP_EXPERT_RELU = 1, PIMHIP_EXPERT_SILU = 2 } PimHipExpertAct;
+
+typedef struct PimHipMoeLayerPlan PimHipMoeLayerPlan;
+
+/* What a layer is made of; all pointers in it are device pointers except the arrays w1 .. w2_mx4 themselves, which lie on the host and are
+ * read by pimhip_moe_layer_plan_create only.  The plan reads the weights where they lie: they have to outlive it. */
+typedef struct PimHipMoeLayerDesc {
+    const void* router_w;         /* [num_experts, d_model], 16-byte aligned */
+    const void* router_b;         /* [num_experts] or NULL; -inf takes an expert out */
+    const void* const* w1;        /* per expert [d_ff, d_model]; gated: [2 * d_ff, d_model], the gate's rows first; 16-byte aligned */
+    const void* const* b1;        /* per expert [d_ff] or [2 * d_ff]; NULL for none */
+    const void* const* w2;        /* per expert [d_model, d_ff] */
+    const void* const* b2;        /* per expert [d_model]; NULL for none */
+    const PimHipMx4Matrix* w1_mx4; /* in place of w1 and w2: the experts' weights in 4 bits */
+    const PimHipMx4Matrix* w2_mx4;
+    int64_t d_model, d_ff;        /* multiples of 8 */
+    int num_experts, top_k;       /* at most 256 and 16 */
+    int dtype;                    /* PIMHIP_F16 or PIMHIP_BF16: x, y, the router, the biases and 16-bit weights */
+    int act;                      /* a PimHipExpertAct */
+    int gated;                    /* hidden = act(gate) * value */
+    int renormalize;              /* shares sum to 1 over the chosen experts; else they are softmax probabilities over all */
+} PimHipMoeLayerDesc;
+
+/* No counterpart in the reference, which runs such a layer op by op with the choice on the host (pimhip_moe_ffn_step is the one-launch form
+ * for one token, one expert and fp16).  Creating a plan allocates, copies and synchronises `stream`; it is refused on a capturing one. */
+int pimhip_moe_layer_plan_create(PimHipMoeLayerPlan** plan, const PimHipMoeLayerDesc* desc, void* stream);
+int pimhip_moe_layer_plan_destroy(PimHipMoeLayerPlan* plan);
+
+/* What pimhip_moe_layer_forward needs in `workspace` for that many tokens. */
+int pimhip_moe_layer_workspace_bytes(const PimHipMoeLayerPlan* plan, int tokens, uint64_t* bytes);
+
+/* y[t] = sum over the top_k experts e with the largest router logits of share[t, e] * expert_e(x[t]) for up to 64 tokens (x: pitch ld_x,
+ * y: dense).  experts and shares [tokens, top_k]: the choice in falling order of logits, equal ones by their index, a NaN above
+ * all, and the experts' shares (fp32).  Router logits, shares and all sums are fp32; hidden values are rounded to dtype between the
+ * two products.  An expert whose share is 0 adds nothing; where every logit is -inf all shares are 0 and so is y.
+ * Allocates and synchronises nothing.  The workspace is the call's until it has run: calls that may overlap, and captured graphs that
+ * are replayed at the same time, need one each; a plan may be shared. */
+int pimhip_moe_layer_forward(PimHipMoeLayerPlan* plan, const void* x, int64_t ld_x, int tokens, void* y, int* experts, float* shares,
+                             void* workspace, void* stream);
+
+/* ---- log probabilities of tokens ------------------------------------------------------------------ */
+
+/* No counterpart in the reference, whose loops take an argmax of the logits (aten_ops_executor.cpp:520-560).  For every row of logits
+ * [rows, vocab] (dtype: any PimHipDataType, pitch ld elements), in one pass with statistics in fp32:
+ *   logp[row]      log softmax(row)[tokens[row]] (tokens: int64 if tokens_int64, else int32); 0 for a negative token (padding), NaN for one
+ *                  from vocab on.  tokens and logp are both NULL or neither
+ *   entropy[row]   -sum p log p; may be NULL
+ *   top_logp, top_ids [rows, top]   the `top` (0 to 32, at most vocab) most likely tokens in falling order, equal ones by their index
+ * Entries of -inf have probability 0.  A row of nothing else: log probabilities -inf, entropy 0.  A row with a NaN or +inf: NaN
+ * throughout, top_ids -1. */
+int pimhip_token_log_probs(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t vocab, const void* tokens, int tokens_int64, int top,
+                           float* logp, float* entropy, float* top_logp, int* top_ids, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

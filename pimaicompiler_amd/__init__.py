@@ -37,3 +37,5 @@ from .ops import (  # noqa: F401
     set_gemv_spin_limit,
 )
 from .mx4 import Mx4Tensor, mx4_dequantize, mx4_linear, mx4_matmul, mx4_quantize  # noqa: F401
+from .log_probs import token_log_probs  # noqa: F401
+from .moe_layer import MoeLayerPlan  # noqa: F401

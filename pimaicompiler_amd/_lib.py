@@ -20,6 +20,14 @@ class Mx4Matrix(ctypes.Structure):
                 ("cols", ctypes.c_int64), ("ld_scales", ctypes.c_int64)]
 
 
+class MoeLayerDesc(ctypes.Structure):
+    """PimHipMoeLayerDesc."""
+    _fields_ = [("router_w", ctypes.c_void_p), ("router_b", ctypes.c_void_p), ("w1", c_void_pp), ("b1", c_void_pp), ("w2", c_void_pp), ("b2", c_void_pp),
+                ("w1_mx4", ctypes.POINTER(Mx4Matrix)), ("w2_mx4", ctypes.POINTER(Mx4Matrix)), ("d_model", ctypes.c_int64), ("d_ff", ctypes.c_int64),
+                ("num_experts", ctypes.c_int), ("top_k", ctypes.c_int), ("dtype", ctypes.c_int), ("act", ctypes.c_int), ("gated", ctypes.c_int),
+                ("renormalize", ctypes.c_int)]
+
+
 c_mx4_p = ctypes.POINTER(Mx4Matrix)
 
 # name -> (restype, argtypes); must list every function include/pimhip.h declares.
@@ -111,6 +119,14 @@ SIGNATURES = {
     "pimhip_mx4_dequantize": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, c_mx4_p, ctypes.c_void_p]),
     "pimhip_mx4_linear": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int64,
                                          c_mx4_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
+    "pimhip_moe_layer_plan_create": (ctypes.c_int, [c_void_pp, ctypes.POINTER(MoeLayerDesc), ctypes.c_void_p]),
+    "pimhip_moe_layer_plan_destroy": (ctypes.c_int, [ctypes.c_void_p]),
+    "pimhip_moe_layer_workspace_bytes": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.POINTER(ctypes.c_uint64)]),
+    "pimhip_moe_layer_forward": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p,
+                                                ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "pimhip_token_log_probs": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
+                                              ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                              ctypes.c_void_p]),
     "pimhip_mx4_matmul": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, c_mx4_p, c_mx4_p, ctypes.c_void_p]),
 }
 
@@ -126,6 +142,7 @@ PIMHIP_ACT_RELU = 1
 PIMHIP_I_X_W = 0
 PIMHIP_W_X_I = 1
 PIMHIP_F16, PIMHIP_BF16, PIMHIP_F32 = 0, 1, 2
+PIMHIP_EXPERT_NONE, PIMHIP_EXPERT_RELU, PIMHIP_EXPERT_SILU = 0, 1, 2
 GEMM_UNKNOWN, GEMM_VV, GEMM_MV, GEMM_VM, GEMM_MM = 0, 1, 2, 3, 4
 
 _lib = None

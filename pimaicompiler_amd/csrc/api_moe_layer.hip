@@ -1,0 +1,191 @@
+// The mixture-of-experts layer for a few tokens of the C ABI (include/pimhip.h).
+#include "api_common.h"
+#include "moe_layer_kernels.h"
+
+using namespace pimhip;
+
+struct PimHipMoeLayerPlan {
+    int device = 0;
+    int num_experts = 0, top_k = 0;
+    int64_t d_model = 0, d_ff = 0;
+    int dtype = 0, act = 0, gated = 0, renormalize = 0, mx4 = 0;
+    int64_t ld_s1 = 0, ld_s2 = 0;
+    const void* router_w = nullptr;
+    const void* router_b = nullptr;
+    ExpertPointers* experts = nullptr;  // device, [E]
+};
+
+namespace
+{
+std::vector<PimHipMoeLayerPlan*> g_moe_layer_plans;
+
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+size_t hidden_bytes(const PimHipMoeLayerPlan* p, int tokens) { return round256((size_t)tokens * p->top_k * p->d_ff * 2); }
+size_t part_bytes(const PimHipMoeLayerPlan* p, int tokens) { return round256((size_t)tokens * p->top_k * p->d_model * sizeof(float)); }
+
+int destroy_moe_layer_plan_locked(PimHipMoeLayerPlan* plan)
+{
+    if (!plan) return PIMHIP_OK;
+    int prev = -1;
+    hipGetDevice(&prev);
+    hipSetDevice(plan->device);
+    hipDeviceSynchronize();
+    if (plan->experts) hipFree(plan->experts);
+    if (prev >= 0) hipSetDevice(prev);
+    for (size_t i = 0; i < g_moe_layer_plans.size(); ++i) {
+        if (g_moe_layer_plans[i] == plan) {
+            g_moe_layer_plans.erase(g_moe_layer_plans.begin() + i);
+            break;
+        }
+    }
+    delete plan;
+    return PIMHIP_OK;
+}
+
+template <class T, bool MX>
+void launch(const PimHipMoeLayerPlan* p, const MoeLayerArgs& a, hipStream_t s)
+{
+    moe_layer_router_kernel<T><<<dim3((unsigned)a.tokens), 256, 0, s>>>(a);
+    const unsigned E = (unsigned)a.E;
+    if (p->gated)
+        moe_layer_first_kernel<T, MX, true, 1, 4><<<dim3((unsigned)((a.d_ff + 15) / 16), E), 256, 0, s>>>(a);
+    else
+        moe_layer_first_kernel<T, MX, false, 2, 4><<<dim3((unsigned)((a.d_ff + 31) / 32), E), 256, 0, s>>>(a);
+    moe_layer_second_kernel<T, MX, 1, 4><<<dim3((unsigned)((a.d_model + 15) / 16), E), 256, 0, s>>>(a);
+    moe_layer_sum_kernel<T><<<dim3((unsigned)((a.d_model + 1023) / 1024), (unsigned)a.tokens), 256, 0, s>>>(a);
+}
+}  // namespace
+
+namespace pimhip
+{
+void destroy_all_moe_layer_plans_locked()
+{
+    while (!g_moe_layer_plans.empty()) destroy_moe_layer_plan_locked(g_moe_layer_plans.back());
+}
+}  // namespace pimhip
+
+extern "C" int pimhip_moe_layer_plan_create(PimHipMoeLayerPlan** plan_out, const PimHipMoeLayerDesc* d, void* stream)
+{
+    DeviceState* st = nullptr;
+    int rc = current_device_state(&st);
+    if (rc != PIMHIP_OK) return rc;
+    if (!plan_out || !d || !d->router_w) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "plan, desc and router_w must be non-null");
+    if (d->dtype != PIMHIP_F16 && d->dtype != PIMHIP_BF16) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "dtype=%d", d->dtype);
+    if (d->num_experts < 1 || d->num_experts > kMoeLayerExperts)
+        return fail(PIMHIP_ERR_UNSUPPORTED, "num_experts=%d not in [1, %d]", d->num_experts, kMoeLayerExperts);
+    if (d->top_k < 1 || d->top_k > kMoeLayerTopK || d->top_k > d->num_experts)
+        return fail(PIMHIP_ERR_UNSUPPORTED, "top_k=%d not in [1, min(%d, num_experts)]", d->top_k, kMoeLayerTopK);
+    constexpr int64_t kMost = 1 << 20;
+    if (d->d_model < 8 || d->d_model > kMost || (d->d_model & 7) || d->d_ff < 8 || d->d_ff > kMost || (d->d_ff & 7))
+        return fail(PIMHIP_ERR_UNSUPPORTED, "d_model=%lld and d_ff=%lld must be multiples of 8 in [8, %lld]", (long long)d->d_model, (long long)d->d_ff, (long long)kMost);
+    if (d->act != PIMHIP_EXPERT_NONE && d->act != PIMHIP_EXPERT_RELU && d->act != PIMHIP_EXPERT_SILU) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "act=%d", d->act);
+    const bool mx = d->w1_mx4 || d->w2_mx4;
+    if (mx ? (!d->w1_mx4 || !d->w2_mx4) : (!d->w1 || !d->w2))
+        return fail(PIMHIP_ERR_INVALID_ARGUMENT, "either w1 and w2 or w1_mx4 and w2_mx4 must be non-null");
+    if (!aligned16(d->router_w)) return fail(PIMHIP_ERR_UNSUPPORTED, "router_w must be 16-byte aligned");
+    const int64_t rows1 = d->gated ? 2 * d->d_ff : d->d_ff;
+    std::vector<ExpertPointers> table((size_t)d->num_experts);
+    for (int e = 0; e < d->num_experts; ++e) {
+        ExpertPointers& p = table[(size_t)e];
+        memset(&p, 0, sizeof(p));
+        if (mx) {
+            const PimHipMx4Matrix *m1 = d->w1_mx4 + e, *m2 = d->w2_mx4 + e;
+            if (m1->rows != rows1 || m1->cols != d->d_model || m2->rows != d->d_model || m2->cols != d->d_ff)
+                return fail(PIMHIP_ERR_INVALID_ARGUMENT, "expert %d: w1 must be [%lld, %lld] and w2 [%lld, %lld]", e, (long long)rows1, (long long)d->d_model,
+                            (long long)d->d_model, (long long)d->d_ff);
+            for (const PimHipMx4Matrix* m : {m1, m2}) {
+                if (!m->packed || !m->scales || !m->tops || !aligned16(m->packed) || !aligned16(m->scales) || (m->ld_scales & 15) ||
+                    m->ld_scales * 32 < m->cols || m->ld_scales != (m == m1 ? d->w1_mx4 : d->w2_mx4)->ld_scales)
+                    return fail(PIMHIP_ERR_INVALID_ARGUMENT, "expert %d: a 4-bit matrix is null, not 16-byte aligned, or has another pitch of scales", e);
+            }
+            p.w1 = m1->packed, p.s1 = m1->scales, p.t1 = m1->tops;
+            p.w2 = m2->packed, p.s2 = m2->scales, p.t2 = m2->tops;
+        } else {
+            p.w1 = d->w1[e], p.w2 = d->w2[e];
+            if (!p.w1 || !p.w2) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "w1[%d] / w2[%d] is null", e, e);
+            if (!aligned16(p.w1) || !aligned16(p.w2)) return fail(PIMHIP_ERR_UNSUPPORTED, "the weights of expert %d must be 16-byte aligned", e);
+        }
+        p.b1 = d->b1 ? d->b1[e] : nullptr;
+        p.b2 = d->b2 ? d->b2[e] : nullptr;
+    }
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    PIMHIP_HIP_CHECK(hipStreamIsCapturing(s, &capture));
+    if (capture != hipStreamCaptureStatusNone) return fail(PIMHIP_ERR_UNSUPPORTED, "a plan allocates: create it before the capture");
+    PimHipMoeLayerPlan* plan = new (std::nothrow) PimHipMoeLayerPlan();
+    if (!plan) return fail(PIMHIP_ERR_HIP, "out of host memory");
+    hipGetDevice(&plan->device);
+    plan->num_experts = d->num_experts, plan->top_k = d->top_k, plan->d_model = d->d_model, plan->d_ff = d->d_ff;
+    plan->dtype = d->dtype, plan->act = d->act, plan->gated = d->gated ? 1 : 0, plan->renormalize = d->renormalize ? 1 : 0, plan->mx4 = mx;
+    plan->ld_s1 = mx ? d->w1_mx4->ld_scales : 0, plan->ld_s2 = mx ? d->w2_mx4->ld_scales : 0;
+    plan->router_w = d->router_w, plan->router_b = d->router_b;
+    const size_t bytes = table.size() * sizeof(ExpertPointers);
+    hipError_t err = hipMalloc(reinterpret_cast<void**>(&plan->experts), bytes);
+    if (err == hipSuccess) err = hipMemcpyAsync(plan->experts, table.data(), bytes, hipMemcpyHostToDevice, s);
+    if (err == hipSuccess) err = hipStreamSynchronize(s);  // (table goes out of scope)
+    std::lock_guard<std::mutex> lock(g_mutex);
+    if (err != hipSuccess) {
+        destroy_moe_layer_plan_locked(plan);
+        return fail(PIMHIP_ERR_HIP, "the table of experts could not be set up: %s", hipGetErrorString(err));
+    }
+    g_moe_layer_plans.push_back(plan);
+    *plan_out = plan;
+    return PIMHIP_OK;
+}
+
+extern "C" int pimhip_moe_layer_plan_destroy(PimHipMoeLayerPlan* plan)
+{
+    if (!plan) return PIMHIP_OK;
+    std::lock_guard<std::mutex> lock(g_mutex);
+    bool known = false;
+    for (PimHipMoeLayerPlan* q : g_moe_layer_plans) known = known || (q == plan);
+    if (!known) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "unknown or already destroyed expert layer plan");
+    return destroy_moe_layer_plan_locked(plan);
+}
+
+extern "C" int pimhip_moe_layer_workspace_bytes(const PimHipMoeLayerPlan* plan, int tokens, uint64_t* bytes)
+{
+    if (!plan || !bytes) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "plan and bytes must be non-null");
+    if (tokens < 0 || tokens > kMoeLayerTokens) return fail(PIMHIP_ERR_UNSUPPORTED, "tokens=%d not in [0, %d]", tokens, kMoeLayerTokens);
+    *bytes = hidden_bytes(plan, tokens) + part_bytes(plan, tokens);
+    return PIMHIP_OK;
+}
+
+extern "C" int pimhip_moe_layer_forward(PimHipMoeLayerPlan* plan, const void* x, int64_t ld_x, int tokens, void* y, int* experts, float* shares,
+                                        void* workspace, void* stream)
+{
+    DeviceState* st = nullptr;
+    int rc = current_device_state(&st);
+    if (rc != PIMHIP_OK) return rc;
+    if (!plan) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "plan is null");
+    int dev = -1;
+    PIMHIP_HIP_CHECK(hipGetDevice(&dev));
+    if (dev != plan->device) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "plan belongs to device %d, current device is %d", plan->device, dev);
+    if (tokens < 0 || tokens > kMoeLayerTokens) return fail(PIMHIP_ERR_UNSUPPORTED, "tokens=%d not in [0, %d]", tokens, kMoeLayerTokens);
+    if (tokens == 0) return PIMHIP_OK;
+    if (!x || !y || !experts || !shares || !workspace) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "x, y, experts, shares and workspace must be non-null");
+    if (!aligned16(workspace)) return fail(PIMHIP_ERR_UNSUPPORTED, "workspace must be 16-byte aligned");
+    if ((reinterpret_cast<uintptr_t>(x) & 1u) || (reinterpret_cast<uintptr_t>(y) & 1u) || (reinterpret_cast<uintptr_t>(experts) & 3u) ||
+        (reinterpret_cast<uintptr_t>(shares) & 3u))
+        return fail(PIMHIP_ERR_INVALID_ARGUMENT, "x, y, experts and shares must be aligned to their elements");
+    if (tokens > 1 && (ld_x < plan->d_model || ld_x > INT32_MAX)) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "ld_x=%lld", (long long)ld_x);
+    MoeLayerArgs a;
+    memset(&a, 0, sizeof(a));
+    a.experts = plan->experts;
+    a.x = x, a.router_w = plan->router_w, a.router_b = plan->router_b, a.y = y;
+    a.chosen = experts, a.share = shares;
+    a.h = workspace;
+    a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + hidden_bytes(plan, tokens));
+    a.tokens = tokens, a.E = plan->num_experts, a.top_k = plan->top_k, a.d_model = (int)plan->d_model, a.d_ff = (int)plan->d_ff;
+    a.ld_x = tokens > 1 ? (int)ld_x : 0;
+    a.ld_s1 = (int)plan->ld_s1, a.ld_s2 = (int)plan->ld_s2;
+    a.act = plan->act, a.renormalize = plan->renormalize;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const bool f16 = plan->dtype == PIMHIP_F16;
+    if (plan->mx4)
+        f16 ? launch<F16, true>(plan, a, s) : launch<BF16, true>(plan, a, s);
+    else
+        f16 ? launch<F16, false>(plan, a, s) : launch<BF16, false>(plan, a, s);
+    PIMHIP_HIP_CHECK(hipGetLastError());
+    return PIMHIP_OK;
+}
