@@ -311,6 +311,207 @@ PyObject* lstm(PyObject*, PyObject* const* args, Py_ssize_t n)
     return out;
 }
 
+// ---- 4-bit matrices, expert layers, log probabilities -----------------------------------------------------------------------
+// The plain case of these: a tensor of one of their types on the current device, torch's current stream, no gradient asked for.
+bool plainTensor(PyObject* o, const at::Tensor*& t)
+{
+    if (!THPVariable_Check(o)) return false;
+    t = &THPVariable_Unpack(o);
+    return t->defined() && t->is_cuda() && t->layout() == at::kStrided && t->dim() >= 1 && t->device().index() == c10::hip::current_device() &&
+           !(t->requires_grad() && at::GradMode::is_enabled());
+}
+
+int typeCode(at::ScalarType t) { return t == at::kHalf ? PIMHIP_F16 : t == at::kBFloat16 ? PIMHIP_BF16 : t == at::kFloat ? PIMHIP_F32 : -1; }
+
+void* currentStream() { return static_cast<void*>(c10::hip::getCurrentHIPStream().stream()); }
+
+at::Tensor newTensor(at::IntArrayRef shape, at::ScalarType type, const at::Device& device) { return at::detail::empty_cuda(shape, type, device, c10::nullopt); }
+
+// The rows of a contiguous tensor of at least one value a row; a matrix may have a pitch.
+bool rowsOf(const at::Tensor& t, int64_t& rows, int64_t& cols, int64_t& ld)
+{
+    cols = t.size(t.dim() - 1);
+    if (cols < 1) return false;
+    rows = t.numel() / cols;
+    ld = cols;
+    if (t.is_contiguous()) return true;
+    if (t.dim() != 2 || t.stride(1) != 1 || t.stride(0) < cols) return false;
+    ld = t.stride(0);
+    return true;
+}
+
+// The address of a PimHipMx4Matrix that a Python object keeps.
+const PimHipMx4Matrix* matrixOf(PyObject* o) { return PyLong_Check(o) ? static_cast<const PimHipMx4Matrix*>(PyLong_AsVoidPtr(o)) : nullptr; }
+
+// mx4_quantize(x): (packed, scales, tops)
+PyObject* mx4Quantize(PyObject*, PyObject* const* args, Py_ssize_t n)
+{
+    const at::Tensor* x;
+    int64_t rows, cols, ld;
+    if (n != 1 || !plainTensor(args[0], x) || typeCode(x->scalar_type()) < 0 || !rowsOf(*x, rows, cols, ld)) return none();
+    const int64_t blocks = (cols + 31) / 32, pitch = (blocks + 15) / 16 * 16;
+    at::Tensor packed = newTensor({rows, blocks * 16}, at::kByte, x->device()), scales = newTensor({rows, pitch}, at::kByte, x->device());
+    at::Tensor tops = newTensor({rows}, at::kByte, x->device());
+    const PimHipMx4Matrix m{packed.data_ptr(), scales.data_ptr(), tops.data_ptr(), rows, cols, pitch};
+    int rc;
+    void* stream = currentStream();
+    Py_BEGIN_ALLOW_THREADS
+    rc = pimhip_mx4_quantize(&m, x->data_ptr(), typeCode(x->scalar_type()), ld, stream);
+    Py_END_ALLOW_THREADS
+    if (rc != PIMHIP_OK) return status(rc);
+    PyObject* out = PyTuple_New(3);
+    if (!out) return nullptr;
+    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(packed)));
+    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(scales)));
+    PyTuple_SET_ITEM(out, 2, THPVariable_Wrap(std::move(tops)));
+    return out;
+}
+
+// A shape given as a tuple, its last entry replaced.
+bool shapeOf(PyObject* o, int64_t last, at::DimVector& shape)
+{
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) < 1) return false;
+    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(o); ++i) {
+        int64_t v;
+        if (!intOf(PyTuple_GET_ITEM(o, i), v)) return false;
+        shape.push_back(v);
+    }
+    shape.back() = last;
+    return true;
+}
+
+// mx4_dequantize(matrix, shape, device index, dtype code): the values
+PyObject* mx4Dequantize(PyObject*, PyObject* const* args, Py_ssize_t n)
+{
+    int64_t device, code;
+    at::DimVector shape;
+    if (n != 4) return none();
+    const PimHipMx4Matrix* m = matrixOf(args[0]);
+    if (!m || !shapeOf(args[1], m->cols, shape) || !intOf(args[2], device) || !intOf(args[3], code) || device != c10::hip::current_device()) return none();
+    at::Tensor out = newTensor(shape, code == PIMHIP_F16 ? at::kHalf : code == PIMHIP_BF16 ? at::kBFloat16 : at::kFloat,
+                               at::Device(at::kCUDA, static_cast<c10::DeviceIndex>(device)));
+    int rc;
+    void* stream = currentStream();
+    Py_BEGIN_ALLOW_THREADS
+    rc = pimhip_mx4_dequantize(out.data_ptr(), (int)code, m->cols, m, stream);
+    Py_END_ALLOW_THREADS
+    return rc == PIMHIP_OK ? THPVariable_Wrap(std::move(out)) : status(rc);
+}
+
+// mx4_linear(x, matrix, the matrix's device index, bias or None, relu): x . matrix^T
+PyObject* mx4Linear(PyObject*, PyObject* const* args, Py_ssize_t n)
+{
+    const at::Tensor *x, *b = nullptr;
+    int64_t device, rows, cols, ld;
+    if (n != 5 || !plainTensor(args[0], x) || (x->scalar_type() != at::kHalf && x->scalar_type() != at::kBFloat16) || !rowsOf(*x, rows, cols, ld)) return none();
+    const PimHipMx4Matrix* m = matrixOf(args[1]);
+    if (!m || m->cols != cols || !intOf(args[2], device) || device != x->device().index()) return none();
+    if (args[3] != Py_None && (!plainTensor(args[3], b) || b->scalar_type() != x->scalar_type() || b->numel() != m->rows || !b->is_contiguous())) return none();
+    at::DimVector shape(x->sizes());
+    shape.back() = m->rows;
+    at::Tensor out = newTensor(shape, x->scalar_type(), x->device());
+    int rc;
+    void* stream = currentStream();
+    Py_BEGIN_ALLOW_THREADS
+    rc = pimhip_mx4_linear(out.data_ptr(), m->rows, x->data_ptr(), ld, typeCode(x->scalar_type()), rows, m, b ? b->data_ptr() : nullptr,
+                           args[4] == Py_True ? PIMHIP_ACT_RELU : PIMHIP_ACT_NONE, stream);
+    Py_END_ALLOW_THREADS
+    return rc == PIMHIP_OK ? THPVariable_Wrap(std::move(out)) : status(rc);
+}
+
+// mx4_matmul(a, a's shape, b, device index of both, dtype code): a . b^T
+PyObject* mx4Matmul(PyObject*, PyObject* const* args, Py_ssize_t n)
+{
+    int64_t device, code;
+    at::DimVector shape;
+    if (n != 5) return none();
+    const PimHipMx4Matrix *a = matrixOf(args[0]), *b = matrixOf(args[2]);
+    if (!a || !b || a->cols != b->cols || !shapeOf(args[1], b->rows, shape) || !intOf(args[3], device) || !intOf(args[4], code) ||
+        device != c10::hip::current_device())
+        return none();
+    at::Tensor out = newTensor(shape, code == PIMHIP_F16 ? at::kHalf : code == PIMHIP_BF16 ? at::kBFloat16 : at::kFloat,
+                               at::Device(at::kCUDA, static_cast<c10::DeviceIndex>(device)));
+    int rc;
+    void* stream = currentStream();
+    Py_BEGIN_ALLOW_THREADS
+    rc = pimhip_mx4_matmul(out.data_ptr(), b->rows, (int)code, a, b, stream);
+    Py_END_ALLOW_THREADS
+    return rc == PIMHIP_OK ? THPVariable_Wrap(std::move(out)) : status(rc);
+}
+
+// log_probs(logits, tokens or None, top): (logp or None, entropy[, top_logp, top_ids])
+PyObject* logProbs(PyObject*, PyObject* const* args, Py_ssize_t n)
+{
+    const at::Tensor *x, *t = nullptr;
+    int64_t top, rows, cols, ld;
+    if (n != 3 || !plainTensor(args[0], x) || typeCode(x->scalar_type()) < 0 || !rowsOf(*x, rows, cols, ld) || !PyLong_CheckExact(args[2]) || !intOf(args[2], top) ||
+        top < 0 || top > cols)
+        return none();
+    const at::IntArrayRef lead = x->sizes().slice(0, x->dim() - 1);
+    if (args[1] != Py_None) {
+        if (!THPVariable_Check(args[1])) return none();
+        t = &THPVariable_Unpack(args[1]);
+        if (!t->defined() || t->device() != x->device() || t->sizes() != lead || !t->is_contiguous() || (t->scalar_type() != at::kLong && t->scalar_type() != at::kInt))
+            return none();
+    }
+    at::DimVector tops(lead);
+    tops.push_back(top);
+    at::Tensor entropy = newTensor(lead, at::kFloat, x->device()), logp, top_logp, top_ids;
+    if (t) logp = newTensor(lead, at::kFloat, x->device());
+    if (top) {
+        top_logp = newTensor(tops, at::kFloat, x->device());
+        top_ids = newTensor(tops, at::kInt, x->device());
+    }
+    int rc;
+    void* stream = currentStream();
+    Py_BEGIN_ALLOW_THREADS
+    rc = pimhip_token_log_probs(x->data_ptr(), typeCode(x->scalar_type()), ld, rows, cols, t ? t->data_ptr() : nullptr, t && t->scalar_type() == at::kLong, (int)top,
+                                t ? static_cast<float*>(logp.data_ptr()) : nullptr, static_cast<float*>(entropy.data_ptr()),
+                                top ? static_cast<float*>(top_logp.data_ptr()) : nullptr, top ? static_cast<int*>(top_ids.data_ptr()) : nullptr, stream);
+    Py_END_ALLOW_THREADS
+    if (rc != PIMHIP_OK) return status(rc);
+    PyObject* out = PyTuple_New(top ? 4 : 2);
+    if (!out) return nullptr;
+    PyTuple_SET_ITEM(out, 0, t ? THPVariable_Wrap(std::move(logp)) : none());
+    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(entropy)));
+    if (top) {
+        PyTuple_SET_ITEM(out, 2, THPVariable_Wrap(std::move(top_logp)));
+        PyTuple_SET_ITEM(out, 3, THPVariable_Wrap(std::move(top_ids)));
+    }
+    return out;
+}
+
+// moe_layer(plan handle, x, d_model, top_k, x's type as a code, device index, most tokens of a launch): (y, experts, shares)
+PyObject* moeLayer(PyObject*, PyObject* const* args, Py_ssize_t n)
+{
+    const at::Tensor* x;
+    int64_t d_model, top_k, code, device, most, rows, cols, ld;
+    if (n != 7 || !PyLong_Check(args[0]) || !plainTensor(args[1], x) || !rowsOf(*x, rows, cols, ld) || !intOf(args[2], d_model) || !intOf(args[3], top_k) ||
+        !intOf(args[4], code) || !intOf(args[5], device) || !intOf(args[6], most))
+        return none();
+    if (typeCode(x->scalar_type()) != code || cols != d_model || device != x->device().index() || rows > most) return none();
+    PimHipMoeLayerPlan* plan = static_cast<PimHipMoeLayerPlan*>(PyLong_AsVoidPtr(args[0]));
+    uint64_t bytes = 0;
+    int rc = pimhip_moe_layer_workspace_bytes(plan, (int)rows, &bytes);
+    if (rc != PIMHIP_OK) return status(rc);
+    at::DimVector choice(x->sizes());
+    choice.back() = top_k;
+    at::Tensor y = newTensor(x->sizes(), x->scalar_type(), x->device()), experts = newTensor(choice, at::kInt, x->device());
+    at::Tensor shares = newTensor(choice, at::kFloat, x->device()), workspace = newTensor({(int64_t)bytes}, at::kByte, x->device());
+    void* stream = currentStream();
+    Py_BEGIN_ALLOW_THREADS
+    rc = pimhip_moe_layer_forward(plan, x->data_ptr(), ld, (int)rows, y.data_ptr(), static_cast<int*>(experts.data_ptr()), static_cast<float*>(shares.data_ptr()),
+                                  workspace.data_ptr(), stream);
+    Py_END_ALLOW_THREADS
+    if (rc != PIMHIP_OK) return status(rc);
+    PyObject* out = PyTuple_New(3);
+    if (!out) return nullptr;
+    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(y)));
+    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(experts)));
+    PyTuple_SET_ITEM(out, 2, THPVariable_Wrap(std::move(shares)));
+    return out;
+}
+
 // ---- bound steps: the buffers of a one-launch step, fixed once, and the call that issues it ---------------------------------
 constexpr const char* kBoundStep = "pimaicompiler_amd.bound_step";
 struct BoundStep {
@@ -439,6 +640,9 @@ void addFastcalls(PyObject* module)
                                     method<projection>("fast_projection"), method<lstmKey>("lstm_key"),
                                     method<lstm>("fast_lstm"),             method<bindMoe>("bind_moe"),
                                     method<bindRnnt>("bind_rnnt"),         method<bindDecoder>("bind_decoder"),
-                                    method<issue>("issue"),                {nullptr, nullptr, 0, nullptr}};
+                                    method<issue>("issue"),                method<mx4Quantize>("fast_mx4_quantize"),
+                                    method<mx4Dequantize>("fast_mx4_dequantize"), method<mx4Linear>("fast_mx4_linear"),
+                                    method<mx4Matmul>("fast_mx4_matmul"),  method<logProbs>("fast_log_probs"),
+                                    method<moeLayer>("fast_moe_layer"),    {nullptr, nullptr, 0, nullptr}};
     if (PyModule_AddFunctions(module, methods) != 0) throw pybind11::error_already_set();
 }

@@ -6,7 +6,7 @@ import torch
 
 from . import _lib as L
 from .mx4 import _CODES, _require, _rows_of
-from .ops import NNRuntimeException, _check, _ensure_init, _Launch, _require_no_gradient
+from .ops import NNRuntimeException, _check, _ensure_init, _Launch, _native, _require_no_gradient, _result
 
 TOP_MOST = 32
 
@@ -23,6 +23,9 @@ def token_log_probs(logits, tokens=None, top=0, stream=None):
 
     One pass over the logits, statistics in fp32.  A row of -inf alone leaves every token impossible: log probabilities -inf, entropy 0.  A row
     with a NaN or +inf has no distribution: NaN throughout, and -1 for its alternatives."""
+    out = _native().fast_log_probs(logits, tokens, top) if stream is None else None
+    if out is not None:
+        return _result(out)
     _require("logits", logits, tuple(_CODES))
     _require_no_gradient(logits)
     if logits.dim() < 1 or logits.size(-1) < 1:

@@ -9,7 +9,7 @@ import torch
 
 from . import _lib as L
 from .mx4 import _CODES, Mx4Tensor, _require, _rows_of
-from .ops import NNRuntimeException, _check, _ensure_init, _Launch, _require_no_gradient
+from .ops import NNRuntimeException, _check, _ensure_init, _Launch, _native, _require_no_gradient, _result
 
 TOKENS_MOST = 64  # tokens of one launch; longer inputs are taken in pieces of that many
 _ACTS = {"none": L.PIMHIP_EXPERT_NONE, "aten::relu": L.PIMHIP_EXPERT_RELU, "aten::silu": L.PIMHIP_EXPERT_SILU}
@@ -102,6 +102,9 @@ class MoeLayerPlan:
     def forward(self, x, stream=None):
         """y [.., d_model], experts [.., top_k] int32, shares [.., top_k] fp32 for x [.., d_model]: the experts in falling order of their logits,
         equal ones by their index.  Nothing is read back.  More than 64 tokens are taken 64 at a time."""
+        out = _native().fast_moe_layer(self._handle.value, x, self.d_model, self.top_k, _CODES[self.dtype], self.device.index, TOKENS_MOST) if stream is None else None
+        if out is not None:
+            return _result(out)
         _require("x", x, (self.dtype,))
         _require_no_gradient(x)
         if x.dim() < 1 or x.size(-1) != self.d_model or x.device != self.device:

@@ -4,10 +4,12 @@ reading back, the product of fp16 / bf16 tokens with 4-bit weights, and the prod
 The reference's weights are fp16 throughout; a product for one token is bound by its weights' bytes, and these are 17 bytes for 32
 values instead of 64.  Errors are NNRuntimeException, as everywhere in this package; there is no CPU path and no backward pass.
 """
+import ctypes
+
 import torch
 
 from . import _lib as L
-from .ops import NNRuntimeException, _act_code, _check, _ensure_init, _Launch, _require_no_gradient
+from .ops import NNRuntimeException, _act_code, _check, _ensure_init, _Launch, _native, _require_no_gradient, _result
 
 BLOCK = 32  # values that share a scale
 _CODES = {torch.float16: L.PIMHIP_F16, torch.bfloat16: L.PIMHIP_BF16, torch.float32: L.PIMHIP_F32}
@@ -76,6 +78,8 @@ class Mx4Tensor:
     def _hold(self, packed, scales, tops, shape):
         self.packed, self.scales, self.tops, self.shape = packed, scales, tops, torch.Size(shape)
         self._c = L.Mx4Matrix(packed.data_ptr(), scales.data_ptr(), tops.data_ptr(), packed.size(0), self.shape[-1], scales.size(1))
+        self._at = ctypes.addressof(self._c)   # (what the native calls read the matrix through)
+        self._device_index = packed.device.index
 
     @classmethod
     def _empty(cls, shape, device):
@@ -107,6 +111,11 @@ def mx4_quantize(x, stream=None):
     """x [.., K] (fp16, bf16 or fp32) as an Mx4Tensor of the same shape.  A block of 32 along K gets the scale 2^(floor(log2(largest
     magnitude)) - 2), its values the nearest 4-bit one, ties to the even code, saturating at 6 scales; a block that holds an infinity or a
     NaN reads back as NaN."""
+    made = _native().fast_mx4_quantize(x) if stream is None else None
+    if made is not None:
+        q = Mx4Tensor.__new__(Mx4Tensor)
+        q._hold(*_result(made), x.shape)
+        return q
     _require("x", x, tuple(_CODES))
     _require_no_gradient(x)
     if x.dim() < 1 or x.size(-1) < 1:
@@ -125,6 +134,9 @@ def mx4_dequantize(q, dtype=torch.float16, stream=None):
         raise NNRuntimeException("an Mx4Tensor is read back")
     if dtype not in _CODES:
         raise NNRuntimeException(f"{dtype} is none of {', '.join(str(d) for d in _CODES)}")
+    out = _native().fast_mx4_dequantize(q._at, q.shape, q._device_index, _CODES[dtype]) if stream is None else None
+    if out is not None:
+        return _result(out)
     _ensure_init(q.packed)
     with _Launch(q.device, stream) as handle:
         out = torch.empty(q.shape, dtype=dtype, device=q.device)
@@ -135,6 +147,10 @@ def mx4_dequantize(q, dtype=torch.float16, stream=None):
 def mx4_linear(x, weight, bias=None, act_type="none", stream=None):
     """act(x . W^T + b) for x [.., K] in fp16 or bf16, W an Mx4Tensor [N, K], b [N] of x's type or None; act_type as
     custom_aten_addmm's.  One token up to whole prompts; the result [.., N] has x's type."""
+    if stream is None and isinstance(weight, Mx4Tensor) and len(weight.shape) == 2:
+        out = _native().fast_mx4_linear(x, weight._at, weight._device_index, bias, act_type == "aten::relu")
+        if out is not None:
+            return _result(out)
     _require("x", x, (torch.float16, torch.bfloat16))
     if not isinstance(weight, Mx4Tensor) or len(weight.shape) != 2:
         raise NNRuntimeException("weight must be a two-dimensional Mx4Tensor")
@@ -170,6 +186,9 @@ def mx4_matmul(a, b, dtype=torch.float16, stream=None):
         raise NNRuntimeException(f"the operands disagree on the reduction width ({a.shape[-1]} vs {b.shape[-1]})")
     if a.device != b.device:
         raise NNRuntimeException(f"a is on {a.device}, b on {b.device}")
+    out = _native().fast_mx4_matmul(a._at, a.shape, b._at, a._device_index, _CODES[dtype]) if stream is None else None
+    if out is not None:
+        return _result(out)
     _ensure_init(a.packed)
     N = b.shape[0]
     with _Launch(a.device, stream) as handle:

@@ -60,6 +60,7 @@ class _WithoutExtension:
         return None
 
     fast_addmm = fast_matmul = fast_linear = fast_group = fast_projection = fast_lstm = lstm_key = _not_taken
+    fast_mx4_quantize = fast_mx4_dequantize = fast_mx4_linear = fast_mx4_matmul = fast_log_probs = fast_moe_layer = _not_taken
 
     @staticmethod
     def bind_moe(*args):
