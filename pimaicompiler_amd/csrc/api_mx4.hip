@@ -1,6 +1,6 @@
 // Microscaled 4-bit matrices of the C ABI (include/pimhip.h): quantisation, reading back, and the products with one or both operands in 4 bits.
 #include "api_common.h"
-#include "mx4_kernels.h"
+#include "mx4_tile_kernels.h"
 
 using namespace pimhip;
 
@@ -53,7 +53,13 @@ int linear(void* out, int64_t ld_out, const void* x, int64_t ld_x, int64_t M, co
 {
     if (M <= 16) return linear_skinny<T, 1, 1, 2, 4>(out, ld_out, x, ld_x, M, w, bias, relu, s);
     if (M <= 32) return linear_skinny<T, 1, 2, 1, 4>(out, ld_out, x, ld_x, M, w, bias, relu, s);
-    return linear_skinny<T, 1, 4, 1, 4>(out, ld_out, x, ld_x, M, w, bias, relu, s);
+    if (M <= 64) return linear_skinny<T, 1, 4, 1, 4>(out, ld_out, x, ld_x, M, w, bias, relu, s);
+    const int64_t tiles = ((w.rows + 127) / 128) * ((M + 127) / 128);
+    const int rc = check_grid(tiles, 1);
+    if (rc != PIMHIP_OK) return rc;
+    mx4_linear_tile_kernel<T, 4, 4, 2, 2><<<dim3((unsigned)tiles), 256, 0, s>>>((const typename T::elem*)x, w, (const typename T::elem*)bias,
+                                                                               (typename T::elem*)out, ld_x, ld_out, M, relu);
+    return PIMHIP_OK;
 }
 
 template <class O>
@@ -67,7 +73,16 @@ int matmul(void* out, int64_t ld_out, const Mx4View& a, const Mx4View& b, hipStr
         return (int)PIMHIP_OK;
     };
     if (a.rows <= 16) return run(mx4_matmul_skinny_kernel<O, 1, 1, 4>, 1, 1, 4);
-    return run(mx4_matmul_skinny_kernel<O, 2, 4, 4>, 2, 4, 4);
+    if (a.rows <= 64) return run(mx4_matmul_skinny_kernel<O, 1, 4, 4>, 1, 4, 4);
+    auto tiled = [&](auto kernel, int n, int t, int threads) {
+        const int64_t tiles = ((b.rows + n - 1) / n) * ((a.rows + t - 1) / t);
+        const int rc = check_grid(tiles, 1);
+        if (rc != PIMHIP_OK) return rc;
+        kernel<<<dim3((unsigned)tiles), threads, 0, s>>>(a, b, (typename O::elem*)out, ld_out);
+        return (int)PIMHIP_OK;
+    };
+    if (((b.rows + 255) / 256) * ((a.rows + 255) / 256) >= 192) return tiled(mx4_matmul_tile_kernel<O, 8, 4, 2, 4>, 256, 256, 512);
+    return tiled(mx4_matmul_tile_kernel<O, 4, 4, 2, 2>, 128, 128, 256);
 }
 }  // namespace
 

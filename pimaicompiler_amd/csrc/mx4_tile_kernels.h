@@ -1,0 +1,264 @@
+// Products of many tokens with 4-bit weights: tiles of the result, operands through LDS.
+//
+// A block has 16 GN WN rows of weights and 16 GT WT tokens, a wavefront of its GN x GT ones WN x WT tiles of 16 x 16.  The next
+// step's operands are on their way to registers while the matrix cores work on this one's in LDS (two buffers, one barrier a step).
+// LDS holds operands in the order the matrix cores' lanes read them, so a wavefront's reads and writes touch every bank alike.
+#pragma once
+
+#include "mx4_kernels.h"
+
+namespace pimhip
+{
+// Which tile a block has: consecutive blocks go to consecutive XCDs, each with an L2 of its own, so an XCD gets a run of tiles, down
+// a column of tokens first: they share the weights' rows.
+__device__ __forceinline__ void tile_of_block(int64_t tiles_n, int64_t tiles_t, int64_t& n, int64_t& t)
+{
+    constexpr int64_t kXcds = 8;
+    const int64_t all = tiles_n * tiles_t, id = blockIdx.x;
+    const int64_t per = all / kXcds, more = all % kXcds, xcd = id % kXcds;
+    const int64_t at = xcd * per + (xcd < more ? xcd : more) + id / kXcds;
+    n = at / tiles_t;
+    t = at % tiles_t;
+}
+
+// ---- x in 16 bits, weights in 4 ----------------------------------------------------------------------------------------------
+// Steps of 64 values of k.  Weights stay packed in LDS and are converted on the way to the matrix cores: a quarter of the LDS reads of
+// converted ones.
+template <class T, int WN, int WT, int GN, int GT>
+__global__ __launch_bounds__(64 * GN * GT) void mx4_linear_tile_kernel(const typename T::elem* x, Mx4View w, const typename T::elem* bias, typename T::elem* out,
+                                                                       int64_t ld_x, int64_t ld_out, int64_t M, int relu)
+{
+    constexpr int kThreads = 64 * GN * GT, kN = 16 * GN * WN, kT = 16 * GT * WT;
+    constexpr int kX = kT * 8 / kThreads;    // 16-byte pieces of x a thread brings each step
+    constexpr int kW = kN * 2 / kThreads;    // blocks of weights
+    static_assert(kX * kThreads == kT * 8 && kW * kThreads == kN * 2, "whole pieces a thread");
+    typedef typename T::frag frag;
+    __shared__ frag xs[2][kT / 16][2][64];
+    __shared__ unsigned int ws[2][kN / 16][2][64];
+    __shared__ float ss[2][kN / 16][2][16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = lane >> 4;
+    const int wn = wave % GN * WN, wt = wave / GN * WT;
+    int64_t tile_n, tile_t;
+    tile_of_block((w.rows + kN - 1) / kN, (M + kT - 1) / kT, tile_n, tile_t);
+    const int64_t n0 = tile_n * kN, t0 = tile_t * kT, K = w.cols, blocks = (K + kMxBlock - 1) / kMxBlock;
+
+    const typename T::elem* xp[kX];
+    int xk[kX];
+#pragma unroll
+    for (int i = 0; i < kX; ++i) {
+        const int p = tid + i * kThreads, l = p & 63;
+        int64_t t = t0 + p / 128 * 16 + (l & 15);
+        t = t < M ? t : M - 1;
+        xk[i] = (p / 64 % 2) * 32 + (l >> 4) * 8;
+        xp[i] = x + t * ld_x;
+    }
+    const uint8_t *wp[kW], *sp[kW];
+    int top[kW];
+#pragma unroll
+    for (int i = 0; i < kW; ++i) {
+        int64_t n = n0 + (tid + i * kThreads) / 2;
+        n = n < w.rows ? n : w.rows - 1;
+        wp[i] = w.packed + (n * blocks + tid % 2) * kMxBlockBytes;
+        sp[i] = w.scales + n * w.ld_scales + tid % 2;
+        top[i] = w.tops[n];
+    }
+    frag xv[kX];
+    uint4_t wv[kW];
+    unsigned int wc[kW];
+    auto fetch = [&](int64_t step) {
+        const int64_t k0 = step * 64;
+        if (k0 + 64 <= K) {
+#pragma unroll
+            for (int i = 0; i < kX; ++i) xv[i] = load8_any<T>(xp[i] + k0 + xk[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kX; ++i) xv[i] = load8_guarded<T>(xp[i], k0 + xk[i], K);
+        }
+#pragma unroll
+        for (int i = 0; i < kW; ++i) {
+            wv[i] = uint4_t{0, 0, 0, 0};
+            wc[i] = 127;
+            if (step * 2 + tid % 2 < blocks) {
+                wv[i] = *reinterpret_cast<const uint4_t*>(wp[i] + step * (2 * kMxBlockBytes));
+                wc[i] = sp[i][step * 2];
+            }
+        }
+    };
+    auto put = [&](int buffer) {
+#pragma unroll
+        for (int i = 0; i < kX; ++i) (&xs[buffer][0][0][0])[tid + i * kThreads] = xv[i];
+#pragma unroll
+        for (int i = 0; i < kW; ++i) {
+            const int n = (tid + i * kThreads) / 2;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) ws[buffer][n / 16][tid % 2][g * 16 + n % 16] = wv[i][g];
+            ss[buffer][n / 16][tid % 2][n % 16] = T::scale(wc[i], top[i]);
+        }
+    };
+
+    float4_t acc[WN][WT] = {};
+    const int64_t steps = (K + 63) / 64;
+    fetch(0);
+    put(0);
+    __syncthreads();
+    for (int64_t s = 0; s < steps; ++s) {
+        const int b = (int)(s & 1);
+        if (s + 1 < steps) fetch(s + 1);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            frag xf[WT];
+#pragma unroll
+            for (int j = 0; j < WT; ++j) xf[j] = xs[b][wt + j][kk][lane];
+#pragma unroll
+            for (int i = 0; i < WN; ++i) {
+                const frag wf = T::from_mx4(ws[b][wn + i][kk][lane], ss[b][wn + i][kk][lane & 15]);
+#pragma unroll
+                for (int j = 0; j < WT; ++j) acc[i][j] = T::mfma(wf, xf[j], acc[i][j]);
+            }
+        }
+        if (s + 1 < steps) put(b ^ 1);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < WN; ++i) {
+        const int64_t n = n0 + (wn + i) * 16 + group * 4;
+        if (n >= w.rows) continue;
+        const int count = w.rows - n < 4 ? (int)(w.rows - n) : 4;
+        int tops[4] = {};
+        float add[4] = {};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (c < count) {
+                tops[c] = w.tops[n + c];
+                if (bias) add[c] = (float)bias[n + c];
+            }
+#pragma unroll
+        for (int j = 0; j < WT; ++j) {
+            const int64_t t = t0 + (wt + j) * 16 + (lane & 15);
+            if (t >= M) continue;
+            float4_t v = acc[i][j];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                v[c] = T::unscale(v[c], tops[c]);
+                if (bias) v[c] += add[c];
+                if (relu) v[c] = relu_f32(v[c]);
+            }
+            store4<T>(out + t * ld_out + n, v, count);
+        }
+    }
+}
+
+// ---- both operands in 4 bits -------------------------------------------------------------------------------------------------
+// Steps of 128 values of k, one product (v_mfma_scale_f32_16x16x128_f8f6f4) a tile: a lane holds one block of each operand.  The scale
+// codes of four tiles' blocks share a 32-bit word of LDS; the instruction picks its byte.
+template <class O, int WN, int WT, int GN, int GT>
+__global__ __launch_bounds__(64 * GN * GT) void mx4_matmul_tile_kernel(Mx4View a, Mx4View b, typename O::elem* out, int64_t ld_out)
+{
+    constexpr int kThreads = 64 * GN * GT, kN = 16 * GN * WN, kT = 16 * GT * WT, kRows = kN + kT;
+    constexpr int kPieces = kRows * 4 / kThreads;  // blocks of either operand a thread brings each step
+    static_assert(kPieces * kThreads == kRows * 4 && kRows <= kThreads && WN % 4 == 0 && WT % 4 == 0, "whole pieces a thread, a row of scales each");
+    __shared__ uint4_t values[2][kRows / 16][64];       // the rows of b, then those of a
+    __shared__ unsigned int codes[2][kRows / 64][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = lane >> 4;
+    const int wn = wave % GN * WN, wt = wave / GN * WT;
+    int64_t tile_n, tile_t;
+    tile_of_block((b.rows + kN - 1) / kN, (a.rows + kT - 1) / kT, tile_n, tile_t);
+    const int64_t n0 = tile_n * kN, t0 = tile_t * kT;
+    const int blocks = (int)((b.cols + kMxBlock - 1) / kMxBlock);
+    // Row r of the tile: its matrix, and its row there (the last one again behind the end).
+    const uint8_t* vp[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        const int r = (tid + i * kThreads) / 64 * 16 + (lane & 15);
+        const int64_t last = (r < kN ? b.rows : a.rows) - 1, at = r < kN ? n0 + r : t0 + r - kN;
+        vp[i] = (r < kN ? b.packed : a.packed) + ((at < last ? at : last) * blocks + group) * kMxBlockBytes;
+    }
+    const uint8_t* cp = nullptr;
+    if (tid < kRows) {
+        const int64_t last = (tid < kN ? b.rows : a.rows) - 1, at = tid < kN ? n0 + tid : t0 + tid - kN;
+        cp = (tid < kN ? b.scales : a.scales) + (at < last ? at : last) * (tid < kN ? b.ld_scales : a.ld_scales);
+    }
+    uint4_t v[kPieces];
+    unsigned int c = 0;
+    auto fetch = [&](int step) {
+        if (step * 4 + 4 <= blocks) {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) v[i] = *reinterpret_cast<const uint4_t*>(vp[i] + (int64_t)step * (4 * kMxBlockBytes));
+            if (tid < kRows) c = *reinterpret_cast<const unsigned int*>(cp + step * 4);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                v[i] = uint4_t{0, 0, 0, 0};
+                if (step * 4 + group < blocks) v[i] = *reinterpret_cast<const uint4_t*>(vp[i] + (int64_t)step * (4 * kMxBlockBytes));
+            }
+            // (whole groups of 16 codes a row) Behind the row's last block: any code but "not a number".
+            if (tid < kRows) {
+                c = *reinterpret_cast<const unsigned int*>(cp + step * 4);
+                const unsigned int in = (1u << (8 * (blocks - step * 4))) - 1;
+                c = (c & in) | (0x7f7f7f7fu & ~in);
+            }
+        }
+    };
+    auto put = [&](int buffer) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) (&values[buffer][0][0])[tid + i * kThreads] = v[i];
+        if (tid < kRows) {
+            uint8_t* to = reinterpret_cast<uint8_t*>(&codes[buffer][tid / 64][tid % 16]) + tid / 16 % 4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[i * 64] = (uint8_t)(c >> (8 * i));
+        }
+    };
+    float4_t acc[WN][WT] = {};
+    const int steps = (blocks + 3) / 4;
+    fetch(0);
+    put(0);
+    __syncthreads();
+    for (int s = 0; s < steps; ++s) {
+        const int buffer = s & 1;
+        if (s + 1 < steps) fetch(s + 1);
+        int8v_t af[WT];
+        int ac[WT / 4];
+#pragma unroll
+        for (int j = 0; j < WT; ++j) {
+            const uint4_t q = values[buffer][kN / 16 + wt + j][lane];
+            af[j] = int8v_t{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int j = 0; j < WT / 4; ++j) ac[j] = (int)codes[buffer][kN / 64 + wt / 4 + j][lane];
+#define PIMHIP_MX_PRODUCT(I, J) \
+    acc[i4 + I][j4 * 4 + J] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[I], af[j4 * 4 + J], acc[i4 + I][j4 * 4 + J], 4, 4, I, bc, J, ac[j4]);
+#define PIMHIP_MX_ROW(I) PIMHIP_MX_PRODUCT(I, 0) PIMHIP_MX_PRODUCT(I, 1) PIMHIP_MX_PRODUCT(I, 2) PIMHIP_MX_PRODUCT(I, 3)
+#pragma unroll
+        for (int i4 = 0; i4 < WN; i4 += 4) {
+            int8v_t bf[4];
+            const int bc = (int)codes[buffer][(wn + i4) / 4][lane];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint4_t q = values[buffer][wn + i4 + i][lane];
+                bf[i] = int8v_t{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int j4 = 0; j4 < WT / 4; ++j4) {
+                PIMHIP_MX_ROW(0)
+                PIMHIP_MX_ROW(1)
+                PIMHIP_MX_ROW(2)
+                PIMHIP_MX_ROW(3)
+            }
+        }
+#undef PIMHIP_MX_ROW
+#undef PIMHIP_MX_PRODUCT
+        if (s + 1 < steps) put(buffer ^ 1);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < WN; ++i) {
+        const int64_t n = n0 + (wn + i) * 16 + group * 4;
+        if (n >= b.rows) continue;
+#pragma unroll
+        for (int j = 0; j < WT; ++j) {
+            const int64_t t = t0 + (wt + j) * 16 + (lane & 15);
+            if (t < a.rows) store4<O>(out + t * ld_out + n, acc[i][j], b.rows - n < 4 ? (int)(b.rows - n) : 4);
+        }
+    }
+}
+}  // namespace pimhip
