@@ -48,10 +48,10 @@ void launch(const PimHipMoeLayerPlan* p, const MoeLayerArgs& a, hipStream_t s)
     moe_layer_router_kernel<T><<<dim3((unsigned)a.tokens), 256, 0, s>>>(a);
     const unsigned E = (unsigned)a.E;
     if (p->gated)
-        moe_layer_first_kernel<T, MX, true, 1, 4><<<dim3((unsigned)((a.d_ff + 15) / 16), E), 256, 0, s>>>(a);
+        moe_layer_first_kernel<T, MX, true, 1, 2, 4><<<dim3((unsigned)((a.d_ff + 15) / 16), E), 256, 0, s>>>(a);
     else
-        moe_layer_first_kernel<T, MX, false, 2, 4><<<dim3((unsigned)((a.d_ff + 31) / 32), E), 256, 0, s>>>(a);
-    moe_layer_second_kernel<T, MX, 1, 4><<<dim3((unsigned)((a.d_model + 15) / 16), E), 256, 0, s>>>(a);
+        moe_layer_first_kernel<T, MX, false, 2, 2, 4><<<dim3((unsigned)((a.d_ff + 31) / 32), E), 256, 0, s>>>(a);
+    moe_layer_second_kernel<T, MX, 1, 2, 4><<<dim3((unsigned)((a.d_model + 15) / 16), E), 256, 0, s>>>(a);
     moe_layer_sum_kernel<T><<<dim3((unsigned)((a.d_model + 1023) / 1024), (unsigned)a.tokens), 256, 0, s>>>(a);
 }
 }  // namespace

@@ -37,13 +37,20 @@ int check_grid(int64_t x, int64_t y)
     return PIMHIP_OK;
 }
 
-template <class T, int RT, int TT, int U, int WK>
+// LDS of a launch's staged tokens, in bytes.
+template <class T>
+int64_t shared_tokens_bytes(int64_t M, int64_t K)
+{
+    return M * SharedTokens<T>::pitch((int)K, Mx4Weights<T>::kUnit) * 16;
+}
+
+template <class T, bool SHARED, int RT, int TT, int U, int WK>
 int linear_skinny(void* out, int64_t ld_out, const void* x, int64_t ld_x, int64_t M, const Mx4View& w, const void* bias, int relu, hipStream_t s)
 {
     const int64_t gx = (w.rows + 16 * RT - 1) / (16 * RT), gy = (M + 16 * TT - 1) / (16 * TT);
     const int rc = check_grid(gx, gy);
     if (rc != PIMHIP_OK) return rc;
-    mx4_linear_skinny_kernel<T, RT, TT, U, WK><<<dim3((unsigned)gx, (unsigned)gy), 64 * WK, 0, s>>>(
+    mx4_linear_skinny_kernel<T, SHARED, RT, TT, U, WK><<<dim3((unsigned)gx, (unsigned)gy), 64 * WK, SHARED ? shared_tokens_bytes<T>(M, w.cols) : 0, s>>>(
         (const typename T::elem*)x, w, (const typename T::elem*)bias, (typename T::elem*)out, ld_x, ld_out, M, relu);
     return PIMHIP_OK;
 }
@@ -51,9 +58,24 @@ int linear_skinny(void* out, int64_t ld_out, const void* x, int64_t ld_x, int64_
 template <class T>
 int linear(void* out, int64_t ld_out, const void* x, int64_t ld_x, int64_t M, const Mx4View& w, const void* bias, int relu, hipStream_t s)
 {
-    if (M <= 16) return linear_skinny<T, 1, 1, 2, 4>(out, ld_out, x, ld_x, M, w, bias, relu, s);
-    if (M <= 32) return linear_skinny<T, 1, 2, 1, 4>(out, ld_out, x, ld_x, M, w, bias, relu, s);
-    if (M <= 64) return linear_skinny<T, 1, 4, 1, 4>(out, ld_out, x, ld_x, M, w, bias, relu, s);
+    // Rows a wavefront has at a time, and wavefronts that share k.  More rows read x less often but make fewer blocks, more wavefronts
+    // the opposite.  Measured on 16384 x 4096 / 4096 x 4096 / 31999 x 1024, weights that no cache holds, in us:
+    //   one token (staged in LDS)   1 tile of 16 rows, 8 wavefronts 10.5 / 4.9 / -      2 tiles, 8: 8.7 / 5.9 / -     (turned by the wavefronts: 12.0 / 5.6)
+    //   16 tokens                   1 tile, 8: 16.1 / 6.3 / 12.9      4 tiles, 8: 10.7 / 9.3 / 10.5      4 tiles, 4: 11.3 / 10.4 / 7.3
+    constexpr int64_t kShared = 32 << 10;
+    const int64_t tiles16 = (w.rows + 15) / 16;
+    const bool long_rows = w.cols > 4 * Mx4Weights<T>::kUnit;
+    auto go = [&](auto kernel) { return kernel(out, ld_out, x, ld_x, M, w, bias, relu, s); };
+    if (M <= 2 && shared_tokens_bytes<T>(M, w.cols) <= kShared) {
+        if (tiles16 < 768) return long_rows ? go(linear_skinny<T, true, 1, 1, 1, 8>) : go(linear_skinny<T, true, 1, 1, 1, 4>);
+        return long_rows ? go(linear_skinny<T, true, 2, 1, 1, 8>) : go(linear_skinny<T, true, 2, 1, 1, 4>);
+    }
+    if (M <= 16) {
+        if (tiles16 < 512) return long_rows ? go(linear_skinny<T, false, 1, 1, 1, 8>) : go(linear_skinny<T, false, 1, 1, 1, 4>);
+        return long_rows ? go(linear_skinny<T, false, 4, 1, 1, 8>) : go(linear_skinny<T, false, 4, 1, 1, 4>);
+    }
+    if (M <= 32) return tiles16 < 512 ? go(linear_skinny<T, false, 1, 2, 1, 4>) : go(linear_skinny<T, false, 4, 2, 1, 4>);
+    if (M <= 64) return tiles16 < 512 ? go(linear_skinny<T, false, 1, 4, 1, 4>) : go(linear_skinny<T, false, 4, 4, 1, 4>);
     const int64_t tiles = ((w.rows + 127) / 128) * ((M + 127) / 128);
     const int rc = check_grid(tiles, 1);
     if (rc != PIMHIP_OK) return rc;

@@ -133,48 +133,46 @@ struct ExpertWeights;
 template <class T>
 struct ExpertWeights<T, false> {
     typedef DenseWeights<T> W;
-    static __device__ __forceinline__ typename W::Row row(const void* w, const void*, const void*, int64_t r, int K, int, int group)
+    static __device__ __forceinline__ typename W::Rows rows(const void* w, const void*, const void*, int, int64_t first, int64_t count, int K)
     {
-        return {(const typename T::elem*)w + r * K + group * 32};
+        return W::rows(w, first, count, K);
     }
     static __device__ __forceinline__ float unscale(float v, const void*, int64_t) { return v; }
 };
 template <class T>
 struct ExpertWeights<T, true> {
     typedef Mx4Weights<T> W;
-    static __device__ __forceinline__ typename W::Row row(const void* w, const void* s, const void* t, int64_t r, int K, int ld, int group)
+    static __device__ __forceinline__ typename W::Rows rows(const void* w, const void* s, const void* t, int ld, int64_t first, int64_t count, int K)
     {
-        const int64_t blocks = (K + kMxBlock - 1) / kMxBlock;
-        return {(const uint8_t*)w + (r * blocks + group) * kMxBlockBytes, (const uint8_t*)s + r * ld, ((const uint8_t*)t)[r]};
+        return W::rows((const uint8_t*)w, (const uint8_t*)s, (const uint8_t*)t, ld, first, count, K);
     }
     static __device__ __forceinline__ float unscale(float v, const void* t, int64_t r) { return T::unscale(v, ((const uint8_t*)t)[r]); }
 };
 
 // The first product of 16 * TT pairs: hidden values 16 * F a block, each with its gate where there is one.
-template <class T, bool MX, bool GATED, int F, int TT, int WK>
+template <class T, bool MX, bool GATED, int F, int TT, int U, int WK>
 __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPointers& p, const short* list, int n, float4_t* part)
 {
     constexpr int RT = GATED ? 2 * F : F;
     typedef ExpertWeights<T, MX> EW;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4;
     const int f0 = blockIdx.x * (16 * F);
-    typename EW::W::Row rows[RT];
+    typedef TurnedTokens<T> X;
+    typename EW::W::Rows rows[RT];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        int f = f0 + i % F * 16 + (lane & 15);
-        f = f < a.d_ff ? f : a.d_ff - 1;
-        rows[i] = EW::row(p.w1, p.s1, p.t1, i < F ? f : a.d_ff + f, a.d_model, a.ld_s1, group);
-    }
-    const typename T::elem* tokens[TT];
+    for (int i = 0; i < RT; ++i)  // (value rows follow the gate rows; each kind ends at its own last row)
+        rows[i] = EW::rows(p.w1, p.s1, p.t1, a.ld_s1, (i < F ? 0 : a.d_ff) + f0 + i % F * 16, i < F ? a.d_ff : 2 * a.d_ff, a.d_model);
+    typename X::Rows tokens[TT];
     int pair[TT];
 #pragma unroll
     for (int j = 0; j < TT; ++j) {
-        const int i = j * 16 + (lane & 15);
-        pair[j] = i < n ? list[i] : -1;
-        tokens[j] = (const typename T::elem*)a.x + (int64_t)(list[i < n ? i : n - 1] / a.top_k) * a.ld_x + group * 32;
+        pair[j] = j * 16 + (lane & 15) < n ? list[j * 16 + (lane & 15)] : -1;
+        tokens[j] = X::rows([&](int i) { return (const typename T::elem*)a.x + (int64_t)(list[j * 16 + i < n ? j * 16 + i : n - 1] / a.top_k) * a.ld_x; });
     }
     float4_t acc[RT][TT] = {};
-    skinny_sum<T, typename EW::W, RT, TT, 1>(acc, rows, tokens, a.d_model, wave, WK);
+    constexpr int kLds = kSkinnyLds<typename EW::W, X>;
+    skinny_sum<T, typename EW::W, X, RT, TT, U>(acc, rows, tokens, a.d_model, wave, WK, reinterpret_cast<uint4_t*>(part) + wave * kLds, [] {});
+    __syncthreads();
     // Gate and value of a hidden unit have to meet: the sums are joined in every wavefront that finishes a tile of them.
 #pragma unroll
     for (int i = 0; i < RT; ++i)
@@ -213,10 +211,14 @@ __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPoi
     __syncthreads();
 }
 
-template <class T, bool MX, bool GATED, int F, int WK>
+// LDS of a product's block: what its wavefronts turn operands in, then their sums.
+template <class T, bool MX, int RT, int WK>
+constexpr int kExpertLds = WK * (kSkinnyLds<typename ExpertWeights<T, MX>::W, TurnedTokens<T>> > RT * 4 * 64 ? kSkinnyLds<typename ExpertWeights<T, MX>::W, TurnedTokens<T>> : RT * 4 * 64);
+
+template <class T, bool MX, bool GATED, int F, int U, int WK>
 __global__ __launch_bounds__(64 * WK) void moe_layer_first_kernel(MoeLayerArgs a)
 {
-    __shared__ float4_t part[WK * (GATED ? 2 * F : F) * 4 * 64];
+    __shared__ float4_t part[kExpertLds<T, MX, GATED ? 2 * F : F, WK>];
     __shared__ short list[kMoeLayerPairs];
     __shared__ int count;
     const int e = blockIdx.y;
@@ -224,37 +226,34 @@ __global__ __launch_bounds__(64 * WK) void moe_layer_first_kernel(MoeLayerArgs a
     if (n == 0) return;
     const ExpertPointers p = a.experts[e];
     if (n <= 16)
-        moe_first<T, MX, GATED, F, 1, WK>(a, p, list, n, part);
+        moe_first<T, MX, GATED, F, 1, U, WK>(a, p, list, n, part);
     else if (n <= 32)
-        moe_first<T, MX, GATED, F, 2, WK>(a, p, list, n, part);
+        moe_first<T, MX, GATED, F, 2, 1, WK>(a, p, list, n, part);
     else
-        moe_first<T, MX, GATED, F, 4, WK>(a, p, list, n, part);
+        moe_first<T, MX, GATED, F, 4, 1, WK>(a, p, list, n, part);
 }
 
 // The second product of 16 * TT pairs: rows of d_model, with the bias, not yet weighted.
-template <class T, bool MX, int RT, int TT, int WK>
+template <class T, bool MX, int RT, int TT, int U, int WK>
 __device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPointers& p, const short* list, int n, float4_t* part)
 {
     typedef ExpertWeights<T, MX> EW;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4;
     const int d0 = blockIdx.x * (16 * RT);
-    typename EW::W::Row rows[RT];
+    typedef TurnedTokens<T> X;
+    typename EW::W::Rows rows[RT];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        int d = d0 + i * 16 + (lane & 15);
-        d = d < a.d_model ? d : a.d_model - 1;
-        rows[i] = EW::row(p.w2, p.s2, p.t2, d, a.d_ff, a.ld_s2, group);
-    }
-    const typename T::elem* hidden[TT];
+    for (int i = 0; i < RT; ++i) rows[i] = EW::rows(p.w2, p.s2, p.t2, a.ld_s2, d0 + i * 16, a.d_model, a.d_ff);
+    typename X::Rows hidden[TT];
     int pair[TT];
 #pragma unroll
     for (int j = 0; j < TT; ++j) {
-        const int i = j * 16 + (lane & 15);
-        pair[j] = i < n ? list[i] : -1;
-        hidden[j] = (const typename T::elem*)a.h + (int64_t)list[i < n ? i : n - 1] * a.d_ff + group * 32;
+        pair[j] = j * 16 + (lane & 15) < n ? list[j * 16 + (lane & 15)] : -1;
+        hidden[j] = X::rows([&](int i) { return (const typename T::elem*)a.h + (int64_t)list[j * 16 + i < n ? j * 16 + i : n - 1] * a.d_ff; });
     }
     float4_t acc[RT][TT] = {};
-    skinny_sum<T, typename EW::W, RT, TT, 1>(acc, rows, hidden, a.d_ff, wave, WK);
+    constexpr int kLds = kSkinnyLds<typename EW::W, X>;
+    skinny_sum<T, typename EW::W, X, RT, TT, U>(acc, rows, hidden, a.d_ff, wave, WK, reinterpret_cast<uint4_t*>(part) + wave * kLds, [] {});
     skinny_join<RT, TT, WK>(acc, part);
 #pragma unroll
     for (int i = 0; i < RT; ++i)
@@ -272,10 +271,10 @@ __device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPo
         }
 }
 
-template <class T, bool MX, int RT, int WK>
+template <class T, bool MX, int RT, int U, int WK>
 __global__ __launch_bounds__(64 * WK) void moe_layer_second_kernel(MoeLayerArgs a)
 {
-    __shared__ float4_t part[WK * RT * 4 * 64];
+    __shared__ float4_t part[kExpertLds<T, MX, RT, WK>];
     __shared__ short list[kMoeLayerPairs];
     __shared__ int count;
     const int e = blockIdx.y;
@@ -283,11 +282,11 @@ __global__ __launch_bounds__(64 * WK) void moe_layer_second_kernel(MoeLayerArgs 
     if (n == 0) return;
     const ExpertPointers p = a.experts[e];
     if (n <= 16)
-        moe_second<T, MX, RT, 1, WK>(a, p, list, n, part);
+        moe_second<T, MX, RT, 1, U, WK>(a, p, list, n, part);
     else if (n <= 32)
-        moe_second<T, MX, RT, 2, WK>(a, p, list, n, part);
+        moe_second<T, MX, RT, 2, 1, WK>(a, p, list, n, part);
     else
-        moe_second<T, MX, RT, 4, WK>(a, p, list, n, part);
+        moe_second<T, MX, RT, 4, 1, WK>(a, p, list, n, part);
 }
 
 // The weighted sum in the order of the choice.  An expert without a share adds nothing, whatever it computed.

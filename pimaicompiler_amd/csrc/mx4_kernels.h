@@ -1,6 +1,8 @@
 // Kernels on microscaled 4-bit values (mx4_format.h): quantisation, reading back, and the products with one or both operands in 4 bits.
 #pragma once
 
+#include <type_traits>
+
 #include "skinny.h"
 
 namespace pimhip
@@ -164,32 +166,47 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint8_t* pack
 }
 
 // ---- x in 16 bits, weights in 4: a few tokens --------------------------------------------------------------------------------
-// y[m, n] = act(sum_k x[m, k] w[n, k] + b[n]).  WK wavefronts share k of 16 * RT rows and up to 16 * TT tokens (skinny.h).
-template <class T, int RT, int TT, int U, int WK>
+// y[m, n] = act(sum_k x[m, k] w[n, k] + b[n]).  WK wavefronts share k of 16 * RT rows and up to 16 * TT tokens (skinny.h).  SHARED: the
+// tokens (at most 16) lie in LDS as a whole, in the launch's dynamic part of it.
+template <class T, bool SHARED, int RT, int TT, int U, int WK>
 __global__ __launch_bounds__(64 * WK) void mx4_linear_skinny_kernel(const typename T::elem* x, Mx4View w, const typename T::elem* bias, typename T::elem* out,
                                                                     int64_t ld_x, int64_t ld_out, int64_t M, int relu)
 {
-    __shared__ float4_t part[WK > 1 ? WK * RT * TT * 64 : 1];
+    typedef Mx4Weights<T> W;
+    typedef typename std::conditional<SHARED, SharedTokens<T>, TurnedTokens<T>>::type X;
+    constexpr int kLds = kSkinnyLds<W, X>, kPart = RT * TT * 64;
+    __shared__ uint4_t lds[WK * (kLds > kPart ? kLds : kPart)];
+    __shared__ int tops[RT * 16];
+    __shared__ float add[RT * 16];
+    extern __shared__ uint4_t xs[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4;
     const int64_t row0 = (int64_t)blockIdx.x * (16 * RT), token0 = (int64_t)blockIdx.y * (16 * TT);
-    const int64_t blocks = (w.cols + kMxBlock - 1) / kMxBlock;
-    typename Mx4Weights<T>::Row rows[RT];
+    typename W::Rows rows[RT];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        int64_t r = row0 + i * 16 + (lane & 15);
-        r = r < w.rows ? r : w.rows - 1;
-        rows[i] = {w.packed + (r * blocks + group) * kMxBlockBytes, w.scales + r * w.ld_scales, w.tops[r]};
-    }
-    const typename T::elem* tokens[TT];
+    for (int i = 0; i < RT; ++i) rows[i] = W::rows(w.packed, w.scales, w.tops, w.ld_scales, row0 + i * 16, w.rows, w.cols);
+    auto token = [&](int64_t t) { return x + (t < M ? t : M - 1) * ld_x; };
+    const int K = (int)w.cols, pitch = SharedTokens<T>::pitch(K, W::kUnit);
+    typename X::Rows tokens[TT];
 #pragma unroll
     for (int j = 0; j < TT; ++j) {
-        int64_t t = token0 + j * 16 + (lane & 15);
-        t = t < M ? t : M - 1;
-        tokens[j] = x + t * ld_x + group * 32;
+        if constexpr (SHARED)
+            tokens[j] = X::rows(xs, (lane & 15) < M ? lane & 15 : (int)M - 1, pitch);
+        else
+            tokens[j] = X::rows([&](int i) { return token(token0 + j * 16 + i); });
+    }
+    // What the results of a row need goes to LDS for the wavefronts that finish them.
+    if (threadIdx.x < 16 * RT) {
+        int64_t n = row0 + threadIdx.x;
+        n = n < w.rows ? n : w.rows - 1;
+        tops[threadIdx.x] = w.tops[n];
+        add[threadIdx.x] = bias ? (float)bias[n] : 0.0f;
     }
     float4_t acc[RT][TT] = {};
-    skinny_sum<T, Mx4Weights<T>, RT, TT, U>(acc, rows, tokens, (int)w.cols, wave, WK);
-    skinny_join<RT, TT, WK>(acc, part);
+    skinny_sum<T, W, X, RT, TT, U>(acc, rows, tokens, K, wave, WK, lds + wave * kLds, [&] {
+        if constexpr (SHARED) SharedTokens<T>::stage(xs, token, (int)M, K, pitch);
+        __syncthreads();
+    });
+    skinny_join<RT, TT, WK>(acc, reinterpret_cast<float4_t*>(lds));
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -197,16 +214,14 @@ __global__ __launch_bounds__(64 * WK) void mx4_linear_skinny_kernel(const typena
             if (WK > 1 && (i * TT + j) % WK != wave) continue;
             const int64_t t = token0 + j * 16 + (lane & 15), n = row0 + i * 16 + group * 4;
             if (t >= M || n >= w.rows) continue;
-            const int count = w.rows - n < 4 ? (int)(w.rows - n) : 4;
             float4_t v = acc[i][j];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                if (c >= count) continue;
-                v[c] = T::unscale(v[c], w.tops[n + c]);
-                if (bias) v[c] += (float)bias[n + c];
+                v[c] = T::unscale(v[c], tops[i * 16 + group * 4 + c]);
+                if (bias) v[c] += add[i * 16 + group * 4 + c];  // (a zero that is no bias would turn -0 into 0)
                 if (relu) v[c] = relu_f32(v[c]);
             }
-            store4<T>(out + t * ld_out + n, v, count);
+            store4<T>(out + t * ld_out + n, v, w.rows - n < 4 ? (int)(w.rows - n) : 4);
         }
 }
 
