@@ -23,6 +23,8 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 size_t hidden_bytes(const PimHipMoeLayerPlan* p, int tokens) { return round256((size_t)tokens * p->top_k * p->d_ff * 2); }
 size_t part_bytes(const PimHipMoeLayerPlan* p, int tokens) { return round256((size_t)tokens * p->top_k * p->d_model * sizeof(float)); }
 
+size_t counter_bytes(const PimHipMoeLayerPlan* p) { return (size_t)(p->d_model + 15) / 16 * sizeof(unsigned int); }
+
 int destroy_moe_layer_plan_locked(PimHipMoeLayerPlan* plan)
 {
     if (!plan) return PIMHIP_OK;
@@ -42,17 +44,54 @@ int destroy_moe_layer_plan_locked(PimHipMoeLayerPlan* plan)
     return PIMHIP_OK;
 }
 
+// LDS that staging the tokens of a product over K values takes, in bytes.
 template <class T, bool MX>
-void launch(const PimHipMoeLayerPlan* p, const MoeLayerArgs& a, hipStream_t s)
+unsigned int shared_bytes(const MoeLayerArgs& a, int K)
 {
-    moe_layer_router_kernel<T><<<dim3((unsigned)a.tokens), 256, 0, s>>>(a);
-    const unsigned E = (unsigned)a.E;
-    if (p->gated)
-        moe_layer_first_kernel<T, MX, true, 1, 2, 4><<<dim3((unsigned)((a.d_ff + 15) / 16), E), 256, 0, s>>>(a);
+    return (unsigned int)(a.tokens * SharedTokens<T>::pitch(K, ExpertWeights<T, MX, 1>::W::kUnit) * 16);
+}
+
+template <class T, bool MX, bool SHARED, bool GATED, int F, int TT>
+void launch_first(const MoeLayerArgs& a, hipStream_t s)
+{
+    constexpr int WK = 4;
+    moe_layer_first_kernel<T, MX, SHARED, GATED, F, TT, WK>
+        <<<dim3((unsigned)((a.d_ff + 16 * F - 1) / (16 * F)), (unsigned)a.E), 64 * WK, SHARED ? shared_bytes<T, MX>(a, a.d_model) : 0, s>>>(a);
+}
+
+template <class T, bool MX, bool SHARED, int RT, int TT, int WK>
+void launch_second(const MoeLayerArgs& a, hipStream_t s)
+{
+    moe_layer_second_kernel<T, MX, SHARED, RT, TT, WK>
+        <<<dim3((unsigned)((a.d_model + 16 * RT - 1) / (16 * RT)), (unsigned)a.E), 64 * WK, SHARED ? shared_bytes<T, MX>(a, a.d_ff) : 0, s>>>(a);
+}
+
+template <class T, bool MX, bool SHARED, int TT>
+void launch(const PimHipMoeLayerPlan* p, MoeLayerArgs& a, hipStream_t s)
+{
+    a.counters_used = (a.d_model + 15) / 16;
+    moe_layer_router_kernel<T><<<dim3((unsigned)a.tokens), kRouterThreads, 0, s>>>(a);
+    p->gated ? launch_first<T, MX, SHARED, true, TT, TT>(a, s) : launch_first<T, MX, SHARED, false, 2 * TT, TT>(a, s);
+    // Blocks of the second product that have something to read.  Where they fill the card several times over a block has two tiles of
+    // rows, else one, and more wavefronts share its long k.
+    const int active = a.E < a.tokens * a.top_k ? a.E : a.tokens * a.top_k;
+    const int64_t blocks = (int64_t)((a.d_model + 15) / 16) * active;
+    if (blocks >= 2048)
+        launch_second<T, MX, SHARED, 2, TT, 4>(a, s);
     else
-        moe_layer_first_kernel<T, MX, false, 2, 2, 4><<<dim3((unsigned)((a.d_ff + 31) / 32), E), 256, 0, s>>>(a);
-    moe_layer_second_kernel<T, MX, 1, 2, 4><<<dim3((unsigned)((a.d_model + 15) / 16), E), 256, 0, s>>>(a);
-    moe_layer_sum_kernel<T><<<dim3((unsigned)((a.d_model + 1023) / 1024), (unsigned)a.tokens), 256, 0, s>>>(a);
+        launch_second<T, MX, SHARED, 1, TT, 8>(a, s);
+}
+
+template <class T, bool MX>
+void launch(const PimHipMoeLayerPlan* p, MoeLayerArgs& a, hipStream_t s)
+{
+    constexpr unsigned int kShared = 20 << 10;  // (a block of the turned kind has 35 KB: four on a CU either way)
+    if (a.tokens <= 2 && shared_bytes<T, MX>(a, a.d_model) <= kShared && shared_bytes<T, MX>(a, a.d_ff) <= kShared)
+        launch<T, MX, true, 1>(p, a, s);
+    else if (a.tokens <= 16)
+        launch<T, MX, false, 1>(p, a, s);
+    else
+        launch<T, MX, false, 2>(p, a, s);
 }
 }  // namespace
 
@@ -147,7 +186,7 @@ extern "C" int pimhip_moe_layer_workspace_bytes(const PimHipMoeLayerPlan* plan, 
 {
     if (!plan || !bytes) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "plan and bytes must be non-null");
     if (tokens < 0 || tokens > kMoeLayerTokens) return fail(PIMHIP_ERR_UNSUPPORTED, "tokens=%d not in [0, %d]", tokens, kMoeLayerTokens);
-    *bytes = hidden_bytes(plan, tokens) + part_bytes(plan, tokens);
+    *bytes = hidden_bytes(plan, tokens) + part_bytes(plan, tokens) + counter_bytes(plan);
     return PIMHIP_OK;
 }
 
@@ -176,6 +215,7 @@ extern "C" int pimhip_moe_layer_forward(PimHipMoeLayerPlan* plan, const void* x,
     a.chosen = experts, a.share = shares;
     a.h = workspace;
     a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + hidden_bytes(plan, tokens));
+    a.counters = reinterpret_cast<unsigned int*>(static_cast<char*>(workspace) + hidden_bytes(plan, tokens) + part_bytes(plan, tokens));
     a.tokens = tokens, a.E = plan->num_experts, a.top_k = plan->top_k, a.d_model = (int)plan->d_model, a.d_ff = (int)plan->d_ff;
     a.ld_x = tokens > 1 ? (int)ld_x : 0;
     a.ld_s1 = (int)plan->ld_s1, a.ld_s2 = (int)plan->ld_s2;

@@ -6,7 +6,7 @@ using namespace pimhip;
 
 namespace
 {
-constexpr int64_t kMaxCols = 1 << 30;
+constexpr int64_t kMaxCols = 1 << 28;  // (16 rows' bytes are counted in 32 bits)
 
 int check_matrix(const char* name, const PimHipMx4Matrix* m, Mx4View* v)
 {
@@ -41,7 +41,7 @@ int check_grid(int64_t x, int64_t y)
 template <class T>
 int64_t shared_tokens_bytes(int64_t M, int64_t K)
 {
-    return M * SharedTokens<T>::pitch((int)K, Mx4Weights<T>::kUnit) * 16;
+    return M * SharedTokens<T>::pitch((int)K, Mx4Weights<T, 2>::kUnit) * 16;
 }
 
 template <class T, bool SHARED, int RT, int TT, int U, int WK>
@@ -64,7 +64,7 @@ int linear(void* out, int64_t ld_out, const void* x, int64_t ld_x, int64_t M, co
     //   16 tokens                   1 tile, 8: 16.1 / 6.3 / 12.9      4 tiles, 8: 10.7 / 9.3 / 10.5      4 tiles, 4: 11.3 / 10.4 / 7.3
     constexpr int64_t kShared = 32 << 10;
     const int64_t tiles16 = (w.rows + 15) / 16;
-    const bool long_rows = w.cols > 4 * Mx4Weights<T>::kUnit;
+    const bool long_rows = w.cols > 4 * Mx4Weights<T, 2>::kUnit;
     auto go = [&](auto kernel) { return kernel(out, ld_out, x, ld_x, M, w, bias, relu, s); };
     if (M <= 2 && shared_tokens_bytes<T>(M, w.cols) <= kShared) {
         if (tiles16 < 768) return long_rows ? go(linear_skinny<T, true, 1, 1, 1, 8>) : go(linear_skinny<T, true, 1, 1, 1, 4>);

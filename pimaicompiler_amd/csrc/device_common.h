@@ -116,6 +116,20 @@ __device__ __forceinline__ float wave_sum(float v)
     return wave_sum_rows(v);
 }
 
+// Maximum over the 64 lanes of a wavefront; every lane returns it.
+__device__ __forceinline__ unsigned int wave_max_u32(unsigned int v)
+{
+    auto larger = [](unsigned int p, unsigned int q) { return p > q ? p : q; };
+    v = larger(v, dpp_u32<kDppQuadXor1>(v));
+    v = larger(v, dpp_u32<kDppQuadXor2>(v));
+    v = larger(v, dpp_u32<kDppRowHalfMirror>(v));
+    v = larger(v, dpp_u32<kDppRowMirror>(v));
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = larger(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return larger(b[0], b[1]);
+}
+
 // The XCD a wavefront runs on: HW_REG_XCC_ID (hardware register 20), bits 3:0.  The probe that reports the placement of a
 // launch and the kernel that relies on it read it through this one function.
 static constexpr unsigned int kXccIdMask = 15u;
@@ -147,6 +161,9 @@ __device__ __forceinline__ bool wait_clock_expired(unsigned int spins, unsigned 
     }
     return now - t_first > kWaitTicks;
 }
+
+// The wavefront's number in its block, as a scalar: what is computed from it is computed once and branches on it are the wavefront's.
+__device__ __forceinline__ int wave_in_block() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
 
 // One 16-byte device-scope load.  Each 8-byte half is validated on its own by the caller, so nothing depends on the
 // 16 bytes being read as a unit.

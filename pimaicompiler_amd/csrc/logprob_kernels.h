@@ -74,7 +74,7 @@ __global__ __launch_bounds__(THREADS) void token_log_probs_kernel(LogProbArgs a)
     __shared__ unsigned long long candidates[kTopCandidates];
     __shared__ unsigned long long bound, found;
     __shared__ int count;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_in_block();
     const int64_t row = blockIdx.x, V = a.V;
     const typename T::elem* x = (const typename T::elem*)a.logits + row * a.ld;
     const int64_t pieces = (V + 7) / 8;

@@ -5,8 +5,8 @@
 //   y = sum_{j in S} c_j (W2_j act(W1_j x + b1_j) + b2_j)      gated: act(g) * u with [g; u] = W1_j x + b1_j
 //
 // Bound by the weights of the experts that some token chose, each read once: the router, then one launch per product in which a block
-// has some rows of one expert and all tokens that chose it (skinny.h), then the sum.  A block finds its tokens in the router's
-// table (at most kMoeLayerPairs entries) by itself; one whose expert nobody chose ends at once.
+// has some rows of one expert and all tokens that chose it (skinny.h).  A block finds its tokens in the router's table (at most
+// kMoeLayerPairs entries) by itself; one whose expert nobody chose has nothing to read.
 #pragma once
 
 #include "skinny.h"
@@ -32,74 +32,100 @@ struct MoeLayerArgs {
     float* share;     // [tokens][top_k]
     void* h;          // [pairs][d_ff]: hidden values, rounded to x's type as operands of the matrix cores
     float* part;      // [pairs][d_model]
+    unsigned int* counters;  // blocks of the second product that are done with a tile of rows
+    int counters_used;
     int tokens, E, top_k, d_model, d_ff, ld_x;
     int ld_s1, ld_s2;  // pitches of 4-bit weights' scale codes
     int act, renormalize;
 };
 
 // ---- router ------------------------------------------------------------------------------------------------------------------
-// One token a block: a wavefront an expert at a time, then the choice by the first wavefront.
+// One token a block.  A wavefront has four experts at a time and 1024 values of each, whose loads do not wait for one another; the first
+// one chooses.
+static constexpr int kRouterThreads = 1024;
+
 template <class T>
-__global__ __launch_bounds__(256) void moe_layer_router_kernel(MoeLayerArgs a)
+__global__ __launch_bounds__(kRouterThreads) void moe_layer_router_kernel(MoeLayerArgs a)
 {
     __shared__ float logits[kMoeLayerExperts];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, token = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = wave_in_block(), token = blockIdx.x;
+    for (int i = token * kRouterThreads + threadIdx.x; i < a.counters_used; i += gridDim.x * kRouterThreads) a.counters[i] = 0u;
     const typename T::elem* x = (const typename T::elem*)a.x + (int64_t)token * a.ld_x;
-    for (int e = wave; e < a.E; e += 4) {
-        const typename T::elem* w = (const typename T::elem*)a.router_w + (int64_t)e * a.d_model;
-        float sum = 0.0f;
-        for (int k = lane * 8; k < a.d_model; k += 512) {
-            const typename T::frag p = load8_any<T>(w + k), q = load8_any<T>(x + k);
+    for (int e0 = wave * 4; e0 < a.E; e0 += kRouterThreads / 64 * 4) {
+        const typename T::elem* w[4];
+        float sum[4] = {};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf((float)p[i], (float)q[i], sum);
+        for (int i = 0; i < 4; ++i) w[i] = (const typename T::elem*)a.router_w + (int64_t)(e0 + i < a.E ? e0 + i : a.E - 1) * a.d_model;
+        for (int k0 = lane * 8; k0 < a.d_model; k0 += 1024) {
+            typename T::frag q[2], p[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int k = k0 + h * 512 < a.d_model ? k0 + h * 512 : k0;  // (what is loaded twice counts once)
+                q[h] = k0 + h * 512 < a.d_model ? load8_any<T>(x + k) : typename T::frag{};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[h][i] = load8_any<T>(w[i] + k);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (k0 + h * 512 >= a.d_model) continue;  // (a zero times an infinity is none)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) sum[i] = fmaf((float)p[h][i][c], (float)q[h][c], sum[i]);
+            }
         }
-        sum = wave_sum(sum);
-        if (lane == 0) logits[e] = sum + (a.router_b ? (float)((const typename T::elem*)a.router_b)[e] : 0.0f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sum[i] = wave_sum(sum[i]);
+            if (lane == 0 && e0 + i < a.E) logits[e0 + i] = sum[i] + (a.router_b ? (float)((const typename T::elem*)a.router_b)[e0 + i] : 0.0f);
+        }
     }
     __syncthreads();
     if (wave != 0) return;
-    // The choice: the largest of the keys (value, lowest index first) again and again.  A NaN counts as the largest value.
-    unsigned long long key[kMoeLayerExperts / 64];
-    float largest = -__builtin_inff(), v[kMoeLayerExperts / 64];
+    // The choice: the largest value that is left, in its lowest place, again and again.  Lane l has experts l, l + 64, ...; places of no
+    // expert and of chosen ones are 0, below every value.  A NaN counts as the largest value, -0 as 0.
+    constexpr int kEach = kMoeLayerExperts / 64;
+    const int each = (a.E + 63) / 64;
+    unsigned int key[kEach];
+    float v[kEach];
 #pragma unroll
-    for (int i = 0; i < kMoeLayerExperts / 64; ++i) {
-        const int e = i * 64 + lane;
+    for (int i = 0; i < kEach; ++i) {
         key[i] = 0;
         v[i] = -__builtin_inff();
-        if (e < a.E) {
-            v[i] = logits[e];
+        if (i < each && i * 64 + lane < a.E) {
+            v[i] = logits[i * 64 + lane];
             const unsigned int b = __builtin_bit_cast(unsigned int, v[i] != v[i] ? __builtin_nanf("") : v[i] + 0.0f);
-            key[i] = ((unsigned long long)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32) | (unsigned int)(kMoeLayerExperts - e);
+            key[i] = b & 0x80000000u ? ~b : b | 0x80000000u;
         }
     }
-    float mine = 0.0f;  // this lane's chosen logit (lane j: choice j)
-    int expert = 0;
+    int expert = 0, first = 0;  // this lane's choice (lane j: choice j), and the first one
     for (int j = 0; j < a.top_k; ++j) {
-        unsigned long long best = key[0];
+        unsigned int best = key[0];
 #pragma unroll
-        for (int i = 1; i < kMoeLayerExperts / 64; ++i) best = key[i] > best ? key[i] : best;
+        for (int i = 1; i < kEach; ++i)
+            if (i < each) best = key[i] > best ? key[i] : best;
+        best = wave_max_u32(best);
+        int e = -1;
 #pragma unroll
-        for (int i = 1; i < 64; i <<= 1) {
-            const unsigned long long o = __shfl_xor(best, i);
-            best = o > best ? o : best;
+        for (int i = 0; i < kEach; ++i) {
+            if (i >= each || e >= 0) continue;
+            const unsigned long long at = __ballot(key[i] == best);
+            if (at == 0ull) continue;
+            e = i * 64 + __builtin_ctzll(at);
+            if (lane == (e & 63)) key[i] = 0;
         }
-#pragma unroll
-        for (int i = 0; i < kMoeLayerExperts / 64; ++i)
-            if (key[i] == best) key[i] = 0;
-        const int e = kMoeLayerExperts - (int)(unsigned int)best;
-        if (j == 0) largest = logits[e];
-        if (lane == j) {
-            expert = e;
-            mine = logits[e];
-        }
+        if (j == 0) first = e;
+        if (lane == j) expert = e;
     }
     // Shares.  Where every logit is -inf no expert has any.
+    const float largest = logits[first], mine = logits[expert];
     float sum = 0.0f;
     if (a.renormalize) {
         sum = lane < a.top_k ? expf(mine - largest) : 0.0f;
     } else {
 #pragma unroll
-        for (int i = 0; i < kMoeLayerExperts / 64; ++i) sum += i * 64 + lane < a.E ? expf(v[i] - largest) : 0.0f;
+        for (int i = 0; i < kEach; ++i)
+            if (i < each) sum += i * 64 + lane < a.E ? expf(v[i] - largest) : 0.0f;
     }
     sum = wave_sum(sum);
     if (lane < a.top_k) {
@@ -128,10 +154,10 @@ __device__ __forceinline__ int pairs_of(const int* chosen, int pairs, int e, sho
     return *count;
 }
 
-template <class T, bool MX>
+template <class T, bool MX, int TT>
 struct ExpertWeights;
-template <class T>
-struct ExpertWeights<T, false> {
+template <class T, int TT>
+struct ExpertWeights<T, false, TT> {
     typedef DenseWeights<T> W;
     static __device__ __forceinline__ typename W::Rows rows(const void* w, const void*, const void*, int, int64_t first, int64_t count, int K)
     {
@@ -139,9 +165,9 @@ struct ExpertWeights<T, false> {
     }
     static __device__ __forceinline__ float unscale(float v, const void*, int64_t) { return v; }
 };
-template <class T>
-struct ExpertWeights<T, true> {
-    typedef Mx4Weights<T> W;
+template <class T, int TT>
+struct ExpertWeights<T, true, TT> {
+    typedef Mx4Weights<T, TT == 1 ? 2 : 1> W;
     static __device__ __forceinline__ typename W::Rows rows(const void* w, const void* s, const void* t, int ld, int64_t first, int64_t count, int K)
     {
         return W::rows((const uint8_t*)w, (const uint8_t*)s, (const uint8_t*)t, ld, first, count, K);
@@ -149,50 +175,86 @@ struct ExpertWeights<T, true> {
     static __device__ __forceinline__ float unscale(float v, const void* t, int64_t r) { return T::unscale(v, ((const uint8_t*)t)[r]); }
 };
 
-// The first product of 16 * TT pairs: hidden values 16 * F a block, each with its gate where there is one.
-template <class T, bool MX, bool GATED, int F, int TT, int U, int WK>
-__device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPointers& p, const short* list, int n, float4_t* part)
+// What a block of the experts' products has in LDS: the tokens that chose its expert, what its wavefronts turn operands in (and then
+// their sums), and, in the launch's dynamic part, the tokens of a call of one or two.
+template <class T, bool MX, int RT, int TT, int WK>
+struct ExpertLds {
+    typedef typename ExpertWeights<T, MX, TT>::W W;
+    static constexpr int kTurn = kSkinnyLds<W, TurnedTokens<T, true>>, kSum = RT * TT * 64;
+    uint4_t turn[WK * (kTurn > kSum ? kTurn : kSum)];
+    short list[kMoeLayerPairs];
+    int count;
+};
+
+// Sums of 16 * RT rows for n (at most 16 * TT) pairs: `columns(i)` is pair i's values.  Ends with every wavefront having the sums of
+// its own k in `lds`, part[wave][i][j][lane].  SHARED: all of the call's tokens, staged in `xs`.
+template <class T, bool MX, bool SHARED, int RT, int TT, int WK, class F>
+__device__ __forceinline__ void expert_sums(const typename ExpertWeights<T, MX, TT>::W::Rows (&rows)[RT], int K, int n, uint4_t* xs, uint4_t* lds, F columns)
 {
-    constexpr int RT = GATED ? 2 * F : F;
-    typedef ExpertWeights<T, MX> EW;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4;
-    const int f0 = blockIdx.x * (16 * F);
-    typedef TurnedTokens<T> X;
-    typename EW::W::Rows rows[RT];
-#pragma unroll
-    for (int i = 0; i < RT; ++i)  // (value rows follow the gate rows; each kind ends at its own last row)
-        rows[i] = EW::rows(p.w1, p.s1, p.t1, a.ld_s1, (i < F ? 0 : a.d_ff) + f0 + i % F * 16, i < F ? a.d_ff : 2 * a.d_ff, a.d_model);
-    typename X::Rows tokens[TT];
-    int pair[TT];
+    typedef typename ExpertWeights<T, MX, TT>::W W;
+    typedef typename std::conditional<SHARED, SharedTokens<T>, TurnedTokens<T, true>>::type X;
+    const int lane = threadIdx.x & 63, wave = wave_in_block();
+    const int pitch = SharedTokens<T>::pitch(K, W::kUnit);
+    float4_t acc[RT][TT] = {};
+    typename X::Rows x[TT];
 #pragma unroll
     for (int j = 0; j < TT; ++j) {
-        pair[j] = j * 16 + (lane & 15) < n ? list[j * 16 + (lane & 15)] : -1;
-        tokens[j] = X::rows([&](int i) { return (const typename T::elem*)a.x + (int64_t)(list[j * 16 + i < n ? j * 16 + i : n - 1] / a.top_k) * a.ld_x; });
+        if constexpr (SHARED)
+            x[j] = X::rows(xs, (lane & 15) < n ? lane & 15 : n - 1, pitch);
+        else
+            x[j] = X::rows([&](int i) { return columns(j * 16 + i < n ? j * 16 + i : n - 1); });
     }
-    float4_t acc[RT][TT] = {};
-    constexpr int kLds = kSkinnyLds<typename EW::W, X>;
-    skinny_sum<T, typename EW::W, X, RT, TT, U>(acc, rows, tokens, a.d_model, wave, WK, reinterpret_cast<uint4_t*>(part) + wave * kLds, [] {});
+    skinny_sum<T, W, X, RT, TT, 1>(acc, rows, x, K, wave, WK, lds + wave * kSkinnyLds<W, X>, [&] {
+        if constexpr (SHARED) {
+            X::stage(xs, columns, n, K, pitch);
+            __syncthreads();
+        }
+    });
     __syncthreads();
-    // Gate and value of a hidden unit have to meet: the sums are joined in every wavefront that finishes a tile of them.
+    float4_t* part = reinterpret_cast<float4_t*>(lds);
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int j = 0; j < TT; ++j) part[((wave * RT + i) * TT + j) * 64 + lane] = acc[i][j];
     __syncthreads();
+}
+
+// Tile (i, j) of the wavefronts' sums, in their order.
+template <int RT, int TT, int WK>
+__device__ __forceinline__ float4_t joined(const uint4_t* lds, int i, int j)
+{
+    const float4_t* part = reinterpret_cast<const float4_t*>(lds) + (i * TT + j) * 64 + (threadIdx.x & 63);
+    float4_t v = part[0];
+#pragma unroll
+    for (int k = 1; k < WK; ++k) v += part[k * RT * TT * 64];
+    return v;
+}
+
+// The first product of up to 16 * TT pairs: hidden values 16 * F a block, each with its gate where there is one.
+template <class T, bool MX, bool SHARED, bool GATED, int F, int TT, int WK>
+__device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPointers& p, const short* list, int n, uint4_t* xs, uint4_t* lds)
+{
+    constexpr int RT = GATED ? 2 * F : F;
+    typedef ExpertWeights<T, MX, TT> EW;
+    const int lane = threadIdx.x & 63, wave = wave_in_block(), group = lane >> 4;
+    const int f0 = blockIdx.x * (16 * F);
+    typename EW::W::Rows rows[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {  // (value rows follow the gate rows; each kind ends at its own last row)
+        const int end = i < F ? a.d_ff : 2 * a.d_ff, at = (i < F ? 0 : a.d_ff) + f0 + i % F * 16;
+        rows[i] = EW::rows(p.w1, p.s1, p.t1, a.ld_s1, at < end ? at : end - 1, end, a.d_model);
+    }
+    expert_sums<T, MX, SHARED, RT, TT, WK>(rows, a.d_model, n, xs, lds,
+                                   [&](int i) { return (const typename T::elem*)a.x + (int64_t)(list[i] / a.top_k) * a.ld_x; });
 #pragma unroll
     for (int i = 0; i < F; ++i)
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
-            if ((i * TT + j) % WK != wave || pair[j] < 0) continue;
-            const int f = f0 + i * 16 + group * 4;
-            if (f >= a.d_ff) continue;
-            float4_t g = {}, u = {};
-#pragma unroll
-            for (int k = 0; k < WK; ++k) {
-                g += part[((k * RT + i) * TT + j) * 64 + lane];
-                if (GATED) u += part[((k * RT + F + i) * TT + j) * 64 + lane];
-            }
-            float4_t h;
+            const int f = f0 + i * 16 + group * 4, column = j * 16 + (lane & 15);
+            if ((i * TT + j) % WK != wave || column >= n || f >= a.d_ff) continue;
+            const float4_t g = joined<RT, TT, WK>(lds, i, j);
+            float4_t u = {}, h;
+            if constexpr (GATED) u = joined<RT, TT, WK>(lds, F + i, j);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 float v = EW::unscale(g[c], p.t1, f + c);
@@ -206,101 +268,87 @@ __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPoi
                 }
                 h[c] = v;
             }
-            store4<T>((typename T::elem*)a.h + (int64_t)pair[j] * a.d_ff + f, h, 4);  // (d_ff is a multiple of 8)
+            store4<T>((typename T::elem*)a.h + (int64_t)list[column] * a.d_ff + f, h, 4);  // (d_ff is a multiple of 8)
         }
     __syncthreads();
 }
 
-// LDS of a product's block: what its wavefronts turn operands in, then their sums.
-template <class T, bool MX, int RT, int WK>
-constexpr int kExpertLds = WK * (kSkinnyLds<typename ExpertWeights<T, MX>::W, TurnedTokens<T>> > RT * 4 * 64 ? kSkinnyLds<typename ExpertWeights<T, MX>::W, TurnedTokens<T>> : RT * 4 * 64);
-
-template <class T, bool MX, bool GATED, int F, int U, int WK>
-__global__ __launch_bounds__(64 * WK) void moe_layer_first_kernel(MoeLayerArgs a)
+template <class T, bool MX, bool SHARED, bool GATED, int F, int TT, int WK>
+__global__ __launch_bounds__(64 * WK, TT == 1 ? 4 : 3) void moe_layer_first_kernel(MoeLayerArgs a)
 {
-    __shared__ float4_t part[kExpertLds<T, MX, GATED ? 2 * F : F, WK>];
-    __shared__ short list[kMoeLayerPairs];
-    __shared__ int count;
-    const int e = blockIdx.y;
-    const int n = pairs_of(a.chosen, a.tokens * a.top_k, e, list, &count);
-    if (n == 0) return;
-    const ExpertPointers p = a.experts[e];
-    if (n <= 16)
-        moe_first<T, MX, GATED, F, 1, U, WK>(a, p, list, n, part);
-    else if (n <= 32)
-        moe_first<T, MX, GATED, F, 2, 1, WK>(a, p, list, n, part);
-    else
-        moe_first<T, MX, GATED, F, 4, 1, WK>(a, p, list, n, part);
+    __shared__ ExpertLds<T, MX, GATED ? 2 * F : F, TT, WK> lds;
+    extern __shared__ uint4_t xs[];
+    const ExpertPointers p = a.experts[blockIdx.y];
+    const int n = pairs_of(a.chosen, a.tokens * a.top_k, blockIdx.y, lds.list, &lds.count);
+    for (int first = 0; first < n; first += 16 * TT) {  // (more than 16 * TT pairs of an expert read its weights again, out of the caches)
+        moe_first<T, MX, SHARED, GATED, F, TT, WK>(a, p, lds.list + first, n - first < 16 * TT ? n - first : 16 * TT, xs, lds.turn);
+        if (TT == 1) break;  // (a call of at most 16 tokens)
+    }
 }
 
-// The second product of 16 * TT pairs: rows of d_model, with the bias, not yet weighted.
-template <class T, bool MX, int RT, int TT, int U, int WK>
-__device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPointers& p, const short* list, int n, float4_t* part)
+// The second product of up to 16 * TT pairs: rows of d_model, with the bias, not yet weighted.
+template <class T, bool MX, bool SHARED, int RT, int TT, int WK>
+__device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPointers& p, const short* list, int n, uint4_t* xs, uint4_t* lds)
 {
-    typedef ExpertWeights<T, MX> EW;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4;
+    typedef ExpertWeights<T, MX, TT> EW;
+    const int lane = threadIdx.x & 63, wave = wave_in_block(), group = lane >> 4;
     const int d0 = blockIdx.x * (16 * RT);
-    typedef TurnedTokens<T> X;
     typename EW::W::Rows rows[RT];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) rows[i] = EW::rows(p.w2, p.s2, p.t2, a.ld_s2, d0 + i * 16, a.d_model, a.d_ff);
-    typename X::Rows hidden[TT];
-    int pair[TT];
-#pragma unroll
-    for (int j = 0; j < TT; ++j) {
-        pair[j] = j * 16 + (lane & 15) < n ? list[j * 16 + (lane & 15)] : -1;
-        hidden[j] = X::rows([&](int i) { return (const typename T::elem*)a.h + (int64_t)list[j * 16 + i < n ? j * 16 + i : n - 1] * a.d_ff; });
-    }
-    float4_t acc[RT][TT] = {};
-    constexpr int kLds = kSkinnyLds<typename EW::W, X>;
-    skinny_sum<T, typename EW::W, X, RT, TT, U>(acc, rows, hidden, a.d_ff, wave, WK, reinterpret_cast<uint4_t*>(part) + wave * kLds, [] {});
-    skinny_join<RT, TT, WK>(acc, part);
+    for (int i = 0; i < RT; ++i) rows[i] = EW::rows(p.w2, p.s2, p.t2, a.ld_s2, d0 + i * 16 < a.d_model ? d0 + i * 16 : a.d_model - 1, a.d_model, a.d_ff);
+    expert_sums<T, MX, SHARED, RT, TT, WK>(rows, a.d_ff, n, xs, lds, [&](int i) { return (const typename T::elem*)a.h + (int64_t)list[i] * a.d_ff; });
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
-            const int d = d0 + i * 16 + group * 4;
-            if ((i * TT + j) % WK != wave || pair[j] < 0 || d >= a.d_model) continue;
-            float4_t v = acc[i][j];
+            const int d = d0 + i * 16 + group * 4, column = j * 16 + (lane & 15);
+            if ((i * TT + j) % WK != wave || column >= n || d >= a.d_model) continue;
+            float4_t v = joined<RT, TT, WK>(lds, i, j);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 v[c] = EW::unscale(v[c], p.t2, d + c);
                 if (p.b2) v[c] += (float)((const typename T::elem*)p.b2)[d + c];
             }
-            *reinterpret_cast<float4_t*>(a.part + (int64_t)pair[j] * a.d_model + d) = v;
+            const uint4_t q = __builtin_bit_cast(uint4_t, v);
+            store16_device_scope(a.part + (int64_t)list[column] * a.d_model + d, q[0] | (unsigned long long)q[1] << 32, q[2] | (unsigned long long)q[3] << 32);
         }
+    __syncthreads();
 }
 
-template <class T, bool MX, int RT, int U, int WK>
-__global__ __launch_bounds__(64 * WK) void moe_layer_second_kernel(MoeLayerArgs a)
+// The block that is last to finish a tile of rows, of all experts' blocks, makes the weighted sum there, in the order of the choice.
+// An expert without a share adds nothing, whatever it computed.  Sums of other blocks come from other XCDs: they were stored past the L2s and
+// are loaded past them, and each block waits for its stores before it counts itself.
+template <class T, bool MX, bool SHARED, int RT, int TT, int WK>
+__global__ __launch_bounds__(64 * WK, TT == 1 ? 4 : 3) void moe_layer_second_kernel(MoeLayerArgs a)
 {
-    __shared__ float4_t part[kExpertLds<T, MX, RT, WK>];
-    __shared__ short list[kMoeLayerPairs];
-    __shared__ int count;
-    const int e = blockIdx.y;
-    const int n = pairs_of(a.chosen, a.tokens * a.top_k, e, list, &count);
-    if (n == 0) return;
-    const ExpertPointers p = a.experts[e];
-    if (n <= 16)
-        moe_second<T, MX, RT, 1, U, WK>(a, p, list, n, part);
-    else if (n <= 32)
-        moe_second<T, MX, RT, 2, 1, WK>(a, p, list, n, part);
-    else
-        moe_second<T, MX, RT, 4, 1, WK>(a, p, list, n, part);
-}
-
-// The weighted sum in the order of the choice.  An expert without a share adds nothing, whatever it computed.
-template <class T>
-__global__ __launch_bounds__(256) void moe_layer_sum_kernel(MoeLayerArgs a)
-{
-    const int d = (blockIdx.x * 256 + threadIdx.x) * 4, token = blockIdx.y;
-    if (d >= a.d_model) return;
-    float4_t y = {};
-    for (int j = 0; j < a.top_k; ++j) {
-        const float c = a.share[token * a.top_k + j];
-        if (c == 0.0f) continue;
-        y += c * *reinterpret_cast<const float4_t*>(a.part + (int64_t)(token * a.top_k + j) * a.d_model + d);
+    __shared__ ExpertLds<T, MX, RT, TT, WK> lds;
+    __shared__ unsigned int before;
+    extern __shared__ uint4_t xs[];
+    const ExpertPointers p = a.experts[blockIdx.y];
+    const int n = pairs_of(a.chosen, a.tokens * a.top_k, blockIdx.y, lds.list, &lds.count);
+    for (int first = 0; first < n; first += 16 * TT) {
+        moe_second<T, MX, SHARED, RT, TT, WK>(a, p, lds.list + first, n - first < 16 * TT ? n - first : 16 * TT, xs, lds.turn);
+        if (TT == 1) break;
     }
-    store4<T>((typename T::elem*)a.y + (int64_t)token * a.d_model + d, y, 4);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) before = __hip_atomic_fetch_add(&a.counters[blockIdx.x], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (before != gridDim.y - 1) return;
+    constexpr int kWords = 16 * RT / 4;  // of four rows
+    for (int i = threadIdx.x; i < a.tokens * kWords; i += 64 * WK) {
+        const int token = i / kWords, d = blockIdx.x * (16 * RT) + i % kWords * 4;
+        if (d >= a.d_model) continue;
+        float4_t y = {};
+        for (int j = 0; j < a.top_k; ++j) {
+            const float c = a.share[token * a.top_k + j];
+            if (c == 0.0f) continue;
+            unsigned long long lo, hi;
+            load16_device_scope(a.part + (int64_t)(token * a.top_k + j) * a.d_model + d, lo, hi);
+            const uint4_t q = {(unsigned int)lo, (unsigned int)(lo >> 32), (unsigned int)hi, (unsigned int)(hi >> 32)};
+            y += c * __builtin_bit_cast(float4_t, q);
+        }
+        store4<T>((typename T::elem*)a.y + (int64_t)token * a.d_model + d, y, 4);
+    }
 }
 }  // namespace pimhip

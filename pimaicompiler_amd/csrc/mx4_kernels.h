@@ -1,8 +1,6 @@
 // Kernels on microscaled 4-bit values (mx4_format.h): quantisation, reading back, and the products with one or both operands in 4 bits.
 #pragma once
 
-#include <type_traits>
-
 #include "skinny.h"
 
 namespace pimhip
@@ -53,7 +51,7 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const typename T::ele
 {
     constexpr int kRows = 4 / WPR;
     __shared__ unsigned int top_of[4];
-    const int wave = threadIdx.x >> 6;
+    const int wave = wave_in_block();
     const int64_t row = (int64_t)blockIdx.x * kRows + wave / WPR;
     const int lane = threadIdx.x % (64 * WPR);
     const int64_t blocks = (cols + kMxBlock - 1) / kMxBlock;
@@ -172,18 +170,21 @@ template <class T, bool SHARED, int RT, int TT, int U, int WK>
 __global__ __launch_bounds__(64 * WK) void mx4_linear_skinny_kernel(const typename T::elem* x, Mx4View w, const typename T::elem* bias, typename T::elem* out,
                                                                     int64_t ld_x, int64_t ld_out, int64_t M, int relu)
 {
-    typedef Mx4Weights<T> W;
-    typedef typename std::conditional<SHARED, SharedTokens<T>, TurnedTokens<T>>::type X;
+    typedef Mx4Weights<T, TT == 1 ? 2 : 1> W;
+    typedef typename std::conditional<SHARED, SharedTokens<T>, TurnedTokens<T, false>>::type X;
     constexpr int kLds = kSkinnyLds<W, X>, kPart = RT * TT * 64;
     __shared__ uint4_t lds[WK * (kLds > kPart ? kLds : kPart)];
     __shared__ int tops[RT * 16];
     __shared__ float add[RT * 16];
     extern __shared__ uint4_t xs[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = wave_in_block(), group = lane >> 4;
     const int64_t row0 = (int64_t)blockIdx.x * (16 * RT), token0 = (int64_t)blockIdx.y * (16 * TT);
     typename W::Rows rows[RT];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) rows[i] = W::rows(w.packed, w.scales, w.tops, w.ld_scales, row0 + i * 16, w.rows, w.cols);
+    for (int i = 0; i < RT; ++i) {
+        const int64_t at = row0 + i * 16;
+        rows[i] = W::rows(w.packed, w.scales, w.tops, w.ld_scales, at < w.rows ? at : w.rows - 1, w.rows, w.cols);
+    }
     auto token = [&](int64_t t) { return x + (t < M ? t : M - 1) * ld_x; };
     const int K = (int)w.cols, pitch = SharedTokens<T>::pitch(K, W::kUnit);
     typename X::Rows tokens[TT];
@@ -232,7 +233,7 @@ template <class O, int RT, int TT, int WK>
 __global__ __launch_bounds__(64 * WK) void mx4_matmul_skinny_kernel(Mx4View a, Mx4View b, typename O::elem* out, int64_t ld_out)
 {
     __shared__ float4_t part[WK > 1 ? WK * RT * TT * 64 : 1];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = wave_in_block(), group = lane >> 4;
     const int64_t row0 = (int64_t)blockIdx.x * (16 * RT), token0 = (int64_t)blockIdx.y * (16 * TT);
     const int blocks = (int)((b.cols + kMxBlock - 1) / kMxBlock);
     const uint8_t *bp[RT], *bs[RT], *ap[TT], *as[TT];

@@ -38,7 +38,7 @@ __global__ __launch_bounds__(64 * GN * GT) void mx4_linear_tile_kernel(const typ
     __shared__ uint4_t xs[kT * 16];  // chunk c of a row at c ^ (row % 8)
     __shared__ uint4_t ws[kN * 4];   // block c of a row at c ^ (row / 4 % 4)
     __shared__ float ss[4][kN];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = lane >> 4, row = lane & 15;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_in_block(), group = lane >> 4, row = lane & 15;
     const int wn = wave % GN * WN, wt = wave / GN * WT;
     int64_t tile_n, tile_t;
     tile_of_block((w.rows + kN - 1) / kN, (M + kT - 1) / kT, tile_n, tile_t);
@@ -167,7 +167,7 @@ __global__ __launch_bounds__(64 * GN * GT) void mx4_matmul_tile_kernel(Mx4View a
     static_assert(kPieces * kThreads == kRows * 4 && kRows <= kThreads && WN % 4 == 0 && WT % 4 == 0, "whole pieces a thread, a row of scales each");
     __shared__ uint4_t values[2][kRows * 4];            // the rows of b, then those of a; block c of a row at c ^ (row / 4 % 4)
     __shared__ unsigned int codes[2][kRows / 64][64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = lane >> 4, row = lane & 15;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_in_block(), group = lane >> 4, row = lane & 15;
     const int wn = wave % GN * WN, wt = wave / GN * WT;
     int64_t tile_n, tile_t;
     tile_of_block((b.rows + kN - 1) / kN, (a.rows + kT - 1) / kT, tile_n, tile_t);

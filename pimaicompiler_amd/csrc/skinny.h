@@ -14,6 +14,8 @@
 // both operands on their way; x is asked for with its weights, since a wavefront's loads come back in order.
 #pragma once
 
+#include <type_traits>
+
 #include "mx4_format.h"
 
 namespace pimhip
@@ -32,31 +34,9 @@ __device__ __forceinline__ void wave_lds_order()
 template <class T>
 struct DenseTile {
     static constexpr int kUnit = 128, kLds = 16 * 16;  // (in 16-byte words)
-    struct Rows {
-        const typename T::elem* p[4];  // the lane's four rows, at its chunk
-    };
     struct Raw {
         typename T::frag v[4];
     };
-    template <bool STREAM>
-    static __device__ __forceinline__ void load(Raw& w, const Rows& r, int unit)
-    {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const typename T::elem* p = r.p[j] + (int64_t)unit * kUnit;
-            if constexpr (STREAM)
-                w.v[j] = __builtin_bit_cast(typename T::frag, (half8_t)__builtin_nontemporal_load(reinterpret_cast<const half8_any_t*>(p)));
-            else
-                w.v[j] = load8_any<T>(p);
-        }
-    }
-    // The same where the rows may end inside the unit.
-    static __device__ __forceinline__ void load_guarded(Raw& w, const Rows& r, int unit, int K)
-    {
-        const int chunk = threadIdx.x & 15;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w.v[j] = load8_guarded<T>(r.p[j] - chunk * 8, (int64_t)unit * kUnit + chunk * 8, K);
-    }
     static __device__ __forceinline__ void to_lds(const Raw& w, uint4_t* lds)
     {
         const int lane = threadIdx.x & 63;
@@ -75,30 +55,45 @@ struct DenseTile {
     }
 };
 
-// 16-bit weights.
+// 16-bit weights; rows are whole groups of eight values.  A tile's rows are addressed from its first one, which all lanes share.
 template <class T>
 struct DenseWeights {
     typedef DenseTile<T> Tile;
     typedef typename Tile::Raw Raw;
-    typedef typename Tile::Rows Rows;
     static constexpr int kUnit = Tile::kUnit, kLds = Tile::kLds;
+    struct Rows {
+        const char* base;
+        unsigned int at[4];  // bytes from there to the lane's four rows' chunks
+    };
     struct Operands {
         typename T::frag f[4];
     };
-    // Rows first .. first + 15 of a matrix of `count` rows of K values; rows behind its end are its last one again.
+    // Rows first .. first + 15 of a matrix of `count` rows of K values (first is one of them); rows behind its end are its last one again.
     static __device__ __forceinline__ Rows rows(const void* w, int64_t first, int64_t count, int64_t K)
     {
         Rows r;
-        const int lane = threadIdx.x & 63;
+        const int lane = threadIdx.x & 63, last = (int)(count - 1 - first < 15 ? count - 1 - first : 15);
+        r.base = (const char*)w + first * K * 2;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int64_t at = first + lane / 16 + 4 * j;
-            r.p[j] = (const typename T::elem*)w + (at < count ? at : count - 1) * K + (lane & 15) * 8;
+            const int at = lane / 16 + 4 * j;
+            r.at[j] = (unsigned int)(at < last ? at : last) * (unsigned int)(K * 2) + (lane & 15) * 16;
         }
         return r;
     }
-    static __device__ __forceinline__ void load(Raw& w, const Rows& r, int unit) { Tile::template load<true>(w, r, unit); }
-    static __device__ __forceinline__ void load_guarded(Raw& w, const Rows& r, int unit, int K) { Tile::load_guarded(w, r, unit, K); }
+    static __device__ __forceinline__ void load(Raw& w, const Rows& r, int unit)
+    {
+        const char* p = r.base + (int64_t)unit * (kUnit * 2);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w.v[j] = __builtin_bit_cast(typename T::frag, __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(p + r.at[j])));
+    }
+    static __device__ __forceinline__ void load_guarded(Raw& w, const Rows& r, int unit, int K)
+    {
+        const char* p = r.base + (int64_t)unit * (kUnit * 2);
+        const bool in = unit * kUnit + (int)(threadIdx.x & 15) * 8 < K;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w.v[j] = in ? __builtin_bit_cast(typename T::frag, *reinterpret_cast<const uint4_t*>(p + r.at[j])) : typename T::frag{};
+    }
     static __device__ __forceinline__ void turn(Operands& o, const Raw& w, const Rows&, uint4_t* lds)
     {
         Tile::to_lds(w, lds);
@@ -109,83 +104,92 @@ struct DenseWeights {
     static __device__ __forceinline__ typename T::frag operand(const Operands& o, int, int product) { return o.f[product]; }
 };
 
-// 4-bit weights, 256 values a unit (two steps); T is the type of x.  Lane l loads chunk l % 8, a block, of rows l / 8 + 8 j, and of the
-// unit's scale codes two of row l / 4.
-template <class T>
+// 4-bit weights, S steps (of 128 values, four blocks) a unit; T is the type of x.  Lane l loads chunk l % (4 S), a block, of rows
+// l / (4 S) + 16 / S j, and of the unit's scale codes S of row l / 4.  Two steps are whole lines of 128 bytes; one step leaves more registers
+// to tokens.
+template <class T, int S>
 struct Mx4Weights {
-    static constexpr int kUnit = 256, kLds = 16 * 8 + 8;  // (rows of 128 bytes, then their codes)
+    static_assert(S == 1 || S == 2, "one or two steps a unit");
+    static constexpr int kUnit = S * kSkinnyStep, kRow = 4 * S, kLds = 16 * kRow + 4 * S;  // (rows of 64 S bytes, then their codes)
+    typedef typename std::conditional<S == 1, uint8_t, uint16_t>::type Codes;
     struct Rows {
-        const uint8_t* p[2];
+        const uint8_t* base;
         const uint8_t* codes;
-        int top;  // the largest scale code of row l % 16
+        unsigned int at[S], codes_at;  // bytes from there to the lane's rows' blocks and codes
+        int top;                       // the largest scale code of row l % 16
     };
     struct Raw {
-        uint4_t v[2];
-        uint16_t codes;
+        uint4_t v[S];
+        Codes codes;
     };
     struct Operands {
-        uint4_t v[2];    // this lane's block of each step
-        float scale[2];
+        uint4_t v[S];    // this lane's block of each step
+        float scale[S];
     };
     static __device__ __forceinline__ Rows rows(const uint8_t* packed, const uint8_t* scales, const uint8_t* tops, int64_t ld_scales, int64_t first, int64_t count,
                                                 int64_t K)
     {
         Rows r;
-        const int lane = threadIdx.x & 63;
-        const int64_t blocks = (K + kMxBlock - 1) / kMxBlock;
-        auto row = [&](int i) { return first + i < count ? first + i : count - 1; };
+        const int lane = threadIdx.x & 63, last = (int)(count - 1 - first < 15 ? count - 1 - first : 15);
+        const int64_t pitch = (K + kMxBlock - 1) / kMxBlock * kMxBlockBytes;
+        auto row = [&](int i) { return (unsigned int)(i < last ? i : last); };
+        r.base = packed + first * pitch;
+        r.codes = scales + first * ld_scales;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) r.p[j] = packed + (row(lane / 8 + 8 * j) * blocks + (lane & 7)) * kMxBlockBytes;
-        r.codes = scales + row(lane / 4) * ld_scales + (lane & 3) * 2;
-        r.top = tops[row(lane & 15)];
+        for (int j = 0; j < S; ++j) r.at[j] = row(lane / kRow + 16 / S * j) * (unsigned int)pitch + lane % kRow * kMxBlockBytes;
+        r.codes_at = row(lane / 4) * (unsigned int)ld_scales + (lane & 3) * S;
+        r.top = tops[first + row(lane & 15)];
         return r;
     }
     static __device__ __forceinline__ void load(Raw& w, const Rows& r, int unit)
     {
+        const uint8_t* p = r.base + (int64_t)unit * (kUnit / 2);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) w.v[j] = __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(r.p[j] + (int64_t)unit * (kUnit / 2)));
-        w.codes = *reinterpret_cast<const uint16_t*>(r.codes + unit * 8);  // (whole groups of 16 codes a row)
+        for (int j = 0; j < S; ++j) w.v[j] = __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(p + r.at[j]));
+        w.codes = *reinterpret_cast<const Codes*>(r.codes + (int64_t)unit * kRow + r.codes_at);  // (whole groups of 16 codes a row)
     }
     static __device__ __forceinline__ void load_guarded(Raw& w, const Rows& r, int unit, int K)
     {
         const int lane = threadIdx.x & 63;
-        const bool in = unit * kUnit + (lane & 7) * kMxBlock < K;
+        const uint8_t* p = r.base + (int64_t)unit * (kUnit / 2);
+        const bool in = unit * kUnit + lane % kRow * kMxBlock < K;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) w.v[j] = in ? *reinterpret_cast<const uint4_t*>(r.p[j] + (int64_t)unit * (kUnit / 2)) : uint4_t{0, 0, 0, 0};
-        w.codes = *reinterpret_cast<const uint16_t*>(r.codes + unit * 8);
+        for (int j = 0; j < S; ++j) w.v[j] = in ? *reinterpret_cast<const uint4_t*>(p + r.at[j]) : uint4_t{0, 0, 0, 0};
+        unsigned int codes = *reinterpret_cast<const Codes*>(r.codes + (int64_t)unit * kRow + r.codes_at);
         // What lies behind the row's last block may be anything: any code but "not a number".
-        const int left = K - unit * kUnit - (lane & 3) * 2 * kMxBlock;
-        if (left <= kMxBlock) w.codes = (uint16_t)((w.codes & 0x00ff) | 0x7f00);
-        if (left <= 0) w.codes = 0x7f7f;
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+            if (unit * kUnit + ((lane & 3) * S + s) * kMxBlock >= K) codes = (codes & ~(255u << (8 * s))) | (127u << (8 * s));
+        w.codes = (Codes)codes;
     }
+    static __device__ __forceinline__ int place(int row, int chunk) { return row * kRow + (chunk ^ (S == 2 ? row & 7 : row / 4 & 3)); }
     static __device__ __forceinline__ void turn(Operands& o, const Raw& w, const Rows& r, uint4_t* lds)
     {
         const int lane = threadIdx.x & 63, row = lane & 15, group = lane >> 4;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int at = lane / 8 + 8 * j;
-            lds[at * 8 + ((lane & 7) ^ (at & 7))] = w.v[j];
-        }
-        reinterpret_cast<uint16_t*>(lds + 16 * 8)[lane] = w.codes;
+        for (int j = 0; j < S; ++j) lds[place(lane / kRow + 16 / S * j, lane % kRow)] = w.v[j];
+        reinterpret_cast<Codes*>(lds + 16 * kRow)[lane] = w.codes;
         wave_lds_order();
-        const uint2_t codes = reinterpret_cast<const uint2_t*>(lds + 16 * 8)[row];
+        const unsigned int* codes = reinterpret_cast<const unsigned int*>(lds + 16 * kRow) + row * S;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            o.v[h] = lds[row * 8 + ((h * 4 + group) ^ (row & 7))];
-            o.scale[h] = T::scale((codes[h] >> (8 * group)) & 255u, r.top);
+        for (int s = 0; s < S; ++s) {
+            o.v[s] = lds[place(row, s * 4 + group)];
+            o.scale[s] = T::scale((codes[s] >> (8 * group)) & 255u, r.top);
         }
         wave_lds_order();
     }
     static __device__ __forceinline__ typename T::frag operand(const Operands& o, int step, int product) { return T::from_mx4(o.v[step][product], o.scale[step]); }
 };
 
-// The tokens of a product, loaded and turned like weights by each wavefront.
-template <class T>
+// The tokens of a product, loaded and turned like weights by each wavefront.  WHOLE: their rows are whole groups of eight values.
+template <class T, bool WHOLE>
 struct TurnedTokens {
     typedef DenseTile<T> Tile;
     typedef typename Tile::Raw Raw;
-    typedef typename Tile::Rows Rows;
     static constexpr int kLds = Tile::kLds;
+    struct Rows {
+        const typename T::elem* p[4];  // the lane's four rows, at its chunk
+    };
     // row(i): the token of column i, as a pointer to its values
     template <class F>
     static __device__ __forceinline__ Rows rows(F row)
@@ -196,8 +200,22 @@ struct TurnedTokens {
         for (int j = 0; j < 4; ++j) r.p[j] = row(lane / 16 + 4 * j) + (lane & 15) * 8;
         return r;
     }
-    static __device__ __forceinline__ void load(Raw& w, const Rows& r, int step) { Tile::template load<false>(w, r, step); }
-    static __device__ __forceinline__ void load_guarded(Raw& w, const Rows& r, int step, int K) { Tile::load_guarded(w, r, step, K); }
+    static __device__ __forceinline__ void load(Raw& w, const Rows& r, int step)
+    {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w.v[j] = load8_any<T>(r.p[j] + (int64_t)step * kSkinnyStep);
+    }
+    static __device__ __forceinline__ void load_guarded(Raw& w, const Rows& r, int step, int K)
+    {
+        const int chunk = threadIdx.x & 15;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (WHOLE)
+                w.v[j] = step * kSkinnyStep + chunk * 8 < K ? load8_any<T>(r.p[j] + (int64_t)step * kSkinnyStep) : typename T::frag{};
+            else
+                w.v[j] = load8_guarded<T>(r.p[j] - chunk * 8, (int64_t)step * kSkinnyStep + chunk * 8, K);
+        }
+    }
     static __device__ __forceinline__ void turn(typename T::frag (&f)[4], const Raw& w, const Rows&, int, uint4_t* lds)
     {
         Tile::to_lds(w, lds);
@@ -317,7 +335,7 @@ template <int RT, int TT, int WK>
 __device__ __forceinline__ void skinny_join(float4_t (&acc)[RT][TT], float4_t* part)
 {
     if constexpr (WK > 1) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int lane = threadIdx.x & 63, wave = wave_in_block();
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < RT; ++i)
