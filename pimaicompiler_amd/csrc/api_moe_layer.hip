@@ -48,50 +48,54 @@ int destroy_moe_layer_plan_locked(PimHipMoeLayerPlan* plan)
 template <class T, bool MX>
 unsigned int shared_bytes(const MoeLayerArgs& a, int K)
 {
-    return (unsigned int)(a.tokens * SharedTokens<T>::pitch(K, ExpertWeights<T, MX, 1>::W::kUnit) * 16);
+    return (unsigned int)((a.tokens < 16 ? a.tokens : 16) * SharedTokens<T>::pitch(K, ExpertWeights<T, MX>::W::kUnit) * 16);
 }
 
-template <class T, bool MX, bool SHARED, bool GATED, int F, int TT>
+template <class T, bool MX, bool SHARED, bool GATED, int F>
 void launch_first(const MoeLayerArgs& a, hipStream_t s)
 {
     constexpr int WK = 4;
-    moe_layer_first_kernel<T, MX, SHARED, GATED, F, TT, WK>
-        <<<dim3((unsigned)((a.d_ff + 16 * F - 1) / (16 * F)), (unsigned)a.E), 64 * WK, SHARED ? shared_bytes<T, MX>(a, a.d_model) : 0, s>>>(a);
+    moe_layer_first_kernel<T, MX, SHARED, GATED, F, WK>
+        <<<dim3((unsigned)((a.d_ff + 16 * F - 1) / (16 * F)), (unsigned)a.E, (unsigned)((a.tokens + 15) / 16)), 64 * WK, SHARED ? shared_bytes<T, MX>(a, a.d_model) : 0, s>>>(a);
 }
 
-template <class T, bool MX, bool SHARED, int RT, int TT, int WK>
+template <class T, bool MX, bool SHARED, int RT, int WK>
 void launch_second(const MoeLayerArgs& a, hipStream_t s)
 {
-    moe_layer_second_kernel<T, MX, SHARED, RT, TT, WK>
-        <<<dim3((unsigned)((a.d_model + 16 * RT - 1) / (16 * RT)), (unsigned)a.E), 64 * WK, SHARED ? shared_bytes<T, MX>(a, a.d_ff) : 0, s>>>(a);
-}
-
-template <class T, bool MX, bool SHARED, int TT>
-void launch(const PimHipMoeLayerPlan* p, MoeLayerArgs& a, hipStream_t s)
-{
-    a.counters_used = (a.d_model + 15) / 16;
-    moe_layer_router_kernel<T><<<dim3((unsigned)a.tokens), kRouterThreads, 0, s>>>(a);
-    p->gated ? launch_first<T, MX, SHARED, true, TT, TT>(a, s) : launch_first<T, MX, SHARED, false, 2 * TT, TT>(a, s);
-    // Blocks of the second product that have something to read.  Where they fill the card several times over a block has two tiles of
-    // rows, else one, and more wavefronts share its long k.
-    const int active = a.E < a.tokens * a.top_k ? a.E : a.tokens * a.top_k;
-    const int64_t blocks = (int64_t)((a.d_model + 15) / 16) * active;
-    if (blocks >= 2048)
-        launch_second<T, MX, SHARED, 2, TT, 4>(a, s);
-    else
-        launch_second<T, MX, SHARED, 1, TT, 8>(a, s);
+    moe_layer_second_kernel<T, MX, SHARED, RT, WK>
+        <<<dim3((unsigned)((a.d_model + 16 * RT - 1) / (16 * RT)), (unsigned)a.E, (unsigned)((a.tokens + 15) / 16)), 64 * WK, SHARED ? shared_bytes<T, MX>(a, a.d_ff) : 0, s>>>(a);
 }
 
 template <class T, bool MX>
 void launch(const PimHipMoeLayerPlan* p, MoeLayerArgs& a, hipStream_t s)
 {
-    constexpr unsigned int kShared = 20 << 10;  // (a block of the turned kind has 35 KB: four on a CU either way)
-    if (a.tokens <= 2 && shared_bytes<T, MX>(a, a.d_model) <= kShared && shared_bytes<T, MX>(a, a.d_ff) <= kShared)
-        launch<T, MX, true, 1>(p, a, s);
-    else if (a.tokens <= 16)
-        launch<T, MX, false, 1>(p, a, s);
+    a.counters_used = (a.d_model + 15) / 16;
+    moe_layer_router_kernel<T><<<dim3((unsigned)a.tokens), kRouterThreads, 0, s>>>(a);
+    // Tokens are staged as a whole where there are one or two, or where an expert has many and 16 of them leave a CU room for three
+    // blocks.
+    const bool many = a.tokens > 16;
+    const unsigned int most = many ? 40 << 10 : a.tokens <= 2 ? 20 << 10 : 0;
+    // With many tokens a block has twice the rows: their values are read, and turned or staged, half as often (64 tokens through 8 gated 4-bit
+    // experts 1024 -> 4096: 29.8 -> 20.8 us; one token through 2 of 8 experts 1024 -> 4096 in fp16, where blocks are few: 6.1 -> 7.9).
+    auto first = [&](auto shared) {
+        constexpr bool S = decltype(shared)::value;
+        if (many)
+            p->gated ? launch_first<T, MX, S, true, 2>(a, s) : launch_first<T, MX, S, false, 4>(a, s);
+        else
+            p->gated ? launch_first<T, MX, S, true, 1>(a, s) : launch_first<T, MX, S, false, 2>(a, s);
+    };
+    shared_bytes<T, MX>(a, a.d_model) <= most ? first(std::true_type{}) : first(std::false_type{});
+    // Blocks of the second product that have something to read.  Where they fill the card several times over a block has two tiles of
+    // rows, else one, and more wavefronts share its long k.
+    const int active = a.E < a.tokens * a.top_k ? a.E : a.tokens * a.top_k;
+    const int64_t blocks = (int64_t)((a.d_model + 15) / 16) * active;
+    const bool shared = shared_bytes<T, MX>(a, a.d_ff) <= most;
+    if (many)
+        shared ? launch_second<T, MX, true, 2, 8>(a, s) : launch_second<T, MX, false, 2, 8>(a, s);
+    else if (blocks >= 2048)
+        shared ? launch_second<T, MX, true, 2, 4>(a, s) : launch_second<T, MX, false, 2, 4>(a, s);
     else
-        launch<T, MX, false, 2>(p, a, s);
+        shared ? launch_second<T, MX, true, 1, 8>(a, s) : launch_second<T, MX, false, 1, 8>(a, s);
 }
 }  // namespace
 

@@ -154,10 +154,10 @@ __device__ __forceinline__ int pairs_of(const int* chosen, int pairs, int e, sho
     return *count;
 }
 
-template <class T, bool MX, int TT>
+template <class T, bool MX>
 struct ExpertWeights;
-template <class T, int TT>
-struct ExpertWeights<T, false, TT> {
+template <class T>
+struct ExpertWeights<T, false> {
     typedef DenseWeights<T> W;
     static __device__ __forceinline__ typename W::Rows rows(const void* w, const void*, const void*, int, int64_t first, int64_t count, int K)
     {
@@ -165,9 +165,9 @@ struct ExpertWeights<T, false, TT> {
     }
     static __device__ __forceinline__ float unscale(float v, const void*, int64_t) { return v; }
 };
-template <class T, int TT>
-struct ExpertWeights<T, true, TT> {
-    typedef Mx4Weights<T, TT == 1 ? 2 : 1> W;
+template <class T>
+struct ExpertWeights<T, true> {
+    typedef Mx4Weights<T, 2> W;
     static __device__ __forceinline__ typename W::Rows rows(const void* w, const void* s, const void* t, int ld, int64_t first, int64_t count, int K)
     {
         return W::rows((const uint8_t*)w, (const uint8_t*)s, (const uint8_t*)t, ld, first, count, K);
@@ -176,35 +176,33 @@ struct ExpertWeights<T, true, TT> {
 };
 
 // What a block of the experts' products has in LDS: the tokens that chose its expert, what its wavefronts turn operands in (and then
-// their sums), and, in the launch's dynamic part, the tokens of a call of one or two.
-template <class T, bool MX, int RT, int TT, int WK>
+// their sums), and, SHARED, in the launch's dynamic part the values of up to 16 pairs.
+template <class T, bool MX, bool SHARED, int RT, int WK>
 struct ExpertLds {
-    typedef typename ExpertWeights<T, MX, TT>::W W;
-    static constexpr int kTurn = kSkinnyLds<W, TurnedTokens<T, true>>, kSum = RT * TT * 64;
+    typedef typename ExpertWeights<T, MX>::W W;
+    typedef typename std::conditional<SHARED, SharedTokens<T>, TurnedTokens<T, true>>::type X;
+    static constexpr int kTurn = kSkinnyLds<W, X>, kSum = RT * 64;
     uint4_t turn[WK * (kTurn > kSum ? kTurn : kSum)];
     short list[kMoeLayerPairs];
     int count;
 };
 
-// Sums of 16 * RT rows for n (at most 16 * TT) pairs: `columns(i)` is pair i's values.  Ends with every wavefront having the sums of
-// its own k in `lds`, part[wave][i][j][lane].  SHARED: all of the call's tokens, staged in `xs`.
-template <class T, bool MX, bool SHARED, int RT, int TT, int WK, class F>
-__device__ __forceinline__ void expert_sums(const typename ExpertWeights<T, MX, TT>::W::Rows (&rows)[RT], int K, int n, uint4_t* xs, uint4_t* lds, F columns)
+// Sums of 16 * RT rows for n (at most 16) pairs: `columns(i)` is pair i's values.  Ends with every wavefront having the sums of
+// its own k in `lds`, part[wave][i][lane].  SHARED: the pairs' values are staged in `xs`.
+template <class T, bool MX, bool SHARED, int RT, int WK, class F>
+__device__ __forceinline__ void expert_sums(const typename ExpertWeights<T, MX>::W::Rows (&rows)[RT], int K, int n, uint4_t* xs, uint4_t* lds, F columns)
 {
-    typedef typename ExpertWeights<T, MX, TT>::W W;
+    typedef typename ExpertWeights<T, MX>::W W;
     typedef typename std::conditional<SHARED, SharedTokens<T>, TurnedTokens<T, true>>::type X;
     const int lane = threadIdx.x & 63, wave = wave_in_block();
     const int pitch = SharedTokens<T>::pitch(K, W::kUnit);
-    float4_t acc[RT][TT] = {};
-    typename X::Rows x[TT];
-#pragma unroll
-    for (int j = 0; j < TT; ++j) {
-        if constexpr (SHARED)
-            x[j] = X::rows(xs, (lane & 15) < n ? lane & 15 : n - 1, pitch);
-        else
-            x[j] = X::rows([&](int i) { return columns(j * 16 + i < n ? j * 16 + i : n - 1); });
-    }
-    skinny_sum<T, W, X, RT, TT, 1>(acc, rows, x, K, wave, WK, lds + wave * kSkinnyLds<W, X>, [&] {
+    float4_t acc[RT][1] = {};
+    typename X::Rows x[1];
+    if constexpr (SHARED)
+        x[0] = X::rows(xs, (lane & 15) < n ? lane & 15 : n - 1, pitch);
+    else
+        x[0] = X::rows([&](int i) { return columns(i < n ? i : n - 1); });
+    skinny_sum<T, W, X, RT, 1, 1>(acc, rows, x, K, wave, WK, lds + wave * kSkinnyLds<W, X>, [&] {
         if constexpr (SHARED) {
             X::stage(xs, columns, n, K, pitch);
             __syncthreads();
@@ -213,29 +211,27 @@ __device__ __forceinline__ void expert_sums(const typename ExpertWeights<T, MX, 
     __syncthreads();
     float4_t* part = reinterpret_cast<float4_t*>(lds);
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int j = 0; j < TT; ++j) part[((wave * RT + i) * TT + j) * 64 + lane] = acc[i][j];
+    for (int i = 0; i < RT; ++i) part[(wave * RT + i) * 64 + lane] = acc[i][0];
     __syncthreads();
 }
 
-// Tile (i, j) of the wavefronts' sums, in their order.
-template <int RT, int TT, int WK>
-__device__ __forceinline__ float4_t joined(const uint4_t* lds, int i, int j)
+// Tile i of the wavefronts' sums, in their order.
+template <int RT, int WK>
+__device__ __forceinline__ float4_t joined(const uint4_t* lds, int i)
 {
-    const float4_t* part = reinterpret_cast<const float4_t*>(lds) + (i * TT + j) * 64 + (threadIdx.x & 63);
+    const float4_t* part = reinterpret_cast<const float4_t*>(lds) + i * 64 + (threadIdx.x & 63);
     float4_t v = part[0];
 #pragma unroll
-    for (int k = 1; k < WK; ++k) v += part[k * RT * TT * 64];
+    for (int k = 1; k < WK; ++k) v += part[k * RT * 64];
     return v;
 }
 
-// The first product of up to 16 * TT pairs: hidden values 16 * F a block, each with its gate where there is one.
-template <class T, bool MX, bool SHARED, bool GATED, int F, int TT, int WK>
+// The first product of up to 16 pairs: hidden values 16 * F a block, each with its gate where there is one.
+template <class T, bool MX, bool SHARED, bool GATED, int F, int WK>
 __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPointers& p, const short* list, int n, uint4_t* xs, uint4_t* lds)
 {
     constexpr int RT = GATED ? 2 * F : F;
-    typedef ExpertWeights<T, MX, TT> EW;
+    typedef ExpertWeights<T, MX> EW;
     const int lane = threadIdx.x & 63, wave = wave_in_block(), group = lane >> 4;
     const int f0 = blockIdx.x * (16 * F);
     typename EW::W::Rows rows[RT];
@@ -244,97 +240,90 @@ __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPoi
         const int end = i < F ? a.d_ff : 2 * a.d_ff, at = (i < F ? 0 : a.d_ff) + f0 + i % F * 16;
         rows[i] = EW::rows(p.w1, p.s1, p.t1, a.ld_s1, at < end ? at : end - 1, end, a.d_model);
     }
-    expert_sums<T, MX, SHARED, RT, TT, WK>(rows, a.d_model, n, xs, lds,
+    expert_sums<T, MX, SHARED, RT, WK>(rows, a.d_model, n, xs, lds,
                                    [&](int i) { return (const typename T::elem*)a.x + (int64_t)(list[i] / a.top_k) * a.ld_x; });
 #pragma unroll
-    for (int i = 0; i < F; ++i)
+    for (int i = 0; i < F; ++i) {
+        const int f = f0 + i * 16 + group * 4, column = lane & 15;
+        if (i % WK != wave || column >= n || f >= a.d_ff) continue;
+        const float4_t g = joined<RT, WK>(lds, i);
+        float4_t u = {}, h;
+        if constexpr (GATED) u = joined<RT, WK>(lds, F + i);
 #pragma unroll
-        for (int j = 0; j < TT; ++j) {
-            const int f = f0 + i * 16 + group * 4, column = j * 16 + (lane & 15);
-            if ((i * TT + j) % WK != wave || column >= n || f >= a.d_ff) continue;
-            const float4_t g = joined<RT, TT, WK>(lds, i, j);
-            float4_t u = {}, h;
-            if constexpr (GATED) u = joined<RT, TT, WK>(lds, F + i, j);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                float v = EW::unscale(g[c], p.t1, f + c);
-                if (p.b1) v += (float)((const typename T::elem*)p.b1)[f + c];
-                if (a.act == PIMHIP_EXPERT_RELU) v = relu_f32(v);
-                if (a.act == PIMHIP_EXPERT_SILU) v = v / (1.0f + __expf(-v));
-                if (GATED) {
-                    float w = EW::unscale(u[c], p.t1, a.d_ff + f + c);
-                    if (p.b1) w += (float)((const typename T::elem*)p.b1)[a.d_ff + f + c];
-                    v *= w;
-                }
-                h[c] = v;
+        for (int c = 0; c < 4; ++c) {
+            float v = EW::unscale(g[c], p.t1, f + c);
+            if (p.b1) v += (float)((const typename T::elem*)p.b1)[f + c];
+            if (a.act == PIMHIP_EXPERT_RELU) v = relu_f32(v);
+            if (a.act == PIMHIP_EXPERT_SILU) v = v / (1.0f + __expf(-v));
+            if (GATED) {
+                float w = EW::unscale(u[c], p.t1, a.d_ff + f + c);
+                if (p.b1) w += (float)((const typename T::elem*)p.b1)[a.d_ff + f + c];
+                v *= w;
             }
-            store4<T>((typename T::elem*)a.h + (int64_t)list[column] * a.d_ff + f, h, 4);  // (d_ff is a multiple of 8)
+            h[c] = v;
         }
+        store4<T>((typename T::elem*)a.h + (int64_t)list[column] * a.d_ff + f, h, 4);  // (d_ff is a multiple of 8)
+    }
     __syncthreads();
 }
 
-template <class T, bool MX, bool SHARED, bool GATED, int F, int TT, int WK>
-__global__ __launch_bounds__(64 * WK, TT == 1 ? 4 : 3) void moe_layer_first_kernel(MoeLayerArgs a)
+// Block (x, y, z): rows x of expert y for its pairs 16 z .. 16 z + 15; those of more than 16 pairs read the weights again, out of the
+// caches.  (A loop over pairs in one block instead costs so many registers that half the wavefronts fit: 39 us against 25 for 64 tokens
+// through 8 gated 4-bit experts 1024 -> 4096.)
+template <class T, bool MX, bool SHARED, bool GATED, int F, int WK>
+__global__ __launch_bounds__(64 * WK, F > 2 || (GATED && F > 1) ? 3 : 4) void moe_layer_first_kernel(MoeLayerArgs a)
 {
-    __shared__ ExpertLds<T, MX, GATED ? 2 * F : F, TT, WK> lds;
+    __shared__ ExpertLds<T, MX, SHARED, GATED ? 2 * F : F, WK> lds;
     extern __shared__ uint4_t xs[];
     const ExpertPointers p = a.experts[blockIdx.y];
-    const int n = pairs_of(a.chosen, a.tokens * a.top_k, blockIdx.y, lds.list, &lds.count);
-    for (int first = 0; first < n; first += 16 * TT) {  // (more than 16 * TT pairs of an expert read its weights again, out of the caches)
-        moe_first<T, MX, SHARED, GATED, F, TT, WK>(a, p, lds.list + first, n - first < 16 * TT ? n - first : 16 * TT, xs, lds.turn);
-        if (TT == 1) break;  // (a call of at most 16 tokens)
-    }
+    const int first = blockIdx.z * 16, n = pairs_of(a.chosen, a.tokens * a.top_k, blockIdx.y, lds.list, &lds.count) - first;
+    if (n > 0) moe_first<T, MX, SHARED, GATED, F, WK>(a, p, lds.list + first, n < 16 ? n : 16, xs, lds.turn);
 }
 
-// The second product of up to 16 * TT pairs: rows of d_model, with the bias, not yet weighted.
-template <class T, bool MX, bool SHARED, int RT, int TT, int WK>
+// The second product of up to 16 pairs: rows of d_model, with the bias, not yet weighted.
+template <class T, bool MX, bool SHARED, int RT, int WK>
 __device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPointers& p, const short* list, int n, uint4_t* xs, uint4_t* lds)
 {
-    typedef ExpertWeights<T, MX, TT> EW;
+    typedef ExpertWeights<T, MX> EW;
     const int lane = threadIdx.x & 63, wave = wave_in_block(), group = lane >> 4;
     const int d0 = blockIdx.x * (16 * RT);
     typename EW::W::Rows rows[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) rows[i] = EW::rows(p.w2, p.s2, p.t2, a.ld_s2, d0 + i * 16 < a.d_model ? d0 + i * 16 : a.d_model - 1, a.d_model, a.d_ff);
-    expert_sums<T, MX, SHARED, RT, TT, WK>(rows, a.d_ff, n, xs, lds, [&](int i) { return (const typename T::elem*)a.h + (int64_t)list[i] * a.d_ff; });
+    expert_sums<T, MX, SHARED, RT, WK>(rows, a.d_ff, n, xs, lds, [&](int i) { return (const typename T::elem*)a.h + (int64_t)list[i] * a.d_ff; });
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
+    for (int i = 0; i < RT; ++i) {
+        const int d = d0 + i * 16 + group * 4, column = lane & 15;
+        if (i % WK != wave || column >= n || d >= a.d_model) continue;
+        float4_t v = joined<RT, WK>(lds, i);
 #pragma unroll
-        for (int j = 0; j < TT; ++j) {
-            const int d = d0 + i * 16 + group * 4, column = j * 16 + (lane & 15);
-            if ((i * TT + j) % WK != wave || column >= n || d >= a.d_model) continue;
-            float4_t v = joined<RT, TT, WK>(lds, i, j);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                v[c] = EW::unscale(v[c], p.t2, d + c);
-                if (p.b2) v[c] += (float)((const typename T::elem*)p.b2)[d + c];
-            }
-            const uint4_t q = __builtin_bit_cast(uint4_t, v);
-            store16_device_scope(a.part + (int64_t)list[column] * a.d_model + d, q[0] | (unsigned long long)q[1] << 32, q[2] | (unsigned long long)q[3] << 32);
+        for (int c = 0; c < 4; ++c) {
+            v[c] = EW::unscale(v[c], p.t2, d + c);
+            if (p.b2) v[c] += (float)((const typename T::elem*)p.b2)[d + c];
         }
+        const uint4_t q = __builtin_bit_cast(uint4_t, v);
+        store16_device_scope(a.part + (int64_t)list[column] * a.d_model + d, q[0] | (unsigned long long)q[1] << 32, q[2] | (unsigned long long)q[3] << 32);
+    }
     __syncthreads();
 }
 
-// The block that is last to finish a tile of rows, of all experts' blocks, makes the weighted sum there, in the order of the choice.
+// Blocks as above.  The one that is last to finish a tile of rows, of all experts' blocks, makes the weighted sum there, in the order of the choice.
 // An expert without a share adds nothing, whatever it computed.  Sums of other blocks come from other XCDs: they were stored past the L2s and
 // are loaded past them, and each block waits for its stores before it counts itself.
-template <class T, bool MX, bool SHARED, int RT, int TT, int WK>
-__global__ __launch_bounds__(64 * WK, TT == 1 ? 4 : 3) void moe_layer_second_kernel(MoeLayerArgs a)
+template <class T, bool MX, bool SHARED, int RT, int WK>
+__global__ __launch_bounds__(64 * WK, 4) void moe_layer_second_kernel(MoeLayerArgs a)
 {
-    __shared__ ExpertLds<T, MX, RT, TT, WK> lds;
+    __shared__ ExpertLds<T, MX, SHARED, RT, WK> lds;
     __shared__ unsigned int before;
     extern __shared__ uint4_t xs[];
     const ExpertPointers p = a.experts[blockIdx.y];
-    const int n = pairs_of(a.chosen, a.tokens * a.top_k, blockIdx.y, lds.list, &lds.count);
-    for (int first = 0; first < n; first += 16 * TT) {
-        moe_second<T, MX, SHARED, RT, TT, WK>(a, p, lds.list + first, n - first < 16 * TT ? n - first : 16 * TT, xs, lds.turn);
-        if (TT == 1) break;
-    }
+    const int first = blockIdx.z * 16, n = pairs_of(a.chosen, a.tokens * a.top_k, blockIdx.y, lds.list, &lds.count) - first;
+    if (n > 0) moe_second<T, MX, SHARED, RT, WK>(a, p, lds.list + first, n < 16 ? n : 16, xs, lds.turn);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) before = __hip_atomic_fetch_add(&a.counters[blockIdx.x], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    if (before != gridDim.y - 1) return;
+    if (before != gridDim.y * gridDim.z - 1) return;
     constexpr int kWords = 16 * RT / 4;  // of four rows
     for (int i = threadIdx.x; i < a.tokens * kWords; i += 64 * WK) {
         const int token = i / kWords, d = blockIdx.x * (16 * RT) + i % kWords * 4;
