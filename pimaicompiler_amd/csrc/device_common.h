@@ -116,6 +116,21 @@ __device__ __forceinline__ float wave_sum(float v)
     return wave_sum_rows(v);
 }
 
+// Maximum over the 64 lanes of a wavefront, a NaN counting as nothing; every lane returns it.
+__device__ __forceinline__ float wave_max_f32(float v)
+{
+    v = fmaxf(v, dpp_f32<kDppQuadXor1>(v));
+    v = fmaxf(v, dpp_f32<kDppQuadXor2>(v));
+    v = fmaxf(v, dpp_f32<kDppRowHalfMirror>(v));
+    v = fmaxf(v, dpp_f32<kDppRowMirror>(v));
+    const unsigned int b = __builtin_bit_cast(unsigned int, v);
+    const auto p = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    v = fmaxf(__builtin_bit_cast(float, (unsigned int)p[0]), __builtin_bit_cast(float, (unsigned int)p[1]));
+    const unsigned int c = __builtin_bit_cast(unsigned int, v);
+    const auto q = __builtin_amdgcn_permlane32_swap(c, c, false, false);
+    return fmaxf(__builtin_bit_cast(float, (unsigned int)q[0]), __builtin_bit_cast(float, (unsigned int)q[1]));
+}
+
 // Maximum over the 64 lanes of a wavefront; every lane returns it.
 __device__ __forceinline__ unsigned int wave_max_u32(unsigned int v)
 {

@@ -6,8 +6,8 @@
 // One pass over a row by one block: every thread keeps m, s and t of its own pieces (eight values each) in fp32 and, for the
 // alternatives, its largest value and the piece that holds it.  Bound by reading the logits.
 // Alternatives: the threads form 64 groups; the k-th largest of the groups' best (value, piece) is a bound that at least k values
-// reach, so only threads whose own best reaches it look at their pieces again (out of the caches).  What reaches the bound goes to LDS,
-// some more than k values as a rule, and is ranked there; ties go to the lowest index.
+// reach, so only pieces of threads whose own best reaches it are looked at again (out of the caches).  What reaches the bound goes to
+// LDS, some more than k values as a rule, and is ranked there; ties go to the lowest index.
 #pragma once
 
 #include "mx4_format.h"
@@ -15,7 +15,6 @@
 namespace pimhip
 {
 static constexpr int kTopMost = 32;            // alternatives a call can ask for
-static constexpr int kTopCandidates = 4096;    // values that may reach the bound before a block goes over to one pass per alternative
 static constexpr float kFarBelow = -10000.0f;  // exp of it is 0, and so is its product with it
 
 // A value's place in the order of all values, as a whole number: -0 with 0, infinities at the ends.
@@ -27,30 +26,71 @@ __device__ __forceinline__ unsigned int ordered_bits(float v)
 
 __device__ __forceinline__ float from_ordered(unsigned int o) { return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 
-// d, but nothing below kFarBelow; a NaN stays one.
-__device__ __forceinline__ float not_far_below(float d) { return d < kFarBelow ? kFarBelow : d; }
-
-// Eight values of a piece as fp32; those behind the row's end are -inf.
+// Eight values of a whole piece as fp32.
 template <class T>
-__device__ __forceinline__ void load_piece(const typename T::elem* row, int64_t piece, int64_t V, float (&v)[8])
+__device__ __forceinline__ void load_piece(const typename T::elem* row, int64_t piece, float (&v)[8])
 {
     typename T::elem e[8];
-    if (piece * 8 + 8 <= V) {
-        const uint4_any_t* p = reinterpret_cast<const uint4_any_t*>(row + piece * 8);
-        if constexpr (sizeof(e[0]) == 2) {
-            const uint4_t q = p[0];
-            __builtin_memcpy(e, &q, 16);
-        } else {
-            const uint4_t q0 = p[0], q1 = p[1];
-            __builtin_memcpy(e, &q0, 16);
-            __builtin_memcpy(e + 4, &q1, 16);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float)e[i];
+    const uint4_any_t* p = reinterpret_cast<const uint4_any_t*>(row + piece * 8);
+    if constexpr (sizeof(e[0]) == 2) {
+        const uint4_t q = p[0];
+        __builtin_memcpy(e, &q, 16);
     } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = piece * 8 + i < V ? (float)row[piece * 8 + i] : -__builtin_inff();
+        const uint4_t q0 = p[0], q1 = p[1];
+        __builtin_memcpy(e, &q0, 16);
+        __builtin_memcpy(e + 4, &q1, 16);
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)e[i];
+}
+
+// The values of a row, eight at a time, those of thread tid being pieces tid, tid + THREADS, ...: f(piece, its values, how many of them
+// there are).  Four pieces are loaded together; behind the row's end they are -inf.
+template <class T, int THREADS, class F>
+__device__ __forceinline__ void each_four_pieces(const typename T::elem* row, int64_t V, F f)
+{
+    const int64_t whole = V / 8;
+    for (int64_t p = threadIdx.x; p < whole; p += 4 * THREADS) {
+        float v[4][8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_piece<T>(row, p + i * THREADS < whole ? p + i * THREADS : whole - 1, v[i]);
+        if (p - threadIdx.x + 4 * THREADS > whole) {
+#pragma unroll
+            for (int i = 1; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) v[i][c] = p + i * THREADS < whole ? v[i][c] : -__builtin_inff();
+        }
+        f(p, v);
+    }
+    if (V % 8 != 0 && threadIdx.x == whole % THREADS) {
+        float v[4][8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            v[0][c] = whole * 8 + c < V ? (float)row[whole * 8 + c] : -__builtin_inff();
+            v[1][c] = v[2][c] = v[3][c] = -__builtin_inff();
+        }
+        f(whole, v);
+    }
+}
+
+// The larger of two keys over the LANES (1, 4 or 16) lanes of a group; every lane returns it.
+template <int LANES>
+__device__ __forceinline__ unsigned long long group_max_u64(unsigned long long k)
+{
+    auto with = [&](unsigned int hi, unsigned int lo) {
+        const unsigned long long o = (unsigned long long)hi << 32 | lo;
+        k = o > k ? o : k;
+    };
+    static_assert(LANES == 1 || LANES == 4 || LANES == 16, "a group is part of a row of 16 lanes");
+    if constexpr (LANES >= 4) {
+        with(dpp_u32<kDppQuadXor1>((unsigned int)(k >> 32)), dpp_u32<kDppQuadXor1>((unsigned int)k));
+        with(dpp_u32<kDppQuadXor2>((unsigned int)(k >> 32)), dpp_u32<kDppQuadXor2>((unsigned int)k));
+    }
+    if constexpr (LANES == 16) {
+        with(dpp_u32<kDppRowHalfMirror>((unsigned int)(k >> 32)), dpp_u32<kDppRowHalfMirror>((unsigned int)k));
+        with(dpp_u32<kDppRowMirror>((unsigned int)(k >> 32)), dpp_u32<kDppRowMirror>((unsigned int)k));
+    }
+    return k;
 }
 
 struct LogProbArgs {
@@ -71,45 +111,53 @@ __global__ __launch_bounds__(THREADS) void token_log_probs_kernel(LogProbArgs a)
     constexpr int kWaves = THREADS / 64, kPerGroup = THREADS / 64;
     __shared__ float wave_f[3][kWaves];
     __shared__ unsigned long long group_best[64];
-    __shared__ unsigned long long candidates[kTopCandidates];
+    constexpr int kCandidates = THREADS == 64 ? 1024 : 4096;
+    __shared__ unsigned long long candidates[kCandidates + 8];
+    __shared__ unsigned short owners[THREADS];
     __shared__ unsigned long long bound, found;
-    __shared__ int count;
+    __shared__ int count, owner_count;
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_in_block();
     const int64_t row = blockIdx.x, V = a.V;
     const typename T::elem* x = (const typename T::elem*)a.logits + row * a.ld;
-    const int64_t pieces = (V + 7) / 8;
 
     // ---- the pass ----
+    // t only wants the product of a value that is far below with its exp to be 0; what is not finite shows in s.
     float m = -3.402823466e+38f, s = 0.0f, t = 0.0f;
     float best = -__builtin_inff();
     unsigned int best_piece = 0xffffffffu;
-    for (int64_t p = tid; p < pieces; p += THREADS) {
-        float v[8];
-        load_piece<T>(x, p, V, v);
-        float top = v[0];
+    each_four_pieces<T, THREADS>(x, V, [&](int64_t p, const float(&v)[4][8]) {
+        float top[4];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) top = fmaxf(top, v[i]);
-        if (top > best || best_piece == 0xffffffffu) {
-            best = top;
-            best_piece = (unsigned int)p;
+        for (int i = 0; i < 4; ++i) {
+            top[i] = v[i][0];
+#pragma unroll
+            for (int c = 1; c < 8; ++c) top[i] = fmaxf(top[i], v[i][c]);
         }
-        const float mn = fmaxf(m, top);
-        const float step = not_far_below(m - mn), f = __expf(step);
+        const float mn = fmaxf(fmaxf(fmaxf(m, top[0]), fmaxf(top[1], top[2])), top[3]);
+        if (mn > best || best_piece == 0xffffffffu) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (top[i] > best || best_piece == 0xffffffffu) {
+                    best = top[i];
+                    best_piece = (unsigned int)p + i * THREADS;
+                }
+        }
+        const float step = fmaxf(m - mn, kFarBelow), f = __expf(step);
         t = f * (t + s * step);
         s *= f;
         m = mn;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float d = not_far_below(v[i] - m), e = __expf(d);
-            s += e;
-            t += e * d;
-        }
-    }
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const float d = v[i][c] - m, e = __expf(d);
+                s += e;
+                t = fmaf(e, fmaxf(d, kFarBelow), t);
+            }
+    });
 
     // ---- the row's m, s, t ----
-    float bm = m;
-#pragma unroll
-    for (int i = 1; i < 64; i <<= 1) bm = fmaxf(bm, __shfl_xor(bm, i));
+    float bm = wave_max_f32(m);
     if (kWaves > 1) {
         if (lane == 0) wave_f[0][wave] = bm;
         __syncthreads();
@@ -118,7 +166,7 @@ __global__ __launch_bounds__(THREADS) void token_log_probs_kernel(LogProbArgs a)
         for (int i = 1; i < kWaves; ++i) bm = fmaxf(bm, wave_f[0][i]);
     }
     {
-        const float step = not_far_below(m - bm), f = __expf(step);
+        const float step = fmaxf(m - bm, kFarBelow), f = __expf(step);
         t = f * (t + s * step);
         s *= f;
     }
@@ -164,15 +212,14 @@ __global__ __launch_bounds__(THREADS) void token_log_probs_kernel(LogProbArgs a)
     auto key_of = [](float v, unsigned int at) { return ((unsigned long long)ordered_bits(v) << 32) | (unsigned int)~at; };
     auto larger = [](unsigned long long p, unsigned long long q) { return p > q ? p : q; };
     const unsigned long long mine = best_piece == 0xffffffffu ? 0ull : key_of(best, best_piece);
-    unsigned long long g = mine;
-#pragma unroll
-    for (int i = 1; i < kPerGroup; i <<= 1) g = larger(g, __shfl_xor(g, i));
+    const unsigned long long g = group_max_u64<kPerGroup>(mine);
     if (tid % kPerGroup == 0) group_best[tid / kPerGroup] = g;
-    if (tid == 0) count = 0;
+    if (tid == 0) count = owner_count = 0;
     __syncthreads();
     if (wave == 0) {
         const unsigned long long k = group_best[lane];
         int rank = 0;  // (empty groups, all 0, go by their number)
+#pragma unroll
         for (int i = 0; i < 64; ++i) {
             const unsigned long long o = group_best[i];
             rank += o > k || (o == k && i < lane) ? 1 : 0;
@@ -180,17 +227,27 @@ __global__ __launch_bounds__(THREADS) void token_log_probs_kernel(LogProbArgs a)
         if (rank == top - 1) bound = k;
     }
     __syncthreads();
+    // The threads whose best reaches the bound name themselves, and the block looks at their pieces, a thread a piece.
     const unsigned long long at_least = bound;
-    if (mine != 0ull && mine >= at_least) {
-        for (int64_t p = tid; p < pieces; p += THREADS) {
-            float v[8];
-            load_piece<T>(x, p, V, v);
+    const float least = at_least == 0ull ? -__builtin_inff() : from_ordered((unsigned int)(at_least >> 32));
+    if (mine != 0ull && mine >= at_least) owners[atomicAdd(&owner_count, 1)] = (unsigned short)tid;
+    __syncthreads();
+    const unsigned int named = (unsigned int)owner_count, pieces = (unsigned int)((V + 7) / 8), each = (pieces + THREADS - 1) / THREADS;
+    for (unsigned int i = tid; i < named * each; i += THREADS) {
+        const unsigned int p = owners[i % named] + i / named * THREADS;
+        if (p >= pieces) continue;
+        float v[8];
+        if ((int64_t)p * 8 + 8 <= V) {
+            load_piece<T>(x, p, v);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (p * 8 + i >= V || key_of(v[i], (unsigned int)p) < at_least) continue;
-                const int n = atomicAdd(&count, 1);
-                if (n < kTopCandidates) candidates[n] = key_of(v[i], (unsigned int)(p * 8 + i));
-            }
+            for (int c = 0; c < 8; ++c) v[c] = (int64_t)p * 8 + c < V ? (float)x[(int64_t)p * 8 + c] : __builtin_nanf("");
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            if (!(v[c] >= least) || key_of(v[c], p) < at_least) continue;
+            const int n = atomicAdd(&count, 1);
+            if (n < kCandidates) candidates[n] = key_of(v[c], p * 8 + c);
         }
     }
     __syncthreads();
@@ -199,11 +256,15 @@ __global__ __launch_bounds__(THREADS) void token_log_probs_kernel(LogProbArgs a)
         a.top_ids[row * top + rank] = (int)~(unsigned int)key;
     };
     const int n = count;
-    if (n <= kTopCandidates) {
+    if (n <= kCandidates) {
+        if (tid < 8) candidates[n + tid] = 0ull;  // (a rank is counted eight at a time)
+        __syncthreads();
         for (int i = tid; i < n; i += THREADS) {
             const unsigned long long k = candidates[i];
             int rank = 0;
-            for (int j = 0; j < n && rank < top; ++j) rank += candidates[j] > k ? 1 : 0;
+            for (int j = 0; j < n && rank < top; j += 8)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) rank += candidates[j + c] > k ? 1 : 0;
             if (rank < top) store(rank, k);
         }
         return;
@@ -212,15 +273,16 @@ __global__ __launch_bounds__(THREADS) void token_log_probs_kernel(LogProbArgs a)
     unsigned long long below = ~0ull;
     for (int i = 0; i < top; ++i) {
         unsigned long long k = 0;
-        for (int64_t p = tid; p < pieces; p += THREADS) {
-            float v[8];
-            load_piece<T>(x, p, V, v);
+        each_four_pieces<T, THREADS>(x, V, [&](int64_t first, const float(&v)[4][8]) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                const unsigned long long q = key_of(v[c], (unsigned int)(p * 8 + c));
-                if (p * 8 + c < V && q < below) k = larger(k, q);
-            }
-        }
+            for (int h = 0; h < 4; ++h)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const int64_t at = (first + h * THREADS) * 8 + c;
+                    const unsigned long long q = key_of(v[h][c], (unsigned int)at);
+                    if (at < V && q < below) k = larger(k, q);
+                }
+        });
         __syncthreads();
         if (tid == 0) found = 0ull;
         __syncthreads();
