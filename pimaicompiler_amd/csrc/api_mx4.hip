@@ -6,7 +6,7 @@ using namespace pimhip;
 
 namespace
 {
-constexpr int64_t kMaxCols = 1 << 28;  // (16 rows' bytes are counted in 32 bits)
+constexpr int64_t kMaxCols = 1 << 26;  // (64 rows' bytes are counted in 32 bits)
 
 int check_matrix(const char* name, const PimHipMx4Matrix* m, Mx4View* v)
 {
@@ -14,8 +14,9 @@ int check_matrix(const char* name, const PimHipMx4Matrix* m, Mx4View* v)
     if (m->rows < 0 || m->cols < 1 || m->cols > kMaxCols)
         return fail(PIMHIP_ERR_INVALID_ARGUMENT, "%s: rows=%lld, cols=%lld (cols in [1, %lld])", name, (long long)m->rows, (long long)m->cols, (long long)kMaxCols);
     const int64_t blocks = (m->cols + kMxBlock - 1) / kMxBlock;
-    if (m->ld_scales < blocks || (m->ld_scales & 15))
-        return fail(PIMHIP_ERR_INVALID_ARGUMENT, "%s: ld_scales=%lld must be a multiple of 16 and at least %lld", name, (long long)m->ld_scales, (long long)blocks);
+    if (m->ld_scales < blocks || m->ld_scales > kMaxCols || (m->ld_scales & 15))
+        return fail(PIMHIP_ERR_INVALID_ARGUMENT, "%s: ld_scales=%lld must be a multiple of 16 in [%lld, %lld]", name, (long long)m->ld_scales, (long long)blocks,
+                    (long long)kMaxCols);
     if (m->rows && (!m->packed || !m->scales || !m->tops)) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "%s: packed, scales and tops must be non-null", name);
     if (!aligned16(m->packed) || !aligned16(m->scales)) return fail(PIMHIP_ERR_UNSUPPORTED, "%s: packed and scales must be 16-byte aligned", name);
     *v = Mx4View{(const uint8_t*)m->packed, (const uint8_t*)m->scales, (const uint8_t*)m->tops, m->rows, m->cols, m->ld_scales};
@@ -96,15 +97,11 @@ int matmul(void* out, int64_t ld_out, const Mx4View& a, const Mx4View& b, hipStr
     };
     if (a.rows <= 16) return run(mx4_matmul_skinny_kernel<O, 1, 1, 4>, 1, 1, 4);
     if (a.rows <= 64) return run(mx4_matmul_skinny_kernel<O, 1, 4, 4>, 1, 4, 4);
-    auto tiled = [&](auto kernel, int n, int t, int threads) {
-        const int64_t tiles = ((b.rows + n - 1) / n) * ((a.rows + t - 1) / t);
-        const int rc = check_grid(tiles, 1);
-        if (rc != PIMHIP_OK) return rc;
-        kernel<<<dim3((unsigned)tiles), threads, 0, s>>>(a, b, (typename O::elem*)out, ld_out);
-        return (int)PIMHIP_OK;
-    };
-    if (((b.rows + 255) / 256) * ((a.rows + 255) / 256) >= 192) return tiled(mx4_matmul_tile_kernel<O, 8, 4, 2, 4>, 256, 256, 512);
-    return tiled(mx4_matmul_tile_kernel<O, 4, 4, 2, 2>, 128, 128, 256);
+    const int64_t tiles = ((b.rows + 127) / 128) * ((a.rows + 127) / 128);
+    const int rc = check_grid(tiles, 1);
+    if (rc != PIMHIP_OK) return rc;
+    mx4_matmul_tile_kernel<O><<<dim3((unsigned)tiles), 256, 0, s>>>(a, b, (typename O::elem*)out, ld_out);
+    return PIMHIP_OK;
 }
 }  // namespace
 

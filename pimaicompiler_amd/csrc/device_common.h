@@ -162,6 +162,28 @@ __device__ __forceinline__ void lds_only_barrier()
     asm volatile("" ::: "memory");
 }
 
+// 16 bytes per lane from memory straight into LDS: lane l's at `lds_base` + 16 l (lds_base: the same in all lanes).  Counted by
+// vmcnt; nothing but an explicit wait orders it.  (The compiler allocates m0 to nothing and sets it in front of each use of its
+// own, but it joins equal settings of m0 where it sees none in between: it is told of this one, and warns that m0 is reserved.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void load_lds16(const void* src, unsigned int lds_base)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_base), "v"(src) : "memory", "m0");
+}
+// The same from `at` bytes behind an address that all lanes have in common.
+__device__ __forceinline__ void load_lds16(const void* src, unsigned int at, unsigned int lds_base)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds_base), "v"(at), "s"(src) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+template <int N>
+__device__ __forceinline__ void wait_loads_and_barrier()
+{
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
+}
+
 // Every bounded wait of the kernels here also ends after kWaitTicks of the constant 100 MHz clock, whatever its poll
 // count: where a poll takes far longer than usual (counter collection serialising the memory system, a tool stepping the
 // device), the poll limit alone bounds nothing useful.  Called every 256 unsuccessful polls; `t_first` keeps the time of

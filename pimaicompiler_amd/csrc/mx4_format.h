@@ -95,6 +95,19 @@ __device__ __forceinline__ typename T::frag load8_guarded(const typename T::elem
     return v;
 }
 
+// Eight results of one row, next to each other from p on.
+template <class O>
+__device__ __forceinline__ void store8(typename O::elem* p, const float4_t v, const float4_t w)
+{
+    if constexpr (sizeof(typename O::elem) == 2) {
+        const typename O::elem r[8] = {O::round(v[0]), O::round(v[1]), O::round(v[2]), O::round(v[3]), O::round(w[0]), O::round(w[1]), O::round(w[2]), O::round(w[3])};
+        *reinterpret_cast<uint4_any_t*>(p) = __builtin_bit_cast(uint4_t, r);
+    } else {
+        reinterpret_cast<uint4_any_t*>(p)[0] = __builtin_bit_cast(uint4_t, v);
+        reinterpret_cast<uint4_any_t*>(p)[1] = __builtin_bit_cast(uint4_t, w);
+    }
+}
+
 // Four results of one row, next to each other from p on, of which `count` exist.
 template <class O>
 __device__ __forceinline__ void store4(typename O::elem* p, const float4_t v, int count)

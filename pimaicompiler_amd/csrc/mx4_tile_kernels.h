@@ -10,16 +10,18 @@
 
 namespace pimhip
 {
-// Which tile a block has: consecutive blocks go to consecutive XCDs, each with an L2 of its own, so an XCD gets a run of tiles, down
-// a column of tokens first: they share the weights' rows.
-__device__ __forceinline__ void tile_of_block(int64_t tiles_n, int64_t tiles_t, int64_t& n, int64_t& t)
+// Tile `id` of a product.  Consecutive blocks go to consecutive XCDs, each with an L2 of its own, so an XCD gets a run of tiles: down
+// a band of eight token tiles first, then to the next weights.  The 32 tiles that an XCD has at work at a time are about as high as
+// wide, so they bring the fewest rows into its L2.
+__device__ __forceinline__ void tile_at(int id, int tiles_n, int tiles_t, int64_t& n, int64_t& t)
 {
-    constexpr int64_t kXcds = 8;
-    const int64_t all = tiles_n * tiles_t, id = blockIdx.x;
-    const int64_t per = all / kXcds, more = all % kXcds, xcd = id % kXcds;
-    const int64_t at = xcd * per + (xcd < more ? xcd : more) + id / kXcds;
-    n = at / tiles_t;
-    t = at % tiles_t;
+    constexpr int kXcds = 8, kBand = 8;
+    const int all = tiles_n * tiles_t, per = all / kXcds, more = all % kXcds, xcd = id % kXcds;
+    const int at = xcd * per + (xcd < more ? xcd : more) + id / kXcds;
+    const int band = at / (kBand * tiles_n), high = tiles_t - band * kBand < kBand ? tiles_t - band * kBand : kBand;
+    const int in = at - band * kBand * tiles_n;
+    n = in / high;
+    t = band * kBand + in % high;
 }
 
 // ---- x in 16 bits, weights in 4 ----------------------------------------------------------------------------------------------
@@ -41,7 +43,7 @@ __global__ __launch_bounds__(64 * GN * GT) void mx4_linear_tile_kernel(const typ
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_in_block(), group = lane >> 4, row = lane & 15;
     const int wn = wave % GN * WN, wt = wave / GN * WT;
     int64_t tile_n, tile_t;
-    tile_of_block((w.rows + kN - 1) / kN, (M + kT - 1) / kT, tile_n, tile_t);
+    tile_at(blockIdx.x, (int)((w.rows + kN - 1) / kN), (int)((M + kT - 1) / kT), tile_n, tile_t);
     const int64_t n0 = tile_n * kN, t0 = tile_t * kT, K = w.cols;
     const int blocks = (int)((K + kMxBlock - 1) / kMxBlock);
 
@@ -157,119 +159,165 @@ __global__ __launch_bounds__(64 * GN * GT) void mx4_linear_tile_kernel(const typ
 }
 
 // ---- both operands in 4 bits -------------------------------------------------------------------------------------------------
-// Steps of 128 values of k, one product (v_mfma_scale_f32_16x16x128_f8f6f4) a tile: a lane holds one block of each operand.  The scale
-// codes of four tiles' blocks share a 32-bit word of LDS; the instruction picks its byte.
-template <class O, int WN, int WT, int GN, int GT>
-__global__ __launch_bounds__(64 * GN * GT) void mx4_matmul_tile_kernel(Mx4View a, Mx4View b, typename O::elem* out, int64_t ld_out)
+// 128 x 128 results a block, a wavefront 64 x 64; steps of 256 values of k: the 128 bytes of a row that are a cache line, two products
+// (v_mfma_scale_f32_16x16x128_f8f6f4) a tile.  A lane holds one block of each operand and its scale code.  A step goes from memory
+// straight into LDS while the one before is multiplied, operands go from LDS to registers a product ahead, and two blocks of a CU fill
+// each other's waits.
+//
+// 4096 x 16384 x 4096: 193 us, 2.85 PFLOP/s (a loop of the instruction alone reaches 7 to 8.8 here).  Two of these blocks' steps take
+// 1.5 us, of which the matrix cores work 0.5 and LDS is read and written 0.7: what is left waits for a step to arrive, which takes a
+// microsecond, and LDS holds no more steps.  Measured besides: steps of 128 values, three or four on their way, 227 (half a line is
+// a whole request); 256 x 256 results a block, one block a CU, 198 with steps of 128, 226 with steps of 256, and slower by half and
+// more where blocks are few; each code word loaded with its step 301 (a row's code is a request, however few bytes it has).
+template <class O>
+__global__ __launch_bounds__(256, 2) void mx4_matmul_tile_kernel(Mx4View a, Mx4View b, typename O::elem* out, int64_t ld_out)
 {
-    constexpr int kThreads = 64 * GN * GT, kN = 16 * GN * WN, kT = 16 * GT * WT, kRows = kN + kT;
-    constexpr int kPieces = kRows * 4 / kThreads;  // blocks of either operand a thread brings each step
-    static_assert(kPieces * kThreads == kRows * 4 && kRows <= kThreads && WN % 4 == 0 && WT % 4 == 0, "whole pieces a thread, a row of scales each");
-    __shared__ uint4_t values[2][kRows * 4];            // the rows of b, then those of a; block c of a row at c ^ (row / 4 % 4)
-    __shared__ unsigned int codes[2][kRows / 64][64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = wave_in_block(), group = lane >> 4, row = lane & 15;
-    const int wn = wave % GN * WN, wt = wave / GN * WT;
+    constexpr int kTile = 128, kRows = 2 * kTile, kPieces = 8;  // (a wavefront brings 64 rows, a load 128 bytes of eight)
+    constexpr int kBuffer = kRows * 128, kCodes = kRows * 16;
+    // A step: the rows of b, then those of a, block c of row r at c ^ turned(r).  16 lanes of a read have 16 different places of two rows'
+    // 256 bytes, whether their rows follow each other or skip four of eight.  Codes come for two steps at a time.
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kBuffer + 2 * kCodes];
+    auto turned = [](int r) { return (r >> 1 ^ (r >> 3 & 2)) & 7; };
+    // The rows that lane `l` multiplies in tile i of four.  Two tiles of weights take turns, four and four: a lane then has eight neighbours
+    // of a row of the result.
+    auto weight_row = [](int l, int i) { return (i & 2) * 16 + l / 4 * 8 + (i & 1) * 4 + l % 4; };
+    auto token_row = [](int l, int i) { return i * 16 + l; };
+    const int lane = threadIdx.x & 63, wave = wave_in_block(), group = lane >> 4, row = lane & 15;
+    const int wn = wave % 2 * 64, wt = wave / 2 * 64;
     int64_t tile_n, tile_t;
-    tile_of_block((b.rows + kN - 1) / kN, (a.rows + kT - 1) / kT, tile_n, tile_t);
-    const int64_t n0 = tile_n * kN, t0 = tile_t * kT;
-    const int blocks = (int)((b.cols + kMxBlock - 1) / kMxBlock);
-    // Row r of the tile: its matrix, and its row there (the last one again behind the end).
-    const uint8_t* vp[kPieces];
-    const int vb = tid % 4;
+    tile_at(blockIdx.x, (int)((b.rows + kTile - 1) / kTile), (int)((a.rows + kTile - 1) / kTile), tile_n, tile_t);
+    const int64_t n0 = tile_n * kTile, t0 = tile_t * kTile;
+    const int blocks = (int)((b.cols + kMxBlock - 1) / kMxBlock), whole = blocks / 8;
+
+    // A wavefront brings rows of one matrix, from `from` on; those behind its end are its last one again.
+    const bool weights = wave < 2;
+    const Mx4View& m = weights ? b : a;
+    const int64_t first = weights ? n0 + wave * 64 : t0 + wave * 64 - kTile, from = first < m.rows ? first : m.rows - 1;
+    const int most = (int)(m.rows - 1 - from < 63 ? m.rows - 1 - from : 63);
+    const uint8_t *vp = m.packed + from * blocks * kMxBlockBytes, *cp = m.scales + from * m.ld_scales;
+    unsigned int v_at[kPieces], c_at;
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-        const int r = (tid + i * kThreads) / 4;
-        const int64_t last = (r < kN ? b.rows : a.rows) - 1, at = r < kN ? n0 + r : t0 + r - kN;
-        vp[i] = (r < kN ? b.packed : a.packed) + ((at < last ? at : last) * blocks + vb) * kMxBlockBytes;
+        const int r = i * 8 + lane / 8;
+        v_at[i] = (unsigned int)((r < most ? r : most) * blocks + ((lane & 7) ^ turned(r))) * kMxBlockBytes;
     }
-    const uint8_t* cp = nullptr;
-    if (tid < kRows) {
-        const int64_t last = (tid < kN ? b.rows : a.rows) - 1, at = tid < kN ? n0 + tid : t0 + tid - kN;
-        cp = (tid < kN ? b.scales : a.scales) + (at < last ? at : last) * (tid < kN ? b.ld_scales : a.ld_scales);
-    }
-    uint4_t v[kPieces];
-    unsigned int c = 0;
-    auto fetch = [&](int step) {
-        if (step * 4 + 4 <= blocks) {
+    const int c_row = weights ? weight_row(row, group) : token_row(row, group);
+    c_at = (unsigned int)(c_row < most ? c_row : most) * (unsigned int)m.ld_scales;
+    const unsigned int lds0 = (unsigned int)(size_t)(__attribute__((address_space(3))) uint8_t*)lds;
+    // Rows a power of two apart have the same step's bytes in the same few channels of an L2: column tiles start k at places of their own.
+    const int turn = whole > 0 && whole % 2 == 0 ? (int)(tile_t & 15) * 4 % whole : 0;
+    auto fetch = [&](int step) __attribute__((always_inline)) {
+        int at = step + turn;
+        at = at < whole ? at : at - whole;
+        if (step % 2 == 0) load_lds16(cp + at * 8, c_at, lds0 + 2 * kBuffer + (unsigned int)(step / 2 % 2) * kCodes + (unsigned int)wave * 1024u);
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) v[i] = *reinterpret_cast<const uint4_t*>(vp[i] + (int64_t)step * (4 * kMxBlockBytes));
-            if (tid < kRows) c = *reinterpret_cast<const unsigned int*>(cp + step * 4);
+        for (int i = 0; i < kPieces; ++i)
+            load_lds16(vp + (int64_t)at * (8 * kMxBlockBytes), v_at[i], lds0 + (unsigned int)(step % 2) * kBuffer + (unsigned int)(wave * kPieces + i) * 1024u);
+    };
+
+    struct Part {  // four tiles' operands, and their codes (byte `group` of what is read) in one register
+        uint4_t v[4];
+        unsigned int c;
+    };
+    const unsigned int pick = 0x0c0c0000u | (unsigned int)(group | (group + 4) << 8);  // (0x0c: a byte of zeros)
+    const int p_at[2] = {((wn + weight_row(row, 0)) * 8 + (group ^ turned(weight_row(row, 0)))) * 16,
+                         ((wn + weight_row(row, 1)) * 8 + (group ^ turned(weight_row(row, 1)))) * 16};
+    const int t_at[2] = {((kTile + wt + row) * 8 + (group ^ turned(row))) * 16, ((kTile + wt + 16 + row) * 8 + (group ^ turned(16 + row))) * 16};
+    const int pc_at = 2 * kBuffer + (wn + row) * 16, tc_at = 2 * kBuffer + (kTile + wt + row) * 16;
+    Part p[2], t[2];
+    // Operands of half `half` of a step's k.
+    auto read = [&](int step, int half) __attribute__((always_inline)) {
+        const int base = step % 2 * kBuffer, word = (step / 2 % 2) * kCodes + (step % 2 * 2 + half) * 4;
+        auto part = [&](Part& x, const int(&at)[2], int c_at) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x.v[i] = *reinterpret_cast<const uint4_t*>(lds + base + (at[i & 1] ^ half * 64) + (i & 2) * 2048);
+            const unsigned int* q = reinterpret_cast<const unsigned int*>(lds + c_at + word);
+            x.c = __builtin_amdgcn_perm(q[64], q[0], pick) | __builtin_amdgcn_perm(q[192], q[128], pick) << 16;
+        };
+        part(t[half], t_at, tc_at);
+        part(p[half], p_at, pc_at);
+    };
+    float4_t acc[4][4] = {};
+    auto multiply = [&](const Part& p, const Part& t) __attribute__((always_inline)) {
+        auto wide = [](const uint4_t& q) { return int8v_t{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0}; };
+        // (which byte of the codes is part of the instruction)
+#define PIMHIP_MX4_STEP(i, j) \
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(p.v[i]), wide(t.v[j]), acc[i][j], 4, 4, i, (int)p.c, j, (int)t.c)
+#define PIMHIP_MX4_STEPS(i) PIMHIP_MX4_STEP(i, 0), PIMHIP_MX4_STEP(i, 1), PIMHIP_MX4_STEP(i, 2), PIMHIP_MX4_STEP(i, 3)
+        PIMHIP_MX4_STEPS(0), PIMHIP_MX4_STEPS(1), PIMHIP_MX4_STEPS(2), PIMHIP_MX4_STEPS(3);
+#undef PIMHIP_MX4_STEPS
+#undef PIMHIP_MX4_STEP
+    };
+    // Half of a step, while the operands of the next half are read, if there is one.
+    auto product = [&](int step, int half, bool next) __attribute__((always_inline)) {
+        if (next) {
+            if (half == 1) {  // everybody has read the step, and the next one is there
+                wait_loads_and_barrier<0>();
+                if (step + 2 < whole) fetch(step + 2);
+            }
+            read(step + half, half ^ 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // (the reads stay before the products that they run under)
+        multiply(p[half], t[half]);
+    };
+
+    if (whole > 0) {
+        fetch(0);
+        if (whole > 1) {
+            fetch(1);
+            wait_loads_and_barrier<kPieces>();  // (those of the second step)
         } else {
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                v[i] = uint4_t{0, 0, 0, 0};
-                if (step * 4 + vb < blocks) v[i] = *reinterpret_cast<const uint4_t*>(vp[i] + (int64_t)step * (4 * kMxBlockBytes));
-            }
-            // (whole groups of 16 codes a row) Behind the row's last block: any code but "not a number".
-            if (tid < kRows) {
-                c = *reinterpret_cast<const unsigned int*>(cp + step * 4);
-                const unsigned int in = (1u << (8 * (blocks - step * 4))) - 1;
-                c = (c & in) | (0x7f7f7f7fu & ~in);
-            }
+            wait_loads_and_barrier<0>();
         }
-    };
-    auto put = [&](int buffer) {
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const int r = (tid + i * kThreads) / 4;
-            values[buffer][r * 4 + (vb ^ (r / 4 & 3))] = v[i];
+        read(0, 0);
+        int s = 0;
+        for (; s + 1 < whole; ++s) {
+            product(s, 0, true);
+            product(s, 1, true);
         }
-        if (tid < kRows) {
-            uint8_t* to = reinterpret_cast<uint8_t*>(&codes[buffer][tid / 64][tid % 16]) + tid / 16 % 4;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) to[i * 64] = (uint8_t)(c >> (8 * i));
-        }
-    };
-    float4_t acc[WN][WT] = {};
-    const int steps = (blocks + 3) / 4;
-    fetch(0);
-    put(0);
-    __syncthreads();
-    for (int s = 0; s < steps; ++s) {
-        const int buffer = s & 1;
-        if (s + 1 < steps) fetch(s + 1);
-        int8v_t af[WT];
-        int ac[WT / 4];
-#pragma unroll
-        for (int j = 0; j < WT; ++j) {
-            const uint4_t q = values[buffer][(kN + (wt + j) * 16 + row) * 4 + (group ^ (row / 4))];
-            af[j] = int8v_t{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int j = 0; j < WT / 4; ++j) ac[j] = (int)codes[buffer][kN / 64 + wt / 4 + j][lane];
-#define PIMHIP_MX_PRODUCT(I, J) \
-    acc[i4 + I][j4 * 4 + J] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[I], af[j4 * 4 + J], acc[i4 + I][j4 * 4 + J], 4, 4, I, bc, J, ac[j4]);
-#define PIMHIP_MX_ROW(I) PIMHIP_MX_PRODUCT(I, 0) PIMHIP_MX_PRODUCT(I, 1) PIMHIP_MX_PRODUCT(I, 2) PIMHIP_MX_PRODUCT(I, 3)
-#pragma unroll
-        for (int i4 = 0; i4 < WN; i4 += 4) {
-            int8v_t bf[4];
-            const int bc = (int)codes[buffer][(wn + i4) / 4][lane];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint4_t q = values[buffer][((wn + i4 + i) * 16 + row) * 4 + (group ^ (row / 4))];
-                bf[i] = int8v_t{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0};
-            }
-#pragma unroll
-            for (int j4 = 0; j4 < WT / 4; ++j4) {
-                PIMHIP_MX_ROW(0)
-                PIMHIP_MX_ROW(1)
-                PIMHIP_MX_ROW(2)
-                PIMHIP_MX_ROW(3)
-            }
-        }
-#undef PIMHIP_MX_ROW
-#undef PIMHIP_MX_PRODUCT
-        if (s + 1 < steps) put(buffer ^ 1);
+        product(s, 0, true);
+        product(s, 1, false);
         __syncthreads();
     }
+    if (blocks % 8 != 0) {
+        // The step that K ends in, by way of registers: behind the end zeros, and any code but "not a number".
+        const int left = blocks - whole * 8;
 #pragma unroll
-    for (int i = 0; i < WN; ++i) {
-        const int64_t n = n0 + (wn + i) * 16 + group * 4;
-        if (n >= b.rows) continue;
+        for (int i = 0; i < kPieces; ++i) {
+            uint4_t q = {0, 0, 0, 0};
+            if (((lane & 7) ^ turned(i * 8 + lane / 8)) < left) q = *reinterpret_cast<const uint4_t*>(vp + (int64_t)whole * (8 * kMxBlockBytes) + v_at[i]);
+            *reinterpret_cast<uint4_t*>(lds + (wave * kPieces + i) * 1024 + lane * 16) = q;
+        }
+        const uint64_t in = ((uint64_t)1 << (8 * left)) - 1;
+        *reinterpret_cast<uint64_t*>(lds + 2 * kBuffer + wave * 1024 + lane * 16) =
+            (*reinterpret_cast<const uint64_t*>(cp + whole * 8 + c_at) & in) | (0x7f7f7f7f7f7f7f7full & ~in);
+        __syncthreads();
+        read(0, 0);
+        product(0, 0, true);
+        product(0, 1, false);
+    }
+
+    const int64_t n = n0 + wn + group * 8, t_row = t0 + wt + row;
+    typename O::elem* to = out + t_row * ld_out + n;
+    if (n0 + kTile <= b.rows && t0 + kTile <= a.rows) {
 #pragma unroll
-        for (int j = 0; j < WT; ++j) {
-            const int64_t t = t0 + (wt + j) * 16 + row;
-            if (t < a.rows) store4<O>(out + t * ld_out + n, acc[i][j], b.rows - n < 4 ? (int)(b.rows - n) : 4);
+        for (int j = 0; j < 4; ++j, to += 16 * ld_out)
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) store8<O>(to + i * 16, acc[i][j], acc[i + 1][j]);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j, to += 16 * ld_out) {
+        if (t_row + j * 16 >= a.rows) continue;
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const int64_t left = b.rows - n - i * 16;
+            if (left >= 8) {
+                store8<O>(to + i * 16, acc[i][j], acc[i + 1][j]);
+            } else if (left > 0) {
+                store4<O>(to + i * 16, acc[i][j], (int)left);
+                store4<O>(to + i * 16 + 4, acc[i + 1][j], (int)left - 4);
+            }
         }
     }
 }

@@ -174,6 +174,17 @@ def test_matmul(ops, M, N, K, dtype):
     check_product(ops.mx4_matmul(a, b, dtype), a.dequantize(torch.float32).cpu(), b.dequantize(torch.float32).cpu(), None, False)
 
 
+# Many tiles: more bands of tokens than one, steps of k that begin in the middle and go round, K that ends in every part of a step.
+@pytest.mark.parametrize("M,N,K", [(1180, 1050, 96), (300, 520, 1536), (257, 129, 2080), (65, 136, 1400), (640, 127, 512), (129, 260, 250), (70, 1029, 800)])
+def test_products_of_many_tiles(ops, M, N, K):
+    g = torch.Generator().manual_seed(M + N + K)
+    x = torch.randn(M, K, generator=g).to(torch.bfloat16)
+    a, b = ops.mx4_quantize(x.to(DEV)), ops.mx4_quantize(weight(N + 2, N, K).to(DEV))
+    w = b.dequantize(torch.float32).cpu()
+    check_product(ops.mx4_matmul(a, b, torch.float32), a.dequantize(torch.float32).cpu(), w, None, False)
+    check_product(ops.mx4_linear(x.to(DEV), b), x, w, None, False)
+
+
 @pytest.mark.parametrize("M", [1, 40, 200])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_linear_with_scales_far_apart_and_far_from_one(ops, M, dtype):
