@@ -77,12 +77,19 @@ int linear(void* out, int64_t ld_out, const void* x, int64_t ld_x, int64_t M, co
     }
     if (M <= 32) return tiles16 < 512 ? go(linear_skinny<T, false, 1, 2, 1, 4>) : go(linear_skinny<T, false, 4, 2, 1, 4>);
     if (M <= 64) return tiles16 < 512 ? go(linear_skinny<T, false, 1, 4, 1, 4>) : go(linear_skinny<T, false, 4, 4, 1, 4>);
-    const int64_t tiles = ((w.rows + 127) / 128) * ((M + 127) / 128);
-    const int rc = check_grid(tiles, 1);
-    if (rc != PIMHIP_OK) return rc;
-    mx4_linear_tile_kernel<T, 4, 4, 2, 2><<<dim3((unsigned)tiles), 256, 0, s>>>((const typename T::elem*)x, w, (const typename T::elem*)bias,
-                                                                               (typename T::elem*)out, ld_x, ld_out, M, relu);
-    return PIMHIP_OK;
+    // Large tiles read operands less often, small ones fill the card.  Measured, 256 x 128 / 128 x 64, in us: 4096 x 16384 x 4096 532 / 634,
+    // 2048 x 4096 x 4096 (256 large tiles) 70 / 86, 1500 x 4608 x 4096 (216) 68 / 84, 1500 x 4096 x 4096 (192) 68 / 65, 200 x 16384 x 4096 (128)
+    // 67 / 48, 512 x 4096 x 4096 (64) 67 / 34.  Up to 64 tokens the kernel of few tokens is faster: 64 x 16384 x 4096 22 (tiles 35), 40 x 4096 x
+    // 4096 13 (34).
+    auto tiled = [&](auto kernel, int rows, int tokens, int threads) {
+        const int64_t tiles = ((w.rows + rows - 1) / rows) * ((M + tokens - 1) / tokens);
+        const int rc = check_grid(tiles, 1);
+        if (rc != PIMHIP_OK) return rc;
+        kernel<<<dim3((unsigned)tiles), threads, 0, s>>>((const typename T::elem*)x, w, (const typename T::elem*)bias, (typename T::elem*)out, ld_x, ld_out, M, relu);
+        return (int)PIMHIP_OK;
+    };
+    if (((w.rows + 255) / 256) * ((M + 127) / 128) > 192) return tiled(mx4_linear_tile_kernel<T, 4, 4, 4, 2>, 256, 128, 512);
+    return tiled(mx4_linear_tile_kernel<T, 4, 2, 2, 2>, 128, 64, 256);
 }
 
 template <class O>

@@ -1,9 +1,4 @@
 // Products of many tokens with 4-bit weights: tiles of the result, operands through LDS.
-//
-// A block has 16 GN WN rows of weights and 16 GT WT tokens, a wavefront of its GN x GT ones WN x WT tiles of 16 x 16.  The next
-// step's operands are on their way to registers while the matrix cores work on this one's in LDS (two buffers, one barrier a step).
-// Loads take whole runs of a row (16 lanes in 16 rows would be 16 requests), and a row's 16-byte chunks lie in LDS in an order that
-// spreads what 8 lanes read or write over all banks.
 #pragma once
 
 #include "mx4_kernels.h"
@@ -25,9 +20,16 @@ __device__ __forceinline__ void tile_at(int id, int tiles_n, int tiles_t, int64_
 }
 
 // ---- x in 16 bits, weights in 4 ----------------------------------------------------------------------------------------------
-// Steps of 128 values of k.  Weights stay packed in LDS and are converted on the way to the matrix cores: a quarter of the LDS reads of
-// converted ones.  One buffer: the next step's operands wait in registers, and while a block writes them another one of its CU
-// computes.
+// A block has 16 GN WN rows of weights and 16 GT WT tokens, a wavefront of its GN x GT ones WN x WT tiles of 16 x 16.  Steps of 128 values
+// of k.  Weights stay packed in LDS and are converted on the way to the matrix cores: a quarter of the LDS reads of converted ones.  One
+// buffer: the next step's operands wait in registers.  Loads take whole runs of a row (16 lanes in 16 rows would be 16 requests), and a
+// row's 16-byte chunks lie in LDS in an order that spreads what 8 lanes read or write over all banks.
+//
+// 4096 x 16384 x 4096: 532 us, 1.03 PFLOP/s; 1500 x 4096 x 4096: 65 us, 0.77 (this card's library multiplies 16-bit matrices of 8192 at 1.27
+// to 1.5).  A block alone takes 1.9 us a step of 256 x 128 x 128: the matrix cores work 0.9 of it, the conversions, one instruction a
+// product, take issue slots, LDS is busy 0.75.  Measured and not better: two steps in registers (the same; three: spills), two buffers
+// (512, but 1500 tokens 73), 128 rows and tokens and four wavefronts (565), 32 x 128 results a wavefront, half the conversions but twice
+// the reads (570), products, reads and conversions told to take turns (594).
 template <class T, int WN, int WT, int GN, int GT>
 __global__ __launch_bounds__(64 * GN * GT) void mx4_linear_tile_kernel(const typename T::elem* x, Mx4View w, const typename T::elem* bias, typename T::elem* out,
                                                                        int64_t ld_x, int64_t ld_out, int64_t M, int relu)
