@@ -1,0 +1,99 @@
+"""The operators of a decoding step in a row, as a server runs them: a 4-bit layer, the experts, the vocabulary in 4 bits, and what the logits say."""
+import pytest
+import torch
+from test_log_probs_gpu import near, reference
+from test_moe_layer_gpu import Layer
+from test_mx4_gpu import check_product
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+class Step:
+    def __init__(self, ops, dtype, D=256, F=320, V=4099):
+        g = torch.Generator().manual_seed(D + V)
+        self.ops, self.D, self.dtype = ops, D, dtype
+        self.bias = torch.randn(D, generator=g).to(dtype)
+        self.layer = ops.mx4_quantize((torch.randn(D, D, generator=g) * D**-0.5).to(DEV))
+        self.head = ops.mx4_quantize((torch.randn(V, D, generator=g) * D**-0.5).to(DEV))
+        self.moe = Layer(ops, 5, 8, 2, D, F, dtype, act="aten::silu", gated=True, mx4=True)
+        self.dev_bias = self.bias.to(DEV)
+        self.x = lambda M, s: torch.randn(M, D, generator=torch.Generator().manual_seed(M + s)).to(dtype)
+
+    def __call__(self, x, tokens):
+        h = self.ops.mx4_linear(x, self.layer, self.dev_bias, "aten::relu")
+        y, experts, shares = self.moe.plan.forward(h)
+        logits = self.ops.mx4_linear(y, self.head)
+        return (h, y, experts, shares, logits, *self.ops.token_log_probs(logits, tokens, top=5))
+
+    def check(self, x, tokens, out):
+        """Each operator against 64 bits on what the one before wrote."""
+        h, y, experts, shares, logits, logp, entropy, top_logp, top_ids = (t.cpu() for t in out)
+        check_product(h, x, self.layer.dequantize(torch.float32).cpu(), self.bias, True)
+        self.moe.check(h, (y, experts, shares))
+        check_product(logits, y, self.head.dequantize(torch.float32).cpu(), None, False)
+        want_logp, want_entropy, order, want_top = reference(logits, tokens, 5)
+        near(logp, want_logp)
+        near(entropy, want_entropy)
+        assert torch.equal(top_ids.long(), order)
+        near(top_logp, want_top)
+
+
+@pytest.mark.parametrize("M", [1, 13, 70])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_decoding_step(ops, dtype, M):
+    step = Step(ops, dtype)
+    tokens = (torch.arange(M) * 37) % 4099
+    x, dev_tokens = step.x(M, 0).to(DEV), tokens.to(DEV)
+    step.check(x.cpu(), tokens, step(x, dev_tokens))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, dev_tokens)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = step(x, dev_tokens)
+    torch.cuda.synchronize()
+    for s in range(1, 5):
+        x.copy_(step.x(M, s))
+        eager = step(x, dev_tokens)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, eager))
+    step.check(x.cpu(), tokens, out)
+
+
+def test_the_calls_without_the_extension_give_the_same(ops, monkeypatch):
+    from pimaicompiler_amd import ops as module
+    step = Step(ops, torch.float16)
+    tokens = torch.tensor([4, -1, 4098], device=DEV)
+    x = step.x(3, 0).to(DEV)
+    made = ops.mx4_quantize(x)
+    first = (*step(x, tokens), made.packed, made.scales[:, :8], made.tops, ops.mx4_dequantize(made, torch.float32), ops.mx4_matmul(made, step.layer))
+    monkeypatch.setattr(module, "_native_module", module._WithoutExtension())
+    made = ops.mx4_quantize(x)
+    again = (*step(x, tokens), made.packed, made.scales[:, :8], made.tops, ops.mx4_dequantize(made, torch.float32), ops.mx4_matmul(made, step.layer))
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def test_two_streams_at_a_time(ops):
+    """One plan, one set of weights, two streams: each has its own workspace."""
+    step = Step(ops, torch.bfloat16)
+    tokens = [torch.arange(M, device=DEV) for M in (9, 33)]
+    xs = [step.x(t.numel(), 3).to(DEV) for t in tokens]
+    want = [step(x, t) for x, t in zip(xs, tokens)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got.append((i, step(xs[i], tokens[i])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for i, out in got for a, b in zip(out, want[i]))
+
+
+def test_nothing_to_do(ops):
+    step = Step(ops, torch.float16)
+    out = step(torch.empty(0, step.D, dtype=torch.float16, device=DEV), torch.empty(0, dtype=torch.int64, device=DEV))
+    assert out[0].shape == (0, 256) and out[2].shape == (0, 2) and out[4].shape == (0, 4099) and out[5].shape == (0,) and out[8].shape == (0, 5)
