@@ -32,7 +32,7 @@ struct MoeLayerArgs {
     float* share;     // [tokens][top_k]
     void* h;          // [pairs][d_ff]: hidden values, rounded to x's type as operands of the matrix cores
     float* part;      // [pairs][d_model]
-    unsigned int* counters;  // blocks of the second product that are done with a tile of rows
+    unsigned int* counters;  // pairs whose second product is done, for each tile of rows
     int counters_used;
     int tokens, E, top_k, d_model, d_ff, ld_x;
     int ld_s1, ld_s2;  // pitches of 4-bit weights' scale codes
@@ -136,17 +136,27 @@ __global__ __launch_bounds__(kRouterThreads) void moe_layer_router_kernel(MoeLay
 }
 
 // ---- the experts' products ---------------------------------------------------------------------------------------------------
-// The pairs (token * top_k + choice) that chose expert e, in their order; every thread returns how many.
+// The pairs (token * top_k + choice) that chose expert e, in their order; every thread returns how many.  The first wavefront looks, four
+// loads at a time.
 __device__ __forceinline__ int pairs_of(const int* chosen, int pairs, int e, short* list, int* count)
 {
     if (threadIdx.x < 64) {
         int n = 0;
-        for (int base = 0; base < pairs; base += 64) {
-            const int p = base + (int)threadIdx.x;
-            const bool is = p < pairs && chosen[p] == e;
-            const unsigned long long all = __ballot(is);
-            if (is) list[n + __popcll(all & ((1ull << threadIdx.x) - 1))] = (short)p;
-            n += __popcll(all);
+        for (int base = 0; base < pairs; base += 256) {
+            int c[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int p = base + i * 64 + (int)threadIdx.x;
+                c[i] = chosen[p < pairs ? p : pairs - 1];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int p = base + i * 64 + (int)threadIdx.x;
+                const bool is = p < pairs && c[i] == e;
+                const unsigned long long all = __ballot(is);
+                if (is) list[n + __popcll(all & ((1ull << threadIdx.x) - 1))] = (short)p;
+                n += __popcll(all);
+            }
         }
         if (threadIdx.x == 0) *count = n;
     }
@@ -269,7 +279,7 @@ __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPoi
 
 // Block (x, y, z): rows x of expert y for its pairs 16 z .. 16 z + 15; those of more than 16 pairs read the weights again, out of the
 // caches.  (A loop over pairs in one block instead costs so many registers that half the wavefronts fit: 39 us against 25 for 64 tokens
-// through 8 gated 4-bit experts 1024 -> 4096.)
+// through 8 gated 4-bit experts 1024 -> 4096, then.)
 template <class T, bool MX, bool SHARED, bool GATED, int F, int WK>
 __global__ __launch_bounds__(64 * WK, F > 2 || (GATED && F > 1) ? 3 : 4) void moe_layer_first_kernel(MoeLayerArgs a)
 {
@@ -307,7 +317,7 @@ __device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPo
     __syncthreads();
 }
 
-// Blocks as above.  The one that is last to finish a tile of rows, of all experts' blocks, makes the weighted sum there, in the order of the choice.
+// Blocks as above.  The one whose pairs are the last of a tile of rows makes the weighted sum there, in the order of the choice.
 // An expert without a share adds nothing, whatever it computed.  Sums of other blocks come from other XCDs: they were stored past the L2s and
 // are loaded past them, and each block waits for its stores before it counts itself.
 template <class T, bool MX, bool SHARED, int RT, int WK>
@@ -317,27 +327,37 @@ __global__ __launch_bounds__(64 * WK, 4) void moe_layer_second_kernel(MoeLayerAr
     __shared__ unsigned int before;
     extern __shared__ uint4_t xs[];
     const ExpertPointers p = a.experts[blockIdx.y];
-    const int first = blockIdx.z * 16, n = pairs_of(a.chosen, a.tokens * a.top_k, blockIdx.y, lds.list, &lds.count) - first;
-    if (n > 0) moe_second<T, MX, SHARED, RT, WK>(a, p, lds.list + first, n < 16 ? n : 16, xs, lds.turn);
+    const int first = blockIdx.z * 16, left = pairs_of(a.chosen, a.tokens * a.top_k, blockIdx.y, lds.list, &lds.count) - first;
+    if (left <= 0) return;
+    const int n = left < 16 ? left : 16;
+    moe_second<T, MX, SHARED, RT, WK>(a, p, lds.list + first, n, xs, lds.turn);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (threadIdx.x == 0) before = __hip_atomic_fetch_add(&a.counters[blockIdx.x], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (threadIdx.x == 0) before = __hip_atomic_fetch_add(&a.counters[blockIdx.x], (unsigned int)n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    if (before != gridDim.y * gridDim.z - 1) return;
-    constexpr int kWords = 16 * RT / 4;  // of four rows
-    for (int i = threadIdx.x; i < a.tokens * kWords; i += 64 * WK) {
-        const int token = i / kWords, d = blockIdx.x * (16 * RT) + i % kWords * 4;
-        if (d >= a.d_model) continue;
-        float4_t y = {};
-        for (int j = 0; j < a.top_k; ++j) {
-            const float c = a.share[token * a.top_k + j];
-            if (c == 0.0f) continue;
+    if (before + n != (unsigned int)(a.tokens * a.top_k)) return;
+    // A thread has one choice of four rows of a token, so that what comes past the L2s comes at once; the first ones of each sum up.
+    constexpr int kWords = 16 * RT / 4;
+    float4_t* parts = reinterpret_cast<float4_t*>(lds.turn);
+    const int at_once = 64 * WK / a.top_k, mine = threadIdx.x / a.top_k, choice = threadIdx.x % a.top_k;
+    for (int i0 = 0; i0 < a.tokens * kWords; i0 += at_once) {
+        const int i = i0 + mine, token = i / kWords, d = blockIdx.x * (16 * RT) + i % kWords * 4;
+        const bool is = mine < at_once && i < a.tokens * kWords && d < a.d_model;
+        if (is) {
+            const int pair = token * a.top_k + choice;
+            const float c = a.share[pair];
             unsigned long long lo, hi;
-            load16_device_scope(a.part + (int64_t)(token * a.top_k + j) * a.d_model + d, lo, hi);
+            load16_device_scope(a.part + (int64_t)pair * a.d_model + d, lo, hi);
             const uint4_t q = {(unsigned int)lo, (unsigned int)(lo >> 32), (unsigned int)hi, (unsigned int)(hi >> 32)};
-            y += c * __builtin_bit_cast(float4_t, q);
+            parts[threadIdx.x] = c == 0.0f ? float4_t{} : c * __builtin_bit_cast(float4_t, q);
         }
-        store4<T>((typename T::elem*)a.y + (int64_t)token * a.d_model + d, y, 4);
+        __syncthreads();
+        if (is && choice == 0) {
+            float4_t y = parts[threadIdx.x];
+            for (int j = 1; j < a.top_k; ++j) y += parts[threadIdx.x + j];
+            store4<T>((typename T::elem*)a.y + (int64_t)token * a.d_model + d, y, 4);
+        }
+        __syncthreads();
     }
 }
 }  // namespace pimhip
