@@ -102,9 +102,15 @@ int matmul(void* out, int64_t ld_out, const Mx4View& a, const Mx4View& b, hipStr
         kernel<<<dim3((unsigned)gx, (unsigned)gy), 64 * WK, 0, s>>>(a, b, (typename O::elem*)out, ld_out);
         return (int)PIMHIP_OK;
     };
-    if (a.rows <= 16) return run(mx4_matmul_skinny_kernel<O, 1, 1, 4>, 1, 1, 4);
-    if (a.rows <= 64) return run(mx4_matmul_skinny_kernel<O, 1, 4, 4>, 1, 4, 4);
-    const int64_t tiles = ((b.rows + 127) / 128) * ((a.rows + 127) / 128);
+    // Few rows of a: blocks of 16 to 64 rows of b whose wavefronts share k.  More rows read a less often, fewer make more blocks.  Measured, in us:
+    //   16 x 16384 x 4096   16 rows 16.8, 64 rows 12.4      16 x 4096 x 4096   16 rows 5.9, 64 rows 11.4      1 x 4096 x 16384   16 rows 15.1, 64 rows 34
+    // From 17 rows of a on, tiles of 128 x 128 (below) where b has 96 of them, else 32 rows of a a block:
+    //   32 x 16384 x 4096   tiles 17.7, blocks 18.0      64 x 16384 x 4096   18.0 / 31.2      48 x 8192 x 1024 (64 tiles)   5.7 / 6.0      64 x 4096 x 4096   14.1 / 9.7
+    if (a.rows <= 16)
+        return (b.rows + 15) / 16 >= 1024 ? run(mx4_matmul_skinny_kernel<O, 4, 1, 8>, 4, 1, 8) : run(mx4_matmul_skinny_kernel<O, 1, 1, 8>, 1, 1, 8);
+    const int64_t columns = (b.rows + 127) / 128;
+    if (a.rows <= 64 && columns < 96) return a.rows <= 32 ? run(mx4_matmul_skinny_kernel<O, 1, 2, 8>, 1, 2, 8) : run(mx4_matmul_skinny_kernel<O, 2, 2, 8>, 2, 2, 8);
+    const int64_t tiles = columns * ((a.rows + 127) / 128);
     const int rc = check_grid(tiles, 1);
     if (rc != PIMHIP_OK) return rc;
     mx4_matmul_tile_kernel<O><<<dim3((unsigned)tiles), 256, 0, s>>>(a, b, (typename O::elem*)out, ld_out);
