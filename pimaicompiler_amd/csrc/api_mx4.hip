@@ -63,6 +63,9 @@ int linear(void* out, int64_t ld_out, const void* x, int64_t ld_x, int64_t M, co
     // the opposite.  Measured on 16384 x 4096 / 4096 x 4096 / 31999 x 1024, weights that no cache holds, in us:
     //   one token (staged in LDS)   1 tile of 16 rows, 8 wavefronts 10.5 / 4.9 / -      2 tiles, 8: 8.7 / 5.9 / -     (turned by the wavefronts: 12.0 / 5.6)
     //   16 tokens                   1 tile, 8: 16.1 / 6.3 / 12.9      4 tiles, 8: 10.7 / 9.3 / 10.5      4 tiles, 4: 11.3 / 10.4 / 7.3
+    //   32 tokens                   1 tile, 8: 24.1 / 8.6 / 17.4      4 tiles, 8: 16.1 / 14.6 / 12.8     4 tiles, 4: 16.8 / 15.7 / 10.0
+    //   64 tokens, 32 a block       2 tiles, 8: 36.2 / 9.7 / 28.0     4 tiles, 8: 30.7 / - / -           4 tiles, 4: 27.1 / 15.3 / 19.2
+    //   64 tokens, 64 a block       1 tile, 8: 45.3 / 12.5 / 39.9     2 tiles, 8: 28.5 / 14.3 / 25.7     4 tiles, 4: 23.9 / 22.2 / 20.6
     constexpr int64_t kShared = 32 << 10;
     const int64_t tiles16 = (w.rows + 15) / 16;
     const bool long_rows = w.cols > 4 * Mx4Weights<T, 2>::kUnit;
@@ -75,8 +78,11 @@ int linear(void* out, int64_t ld_out, const void* x, int64_t ld_x, int64_t M, co
         if (tiles16 < 512) return long_rows ? go(linear_skinny<T, false, 1, 1, 1, 8>) : go(linear_skinny<T, false, 1, 1, 1, 4>);
         return long_rows ? go(linear_skinny<T, false, 4, 1, 1, 8>) : go(linear_skinny<T, false, 4, 1, 1, 4>);
     }
-    if (M <= 32) return tiles16 < 512 ? go(linear_skinny<T, false, 1, 2, 1, 4>) : go(linear_skinny<T, false, 4, 2, 1, 4>);
-    if (M <= 64) return tiles16 < 512 ? go(linear_skinny<T, false, 1, 4, 1, 4>) : go(linear_skinny<T, false, 4, 4, 1, 4>);
+    if (M <= 64) {
+        if (tiles16 <= 512) return M <= 32 ? go(linear_skinny<T, false, 1, 2, 1, 8>) : go(linear_skinny<T, false, 2, 2, 1, 8>);
+        if (!long_rows) return go(linear_skinny<T, false, 4, 2, 1, 4>);
+        return M <= 32 ? go(linear_skinny<T, false, 4, 2, 1, 8>) : go(linear_skinny<T, false, 4, 4, 1, 4>);
+    }
     // Large tiles read operands less often, small ones fill the card.  Measured, 256 x 128 / 128 x 64, in us: 4096 x 16384 x 4096 532 / 634,
     // 2048 x 4096 x 4096 (256 large tiles) 70 / 86, 1500 x 4608 x 4096 (216) 68 / 84, 1500 x 4096 x 4096 (192) 68 / 65, 200 x 16384 x 4096 (128)
     // 67 / 48, 512 x 4096 x 4096 (64) 67 / 34.  Up to 64 tokens the kernel of few tokens is faster: 64 x 16384 x 4096 22 (tiles 35), 40 x 4096 x
