@@ -14,6 +14,8 @@ extern "C" int pimhip_token_log_probs(const void* logits, int dtype, int64_t ld,
         return fail(PIMHIP_ERR_INVALID_ARGUMENT, "rows=%lld, vocab=%lld", (long long)rows, (long long)vocab);
     if (dtype != PIMHIP_F16 && dtype != PIMHIP_BF16 && dtype != PIMHIP_F32) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "dtype=%d", dtype);
     if (top < 0 || top > kTopMost || top > vocab) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "top=%d not in [0, min(%d, vocab)]", top, kTopMost);
+    const int threads = vocab <= 1024 ? 64 : vocab <= 8192 ? 256 : 1024;
+    if (rows * threads > UINT32_MAX) return fail(PIMHIP_ERR_UNSUPPORTED, "%lld rows are too many for one launch", (long long)rows);
     if (rows == 0) return PIMHIP_OK;
     if (!logits || (rows > 1 && ld < vocab)) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "logits is null, or ld=%lld is less than vocab=%lld", (long long)ld, (long long)vocab);
     if (reinterpret_cast<uintptr_t>(logits) & (dtype == PIMHIP_F32 ? 3u : 1u)) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "logits is not aligned to its elements");
@@ -23,9 +25,9 @@ extern "C" int pimhip_token_log_probs(const void* logits, int dtype, int64_t ld,
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto run = [&](auto type) {
         typedef decltype(type) T;
-        if (vocab <= 1024)
+        if (threads == 64)
             token_log_probs_kernel<T, 64><<<dim3((unsigned)rows), 64, 0, s>>>(a);
-        else if (vocab <= 8192)
+        else if (threads == 256)
             token_log_probs_kernel<T, 256><<<dim3((unsigned)rows), 256, 0, s>>>(a);
         else
             token_log_probs_kernel<T, 1024><<<dim3((unsigned)rows), 1024, 0, s>>>(a);

@@ -25,6 +25,20 @@ size_t part_bytes(const PimHipMoeLayerPlan* p, int tokens) { return round256((si
 
 size_t counter_bytes(const PimHipMoeLayerPlan* p) { return (size_t)(p->d_model + 15) / 16 * sizeof(unsigned int); }
 
+bool known_locked(const PimHipMoeLayerPlan* plan)
+{
+    for (const PimHipMoeLayerPlan* q : g_moe_layer_plans)
+        if (q == plan) return true;
+    return false;
+}
+
+// A plan that shutting the library down, or its owner, has destroyed is refused.
+int check_plan(const PimHipMoeLayerPlan* plan)
+{
+    std::lock_guard<std::mutex> lock(g_mutex);
+    return known_locked(plan) ? (int)PIMHIP_OK : fail(PIMHIP_ERR_INVALID_ARGUMENT, "unknown or already destroyed expert layer plan");
+}
+
 int destroy_moe_layer_plan_locked(PimHipMoeLayerPlan* plan)
 {
     if (!plan) return PIMHIP_OK;
@@ -127,9 +141,9 @@ extern "C" int pimhip_moe_layer_plan_create(PimHipMoeLayerPlan** plan_out, const
         return fail(PIMHIP_ERR_INVALID_ARGUMENT, "either w1 and w2 or w1_mx4 and w2_mx4 must be non-null");
     if (!aligned16(d->router_w)) return fail(PIMHIP_ERR_UNSUPPORTED, "router_w must be 16-byte aligned");
     const int64_t rows1 = d->gated ? 2 * d->d_ff : d->d_ff;
-    std::vector<ExpertPointers> table((size_t)d->num_experts);
+    ExpertPointers table[kMoeLayerExperts];
     for (int e = 0; e < d->num_experts; ++e) {
-        ExpertPointers& p = table[(size_t)e];
+        ExpertPointers& p = table[e];
         memset(&p, 0, sizeof(p));
         if (mx) {
             const PimHipMx4Matrix *m1 = d->w1_mx4 + e, *m2 = d->w2_mx4 + e;
@@ -138,7 +152,7 @@ extern "C" int pimhip_moe_layer_plan_create(PimHipMoeLayerPlan** plan_out, const
                             (long long)d->d_model, (long long)d->d_ff);
             for (const PimHipMx4Matrix* m : {m1, m2}) {
                 if (!m->packed || !m->scales || !m->tops || !aligned16(m->packed) || !aligned16(m->scales) || (m->ld_scales & 15) ||
-                    m->ld_scales * 32 < m->cols || m->ld_scales != (m == m1 ? d->w1_mx4 : d->w2_mx4)->ld_scales)
+                    m->ld_scales < (m->cols + 31) / 32 || m->ld_scales > INT32_MAX / 16 || m->ld_scales != (m == m1 ? d->w1_mx4 : d->w2_mx4)->ld_scales)
                     return fail(PIMHIP_ERR_INVALID_ARGUMENT, "expert %d: a 4-bit matrix is null, not 16-byte aligned, or has another pitch of scales", e);
             }
             p.w1 = m1->packed, p.s1 = m1->scales, p.t1 = m1->tops;
@@ -162,16 +176,21 @@ extern "C" int pimhip_moe_layer_plan_create(PimHipMoeLayerPlan** plan_out, const
     plan->dtype = d->dtype, plan->act = d->act, plan->gated = d->gated ? 1 : 0, plan->renormalize = d->renormalize ? 1 : 0, plan->mx4 = mx;
     plan->ld_s1 = mx ? d->w1_mx4->ld_scales : 0, plan->ld_s2 = mx ? d->w2_mx4->ld_scales : 0;
     plan->router_w = d->router_w, plan->router_b = d->router_b;
-    const size_t bytes = table.size() * sizeof(ExpertPointers);
+    const size_t bytes = (size_t)d->num_experts * sizeof(ExpertPointers);
     hipError_t err = hipMalloc(reinterpret_cast<void**>(&plan->experts), bytes);
-    if (err == hipSuccess) err = hipMemcpyAsync(plan->experts, table.data(), bytes, hipMemcpyHostToDevice, s);
+    if (err == hipSuccess) err = hipMemcpyAsync(plan->experts, table, bytes, hipMemcpyHostToDevice, s);
     if (err == hipSuccess) err = hipStreamSynchronize(s);  // (table goes out of scope)
     std::lock_guard<std::mutex> lock(g_mutex);
     if (err != hipSuccess) {
         destroy_moe_layer_plan_locked(plan);
         return fail(PIMHIP_ERR_HIP, "the table of experts could not be set up: %s", hipGetErrorString(err));
     }
-    g_moe_layer_plans.push_back(plan);
+    try {
+        g_moe_layer_plans.push_back(plan);
+    } catch (...) {
+        destroy_moe_layer_plan_locked(plan);
+        return fail(PIMHIP_ERR_HIP, "out of host memory");
+    }
     *plan_out = plan;
     return PIMHIP_OK;
 }
@@ -180,15 +199,15 @@ extern "C" int pimhip_moe_layer_plan_destroy(PimHipMoeLayerPlan* plan)
 {
     if (!plan) return PIMHIP_OK;
     std::lock_guard<std::mutex> lock(g_mutex);
-    bool known = false;
-    for (PimHipMoeLayerPlan* q : g_moe_layer_plans) known = known || (q == plan);
-    if (!known) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "unknown or already destroyed expert layer plan");
+    if (!known_locked(plan)) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "unknown or already destroyed expert layer plan");
     return destroy_moe_layer_plan_locked(plan);
 }
 
 extern "C" int pimhip_moe_layer_workspace_bytes(const PimHipMoeLayerPlan* plan, int tokens, uint64_t* bytes)
 {
     if (!plan || !bytes) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "plan and bytes must be non-null");
+    const int rc = check_plan(plan);
+    if (rc != PIMHIP_OK) return rc;
     if (tokens < 0 || tokens > kMoeLayerTokens) return fail(PIMHIP_ERR_UNSUPPORTED, "tokens=%d not in [0, %d]", tokens, kMoeLayerTokens);
     *bytes = hidden_bytes(plan, tokens) + part_bytes(plan, tokens) + counter_bytes(plan);
     return PIMHIP_OK;
@@ -201,6 +220,7 @@ extern "C" int pimhip_moe_layer_forward(PimHipMoeLayerPlan* plan, const void* x,
     int rc = current_device_state(&st);
     if (rc != PIMHIP_OK) return rc;
     if (!plan) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "plan is null");
+    if ((rc = check_plan(plan)) != PIMHIP_OK) return rc;
     int dev = -1;
     PIMHIP_HIP_CHECK(hipGetDevice(&dev));
     if (dev != plan->device) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "plan belongs to device %d, current device is %d", plan->device, dev);

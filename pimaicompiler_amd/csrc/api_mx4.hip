@@ -31,10 +31,11 @@ int check_element(const char* name, const void* p, int dtype, bool fp32_too)
     return PIMHIP_OK;
 }
 
-// The two-dimensional grid of a product: row groups by token groups.
-int check_grid(int64_t x, int64_t y)
+// A launch's workgroups, and its threads, which are counted in 32 bits along x.
+int check_grid(int64_t x, int64_t y, int threads)
 {
-    if (x > INT32_MAX || y > 65535) return fail(PIMHIP_ERR_UNSUPPORTED, "the product is too large for one launch (%lld x %lld workgroups)", (long long)x, (long long)y);
+    if (x > INT32_MAX || x * threads > UINT32_MAX || y > 65535)
+        return fail(PIMHIP_ERR_UNSUPPORTED, "too large for one launch (%lld x %lld workgroups of %d threads)", (long long)x, (long long)y, threads);
     return PIMHIP_OK;
 }
 
@@ -49,7 +50,7 @@ template <class T, bool SHARED, int RT, int TT, int U, int WK>
 int linear_skinny(void* out, int64_t ld_out, const void* x, int64_t ld_x, int64_t M, const Mx4View& w, const void* bias, int relu, hipStream_t s)
 {
     const int64_t gx = (w.rows + 16 * RT - 1) / (16 * RT), gy = (M + 16 * TT - 1) / (16 * TT);
-    const int rc = check_grid(gx, gy);
+    const int rc = check_grid(gx, gy, 64 * WK);
     if (rc != PIMHIP_OK) return rc;
     mx4_linear_skinny_kernel<T, SHARED, RT, TT, U, WK><<<dim3((unsigned)gx, (unsigned)gy), 64 * WK, SHARED ? shared_tokens_bytes<T>(M, w.cols) : 0, s>>>(
         (const typename T::elem*)x, w, (const typename T::elem*)bias, (typename T::elem*)out, ld_x, ld_out, M, relu);
@@ -89,7 +90,7 @@ int linear(void* out, int64_t ld_out, const void* x, int64_t ld_x, int64_t M, co
     // 4096 13 (34).
     auto tiled = [&](auto kernel, int rows, int tokens, int threads) {
         const int64_t tiles = ((w.rows + rows - 1) / rows) * ((M + tokens - 1) / tokens);
-        const int rc = check_grid(tiles, 1);
+        const int rc = check_grid(tiles, 1, threads);
         if (rc != PIMHIP_OK) return rc;
         kernel<<<dim3((unsigned)tiles), threads, 0, s>>>((const typename T::elem*)x, w, (const typename T::elem*)bias, (typename T::elem*)out, ld_x, ld_out, M, relu);
         return (int)PIMHIP_OK;
@@ -103,7 +104,7 @@ int matmul(void* out, int64_t ld_out, const Mx4View& a, const Mx4View& b, hipStr
 {
     auto run = [&](auto kernel, int RT, int TT, int WK) {
         const int64_t gx = (b.rows + 16 * RT - 1) / (16 * RT), gy = (a.rows + 16 * TT - 1) / (16 * TT);
-        const int rc = check_grid(gx, gy);
+        const int rc = check_grid(gx, gy, 64 * WK);
         if (rc != PIMHIP_OK) return rc;
         kernel<<<dim3((unsigned)gx, (unsigned)gy), 64 * WK, 0, s>>>(a, b, (typename O::elem*)out, ld_out);
         return (int)PIMHIP_OK;
@@ -117,7 +118,7 @@ int matmul(void* out, int64_t ld_out, const Mx4View& a, const Mx4View& b, hipStr
     const int64_t columns = (b.rows + 127) / 128;
     if (a.rows <= 64 && columns < 96) return a.rows <= 32 ? run(mx4_matmul_skinny_kernel<O, 1, 2, 8>, 1, 2, 8) : run(mx4_matmul_skinny_kernel<O, 2, 2, 8>, 2, 2, 8);
     const int64_t tiles = columns * ((a.rows + 127) / 128);
-    const int rc = check_grid(tiles, 1);
+    const int rc = check_grid(tiles, 1, 256);
     if (rc != PIMHIP_OK) return rc;
     mx4_matmul_tile_kernel<O><<<dim3((unsigned)tiles), 256, 0, s>>>(a, b, (typename O::elem*)out, ld_out);
     return PIMHIP_OK;
@@ -137,7 +138,7 @@ extern "C" int pimhip_mx4_quantize(const PimHipMx4Matrix* out, const void* x, in
     // A row of up to 1024 values is one wavefront's (at most two rounds of 512), a longer one a block's.
     const bool short_rows = v.cols <= 1024;
     const int64_t grid = short_rows ? (v.rows + 3) / 4 : v.rows;
-    if ((rc = check_grid(grid, 1)) != PIMHIP_OK) return rc;
+    if ((rc = check_grid(grid, 1, 256)) != PIMHIP_OK) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto run = [&](auto type) {
         typedef decltype(type) T;
@@ -158,7 +159,7 @@ extern "C" int pimhip_mx4_find_tops(const PimHipMx4Matrix* m, void* stream)
     Mx4View v;
     if ((rc = check_matrix("matrix", m, &v)) != PIMHIP_OK) return rc;
     if (v.rows == 0) return PIMHIP_OK;
-    if ((rc = check_grid((v.rows + 3) / 4, 1)) != PIMHIP_OK) return rc;
+    if ((rc = check_grid((v.rows + 3) / 4, 1, 256)) != PIMHIP_OK) return rc;
     mx4_tops_kernel<<<dim3((unsigned)((v.rows + 3) / 4)), 256, 0, static_cast<hipStream_t>(stream)>>>(v.scales, v.ld_scales, v.rows, (v.cols + kMxBlock - 1) / kMxBlock,
                                                                                                      (uint8_t*)m->tops);
     PIMHIP_HIP_CHECK(hipGetLastError());

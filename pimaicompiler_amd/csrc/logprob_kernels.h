@@ -44,8 +44,8 @@ __device__ __forceinline__ void load_piece(const typename T::elem* row, int64_t 
     for (int i = 0; i < 8; ++i) v[i] = (float)e[i];
 }
 
-// The values of a row, eight at a time, those of thread tid being pieces tid, tid + THREADS, ...: f(piece, its values, how many of them
-// there are).  Four pieces are loaded together; behind the row's end they are -inf.
+// The values of a row, eight at a time, those of thread tid being pieces tid, tid + THREADS, ...: f(piece, its values and those of the next
+// three of the thread).  Four pieces are loaded together; behind the row's end, and where there is no piece, they are -inf.
 template <class T, int THREADS, class F>
 __device__ __forceinline__ void each_four_pieces(const typename T::elem* row, int64_t V, F f)
 {
@@ -280,7 +280,7 @@ __global__ __launch_bounds__(THREADS) void token_log_probs_kernel(LogProbArgs a)
                 for (int c = 0; c < 8; ++c) {
                     const int64_t at = (first + h * THREADS) * 8 + c;
                     const unsigned long long q = key_of(v[h][c], (unsigned int)at);
-                    if (at < V && q < below) k = larger(k, q);
+                    if (at < V && q < below && (h == 0 || first + h * THREADS < V / 8)) k = larger(k, q);  // (the others are no pieces of the row)
                 }
         });
         __syncthreads();

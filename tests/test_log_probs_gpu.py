@@ -180,3 +180,10 @@ def test_refusals_on_the_gpu(ops):
                  lambda: ops.token_log_probs(x.clone().requires_grad_(), t)):
         with pytest.raises(ops.NNRuntimeException):
             call()
+
+
+def test_more_rows_than_a_launch_holds_are_refused(ops):
+    from pimaicompiler_amd import _lib as L
+    x = torch.zeros(8, device=DEV)
+    for rows, V in ((1 << 22, 9000), (1 << 24, 2000), (1 << 26, 64)):
+        assert L.load().pimhip_token_log_probs(x.data_ptr(), L.PIMHIP_F32, V, rows, V, None, 0, 0, None, x.data_ptr(), None, None, None) == L.PIMHIP_ERR_UNSUPPORTED

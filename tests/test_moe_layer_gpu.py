@@ -222,3 +222,15 @@ def test_refusals_on_the_gpu(ops):
     n = ctypes.c_uint64()
     assert L.load().pimhip_moe_layer_workspace_bytes(plan._handle, 65, ctypes.byref(n)) == L.PIMHIP_ERR_UNSUPPORTED
     assert L.load().pimhip_moe_layer_forward(plan._handle, None, 64, 1, None, None, None, None, None) == L.PIMHIP_ERR_INVALID_ARGUMENT
+
+
+def test_a_destroyed_plan_is_refused(ops):
+    from pimaicompiler_amd import _lib as L
+    layer = Layer(ops, 3, 4, 2, 64, 32)
+    x = layer.x(2).to(DEV)
+    layer.plan.forward(x)
+    assert L.load().pimhip_moe_layer_plan_destroy(layer.plan._handle) == L.PIMHIP_OK
+    for stream in (None, torch.cuda.Stream()):
+        with pytest.raises(ops.NNRuntimeException):
+            layer.plan.forward(x, stream=stream)
+    assert L.load().pimhip_moe_layer_plan_destroy(layer.plan._handle) == L.PIMHIP_ERR_INVALID_ARGUMENT

@@ -317,3 +317,16 @@ def test_refusals_on_the_gpu(ops):
             call()
     with torch.no_grad():
         ops.mx4_linear(x.clone().requires_grad_(), q)
+
+
+def test_the_c_interface_refuses_what_no_launch_can_hold(ops):
+    from pimaicompiler_amd import _lib as L
+    lib = L.load()
+    q = ops.mx4_quantize(torch.zeros(2, 2048, dtype=torch.float16, device=DEV))
+    at = (q.packed.data_ptr(), q.scales.data_ptr(), q.tops.data_ptr())
+    for rows, cols, ld, want in ((1 << 34, 2048, 64, L.PIMHIP_ERR_UNSUPPORTED), (1 << 36, 32, 16, L.PIMHIP_ERR_UNSUPPORTED), (2, (1 << 26) + 1, 1 << 22, L.PIMHIP_ERR_INVALID_ARGUMENT),
+                                 (2, 2048, 48, L.PIMHIP_ERR_INVALID_ARGUMENT), (2, 2048, 72, L.PIMHIP_ERR_INVALID_ARGUMENT), (2, 2048, 1 << 27, L.PIMHIP_ERR_INVALID_ARGUMENT)):
+        assert lib.pimhip_mx4_quantize(L.Mx4Matrix(*at, rows, cols, ld), q.packed.data_ptr(), L.PIMHIP_F16, cols, None) == want
+    big = L.Mx4Matrix(*at, 1 << 33, 2048, 64)
+    assert lib.pimhip_mx4_linear(q.packed.data_ptr(), 1 << 33, q.packed.data_ptr(), 2048, L.PIMHIP_F16, 4096, big, None, 0, None) == L.PIMHIP_ERR_UNSUPPORTED
+    assert lib.pimhip_mx4_matmul(q.packed.data_ptr(), 1 << 33, L.PIMHIP_F16, big, big, None) == L.PIMHIP_ERR_UNSUPPORTED

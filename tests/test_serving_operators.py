@@ -53,3 +53,8 @@ def test_limits_in_python_and_c_agree():
     src = "".join(open(os.path.join(ROOT, "pimaicompiler_amd", "csrc", f)).read() for f in ("logprob_kernels.h", "moe_layer_kernels.h"))
     assert int(re.search(r"kTopMost = (\d+)", src).group(1)) == log_probs.TOP_MOST
     assert int(re.search(r"kMoeLayerTokens = (\d+)", src).group(1)) == moe_layer.TOKENS_MOST
+
+
+def test_a_plan_that_is_none_is_refused():
+    n = ctypes.c_uint64()
+    assert L.load().pimhip_moe_layer_workspace_bytes(ctypes.c_void_p(64), 1, ctypes.byref(n)) == L.PIMHIP_ERR_INVALID_ARGUMENT
