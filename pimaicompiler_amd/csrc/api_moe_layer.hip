@@ -20,7 +20,7 @@ namespace
 std::vector<PimHipMoeLayerPlan*> g_moe_layer_plans;
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
-size_t hidden_bytes(const PimHipMoeLayerPlan* p, int tokens) { return round256((size_t)tokens * p->top_k * p->d_ff * 2); }
+size_t hidden_bytes(const PimHipMoeLayerPlan* p, int tokens) { return round256((size_t)tokens * p->top_k * p->d_ff * 4); }
 size_t part_bytes(const PimHipMoeLayerPlan* p, int tokens) { return round256((size_t)tokens * p->top_k * p->d_model * sizeof(float)); }
 
 size_t counter_bytes(const PimHipMoeLayerPlan* p) { return (size_t)(p->d_model + 15) / 16 * sizeof(unsigned int); }
@@ -58,11 +58,11 @@ int destroy_moe_layer_plan_locked(PimHipMoeLayerPlan* plan)
     return PIMHIP_OK;
 }
 
-// LDS that staging the tokens of a product over K values takes, in bytes.
+// LDS that staging the columns of a product over K values takes, in bytes; each token makes `each` of them.
 template <class T, bool MX>
-unsigned int shared_bytes(const MoeLayerArgs& a, int K)
+unsigned int shared_bytes(const MoeLayerArgs& a, int K, int each)
 {
-    return (unsigned int)((a.tokens < 16 ? a.tokens : 16) * SharedTokens<T>::pitch(K, ExpertWeights<T, MX>::W::kUnit) * 16);
+    return (unsigned int)((a.tokens * each < 16 ? a.tokens * each : 16) * SharedTokens<T>::pitch(K, ExpertWeights<T, MX>::W::kUnit) * 16);
 }
 
 template <class T, bool MX, bool SHARED, bool GATED, int F>
@@ -70,14 +70,14 @@ void launch_first(const MoeLayerArgs& a, hipStream_t s)
 {
     constexpr int WK = 4;
     moe_layer_first_kernel<T, MX, SHARED, GATED, F, WK>
-        <<<dim3((unsigned)((a.d_ff + 16 * F - 1) / (16 * F)), (unsigned)a.E, (unsigned)((a.tokens + 15) / 16)), 64 * WK, SHARED ? shared_bytes<T, MX>(a, a.d_model) : 0, s>>>(a);
+        <<<dim3((unsigned)((a.d_ff + 16 * F - 1) / (16 * F)), (unsigned)a.E, (unsigned)((a.tokens + 15) / 16)), 64 * WK, SHARED ? shared_bytes<T, MX>(a, a.d_model, 1) : 0, s>>>(a);
 }
 
 template <class T, bool MX, bool SHARED, int RT, int WK>
 void launch_second(const MoeLayerArgs& a, hipStream_t s)
 {
     moe_layer_second_kernel<T, MX, SHARED, RT, WK>
-        <<<dim3((unsigned)((a.d_model + 16 * RT - 1) / (16 * RT)), (unsigned)a.E, (unsigned)((a.tokens + 15) / 16)), 64 * WK, SHARED ? shared_bytes<T, MX>(a, a.d_ff) : 0, s>>>(a);
+        <<<dim3((unsigned)((a.d_model + 16 * RT - 1) / (16 * RT)), (unsigned)a.E, (unsigned)((a.tokens + 7) / 8)), 64 * WK, SHARED ? shared_bytes<T, MX>(a, a.d_ff, 2) : 0, s>>>(a);
 }
 
 template <class T, bool MX>
@@ -98,12 +98,12 @@ void launch(const PimHipMoeLayerPlan* p, MoeLayerArgs& a, hipStream_t s)
         else
             p->gated ? launch_first<T, MX, S, true, 1>(a, s) : launch_first<T, MX, S, false, 2>(a, s);
     };
-    shared_bytes<T, MX>(a, a.d_model) <= most ? first(std::true_type{}) : first(std::false_type{});
+    shared_bytes<T, MX>(a, a.d_model, 1) <= most ? first(std::true_type{}) : first(std::false_type{});
     // Blocks of the second product that have something to read.  Where they fill the card several times over a block has two tiles of
     // rows, else one, and more wavefronts share its long k.
     const int active = a.E < a.tokens * a.top_k ? a.E : a.tokens * a.top_k;
     const int64_t blocks = (int64_t)((a.d_model + 15) / 16) * active;
-    const bool shared = shared_bytes<T, MX>(a, a.d_ff) <= most;
+    const bool shared = shared_bytes<T, MX>(a, a.d_ff, 2) <= most;
     if (many)
         shared ? launch_second<T, MX, true, 2, 8>(a, s) : launch_second<T, MX, false, 2, 8>(a, s);
     else if (blocks >= 2048)

@@ -30,7 +30,7 @@ struct MoeLayerArgs {
     void* y;
     int* chosen;      // [tokens][top_k]
     float* share;     // [tokens][top_k]
-    void* h;          // [pairs][d_ff]: hidden values, rounded to x's type as operands of the matrix cores
+    void* h;          // [pairs][2][d_ff]: hidden values rounded to x's type, and what that left over, rounded too
     float* part;      // [pairs][d_model]
     unsigned int* counters;  // pairs whose second product is done, for each tile of rows
     int counters_used;
@@ -186,7 +186,7 @@ struct ExpertWeights<T, true> {
 };
 
 // What a block of the experts' products has in LDS: the tokens that chose its expert, what its wavefronts turn operands in (and then
-// their sums), and, SHARED, in the launch's dynamic part the values of up to 16 pairs.
+// their sums), and, SHARED, in the launch's dynamic part the values of up to 16 columns.
 template <class T, bool MX, bool SHARED, int RT, int WK>
 struct ExpertLds {
     typedef typename ExpertWeights<T, MX>::W W;
@@ -197,8 +197,8 @@ struct ExpertLds {
     int count;
 };
 
-// Sums of 16 * RT rows for n (at most 16) pairs: `columns(i)` is pair i's values.  Ends with every wavefront having the sums of
-// its own k in `lds`, part[wave][i][lane].  SHARED: the pairs' values are staged in `xs`.
+// Sums of 16 * RT rows for n (at most 16) columns: `columns(i)` is column i's values.  Ends with every wavefront having the sums of
+// its own k in `lds`, part[wave][i][lane].  SHARED: the columns are staged in `xs`.
 template <class T, bool MX, bool SHARED, int RT, int WK, class F>
 __device__ __forceinline__ void expert_sums(const typename ExpertWeights<T, MX>::W::Rows (&rows)[RT], int K, int n, uint4_t* xs, uint4_t* lds, F columns)
 {
@@ -257,7 +257,7 @@ __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPoi
         const int f = f0 + i * 16 + group * 4, column = lane & 15;
         if (i % WK != wave || column >= n || f >= a.d_ff) continue;
         const float4_t g = joined<RT, WK>(lds, i);
-        float4_t u = {}, h;
+        float4_t u = {}, h, left;
         if constexpr (GATED) u = joined<RT, WK>(lds, F + i);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -270,9 +270,13 @@ __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPoi
                 if (p.b1) w += (float)((const typename T::elem*)p.b1)[a.d_ff + f + c];
                 v *= w;
             }
-            h[c] = v;
+            // A hidden value is two operands of the next product: rounded to 16 bits alone it would be what limits y.
+            h[c] = (float)T::round(v);
+            left[c] = fabsf(h[c]) < __builtin_inff() ? v - h[c] : 0.0f;
         }
-        store4<T>((typename T::elem*)a.h + (int64_t)list[column] * a.d_ff + f, h, 4);  // (d_ff is a multiple of 8)
+        typename T::elem* to = (typename T::elem*)a.h + (int64_t)list[column] * 2 * a.d_ff + f;
+        store4<T>(to, h, 4);  // (d_ff is a multiple of 8)
+        store4<T>(to + a.d_ff, left, 4);
     }
     __syncthreads();
 }
@@ -290,7 +294,7 @@ __global__ __launch_bounds__(64 * WK, F > 2 || (GATED && F > 1) ? 3 : 4) void mo
     if (n > 0) moe_first<T, MX, SHARED, GATED, F, WK>(a, p, lds.list + first, n < 16 ? n : 16, xs, lds.turn);
 }
 
-// The second product of up to 16 pairs: rows of d_model, with the bias, not yet weighted.
+// The second product of up to 8 pairs, two columns each: rows of d_model, with the bias, not yet weighted.
 template <class T, bool MX, bool SHARED, int RT, int WK>
 __device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPointers& p, const short* list, int n, uint4_t* xs, uint4_t* lds)
 {
@@ -300,24 +304,26 @@ __device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPo
     typename EW::W::Rows rows[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) rows[i] = EW::rows(p.w2, p.s2, p.t2, a.ld_s2, d0 + i * 16 < a.d_model ? d0 + i * 16 : a.d_model - 1, a.d_model, a.d_ff);
-    expert_sums<T, MX, SHARED, RT, WK>(rows, a.d_ff, n, xs, lds, [&](int i) { return (const typename T::elem*)a.h + (int64_t)list[i] * a.d_ff; });
+    expert_sums<T, MX, SHARED, RT, WK>(rows, a.d_ff, 2 * n, xs, lds,
+                                       [&](int i) { return (const typename T::elem*)a.h + ((int64_t)list[i / 2] * 2 + i % 2) * a.d_ff; });
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-        const int d = d0 + i * 16 + group * 4, column = lane & 15;
-        if (i % WK != wave || column >= n || d >= a.d_model) continue;
+        const int d = d0 + i * 16 + group * 4, pair = (lane & 15) / 2;
+        if (i % WK != wave || pair >= n || d >= a.d_model) continue;  // (two lanes at a time)
         float4_t v = joined<RT, WK>(lds, i);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
+            v[c] += dpp_f32<kDppQuadXor1>(v[c]);  // (the pair's other column)
             v[c] = EW::unscale(v[c], p.t2, d + c);
             if (p.b2) v[c] += (float)((const typename T::elem*)p.b2)[d + c];
         }
         const uint4_t q = __builtin_bit_cast(uint4_t, v);
-        store16_device_scope(a.part + (int64_t)list[column] * a.d_model + d, q[0] | (unsigned long long)q[1] << 32, q[2] | (unsigned long long)q[3] << 32);
+        if (lane % 2 == 0) store16_device_scope(a.part + (int64_t)list[pair] * a.d_model + d, q[0] | (unsigned long long)q[1] << 32, q[2] | (unsigned long long)q[3] << 32);
     }
     __syncthreads();
 }
 
-// Blocks as above.  The one whose pairs are the last of a tile of rows makes the weighted sum there, in the order of the choice.
+// Blocks as above, with 8 pairs.  The one whose pairs are the last of a tile of rows makes the weighted sum there, in the order of the choice.
 // An expert without a share adds nothing, whatever it computed.  Sums of other blocks come from other XCDs: they were stored past the L2s and
 // are loaded past them, and each block waits for its stores before it counts itself.
 template <class T, bool MX, bool SHARED, int RT, int WK>
@@ -327,9 +333,9 @@ __global__ __launch_bounds__(64 * WK, 4) void moe_layer_second_kernel(MoeLayerAr
     __shared__ unsigned int before;
     extern __shared__ uint4_t xs[];
     const ExpertPointers p = a.experts[blockIdx.y];
-    const int first = blockIdx.z * 16, left = pairs_of(a.chosen, a.tokens * a.top_k, blockIdx.y, lds.list, &lds.count) - first;
+    const int first = blockIdx.z * 8, left = pairs_of(a.chosen, a.tokens * a.top_k, blockIdx.y, lds.list, &lds.count) - first;
     if (left <= 0) return;
-    const int n = left < 16 ? left : 16;
+    const int n = left < 8 ? left : 8;
     moe_second<T, MX, SHARED, RT, WK>(a, p, lds.list + first, n, xs, lds.turn);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();

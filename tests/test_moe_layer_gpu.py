@@ -37,8 +37,8 @@ class Layer:
 
     def reference(self, x):
         """y, its bound, experts, shares, and which tokens' choice is clear.  Products of fp32 sums: (n + 3) 2^-24 of the sum of magnitudes; the
-        activation has a slope of at most 1.1 and, as SiLU, (8 + |v|) 2^-23 of its value from exp and the division; hidden values and y
-        are rounded by half a step of their type; shares are off by (2 + difference of logits) 2^-22."""
+        activation has a slope of at most 1.1 and, as SiLU, (8 + |v|) 2^-23 of its value from exp and the division; hidden values are kept
+        in two pieces of their type, the second rounded by half a step of at most half a step of the first, y in one; shares are off by (2 + difference of logits) 2^-22."""
         x = x.double()
         logits = x @ self.wr.double().t()
         size = x.abs() @ self.wr.double().abs().t()
@@ -71,7 +71,7 @@ class Layer:
                 if self.gated:
                     off_a = off_a * h[self.F:].abs() + a.abs() * off[self.F:] + off_a * off[self.F:]
                     a = a * h[self.F:]
-                off_a = off_a + a.abs() * (half + 2.0**-23) + torch.finfo(self.dtype).tiny * half
+                off_a = off_a + a.abs() * (half * half + 2.0**-23) + torch.finfo(self.dtype).tiny * half
                 o, size_o = a @ self.w2[n].t(), a.abs() @ self.w2[n].abs().t()
                 if self.b2 is not None:
                     o, size_o = o + self.b2[n].double(), size_o + self.b2[n].double().abs()
