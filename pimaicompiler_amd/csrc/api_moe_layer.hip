@@ -62,7 +62,7 @@ int destroy_moe_layer_plan_locked(PimHipMoeLayerPlan* plan)
 template <class T, bool MX>
 unsigned int shared_bytes(const MoeLayerArgs& a, int K, int each)
 {
-    return (unsigned int)((a.tokens * each < 16 ? a.tokens * each : 16) * SharedTokens<T>::pitch(K, ExpertWeights<T, MX>::W::kUnit) * 16);
+    return (unsigned int)((a.tokens < 16 ? a.tokens : 16) * each * SharedTokens<T>::pitch(K, ExpertWeights<T, MX, 1>::W::kUnit) * 16);
 }
 
 template <class T, bool MX, bool SHARED, bool GATED, int F>
@@ -73,11 +73,11 @@ void launch_first(const MoeLayerArgs& a, hipStream_t s)
         <<<dim3((unsigned)((a.d_ff + 16 * F - 1) / (16 * F)), (unsigned)a.E, (unsigned)((a.tokens + 15) / 16)), 64 * WK, SHARED ? shared_bytes<T, MX>(a, a.d_model, 1) : 0, s>>>(a);
 }
 
-template <class T, bool MX, bool SHARED, int RT, int WK>
+template <class T, bool MX, bool SHARED, int RT, int WK, int TT>
 void launch_second(const MoeLayerArgs& a, hipStream_t s)
 {
-    moe_layer_second_kernel<T, MX, SHARED, RT, WK>
-        <<<dim3((unsigned)((a.d_model + 16 * RT - 1) / (16 * RT)), (unsigned)a.E, (unsigned)((a.tokens + 7) / 8)), 64 * WK, SHARED ? shared_bytes<T, MX>(a, a.d_ff, 2) : 0, s>>>(a);
+    moe_layer_second_kernel<T, MX, SHARED, RT, WK, TT>
+        <<<dim3((unsigned)((a.d_model + 16 * RT - 1) / (16 * RT)), (unsigned)a.E, (unsigned)((a.tokens + 8 * TT - 1) / (8 * TT))), 64 * WK, SHARED ? shared_bytes<T, MX>(a, a.d_ff, 2) : 0, s>>>(a);
 }
 
 template <class T, bool MX>
@@ -100,16 +100,21 @@ void launch(const PimHipMoeLayerPlan* p, MoeLayerArgs& a, hipStream_t s)
     };
     shared_bytes<T, MX>(a, a.d_model, 1) <= most ? first(std::true_type{}) : first(std::false_type{});
     // Blocks of the second product that have something to read.  Where they fill the card several times over a block has two tiles of
-    // rows, else one, and more wavefronts share its long k.
-    const int active = a.E < a.tokens * a.top_k ? a.E : a.tokens * a.top_k;
-    const int64_t blocks = (int64_t)((a.d_model + 15) / 16) * active;
+    // rows and four wavefronts, else eight wavefronts share its long k.  Where experts have more than 8 pairs, which some have from 5 on the
+    // average on, 16 of them a block read their weights half as often.  In us a call, 16 / 8 pairs a block: 64 tokens through 8 gated 4-bit experts 1024
+    // -> 4096, two chosen (16 pairs an expert) 44.6 / 46.6, 32 tokens (8) 32.4 / 30.9, 17 tokens (4) 31 / 26; 64 tokens through 64 gated bf16 experts
+    // 2048 -> 1024, six chosen (6) 178 / 191.
+    const int pairs = a.tokens * a.top_k;
+    const int64_t blocks = (int64_t)((a.d_model + 15) / 16) * (a.E < pairs ? a.E : pairs);
     const bool shared = shared_bytes<T, MX>(a, a.d_ff, 2) <= most;
-    if (many)
-        shared ? launch_second<T, MX, true, 2, 8>(a, s) : launch_second<T, MX, false, 2, 8>(a, s);
+    if (pairs > 5 * a.E)
+        shared ? launch_second<T, MX, true, 2, 4, 2>(a, s) : launch_second<T, MX, false, 2, 4, 2>(a, s);
     else if (blocks >= 2048)
-        shared ? launch_second<T, MX, true, 2, 4>(a, s) : launch_second<T, MX, false, 2, 4>(a, s);
+        shared ? launch_second<T, MX, true, 2, 4, 1>(a, s) : launch_second<T, MX, false, 2, 4, 1>(a, s);
+    else if (many)
+        shared ? launch_second<T, MX, true, 2, 8, 1>(a, s) : launch_second<T, MX, false, 2, 8, 1>(a, s);
     else
-        shared ? launch_second<T, MX, true, 1, 8>(a, s) : launch_second<T, MX, false, 1, 8>(a, s);
+        shared ? launch_second<T, MX, true, 1, 8, 1>(a, s) : launch_second<T, MX, false, 1, 8, 1>(a, s);
 }
 }  // namespace
 

@@ -41,7 +41,7 @@ struct MoeLayerArgs {
 
 // ---- router ------------------------------------------------------------------------------------------------------------------
 // One token a block.  A wavefront has four experts at a time and 1024 values of each, whose loads do not wait for one another; the first
-// one chooses.
+// one chooses.  Bound by latency: 3.4 us for one token and 8 experts of 1024 values, 6.9 for 13 tokens and 64 of 2048.
 static constexpr int kRouterThreads = 1024;
 
 template <class T>
@@ -164,10 +164,11 @@ __device__ __forceinline__ int pairs_of(const int* chosen, int pairs, int e, sho
     return *count;
 }
 
-template <class T, bool MX>
+// (of 4-bit weights one step a unit leaves the registers that two columns a pair take)
+template <class T, bool MX, int TT>
 struct ExpertWeights;
-template <class T>
-struct ExpertWeights<T, false> {
+template <class T, int TT>
+struct ExpertWeights<T, false, TT> {
     typedef DenseWeights<T> W;
     static __device__ __forceinline__ typename W::Rows rows(const void* w, const void*, const void*, int, int64_t first, int64_t count, int K)
     {
@@ -175,9 +176,9 @@ struct ExpertWeights<T, false> {
     }
     static __device__ __forceinline__ float unscale(float v, const void*, int64_t) { return v; }
 };
-template <class T>
-struct ExpertWeights<T, true> {
-    typedef Mx4Weights<T, 2> W;
+template <class T, int TT>
+struct ExpertWeights<T, true, TT> {
+    typedef Mx4Weights<T, TT == 1 ? 2 : 1> W;
     static __device__ __forceinline__ typename W::Rows rows(const void* w, const void* s, const void* t, int ld, int64_t first, int64_t count, int K)
     {
         return W::rows((const uint8_t*)w, (const uint8_t*)s, (const uint8_t*)t, ld, first, count, K);
@@ -187,9 +188,9 @@ struct ExpertWeights<T, true> {
 
 // What a block of the experts' products has in LDS: the tokens that chose its expert, what its wavefronts turn operands in (and then
 // their sums), and, SHARED, in the launch's dynamic part the values of up to 16 columns.
-template <class T, bool MX, bool SHARED, int RT, int WK>
+template <class T, bool MX, bool SHARED, int RT, int WK, int TT>
 struct ExpertLds {
-    typedef typename ExpertWeights<T, MX>::W W;
+    typedef typename ExpertWeights<T, MX, TT>::W W;
     typedef typename std::conditional<SHARED, SharedTokens<T>, TurnedTokens<T, true>>::type X;
     static constexpr int kTurn = kSkinnyLds<W, X>, kSum = RT * 64;
     uint4_t turn[WK * (kTurn > kSum ? kTurn : kSum)];
@@ -197,31 +198,34 @@ struct ExpertLds {
     int count;
 };
 
-// Sums of 16 * RT rows for n (at most 16) columns: `columns(i)` is column i's values.  Ends with every wavefront having the sums of
-// its own k in `lds`, part[wave][i][lane].  SHARED: the columns are staged in `xs`.
-template <class T, bool MX, bool SHARED, int RT, int WK, class F>
-__device__ __forceinline__ void expert_sums(const typename ExpertWeights<T, MX>::W::Rows (&rows)[RT], int K, int n, uint4_t* xs, uint4_t* lds, F columns)
+// Sums of 16 * RT rows for n (at most 16) columns: column i's values are `columns(i)`, or the sum of TT of them, n apart.  Ends with
+// every wavefront having the sums of its own k in `lds`, part[wave][i][lane].  SHARED: the values are staged in `xs`.
+template <class T, bool MX, bool SHARED, int RT, int WK, int TT, class F>
+__device__ __forceinline__ void expert_sums(const typename ExpertWeights<T, MX, TT>::W::Rows (&rows)[RT], int K, int n, uint4_t* xs, uint4_t* lds, F columns)
 {
-    typedef typename ExpertWeights<T, MX>::W W;
+    typedef typename ExpertWeights<T, MX, TT>::W W;
     typedef typename std::conditional<SHARED, SharedTokens<T>, TurnedTokens<T, true>>::type X;
     const int lane = threadIdx.x & 63, wave = wave_in_block();
     const int pitch = SharedTokens<T>::pitch(K, W::kUnit);
-    float4_t acc[RT][1] = {};
-    typename X::Rows x[1];
-    if constexpr (SHARED)
-        x[0] = X::rows(xs, (lane & 15) < n ? lane & 15 : n - 1, pitch);
-    else
-        x[0] = X::rows([&](int i) { return columns(i < n ? i : n - 1); });
-    skinny_sum<T, W, X, RT, 1, 1>(acc, rows, x, K, wave, WK, lds + wave * kSkinnyLds<W, X>, [&] {
+    float4_t acc[RT][TT] = {};
+    typename X::Rows x[TT];
+#pragma unroll
+    for (int j = 0; j < TT; ++j) {
+        if constexpr (SHARED)
+            x[j] = X::rows(xs, j * n + ((lane & 15) < n ? lane & 15 : n - 1), pitch);
+        else
+            x[j] = X::rows([&](int i) { return columns(j * n + (i < n ? i : n - 1)); });
+    }
+    skinny_sum<T, W, X, RT, TT, 1>(acc, rows, x, K, wave, WK, lds + wave * kSkinnyLds<W, X>, [&] {
         if constexpr (SHARED) {
-            X::stage(xs, columns, n, K, pitch);
+            X::stage(xs, columns, TT * n, K, pitch);
             __syncthreads();
         }
     });
     __syncthreads();
     float4_t* part = reinterpret_cast<float4_t*>(lds);
 #pragma unroll
-    for (int i = 0; i < RT; ++i) part[(wave * RT + i) * 64 + lane] = acc[i][0];
+    for (int i = 0; i < RT; ++i) part[(wave * RT + i) * 64 + lane] = TT == 1 ? acc[i][0] : acc[i][0] + acc[i][TT - 1];
     __syncthreads();
 }
 
@@ -241,7 +245,7 @@ template <class T, bool MX, bool SHARED, bool GATED, int F, int WK>
 __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPointers& p, const short* list, int n, uint4_t* xs, uint4_t* lds)
 {
     constexpr int RT = GATED ? 2 * F : F;
-    typedef ExpertWeights<T, MX> EW;
+    typedef ExpertWeights<T, MX, 1> EW;
     const int lane = threadIdx.x & 63, wave = wave_in_block(), group = lane >> 4;
     const int f0 = blockIdx.x * (16 * F);
     typename EW::W::Rows rows[RT];
@@ -250,7 +254,7 @@ __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPoi
         const int end = i < F ? a.d_ff : 2 * a.d_ff, at = (i < F ? 0 : a.d_ff) + f0 + i % F * 16;
         rows[i] = EW::rows(p.w1, p.s1, p.t1, a.ld_s1, at < end ? at : end - 1, end, a.d_model);
     }
-    expert_sums<T, MX, SHARED, RT, WK>(rows, a.d_model, n, xs, lds,
+    expert_sums<T, MX, SHARED, RT, WK, 1>(rows, a.d_model, n, xs, lds,
                                    [&](int i) { return (const typename T::elem*)a.x + (int64_t)(list[i] / a.top_k) * a.ld_x; });
 #pragma unroll
     for (int i = 0; i < F; ++i) {
@@ -283,60 +287,66 @@ __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPoi
 
 // Block (x, y, z): rows x of expert y for its pairs 16 z .. 16 z + 15; those of more than 16 pairs read the weights again, out of the
 // caches.  (A loop over pairs in one block instead costs so many registers that half the wavefronts fit: 39 us against 25 for 64 tokens
-// through 8 gated 4-bit experts 1024 -> 4096, then.)
+// through 8 gated 4-bit experts 1024 -> 4096, before blocks had twice the rows.)  That case takes 20 us now, 35.7 MB; a block's chain of loads (its
+// pairs, then weights and values, k being one unit a wavefront) is what it waits for.  13 tokens through 64 gated bf16 experts 2048 -> 1024, six
+// chosen: 61 us, 6.3 TB/s.
 template <class T, bool MX, bool SHARED, bool GATED, int F, int WK>
 __global__ __launch_bounds__(64 * WK, F > 2 || (GATED && F > 1) ? 3 : 4) void moe_layer_first_kernel(MoeLayerArgs a)
 {
-    __shared__ ExpertLds<T, MX, SHARED, GATED ? 2 * F : F, WK> lds;
+    __shared__ ExpertLds<T, MX, SHARED, GATED ? 2 * F : F, WK, 1> lds;
     extern __shared__ uint4_t xs[];
     const ExpertPointers p = a.experts[blockIdx.y];
     const int first = blockIdx.z * 16, n = pairs_of(a.chosen, a.tokens * a.top_k, blockIdx.y, lds.list, &lds.count) - first;
     if (n > 0) moe_first<T, MX, SHARED, GATED, F, WK>(a, p, lds.list + first, n < 16 ? n : 16, xs, lds.turn);
 }
 
-// The second product of up to 8 pairs, two columns each: rows of d_model, with the bias, not yet weighted.
-template <class T, bool MX, bool SHARED, int RT, int WK>
+// The second product: rows of d_model, with the bias, not yet weighted.  TT 1: of up to 8 pairs, two columns each; TT 2: of up to 16.
+template <class T, bool MX, bool SHARED, int RT, int WK, int TT>
 __device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPointers& p, const short* list, int n, uint4_t* xs, uint4_t* lds)
 {
-    typedef ExpertWeights<T, MX> EW;
+    typedef ExpertWeights<T, MX, TT> EW;
     const int lane = threadIdx.x & 63, wave = wave_in_block(), group = lane >> 4;
     const int d0 = blockIdx.x * (16 * RT);
     typename EW::W::Rows rows[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) rows[i] = EW::rows(p.w2, p.s2, p.t2, a.ld_s2, d0 + i * 16 < a.d_model ? d0 + i * 16 : a.d_model - 1, a.d_model, a.d_ff);
-    expert_sums<T, MX, SHARED, RT, WK>(rows, a.d_ff, 2 * n, xs, lds,
-                                       [&](int i) { return (const typename T::elem*)a.h + ((int64_t)list[i / 2] * 2 + i % 2) * a.d_ff; });
+    const typename T::elem* h = (const typename T::elem*)a.h;
+    if constexpr (TT == 1)
+        expert_sums<T, MX, SHARED, RT, WK, 1>(rows, a.d_ff, 2 * n, xs, lds, [&](int i) { return h + ((int64_t)list[i / 2] * 2 + i % 2) * a.d_ff; });
+    else
+        expert_sums<T, MX, SHARED, RT, WK, 2>(rows, a.d_ff, n, xs, lds, [&](int i) { return h + ((int64_t)list[i < n ? i : i - n] * 2 + (i < n ? 0 : 1)) * a.d_ff; });
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-        const int d = d0 + i * 16 + group * 4, pair = (lane & 15) / 2;
+        const int d = d0 + i * 16 + group * 4, pair = TT == 1 ? (lane & 15) / 2 : lane & 15;
         if (i % WK != wave || pair >= n || d >= a.d_model) continue;  // (two lanes at a time)
         float4_t v = joined<RT, WK>(lds, i);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            v[c] += dpp_f32<kDppQuadXor1>(v[c]);  // (the pair's other column)
+            if (TT == 1) v[c] += dpp_f32<kDppQuadXor1>(v[c]);  // (the pair's other column)
             v[c] = EW::unscale(v[c], p.t2, d + c);
             if (p.b2) v[c] += (float)((const typename T::elem*)p.b2)[d + c];
         }
         const uint4_t q = __builtin_bit_cast(uint4_t, v);
-        if (lane % 2 == 0) store16_device_scope(a.part + (int64_t)list[pair] * a.d_model + d, q[0] | (unsigned long long)q[1] << 32, q[2] | (unsigned long long)q[3] << 32);
+        if (TT == 2 || lane % 2 == 0) store16_device_scope(a.part + (int64_t)list[pair] * a.d_model + d, q[0] | (unsigned long long)q[1] << 32, q[2] | (unsigned long long)q[3] << 32);
     }
     __syncthreads();
 }
 
-// Blocks as above, with 8 pairs.  The one whose pairs are the last of a tile of rows makes the weighted sum there, in the order of the choice.
+// Blocks as above, with 8 TT pairs.  The one whose pairs are the last of a tile of rows makes the weighted sum there, in the order of the choice.
 // An expert without a share adds nothing, whatever it computed.  Sums of other blocks come from other XCDs: they were stored past the L2s and
-// are loaded past them, and each block waits for its stores before it counts itself.
-template <class T, bool MX, bool SHARED, int RT, int WK>
-__global__ __launch_bounds__(64 * WK, 4) void moe_layer_second_kernel(MoeLayerArgs a)
+// are loaded past them, and each block waits for its stores before it counts its pairs.  One token through 2 of 8 fp16 experts 1024 -> 4096: 8.3 us
+// (16.8 MB; dividing its k among two or four blocks is no faster); 13 tokens as above: 37 us, 5.2 TB/s; 64 as above: 18 us.
+template <class T, bool MX, bool SHARED, int RT, int WK, int TT>
+__global__ __launch_bounds__(64 * WK, TT == 2 ? 3 : 4) void moe_layer_second_kernel(MoeLayerArgs a)
 {
-    __shared__ ExpertLds<T, MX, SHARED, RT, WK> lds;
+    __shared__ ExpertLds<T, MX, SHARED, RT, WK, TT> lds;
     __shared__ unsigned int before;
     extern __shared__ uint4_t xs[];
     const ExpertPointers p = a.experts[blockIdx.y];
-    const int first = blockIdx.z * 8, left = pairs_of(a.chosen, a.tokens * a.top_k, blockIdx.y, lds.list, &lds.count) - first;
+    const int first = blockIdx.z * (8 * TT), left = pairs_of(a.chosen, a.tokens * a.top_k, blockIdx.y, lds.list, &lds.count) - first;
     if (left <= 0) return;
-    const int n = left < 8 ? left : 8;
-    moe_second<T, MX, SHARED, RT, WK>(a, p, lds.list + first, n, xs, lds.turn);
+    const int n = left < 8 * TT ? left : 8 * TT;
+    moe_second<T, MX, SHARED, RT, WK, TT>(a, p, lds.list + first, n, xs, lds.turn);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) before = __hip_atomic_fetch_add(&a.counters[blockIdx.x], (unsigned int)n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
