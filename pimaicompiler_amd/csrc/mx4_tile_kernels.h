@@ -25,7 +25,7 @@ __device__ __forceinline__ void tile_at(int id, int tiles_n, int tiles_t, int64_
 // buffer: the next step's operands wait in registers.  Loads take whole runs of a row (16 lanes in 16 rows would be 16 requests), and a
 // row's 16-byte chunks lie in LDS in an order that spreads what 8 lanes read or write over all banks.
 //
-// 4096 x 16384 x 4096: 532 us, 1.03 PFLOP/s; 1500 x 4096 x 4096: 65 us, 0.77 (this card's library multiplies 16-bit matrices of 8192 at 1.27
+// 4096 x 16384 x 4096: 528 us, 1.04 PFLOP/s; 1500 x 4096 x 4096: 63 us, 0.80 (this card's library multiplies 16-bit matrices of 8192 at 1.27
 // to 1.5).  A block alone takes 1.9 us a step of 256 x 128 x 128: the matrix cores work 0.9 of it, the conversions, one instruction a
 // product, take issue slots, LDS is busy 0.75.  Measured and not better: two steps in registers (the same; three: spills), two buffers
 // (512, but 1500 tokens 73), 128 rows and tokens and four wavefronts (565), 32 x 128 results a wavefront, half the conversions but twice
@@ -166,11 +166,12 @@ __global__ __launch_bounds__(64 * GN * GT) void mx4_linear_tile_kernel(const typ
 // straight into LDS while the one before is multiplied, operands go from LDS to registers a product ahead, and two blocks of a CU fill
 // each other's waits.
 //
-// 4096 x 16384 x 4096: 193 us, 2.85 PFLOP/s (a loop of the instruction alone reaches 7 to 8.8 here).  Two of these blocks' steps take
-// 1.5 us, of which the matrix cores work 0.5 and LDS is read and written 0.7: what is left waits for a step to arrive, which takes a
+// 4096 x 16384 x 4096: 177 us, 3.1 PFLOP/s (a loop of the instruction alone reaches 7 to 8.8 here).  Two of these blocks' steps take
+// 1.4 us, of which the matrix cores work 0.5 and LDS is read and written 0.7: what is left waits for a step to arrive, which takes a
 // microsecond, and LDS holds no more steps.  Measured besides: steps of 128 values, three or four on their way, 227 (half a line is
 // a whole request); 256 x 256 results a block, one block a CU, 198 with steps of 128, 226 with steps of 256, and slower by half and
-// more where blocks are few; each code word loaded with its step 301 (a row's code is a request, however few bytes it has).
+// more where blocks are few; each code word loaded with its step 301 (a row's code is a request, however few bytes it has); k begun in another place by each column of tiles
+// the same, and 181 instead of 165 for 4096 x 4096 x 16384 (rows that blocks have in common then leave the L2 before all have read them).
 template <class O>
 __global__ __launch_bounds__(256, 2) void mx4_matmul_tile_kernel(Mx4View a, Mx4View b, typename O::elem* out, int64_t ld_out)
 {
@@ -206,15 +207,11 @@ __global__ __launch_bounds__(256, 2) void mx4_matmul_tile_kernel(Mx4View a, Mx4V
     const int c_row = weights ? weight_row(row, group) : token_row(row, group);
     c_at = (unsigned int)(c_row < most ? c_row : most) * (unsigned int)m.ld_scales;
     const unsigned int lds0 = (unsigned int)(size_t)(__attribute__((address_space(3))) uint8_t*)lds;
-    // Rows a power of two apart have the same step's bytes in the same few channels of an L2: column tiles start k at places of their own.
-    const int turn = whole > 0 && whole % 2 == 0 ? (int)(tile_t & 15) * 4 % whole : 0;
     auto fetch = [&](int step) __attribute__((always_inline)) {
-        int at = step + turn;
-        at = at < whole ? at : at - whole;
-        if (step % 2 == 0) load_lds16(cp + at * 8, c_at, lds0 + 2 * kBuffer + (unsigned int)(step / 2 % 2) * kCodes + (unsigned int)wave * 1024u);
+        if (step % 2 == 0) load_lds16(cp + step * 8, c_at, lds0 + 2 * kBuffer + (unsigned int)(step / 2 % 2) * kCodes + (unsigned int)wave * 1024u);
 #pragma unroll
         for (int i = 0; i < kPieces; ++i)
-            load_lds16(vp + (int64_t)at * (8 * kMxBlockBytes), v_at[i], lds0 + (unsigned int)(step % 2) * kBuffer + (unsigned int)(wave * kPieces + i) * 1024u);
+            load_lds16(vp + (int64_t)step * (8 * kMxBlockBytes), v_at[i], lds0 + (unsigned int)(step % 2) * kBuffer + (unsigned int)(wave * kPieces + i) * 1024u);
     };
 
     struct Part {  // four tiles' operands, and their codes (byte `group` of what is read) in one register
