@@ -343,7 +343,7 @@ bool rowsOf(const at::Tensor& t, int64_t& rows, int64_t& cols, int64_t& ld)
 // The address of a PimHipMx4Matrix that a Python object keeps.
 const PimHipMx4Matrix* matrixOf(PyObject* o) { return PyLong_Check(o) ? static_cast<const PimHipMx4Matrix*>(PyLong_AsVoidPtr(o)) : nullptr; }
 
-// mx4_quantize(x): (packed, scales, tops)
+// mx4_quantize(x): (packed, scales, tops, the bytes of a PimHipMx4Matrix of them, their address, device index)
 PyObject* mx4Quantize(PyObject*, PyObject* const* args, Py_ssize_t n)
 {
     const at::Tensor* x;
@@ -359,11 +359,18 @@ PyObject* mx4Quantize(PyObject*, PyObject* const* args, Py_ssize_t n)
     rc = pimhip_mx4_quantize(&m, x->data_ptr(), typeCode(x->scalar_type()), ld, stream);
     Py_END_ALLOW_THREADS
     if (rc != PIMHIP_OK) return status(rc);
-    PyObject* out = PyTuple_New(3);
-    if (!out) return nullptr;
+    PyObject* bytes = PyBytes_FromStringAndSize(reinterpret_cast<const char*>(&m), sizeof(m));
+    PyObject* out = bytes ? PyTuple_New(6) : nullptr;
+    if (!out) {
+        Py_XDECREF(bytes);
+        return nullptr;
+    }
     PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(packed)));
     PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(scales)));
     PyTuple_SET_ITEM(out, 2, THPVariable_Wrap(std::move(tops)));
+    PyTuple_SET_ITEM(out, 3, bytes);
+    PyTuple_SET_ITEM(out, 4, PyLong_FromVoidPtr(PyBytes_AS_STRING(bytes)));
+    PyTuple_SET_ITEM(out, 5, PyLong_FromLong(x->device().index()));
     return out;
 }
 

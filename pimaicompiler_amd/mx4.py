@@ -77,8 +77,8 @@ class Mx4Tensor:
 
     def _hold(self, packed, scales, tops, shape):
         self.packed, self.scales, self.tops, self.shape = packed, scales, tops, torch.Size(shape)
-        self._c = L.Mx4Matrix(packed.data_ptr(), scales.data_ptr(), tops.data_ptr(), packed.size(0), self.shape[-1], scales.size(1))
-        self._at = ctypes.addressof(self._c)   # (what the native calls read the matrix through)
+        self._keep = L.Mx4Matrix(packed.data_ptr(), scales.data_ptr(), tops.data_ptr(), packed.size(0), self.shape[-1], scales.size(1))
+        self._at = ctypes.addressof(self._keep)   # (what the native calls read the matrix through)
         self._device_index = packed.device.index
 
     @classmethod
@@ -91,6 +91,10 @@ class Mx4Tensor:
         self._hold(torch.empty((rows, blocks * 16), dtype=torch.uint8, device=device),
                    torch.empty((rows, -(-blocks // 16) * 16), dtype=torch.uint8, device=device), torch.empty(rows, dtype=torch.uint8, device=device), shape)
         return self
+
+    @property
+    def _c(self):
+        return L.Mx4Matrix.from_address(self._at)
 
     @property
     def device(self):
@@ -114,7 +118,8 @@ def mx4_quantize(x, stream=None):
     made = _native().fast_mx4_quantize(x) if stream is None else None
     if made is not None:
         q = Mx4Tensor.__new__(Mx4Tensor)
-        q._hold(*_result(made), x.shape)
+        q.packed, q.scales, q.tops, q._keep, q._at, q._device_index = _result(made)
+        q.shape = x.shape
         return q
     _require("x", x, tuple(_CODES))
     _require_no_gradient(x)
@@ -184,7 +189,7 @@ def mx4_matmul(a, b, dtype=torch.float16, stream=None):
         raise NNRuntimeException(f"{dtype} is none of {', '.join(str(d) for d in _CODES)}")
     if a.shape[-1] != b.shape[-1]:
         raise NNRuntimeException(f"the operands disagree on the reduction width ({a.shape[-1]} vs {b.shape[-1]})")
-    if a.device != b.device:
+    if a._device_index != b._device_index:
         raise NNRuntimeException(f"a is on {a.device}, b on {b.device}")
     out = _native().fast_mx4_matmul(a._at, a.shape, b._at, a._device_index, _CODES[dtype]) if stream is None else None
     if out is not None:
