@@ -65,12 +65,12 @@ unsigned int shared_bytes(const MoeLayerArgs& a, int K, int each)
     return (unsigned int)((a.tokens < 16 ? a.tokens : 16) * each * SharedTokens<T>::pitch(K, ExpertWeights<T, MX, 1>::W::kUnit) * 16);
 }
 
-template <class T, bool MX, bool SHARED, bool GATED, int F>
+template <class T, bool MX, bool SHARED, bool GATED, int F, int TT>
 void launch_first(const MoeLayerArgs& a, hipStream_t s)
 {
     constexpr int WK = 4;
-    moe_layer_first_kernel<T, MX, SHARED, GATED, F, WK>
-        <<<dim3((unsigned)((a.d_ff + 16 * F - 1) / (16 * F)), (unsigned)a.E, (unsigned)((a.tokens + 15) / 16)), 64 * WK, SHARED ? shared_bytes<T, MX>(a, a.d_model, 1) : 0, s>>>(a);
+    moe_layer_first_kernel<T, MX, SHARED, GATED, F, WK, TT>
+        <<<dim3((unsigned)((a.d_ff + 16 * F - 1) / (16 * F)), (unsigned)a.E, (unsigned)((a.tokens + 16 * TT - 1) / (16 * TT))), 64 * WK, SHARED ? shared_bytes<T, MX>(a, a.d_model, 1) : 0, s>>>(a);
 }
 
 template <class T, bool MX, bool SHARED, int RT, int WK, int TT>
@@ -94,17 +94,23 @@ void launch(const PimHipMoeLayerPlan* p, MoeLayerArgs& a, hipStream_t s)
     auto first = [&](auto shared) {
         constexpr bool S = decltype(shared)::value;
         if (many)
-            p->gated ? launch_first<T, MX, S, true, 2>(a, s) : launch_first<T, MX, S, false, 4>(a, s);
+            p->gated ? launch_first<T, MX, S, true, 2, 1>(a, s) : launch_first<T, MX, S, false, 4, 1>(a, s);
         else
-            p->gated ? launch_first<T, MX, S, true, 1>(a, s) : launch_first<T, MX, S, false, 2>(a, s);
+            p->gated ? launch_first<T, MX, S, true, 1, 1>(a, s) : launch_first<T, MX, S, false, 2, 1>(a, s);
     };
-    shared_bytes<T, MX>(a, a.d_model, 1) <= most ? first(std::true_type{}) : first(std::false_type{});
+    // Where experts have more than 16 pairs, which some have from 10 on the average on, 32 of them a block read their weights half as often.
+    // In us a call, 32 / 16 pairs a block, 64 tokens through 8 experts 1024 -> 4096, two chosen: gated in 4 bits 41.3 / 44.7, gated fp16 64 / 79, fp16
+    // 51 / 54; 16 tokens through both of 2 experts 512 -> 1024, which have 16 pairs at the most, 17.9 / 15.9.
+    const int pairs = a.tokens * a.top_k;
+    if (many && pairs > 10 * a.E)
+        p->gated ? launch_first<T, MX, false, true, 2, 2>(a, s) : launch_first<T, MX, false, false, 4, 2>(a, s);
+    else
+        shared_bytes<T, MX>(a, a.d_model, 1) <= most ? first(std::true_type{}) : first(std::false_type{});
     // Blocks of the second product that have something to read.  Where they fill the card several times over a block has two tiles of
     // rows and four wavefronts, else eight wavefronts share its long k.  Where experts have more than 8 pairs, which some have from 5 on the
     // average on, 16 of them a block read their weights half as often.  In us a call, 16 / 8 pairs a block: 64 tokens through 8 gated 4-bit experts 1024
     // -> 4096, two chosen (16 pairs an expert) 44.6 / 46.6, 32 tokens (8) 32.4 / 30.9, 17 tokens (4) 31 / 26; 64 tokens through 64 gated bf16 experts
     // 2048 -> 1024, six chosen (6) 178 / 191.
-    const int pairs = a.tokens * a.top_k;
     const int64_t blocks = (int64_t)((a.d_model + 15) / 16) * (a.E < pairs ? a.E : pairs);
     const bool shared = shared_bytes<T, MX>(a, a.d_ff, 2) <= most;
     if (pairs > 5 * a.E)

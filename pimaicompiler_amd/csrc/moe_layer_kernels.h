@@ -188,19 +188,19 @@ struct ExpertWeights<T, true, TT> {
 
 // What a block of the experts' products has in LDS: the tokens that chose its expert, what its wavefronts turn operands in (and then
 // their sums), and, SHARED, in the launch's dynamic part the values of up to 16 columns.
-template <class T, bool MX, bool SHARED, int RT, int WK, int TT>
+template <class T, bool MX, bool SHARED, int RT, int WK, int TT, int PARTS>
 struct ExpertLds {
     typedef typename ExpertWeights<T, MX, TT>::W W;
     typedef typename std::conditional<SHARED, SharedTokens<T>, TurnedTokens<T, true>>::type X;
-    static constexpr int kTurn = kSkinnyLds<W, X>, kSum = RT * 64;
+    static constexpr int kTurn = kSkinnyLds<W, X>, kSum = RT * PARTS * 64;
     uint4_t turn[WK * (kTurn > kSum ? kTurn : kSum)];
     short list[kMoeLayerPairs];
     int count;
 };
 
-// Sums of 16 * RT rows for n (at most 16) columns: column i's values are `columns(i)`, or the sum of TT of them, n apart.  Ends with
-// every wavefront having the sums of its own k in `lds`, part[wave][i][lane].  SHARED: the values are staged in `xs`.
-template <class T, bool MX, bool SHARED, int RT, int WK, int TT, class F>
+// Sums of 16 * RT rows for n columns, whose values are `columns(i)`.  TT 2, PARTS 1: of n (at most 16) sums of two, n apart.  Else n is at most 16 TT.
+// Ends with every wavefront having the sums of its own k in `lds`, part[wave][i][j][lane].  SHARED: the values are staged in `xs`.
+template <class T, bool MX, bool SHARED, int RT, int WK, int TT, int PARTS, class F>
 __device__ __forceinline__ void expert_sums(const typename ExpertWeights<T, MX, TT>::W::Rows (&rows)[RT], int K, int n, uint4_t* xs, uint4_t* lds, F columns)
 {
     typedef typename ExpertWeights<T, MX, TT>::W W;
@@ -211,21 +211,25 @@ __device__ __forceinline__ void expert_sums(const typename ExpertWeights<T, MX, 
     typename X::Rows x[TT];
 #pragma unroll
     for (int j = 0; j < TT; ++j) {
+        // (columns behind the last one: that one again)
+        auto at = [&](int i) { return PARTS == TT ? (j * 16 + i < n ? j * 16 + i : n - 1) : j * n + (i < n ? i : n - 1); };
         if constexpr (SHARED)
-            x[j] = X::rows(xs, j * n + ((lane & 15) < n ? lane & 15 : n - 1), pitch);
+            x[j] = X::rows(xs, at(lane & 15), pitch);
         else
-            x[j] = X::rows([&](int i) { return columns(j * n + (i < n ? i : n - 1)); });
+            x[j] = X::rows([&](int i) { return columns(at(i)); });
     }
     skinny_sum<T, W, X, RT, TT, 1>(acc, rows, x, K, wave, WK, lds + wave * kSkinnyLds<W, X>, [&] {
         if constexpr (SHARED) {
-            X::stage(xs, columns, TT * n, K, pitch);
+            X::stage(xs, columns, PARTS == TT ? n : TT * n, K, pitch);
             __syncthreads();
         }
     });
     __syncthreads();
     float4_t* part = reinterpret_cast<float4_t*>(lds);
 #pragma unroll
-    for (int i = 0; i < RT; ++i) part[(wave * RT + i) * 64 + lane] = TT == 1 ? acc[i][0] : acc[i][0] + acc[i][TT - 1];
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < PARTS; ++j) part[((wave * RT + i) * PARTS + j) * 64 + lane] = PARTS == TT ? acc[i][j] : acc[i][0] + acc[i][TT - 1];
     __syncthreads();
 }
 
@@ -240,12 +244,12 @@ __device__ __forceinline__ float4_t joined(const uint4_t* lds, int i)
     return v;
 }
 
-// The first product of up to 16 pairs: hidden values 16 * F a block, each with its gate where there is one.
-template <class T, bool MX, bool SHARED, bool GATED, int F, int WK>
+// The first product of up to 16 TT pairs: hidden values 16 * F a block, each with its gate where there is one.
+template <class T, bool MX, bool SHARED, bool GATED, int F, int WK, int TT>
 __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPointers& p, const short* list, int n, uint4_t* xs, uint4_t* lds)
 {
     constexpr int RT = GATED ? 2 * F : F;
-    typedef ExpertWeights<T, MX, 1> EW;
+    typedef ExpertWeights<T, MX, TT> EW;
     const int lane = threadIdx.x & 63, wave = wave_in_block(), group = lane >> 4;
     const int f0 = blockIdx.x * (16 * F);
     typename EW::W::Rows rows[RT];
@@ -254,15 +258,15 @@ __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPoi
         const int end = i < F ? a.d_ff : 2 * a.d_ff, at = (i < F ? 0 : a.d_ff) + f0 + i % F * 16;
         rows[i] = EW::rows(p.w1, p.s1, p.t1, a.ld_s1, at < end ? at : end - 1, end, a.d_model);
     }
-    expert_sums<T, MX, SHARED, RT, WK, 1>(rows, a.d_model, n, xs, lds,
+    expert_sums<T, MX, SHARED, RT, WK, TT, TT>(rows, a.d_model, n, xs, lds,
                                    [&](int i) { return (const typename T::elem*)a.x + (int64_t)(list[i] / a.top_k) * a.ld_x; });
 #pragma unroll
-    for (int i = 0; i < F; ++i) {
-        const int f = f0 + i * 16 + group * 4, column = lane & 15;
-        if (i % WK != wave || column >= n || f >= a.d_ff) continue;
-        const float4_t g = joined<RT, WK>(lds, i);
+    for (int k = 0; k < F * TT; ++k) {
+        const int i = k / TT, j = k % TT, f = f0 + i * 16 + group * 4, column = j * 16 + (lane & 15);
+        if (k % WK != wave || column >= n || f >= a.d_ff) continue;
+        const float4_t g = joined<RT * TT, WK>(lds, k);
         float4_t u = {}, h, left;
-        if constexpr (GATED) u = joined<RT, WK>(lds, F + i);
+        if constexpr (GATED) u = joined<RT * TT, WK>(lds, (F + i) * TT + j);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             float v = EW::unscale(g[c], p.t1, f + c);
@@ -285,19 +289,19 @@ __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPoi
     __syncthreads();
 }
 
-// Block (x, y, z): rows x of expert y for its pairs 16 z .. 16 z + 15; those of more than 16 pairs read the weights again, out of the
+// Block (x, y, z): rows x of expert y for 16 TT of its pairs, from 16 TT z on; those of more pairs read the weights again, out of the
 // caches.  (A loop over pairs in one block instead costs so many registers that half the wavefronts fit: 39 us against 25 for 64 tokens
 // through 8 gated 4-bit experts 1024 -> 4096, before blocks had twice the rows.)  That case takes 20 us now, 35.7 MB; a block's chain of loads (its
 // pairs, then weights and values, k being one unit a wavefront) is what it waits for.  13 tokens through 64 gated bf16 experts 2048 -> 1024, six
 // chosen: 61 us, 6.3 TB/s.
-template <class T, bool MX, bool SHARED, bool GATED, int F, int WK>
-__global__ __launch_bounds__(64 * WK, F > 2 || (GATED && F > 1) ? 3 : 4) void moe_layer_first_kernel(MoeLayerArgs a)
+template <class T, bool MX, bool SHARED, bool GATED, int F, int WK, int TT>
+__global__ __launch_bounds__(64 * WK, TT > 1 ? 2 : F > 2 || (GATED && F > 1) ? 3 : 4) void moe_layer_first_kernel(MoeLayerArgs a)
 {
-    __shared__ ExpertLds<T, MX, SHARED, GATED ? 2 * F : F, WK, 1> lds;
+    __shared__ ExpertLds<T, MX, SHARED, GATED ? 2 * F : F, WK, TT, TT> lds;
     extern __shared__ uint4_t xs[];
     const ExpertPointers p = a.experts[blockIdx.y];
-    const int first = blockIdx.z * 16, n = pairs_of(a.chosen, a.tokens * a.top_k, blockIdx.y, lds.list, &lds.count) - first;
-    if (n > 0) moe_first<T, MX, SHARED, GATED, F, WK>(a, p, lds.list + first, n < 16 ? n : 16, xs, lds.turn);
+    const int first = blockIdx.z * (16 * TT), n = pairs_of(a.chosen, a.tokens * a.top_k, blockIdx.y, lds.list, &lds.count) - first;
+    if (n > 0) moe_first<T, MX, SHARED, GATED, F, WK, TT>(a, p, lds.list + first, n < 16 * TT ? n : 16 * TT, xs, lds.turn);
 }
 
 // The second product: rows of d_model, with the bias, not yet weighted.  TT 1: of up to 8 pairs, two columns each; TT 2: of up to 16.
@@ -312,9 +316,9 @@ __device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPo
     for (int i = 0; i < RT; ++i) rows[i] = EW::rows(p.w2, p.s2, p.t2, a.ld_s2, d0 + i * 16 < a.d_model ? d0 + i * 16 : a.d_model - 1, a.d_model, a.d_ff);
     const typename T::elem* h = (const typename T::elem*)a.h;
     if constexpr (TT == 1)
-        expert_sums<T, MX, SHARED, RT, WK, 1>(rows, a.d_ff, 2 * n, xs, lds, [&](int i) { return h + ((int64_t)list[i / 2] * 2 + i % 2) * a.d_ff; });
+        expert_sums<T, MX, SHARED, RT, WK, 1, 1>(rows, a.d_ff, 2 * n, xs, lds, [&](int i) { return h + ((int64_t)list[i / 2] * 2 + i % 2) * a.d_ff; });
     else
-        expert_sums<T, MX, SHARED, RT, WK, 2>(rows, a.d_ff, n, xs, lds, [&](int i) { return h + ((int64_t)list[i < n ? i : i - n] * 2 + (i < n ? 0 : 1)) * a.d_ff; });
+        expert_sums<T, MX, SHARED, RT, WK, 2, 1>(rows, a.d_ff, n, xs, lds, [&](int i) { return h + ((int64_t)list[i < n ? i : i - n] * 2 + (i < n ? 0 : 1)) * a.d_ff; });
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
         const int d = d0 + i * 16 + group * 4, pair = TT == 1 ? (lane & 15) / 2 : lane & 15;
@@ -339,7 +343,7 @@ __device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPo
 template <class T, bool MX, bool SHARED, int RT, int WK, int TT>
 __global__ __launch_bounds__(64 * WK, TT == 2 ? 3 : 4) void moe_layer_second_kernel(MoeLayerArgs a)
 {
-    __shared__ ExpertLds<T, MX, SHARED, RT, WK, TT> lds;
+    __shared__ ExpertLds<T, MX, SHARED, RT, WK, TT, 1> lds;
     __shared__ unsigned int before;
     extern __shared__ uint4_t xs[];
     const ExpertPointers p = a.experts[blockIdx.y];
