@@ -113,9 +113,14 @@ void launch(const PimHipMoeLayerPlan* p, MoeLayerArgs& a, hipStream_t s)
     // 2048 -> 1024, six chosen (6) 178 / 191.
     const int64_t blocks = (int64_t)((a.d_model + 15) / 16) * (a.E < pairs ? a.E : pairs);
     const bool shared = shared_bytes<T, MX>(a, a.d_ff, 2) <= most;
-    if (pairs > 5 * a.E)
+    if (pairs > 5 * a.E) {
+        if constexpr (!MX) {
+            // (16-bit weights are four times the bytes: 64 tokens through 8 fp16 experts 1024 -> 4096 46.5 with eight wavefronts and a tile, 51 with two
+            // tiles and four; in 4 bits 46.0 / 41.3, the values being turned for each tile of rows)
+            if (blocks < 2048) return shared ? launch_second<T, MX, true, 1, 8, 2>(a, s) : launch_second<T, MX, false, 1, 8, 2>(a, s);
+        }
         shared ? launch_second<T, MX, true, 2, 4, 2>(a, s) : launch_second<T, MX, false, 2, 4, 2>(a, s);
-    else if (blocks >= 2048)
+    } else if (blocks >= 2048)
         shared ? launch_second<T, MX, true, 2, 4, 1>(a, s) : launch_second<T, MX, false, 2, 4, 1>(a, s);
     else if (many)
         shared ? launch_second<T, MX, true, 2, 8, 1>(a, s) : launch_second<T, MX, false, 2, 8, 1>(a, s);

@@ -291,8 +291,8 @@ __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPoi
 
 // Block (x, y, z): rows x of expert y for 16 TT of its pairs, from 16 TT z on; those of more pairs read the weights again, out of the
 // caches.  (A loop over pairs in one block instead costs so many registers that half the wavefronts fit: 39 us against 25 for 64 tokens
-// through 8 gated 4-bit experts 1024 -> 4096, before blocks had twice the rows.)  That case takes 20 us now, 35.7 MB; a block's chain of loads (its
-// pairs, then weights and values, k being one unit a wavefront) is what it waits for.  13 tokens through 64 gated bf16 experts 2048 -> 1024, six
+// through 8 gated 4-bit experts 1024 -> 4096, before blocks had twice the rows.)  That case takes 18 us now with TT 2, 35.7 MB; a block's chain of
+// loads (its pairs, then weights and values, k being a unit or two a wavefront) is what it waits for.  13 tokens through 64 gated bf16 experts 2048 -> 1024, six
 // chosen: 61 us, 6.3 TB/s.
 template <class T, bool MX, bool SHARED, bool GATED, int F, int WK, int TT>
 __global__ __launch_bounds__(64 * WK, TT > 1 ? 2 : F > 2 || (GATED && F > 1) ? 3 : 4) void moe_layer_first_kernel(MoeLayerArgs a)

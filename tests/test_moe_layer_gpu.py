@@ -97,6 +97,7 @@ CASES = [
     # E, k, D, F, M
     (8, 2, 1024, 4096, 1), (8, 2, 256, 512, 5), (4, 1, 136, 520, 16), (1, 1, 8, 8, 3), (3, 3, 64, 24, 33), (60, 6, 200, 72, 13), (256, 16, 128, 64, 20),
     (2, 2, 264, 136, 64), (5, 4, 2048, 96, 40), (8, 2, 320, 1000, 65), (4, 2, 96, 160, 150),
+    (32, 6, 1024, 520, 64), (3, 2, 128, 1032, 37),
 ]
 
 
