@@ -541,7 +541,7 @@ typedef struct PimHipMoeLayerDesc {
     const void* const* b2;        /* per expert [d_model]; NULL for none */
     const PimHipMx4Matrix* w1_mx4; /* in place of w1 and w2: the experts' weights in 4 bits */
     const PimHipMx4Matrix* w2_mx4;
-    int64_t d_model, d_ff;        /* multiples of 8 */
+    int64_t d_model, d_ff;        /* d_model a multiple of 8; up to 2^20 */
     int num_experts, top_k;       /* at most 256 and 16 */
     int dtype;                    /* PIMHIP_F16 or PIMHIP_BF16: x, y, the router, the biases and 16-bit weights */
     int act;                      /* a PimHipExpertAct */

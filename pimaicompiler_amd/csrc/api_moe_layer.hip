@@ -20,7 +20,8 @@ namespace
 std::vector<PimHipMoeLayerPlan*> g_moe_layer_plans;
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
-size_t hidden_bytes(const PimHipMoeLayerPlan* p, int tokens) { return round256((size_t)tokens * p->top_k * p->d_ff * 4); }
+int64_t hidden_pitch(const PimHipMoeLayerPlan* p) { return (p->d_ff + 7) / 8 * 8; }
+size_t hidden_bytes(const PimHipMoeLayerPlan* p, int tokens) { return round256((size_t)tokens * p->top_k * hidden_pitch(p) * 4); }
 size_t part_bytes(const PimHipMoeLayerPlan* p, int tokens) { return round256((size_t)tokens * p->top_k * p->d_model * sizeof(float)); }
 
 size_t counter_bytes(const PimHipMoeLayerPlan* p) { return (size_t)(p->d_model + 15) / 16 * sizeof(unsigned int); }
@@ -149,8 +150,9 @@ extern "C" int pimhip_moe_layer_plan_create(PimHipMoeLayerPlan** plan_out, const
     if (d->top_k < 1 || d->top_k > kMoeLayerTopK || d->top_k > d->num_experts)
         return fail(PIMHIP_ERR_UNSUPPORTED, "top_k=%d not in [1, min(%d, num_experts)]", d->top_k, kMoeLayerTopK);
     constexpr int64_t kMost = 1 << 20;
-    if (d->d_model < 8 || d->d_model > kMost || (d->d_model & 7) || d->d_ff < 8 || d->d_ff > kMost || (d->d_ff & 7))
-        return fail(PIMHIP_ERR_UNSUPPORTED, "d_model=%lld and d_ff=%lld must be multiples of 8 in [8, %lld]", (long long)d->d_model, (long long)d->d_ff, (long long)kMost);
+    if (d->d_model < 8 || d->d_model > kMost || (d->d_model & 7) || d->d_ff < 1 || d->d_ff > kMost)
+        return fail(PIMHIP_ERR_UNSUPPORTED, "d_model=%lld must be a multiple of 8, d_model and d_ff=%lld at most %lld", (long long)d->d_model, (long long)d->d_ff,
+                    (long long)kMost);
     if (d->act != PIMHIP_EXPERT_NONE && d->act != PIMHIP_EXPERT_RELU && d->act != PIMHIP_EXPERT_SILU) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "act=%d", d->act);
     const bool mx = d->w1_mx4 || d->w2_mx4;
     if (mx ? (!d->w1_mx4 || !d->w2_mx4) : (!d->w1 || !d->w2))
@@ -257,6 +259,7 @@ extern "C" int pimhip_moe_layer_forward(PimHipMoeLayerPlan* plan, const void* x,
     a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + hidden_bytes(plan, tokens));
     a.counters = reinterpret_cast<unsigned int*>(static_cast<char*>(workspace) + hidden_bytes(plan, tokens) + part_bytes(plan, tokens));
     a.tokens = tokens, a.E = plan->num_experts, a.top_k = plan->top_k, a.d_model = (int)plan->d_model, a.d_ff = (int)plan->d_ff;
+    a.ld_h = (int)hidden_pitch(plan);
     a.ld_x = tokens > 1 ? (int)ld_x : 0;
     a.ld_s1 = (int)plan->ld_s1, a.ld_s2 = (int)plan->ld_s2;
     a.act = plan->act, a.renormalize = plan->renormalize;

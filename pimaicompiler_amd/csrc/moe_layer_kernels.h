@@ -30,11 +30,12 @@ struct MoeLayerArgs {
     void* y;
     int* chosen;      // [tokens][top_k]
     float* share;     // [tokens][top_k]
-    void* h;          // [pairs][2][d_ff]: hidden values rounded to x's type, and what that left over, rounded too
+    void* h;          // [pairs][2][ld_h]: hidden values rounded to x's type, and what that left over, rounded too
     float* part;      // [pairs][d_model]
     unsigned int* counters;  // pairs whose second product is done, for each tile of rows
     int counters_used;
     int tokens, E, top_k, d_model, d_ff, ld_x;
+    int ld_h;         // d_ff filled up to whole groups of eight, with zeros
     int ld_s1, ld_s2;  // pitches of 4-bit weights' scale codes
     int act, renormalize;
 };
@@ -263,12 +264,14 @@ __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPoi
 #pragma unroll
     for (int k = 0; k < F * TT; ++k) {
         const int i = k / TT, j = k % TT, f = f0 + i * 16 + group * 4, column = j * 16 + (lane & 15);
-        if (k % WK != wave || column >= n || f >= a.d_ff) continue;
+        if (k % WK != wave || column >= n || f >= a.ld_h) continue;
         const float4_t g = joined<RT * TT, WK>(lds, k);
         float4_t u = {}, h, left;
         if constexpr (GATED) u = joined<RT * TT, WK>(lds, (F + i) * TT + j);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
+            h[c] = left[c] = 0.0f;
+            if (f + c >= a.d_ff) continue;
             float v = EW::unscale(g[c], p.t1, f + c);
             if (p.b1) v += (float)((const typename T::elem*)p.b1)[f + c];
             if (a.act == PIMHIP_EXPERT_RELU) v = relu_f32(v);
@@ -282,9 +285,9 @@ __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPoi
             h[c] = (float)T::round(v);
             left[c] = fabsf(h[c]) < __builtin_inff() ? v - h[c] : 0.0f;
         }
-        typename T::elem* to = (typename T::elem*)a.h + (int64_t)list[column] * 2 * a.d_ff + f;
-        store4<T>(to, h, 4);  // (d_ff is a multiple of 8)
-        store4<T>(to + a.d_ff, left, 4);
+        typename T::elem* to = (typename T::elem*)a.h + (int64_t)list[column] * 2 * a.ld_h + f;
+        store4<T>(to, h, 4);
+        store4<T>(to + a.ld_h, left, 4);
     }
     __syncthreads();
 }
@@ -316,9 +319,9 @@ __device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPo
     for (int i = 0; i < RT; ++i) rows[i] = EW::rows(p.w2, p.s2, p.t2, a.ld_s2, d0 + i * 16 < a.d_model ? d0 + i * 16 : a.d_model - 1, a.d_model, a.d_ff);
     const typename T::elem* h = (const typename T::elem*)a.h;
     if constexpr (TT == 1)
-        expert_sums<T, MX, SHARED, RT, WK, 1, 1>(rows, a.d_ff, 2 * n, xs, lds, [&](int i) { return h + ((int64_t)list[i / 2] * 2 + i % 2) * a.d_ff; });
+        expert_sums<T, MX, SHARED, RT, WK, 1, 1>(rows, a.d_ff, 2 * n, xs, lds, [&](int i) { return h + ((int64_t)list[i / 2] * 2 + i % 2) * a.ld_h; });
     else
-        expert_sums<T, MX, SHARED, RT, WK, 2, 1>(rows, a.d_ff, n, xs, lds, [&](int i) { return h + ((int64_t)list[i < n ? i : i - n] * 2 + (i < n ? 0 : 1)) * a.d_ff; });
+        expert_sums<T, MX, SHARED, RT, WK, 2, 1>(rows, a.d_ff, n, xs, lds, [&](int i) { return h + ((int64_t)list[i < n ? i : i - n] * 2 + (i < n ? 0 : 1)) * a.ld_h; });
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
         const int d = d0 + i * 16 + group * 4, pair = TT == 1 ? (lane & 15) / 2 : lane & 15;

@@ -55,7 +55,7 @@ struct DenseTile {
     }
 };
 
-// 16-bit weights; rows are whole groups of eight values.  A tile's rows are addressed from its first one, which all lanes share.
+// 16-bit weights, rows of any length at any address of a value.  A tile's rows are addressed from its first one, which all lanes share.
 template <class T>
 struct DenseWeights {
     typedef DenseTile<T> Tile;
@@ -85,14 +85,17 @@ struct DenseWeights {
     {
         const char* p = r.base + (int64_t)unit * (kUnit * 2);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w.v[j] = __builtin_bit_cast(typename T::frag, __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(p + r.at[j])));
+        for (int j = 0; j < 4; ++j) w.v[j] = __builtin_bit_cast(typename T::frag, (uint4_t)__builtin_nontemporal_load(reinterpret_cast<const uint4_any_t*>(p + r.at[j])));
     }
     static __device__ __forceinline__ void load_guarded(Raw& w, const Rows& r, int unit, int K)
     {
         const char* p = r.base + (int64_t)unit * (kUnit * 2);
-        const bool in = unit * kUnit + (int)(threadIdx.x & 15) * 8 < K;
+        const int left = K - unit * kUnit - (int)(threadIdx.x & 15) * 8;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w.v[j] = in ? __builtin_bit_cast(typename T::frag, *reinterpret_cast<const uint4_t*>(p + r.at[j])) : typename T::frag{};
+        for (int j = 0; j < 4; ++j) w.v[j] = left >= 8 ? load8_any<T>(reinterpret_cast<const typename T::elem*>(p + r.at[j])) : typename T::frag{};
+        if (K % 8 != 0 && left > 0 && left < 8)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w.v[j] = load8_guarded<T>(reinterpret_cast<const typename T::elem*>(p + r.at[j]), 0, left);
     }
     static __device__ __forceinline__ void turn(Operands& o, const Raw& w, const Rows&, uint4_t* lds)
     {

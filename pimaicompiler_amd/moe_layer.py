@@ -24,7 +24,7 @@ class MoeLayerPlan:
     renormalize: a token's shares are the softmax over its chosen experts; else over all.
 
     Sums are fp32 and a hidden value is kept in two pieces of the router's type, so y is rounded once; a hidden value beyond that type's range is
-    infinite.  E up to 256, top_k up to 16, d_model and d_ff multiples of 8.  The plan reads the weights where they lie (contiguous copies where they are
+    infinite.  E up to 256, top_k up to 16, d_model a multiple of 8.  The plan reads the weights where they lie (contiguous copies where they are
     not contiguous) and may be used on several streams at a time."""
 
     def __init__(self, router, w1, w2, b1=None, b2=None, top_k=2, act_type="aten::silu", gated=False, renormalize=True, stream=None):

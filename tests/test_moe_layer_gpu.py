@@ -98,6 +98,8 @@ CASES = [
     (8, 2, 1024, 4096, 1), (8, 2, 256, 512, 5), (4, 1, 136, 520, 16), (1, 1, 8, 8, 3), (3, 3, 64, 24, 33), (60, 6, 200, 72, 13), (256, 16, 128, 64, 20),
     (2, 2, 264, 136, 64), (5, 4, 2048, 96, 40), (8, 2, 320, 1000, 65), (4, 2, 96, 160, 150),
     (32, 6, 1024, 520, 64), (3, 2, 128, 1032, 37),
+    # hidden layers of sizes that are multiples of nothing
+    (4, 2, 64, 65, 5), (8, 2, 136, 333, 40), (3, 1, 72, 1, 2), (60, 3, 200, 71, 13), (2, 1, 1160, 1615, 1), (8, 2, 64, 1027, 64),
 ]
 
 
