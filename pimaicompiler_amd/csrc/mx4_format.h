@@ -76,6 +76,19 @@ struct F32 {
     static __device__ __forceinline__ elem round(float v) { return v; }
 };
 
+// A load by a pointer that was itself loaded, which the compiler would take for one that may point to LDS: such loads are counted with LDS
+// accesses, and a wait for those would wait for them too.
+template <class V>
+__device__ __forceinline__ V load_global(const void* p)
+{
+    return *(const __attribute__((address_space(1))) V*)p;
+}
+template <class V>
+__device__ __forceinline__ V load_global_once(const void* p)  // (and is not kept in the caches)
+{
+    return __builtin_nontemporal_load((const __attribute__((address_space(1))) V*)p);
+}
+
 // Eight 16-bit values at any address.
 template <class T>
 __device__ __forceinline__ typename T::frag load8_any(const typename T::elem* p)

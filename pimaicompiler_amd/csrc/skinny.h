@@ -85,14 +85,14 @@ struct DenseWeights {
     {
         const char* p = r.base + (int64_t)unit * (kUnit * 2);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w.v[j] = __builtin_bit_cast(typename T::frag, (uint4_t)__builtin_nontemporal_load(reinterpret_cast<const uint4_any_t*>(p + r.at[j])));
+        for (int j = 0; j < 4; ++j) w.v[j] = __builtin_bit_cast(typename T::frag, (uint4_t)load_global_once<uint4_any_t>(p + r.at[j]));
     }
     static __device__ __forceinline__ void load_guarded(Raw& w, const Rows& r, int unit, int K)
     {
         const char* p = r.base + (int64_t)unit * (kUnit * 2);
         const int left = K - unit * kUnit - (int)(threadIdx.x & 15) * 8;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w.v[j] = left >= 8 ? load8_any<T>(reinterpret_cast<const typename T::elem*>(p + r.at[j])) : typename T::frag{};
+        for (int j = 0; j < 4; ++j) w.v[j] = left >= 8 ? __builtin_bit_cast(typename T::frag, (uint4_t)load_global<uint4_any_t>(p + r.at[j])) : typename T::frag{};
         if (K % 8 != 0 && left > 0 && left < 8)
 #pragma unroll
             for (int j = 0; j < 4; ++j) w.v[j] = load8_guarded<T>(reinterpret_cast<const typename T::elem*>(p + r.at[j]), 0, left);
@@ -148,8 +148,8 @@ struct Mx4Weights {
     {
         const uint8_t* p = r.base + (int64_t)unit * (kUnit / 2);
 #pragma unroll
-        for (int j = 0; j < S; ++j) w.v[j] = __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(p + r.at[j]));
-        w.codes = *reinterpret_cast<const Codes*>(r.codes + (int64_t)unit * kRow + r.codes_at);  // (whole groups of 16 codes a row)
+        for (int j = 0; j < S; ++j) w.v[j] = load_global_once<uint4_t>(p + r.at[j]);
+        w.codes = load_global<Codes>(r.codes + (int64_t)unit * kRow + r.codes_at);  // (whole groups of 16 codes a row)
     }
     static __device__ __forceinline__ void load_guarded(Raw& w, const Rows& r, int unit, int K)
     {
@@ -157,8 +157,8 @@ struct Mx4Weights {
         const uint8_t* p = r.base + (int64_t)unit * (kUnit / 2);
         const bool in = unit * kUnit + lane % kRow * kMxBlock < K;
 #pragma unroll
-        for (int j = 0; j < S; ++j) w.v[j] = in ? *reinterpret_cast<const uint4_t*>(p + r.at[j]) : uint4_t{0, 0, 0, 0};
-        unsigned int codes = *reinterpret_cast<const Codes*>(r.codes + (int64_t)unit * kRow + r.codes_at);
+        for (int j = 0; j < S; ++j) w.v[j] = in ? load_global<uint4_t>(p + r.at[j]) : uint4_t{0, 0, 0, 0};
+        unsigned int codes = load_global<Codes>(r.codes + (int64_t)unit * kRow + r.codes_at);
         // What lies behind the row's last block may be anything: any code but "not a number".
 #pragma unroll
         for (int s = 0; s < S; ++s)
