@@ -95,8 +95,11 @@ int linear(void* out, int64_t ld_out, const void* x, int64_t ld_x, int64_t M, co
         kernel<<<dim3((unsigned)tiles), threads, 0, s>>>((const typename T::elem*)x, w, (const typename T::elem*)bias, (typename T::elem*)out, ld_x, ld_out, M, relu);
         return (int)PIMHIP_OK;
     };
-    if (((w.rows + 255) / 256) * ((M + 127) / 128) > 192) return tiled(mx4_linear_tile_kernel<T, 4, 4, 4, 2>, 256, 128, 512);
-    return tiled(mx4_linear_tile_kernel<T, 4, 2, 2, 2>, 128, 64, 256);
+    if (((w.rows + 255) / 256) * ((M + 127) / 128) > 192) return tiled(mx4_linear_tile_kernel<T, 4, 4, 4, 2, 1>, 256, 128, 512);
+    // Where every tile has a CU to itself, two groups of wavefronts share its k: 512 x 4096 x 4096 (256 tiles) 31 / 33 us with one group, 300 x 300 x
+    // 14000 (15) 94 / 106, 200 x 16384 x 4096 (512) 55 / 48; four groups, 1024 threads: 39 for the first.
+    if (((w.rows + 127) / 128) * ((M + 63) / 64) <= 256) return tiled(mx4_linear_tile_kernel<T, 4, 2, 2, 2, 2>, 128, 64, 512);
+    return tiled(mx4_linear_tile_kernel<T, 4, 2, 2, 2, 1>, 128, 64, 256);
 }
 
 template <class O>

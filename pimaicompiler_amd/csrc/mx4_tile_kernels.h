@@ -21,7 +21,7 @@ __device__ __forceinline__ void tile_at(int id, int tiles_n, int tiles_t, int64_
 
 // ---- x in 16 bits, weights in 4 ----------------------------------------------------------------------------------------------
 // A block has 16 GN WN rows of weights and 16 GT WT tokens, a wavefront of its GN x GT ones WN x WT tiles of 16 x 16.  Steps of 128 values
-// of k.  Weights stay packed in LDS and are converted on the way to the matrix cores: a quarter of the LDS reads of converted ones.  One
+// of k, which KS groups of wavefronts take in turn.  Weights stay packed in LDS and are converted on the way to the matrix cores: a quarter of the LDS reads of converted ones.  One
 // buffer: the next step's operands wait in registers.  Loads take whole runs of a row (16 lanes in 16 rows would be 16 requests), and a
 // row's 16-byte chunks lie in LDS in an order that spreads what 8 lanes read or write over all banks.
 //
@@ -30,8 +30,8 @@ __device__ __forceinline__ void tile_at(int id, int tiles_n, int tiles_t, int64_
 // product, take issue slots, LDS is busy 0.75.  Measured and not better: two steps in registers (the same; three: spills), two buffers
 // (512, but 1500 tokens 73), 128 rows and tokens and four wavefronts (565), 32 x 128 results a wavefront, half the conversions but twice
 // the reads (570), products, reads and conversions told to take turns (594).
-template <class T, int WN, int WT, int GN, int GT>
-__global__ __launch_bounds__(64 * GN * GT) void mx4_linear_tile_kernel(const typename T::elem* x, Mx4View w, const typename T::elem* bias, typename T::elem* out,
+template <class T, int WN, int WT, int GN, int GT, int KS>
+__global__ __launch_bounds__(64 * GN * GT * KS) void mx4_linear_tile_kernel(const typename T::elem* x, Mx4View w, const typename T::elem* bias, typename T::elem* out,
                                                                        int64_t ld_x, int64_t ld_out, int64_t M, int relu)
 {
     constexpr int kThreads = 64 * GN * GT, kN = 16 * GN * WN, kT = 16 * GT * WT, kStep = 128;
@@ -39,10 +39,14 @@ __global__ __launch_bounds__(64 * GN * GT) void mx4_linear_tile_kernel(const typ
     constexpr int kW = kN * 4 / kThreads;    // blocks of weights
     static_assert(kX * kThreads == kT * 16 && kW * kThreads == kN * 4, "whole chunks a thread");
     typedef typename T::frag frag;
-    __shared__ uint4_t xs[kT * 16];  // chunk c of a row at c ^ (row % 8)
-    __shared__ uint4_t ws[kN * 4];   // block c of a row at c ^ (row / 4 % 4)
-    __shared__ float ss[4][kN];
-    const int tid = threadIdx.x, lane = tid & 63, wave = wave_in_block(), group = lane >> 4, row = lane & 15;
+    // (for each of the KS groups of wavefronts, which take steps of k in turn)
+    __shared__ uint4_t xs_[KS][kT * 16];  // chunk c of a row at c ^ (row % 8)
+    __shared__ uint4_t ws_[KS][kN * 4];   // block c of a row at c ^ (row / 4 % 4)
+    __shared__ float ss_[KS][4][kN];
+    const int share = KS == 1 ? 0 : wave_in_block() / (GN * GT), wave = KS == 1 ? wave_in_block() : wave_in_block() % (GN * GT);
+    uint4_t *xs = xs_[share], *ws = ws_[share];
+    auto ss = ss_[share];
+    const int tid = (int)threadIdx.x - share * kThreads, lane = tid & 63, group = lane >> 4, row = lane & 15;
     const int wn = wave % GN * WN, wt = wave / GN * WT;
     int64_t tile_n, tile_t;
     tile_at(blockIdx.x, (int)((w.rows + kN - 1) / kN), (int)((M + kT - 1) / kT), tile_n, tile_t);
@@ -91,22 +95,26 @@ __global__ __launch_bounds__(64 * GN * GT) void mx4_linear_tile_kernel(const typ
     };
     float4_t acc[WN][WT] = {};
     const int steps = (int)((K + kStep - 1) / kStep);
-    fetch(0);
-    for (int s = 0; s < steps; ++s) {
-        if (s) __syncthreads();
+    if (share < steps) fetch(share);
+    for (int s0 = 0; s0 < steps; s0 += KS) {
+        const int s = s0 + share;
+        if (s0) __syncthreads();
+        if (s < steps) {
 #pragma unroll
-        for (int i = 0; i < kX; ++i) {
-            const int r = (tid + i * kThreads) / 16;
-            xs[r * 16 + (xc ^ (r & 7))] = __builtin_bit_cast(uint4_t, xv[i]);
-        }
+            for (int i = 0; i < kX; ++i) {
+                const int r = (tid + i * kThreads) / 16;
+                xs[r * 16 + (xc ^ (r & 7))] = __builtin_bit_cast(uint4_t, xv[i]);
+            }
 #pragma unroll
-        for (int i = 0; i < kW; ++i) {
-            const int r = (tid + i * kThreads) / 4;
-            ws[r * 4 + (wc ^ (r / 4 & 3))] = wv[i];
-            ss[wc][r] = T::scale(code[i], top[i]);
+            for (int i = 0; i < kW; ++i) {
+                const int r = (tid + i * kThreads) / 4;
+                ws[r * 4 + (wc ^ (r / 4 & 3))] = wv[i];
+                ss[wc][r] = T::scale(code[i], top[i]);
+            }
         }
         __syncthreads();
-        if (s + 1 < steps) fetch(s + 1);
+        if (s >= steps) continue;
+        if (s + KS < steps) fetch(s + KS);
         uint4_t wq[WN];
         float scale[WN];
 #pragma unroll
@@ -130,6 +138,26 @@ __global__ __launch_bounds__(64 * GN * GT) void mx4_linear_tile_kernel(const typ
                 for (int j = 0; j < WT; ++j) acc[i][j] = T::mfma(wf, xf[j], acc[i][j]);
             }
         }
+    }
+    if constexpr (KS > 1) {
+        // The groups' sums, in their order.
+        static_assert((KS - 1) * GN * GT * WN * WT * 64 <= KS * kT * 16, "the sums fit where the tokens were");
+        float4_t* sums = reinterpret_cast<float4_t*>(xs_);
+        __syncthreads();
+        if (share > 0) {
+#pragma unroll
+            for (int i = 0; i < WN; ++i)
+#pragma unroll
+                for (int j = 0; j < WT; ++j) sums[((((share - 1) * GN * GT + wave) * WN + i) * WT + j) * 64 + lane] = acc[i][j];
+        }
+        __syncthreads();
+        if (share > 0) return;
+#pragma unroll
+        for (int k = 0; k < KS - 1; ++k)
+#pragma unroll
+            for (int i = 0; i < WN; ++i)
+#pragma unroll
+                for (int j = 0; j < WT; ++j) acc[i][j] += sums[(((k * GN * GT + wave) * WN + i) * WT + j) * 64 + lane];
     }
 #pragma unroll
     for (int i = 0; i < WN; ++i) {

@@ -175,7 +175,8 @@ def test_matmul(ops, M, N, K, dtype):
 
 
 # Many tiles: more bands of tokens than one, steps of k that begin in the middle and go round, K that ends in every part of a step.
-@pytest.mark.parametrize("M,N,K", [(1180, 1050, 96), (300, 520, 1536), (257, 129, 2080), (65, 136, 1400), (640, 127, 512), (129, 260, 250), (70, 1029, 800),
+@pytest.mark.parametrize("M,N,K", [(1180, 1050, 96), (300, 520, 1536), (257, 129, 2080), (65, 136, 1400), (640, 127, 512), (129, 260, 250), (70, 1029, 800), (66, 100, 200), (200, 140, 1300),
+                                   (600, 2100, 416),
                                    (40, 12300, 64), (3, 16400, 160), (16, 16385, 33)])
 def test_products_of_many_tiles(ops, M, N, K):
     g = torch.Generator().manual_seed(M + N + K)
