@@ -38,7 +38,7 @@ def token_log_probs(logits, tokens=None, top=0, stream=None):
         if tokens.shape != lead or tokens.device != logits.device:
             raise NNRuntimeException(f"tokens must be {tuple(lead)} on {logits.device}, got {tuple(tokens.shape)} on {tokens.device}")
     _ensure_init(logits)
-    with _Launch(logits.device, stream) as handle:
+    with _Launch(logits.device, stream, logits, tokens) as handle:
         x, ld = _rows_of(logits)
         if tokens is not None:
             tokens = tokens.contiguous()

@@ -111,7 +111,7 @@ class MoeLayerPlan:
         if x.dim() < 1 or x.size(-1) != self.d_model or x.device != self.device:
             raise NNRuntimeException(f"x must be [.., {self.d_model}] on {self.device}, got {tuple(x.shape)} on {x.device}")
         lib = L.load()
-        with _Launch(self.device, stream) as handle:
+        with _Launch(self.device, stream, x) as handle:
             x2, ld = _rows_of(x)
             M, k = x2.size(0), self.top_k
             y = torch.empty(x.shape, dtype=self.dtype, device=self.device)

@@ -57,7 +57,7 @@ class Mx4Tensor:
         if packed.device != scales.device:
             raise NNRuntimeException(f"packed is on {packed.device}, scales on {scales.device}")
         _ensure_init(packed)
-        with _Launch(packed.device, stream) as handle:
+        with _Launch(packed.device, stream, packed, scales) as handle:
             packed = packed.contiguous()
             if packed.data_ptr() % 16:
                 packed = packed.clone()
@@ -91,6 +91,9 @@ class Mx4Tensor:
         self._hold(torch.empty((rows, blocks * 16), dtype=torch.uint8, device=device),
                    torch.empty((rows, -(-blocks // 16) * 16), dtype=torch.uint8, device=device), torch.empty(rows, dtype=torch.uint8, device=device), shape)
         return self
+
+    def _tensors(self):
+        return self.packed, self.scales, self.tops
 
     @property
     def _c(self):
@@ -126,7 +129,7 @@ def mx4_quantize(x, stream=None):
     if x.dim() < 1 or x.size(-1) < 1:
         raise NNRuntimeException("x must have at least one dimension, the last of at least one value")
     _ensure_init(x)
-    with _Launch(x.device, stream) as handle:
+    with _Launch(x.device, stream, x) as handle:
         x2, ld = _rows_of(x)
         q = Mx4Tensor._empty(x.shape, x.device)
         _check(L.load().pimhip_mx4_quantize(q._c, x2.data_ptr(), _CODES[x.dtype], ld, handle))
@@ -143,7 +146,7 @@ def mx4_dequantize(q, dtype=torch.float16, stream=None):
     if out is not None:
         return _result(out)
     _ensure_init(q.packed)
-    with _Launch(q.device, stream) as handle:
+    with _Launch(q.device, stream, *q._tensors()) as handle:
         out = torch.empty(q.shape, dtype=dtype, device=q.device)
         _check(L.load().pimhip_mx4_dequantize(out.data_ptr(), _CODES[dtype], q.shape[-1], q._c, handle))
     return out
@@ -171,7 +174,7 @@ def mx4_linear(x, weight, bias=None, act_type="none", stream=None):
         if t is not None and t.device != x.device:
             raise NNRuntimeException(f"x is on {x.device}, weight or bias on {t.device}")
     _ensure_init(x)
-    with _Launch(x.device, stream) as handle:
+    with _Launch(x.device, stream, x, bias, *weight._tensors()) as handle:
         x2, ld = _rows_of(x)
         if bias is not None:
             bias = bias.contiguous()
@@ -196,7 +199,7 @@ def mx4_matmul(a, b, dtype=torch.float16, stream=None):
         return _result(out)
     _ensure_init(a.packed)
     N = b.shape[0]
-    with _Launch(a.device, stream) as handle:
+    with _Launch(a.device, stream, *a._tensors(), *b._tensors()) as handle:
         out = torch.empty((*a.shape[:-1], N), dtype=dtype, device=a.device)
         _check(L.load().pimhip_mx4_matmul(out.data_ptr(), N, _CODES[dtype], a._c, b._c, handle))
     return out

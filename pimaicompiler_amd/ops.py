@@ -153,12 +153,13 @@ def _stream_arg(stream):
 
 
 class _Launch:
-    """`with _Launch(device, stream) as handle`: the device is the current one inside, `stream` (None, a torch stream or an integer
+    """`with _Launch(device, stream, *tensors) as handle`: the device is the current one inside, `stream` (None, a torch stream or an integer
     handle) torch's current stream, and `handle` its hipStream_t.  What a call allocates inside belongs to the stream it
-    launches on, also where that is not the caller's current one."""
+    launches on, also where that is not the caller's current one; the memory of `tensors`, which the call reads, is not given to others
+    before a stream that was asked for is done with it."""
 
-    def __init__(self, device, stream):
-        self._device = device
+    def __init__(self, device, stream, *tensors):
+        self._device, self._tensors = device, tensors
         if stream is None:
             self._stream = None
         elif isinstance(stream, torch.cuda.Stream):
@@ -176,6 +177,9 @@ class _Launch:
         self._entered.enter_context(torch.cuda.device(self._device))
         if self._stream is not None:
             self._entered.enter_context(torch.cuda.stream(self._stream))
+            for t in self._tensors:
+                if t is not None:
+                    t.record_stream(self._stream)
         return torch.cuda.current_stream().cuda_stream
 
     def __exit__(self, *exc):

@@ -97,3 +97,33 @@ def test_nothing_to_do(ops):
     step = Step(ops, torch.float16)
     out = step(torch.empty(0, step.D, dtype=torch.float16, device=DEV), torch.empty(0, dtype=torch.int64, device=DEV))
     assert out[0].shape == (0, 256) and out[2].shape == (0, 2) and out[4].shape == (0, 4099) and out[5].shape == (0,) and out[8].shape == (0, 5)
+
+
+def test_inputs_freed_right_after_a_call_on_another_stream(ops):
+    """Their memory is not handed out while that stream has yet to read it."""
+    step = Step(ops, torch.float16)
+    side = torch.cuda.Stream()
+    x0, t0 = step.x(64, 1).to(DEV), torch.arange(64, device=DEV)
+    h0 = ops.mx4_linear(x0, step.layer)
+    l0 = ops.mx4_linear(h0, step.head)
+    want = [h0, *ops.token_log_probs(l0, t0, top=3), *step.moe.plan.forward(x0), ops.mx4_quantize(x0).packed, ops.mx4_matmul(ops.mx4_quantize(x0), step.layer)]
+    busy = torch.randn(4096, 4096, device=DEV)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(8):
+            busy = torch.sin(busy)   # (the calls below wait behind this)
+    got = []
+    x, q = x0.clone(), ops.mx4_quantize(x0)
+    logits, tokens = l0.clone(), t0.clone()
+    side.wait_stream(torch.cuda.current_stream())
+    got.append(ops.mx4_linear(x, step.layer, stream=side))
+    got += ops.token_log_probs(logits, tokens, top=3, stream=side)
+    got += step.moe.plan.forward(x, stream=side)
+    got.append(ops.mx4_quantize(x, stream=side).packed)
+    got.append(ops.mx4_matmul(q, step.layer, stream=side))
+    sizes = [(t.shape, t.dtype) for t in (x, q.packed, q.scales, q.tops, logits, tokens)]
+    del x, q, logits, tokens
+    for shape, dtype in sizes:
+        torch.empty(shape, dtype=dtype, device=DEV).fill_(1)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
