@@ -188,7 +188,7 @@ struct ExpertWeights<T, true, TT> {
 };
 
 // What a block of the experts' products has in LDS: the tokens that chose its expert, what its wavefronts turn operands in (and then
-// their sums), and, SHARED, in the launch's dynamic part the values of up to 16 columns.
+// their sums), and, SHARED, in the launch's dynamic part the values of its columns.
 template <class T, bool MX, bool SHARED, int RT, int WK, int TT, int PARTS>
 struct ExpertLds {
     typedef typename ExpertWeights<T, MX, TT>::W W;
