@@ -24,7 +24,9 @@ int64_t hidden_pitch(const PimHipMoeLayerPlan* p) { return (p->d_ff + 7) / 8 * 8
 size_t hidden_bytes(const PimHipMoeLayerPlan* p, int tokens) { return round256((size_t)tokens * p->top_k * hidden_pitch(p) * 4); }
 size_t part_bytes(const PimHipMoeLayerPlan* p, int tokens) { return round256((size_t)tokens * p->top_k * p->d_model * sizeof(float)); }
 
-size_t counter_bytes(const PimHipMoeLayerPlan* p) { return (size_t)(p->d_model + 15) / 16 * sizeof(unsigned int); }
+size_t counter_bytes(const PimHipMoeLayerPlan* p) { return round256((size_t)(p->d_model + 15) / 16 * sizeof(unsigned int)); }
+int64_t most_pitch(const PimHipMoeLayerPlan* p) { return (p->d_ff + 255) / 256 * 16; }
+size_t most_bytes(const PimHipMoeLayerPlan* p, int tokens) { return (size_t)tokens * p->top_k * most_pitch(p); }
 
 bool known_locked(const PimHipMoeLayerPlan* plan)
 {
@@ -59,32 +61,37 @@ int destroy_moe_layer_plan_locked(PimHipMoeLayerPlan* plan)
     return PIMHIP_OK;
 }
 
-// LDS that staging the columns of a product over K values takes, in bytes; each token makes `each` of them.
+// LDS that staging `columns` of a product over K values takes, in bytes (weights of T's units).
 template <class T, bool MX>
-unsigned int shared_bytes(const MoeLayerArgs& a, int K, int each)
+unsigned int shared_bytes(int columns, int K)
 {
-    return (unsigned int)((a.tokens < 16 ? a.tokens : 16) * each * SharedTokens<T>::pitch(K, ExpertWeights<T, MX, 1>::W::kUnit) * 16);
+    return (unsigned int)(columns * SharedTokens<T>::pitch(K, ExpertWeights<T, MX, 1>::W::kUnit) * 16);
 }
 
 template <class T, bool MX, bool SHARED, bool GATED, int F, int TT>
-void launch_first(const MoeLayerArgs& a, hipStream_t s)
+void launch_first(const MoeLayerArgs& a, unsigned int bytes, hipStream_t s)
 {
     constexpr int WK = 4;
     moe_layer_first_kernel<T, MX, SHARED, GATED, F, WK, TT>
-        <<<dim3((unsigned)((a.d_ff + 16 * F - 1) / (16 * F)), (unsigned)a.E, (unsigned)((a.tokens + 16 * TT - 1) / (16 * TT))), 64 * WK, SHARED ? shared_bytes<T, MX>(a, a.d_model, 1) : 0, s>>>(a);
+        <<<dim3((unsigned)((a.d_ff + 16 * F - 1) / (16 * F)), (unsigned)a.E, (unsigned)((a.tokens + 16 * TT - 1) / (16 * TT))), 64 * WK, SHARED ? bytes : 0, s>>>(a);
 }
 
-template <class T, bool MX, bool SHARED, int RT, int WK, int TT>
-void launch_second(const MoeLayerArgs& a, hipStream_t s)
+// `most`: LDS that staged columns may take.
+template <class T, bool MX, int RT, int WK, bool FEW>
+void launch_second(const MoeLayerArgs& a, unsigned int most, hipStream_t s)
 {
-    moe_layer_second_kernel<T, MX, SHARED, RT, WK, TT>
-        <<<dim3((unsigned)((a.d_model + 16 * RT - 1) / (16 * RT)), (unsigned)a.E, (unsigned)((a.tokens + 8 * TT - 1) / (8 * TT))), 64 * WK, SHARED ? shared_bytes<T, MX>(a, a.d_ff, 2) : 0, s>>>(a);
+    typedef SecondColumns<T, MX, true, FEW> C;
+    const dim3 grid((unsigned)((a.d_model + 16 * RT - 1) / (16 * RT)), (unsigned)a.E, (unsigned)((a.tokens + C::kPairs - 1) / C::kPairs));
+    const unsigned int bytes = shared_bytes<typename C::H, MX>((a.tokens < C::kPairs ? a.tokens : C::kPairs) * C::kPieces, a.d_ff);
+    if (bytes <= most)
+        moe_layer_second_kernel<T, MX, true, RT, WK, FEW><<<grid, 64 * WK, bytes, s>>>(a);
+    else
+        moe_layer_second_kernel<T, MX, false, RT, WK, FEW><<<grid, 64 * WK, 0, s>>>(a);
 }
 
 template <class T, bool MX>
 void launch(const PimHipMoeLayerPlan* p, MoeLayerArgs& a, hipStream_t s)
 {
-    a.counters_used = (a.d_model + 15) / 16;
     moe_layer_router_kernel<T><<<dim3((unsigned)a.tokens), kRouterThreads, 0, s>>>(a);
     // Tokens are staged as a whole where there are one or two, or where an expert has many and 16 of them leave a CU room for three
     // blocks.
@@ -92,41 +99,41 @@ void launch(const PimHipMoeLayerPlan* p, MoeLayerArgs& a, hipStream_t s)
     const unsigned int most = many ? 40 << 10 : a.tokens <= 2 ? 20 << 10 : 0;
     // With many tokens a block has twice the rows: their values are read, and turned or staged, half as often (64 tokens through 8 gated 4-bit
     // experts 1024 -> 4096: 29.8 -> 20.8 us; one token through 2 of 8 experts 1024 -> 4096 in fp16, where blocks are few: 6.1 -> 7.9).
+    const unsigned int staged = shared_bytes<T, MX>(a.tokens < 16 ? a.tokens : 16, a.d_model);
     auto first = [&](auto shared) {
         constexpr bool S = decltype(shared)::value;
         if (many)
-            p->gated ? launch_first<T, MX, S, true, 2, 1>(a, s) : launch_first<T, MX, S, false, 4, 1>(a, s);
+            p->gated ? launch_first<T, MX, S, true, 2, 1>(a, staged, s) : launch_first<T, MX, S, false, 4, 1>(a, staged, s);
         else
-            p->gated ? launch_first<T, MX, S, true, 1, 1>(a, s) : launch_first<T, MX, S, false, 2, 1>(a, s);
+            p->gated ? launch_first<T, MX, S, true, 1, 1>(a, staged, s) : launch_first<T, MX, S, false, 2, 1>(a, staged, s);
     };
     // Where experts have more than 16 pairs, which some have from 10 on the average on, 32 of them a block read their weights half as often.
     // In us a call, 32 / 16 pairs a block, 64 tokens through 8 experts 1024 -> 4096, two chosen: gated in 4 bits 41.3 / 44.7, gated fp16 64 / 79, fp16
     // 51 / 54; 16 tokens through both of 2 experts 512 -> 1024, which have 16 pairs at the most, 17.9 / 15.9.
     const int pairs = a.tokens * a.top_k;
     if (many && pairs > 10 * a.E)
-        p->gated ? launch_first<T, MX, false, true, 2, 2>(a, s) : launch_first<T, MX, false, false, 4, 2>(a, s);
+        p->gated ? launch_first<T, MX, false, true, 2, 2>(a, 0, s) : launch_first<T, MX, false, false, 4, 2>(a, 0, s);
     else
-        shared_bytes<T, MX>(a, a.d_model, 1) <= most ? first(std::true_type{}) : first(std::false_type{});
+        staged <= most ? first(std::true_type{}) : first(std::false_type{});
     // Blocks of the second product that have something to read.  Where they fill the card several times over a block has two tiles of
     // rows and four wavefronts, else eight wavefronts share its long k.  Where experts have more than 8 pairs, which some have from 5 on the
     // average on, 16 of them a block read their weights half as often.  In us a call, 16 / 8 pairs a block: 64 tokens through 8 gated 4-bit experts 1024
     // -> 4096, two chosen (16 pairs an expert) 44.6 / 46.6, 32 tokens (8) 32.4 / 30.9, 17 tokens (4) 31 / 26; 64 tokens through 64 gated bf16 experts
     // 2048 -> 1024, six chosen (6) 178 / 191.
     const int64_t blocks = (int64_t)((a.d_model + 15) / 16) * (a.E < pairs ? a.E : pairs);
-    const bool shared = shared_bytes<T, MX>(a, a.d_ff, 2) <= most;
     if (pairs > 5 * a.E) {
         if constexpr (!MX) {
             // (16-bit weights are four times the bytes: 64 tokens through 8 fp16 experts 1024 -> 4096 46.5 with eight wavefronts and a tile, 51 with two
             // tiles and four; in 4 bits 46.0 / 41.3, the values being turned for each tile of rows)
-            if (blocks < 2048) return shared ? launch_second<T, MX, true, 1, 8, 2>(a, s) : launch_second<T, MX, false, 1, 8, 2>(a, s);
+            if (blocks < 2048) return launch_second<T, MX, 1, 8, false>(a, most, s);
         }
-        shared ? launch_second<T, MX, true, 2, 4, 2>(a, s) : launch_second<T, MX, false, 2, 4, 2>(a, s);
+        launch_second<T, MX, 2, 4, false>(a, most, s);
     } else if (blocks >= 2048)
-        shared ? launch_second<T, MX, true, 2, 4, 1>(a, s) : launch_second<T, MX, false, 2, 4, 1>(a, s);
+        launch_second<T, MX, 2, 4, true>(a, most, s);
     else if (many)
-        shared ? launch_second<T, MX, true, 2, 8, 1>(a, s) : launch_second<T, MX, false, 2, 8, 1>(a, s);
+        launch_second<T, MX, 2, 8, true>(a, most, s);
     else
-        shared ? launch_second<T, MX, true, 1, 8, 1>(a, s) : launch_second<T, MX, false, 1, 8, 1>(a, s);
+        launch_second<T, MX, 1, 8, true>(a, most, s);
 }
 }  // namespace
 
@@ -227,7 +234,7 @@ extern "C" int pimhip_moe_layer_workspace_bytes(const PimHipMoeLayerPlan* plan, 
     const int rc = check_plan(plan);
     if (rc != PIMHIP_OK) return rc;
     if (tokens < 0 || tokens > kMoeLayerTokens) return fail(PIMHIP_ERR_UNSUPPORTED, "tokens=%d not in [0, %d]", tokens, kMoeLayerTokens);
-    *bytes = hidden_bytes(plan, tokens) + part_bytes(plan, tokens) + counter_bytes(plan);
+    *bytes = hidden_bytes(plan, tokens) + part_bytes(plan, tokens) + counter_bytes(plan) + most_bytes(plan, tokens);
     return PIMHIP_OK;
 }
 
@@ -255,11 +262,13 @@ extern "C" int pimhip_moe_layer_forward(PimHipMoeLayerPlan* plan, const void* x,
     a.experts = plan->experts;
     a.x = x, a.router_w = plan->router_w, a.router_b = plan->router_b, a.y = y;
     a.chosen = experts, a.share = shares;
-    a.h = workspace;
+    a.h = static_cast<float*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + hidden_bytes(plan, tokens));
     a.counters = reinterpret_cast<unsigned int*>(static_cast<char*>(workspace) + hidden_bytes(plan, tokens) + part_bytes(plan, tokens));
     a.tokens = tokens, a.E = plan->num_experts, a.top_k = plan->top_k, a.d_model = (int)plan->d_model, a.d_ff = (int)plan->d_ff;
-    a.ld_h = (int)hidden_pitch(plan);
+    a.h_most = reinterpret_cast<uint8_t*>(a.counters) + counter_bytes(plan);
+    a.counters_used = (a.d_model + 15) / 16;
+    a.ld_h = (int)hidden_pitch(plan), a.ld_most = (int)most_pitch(plan);
     a.ld_x = tokens > 1 ? (int)ld_x : 0;
     a.ld_s1 = (int)plan->ld_s1, a.ld_s2 = (int)plan->ld_s2;
     a.act = plan->act, a.renormalize = plan->renormalize;

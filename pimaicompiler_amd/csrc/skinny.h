@@ -185,11 +185,13 @@ struct Mx4Weights {
 };
 
 // The tokens of a product, loaded and turned like weights by each wavefront.  WHOLE: their rows are whole groups of eight values.
+// (raws: how many loads of a step the tiles of 16 columns make.)
 template <class T, bool WHOLE>
 struct TurnedTokens {
     typedef DenseTile<T> Tile;
     typedef typename Tile::Raw Raw;
     static constexpr int kLds = Tile::kLds;
+    static constexpr int raws(int tiles) { return tiles; }
     struct Rows {
         const typename T::elem* p[4];  // the lane's four rows, at its chunk
     };
@@ -219,7 +221,7 @@ struct TurnedTokens {
                 w.v[j] = load8_guarded<T>(r.p[j] - chunk * 8, (int64_t)step * kSkinnyStep + chunk * 8, K);
         }
     }
-    static __device__ __forceinline__ void turn(typename T::frag (&f)[4], const Raw& w, const Rows&, int, uint4_t* lds)
+    static __device__ __forceinline__ void turn(typename T::frag (&f)[4], Raw& w, const Rows&, int, int, uint4_t* lds)
     {
         Tile::to_lds(w, lds);
         wave_lds_order();
@@ -237,6 +239,7 @@ struct SharedTokens {
         const uint4_t* p;
     };
     static constexpr int kLds = 0;
+    static constexpr int raws(int tiles) { return tiles; }
     // 16-byte words of a token, of K values filled up to whole units.
     static __host__ __device__ constexpr int pitch(int K, int unit) { return (K + unit - 1) / unit * (unit / 8) + 1; }
     static __device__ __forceinline__ Rows rows(const uint4_t* xs, int token, int pitch) { return {xs + token * pitch + ((threadIdx.x & 63) >> 4) * 4}; }
@@ -251,7 +254,7 @@ struct SharedTokens {
     }
     static __device__ __forceinline__ void load(Raw&, const Rows&, int) {}
     static __device__ __forceinline__ void load_guarded(Raw&, const Rows&, int, int) {}
-    static __device__ __forceinline__ void turn(typename T::frag (&f)[4], const Raw&, const Rows& r, int step, uint4_t*)
+    static __device__ __forceinline__ void turn(typename T::frag (&f)[4], Raw&, const Rows& r, int step, int, uint4_t*)
     {
 #pragma unroll
         for (int o = 0; o < 4; ++o) f[o] = __builtin_bit_cast(typename T::frag, r.p[step * (kSkinnyStep / 8) + o]);
@@ -265,25 +268,25 @@ constexpr int kSkinnyLds = W::kLds + X::kLds;
 // acc[i][j] += 16 rows i x 16 tokens j over units first, first + stride, ... of K.  `lds`: this wavefront's kSkinnyLds words.
 // ready() is called once, behind the first loads of weights: there a block stages what its wavefronts share.
 template <class T, class W, class X, int RT, int TT, int U, class R>
-__device__ __forceinline__ void skinny_sum(float4_t (&acc)[RT][TT], const typename W::Rows (&w)[RT], const typename X::Rows (&x)[TT], int K, int first, int stride,
+__device__ __forceinline__ void skinny_sum(float4_t (&acc)[RT][TT], const typename W::Rows (&w)[RT], const typename X::Rows (&x)[X::raws(TT)], int K, int first, int stride,
                                            uint4_t* lds, R ready)
 {
     typedef typename T::frag frag;
-    constexpr int S = W::kUnit / kSkinnyStep;  // steps of a unit
+    constexpr int S = W::kUnit / kSkinnyStep, XR = X::raws(TT);  // steps of a unit
     const int whole = K / W::kUnit;
     const int mine = first < whole ? (whole - first + stride - 1) / stride : 0;  // this wavefront's whole units
     typename W::Raw wv[U][RT];
-    typename X::Raw xv[U][S][TT];
+    typename X::Raw xv[U][S][XR];
     auto ask = [&](int u, int n) {
         const int unit = first + n * stride;
 #pragma unroll
         for (int s = 0; s < S; ++s)
 #pragma unroll
-            for (int j = 0; j < TT; ++j) X::load(xv[u][s][j], x[j], unit * S + s);
+            for (int j = 0; j < XR; ++j) X::load(xv[u][s][j], x[j], unit * S + s);
 #pragma unroll
         for (int i = 0; i < RT; ++i) W::load(wv[u][i], w[i], unit);
     };
-    auto products = [&](const typename W::Raw(&wr)[RT], const typename X::Raw(&xr)[S][TT], int unit) {
+    auto products = [&](const typename W::Raw(&wr)[RT], typename X::Raw(&xr)[S][XR], int unit) {
         typename W::Operands a[RT];
 #pragma unroll
         for (int i = 0; i < RT; ++i) W::turn(a[i], wr[i], w[i], lds);
@@ -292,7 +295,7 @@ __device__ __forceinline__ void skinny_sum(float4_t (&acc)[RT][TT], const typena
 #pragma unroll
             for (int j = 0; j < TT; ++j) {
                 frag f[4];
-                X::turn(f, xr[s][j], x[j], unit * S + s, lds + W::kLds);
+                X::turn(f, xr[s][j % XR], x[j % XR], unit * S + s, j, lds + W::kLds);
 #pragma unroll
                 for (int o = 0; o < 4; ++o)
 #pragma unroll
@@ -327,7 +330,7 @@ __device__ __forceinline__ void skinny_sum(float4_t (&acc)[RT][TT], const typena
 #pragma unroll
         for (int s = 0; s < S; ++s)
 #pragma unroll
-            for (int j = 0; j < TT; ++j) X::load_guarded(xv[0][s][j], x[j], whole * S + s, K);
+            for (int j = 0; j < XR; ++j) X::load_guarded(xv[0][s][j], x[j], whole * S + s, K);
         products(wv[0], xv[0], whole);
     }
 }

@@ -23,8 +23,7 @@ class MoeLayerPlan:
     (and b1[e] [2 d_ff]), the gate's rows first, and hidden = act(gate) * value.  act_type "none", "aten::relu" or "aten::silu".
     renormalize: a token's shares are the softmax over its chosen experts; else over all.
 
-    Sums are fp32 and a hidden value is kept in two pieces of the router's type, so y is rounded once; a hidden value beyond that type's range is
-    infinite.  E up to 256, top_k up to 16, d_model a multiple of 8.  The plan reads the weights where they lie (contiguous copies where they are
+    Sums and hidden values are fp32, so y is rounded once.  E up to 256, top_k up to 16, d_model a multiple of 8.  The plan reads the weights where they lie (contiguous copies where they are
     not contiguous) and may be used on several streams at a time."""
 
     def __init__(self, router, w1, w2, b1=None, b2=None, top_k=2, act_type="aten::silu", gated=False, renormalize=True, stream=None):
