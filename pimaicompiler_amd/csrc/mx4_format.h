@@ -42,8 +42,9 @@ struct F16 {
     static __device__ __forceinline__ float4_t mfma(const frag a, const frag b, const float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ float scale(unsigned int code, int top)
     {
+        // (no code is above its row's top, and 254 stands for one that was written there later: 255 is the exponent of infinities and NaN)
         const int e = (int)code - top + 127 + kLift;
-        return __builtin_bit_cast(float, code == kMxNan ? 0x7fc00000u : (unsigned int)(e > 0 ? e : 0) << 23);
+        return __builtin_bit_cast(float, code == kMxNan ? 0x7fc00000u : (unsigned int)(e < 0 ? 0 : e > 254 ? 254 : e) << 23);
     }
     static __device__ __forceinline__ float unscale(float v, int top) { return __builtin_amdgcn_ldexpf(v, top - 127 - kLift); }
     static __device__ __forceinline__ frag from_mx4(unsigned int d, float s)

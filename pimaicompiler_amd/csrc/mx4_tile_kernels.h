@@ -86,7 +86,7 @@ __global__ __launch_bounds__(64 * GN * GT * KS) void mx4_linear_tile_kernel(cons
 #pragma unroll
         for (int i = 0; i < kW; ++i) {
             wv[i] = uint4_t{0, 0, 0, 0};
-            code[i] = 127;
+            code[i] = 0;  // (above no row's top)
             if (step * 4 + wc < blocks) {
                 wv[i] = *reinterpret_cast<const uint4_t*>(wp[i] + (int64_t)step * (4 * kMxBlockBytes));
                 code[i] = sp[i][step * 4];

@@ -159,10 +159,10 @@ struct Mx4Weights {
 #pragma unroll
         for (int j = 0; j < S; ++j) w.v[j] = in ? load_global<uint4_t>(p + r.at[j]) : uint4_t{0, 0, 0, 0};
         unsigned int codes = load_global<Codes>(r.codes + (int64_t)unit * kRow + r.codes_at);
-        // What lies behind the row's last block may be anything: any code but "not a number".
+        // What lies behind the row's last block may be anything: 0, the one code that is above no row's top.
 #pragma unroll
         for (int s = 0; s < S; ++s)
-            if (unit * kUnit + ((lane & 3) * S + s) * kMxBlock >= K) codes = (codes & ~(255u << (8 * s))) | (127u << (8 * s));
+            if (unit * kUnit + ((lane & 3) * S + s) * kMxBlock >= K) codes &= ~(255u << (8 * s));
         w.codes = (Codes)codes;
     }
     static __device__ __forceinline__ int place(int row, int chunk) { return row * kRow + (chunk ^ (S == 2 ? row & 7 : row / 4 & 3)); }
