@@ -92,6 +92,17 @@ class Mx4Tensor:
                    torch.empty((rows, -(-blocks // 16) * 16), dtype=torch.uint8, device=device), torch.empty(rows, dtype=torch.uint8, device=device), shape)
         return self
 
+    @classmethod
+    def _again(cls, packed, scales, in_features, shape):
+        self = cls(packed, scales, in_features)
+        self.shape = torch.Size(shape)
+        return self
+
+    def __reduce__(self):
+        """A deep copy, or one read from a file, is made of its own tensors: what the native calls read it through holds addresses."""
+        K = self.shape[-1]
+        return Mx4Tensor._again, (self.packed, self.scales[:, :-(-K // BLOCK)], K, tuple(self.shape))
+
     def _tensors(self):
         return self.packed, self.scales, self.tops
 

@@ -27,3 +27,17 @@ def test_the_c_interface_needs_an_initialised_device():
 
 def test_the_struct_of_the_binding_is_the_header_s():
     assert ctypes.sizeof(L.Mx4Matrix) == 48 and [n for n, _ in L.Mx4Matrix._fields_] == ["packed", "scales", "tops", "rows", "cols", "ld_scales"]
+
+
+def test_a_copy_takes_no_address_along():
+    """What a matrix is read through holds the addresses of its tensors: a deep copy and one that was pickled are made anew, which needs the GPU."""
+    import copy
+    import pickle
+    packed, scales, tops = (torch.zeros(2, n, dtype=torch.uint8) for n in (16, 16, 1))
+    kept = L.Mx4Matrix(packed.data_ptr(), scales.data_ptr(), tops.data_ptr(), 2, 32, 16)
+    q = P.Mx4Tensor.__new__(P.Mx4Tensor)   # as the native call leaves it: the description as bytes, and where they are
+    q.packed, q.scales, q.tops, q.shape, q._keep = packed, scales, tops, torch.Size([2, 32]), bytes(kept)
+    q._at, q._device_index = id(q._keep), 0
+    for call in (lambda: copy.deepcopy(q), lambda: pickle.loads(pickle.dumps(q))):
+        with pytest.raises(P.NNRuntimeException):
+            call()
