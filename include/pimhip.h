@@ -514,7 +514,8 @@ int pimhip_mx4_dequantize(void* out, int dtype, int64_t ld_out, const PimHipMx4M
 
 /* out[t, n] = act(sum_k x[t, k] * weight[n, k] + bias[n]) for `tokens` rows of x (dtype PIMHIP_F16 or PIMHIP_BF16, pitch ld_x; out and
  * bias are of the same type, bias may be NULL, act a PimHipActFunc).  Weights are converted to dtype on the way to the matrix cores:
- * exactly in bfloat16; in fp16 relative to the row's largest scale, where values below 2^-38 of the row's largest lose bits.
+ * exactly in bfloat16 (but for blocks of codes 0 and 1 in a row with codes 253 or 254); in fp16 relative to the row's largest scale, where values
+ * below 2^-38 of the row's largest lose bits.
  * Sums in fp32, one rounding at the store.  Any sizes, pitches and element-aligned addresses. */
 int pimhip_mx4_linear(void* out, int64_t ld_out, const void* x, int64_t ld_x, int dtype, int64_t tokens, const PimHipMx4Matrix* weight,
                       const void* bias, int act, void* stream);
@@ -560,7 +561,7 @@ int pimhip_moe_layer_workspace_bytes(const PimHipMoeLayerPlan* plan, int tokens,
 /* y[t] = sum over the top_k experts e with the largest router logits of share[t, e] * expert_e(x[t]) for up to 64 tokens (x: pitch ld_x,
  * y: dense).  experts and shares [tokens, top_k]: the choice in falling order of logits, equal ones by their index, a NaN above
  * all, and the experts' shares (fp32).  Router logits, shares, hidden values and all sums are fp32; a hidden value goes through the second product
- * whole in bfloat16 and with 4-bit weights (three pieces of eight bits), with 22 of its bits in fp16, which what is below 2^-29 of its token's largest
+ * whole in bfloat16 and with 4-bit weights (three pieces of eight bits), with 22 of its bits in fp16, which what is below 2^-29 of its pair's largest
  * one loses first.  An expert whose share is 0 adds nothing; where every logit is -inf all shares are 0 and so is y.
  * Allocates and synchronises nothing.  The workspace is the call's until it has run: calls that may overlap, and captured graphs that
  * are replayed at the same time, need one each; a plan may be shared. */

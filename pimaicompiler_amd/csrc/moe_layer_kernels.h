@@ -193,7 +193,8 @@ struct ExpertWeights<T, true, TT> {
 // A hidden value is fp32; the second product takes it in pieces of the matrix cores' 16-bit type, each a column of its own, so that
 // 16-bit hidden values are not what limits y.  Where a first piece's sum is not finite (an infinity among the hidden values or the
 // weights) it is the result: the other pieces have a zero, or a NaN, in that place.
-//   bfloat16 has fp32's range and 8 of its 24 bits: three pieces of eight bits are the value itself.
+//   bfloat16 has fp32's range and 8 of its 24 bits: three pieces of eight bits are the value itself (from 2^-110 on:
+//   below, the last bits are under its smallest subnormal).
 //   fp16 has not the range.  A pair's hidden values are multiplied by the power of two that brings the largest one to 2^14 or above, and y
 //   by its inverse; the second piece is what the first left over, 2^11 times: 22 bits of what is above 2^-29 of the pair's largest, and
 //   2^-50 of that for the rest.

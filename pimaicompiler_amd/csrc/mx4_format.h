@@ -31,7 +31,9 @@ __device__ __forceinline__ float mx_scale_f32(unsigned int code)
 }
 
 // The 16-bit types of activations.  `scale` of a row of 4-bit weights that meets them on the matrix cores:
-//   bfloat16 has the range of every scale: elements are converted with their block's own scale, exactly.
+//   bfloat16 has the range of every scale but the two largest, whose elements 4 and 6, or 2 to 6, are above it: elements are converted
+//   with their block's own scale, exactly; in a row whose largest code is 253 or 254 with a half or a quarter of it, which the sum is
+//   multiplied by at the end (such a row's blocks of codes 0 and 1, 2^-252 of its largest, come out larger by that).
 //   fp16 has not.  Elements are converted relative to the row's largest scale code `top` (the largest element is below 2^15 then),
 //   and the sum is multiplied by 2^(top - 127 - 12) at the end.  Exact for blocks down to 2^-35 of the row's largest scale; what is
 //   further below loses bits that are under 2^-38 of the row's largest value.
@@ -60,8 +62,13 @@ struct BF16 {
     typedef bf16_t elem;
     typedef bf16x8_t frag;
     static __device__ __forceinline__ float4_t mfma(const frag a, const frag b, const float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-    static __device__ __forceinline__ float scale(unsigned int code, int) { return mx_scale_f32(code); }
-    static __device__ __forceinline__ float unscale(float v, int) { return v; }
+    static __device__ __forceinline__ int above(int top) { return top > 252 ? top - 252 : 0; }
+    static __device__ __forceinline__ float scale(unsigned int code, int top)
+    {
+        const int e = (int)code - above(top);
+        return mx_scale_f32(code == kMxNan ? code : (unsigned int)(e > 0 ? e : 0));
+    }
+    static __device__ __forceinline__ float unscale(float v, int top) { return __builtin_amdgcn_ldexpf(v, above(top)); }
     static __device__ __forceinline__ frag from_mx4(unsigned int d, float s)
     {
         const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 1);
