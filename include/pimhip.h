@@ -503,7 +503,7 @@ typedef struct PimHipMx4Matrix {
 /* Quantises x [out->rows, out->cols] (dtype: any PimHipDataType; pitch ld_x elements) into the memory `out` names.  A block's scale is the
  * largest power of two not above its largest magnitude, divided by 4 (2^-127 at least); its values are rounded to the nearest
  * element, ties to the one with an even code, and saturate at 6.  A block that holds an infinity or a NaN gets scale code 255.
- * Equal inputs give equal bytes. */
+ * Equal inputs give equal bytes; what lies behind a row's codes stays as it is. */
 int pimhip_mx4_quantize(const PimHipMx4Matrix* out, const void* x, int dtype, int64_t ld_x, void* stream);
 
 /* Writes m->tops from m->scales: for a matrix whose bytes come from elsewhere. */

@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const typename T::ele
     unsigned int top = 0;
     if (row < rows) {
         const typename T::elem* src = x + row * ld;
-        for (int64_t k = lane * 8; k < ld_scales * kMxBlock; k += 64 * WPR * 8) {
+        for (int64_t k = lane * 8; k < blocks * kMxBlock; k += 64 * WPR * 8) {
             const int64_t block = k / kMxBlock;
             QuantLane<T> q;
             q.load(src, k, cols);
@@ -81,11 +81,9 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const typename T::ele
             d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, q.v[4], q.v[5], s, 2);
             d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, q.v[6], q.v[7], s, 3);
             if (code == kMxNan) d = 0;
-            if (block < blocks) {
-                reinterpret_cast<unsigned int*>(packed + row * blocks * kMxBlockBytes)[k / 8] = d;
-                if (code != kMxNan && code > top) top = code;
-            }
-            if ((lane & 3) == 0) scales[row * ld_scales + block] = (uint8_t)(block < blocks ? code : 0u);
+            reinterpret_cast<unsigned int*>(packed + row * blocks * kMxBlockBytes)[k / 8] = d;
+            if (code != kMxNan && code > top) top = code;
+            if ((lane & 3) == 0) scales[row * ld_scales + block] = (uint8_t)code;
         }
     }
     // The row's largest scale code.

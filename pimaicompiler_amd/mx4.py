@@ -40,7 +40,7 @@ class Mx4Tensor:
 
     shape       the shape of the values, K last
     packed      [rows, ceil(K / 32) * 16] uint8
-    scales      [rows, pitch] uint8, the pitch ceil(K / 32) rounded up to 16
+    scales      [rows, pitch] uint8, the pitch ceil(K / 32) rounded up to 16; what lies behind a row's codes may be anything
     tops        [rows] uint8, the largest scale code of each row
     """
 
