@@ -312,13 +312,14 @@ PyObject* lstm(PyObject*, PyObject* const* args, Py_ssize_t n)
 }
 
 // ---- 4-bit matrices, expert layers, log probabilities -----------------------------------------------------------------------
-// The plain case of these: a tensor of one of their types on the current device, torch's current stream, no gradient asked for.
+// The plain case of these: a tensor of one of their types on the current device, torch's current stream, no gradient asked for and no
+// tangent carried (of level 0, the one there is).
 bool plainTensor(PyObject* o, const at::Tensor*& t)
 {
     if (!THPVariable_Check(o)) return false;
     t = &THPVariable_Unpack(o);
     return t->defined() && t->is_cuda() && t->layout() == at::kStrided && t->dim() >= 1 && t->device().index() == c10::hip::current_device() &&
-           !(t->requires_grad() && at::GradMode::is_enabled());
+           !(t->requires_grad() && at::GradMode::is_enabled()) && !t->_fw_grad(0).defined();
 }
 
 int typeCode(at::ScalarType t) { return t == at::kHalf ? PIMHIP_F16 : t == at::kBFloat16 ? PIMHIP_BF16 : t == at::kFloat ? PIMHIP_F32 : -1; }

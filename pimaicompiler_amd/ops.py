@@ -188,9 +188,10 @@ class _Launch:
 
 
 def _require_no_gradient(*tensors):
-    """For operators without a backward pass: a tensor that would need one is refused rather than cut off silently."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise NNRuntimeException("this operator has no backward pass: call it under torch.no_grad() or on detached tensors")
+    """For operators without derivatives: a tensor that asks for a gradient, or carries a tangent (forward mode, which no_grad does not end), is
+    refused rather than cut off silently."""
+    if any(t is not None and (t.requires_grad and torch.is_grad_enabled() or torch.autograd.forward_ad.unpack_dual(t).tangent is not None) for t in tensors):
+        raise NNRuntimeException("this operator has no derivative: call it under torch.no_grad(), or on detached tensors without a tangent")
 
 
 def gemv_status(stream=None):

@@ -41,3 +41,19 @@ def test_a_copy_takes_no_address_along():
     for call in (lambda: copy.deepcopy(q), lambda: pickle.loads(pickle.dumps(q))):
         with pytest.raises(P.NNRuntimeException):
             call()
+
+
+def test_a_tensor_that_carries_a_tangent_is_refused():
+    import torch.autograd.forward_ad as forward
+    from pimaicompiler_amd.ops import _require_no_gradient
+    x = torch.zeros(2, 64)
+    _require_no_gradient(x, None)
+    with forward.dual_level():
+        _require_no_gradient(x, None)
+        dual = forward.make_dual(x, torch.ones_like(x))
+        for call in (lambda: _require_no_gradient(dual), lambda: _require_no_gradient(None, x, dual)):
+            with pytest.raises(P.NNRuntimeException):
+                call()
+            with torch.no_grad(), pytest.raises(P.NNRuntimeException):
+                call()
+    _require_no_gradient(x)
