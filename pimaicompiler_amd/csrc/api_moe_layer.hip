@@ -4,7 +4,10 @@
 
 using namespace pimhip;
 
-struct PimHipMoeLayerPlan {
+namespace
+{
+struct Plan {
+    uintptr_t number = 0;  // what a PimHipMoeLayerPlan* holds
     int device = 0;
     int num_experts = 0, top_k = 0;
     int64_t d_model = 0, d_ff = 0;
@@ -15,34 +18,35 @@ struct PimHipMoeLayerPlan {
     ExpertPointers* experts = nullptr;  // device, [E]
 };
 
-namespace
-{
-std::vector<PimHipMoeLayerPlan*> g_moe_layer_plans;
+// A plan's handle is its number and no address, which the next plan might get: the handle of a destroyed plan is no other's.
+std::vector<Plan*> g_moe_layer_plans;
+uintptr_t g_moe_layer_plans_made = 0;
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
-int64_t hidden_pitch(const PimHipMoeLayerPlan* p) { return (p->d_ff + 7) / 8 * 8; }
-size_t hidden_bytes(const PimHipMoeLayerPlan* p, int tokens) { return round256((size_t)tokens * p->top_k * hidden_pitch(p) * 4); }
-size_t part_bytes(const PimHipMoeLayerPlan* p, int tokens) { return round256((size_t)tokens * p->top_k * p->d_model * sizeof(float)); }
+int64_t hidden_pitch(const Plan* p) { return (p->d_ff + 7) / 8 * 8; }
+size_t hidden_bytes(const Plan* p, int tokens) { return round256((size_t)tokens * p->top_k * hidden_pitch(p) * 4); }
+size_t part_bytes(const Plan* p, int tokens) { return round256((size_t)tokens * p->top_k * p->d_model * sizeof(float)); }
 
-size_t counter_bytes(const PimHipMoeLayerPlan* p) { return round256((size_t)(p->d_model + 15) / 16 * sizeof(unsigned int)); }
-int64_t most_pitch(const PimHipMoeLayerPlan* p) { return (p->d_ff + 255) / 256 * 16; }
-size_t most_bytes(const PimHipMoeLayerPlan* p, int tokens) { return (size_t)tokens * p->top_k * most_pitch(p); }
+size_t counter_bytes(const Plan* p) { return round256((size_t)(p->d_model + 15) / 16 * sizeof(unsigned int)); }
+int64_t most_pitch(const Plan* p) { return (p->d_ff + 255) / 256 * 16; }
+size_t most_bytes(const Plan* p, int tokens) { return (size_t)tokens * p->top_k * most_pitch(p); }
 
-bool known_locked(const PimHipMoeLayerPlan* plan)
+Plan* find_locked(const PimHipMoeLayerPlan* handle)
 {
-    for (const PimHipMoeLayerPlan* q : g_moe_layer_plans)
-        if (q == plan) return true;
-    return false;
+    for (Plan* p : g_moe_layer_plans)
+        if (p->number == reinterpret_cast<uintptr_t>(handle)) return p;
+    return nullptr;
 }
 
 // A plan that shutting the library down, or its owner, has destroyed is refused.
-int check_plan(const PimHipMoeLayerPlan* plan)
+int find_plan(const PimHipMoeLayerPlan* handle, Plan** plan)
 {
     std::lock_guard<std::mutex> lock(g_mutex);
-    return known_locked(plan) ? (int)PIMHIP_OK : fail(PIMHIP_ERR_INVALID_ARGUMENT, "unknown or already destroyed expert layer plan");
+    *plan = find_locked(handle);
+    return *plan ? (int)PIMHIP_OK : fail(PIMHIP_ERR_INVALID_ARGUMENT, "unknown or already destroyed expert layer plan");
 }
 
-int destroy_moe_layer_plan_locked(PimHipMoeLayerPlan* plan)
+int destroy_moe_layer_plan_locked(Plan* plan)
 {
     if (!plan) return PIMHIP_OK;
     int prev = -1;
@@ -90,7 +94,7 @@ void launch_second(const MoeLayerArgs& a, unsigned int most, hipStream_t s)
 }
 
 template <class T, bool MX>
-void launch(const PimHipMoeLayerPlan* p, MoeLayerArgs& a, hipStream_t s)
+void launch(const Plan* p, MoeLayerArgs& a, hipStream_t s)
 {
     moe_layer_router_kernel<T><<<dim3((unsigned)a.tokens), kRouterThreads, 0, s>>>(a);
     // Tokens are staged as a whole where there are one or two, or where an expert has many and 16 of them leave a CU room for three
@@ -194,7 +198,7 @@ extern "C" int pimhip_moe_layer_plan_create(PimHipMoeLayerPlan** plan_out, const
     hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
     PIMHIP_HIP_CHECK(hipStreamIsCapturing(s, &capture));
     if (capture != hipStreamCaptureStatusNone) return fail(PIMHIP_ERR_UNSUPPORTED, "a plan allocates: create it before the capture");
-    PimHipMoeLayerPlan* plan = new (std::nothrow) PimHipMoeLayerPlan();
+    Plan* plan = new (std::nothrow) Plan();
     if (!plan) return fail(PIMHIP_ERR_HIP, "out of host memory");
     hipGetDevice(&plan->device);
     plan->num_experts = d->num_experts, plan->top_k = d->top_k, plan->d_model = d->d_model, plan->d_ff = d->d_ff;
@@ -212,40 +216,44 @@ extern "C" int pimhip_moe_layer_plan_create(PimHipMoeLayerPlan** plan_out, const
     }
     try {
         g_moe_layer_plans.push_back(plan);
+        plan->number = ++g_moe_layer_plans_made;
     } catch (...) {
         destroy_moe_layer_plan_locked(plan);
         return fail(PIMHIP_ERR_HIP, "out of host memory");
     }
-    *plan_out = plan;
+    *plan_out = reinterpret_cast<PimHipMoeLayerPlan*>(plan->number);
     return PIMHIP_OK;
 }
 
-extern "C" int pimhip_moe_layer_plan_destroy(PimHipMoeLayerPlan* plan)
+extern "C" int pimhip_moe_layer_plan_destroy(PimHipMoeLayerPlan* handle)
 {
-    if (!plan) return PIMHIP_OK;
+    if (!handle) return PIMHIP_OK;
     std::lock_guard<std::mutex> lock(g_mutex);
-    if (!known_locked(plan)) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "unknown or already destroyed expert layer plan");
+    Plan* plan = find_locked(handle);
+    if (!plan) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "unknown or already destroyed expert layer plan");
     return destroy_moe_layer_plan_locked(plan);
 }
 
-extern "C" int pimhip_moe_layer_workspace_bytes(const PimHipMoeLayerPlan* plan, int tokens, uint64_t* bytes)
+extern "C" int pimhip_moe_layer_workspace_bytes(const PimHipMoeLayerPlan* handle, int tokens, uint64_t* bytes)
 {
-    if (!plan || !bytes) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "plan and bytes must be non-null");
-    const int rc = check_plan(plan);
+    if (!handle || !bytes) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "plan and bytes must be non-null");
+    Plan* plan;
+    const int rc = find_plan(handle, &plan);
     if (rc != PIMHIP_OK) return rc;
     if (tokens < 0 || tokens > kMoeLayerTokens) return fail(PIMHIP_ERR_UNSUPPORTED, "tokens=%d not in [0, %d]", tokens, kMoeLayerTokens);
     *bytes = hidden_bytes(plan, tokens) + part_bytes(plan, tokens) + counter_bytes(plan) + most_bytes(plan, tokens);
     return PIMHIP_OK;
 }
 
-extern "C" int pimhip_moe_layer_forward(PimHipMoeLayerPlan* plan, const void* x, int64_t ld_x, int tokens, void* y, int* experts, float* shares,
+extern "C" int pimhip_moe_layer_forward(PimHipMoeLayerPlan* handle, const void* x, int64_t ld_x, int tokens, void* y, int* experts, float* shares,
                                         void* workspace, void* stream)
 {
     DeviceState* st = nullptr;
     int rc = current_device_state(&st);
     if (rc != PIMHIP_OK) return rc;
-    if (!plan) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "plan is null");
-    if ((rc = check_plan(plan)) != PIMHIP_OK) return rc;
+    if (!handle) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "plan is null");
+    Plan* plan;
+    if ((rc = find_plan(handle, &plan)) != PIMHIP_OK) return rc;
     int dev = -1;
     PIMHIP_HIP_CHECK(hipGetDevice(&dev));
     if (dev != plan->device) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "plan belongs to device %d, current device is %d", plan->device, dev);
