@@ -46,13 +46,13 @@ int64_t shared_tokens_bytes(int64_t M, int64_t K)
     return M * SharedTokens<T>::pitch((int)K, Mx4Weights<T, 2>::kUnit) * 16;
 }
 
-template <class T, bool SHARED, int RT, int TT, int U, int WK>
+template <class T, bool SHARED, int RT, int TT, int WK>
 int linear_skinny(void* out, int64_t ld_out, const void* x, int64_t ld_x, int64_t M, const Mx4View& w, const void* bias, int relu, hipStream_t s)
 {
     const int64_t gx = (w.rows + 16 * RT - 1) / (16 * RT), gy = (M + 16 * TT - 1) / (16 * TT);
     const int rc = check_grid(gx, gy, 64 * WK);
     if (rc != PIMHIP_OK) return rc;
-    mx4_linear_skinny_kernel<T, SHARED, RT, TT, U, WK><<<dim3((unsigned)gx, (unsigned)gy), 64 * WK, SHARED ? shared_tokens_bytes<T>(M, w.cols) : 0, s>>>(
+    mx4_linear_skinny_kernel<T, SHARED, RT, TT, WK><<<dim3((unsigned)gx, (unsigned)gy), 64 * WK, SHARED ? shared_tokens_bytes<T>(M, w.cols) : 0, s>>>(
         (const typename T::elem*)x, w, (const typename T::elem*)bias, (typename T::elem*)out, ld_x, ld_out, M, relu);
     return PIMHIP_OK;
 }
@@ -72,17 +72,17 @@ int linear(void* out, int64_t ld_out, const void* x, int64_t ld_x, int64_t M, co
     const bool long_rows = w.cols > 4 * Mx4Weights<T, 2>::kUnit;
     auto go = [&](auto kernel) { return kernel(out, ld_out, x, ld_x, M, w, bias, relu, s); };
     if (M <= 2 && shared_tokens_bytes<T>(M, w.cols) <= kShared) {
-        if (tiles16 < 768) return long_rows ? go(linear_skinny<T, true, 1, 1, 1, 8>) : go(linear_skinny<T, true, 1, 1, 1, 4>);
-        return long_rows ? go(linear_skinny<T, true, 2, 1, 1, 8>) : go(linear_skinny<T, true, 2, 1, 1, 4>);
+        if (tiles16 < 768) return long_rows ? go(linear_skinny<T, true, 1, 1, 8>) : go(linear_skinny<T, true, 1, 1, 4>);
+        return long_rows ? go(linear_skinny<T, true, 2, 1, 8>) : go(linear_skinny<T, true, 2, 1, 4>);
     }
     if (M <= 16) {
-        if (tiles16 < 512) return long_rows ? go(linear_skinny<T, false, 1, 1, 1, 8>) : go(linear_skinny<T, false, 1, 1, 1, 4>);
-        return long_rows ? go(linear_skinny<T, false, 4, 1, 1, 8>) : go(linear_skinny<T, false, 4, 1, 1, 4>);
+        if (tiles16 < 512) return long_rows ? go(linear_skinny<T, false, 1, 1, 8>) : go(linear_skinny<T, false, 1, 1, 4>);
+        return long_rows ? go(linear_skinny<T, false, 4, 1, 8>) : go(linear_skinny<T, false, 4, 1, 4>);
     }
     if (M <= 64) {
-        if (tiles16 <= 512) return M <= 32 ? go(linear_skinny<T, false, 1, 2, 1, 8>) : go(linear_skinny<T, false, 2, 2, 1, 8>);
-        if (!long_rows) return go(linear_skinny<T, false, 4, 2, 1, 4>);
-        return M <= 32 ? go(linear_skinny<T, false, 4, 2, 1, 8>) : go(linear_skinny<T, false, 4, 4, 1, 4>);
+        if (tiles16 <= 512) return M <= 32 ? go(linear_skinny<T, false, 1, 2, 8>) : go(linear_skinny<T, false, 2, 2, 8>);
+        if (!long_rows) return go(linear_skinny<T, false, 4, 2, 4>);
+        return M <= 32 ? go(linear_skinny<T, false, 4, 2, 8>) : go(linear_skinny<T, false, 4, 4, 4>);
     }
     // Large tiles read operands less often, small ones fill the card.  Measured, 256 x 128 / 128 x 64, in us: 4096 x 16384 x 4096 532 / 634,
     // 2048 x 4096 x 4096 (256 large tiles) 70 / 86, 1500 x 4608 x 4096 (216) 68 / 84, 1500 x 4096 x 4096 (192) 68 / 65, 200 x 16384 x 4096 (128)

@@ -398,7 +398,7 @@ __device__ __forceinline__ void expert_sums(const typename W::Rows (&rows)[RT], 
 {
     const int lane = threadIdx.x & 63, wave = wave_in_block();
     float4_t acc[RT][TT] = {};
-    skinny_sum<T, W, X, RT, TT, 1>(acc, rows, x, K, wave, WK, lds + wave * kSkinnyLds<W, X>, ready);
+    skinny_sum<T, W, X, RT, TT>(acc, rows, x, K, wave, WK, lds + wave * kSkinnyLds<W, X>, ready);
     __syncthreads();
     float4_t* part = reinterpret_cast<float4_t*>(lds);
 #pragma unroll

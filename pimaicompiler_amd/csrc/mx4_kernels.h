@@ -167,7 +167,7 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint8_t* pack
 // tokens (at most 16) lie in LDS as a whole, in the launch's dynamic part of it.  Bound by the weights' bytes: 16384 x 4096 for one token
 // 8.1 us, 4.4 TB/s; 31999 x 1024 for 16 tokens 6.8 us, 2.6 TB/s, a block's chain of loads being half of that.  What was measured to choose
 // the tile and the wavefronts stands with the rule that chooses.
-template <class T, bool SHARED, int RT, int TT, int U, int WK>
+template <class T, bool SHARED, int RT, int TT, int WK>
 __global__ __launch_bounds__(64 * WK) void mx4_linear_skinny_kernel(const typename T::elem* x, Mx4View w, const typename T::elem* bias, typename T::elem* out,
                                                                     int64_t ld_x, int64_t ld_out, int64_t M, int relu)
 {
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(64 * WK) void mx4_linear_skinny_kernel(const typena
         add[threadIdx.x] = bias ? (float)bias[n] : 0.0f;
     }
     float4_t acc[RT][TT] = {};
-    skinny_sum<T, W, X, RT, TT, U>(acc, rows, tokens, K, wave, WK, lds + wave * kLds, [&] {
+    skinny_sum<T, W, X, RT, TT>(acc, rows, tokens, K, wave, WK, lds + wave * kLds, [&] {
         if constexpr (SHARED) SharedTokens<T>::stage(xs, token, (int)M, K, pitch);
         __syncthreads();
     });
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(64 * WK) void mx4_linear_skinny_kernel(const typena
     for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
-            if (WK > 1 && (i * TT + j) % WK != wave) continue;
+            if ((i * TT + j) % WK != wave) continue;
             const int64_t t = token0 + j * 16 + (lane & 15), n = row0 + i * 16 + group * 4;
             if (t >= M || n >= w.rows) continue;
             float4_t v = acc[i][j];
@@ -234,7 +234,7 @@ __global__ __launch_bounds__(64 * WK) void mx4_linear_skinny_kernel(const typena
 template <class O, int RT, int TT, int WK>
 __global__ __launch_bounds__(64 * WK) void mx4_matmul_skinny_kernel(Mx4View a, Mx4View b, typename O::elem* out, int64_t ld_out)
 {
-    __shared__ float4_t part[WK > 1 ? WK * RT * TT * 64 : 1];
+    __shared__ float4_t part[WK * RT * TT * 64];
     const int lane = threadIdx.x & 63, wave = wave_in_block(), group = lane >> 4;
     const int64_t row0 = (int64_t)blockIdx.x * (16 * RT), token0 = (int64_t)blockIdx.y * (16 * TT);
     const int blocks = (int)((b.cols + kMxBlock - 1) / kMxBlock);
@@ -293,7 +293,7 @@ __global__ __launch_bounds__(64 * WK) void mx4_matmul_skinny_kernel(Mx4View a, M
     for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
-            if (WK > 1 && (i * TT + j) % WK != wave) continue;
+            if ((i * TT + j) % WK != wave) continue;
             const int64_t t = token0 + j * 16 + (lane & 15), n = row0 + i * 16 + group * 4;
             if (t >= a.rows || n >= b.rows) continue;
             store4<O>(out + t * ld_out + n, acc[i][j], b.rows - n < 4 ? (int)(b.rows - n) : 4);

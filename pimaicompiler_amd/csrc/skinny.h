@@ -10,8 +10,9 @@
 // place c ^ (row % 8) there, which spreads 8 rows' equal chunks over all banks.
 //
 // k is taken in steps of 128 (four products) and in units: of a unit, lane l has the 32 values from 32 (l / 16) on of each step, the
-// products take eight of them each.  The order of k is the same for both operands and otherwise free.  Each wavefront has U units of
-// both operands on their way; x is asked for with its weights, since a wavefront's loads come back in order.
+// products take eight of them each.  The order of k is the same for both operands and otherwise free.  A wavefront asks for a unit of both
+// operands behind the products of the one before, and others of its CU fill the wait; x is asked for with its weights, since a
+// wavefront's loads come back in order.
 #pragma once
 
 #include <type_traits>
@@ -267,7 +268,7 @@ constexpr int kSkinnyLds = W::kLds + X::kLds;
 
 // acc[i][j] += 16 rows i x 16 tokens j over units first, first + stride, ... of K.  `lds`: this wavefront's kSkinnyLds words.
 // ready() is called once, behind the first loads of weights: there a block stages what its wavefronts share.
-template <class T, class W, class X, int RT, int TT, int U, class R>
+template <class T, class W, class X, int RT, int TT, class R>
 __device__ __forceinline__ void skinny_sum(float4_t (&acc)[RT][TT], const typename W::Rows (&w)[RT], const typename X::Rows (&x)[X::raws(TT)], int K, int first, int stride,
                                            uint4_t* lds, R ready)
 {
@@ -275,63 +276,49 @@ __device__ __forceinline__ void skinny_sum(float4_t (&acc)[RT][TT], const typena
     constexpr int S = W::kUnit / kSkinnyStep, XR = X::raws(TT);  // steps of a unit
     const int whole = K / W::kUnit;
     const int mine = first < whole ? (whole - first + stride - 1) / stride : 0;  // this wavefront's whole units
-    typename W::Raw wv[U][RT];
-    typename X::Raw xv[U][S][XR];
-    auto ask = [&](int u, int n) {
+    typename W::Raw wv[RT];
+    typename X::Raw xv[S][XR];
+    auto ask = [&](int n) {
         const int unit = first + n * stride;
 #pragma unroll
         for (int s = 0; s < S; ++s)
 #pragma unroll
-            for (int j = 0; j < XR; ++j) X::load(xv[u][s][j], x[j], unit * S + s);
+            for (int j = 0; j < XR; ++j) X::load(xv[s][j], x[j], unit * S + s);
 #pragma unroll
-        for (int i = 0; i < RT; ++i) W::load(wv[u][i], w[i], unit);
+        for (int i = 0; i < RT; ++i) W::load(wv[i], w[i], unit);
     };
-    auto products = [&](const typename W::Raw(&wr)[RT], typename X::Raw(&xr)[S][XR], int unit) {
+    auto products = [&](int unit) {
         typename W::Operands a[RT];
 #pragma unroll
-        for (int i = 0; i < RT; ++i) W::turn(a[i], wr[i], w[i], lds);
+        for (int i = 0; i < RT; ++i) W::turn(a[i], wv[i], w[i], lds);
 #pragma unroll
         for (int s = 0; s < S; ++s)
 #pragma unroll
             for (int j = 0; j < TT; ++j) {
                 frag f[4];
-                X::turn(f, xr[s][j % XR], x[j % XR], unit * S + s, j, lds + W::kLds);
+                X::turn(f, xv[s][j % XR], x[j % XR], unit * S + s, j, lds + W::kLds);
 #pragma unroll
                 for (int o = 0; o < 4; ++o)
 #pragma unroll
                     for (int i = 0; i < RT; ++i) acc[i][j] = T::mfma(W::operand(a[i], s, o), f[o], acc[i][j]);
             }
     };
-    // The loop without conditions lets the compiler count loads exactly; what it leaves, fewer than 2 U units, goes by conditions.
-    int n = 0;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (u < mine) ask(u, u);
+    if (mine > 0) ask(0);
     ready();
-    for (; n + 2 * U <= mine; n += U) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            products(wv[u], xv[u], first + (n + u) * stride);
-            ask(u, n + U + u);
-        }
+    for (int n = 0; n + 1 < mine; ++n) {
+        products(first + n * stride);
+        ask(n + 1);
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        if (n + u < mine) products(wv[u], xv[u], first + (n + u) * stride);
-        if (n + U + u < mine) ask(u, n + U + u);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (n + U + u < mine) products(wv[u], xv[u], first + (n + U + u) * stride);
+    if (mine > 0) products(first + (mine - 1) * stride);
     // The unit that K ends in.
     if (K % W::kUnit != 0 && whole % stride == first) {
 #pragma unroll
-        for (int i = 0; i < RT; ++i) W::load_guarded(wv[0][i], w[i], whole, K);
+        for (int i = 0; i < RT; ++i) W::load_guarded(wv[i], w[i], whole, K);
 #pragma unroll
         for (int s = 0; s < S; ++s)
 #pragma unroll
-            for (int j = 0; j < XR; ++j) X::load_guarded(xv[0][s][j], x[j], whole * S + s, K);
-        products(wv[0], xv[0], whole);
+            for (int j = 0; j < XR; ++j) X::load_guarded(xv[s][j], x[j], whole * S + s, K);
+        products(whole);
     }
 }
 
@@ -340,24 +327,22 @@ __device__ __forceinline__ void skinny_sum(float4_t (&acc)[RT][TT], const typena
 template <int RT, int TT, int WK>
 __device__ __forceinline__ void skinny_join(float4_t (&acc)[RT][TT], float4_t* part)
 {
-    if constexpr (WK > 1) {
-        const int lane = threadIdx.x & 63, wave = wave_in_block();
-        __syncthreads();
+    const int lane = threadIdx.x & 63, wave = wave_in_block();
+    __syncthreads();
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
-            for (int j = 0; j < TT; ++j) part[((wave * RT + i) * TT + j) * 64 + lane] = acc[i][j];
-        __syncthreads();
+        for (int j = 0; j < TT; ++j) part[((wave * RT + i) * TT + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
-            for (int j = 0; j < TT; ++j) {
-                if ((i * TT + j) % WK != wave) continue;
-                float4_t v = part[(i * TT + j) * 64 + lane];
+        for (int j = 0; j < TT; ++j) {
+            if ((i * TT + j) % WK != wave) continue;
+            float4_t v = part[(i * TT + j) * 64 + lane];
 #pragma unroll
-                for (int k = 1; k < WK; ++k) v += part[((k * RT + i) * TT + j) * 64 + lane];
-                acc[i][j] = v;
-            }
-    }
+            for (int k = 1; k < WK; ++k) v += part[((k * RT + i) * TT + j) * 64 + lane];
+            acc[i][j] = v;
+        }
 }
 }  // namespace pimhip
