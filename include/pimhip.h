@@ -561,7 +561,7 @@ int pimhip_moe_layer_workspace_bytes(const PimHipMoeLayerPlan* plan, int tokens,
 /* y[t] = sum over the top_k experts e with the largest router logits of share[t, e] * expert_e(x[t]) for up to 64 tokens (x: pitch ld_x,
  * y: dense).  experts and shares [tokens, top_k]: the choice in falling order of logits, equal ones by their index, a NaN above
  * all, and the experts' shares (fp32).  Router logits, shares, hidden values and all sums are fp32; a hidden value goes through the second product
- * whole in bfloat16 and with 4-bit weights (three pieces of eight bits), with 22 of its bits in fp16, which what is below 2^-29 of its pair's largest
+ * whole in bfloat16 (three pieces of eight bits), with 22 of its bits in fp16, which what is below 2^-29 of its pair's largest
  * one loses first.  An expert whose share is 0 adds nothing; where every logit is -inf all shares are 0 and so is y.
  * Allocates and synchronises nothing.  The workspace is the call's until it has run: calls that may overlap, and captured graphs that
  * are replayed at the same time, need one each; a plan may be shared. */

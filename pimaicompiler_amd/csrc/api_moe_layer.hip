@@ -86,7 +86,7 @@ void launch_second(const MoeLayerArgs& a, unsigned int most, hipStream_t s)
 {
     typedef SecondColumns<T, MX, true, FEW> C;
     const dim3 grid((unsigned)((a.d_model + 16 * RT - 1) / (16 * RT)), (unsigned)a.E, (unsigned)((a.tokens + C::kPairs - 1) / C::kPairs));
-    const unsigned int bytes = shared_bytes<typename C::H, MX>((a.tokens < C::kPairs ? a.tokens : C::kPairs) * C::kPieces, a.d_ff);
+    const unsigned int bytes = shared_bytes<T, MX>((a.tokens < 16 ? a.tokens : 16) * C::kPieces, a.d_ff);
     if (bytes <= most)
         moe_layer_second_kernel<T, MX, true, RT, WK, FEW><<<grid, 64 * WK, bytes, s>>>(a);
     else
@@ -97,10 +97,10 @@ template <class T, bool MX>
 void launch(const Plan* p, MoeLayerArgs& a, hipStream_t s)
 {
     moe_layer_router_kernel<T><<<dim3((unsigned)a.tokens), kRouterThreads, 0, s>>>(a);
-    // Tokens are staged as a whole where there are one or two, or where an expert has many and 16 of them leave a CU room for three
-    // blocks.
+    // Columns are staged as a whole where tokens are one or two, or where an expert has many and 16 of them leave a CU room for three
+    // blocks (the second product of one token and 4096 hidden values in three pieces, 24 KB: 18.2 us a call, 21.7 turned).
     const bool many = a.tokens > 16;
-    const unsigned int most = many ? 40 << 10 : a.tokens <= 2 ? 20 << 10 : 0;
+    const unsigned int most = many ? 40 << 10 : a.tokens <= 2 ? 26 << 10 : 0;
     // With many tokens a block has twice the rows: their values are read, and turned or staged, half as often (64 tokens through 8 gated 4-bit
     // experts 1024 -> 4096: 29.8 -> 20.8 us; one token through 2 of 8 experts 1024 -> 4096 in fp16, where blocks are few: 6.1 -> 7.9).
     const unsigned int staged = shared_bytes<T, MX>(a.tokens < 16 ? a.tokens : 16, a.d_model);
@@ -120,12 +120,16 @@ void launch(const Plan* p, MoeLayerArgs& a, hipStream_t s)
     else
         staged <= most ? first(std::true_type{}) : first(std::false_type{});
     // Blocks of the second product that have something to read.  Where they fill the card several times over a block has two tiles of
-    // rows and four wavefronts, else eight wavefronts share its long k.  Where experts have more than 8 pairs, which some have from 5 on the
-    // average on, 16 of them a block read their weights half as often.  In us a call, 16 / 8 pairs a block: 64 tokens through 8 gated 4-bit experts 1024
-    // -> 4096, two chosen (16 pairs an expert) 44.6 / 46.6, 32 tokens (8) 32.4 / 30.9, 17 tokens (4) 31 / 26; 64 tokens through 64 gated bf16 experts
-    // 2048 -> 1024, six chosen (6) 178 / 191.
+    // rows and four wavefronts, else eight wavefronts share its long k.  The pieces of 8 pairs (fp16) or 5 (bfloat16) are a tile; 16 pairs in a tile a
+    // piece read an expert's weights less often where experts have many pairs, and turn and multiply more where they have few.  In us a call, 16 / 8 or 5
+    // pairs a block, by pairs an expert on the average, 8 gated experts 1024 -> 4096, two chosen, and 64 of 2048 -> 1024, six chosen:
+    //   fp16        3.3: 44.8 / 42.6   5: 48.5 / 48.5   6: 49.3 / 53.6   16: 63 / 69
+    //   bfloat16    2.5: 44.1 / 42.0   3.3: 44.5 / 46.9   4.3: 46.3 / 54.1   16: 58 / 84      64 experts   2.3: 160 / 158   3.8: 169 / 174   6: 182 / 224
+    //   4 bits, fp16 x    6: 36.0 / 32.0   7: 37.6 / 37.1   8: 37.2 / 37.6   16: 43.7 / 50.4
+    //   4 bits, bfloat16 x    6: 36.9 / 33.3   7: 38.2 / 34.8   8: 37.5 / 35.8   16: 43.8 / 49.9      64 experts   3.8: 95.6 / 90.0   6: 107.6 / 128.2
     const int64_t blocks = (int64_t)((a.d_model + 15) / 16) * (a.E < pairs ? a.E : pairs);
-    if (pairs > 5 * a.E) {
+    const int border = MX ? (blocks >= 2048 ? 5 : 7) : Pieces<T>::kCount > 2 ? 3 : 5;
+    if (pairs > border * a.E) {
         if constexpr (!MX) {
             // (16-bit weights are four times the bytes: 64 tokens through 8 fp16 experts 1024 -> 4096 46.5 with eight wavefronts and a tile, 51 with two
             // tiles and four; in 4 bits 46.0 / 41.3, the values being turned for each tile of rows)

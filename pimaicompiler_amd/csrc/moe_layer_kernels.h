@@ -177,7 +177,6 @@ struct ExpertWeights<T, false, TT> {
     {
         return W::rows(w, first, count, K);
     }
-    static __device__ __forceinline__ float unscale(float v, const void*, int64_t) { return v; }
 };
 template <class T, int TT>
 struct ExpertWeights<T, true, TT> {
@@ -186,7 +185,6 @@ struct ExpertWeights<T, true, TT> {
     {
         return W::rows((const uint8_t*)w, (const uint8_t*)s, (const uint8_t*)t, ld, first, count, K);
     }
-    static __device__ __forceinline__ float unscale(float v, const void* t, int64_t r) { return T::unscale(v, ((const uint8_t*)t)[r]); }
 };
 
 // ---- hidden values as operands -----------------------------------------------------------------------------------------------
@@ -198,16 +196,8 @@ struct ExpertWeights<T, true, TT> {
 //   fp16 has not the range.  A pair's hidden values are multiplied by the power of two that brings the largest one to 2^14 or above, and y
 //   by its inverse; the second piece is what the first left over, 2^11 times: 22 bits of what is above 2^-29 of the pair's largest, and
 //   2^-50 of that for the rest.
-// 4-bit weights are values of bfloat16, whatever the type of x, so only 16-bit ones in fp16 need the second way.
-template <class T, bool MX>
-struct HiddenType {
-    typedef T type;
-};
-template <class T>
-struct HiddenType<T, true> {
-    typedef BF16 type;
-};
-
+// They are taken apart by each block of the second product: stored in pieces by the first one they are more bytes, 64 tokens through 8 gated
+// bfloat16 experts 1024 -> 4096 66.8 us a call, not 58.
 template <class T>
 struct Pieces;
 template <>
@@ -387,6 +377,7 @@ template <class W, class X, int RT, int WK, int PARTS>
 struct ExpertLds {
     static constexpr int kTurn = kSkinnyLds<W, X>, kSum = RT * PARTS * 64;
     uint4_t turn[WK * (kTurn > kSum ? kTurn : kSum)];
+    uint8_t tops[16 * RT];  // the largest scale codes of a block's rows, where they are in 4 bits
     short list[kMoeLayerPairs];
     int count;
 };
@@ -426,7 +417,7 @@ struct FirstColumns {
     typedef typename std::conditional<SHARED, SharedTokens<T>, TurnedTokens<T, true>>::type X;
 };
 template <class T, bool MX, bool SHARED, bool GATED, int F, int WK, int TT>
-__device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPointers& p, const short* list, int n, uint4_t* xs, uint4_t* lds)
+__device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPointers& p, const short* list, int n, uint8_t* tops, uint4_t* xs, uint4_t* lds)
 {
     constexpr int RT = GATED ? 2 * F : F;
     static_assert(!SHARED || TT == 1, "tokens are staged as one tile");
@@ -435,12 +426,17 @@ __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPoi
     typedef typename FirstColumns<T, MX, SHARED, TT>::X X;
     const int lane = threadIdx.x & 63, wave = wave_in_block(), group = lane >> 4;
     const int f0 = blockIdx.x * (16 * F), pitch = SharedTokens<T>::pitch(a.d_model, W::kUnit);
+    // (value rows follow the gate rows; each kind ends at its own last row)
+    auto end_of = [&](int i) { return i < F ? a.d_ff : 2 * a.d_ff; };
+    auto row_at = [&](int i, int r) {
+        const int at = (i < F ? 0 : a.d_ff) + f0 + i % F * 16 + r;
+        return at < end_of(i) ? at : end_of(i) - 1;
+    };
+    uint8_t top = 0;
+    if (MX && threadIdx.x < 16 * RT) top = ((const uint8_t*)p.t1)[row_at(threadIdx.x / 16, threadIdx.x % 16)];
     typename W::Rows rows[RT];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {  // (value rows follow the gate rows; each kind ends at its own last row)
-        const int end = i < F ? a.d_ff : 2 * a.d_ff, at = (i < F ? 0 : a.d_ff) + f0 + i % F * 16;
-        rows[i] = EW::rows(p.w1, p.s1, p.t1, a.ld_s1, at < end ? at : end - 1, end, a.d_model);
-    }
+    for (int i = 0; i < RT; ++i) rows[i] = EW::rows(p.w1, p.s1, p.t1, a.ld_s1, row_at(i, 0), end_of(i), a.d_model);
     auto token = [&](int i) { return (const typename T::elem*)a.x + (int64_t)(list[i] / a.top_k) * a.ld_x; };
     typename X::Rows x[TT];
 #pragma unroll
@@ -454,6 +450,7 @@ __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPoi
     expert_sums<T, W, X, RT, TT, WK, TT>(
         rows, x, a.d_model, lds,
         [&] {
+            if (MX && threadIdx.x < 16 * RT) tops[threadIdx.x] = top;
             if constexpr (SHARED) {
                 X::stage(xs, token, n, a.d_model, pitch);
                 __syncthreads();
@@ -473,12 +470,12 @@ __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPoi
             for (int c = 0; c < 4; ++c) {
                 h[c] = 0.0f;
                 if (f + c >= a.d_ff) continue;
-                float v = EW::unscale(g[c], p.t1, f + c);
+                float v = MX ? __builtin_amdgcn_ldexpf(g[c], T::exponent(tops[i * 16 + group * 4 + c])) : g[c];
                 if (p.b1) v += (float)((const typename T::elem*)p.b1)[f + c];
                 if (a.act == PIMHIP_EXPERT_RELU) v = relu_f32(v);
                 if (a.act == PIMHIP_EXPERT_SILU) v = v / (1.0f + expf(-v));
                 if (GATED) {
-                    float w = EW::unscale(u[c], p.t1, a.d_ff + f + c);
+                    float w = MX ? __builtin_amdgcn_ldexpf(u[c], T::exponent(tops[(F + i) * 16 + group * 4 + c])) : u[c];
                     if (p.b1) w += (float)((const typename T::elem*)p.b1)[a.d_ff + f + c];
                     v *= w;
                 }
@@ -488,7 +485,7 @@ __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPoi
             }
             *reinterpret_cast<float4_t*>(a.h + (int64_t)list[column] * a.ld_h + f) = h;
         }
-        if constexpr (Pieces<typename HiddenType<T, MX>::type>::kScaled) {
+        if constexpr (Pieces<T>::kScaled) {
             const auto q = __builtin_amdgcn_permlane16_swap(most, most, false, false);
             most = q[0] > q[1] ? q[0] : q[1];
             const auto r = __builtin_amdgcn_permlane32_swap(most, most, false, false);
@@ -511,33 +508,34 @@ __global__ __launch_bounds__(64 * WK, TT > 1 ? 2 : F > 2 || (GATED && F > 1) ? 3
     extern __shared__ uint4_t xs[];
     const ExpertPointers p = a.experts[blockIdx.y];
     const int first = blockIdx.z * (16 * TT), n = pairs_of(a.chosen, a.tokens * a.top_k, blockIdx.y, lds.list, &lds.count) - first;
-    if (n > 0) moe_first<T, MX, SHARED, GATED, F, WK, TT>(a, p, lds.list + first, n < 16 * TT ? n : 16 * TT, xs, lds.turn);
+    if (n > 0) moe_first<T, MX, SHARED, GATED, F, WK, TT>(a, p, lds.list + first, n < 16 * TT ? n : 16 * TT, lds.tops, xs, lds.turn);
 }
 
 // The second product: rows of d_model, with the bias, not yet weighted.  FEW: of as many pairs as have their pieces in one tile; else of up to 16.
 template <class T, bool MX, bool SHARED, bool FEW>
 struct SecondColumns {
-    typedef typename HiddenType<T, MX>::type H;
-    typedef ExpertWeights<H, MX, FEW ? 1 : 2> EW;
+    typedef ExpertWeights<T, MX, FEW ? 1 : 2> EW;
     typedef typename EW::W W;
-    typedef HiddenTokens<H, FEW> Turned;
-    typedef typename std::conditional<SHARED, SharedTokens<H>, Turned>::type X;
-    static constexpr int kPieces = Pieces<H>::kCount, kTiles = FEW ? 1 : kPieces, kPairs = FEW ? 16 / kPieces : 16;
+    typedef HiddenTokens<T, FEW> Turned;
+    typedef typename std::conditional<SHARED, SharedTokens<T>, Turned>::type X;
+    static constexpr int kPieces = Pieces<T>::kCount, kTiles = FEW ? 1 : kPieces, kPairs = FEW ? 16 / kPieces : 16;
 };
 template <class T, bool MX, bool SHARED, int RT, int WK, bool FEW>
-__device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPointers& p, const short* list, int n, int* lift, uint4_t* xs, uint4_t* lds)
+__device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPointers& p, const short* list, int n, int* lift, uint8_t* tops, uint4_t* xs, uint4_t* lds)
 {
     typedef SecondColumns<T, MX, SHARED, FEW> C;
-    typedef typename C::H H;
     typedef typename C::EW EW;
     typedef typename C::W W;
     typedef typename C::X X;
     constexpr int P = C::kPieces, TT = C::kTiles;
     const int lane = threadIdx.x & 63, wave = wave_in_block(), group = lane >> 4;
-    const int d0 = blockIdx.x * (16 * RT), pitch = SharedTokens<H>::pitch(a.d_ff, W::kUnit);
+    const int d0 = blockIdx.x * (16 * RT), pitch = SharedTokens<T>::pitch(a.d_ff, W::kUnit);
+    auto row_at = [&](int r) { return d0 + r < a.d_model ? d0 + r : a.d_model - 1; };
+    uint8_t top = 0;
+    if (MX && threadIdx.x < 16 * RT) top = ((const uint8_t*)p.t2)[row_at(threadIdx.x)];
     typename W::Rows rows[RT];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) rows[i] = EW::rows(p.w2, p.s2, p.t2, a.ld_s2, d0 + i * 16 < a.d_model ? d0 + i * 16 : a.d_model - 1, a.d_model, a.d_ff);
+    for (int i = 0; i < RT; ++i) rows[i] = EW::rows(p.w2, p.s2, p.t2, a.ld_s2, row_at(i * 16), a.d_model, a.d_ff);
     auto pair_at = [&](int i) { return (int)list[i]; };
     typename X::Rows x[X::raws(TT)];
     if constexpr (SHARED) {
@@ -549,10 +547,11 @@ __device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPo
     } else {
         x[0] = X::rows(a, n, pair_at, lift);
     }
-    expert_sums<H, W, X, RT, TT, WK, 1>(
+    expert_sums<T, W, X, RT, TT, WK, 1>(
         rows, x, a.d_ff, lds,
         [&] {
-            find_lifts<H, WK>(a, n, pair_at, lift);
+            if (MX && threadIdx.x < 16 * RT) tops[threadIdx.x] = top;
+            find_lifts<T, WK>(a, n, pair_at, lift);
             if constexpr (SHARED) {
                 C::Turned::stage(xs, a, n, pair_at, lift, a.d_ff, pitch);
                 __syncthreads();
@@ -566,7 +565,7 @@ __device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPo
                 float q[C::kPieces];
 #pragma unroll
                 for (int j = 0; j < C::kPieces; ++j) q[j] = acc[j % C::kTiles][c];
-                v[c] = join_pieces<H>(q);
+                v[c] = join_pieces<T>(q);
             }
             return v;
         });
@@ -584,7 +583,7 @@ __device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPo
                 float s[P];
 #pragma unroll
                 for (int j = 0; j < P; ++j) s[j] = q[j][c];
-                v[c] = join_pieces<H>(s);
+                v[c] = join_pieces<T>(s);
             }
         } else {
             v = joined<RT, WK>(lds, i, lane);
@@ -592,7 +591,8 @@ __device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPo
         const int at = list[pair];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            v[c] = EW::unscale(Pieces<H>::kScaled ? __builtin_amdgcn_ldexpf(v[c], -lift[pair]) : v[c], p.t2, d + c);
+            const int up = (MX ? T::exponent(tops[i * 16 + group * 4 + c]) : 0) - (Pieces<T>::kScaled ? lift[pair] : 0);
+            if (MX || Pieces<T>::kScaled) v[c] = __builtin_amdgcn_ldexpf(v[c], up);
             if (p.b2) v[c] += (float)((const typename T::elem*)p.b2)[d + c];
         }
         const uint4_t q = __builtin_bit_cast(uint4_t, v);
@@ -605,7 +605,7 @@ __device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPo
 // are loaded past them, and each block waits for its stores before it counts its pairs.  One token through 2 of 8 fp16 experts 1024 -> 4096: 8.3 us
 // (16.8 MB; dividing its k among two or four blocks is no faster); 13 tokens as above: 37 us, 5.2 TB/s; 64 as above: 18 us.
 template <class T, bool MX, bool SHARED, int RT, int WK, bool FEW>
-__global__ __launch_bounds__(64 * WK, FEW ? 4 : 3) void moe_layer_second_kernel(MoeLayerArgs a)
+__global__ __launch_bounds__(64 * WK, FEW || WK == 8 ? 4 : 3) void moe_layer_second_kernel(MoeLayerArgs a)
 {
     typedef SecondColumns<T, MX, SHARED, FEW> C;
     __shared__ ExpertLds<typename C::W, typename C::X, RT, WK, 1> lds;
@@ -616,7 +616,7 @@ __global__ __launch_bounds__(64 * WK, FEW ? 4 : 3) void moe_layer_second_kernel(
     const int first = blockIdx.z * C::kPairs, left = pairs_of(a.chosen, a.tokens * a.top_k, blockIdx.y, lds.list, &lds.count) - first;
     if (left <= 0) return;
     const int n = left < C::kPairs ? left : C::kPairs;
-    moe_second<T, MX, SHARED, RT, WK, FEW>(a, p, lds.list + first, n, lift, xs, lds.turn);
+    moe_second<T, MX, SHARED, RT, WK, FEW>(a, p, lds.list + first, n, lift, lds.tops, xs, lds.turn);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) before = __hip_atomic_fetch_add(&a.counters[blockIdx.x], (unsigned int)n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);

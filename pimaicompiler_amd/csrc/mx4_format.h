@@ -42,13 +42,15 @@ struct F16 {
     typedef half8_t frag;
     static constexpr int kLift = 12;
     static __device__ __forceinline__ float4_t mfma(const frag a, const frag b, const float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-    static __device__ __forceinline__ float scale(unsigned int code, int top)
+    // What `scale` takes of a row's top, and the power of two that its sums are multiplied by.
+    static __device__ __forceinline__ int prepared(int top) { return top - 127 - kLift; }
+    static __device__ __forceinline__ int exponent(int top) { return top - 127 - kLift; }
+    static __device__ __forceinline__ float scale(unsigned int code, int row)
     {
         // (no code is above its row's top, and 254 stands for one that was written there later: 255 is the exponent of infinities and NaN)
-        const int e = (int)code - top + 127 + kLift;
+        const int e = (int)code - row;
         return __builtin_bit_cast(float, code == kMxNan ? 0x7fc00000u : (unsigned int)(e < 0 ? 0 : e > 254 ? 254 : e) << 23);
     }
-    static __device__ __forceinline__ float unscale(float v, int top) { return __builtin_amdgcn_ldexpf(v, top - 127 - kLift); }
     static __device__ __forceinline__ frag from_mx4(unsigned int d, float s)
     {
         const half2_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, s, 1);
@@ -62,13 +64,13 @@ struct BF16 {
     typedef bf16_t elem;
     typedef bf16x8_t frag;
     static __device__ __forceinline__ float4_t mfma(const frag a, const frag b, const float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-    static __device__ __forceinline__ int above(int top) { return top > 252 ? top - 252 : 0; }
-    static __device__ __forceinline__ float scale(unsigned int code, int top)
+    static __device__ __forceinline__ int exponent(int top) { return top > 252 ? top - 252 : 0; }
+    static __device__ __forceinline__ int prepared(int top) { return exponent(top) << 23; }
+    static __device__ __forceinline__ float scale(unsigned int code, int row)
     {
-        const int e = (int)code - above(top);
-        return mx_scale_f32(code == kMxNan ? code : (unsigned int)(e > 0 ? e : 0));
+        const int bits = (int)(code << 23) - row;  // (below 2^-127: 2^-127)
+        return __builtin_bit_cast(float, code == kMxNan ? 0x7fc00000 : bits > 0x00400000 ? bits : 0x00400000);
     }
-    static __device__ __forceinline__ float unscale(float v, int top) { return __builtin_amdgcn_ldexpf(v, above(top)); }
     static __device__ __forceinline__ frag from_mx4(unsigned int d, float s)
     {
         const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 1);

@@ -61,7 +61,7 @@ __global__ __launch_bounds__(64 * GN * GT * KS) void mx4_linear_tile_kernel(cons
         xp[i] = x + (t < M ? t : M - 1) * ld_x;
     }
     const uint8_t *wp[kW], *sp[kW];
-    int top[kW];
+    int row_of[kW];
     const int wc = tid % 4;
 #pragma unroll
     for (int i = 0; i < kW; ++i) {
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(64 * GN * GT * KS) void mx4_linear_tile_kernel(cons
         n = n < w.rows ? n : w.rows - 1;
         wp[i] = w.packed + (n * blocks + wc) * kMxBlockBytes;
         sp[i] = w.scales + n * w.ld_scales + wc;
-        top[i] = w.tops[n];
+        row_of[i] = T::prepared(w.tops[n]);
     }
     frag xv[kX];
     uint4_t wv[kW];
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(64 * GN * GT * KS) void mx4_linear_tile_kernel(cons
             for (int i = 0; i < kW; ++i) {
                 const int r = (tid + i * kThreads) / 4;
                 ws[r * 4 + (wc ^ (r / 4 & 3))] = wv[i];
-                ss[wc][r] = T::scale(code[i], top[i]);
+                ss[wc][r] = T::scale(code[i], row_of[i]);
             }
         }
         __syncthreads();
@@ -164,12 +164,12 @@ __global__ __launch_bounds__(64 * GN * GT * KS) void mx4_linear_tile_kernel(cons
         const int64_t n = n0 + (wn + i) * 16 + group * 4;
         if (n >= w.rows) continue;
         const int count = w.rows - n < 4 ? (int)(w.rows - n) : 4;
-        int tops[4] = {};
+        int exponent[4] = {};
         float add[4] = {};
 #pragma unroll
         for (int c = 0; c < 4; ++c)
             if (c < count) {
-                tops[c] = w.tops[n + c];
+                exponent[c] = T::exponent(w.tops[n + c]);
                 if (bias) add[c] = (float)bias[n + c];
             }
 #pragma unroll
@@ -179,7 +179,7 @@ __global__ __launch_bounds__(64 * GN * GT * KS) void mx4_linear_tile_kernel(cons
             float4_t v = acc[i][j];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                v[c] = T::unscale(v[c], tops[c]);
+                v[c] = __builtin_amdgcn_ldexpf(v[c], exponent[c]);
                 if (bias) v[c] += add[c];
                 if (relu) v[c] = relu_f32(v[c]);
             }
