@@ -30,7 +30,7 @@ __device__ __forceinline__ float mx_scale_f32(unsigned int code)
     return __builtin_bit_cast(float, bits > 0x00400000u ? bits : 0x00400000u);
 }
 
-// The 16-bit types of activations.  `scale` of a row of 4-bit weights that meets them on the matrix cores:
+// The 16-bit types of activations.  `scale` of a block in a row of 4-bit weights that meets them on the matrix cores:
 //   bfloat16 has the range of every scale but the two largest, whose elements 4 and 6, or 2 to 6, are above it: elements are converted
 //   with their block's own scale, exactly; in a row whose largest code is 253 or 254 with a half or a quarter of it, which the sum is
 //   multiplied by at the end (such a row's blocks of codes 0 and 1, 2^-252 of its largest, come out larger by that).
@@ -42,13 +42,12 @@ struct F16 {
     typedef half8_t frag;
     static constexpr int kLift = 12;
     static __device__ __forceinline__ float4_t mfma(const frag a, const frag b, const float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-    // What `scale` takes of a row's top, and the power of two that its sums are multiplied by.
-    static __device__ __forceinline__ int prepared(int top) { return top - 127 - kLift; }
+    // The power of two that a row's sums are multiplied by.
     static __device__ __forceinline__ int exponent(int top) { return top - 127 - kLift; }
-    static __device__ __forceinline__ float scale(unsigned int code, int row)
+    static __device__ __forceinline__ float scale(unsigned int code, int top)
     {
         // (no code is above its row's top, and 254 stands for one that was written there later: 255 is the exponent of infinities and NaN)
-        const int e = (int)code - row;
+        const int e = (int)code - top + 127 + kLift;
         return __builtin_bit_cast(float, code == kMxNan ? 0x7fc00000u : (unsigned int)(e < 0 ? 0 : e > 254 ? 254 : e) << 23);
     }
     static __device__ __forceinline__ frag from_mx4(unsigned int d, float s)
@@ -65,10 +64,10 @@ struct BF16 {
     typedef bf16x8_t frag;
     static __device__ __forceinline__ float4_t mfma(const frag a, const frag b, const float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ int exponent(int top) { return top > 252 ? top - 252 : 0; }
-    static __device__ __forceinline__ int prepared(int top) { return exponent(top) << 23; }
-    static __device__ __forceinline__ float scale(unsigned int code, int row)
+    static __device__ __forceinline__ float scale(unsigned int code, int top)
     {
-        const int bits = (int)(code << 23) - row;  // (below 2^-127: 2^-127)
+        const int lower = (int)code - top + 252;
+        const int bits = (lower < (int)code ? lower : (int)code) << 23;  // (below 2^-127: 2^-127)
         return __builtin_bit_cast(float, code == kMxNan ? 0x7fc00000 : bits > 0x00400000 ? bits : 0x00400000);
     }
     static __device__ __forceinline__ frag from_mx4(unsigned int d, float s)

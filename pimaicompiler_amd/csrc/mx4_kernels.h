@@ -175,7 +175,7 @@ __global__ __launch_bounds__(64 * WK) void mx4_linear_skinny_kernel(const typena
     typedef typename std::conditional<SHARED, SharedTokens<T>, TurnedTokens<T, false>>::type X;
     constexpr int kLds = kSkinnyLds<W, X>, kPart = RT * TT * 64;
     __shared__ uint4_t lds[WK * (kLds > kPart ? kLds : kPart)];
-    __shared__ int exponents[RT * 16];
+    __shared__ int tops[RT * 16];
     __shared__ float add[RT * 16];
     extern __shared__ uint4_t xs[];
     const int lane = threadIdx.x & 63, wave = wave_in_block(), group = lane >> 4;
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(64 * WK) void mx4_linear_skinny_kernel(const typena
     if (threadIdx.x < 16 * RT) {
         int64_t n = row0 + threadIdx.x;
         n = n < w.rows ? n : w.rows - 1;
-        exponents[threadIdx.x] = T::exponent(w.tops[n]);
+        tops[threadIdx.x] = w.tops[n];
         add[threadIdx.x] = bias ? (float)bias[n] : 0.0f;
     }
     float4_t acc[RT][TT] = {};
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(64 * WK) void mx4_linear_skinny_kernel(const typena
             float4_t v = acc[i][j];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                v[c] = __builtin_amdgcn_ldexpf(v[c], exponents[i * 16 + group * 4 + c]);
+                v[c] = __builtin_amdgcn_ldexpf(v[c], T::exponent(tops[i * 16 + group * 4 + c]));
                 if (bias) v[c] += add[i * 16 + group * 4 + c];  // (a zero that is no bias would turn -0 into 0)
                 if (relu) v[c] = relu_f32(v[c]);
             }

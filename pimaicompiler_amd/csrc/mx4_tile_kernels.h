@@ -61,7 +61,7 @@ __global__ __launch_bounds__(64 * GN * GT * KS) void mx4_linear_tile_kernel(cons
         xp[i] = x + (t < M ? t : M - 1) * ld_x;
     }
     const uint8_t *wp[kW], *sp[kW];
-    int row_of[kW];
+    int top[kW];
     const int wc = tid % 4;
 #pragma unroll
     for (int i = 0; i < kW; ++i) {
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(64 * GN * GT * KS) void mx4_linear_tile_kernel(cons
         n = n < w.rows ? n : w.rows - 1;
         wp[i] = w.packed + (n * blocks + wc) * kMxBlockBytes;
         sp[i] = w.scales + n * w.ld_scales + wc;
-        row_of[i] = T::prepared(w.tops[n]);
+        top[i] = w.tops[n];
     }
     frag xv[kX];
     uint4_t wv[kW];
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(64 * GN * GT * KS) void mx4_linear_tile_kernel(cons
             for (int i = 0; i < kW; ++i) {
                 const int r = (tid + i * kThreads) / 4;
                 ws[r * 4 + (wc ^ (r / 4 & 3))] = wv[i];
-                ss[wc][r] = T::scale(code[i], row_of[i]);
+                ss[wc][r] = T::scale(code[i], top[i]);
             }
         }
         __syncthreads();

@@ -120,7 +120,7 @@ struct Mx4Weights {
         const uint8_t* base;
         const uint8_t* codes;
         unsigned int at[S], codes_at;  // bytes from there to the lane's rows' blocks and codes
-        int row;                       // what scales of row l % 16 are relative to
+        int top;                       // the largest scale code of row l % 16
     };
     struct Raw {
         uint4_t v[S];
@@ -142,7 +142,7 @@ struct Mx4Weights {
 #pragma unroll
         for (int j = 0; j < S; ++j) r.at[j] = row(lane / kRow + 16 / S * j) * (unsigned int)pitch + lane % kRow * kMxBlockBytes;
         r.codes_at = row(lane / 4) * (unsigned int)ld_scales + (lane & 3) * S;
-        r.row = T::prepared(tops[first + row(lane & 15)]);
+        r.top = tops[first + row(lane & 15)];
         return r;
     }
     static __device__ __forceinline__ void load(Raw& w, const Rows& r, int unit)
@@ -178,7 +178,7 @@ struct Mx4Weights {
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             o.v[s] = lds[place(row, s * 4 + group)];
-            o.scale[s] = T::scale((codes[s] >> (8 * group)) & 255u, r.row);
+            o.scale[s] = T::scale((codes[s] >> (8 * group)) & 255u, r.top);
         }
         wave_lds_order();
     }
