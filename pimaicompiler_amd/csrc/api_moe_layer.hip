@@ -112,8 +112,8 @@ void launch(const Plan* p, MoeLayerArgs& a, hipStream_t s)
             p->gated ? launch_first<T, MX, S, true, 1, 1>(a, staged, s) : launch_first<T, MX, S, false, 2, 1>(a, staged, s);
     };
     // Where experts have more than 16 pairs, which some have from 10 on the average on, 32 of them a block read their weights half as often.
-    // In us a call, 32 / 16 pairs a block, 64 tokens through 8 experts 1024 -> 4096, two chosen: gated in 4 bits 41.3 / 44.7, gated fp16 64 / 79, fp16
-    // 51 / 54; 16 tokens through both of 2 experts 512 -> 1024, which have 16 pairs at the most, 17.9 / 15.9.
+    // In us a call, 32 / 16 pairs a block, 64 tokens through 8 experts 1024 -> 4096, two chosen: gated in 4 bits 44.4 / 48.7, gated fp16 63 / 73, fp16
+    // 49.5 / 52.8; 16 tokens through both of 2 experts 512 -> 1024, which have 16 pairs at the most, 17.6 / 14.8.
     const int pairs = a.tokens * a.top_k;
     if (many && pairs > 10 * a.E)
         p->gated ? launch_first<T, MX, false, true, 2, 2>(a, 0, s) : launch_first<T, MX, false, false, 4, 2>(a, 0, s);
@@ -131,8 +131,8 @@ void launch(const Plan* p, MoeLayerArgs& a, hipStream_t s)
     const int border = MX ? (blocks >= 2048 ? 5 : 7) : Pieces<T>::kCount > 2 ? 3 : 5;
     if (pairs > border * a.E) {
         if constexpr (!MX) {
-            // (16-bit weights are four times the bytes: 64 tokens through 8 fp16 experts 1024 -> 4096 46.5 with eight wavefronts and a tile, 51 with two
-            // tiles and four; in 4 bits 46.0 / 41.3, the values being turned for each tile of rows)
+            // (16-bit weights are four times the bytes: 64 tokens through 8 fp16 experts 1024 -> 4096 49.5 with eight wavefronts and a tile, 53.7 with two
+            // tiles and four; in 4 bits 48.4 / 44.4, the values being turned for each tile of rows)
             if (blocks < 2048) return launch_second<T, MX, 1, 8, false>(a, most, s);
         }
         launch_second<T, MX, 2, 4, false>(a, most, s);

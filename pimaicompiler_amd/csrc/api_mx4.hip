@@ -86,8 +86,11 @@ int linear(void* out, int64_t ld_out, const void* x, int64_t ld_x, int64_t M, co
     }
     // Large tiles read operands less often, small ones fill the card.  Measured, 256 x 128 / 128 x 64, in us: 4096 x 16384 x 4096 532 / 634,
     // 2048 x 4096 x 4096 (256 large tiles) 70 / 86, 1500 x 4608 x 4096 (216) 68 / 84, 1500 x 4096 x 4096 (192) 68 / 65, 200 x 16384 x 4096 (128)
-    // 67 / 48, 512 x 4096 x 4096 (64) 67 / 34.  Up to 64 tokens the kernel of few tokens is faster: 64 x 16384 x 4096 22 (tiles 35), 40 x 4096 x
-    // 4096 13 (34).
+    // 67 / 48, 512 x 4096 x 4096 (64) 67 / 34.
+    // The kernel of few tokens ends at 64, where a block of it does; that is not where tiles become faster.  Tiles / that kernel with more blocks of
+    // tokens: 64 x 16384 x 4096 35 / 22, 65 x 16384 x 4096 32 / 43, 128 x 16384 x 4096 33 / 45, but 65 x 4096 x 4096 29 / 16, 128 x 4096 x 4096 29 / 17,
+    // 200 x 4096 x 4096 29 / 30, 65 x 1024 x 1024 11.0 / 4.4, 512 x 512 x 4096 28 / 9.5, 300 x 300 x 14000 94 / 38, 65 x 17 x 16384 92 / 18: a tile does all of
+    // its k in one block, so where tiles are far fewer than CUs the time is that of k, whatever the tokens.
     auto tiled = [&](auto kernel, int rows, int tokens, int threads) {
         const int64_t tiles = ((w.rows + rows - 1) / rows) * ((M + tokens - 1) / tokens);
         const int rc = check_grid(tiles, 1, threads);

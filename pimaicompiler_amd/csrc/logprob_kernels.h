@@ -8,6 +8,7 @@
 // Alternatives: the threads form 64 groups; the k-th largest of the groups' best (value, piece) is a bound that at least k values
 // reach, so only pieces of threads whose own best reaches it are looked at again (out of the caches).  What reaches the bound goes to
 // LDS, some more than k values as a rule, and is ranked there; ties go to the lowest index.
+// exp of a value's distance d to m by __expf, off by (1 + |d|) 2^-23 of itself: at most 2^-23 of the row's largest term, since (1 + |d|) e^d <= 1.
 // 509 rows of 100003 bf16 logits: 23 us without alternatives (4.4 TB/s; the eight vector instructions and the exponential of a value take about
 // 15 of it), 32 with 20 of them: all rows are at work at once, so that the few dependent steps at their ends are not hidden.  Asking for four
 // pieces while the four before are looked at: 33.  One row of 32000: 8 us, the steps' latencies.

@@ -497,9 +497,9 @@ __device__ __forceinline__ void moe_first(const MoeLayerArgs& a, const ExpertPoi
 
 // Block (x, y, z): rows x of expert y for 16 TT of its pairs, from 16 TT z on; those of more pairs read the weights again, out of the
 // caches.  (A loop over pairs in one block instead costs so many registers that half the wavefronts fit: 39 us against 25 for 64 tokens
-// through 8 gated 4-bit experts 1024 -> 4096, before blocks had twice the rows.)  That case takes 18 us now with TT 2, 35.7 MB; a block's chain of
+// through 8 gated 4-bit experts 1024 -> 4096, before blocks had twice the rows.)  That case takes 19.5 us now with TT 2, 35.7 MB; a block's chain of
 // loads (its pairs, then weights and values, k being a unit or two a wavefront) is what it waits for.  13 tokens through 64 gated bf16 experts 2048 -> 1024, six
-// chosen: 61 us, 6.3 TB/s.
+// chosen: 61 us, 5.5 TB/s.
 template <class T, bool MX, bool SHARED, bool GATED, int F, int WK, int TT>
 __global__ __launch_bounds__(64 * WK, TT > 1 ? 2 : F > 2 || (GATED && F > 1) ? 3 : 4) void moe_layer_first_kernel(MoeLayerArgs a)
 {
@@ -602,8 +602,8 @@ __device__ __forceinline__ void moe_second(const MoeLayerArgs& a, const ExpertPo
 
 // Blocks as above, with kPairs pairs.  The one whose pairs are the last of a tile of rows makes the weighted sum there, in the order of the choice.
 // An expert without a share adds nothing, whatever it computed.  Sums of other blocks come from other XCDs: they were stored past the L2s and
-// are loaded past them, and each block waits for its stores before it counts its pairs.  One token through 2 of 8 fp16 experts 1024 -> 4096: 8.3 us
-// (16.8 MB; dividing its k among two or four blocks is no faster); 13 tokens as above: 37 us, 5.2 TB/s; 64 as above: 18 us.
+// are loaded past them, and each block waits for its stores before it counts its pairs.  One token through 2 of 8 fp16 experts 1024 -> 4096: 8.5 us
+// (16.8 MB; dividing its k among two or four blocks is no faster); 13 tokens as above: 34 us, 5.0 TB/s; 64 as above: 22 us.
 template <class T, bool MX, bool SHARED, int RT, int WK, bool FEW>
 __global__ __launch_bounds__(64 * WK, FEW || WK == 8 ? 4 : 3) void moe_layer_second_kernel(MoeLayerArgs a)
 {

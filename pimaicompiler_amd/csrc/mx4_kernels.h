@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint8_t* pack
 // ---- x in 16 bits, weights in 4: a few tokens --------------------------------------------------------------------------------
 // y[m, n] = act(sum_k x[m, k] w[n, k] + b[n]).  WK wavefronts share k of 16 * RT rows and up to 16 * TT tokens (skinny.h).  SHARED: the
 // tokens (at most 16) lie in LDS as a whole, in the launch's dynamic part of it.  Bound by the weights' bytes: 16384 x 4096 for one token
-// 8.1 us, 4.4 TB/s; 31999 x 1024 for 16 tokens 6.8 us, 2.6 TB/s, a block's chain of loads being half of that.  What was measured to choose
+// 8.1 us, 4.4 TB/s; 31999 x 1024 for 16 tokens 7.0 us, 2.5 TB/s, a block's chain of loads being half of that.  What was measured to choose
 // the tile and the wavefronts stands with the rule that chooses.
 template <class T, bool SHARED, int RT, int TT, int WK>
 __global__ __launch_bounds__(64 * WK) void mx4_linear_skinny_kernel(const typename T::elem* x, Mx4View w, const typename T::elem* bias, typename T::elem* out,
@@ -230,7 +230,8 @@ __global__ __launch_bounds__(64 * WK) void mx4_linear_skinny_kernel(const typena
 // ---- both operands in 4 bits: a few rows of a --------------------------------------------------------------------------------
 // y[m, n] = sum_k a[m, k] b[n, k] on v_mfma_scale_f32_16x16x128_f8f6f4, which multiplies the scales in: 16 rows of b and 16 of a
 // a product, one block and its scale code a lane.  Bound by latency or by b's bytes: 1024 x 1024 for one row 2.9 us, 16384 x 4096 for 16 rows
-// 12.4 us, 2.9 TB/s (operands are read as the instruction wants them, 16 bytes of 16 rows a request each).
+// 12.4 us, 2.9 TB/s (operands are read as the instruction wants them, 16 bytes of 16 rows
+// a request each; loading runs of a row and turning them, as skinny.h does, has not been tried here).
 template <class O, int RT, int TT, int WK>
 __global__ __launch_bounds__(64 * WK) void mx4_matmul_skinny_kernel(Mx4View a, Mx4View b, typename O::elem* out, int64_t ld_out)
 {

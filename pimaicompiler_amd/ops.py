@@ -156,7 +156,7 @@ class _Launch:
     """`with _Launch(device, stream, *tensors) as handle`: the device is the current one inside, `stream` (None, a torch stream or an integer
     handle) torch's current stream, and `handle` its hipStream_t.  What a call allocates inside belongs to the stream it
     launches on, also where that is not the caller's current one; the memory of `tensors`, which the call reads, is not given to others
-    before a stream that was asked for is done with it."""
+    before a stream that was asked for is done with it (so the stream behind an integer handle has to live until they are freed)."""
 
     def __init__(self, device, stream, *tensors):
         self._device, self._tensors = device, tensors
