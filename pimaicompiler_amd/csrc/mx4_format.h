@@ -67,7 +67,7 @@ struct BF16 {
     static __device__ __forceinline__ float scale(unsigned int code, int top)
     {
         const int lower = (int)code - top + 252;
-        const int bits = (lower < (int)code ? lower : (int)code) << 23;  // (below 2^-127: 2^-127)
+        const int bits = (lower < (int)code ? lower : (int)code) * (1 << 23);  // (below 2^-127: 2^-127)
         return __builtin_bit_cast(float, code == kMxNan ? 0x7fc00000 : bits > 0x00400000 ? bits : 0x00400000);
     }
     static __device__ __forceinline__ frag from_mx4(unsigned int d, float s)
