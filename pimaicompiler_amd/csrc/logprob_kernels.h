@@ -150,14 +150,19 @@ __global__ __launch_bounds__(THREADS) void token_log_probs_kernel(LogProbArgs a)
         t = f * (t + s * step);
         s *= f;
         m = mn;
+        float ps[4], pt[4];  // (a row's sums grow by a piece's: fewer roundings of what they have)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
+            ps[i] = pt[i] = 0.0f;
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
                 const float d = v[i][c] - m, e = __expf(d);
-                s += e;
-                t = fmaf(e, fmaxf(d, kFarBelow), t);
+                ps[i] += e;
+                pt[i] = fmaf(e, fmaxf(d, kFarBelow), pt[i]);
             }
+        }
+        s += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+        t += (pt[0] + pt[1]) + (pt[2] + pt[3]);
     });
 
     // ---- the row's m, s, t ----
