@@ -581,6 +581,97 @@ int pimhip_moe_layer_forward(PimHipMoeLayerPlan* plan, const void* x, int64_t ld
 int pimhip_token_log_probs(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t vocab, const void* tokens, int tokens_int64, int top,
                            float* logp, float* entropy, float* top_logp, int* top_ids, void* stream);
 
+/* ---- a cache of keys and values in pages ----------------------------------------------------------- */
+
+/* No counterpart in the reference, whose attention reads an encoder's outputs (pimhip_decoder_step).  A layer's keys and values of all
+ * sequences lie in pages of `page_size` tokens; a table names each sequence's pages in order. */
+
+/* The type of a cache in 8 bits (E4M3 of the OCP: largest 448, no infinities) beside PIMHIP_F16 and PIMHIP_BF16. */
+enum { PIMHIP_F8E4M3 = 3 };
+
+/* [pages, kv_heads, page_size, head_dim] keys and values in the caller's device memory (this struct itself lies on the host).  Strides in
+ * elements from page to page, head to head and token to token; a head's values lie next to each other.  head_dim: a multiple of 8 (of 16 in 8 bits)
+ * up to 256; page_size up to 65536.  k_scale and v_scale [kv_heads]: an 8-bit value times its head's scale is what it stands for;
+ * NULL for 16-bit caches. */
+typedef struct PimHipPagedCache {
+    void* k;
+    void* v;
+    const float* k_scale;
+    const float* v_scale;
+    int64_t k_strides[3];
+    int64_t v_strides[3];
+    int64_t pages;
+    int kv_heads, page_size, head_dim;
+    int dtype; /* PIMHIP_F16, PIMHIP_BF16 or PIMHIP_F8E4M3 */
+} PimHipPagedCache;
+
+/* page_table [sequences, table_width] (pitch ld_table) and lengths [sequences]: tokens of each sequence, those of this call among them.  A row's
+ * entries behind its sequence's last page may be anything; a page outside of the cache is none: its tokens are not stored and not seen. */
+typedef struct PimHipPagedBatch {
+    const int* page_table;
+    const int* lengths;
+    int64_t ld_table;
+    int sequences, table_width;
+} PimHipPagedBatch;
+
+/* [tokens, heads, head_dim], strides in elements. */
+typedef struct PimHipPagedRows {
+    const void* data;
+    int64_t token_stride, head_stride;
+} PimHipPagedRows;
+
+/* Stores k and v [tokens, kv_heads, head_dim] (dtype PIMHIP_F16 or PIMHIP_BF16; the cache is of the same type or in 8 bits).  starts [sequences + 1],
+ * rising: tokens starts[s] .. starts[s + 1] - 1 are the last of sequence s, others are nobody's; NULL: one token for each sequence.  A token at a
+ * position outside of 0 .. table_width * page_size - 1 is not stored.
+ * rotary_dim > 0: the first rotary_dim values of each key, and of each query q [tokens, q_heads, head_dim] (q may be NULL), are turned in pairs by
+ * the token's position, in fp32: values i and rotary_dim / 2 + i, or 2 i and 2 i + 1 if interleaved, by angles[position, i] (cosines) and
+ * angles[position, rotary_dim / 2 + i] (sines); angles has table_width * page_size rows at least.  Queries go to q_out [tokens, q_heads, head_dim],
+ * zeros for a token that is nobody's or at no position.
+ * 16-bit values are rounded once; 8-bit ones are x / scale, rounded once, saturating at 448.  Two tokens of a call that are given the same place
+ * leave either's values there, each of eight by itself. */
+int pimhip_paged_append(const PimHipPagedCache* cache, const PimHipPagedBatch* batch, const int* starts, int64_t tokens, const PimHipPagedRows* k,
+                        const PimHipPagedRows* v, const PimHipPagedRows* q, int q_heads, void* q_out, int dtype, const float* angles, int64_t angle_rows,
+                        int64_t ld_angles, int rotary_dim, int interleaved, void* stream);
+
+/* What pimhip_paged_attend needs in `workspace`; it depends on sizes only. */
+int pimhip_paged_attend_workspace_bytes(const PimHipPagedCache* cache, const PimHipPagedBatch* batch, int q_heads, uint64_t* bytes);
+
+/* out[s, h] = softmax over the tokens j of sequence s of (scale * q[s, h] . k[j, h'])  times  v[j, h'], h' = h / (q_heads / kv_heads): attention of one new
+ * token of each sequence, q and out [sequences, q_heads, head_dim] (out dense).  window > 0: the last `window` tokens only.  lse [sequences, q_heads] or
+ * NULL: the logarithm of the sum of the softmax's exponentials.  Sums, statistics and the weights of the values are fp32, out is rounded once.  A
+ * sequence without tokens: zeros, lse -inf.  What lies in places that are not seen, NaN included, has no influence.
+ * Allocates and synchronises nothing.  The workspace is the call's until it has run: calls that may overlap, and captured graphs that are replayed
+ * at the same time, need one each. */
+int pimhip_paged_attend(const PimHipPagedCache* cache, const PimHipPagedBatch* batch, const PimHipPagedRows* q, int q_heads, int dtype, float scale,
+                        int window, void* out, float* lse, void* workspace, void* stream);
+
+/* ---- sampling ----------------------------------------------------------------------------------- */
+
+/* A row's setting: one for each row in device memory, or (NULL) one number for all. */
+typedef struct PimHipSampleSettings {
+    const float* temperatures;
+    const int* top_ks;
+    const float* top_ps;
+    const float* min_ps;
+    float temperature;
+    int top_k;
+    float top_p;
+    float min_p;
+} PimHipSampleSettings;
+
+/* Draws a token from each row of logits [rows, vocab] (dtype: any PimHipDataType, pitch ld elements; vocab up to 2^21) by a number uniform[row] in [0, 1).
+ * w = exp((x - max x) / temperature).  Of the tokens in falling order of x, equal ones by their index,
+ *   top_k > 0      the first top_k stay;
+ *   top_p < 1      of them those before which less than top_p of their sum has been reached, the first always;
+ *   min_p > 0      of them those with w >= min_p.
+ * tokens[row] (int64) is the first in the order of indices at which the running sum of w over what stayed exceeds uniform[row] times the whole,
+ * logp[row] the logarithm of its share of it.  temperature 0: the first of the largest.  Weights are worked out to 2^-38 of themselves and summed exactly in
+ * whole numbers of 64 bits, so results do not depend on an order of work.
+ * A row with a NaN or +inf, of a temperature that is negative, infinite or NaN, or of a NaN elsewhere in its settings or its number: token -1 and
+ * logp NaN; a row of -inf alone: -1 and -inf.  A number outside of [0, 1) is taken as the nearest in it. */
+int pimhip_sample_tokens(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t vocab, const float* uniform, const PimHipSampleSettings* settings,
+                         int64_t* tokens, float* logp, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

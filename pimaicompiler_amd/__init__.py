@@ -39,3 +39,5 @@ from .ops import (  # noqa: F401
 from .mx4 import Mx4Tensor, mx4_dequantize, mx4_linear, mx4_matmul, mx4_quantize  # noqa: F401
 from .log_probs import token_log_probs  # noqa: F401
 from .moe_layer import MoeLayerPlan  # noqa: F401
+from .paged import PagedCache, rotary_table  # noqa: F401
+from .sampling import sample_tokens  # noqa: F401

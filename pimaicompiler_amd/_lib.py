@@ -28,6 +28,29 @@ class MoeLayerDesc(ctypes.Structure):
                 ("renormalize", ctypes.c_int)]
 
 
+class PagedCache(ctypes.Structure):
+    """PimHipPagedCache."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("k_strides", ctypes.c_int64 * 3),
+                ("v_strides", ctypes.c_int64 * 3), ("pages", ctypes.c_int64), ("kv_heads", ctypes.c_int), ("page_size", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("dtype", ctypes.c_int)]
+
+
+class PagedBatch(ctypes.Structure):
+    """PimHipPagedBatch."""
+    _fields_ = [("page_table", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("ld_table", ctypes.c_int64), ("sequences", ctypes.c_int), ("table_width", ctypes.c_int)]
+
+
+class PagedRows(ctypes.Structure):
+    """PimHipPagedRows."""
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class SampleSettings(ctypes.Structure):
+    """PimHipSampleSettings."""
+    _fields_ = [("temperatures", ctypes.c_void_p), ("top_ks", ctypes.c_void_p), ("top_ps", ctypes.c_void_p), ("min_ps", ctypes.c_void_p), ("temperature", ctypes.c_float),
+                ("top_k", ctypes.c_int), ("top_p", ctypes.c_float), ("min_p", ctypes.c_float)]
+
+
 c_mx4_p = ctypes.POINTER(Mx4Matrix)
 
 # name -> (restype, argtypes); must list every function include/pimhip.h declares.
@@ -127,6 +150,14 @@ SIGNATURES = {
     "pimhip_token_log_probs": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
                                               ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                               ctypes.c_void_p]),
+    "pimhip_paged_append": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(PagedBatch), ctypes.c_void_p, ctypes.c_int64, ctypes.POINTER(PagedRows),
+                                           ctypes.POINTER(PagedRows), ctypes.POINTER(PagedRows), ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
+                                           ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]),
+    "pimhip_paged_attend_workspace_bytes": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(PagedBatch), ctypes.c_int, ctypes.POINTER(ctypes.c_uint64)]),
+    "pimhip_paged_attend": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(PagedBatch), ctypes.POINTER(PagedRows), ctypes.c_int, ctypes.c_int, ctypes.c_float,
+                                           ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "pimhip_sample_tokens": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
+                                            ctypes.POINTER(SampleSettings), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "pimhip_mx4_matmul": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, c_mx4_p, c_mx4_p, ctypes.c_void_p]),
 }
 
@@ -142,6 +173,7 @@ PIMHIP_ACT_RELU = 1
 PIMHIP_I_X_W = 0
 PIMHIP_W_X_I = 1
 PIMHIP_F16, PIMHIP_BF16, PIMHIP_F32 = 0, 1, 2
+PIMHIP_F8E4M3 = 3
 PIMHIP_EXPERT_NONE, PIMHIP_EXPERT_RELU, PIMHIP_EXPERT_SILU = 0, 1, 2
 GEMM_UNKNOWN, GEMM_VV, GEMM_MV, GEMM_VM, GEMM_MM = 0, 1, 2, 3, 4
 

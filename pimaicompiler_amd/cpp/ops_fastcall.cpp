@@ -520,6 +520,183 @@ PyObject* moeLayer(PyObject*, PyObject* const* args, Py_ssize_t n)
     return out;
 }
 
+// ---- paged caches and sampling ----------------------------------------------------------------------------------------------
+bool realOf(PyObject* o, float& v)
+{
+    if (!PyFloat_CheckExact(o)) return false;
+    v = static_cast<float>(PyFloat_AS_DOUBLE(o));
+    return true;
+}
+
+// A contiguous int32 tensor of `dims` dimensions on the cache's device.
+bool indicesOf(PyObject* o, int64_t dims, int64_t device, const at::Tensor*& t)
+{
+    if (!THPVariable_Check(o)) return false;
+    t = &THPVariable_Unpack(o);
+    return t->defined() && t->is_cuda() && t->layout() == at::kStrided && t->dim() == dims && t->device().index() == device && t->scalar_type() == at::kInt &&
+           t->is_contiguous();
+}
+
+// [tokens, heads, the cache's head size] of a type that goes with the cache, the values of a head next to each other.
+bool pagedRowsOf(PyObject* o, const PimHipPagedCache* c, int64_t device, const at::Tensor*& t, PimHipPagedRows& rows)
+{
+    if (!plainTensor(o, t) || t->dim() != 3 || t->device().index() != device || t->size(1) < 1 || t->size(2) != c->head_dim || t->stride(2) != 1) return false;
+    const int code = typeCode(t->scalar_type());
+    if (code == PIMHIP_F32 || code < 0 || (c->dtype != PIMHIP_F8E4M3 && c->dtype != code)) return false;
+    rows = PimHipPagedRows{t->data_ptr(), t->stride(0), t->stride(1)};
+    return true;
+}
+
+// page_table and lengths as both calls take them.
+bool pagedBatchOf(PyObject* table, PyObject* lengths, int64_t device, PimHipPagedBatch& batch)
+{
+    const at::Tensor *t, *n;
+    if (!indicesOf(table, 2, device, t) || !indicesOf(lengths, 1, device, n) || t->size(0) != n->size(0) || t->size(1) < 1 || t->size(1) > INT32_MAX ||
+        n->size(0) > INT32_MAX)
+        return false;
+    batch = PimHipPagedBatch{static_cast<const int*>(t->data_ptr()), static_cast<const int*>(n->data_ptr()), t->size(1), (int)n->size(0), (int)t->size(1)};
+    return true;
+}
+
+const PimHipPagedCache* pagedCacheOf(PyObject* o) { return PyLong_Check(o) ? static_cast<const PimHipPagedCache*>(PyLong_AsVoidPtr(o)) : nullptr; }
+
+// paged_append(cache, its device index, k, v, page_table, lengths, starts or None, q or None, rotary or None, interleaved): (q turned or None,)
+PyObject* pagedAppend(PyObject*, PyObject* const* args, Py_ssize_t n)
+{
+    int64_t device;
+    PimHipPagedBatch batch;
+    PimHipPagedRows kr, vr, qr;
+    const at::Tensor *k, *v, *q = nullptr, *starts = nullptr, *rotary = nullptr;
+    if (n != 10) return none();
+    const PimHipPagedCache* c = pagedCacheOf(args[0]);
+    if (!c || !intOf(args[1], device) || device != c10::hip::current_device() || !pagedRowsOf(args[2], c, device, k, kr) || !pagedRowsOf(args[3], c, device, v, vr) ||
+        !pagedBatchOf(args[4], args[5], device, batch))
+        return none();
+    if (k->size(1) != c->kv_heads || v->sizes() != k->sizes() || v->scalar_type() != k->scalar_type()) return none();
+    if (args[6] != Py_None ? !indicesOf(args[6], 1, device, starts) || starts->size(0) != batch.sequences + 1 : k->size(0) != batch.sequences) return none();
+    if (args[8] != Py_None && (!plainTensor(args[8], rotary) || rotary->scalar_type() != at::kFloat || rotary->dim() != 2 || !rotary->is_contiguous() ||
+                               rotary->device().index() != device || rotary->size(1) < 2 || rotary->size(1) % 2 || rotary->size(1) > c->head_dim ||
+                               rotary->size(0) < (int64_t)batch.table_width * c->page_size))
+        return none();
+    if (args[7] != Py_None && (!rotary || !pagedRowsOf(args[7], c, device, q, qr) || q->size(0) != k->size(0) || q->scalar_type() != k->scalar_type())) return none();
+    if (args[9] != Py_True && args[9] != Py_False) return none();
+    at::Tensor out;
+    if (q) out = newTensor(q->sizes(), q->scalar_type(), q->device());
+    int rc;
+    void* stream = currentStream();
+    Py_BEGIN_ALLOW_THREADS
+    rc = pimhip_paged_append(c, &batch, starts ? static_cast<const int*>(starts->data_ptr()) : nullptr, k->size(0), &kr, &vr, q ? &qr : nullptr, q ? (int)q->size(1) : 0,
+                             q ? out.data_ptr() : nullptr, typeCode(k->scalar_type()), rotary ? static_cast<const float*>(rotary->data_ptr()) : nullptr,
+                             rotary ? rotary->size(0) : 0, rotary ? rotary->size(1) : 0, rotary ? (int)rotary->size(1) : 0, args[9] == Py_True, stream);
+    Py_END_ALLOW_THREADS
+    if (rc != PIMHIP_OK) return status(rc);
+    PyObject* result = PyTuple_New(1);
+    if (!result) return nullptr;
+    PyTuple_SET_ITEM(result, 0, q ? THPVariable_Wrap(std::move(out)) : none());
+    return result;
+}
+
+// paged_attend(cache, its device index, q, page_table, lengths, scale, window, lse): out, or (out, lse)
+PyObject* pagedAttend(PyObject*, PyObject* const* args, Py_ssize_t n)
+{
+    int64_t device, window;
+    float scale;
+    PimHipPagedBatch batch;
+    PimHipPagedRows qr;
+    const at::Tensor* q;
+    if (n != 8) return none();
+    const PimHipPagedCache* c = pagedCacheOf(args[0]);
+    if (!c || !intOf(args[1], device) || device != c10::hip::current_device() || !pagedRowsOf(args[2], c, device, q, qr) || !pagedBatchOf(args[3], args[4], device, batch) ||
+        !realOf(args[5], scale) || !(scale - scale == 0.0f) || !PyLong_CheckExact(args[6]) || !intOf(args[6], window) || window < 0 || window > INT32_MAX ||
+        (args[7] != Py_True && args[7] != Py_False))
+        return none();
+    if (q->size(0) != batch.sequences || q->size(1) % c->kv_heads || q->size(1) > 65535) return none();
+    uint64_t bytes = 0;
+    int rc = pimhip_paged_attend_workspace_bytes(c, &batch, (int)q->size(1), &bytes);
+    if (rc != PIMHIP_OK) return status(rc);
+    at::Tensor out = newTensor(q->sizes(), q->scalar_type(), q->device()), workspace = newTensor({(int64_t)bytes}, at::kByte, q->device()), lse;
+    if (args[7] == Py_True) lse = newTensor(q->sizes().slice(0, 2), at::kFloat, q->device());
+    void* stream = currentStream();
+    Py_BEGIN_ALLOW_THREADS
+    rc = pimhip_paged_attend(c, &batch, &qr, (int)q->size(1), typeCode(q->scalar_type()), scale, (int)window, out.data_ptr(),
+                             lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr, workspace.data_ptr(), stream);
+    Py_END_ALLOW_THREADS
+    if (rc != PIMHIP_OK) return status(rc);
+    if (!lse.defined()) return THPVariable_Wrap(std::move(out));
+    PyObject* result = PyTuple_New(2);
+    if (!result) return nullptr;
+    PyTuple_SET_ITEM(result, 0, THPVariable_Wrap(std::move(out)));
+    PyTuple_SET_ITEM(result, 1, THPVariable_Wrap(std::move(lse)));
+    return result;
+}
+
+// A setting of sampling: a number that is allowed, or a contiguous tensor of one for each row.
+template <class V>
+bool settingOf(PyObject* o, const at::Tensor& logits, at::ScalarType type, V most, const V*& each, V& one)
+{
+    if (THPVariable_Check(o)) {
+        const at::Tensor* t;
+        if (!THPVariable_Check(o)) return false;
+        t = &THPVariable_Unpack(o);
+        if (!t->defined() || t->scalar_type() != type || t->device() != logits.device() || t->sizes() != logits.sizes().slice(0, logits.dim() - 1) || !t->is_contiguous() ||
+            (t->requires_grad() && at::GradMode::is_enabled()) || (type == at::kFloat && t->_fw_grad(0).defined()))
+            return false;
+        each = static_cast<const V*>(t->data_ptr());
+        return true;
+    }
+    if constexpr (std::is_same<V, float>::value) {
+        double v;
+        if (PyFloat_CheckExact(o))
+            v = PyFloat_AS_DOUBLE(o);
+        else if (PyLong_CheckExact(o))
+            v = PyLong_AsDouble(o);
+        else
+            return false;
+        if (PyErr_Occurred()) {
+            PyErr_Clear();
+            return false;
+        }
+        if (!(v >= 0.0 && v <= most)) return false;
+        one = static_cast<float>(v);
+    } else {
+        int64_t v;
+        if (!PyLong_CheckExact(o) || !intOf(o, v) || v < 0 || v > most) return false;
+        one = static_cast<V>(v);
+    }
+    return true;
+}
+
+// sample_tokens(logits, uniform, temperature, top_k, top_p, min_p): (tokens, logp)
+PyObject* sampleTokens(PyObject*, PyObject* const* args, Py_ssize_t n)
+{
+    const at::Tensor* x;
+    int64_t rows, cols, ld;
+    if (n != 6 || !plainTensor(args[0], x) || typeCode(x->scalar_type()) < 0 || !rowsOf(*x, rows, cols, ld) || cols > (1 << 21) || !THPVariable_Check(args[1])) return none();
+    const at::IntArrayRef lead = x->sizes().slice(0, x->dim() - 1);
+    const at::Tensor& u = THPVariable_Unpack(args[1]);
+    if (!u.defined() || u.scalar_type() != at::kFloat || u.device() != x->device() || u.sizes() != lead || !u.is_contiguous() ||
+        (u.requires_grad() && at::GradMode::is_enabled()) || u._fw_grad(0).defined())
+        return none();
+    PimHipSampleSettings s{};
+    const float largest = 3.4e38f;
+    if (!settingOf<float>(args[2], *x, at::kFloat, largest, s.temperatures, s.temperature) || !settingOf<int>(args[3], *x, at::kInt, INT32_MAX, s.top_ks, s.top_k) ||
+        !settingOf<float>(args[4], *x, at::kFloat, 1.0f, s.top_ps, s.top_p) || !settingOf<float>(args[5], *x, at::kFloat, 1.0f, s.min_ps, s.min_p))
+        return none();
+    at::Tensor tokens = newTensor(lead, at::kLong, x->device()), logp = newTensor(lead, at::kFloat, x->device());
+    int rc;
+    void* stream = currentStream();
+    Py_BEGIN_ALLOW_THREADS
+    rc = pimhip_sample_tokens(x->data_ptr(), typeCode(x->scalar_type()), ld, rows, cols, static_cast<const float*>(u.data_ptr()), &s,
+                              static_cast<int64_t*>(tokens.data_ptr()), static_cast<float*>(logp.data_ptr()), stream);
+    Py_END_ALLOW_THREADS
+    if (rc != PIMHIP_OK) return status(rc);
+    PyObject* out = PyTuple_New(2);
+    if (!out) return nullptr;
+    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(tokens)));
+    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(logp)));
+    return out;
+}
+
 // ---- bound steps: the buffers of a one-launch step, fixed once, and the call that issues it ---------------------------------
 constexpr const char* kBoundStep = "pimaicompiler_amd.bound_step";
 struct BoundStep {
@@ -651,6 +828,8 @@ void addFastcalls(PyObject* module)
                                     method<issue>("issue"),                method<mx4Quantize>("fast_mx4_quantize"),
                                     method<mx4Dequantize>("fast_mx4_dequantize"), method<mx4Linear>("fast_mx4_linear"),
                                     method<mx4Matmul>("fast_mx4_matmul"),  method<logProbs>("fast_log_probs"),
-                                    method<moeLayer>("fast_moe_layer"),    {nullptr, nullptr, 0, nullptr}};
+                                    method<moeLayer>("fast_moe_layer"),
+                                    method<pagedAppend>("fast_paged_append"), method<pagedAttend>("fast_paged_attend"),
+                                    method<sampleTokens>("fast_sample_tokens"), {nullptr, nullptr, 0, nullptr}};
     if (PyModule_AddFunctions(module, methods) != 0) throw pybind11::error_already_set();
 }

@@ -1,0 +1,45 @@
+// Sampling, of the C ABI (include/pimhip.h).
+#include "api_common.h"
+#include "sample_kernels.h"
+
+using namespace pimhip;
+
+extern "C" int pimhip_sample_tokens(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t vocab, const float* uniform, const PimHipSampleSettings* settings,
+                                    int64_t* tokens, float* logp, void* stream)
+{
+    DeviceState* st = nullptr;
+    const int rc = current_device_state(&st);
+    if (rc != PIMHIP_OK) return rc;
+    if (rows < 0 || rows > INT32_MAX || vocab < 1 || vocab > kSampleMost)
+        return fail(PIMHIP_ERR_INVALID_ARGUMENT, "rows=%lld, vocab=%lld (at most %d)", (long long)rows, (long long)vocab, kSampleMost);
+    if (dtype != PIMHIP_F16 && dtype != PIMHIP_BF16 && dtype != PIMHIP_F32) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "dtype=%d", dtype);
+    if (!settings) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "settings must be non-null");
+    const int threads = vocab <= 2048 ? 256 : 1024;
+    if (rows * threads > UINT32_MAX) return fail(PIMHIP_ERR_UNSUPPORTED, "%lld rows are too many for one launch", (long long)rows);
+    if (rows == 0) return PIMHIP_OK;
+    if (!logits || (rows > 1 && ld < vocab)) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "logits is null, or ld=%lld is less than vocab=%lld", (long long)ld, (long long)vocab);
+    if (!uniform || !tokens || !logp) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "uniform, tokens and logp must be non-null");
+    auto off = [](const void* p, uintptr_t size) { return (reinterpret_cast<uintptr_t>(p) & (size - 1)) != 0; };
+    if (off(logits, dtype == PIMHIP_F32 ? 4 : 2) || off(uniform, 4) || off(tokens, 8) || off(logp, 4) || off(settings->temperatures, 4) || off(settings->top_ks, 4) ||
+        off(settings->top_ps, 4) || off(settings->min_ps, 4))
+        return fail(PIMHIP_ERR_INVALID_ARGUMENT, "a pointer is not aligned to its elements");
+    SampleArgs a;
+    memset(&a, 0, sizeof(a));
+    a.logits = logits, a.ld = ld, a.uniform = uniform;
+    a.temperatures = settings->temperatures, a.top_ks = settings->top_ks, a.top_ps = settings->top_ps, a.min_ps = settings->min_ps;
+    a.temperature = settings->temperature, a.top_k = settings->top_k, a.top_p = settings->top_p, a.min_p = settings->min_p;
+    a.tokens = tokens, a.logp = logp, a.V = (int)vocab;
+    a.shift = 45;
+    while (vocab > (int64_t)1 << (62 - a.shift)) --a.shift;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    auto run = [&](auto type) {
+        typedef decltype(type) T;
+        if (threads == 256)
+            sample_kernel<T, 256><<<dim3((unsigned)rows), 256, 0, s>>>(a);
+        else
+            sample_kernel<T, 1024><<<dim3((unsigned)rows), 1024, 0, s>>>(a);
+    };
+    dtype == PIMHIP_F16 ? run(F16{}) : dtype == PIMHIP_BF16 ? run(BF16{}) : run(F32{});
+    PIMHIP_HIP_CHECK(hipGetLastError());
+    return PIMHIP_OK;
+}
