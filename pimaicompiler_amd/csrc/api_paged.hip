@@ -65,12 +65,14 @@ int cut_of(const PagedView& v, int group, int num_cus, AttendCut* cut)
     cut->tiles = group > 16 && v.dim <= 128 ? 2 : 1;  // (for longer heads the registers do not hold 32 results' sums)
     cut->tiles_of_heads = (group + 16 * cut->tiles - 1) / (16 * cut->tiles);
     const int64_t heads = (int64_t)v.kv_heads * cut->tiles_of_heads, units = (v.most + 15 + kUnit - 1) / kUnit;
-    if (heads * units > INT32_MAX || (int64_t)v.sequences * heads > (1 << 23))
+    if (heads * units > INT32_MAX || (int64_t)v.sequences * v.kv_heads * group > (1 << 23))
         return fail(PIMHIP_ERR_UNSUPPORTED, "%d sequences of up to %d tokens with %d key heads are too many for one launch", v.sequences, v.most, v.kv_heads);
-    const int64_t most = (int64_t)v.sequences * heads * units, wanted = 2 * (int64_t)num_cus;
+    const int64_t most = (int64_t)v.sequences * heads * units, wanted = attend_waves((v.dim + 63) / 64, cut->tiles) * (int64_t)num_cus;
     cut->blocks = (int)(most < wanted ? most : wanted);
     return PIMHIP_OK;
 }
+
+uint64_t part_bytes(const AttendCut& cut, int dim) { return (uint64_t)cut.blocks * 2 * 16 * cut.tiles * (dim + 4) * sizeof(float); }
 
 template <class T, bool FP8, int NC, int MT>
 void launch_attend(const AttendArgs& a, int blocks, hipStream_t s)
@@ -96,7 +98,7 @@ template <class T>
 void launch_attend(const AttendArgs& a, const AttendCut& cut, hipStream_t s)
 {
     a.c.k_scale ? launch_attend<T, true>(a, cut, s) : launch_attend<T, false>(a, cut, s);
-    paged_join_kernel<T><<<dim3(a.c.sequences * a.c.kv_heads * a.tiles_of_heads), 256, 0, s>>>(a, cut.blocks, 16 * cut.tiles);
+    paged_join_kernel<T><<<dim3(a.c.sequences * a.c.kv_heads * a.group), 256, 0, s>>>(a, 16 * cut.tiles);
 }
 }  // namespace
 
@@ -155,7 +157,7 @@ extern "C" int pimhip_paged_attend_workspace_bytes(const PimHipPagedCache* cache
     if (!bytes || q_heads < 1 || q_heads % v.kv_heads || q_heads > 65535) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "q_heads=%d with %d key heads, or bytes is null", q_heads, v.kv_heads);
     AttendCut cut;
     if ((rc = cut_of(v, q_heads / v.kv_heads, st->num_cus, &cut)) != PIMHIP_OK) return rc;
-    *bytes = (uint64_t)cut.blocks * 2 * 16 * cut.tiles * (v.dim + 4) * sizeof(float);
+    *bytes = part_bytes(cut, v.dim) + (uint64_t)v.sequences * v.kv_heads * cut.tiles_of_heads * sizeof(int2);
     return PIMHIP_OK;
 }
 
@@ -181,6 +183,7 @@ extern "C" int pimhip_paged_attend(const PimHipPagedCache* cache, const PimHipPa
         return fail(PIMHIP_ERR_INVALID_ARGUMENT, "out and lse must be aligned to their elements, workspace to 16 bytes");
     a.q = q->data, a.q_seq = q->token_stride, a.q_head = q->head_stride;
     a.out = out, a.lse = lse, a.work = static_cast<float*>(workspace);
+    a.pieces = reinterpret_cast<int2*>(static_cast<char*>(workspace) + part_bytes(cut, a.c.dim));
     a.group = q_heads / a.c.kv_heads, a.tiles_of_heads = cut.tiles_of_heads, a.window = window;
     a.scale_log2 = scale * 1.4426950408889634f;
     hipStream_t s = static_cast<hipStream_t>(stream);

@@ -182,11 +182,21 @@ struct AttendArgs {
     const void* q;
     void* out;
     float* lse;   // [sequences, heads] or null
-    float* work;  // [blocks][2][16 * tiles][dim + 4]
+    float* work;  // [blocks][2][16 * tiles][dim + 4]: sums, then their maximum and weight
+    int2* pieces; // [sequences * kv_heads * tiles_of_heads]: the first and the last block that worked on each
     int64_t q_seq, q_head;  // elements
     int group, tiles_of_heads, window;
     float scale_log2;
 };
+
+// Four results of a head, and its sum's logarithm beside the first.
+template <class T>
+__device__ __forceinline__ void store_attended(const AttendArgs& a, int64_t head, int d, const float4_t sum, float weight, float top, float scale)
+{
+    const float f = weight == 0.0f ? 0.0f : scale / weight;
+    store4<T>((typename T::elem*)a.out + head * a.c.dim + d, sum * f, 4);
+    if (a.lse && d == 0) a.lse[head] = (top + __builtin_amdgcn_logf(weight)) * 0.6931471805599453f;
+}
 
 struct PagedSpan {
     int first, base, end, units;  // tokens first .. end - 1 are seen; tiles begin at base
@@ -276,12 +286,12 @@ struct ValuePiece {
     unsigned int w[kWords];
     __device__ __forceinline__ void load(const char* p)
     {
-        typedef unsigned int words_t __attribute__((ext_vector_type(kWords)));
-        typedef words_t words_any_t __attribute__((aligned(1)));
         if constexpr (kWords == 1) {
             typedef unsigned int word_any_t __attribute__((aligned(1)));
             w[0] = load_global<word_any_t>(p);
         } else {
+            typedef unsigned int words_t __attribute__((ext_vector_type(kWords)));
+            typedef words_t words_any_t __attribute__((aligned(1)));
             const words_t q = load_global<words_any_t>(p);
 #pragma unroll
             for (int i = 0; i < kWords; ++i) w[i] = q[i];
@@ -297,7 +307,7 @@ struct ValuePiece {
         if constexpr (FP8) {
             const float2_t two = i % 4 < 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(w[i / 4], false) : __builtin_amdgcn_cvt_pk_f32_fp8(w[i / 4], true);
             return two[i % 2];
-        } else if constexpr (sizeof(typename T::elem) == 2 && __is_same(T, BF16)) {
+        } else if constexpr (__is_same(T, BF16)) {
             return __builtin_bit_cast(float, i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
         } else {
             return (float)__builtin_bit_cast(half2_t, w[i / 2])[i % 2];
@@ -305,9 +315,13 @@ struct ValuePiece {
     }
 };
 
+// Wavefronts of a SIMD that the registers are bounded for, and tiles whose loads are in flight (below).
+constexpr int attend_waves(int nc, int mt) { return nc <= 2 && mt == 1 ? 3 : 2; }
+constexpr int attend_depth(bool fp8, int nc, int mt) { return fp8 && nc <= 2 && mt == 1 ? 2 : 1; }
+
 // NC: the head's size in 64 columns, rounded up; MT: 16 query heads each; ONE: pages are whole tiles of 16 tokens.
 template <class T, bool FP8, int NC, int MT, bool ONE>
-__global__ __launch_bounds__(256, 2) void paged_attend_kernel(AttendArgs a)
+__global__ __launch_bounds__(256, attend_waves(NC, MT)) void paged_attend_kernel(AttendArgs a)
 {
     typedef typename T::elem elem;
     typedef typename T::frag frag;
@@ -315,8 +329,9 @@ __global__ __launch_bounds__(256, 2) void paged_attend_kernel(AttendArgs a)
     constexpr int kLoads = FP8 ? NC : kSteps;        // 16-byte loads of a key's row by a lane
     constexpr int kWide = NC / 2, kNarrow = NC % 2;  // pieces of eight and of four columns of a lane
     constexpr int kCols = NC * 4, kSize = FP8 ? 1 : 2;
+    constexpr int kDepth = attend_depth(FP8, NC, MT);
     __shared__ float wave_m[4][16 * MT], wave_l[4][16 * MT];
-    __shared__ float parts[2][16 * MT][NC * 64 + 4];
+    __shared__ float parts[4][16 * MT][NC * 64 + 4];
     const int lane = threadIdx.x & 63, wave = wave_in_block(), n = lane & 15, g = lane >> 4;
     const PagedView& c = a.c;
     const int D = c.dim;
@@ -369,64 +384,72 @@ __global__ __launch_bounds__(256, 2) void paged_attend_kernel(AttendArgs a)
         }
 
         // ---- tiles: 16 tokens of each unit ----
-        uint4_t k[kLoads];
-        ValuePiece<T, FP8, 8> wide[4][kWide ? kWide : 1];
-        ValuePiece<T, FP8, 4> narrow[4][kNarrow ? kNarrow : 1];
+        uint4_t k[kDepth][kLoads];
+        ValuePiece<T, FP8, 8> wide[kDepth][4][kWide ? kWide : 1];
+        ValuePiece<T, FP8, 4> narrow[kDepth][4][kNarrow ? kNarrow : 1];
+        unsigned int page_ok[kDepth];  // a bit for each token of a tile
         // This wavefront's first token of a unit; a unit behind the stretch's end has none.
         auto token_of = [&](int unit) { return unit < last ? span.base + unit * kUnit + wave * 16 : span.end; };
-        // A tile's page (ONE), or the page of each of its 16 tokens (a lane each, the same in the four groups); -1: none.
-        auto page_at = [&](int token) {
-            const int mine = token + (ONE ? 0 : n);
-            return token < span.end && mine < span.end ? row[c.page_of(mine)] : -1;
+        // Pages: a lane has that of one of the next 64 tiles (ONE), or of a token of one of the next 4; the group after that is on its way.
+        constexpr int kGroup = ONE ? 64 : 4;
+        auto pages_of = [&](int unit) {
+            const int first_token = token_of(unit + (ONE ? lane : g)), token = first_token + (ONE ? 0 : n);
+            return first_token < span.end && token < span.end ? row[c.page_of(token)] : -1;
         };
-        // Where they lie: a page that is none is read as page 0, and not seen.
-        struct Place {
-            int page, in;
-            unsigned int ok;  // a bit for each token
-        };
-        auto place_of = [&](int token, int page) {
-            const int mine = token + (ONE ? 0 : n);
-            const bool ok = page >= 0 && page < c.pages;
-            return Place{ok ? page : 0, mine - c.page_of(mine) * c.page_size, ONE ? (ok ? 0xffffu : 0u) : (unsigned int)__ballot(ok) & 0xffffu};
-        };
-        auto load_keys = [&](const Place& p) {
-            const char* kp = kh + p.page * c.k_page + (int64_t)(p.in + (ONE ? n : 0)) * c.k_tok;
+        int ids = pages_of(first), ids_next = pages_of(first + kGroup);
+        // The loads of a unit's tile, in two parts: its place and keys, its values.  A page that is none is read as page 0, and not seen.
+        int page = 0, in = 0;
+        auto load_keys = [&](int j, int unit) {
+            const int token = token_of(unit), i = (unit - first) & (kGroup - 1);
+            if (i == 0 && unit != first) {
+                ids = ids_next;
+                ids_next = pages_of(unit + kGroup);
+            }
+            if constexpr (ONE) {
+                const int id = __builtin_amdgcn_readlane(ids, i);
+                const bool ok = id >= 0 && id < c.pages;
+                page_ok[j] = ok ? 0xffffu : 0u;
+                page = ok ? id : 0;
+                in = token - c.page_of(token) * c.page_size;
+            } else {
+                const int id = __shfl(ids, i * 16 + n);
+                const bool ok = id >= 0 && id < c.pages;
+                page_ok[j] = (unsigned int)__ballot(ok) & 0xffffu;
+                page = ok ? id : 0;
+                in = token + n - c.page_of(token + n) * c.page_size;
+            }
+            const char* kp = ONE ? kh + page * c.k_page + in * c.k_tok + (unsigned int)(n * c.k_tok + g * 16) : kh + page * c.k_page + in * c.k_tok + g * 16;
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                const int byte = i * 64 + g * 16;
-                k[i] = uint4_t{0, 0, 0, 0};
-                if (byte < D * kSize) k[i] = load_global<uint4_any_t>(kp + byte);
+                k[j][i] = uint4_t{0, 0, 0, 0};
+                if (i * 64 + g * 16 < D * kSize) k[j][i] = load_global<uint4_any_t>(kp + i * 64);
             }
         };
-        auto load_values = [&](const Place& p, int r) {
-            const int page = ONE ? p.page : __shfl(p.page, g * 4 + r), in = ONE ? p.in + g * 4 + r : __shfl(p.in, g * 4 + r);
-            const char* vp = vh + page * c.v_page + (int64_t)in * c.v_tok;
+        auto load_values = [&](int j, int r) {
+            const char* vp = ONE ? vh + page * c.v_page + (in + r) * c.v_tok + (unsigned int)(g * 4 * c.v_tok)
+                                 : vh + __shfl(page, g * 4 + r) * c.v_page + __shfl(in, g * 4 + r) * c.v_tok;
 #pragma unroll
             for (int i = 0; i < kWide; ++i) {
-                wide[r][i].clear();
-                if (i * 128 + n * 8 < D) wide[r][i].load(vp + (i * 128 + n * 8) * kSize);
+                wide[j][r][i].clear();
+                if (i * 128 + n * 8 < D) wide[j][r][i].load(vp + (i * 128 + n * 8) * kSize);
             }
             if constexpr (kNarrow) {
-                narrow[r][0].clear();
-                if (kWide * 128 + n * 4 < D) narrow[r][0].load(vp + (kWide * 128 + n * 4) * kSize);
+                narrow[j][r][0].clear();
+                if (kWide * 128 + n * 4 < D) narrow[j][r][0].load(vp + (kWide * 128 + n * 4) * kSize);
             }
         };
-
-        int token = token_of(first), next = token_of(first + 1);
-        Place place = place_of(token < span.end ? token : span.base, page_at(token));
-        if (token < span.end) {
-            load_keys(place);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) load_values(place, r);
-        }
-        int page = page_at(next);
-        for (int unit = first; token < span.end; ++unit) {
-            const bool more = next < span.end;
-            const Place then = place_of(more ? next : span.base, page);
-            const int next2 = token_of(unit + 2);
-            page = page_at(next2);
+        for (int j = 0; j < kDepth; ++j)
+            if (token_of(first + j) < span.end) {
+                load_keys(j, first + j);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) load_values(j, r);
+            }
+        auto tile = [&](int j, int unit) {
+            const int token = token_of(unit);
+            const bool more = token_of(unit + kDepth) < span.end;
             // Tokens that are not the sequence's, or not in the window, or of no page, are left out, whatever lies there.
-            unsigned int seen = place.ok;
+            unsigned int seen = page_ok[j];
             if (token < span.first) seen &= 0xffffu << (span.first - token);
             if (token + 16 > span.end) seen &= 0xffffu >> (token + 16 - span.end);
 
@@ -437,13 +460,13 @@ __global__ __launch_bounds__(256, 2) void paged_attend_kernel(AttendArgs a)
             for (int i = 0; i < kSteps; ++i) {
                 frag kf;
                 if constexpr (FP8)
-                    kf = from_e4m3x8<T>(i % 2 ? uint2_t{k[i / 2][2], k[i / 2][3]} : uint2_t{k[i / 2][0], k[i / 2][1]});
+                    kf = from_e4m3x8<T>(i % 2 ? uint2_t{k[j][i / 2][2], k[j][i / 2][3]} : uint2_t{k[j][i / 2][0], k[j][i / 2][1]});
                 else
-                    kf = __builtin_bit_cast(frag, k[i]);
+                    kf = __builtin_bit_cast(frag, k[j][i]);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) sc[mt] = T::mfma(kf, q[mt][i], sc[mt]);
             }
-            if (more) load_keys(then);
+            if (more) load_keys(j, unit + kDepth);
             bool above = false;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
@@ -482,33 +505,36 @@ __global__ __launch_bounds__(256, 2) void paged_attend_kernel(AttendArgs a)
                 }
                 if (seen != 0xffffu && !(seen >> (g * 4 + r) & 1)) {
 #pragma unroll
-                    for (int i = 0; i < kWide; ++i) wide[r][i].clear();
-                    if constexpr (kNarrow) narrow[r][0].clear();
+                    for (int i = 0; i < kWide; ++i) wide[j][r][i].clear();
+                    if constexpr (kNarrow) narrow[j][r][0].clear();
                 }
 #pragma unroll
                 for (int i = 0; i < kWide; ++i)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float v = wide[r][i].value(e);
+                        const float v = wide[j][r][i].value(e);
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) o[mt][i * 8 + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[mt], v, o[mt][i * 8 + e], 0, 0, 0);
                     }
                 if constexpr (kNarrow)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float v = narrow[r][0].value(e);
+                        const float v = narrow[j][r][0].value(e);
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt)
                             o[mt][kWide * 8 + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[mt], v, o[mt][kWide * 8 + e], 0, 0, 0);
                     }
-                if (more) load_values(then, r);
+                if (more) load_values(j, r);
             }
-            place = then;
-            token = next;
-            next = next2;
+        };
+        for (int unit = first; token_of(unit) < span.end; unit += kDepth) {
+#pragma unroll
+            for (int j = 0; j < kDepth; ++j)
+                if (j == 0 || token_of(unit + j) < span.end) tile(j, unit + j);
         }
 
-        // ---- the four wavefronts' parts ----
+        // ---- the four wavefronts' parts, joined by all of the block ----
+        const int rows = a.group - head0 < 16 * MT ? a.group - head0 : 16 * MT;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             l[mt] += __shfl_xor(l[mt], 16);
@@ -517,77 +543,47 @@ __global__ __launch_bounds__(256, 2) void paged_attend_kernel(AttendArgs a)
                 wave_m[wave][mt * 16 + n] = m[mt];
                 wave_l[wave][mt * 16 + n] = l[mt];
             }
-        }
-        __syncthreads();
-        auto column = [&](int i) { return i < kWide * 8 ? i / 8 * 128 + n * 8 + i % 8 : kWide * 128 + n * 4 + i - kWide * 8; };
-        float all_l[MT][4], all_m[MT][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int h = mt * 16 + g * 4 + r;
-                const float top = fmaxf(fmaxf(wave_m[0][h], wave_m[1][h]), fmaxf(wave_m[2][h], wave_m[3][h]));
-                float sum = 0.0f, f = 0.0f;
+                if (h >= rows) continue;
+                float* part = parts[wave][h];
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const float fw = wave_m[w][h] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(wave_m[w][h] - top);
-                    sum += fw * wave_l[w][h];
-                    if (w == wave) f = fw;
-                }
-                all_m[mt][r] = top;
-                all_l[mt][r] = sum;
+                for (int i = 0; i < kWide; ++i)
 #pragma unroll
-                for (int i = 0; i < kCols; ++i) o[mt][i][r] *= f;
+                    for (int e = 0; e < 8; e += 4)
+                        *reinterpret_cast<float4_t*>(part + i * 128 + n * 8 + e) = float4_t{o[mt][i * 8 + e][r], o[mt][i * 8 + e + 1][r], o[mt][i * 8 + e + 2][r], o[mt][i * 8 + e + 3][r]};
+                if constexpr (kNarrow)
+                    *reinterpret_cast<float4_t*>(part + kWide * 128 + n * 4) =
+                        float4_t{o[mt][kWide * 8][r], o[mt][kWide * 8 + 1][r], o[mt][kWide * 8 + 2][r], o[mt][kWide * 8 + 3][r]};
             }
-        for (int half = 2; half >= 1; half /= 2) {
-            if (wave >= half && wave < 2 * half) {
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-#pragma unroll
-                        for (int i = 0; i < kCols; ++i) parts[wave - half][mt * 16 + g * 4 + r][column(i)] = o[mt][i][r];
-            }
-            __syncthreads();
-            if (wave < half) {
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-#pragma unroll
-                        for (int i = 0; i < kCols; ++i) o[mt][i][r] += parts[wave][mt * 16 + g * 4 + r][column(i)];
-            }
-            __syncthreads();
         }
-        if (wave == 0) {
-            const bool complete = first == 0 && last == span.units;
-            const float vs = FP8 ? c.v_scale[kvh] : 1.0f;
+        __syncthreads();
+        const bool complete = first == 0 && last == span.units;
+        const float vs = FP8 ? c.v_scale[kvh] : 1.0f;
+        const int64_t out0 = (int64_t)s * c.kv_heads * a.group + kvh * a.group + head0;
+        float* piece = a.work + ((int64_t)blockIdx.x * 2 + (first == 0 ? 1 : 0)) * 16 * MT * (D + 4);
+        const int each = D / 4;
+        for (int i = threadIdx.x; i < rows * each; i += 256) {
+            const int h = i / each, d = (i - h * each) * 4;
+            const float top = fmaxf(fmaxf(wave_m[0][h], wave_m[1][h]), fmaxf(wave_m[2][h], wave_m[3][h]));
+            float4_t sum = {0, 0, 0, 0};
+            float weight = 0.0f;
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int h = head0 + mt * 16 + g * 4 + r;
-                    if (h >= a.group) continue;
-                    if (complete) {
-                        const float f = all_l[mt][r] == 0.0f ? 0.0f : vs / all_l[mt][r];
-                        const int64_t at_out = (int64_t)s * c.kv_heads * a.group + kvh * a.group + h;
-                        elem* out = (elem*)a.out + at_out * D;
-#pragma unroll
-                        for (int i = 0; i < kCols; ++i)
-                            if (column(i) < D) out[column(i)] = T::round(o[mt][i][r] * f);
-                        if (a.lse && n == 0) a.lse[at_out] = (all_m[mt][r] + __builtin_amdgcn_logf(all_l[mt][r])) * 0.6931471805599453f;
-                    } else {
-                        float* part = a.work + (((int64_t)blockIdx.x * 2 + (first == 0 ? 1 : 0)) * 16 * MT + mt * 16 + g * 4 + r) * (D + 4);
-#pragma unroll
-                        for (int i = 0; i < kCols; ++i)
-                            if (column(i) < D) part[column(i)] = o[mt][i][r];
-                        if (n == 0) {
-                            part[D] = all_m[mt][r];
-                            part[D + 1] = all_l[mt][r];
-                        }
-                    }
-                }
+            for (int w = 0; w < 4; ++w) {
+                const float f = wave_m[w][h] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(wave_m[w][h] - top);
+                weight += f * wave_l[w][h];
+                sum += f * *reinterpret_cast<const float4_t*>(&parts[w][h][d]);
+            }
+            if (complete) {
+                store_attended<T>(a, out0 + h, d, sum, weight, top, vs);
+            } else {
+                *reinterpret_cast<float4_t*>(piece + h * (D + 4) + d) = sum;
+                if (d == 0) *reinterpret_cast<float2_t*>(piece + h * (D + 4) + D) = float2_t{top, weight};
+            }
         }
+        if (threadIdx.x == 0 && last == span.units) a.pieces[s * heads_of_units + hg] = int2{(int)((u - first) / per), (int)blockIdx.x};
+        __syncthreads();
         u += take;
         if (rel + take == heads_of_units * span.units) {
             before += span.units;
@@ -596,43 +592,62 @@ __global__ __launch_bounds__(256, 2) void paged_attend_kernel(AttendArgs a)
     }
 }
 
-// The pieces of each (sequence, key head) that more than one block worked on.  `blocks`: those of the kernel before.
+// The pieces of each (sequence, key head) that more than one block worked on: a block a head, its wavefronts a quarter of the pieces each.
 template <class T>
-__global__ __launch_bounds__(256) void paged_join_kernel(AttendArgs a, int blocks, int rows)
+__global__ __launch_bounds__(256) void paged_join_kernel(AttendArgs a, int rows)
 {
-    typedef typename T::elem elem;
     const PagedView& c = a.c;
-    const int D = c.dim;
-    const int hgs = c.kv_heads * a.tiles_of_heads, s = blockIdx.x / hgs, hg = blockIdx.x - s * hgs;
-    const PagedFound at = paged_find(c, a.window, hgs, [&](int64_t) { return (int64_t)-1 - s; });
-    const int units = paged_span(c, a.window, s).units;
-    const int64_t per = (at.total + blocks - 1) / blocks;
-    const int64_t u0 = at.before * hgs + (int64_t)hg * units;
-    const int b0 = (int)(u0 / per), b1 = (int)((u0 + units - 1) / per);
-    if (b0 == b1) return;
-    const int kvh = hg / a.tiles_of_heads, head0 = (hg - kvh * a.tiles_of_heads) * rows;
-    const int mine = a.group - head0 < rows ? a.group - head0 : rows, each = D / 4;
-    const float vs = c.v_scale ? c.v_scale[kvh] : 1.0f;
-    for (int i = threadIdx.x; i < mine * each; i += 256) {
-        const int h = i / each, d = (i - h * each) * 4;
-        // (a piece's place: the block's second where the sequence begins in it, else its first)
-        auto part = [&](int b) { return a.work + (((int64_t)b * 2 + (b == b0 ? 1 : 0)) * rows + h) * (D + 4); };
-        float top = -__builtin_inff();
-        for (int b = b0; b <= b1; ++b) top = fmaxf(top, part(b)[D]);
-        float4_t sum = {0, 0, 0, 0};
-        float l = 0.0f;
-        for (int b = b0; b <= b1; ++b) {
-            const float* p = part(b);
-            const float f = p[D] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(p[D] - top);
-            l += f * p[D + 1];
-            sum += f * *reinterpret_cast<const float4_t*>(p + d);
-        }
-        const float f = l == 0.0f ? 0.0f : vs / l;
-        const int64_t at_out = (int64_t)s * c.kv_heads * a.group + kvh * a.group + head0 + h;
-        elem* out = (elem*)a.out + at_out * D + d;
+    const int D = c.dim, heads = c.kv_heads * a.group;
+    const int s = blockIdx.x / heads, h_all = blockIdx.x - s * heads, kvh = h_all / a.group, h_in = h_all - kvh * a.group, tile = h_in / rows, h = h_in - tile * rows;
+    const int2 blocks = a.pieces[((int64_t)s * c.kv_heads + kvh) * a.tiles_of_heads + tile];
+    if (blocks.x == blocks.y) return;
+    __shared__ float wave_m[4], wave_l[4];
+    __shared__ float parts[4][256];
+    const int lane = threadIdx.x & 63, wave = wave_in_block(), d = lane * 4;
+    // (a piece's place: the block's second where the sequence begins in it, else its first)
+    auto part = [&](int b) { return a.work + (((int64_t)b * 2 + (b == blocks.x ? 1 : 0)) * rows + h) * (D + 4); };
+    float top = -__builtin_inff(), l = 0.0f;
+    float4_t sum = {0, 0, 0, 0};
+    for (int b = blocks.x + wave; b <= blocks.y; b += 16) {
+        float2_t ml[4];
+        float4_t v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) out[e] = T::round(sum[e] * f);
-        if (a.lse && d == 0) a.lse[at_out] = (top + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+        for (int i = 0; i < 4; ++i) {
+            const float* p = part(b + 4 * i <= blocks.y ? b + 4 * i : b);
+            ml[i] = *reinterpret_cast<const float2_t*>(p + D);
+            v[i] = d < D ? *reinterpret_cast<const float4_t*>(p + d) : float4_t{0, 0, 0, 0};
+        }
+        float now = top;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) now = fmaxf(now, ml[i][0]);
+        const float f = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(top - now);
+        l *= f;
+        sum *= f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (b + 4 * i > blocks.y) continue;
+            const float fi = ml[i][0] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ml[i][0] - now);
+            l += fi * ml[i][1];
+            sum += fi * v[i];
+        }
+        top = now;
     }
+    if (lane == 0) {
+        wave_m[wave] = top;
+        wave_l[wave] = l;
+    }
+    *reinterpret_cast<float4_t*>(&parts[wave][d]) = sum;
+    __syncthreads();
+    if (wave != 0 || d >= D) return;
+    const float all = fmaxf(fmaxf(wave_m[0], wave_m[1]), fmaxf(wave_m[2], wave_m[3]));
+    float weight = 0.0f;
+    sum = float4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float f = wave_m[w] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(wave_m[w] - all);
+        weight += f * wave_l[w];
+        sum += f * *reinterpret_cast<const float4_t*>(&parts[w][d]);
+    }
+    store_attended<T>(a, blockIdx.x, d, sum, weight, all, c.v_scale ? c.v_scale[kvh] : 1.0f);
 }
 }  // namespace pimhip
