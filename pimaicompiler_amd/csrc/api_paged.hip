@@ -56,49 +56,58 @@ int check_rows(const char* name, const PimHipPagedRows& r)
     return PIMHIP_OK;
 }
 
-// How an attention call is cut: 16 or 32 query heads at a time, blocks of its grid.
+// How an attention call is cut: query heads at a time, their tiles of a key head, blocks of its grid.
 struct AttendCut {
-    int tiles, tiles_of_heads, blocks;
+    int heads, tiles_of_heads, blocks;
 };
 int cut_of(const PagedView& v, int group, int num_cus, AttendCut* cut)
 {
-    cut->tiles = group > 16 && v.dim <= 128 ? 2 : 1;  // (for longer heads the registers do not hold 32 results' sums)
-    cut->tiles_of_heads = (group + 16 * cut->tiles - 1) / (16 * cut->tiles);
+    const int nc = (v.dim + 63) / 64;
+    // (for heads longer than 128 the registers do not hold 32 results' sums)
+    cut->heads = group <= 4 ? 4 : group <= 8 && nc <= 2 ? 8 : group > 16 && nc <= 2 ? 32 : 16;
+    cut->tiles_of_heads = (group + cut->heads - 1) / cut->heads;
     const int64_t heads = (int64_t)v.kv_heads * cut->tiles_of_heads, units = (v.most + 15 + kUnit - 1) / kUnit;
     if (heads * units > INT32_MAX || (int64_t)v.sequences * v.kv_heads * group > (1 << 23))
         return fail(PIMHIP_ERR_UNSUPPORTED, "%d sequences of up to %d tokens with %d key heads are too many for one launch", v.sequences, v.most, v.kv_heads);
-    const int64_t most = (int64_t)v.sequences * heads * units, wanted = attend_waves((v.dim + 63) / 64, cut->tiles) * (int64_t)num_cus;
+    const int64_t most = (int64_t)v.sequences * heads * units, wanted = attend_waves(v.k_scale != nullptr, nc, cut->heads) * (int64_t)num_cus;
     cut->blocks = (int)(most < wanted ? most : wanted);
     return PIMHIP_OK;
 }
 
-uint64_t part_bytes(const AttendCut& cut, int dim) { return (uint64_t)cut.blocks * 2 * 16 * cut.tiles * (dim + 4) * sizeof(float); }
+uint64_t part_bytes(const AttendCut& cut, int dim) { return (uint64_t)cut.blocks * 2 * cut.heads * (dim + 4) * sizeof(float); }
 
-template <class T, bool FP8, int NC, int MT>
+template <class T, bool FP8, int NC, int HT>
 void launch_attend(const AttendArgs& a, int blocks, hipStream_t s)
 {
-    if (a.c.page_size % 16 == 0)
-        paged_attend_kernel<T, FP8, NC, MT, true><<<dim3(blocks), 256, 0, s>>>(a);
+    if (a.c.page_size % 16 == 0 && a.c.dim == 64 * NC)
+        paged_attend_kernel<T, FP8, NC, HT, true><<<dim3(blocks), 256, 0, s>>>(a);
     else
-        paged_attend_kernel<T, FP8, NC, MT, false><<<dim3(blocks), 256, 0, s>>>(a);
+        paged_attend_kernel<T, FP8, NC, HT, false><<<dim3(blocks), 256, 0, s>>>(a);
+}
+template <class T, bool FP8, int NC>
+void launch_attend(const AttendArgs& a, const AttendCut& cut, hipStream_t s)
+{
+    if (cut.heads == 4) return launch_attend<T, FP8, NC, 4>(a, cut.blocks, s);
+    if constexpr (NC <= 2) {
+        if (cut.heads == 8) return launch_attend<T, FP8, NC, 8>(a, cut.blocks, s);
+        if (cut.heads == 32) return launch_attend<T, FP8, NC, 32>(a, cut.blocks, s);
+    }
+    launch_attend<T, FP8, NC, 16>(a, cut.blocks, s);
 }
 template <class T, bool FP8>
 void launch_attend(const AttendArgs& a, const AttendCut& cut, hipStream_t s)
 {
     const int nc = (a.c.dim + 63) / 64;
-    if (cut.tiles == 2)
-        nc == 1 ? launch_attend<T, FP8, 1, 2>(a, cut.blocks, s) : launch_attend<T, FP8, 2, 2>(a, cut.blocks, s);
-    else
-        nc == 1   ? launch_attend<T, FP8, 1, 1>(a, cut.blocks, s)
-        : nc == 2 ? launch_attend<T, FP8, 2, 1>(a, cut.blocks, s)
-        : nc == 3 ? launch_attend<T, FP8, 3, 1>(a, cut.blocks, s)
-                  : launch_attend<T, FP8, 4, 1>(a, cut.blocks, s);
+    nc == 1   ? launch_attend<T, FP8, 1>(a, cut, s)
+    : nc == 2 ? launch_attend<T, FP8, 2>(a, cut, s)
+    : nc == 3 ? launch_attend<T, FP8, 3>(a, cut, s)
+              : launch_attend<T, FP8, 4>(a, cut, s);
 }
 template <class T>
 void launch_attend(const AttendArgs& a, const AttendCut& cut, hipStream_t s)
 {
     a.c.k_scale ? launch_attend<T, true>(a, cut, s) : launch_attend<T, false>(a, cut, s);
-    paged_join_kernel<T><<<dim3(a.c.sequences * a.c.kv_heads * a.group), 256, 0, s>>>(a, 16 * cut.tiles);
+    paged_join_kernel<T><<<dim3(a.c.sequences * a.c.kv_heads * a.group), 256, 0, s>>>(a, cut.heads);
 }
 }  // namespace
 

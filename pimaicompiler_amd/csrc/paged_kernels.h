@@ -6,6 +6,8 @@
 //   attend    o = sum_j e_j v_j / sum_j e_j,  e_j = exp(scale q . k_j - m),  j over the sequence's last `window` tokens
 #pragma once
 
+#include <type_traits>
+
 #include "mx4_format.h"
 
 namespace pimhip
@@ -172,7 +174,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
 //   scores    K [16 tokens x dim] . Q^T [dim x 16 heads] on the 16-bit matrix instruction (8-bit keys become Q's type, exactly): a lane has
 //             the scores of head l % 16 and tokens 4 (l / 16) + r
 //   values    P [16 heads x 4 tokens] . V [4 tokens x 16 columns] on the 32-bit one, for tokens r, 4 + r, 8 + r, 12 + r: a lane's e_j are its
-//             operand as they are, unrounded, and V is one that 16 lanes read as one row: nothing is turned or exchanged
+//             operand as they are, unrounded, and V is one that 16 lanes read as one row: nothing is turned or exchanged.
+//             Where a key head has up to 8 query heads most of those 16 rows are empty: Q's columns repeat every 4 (8) heads then, and the
+//             matrix instruction of 16 blocks [4 heads x 1 token] . [1 x 4 columns] takes a lane's e_j and its own value of V, a quarter (half) of the
+//             time; the four groups of lanes have sums over tokens of their own, which are added at the end
 // Values lie in registers from memory on; a tile's loads are issued while the one before is worked on.
 static constexpr int kUnit = 64;           // tokens that the four wavefronts of a block take together
 static constexpr float kLazy = 40.0f;      // a running maximum moves on when a score is above it by so many powers of two
@@ -182,7 +187,7 @@ struct AttendArgs {
     const void* q;
     void* out;
     float* lse;   // [sequences, heads] or null
-    float* work;  // [blocks][2][16 * tiles][dim + 4]: sums, then their maximum and weight
+    float* work;  // [blocks][2][heads at a time][dim + 4]: sums, then their maximum and weight
     int2* pieces; // [sequences * kv_heads * tiles_of_heads]: the first and the last block that worked on each
     int64_t q_seq, q_head;  // elements
     int group, tiles_of_heads, window;
@@ -288,11 +293,11 @@ struct ValuePiece {
     {
         if constexpr (kWords == 1) {
             typedef unsigned int word_any_t __attribute__((aligned(1)));
-            w[0] = load_global<word_any_t>(p);
+            w[0] = load_global_once<word_any_t>(p);
         } else {
             typedef unsigned int words_t __attribute__((ext_vector_type(kWords)));
             typedef words_t words_any_t __attribute__((aligned(1)));
-            const words_t q = load_global<words_any_t>(p);
+            const words_t q = load_global_once<words_any_t>(p);
 #pragma unroll
             for (int i = 0; i < kWords; ++i) w[i] = q[i];
         }
@@ -316,12 +321,13 @@ struct ValuePiece {
 };
 
 // Wavefronts of a SIMD that the registers are bounded for, and tiles whose loads are in flight (below).
-constexpr int attend_waves(int nc, int mt) { return nc <= 2 && mt == 1 ? 3 : 2; }
-constexpr int attend_depth(bool fp8, int nc, int mt) { return fp8 && nc <= 2 && mt == 1 ? 2 : 1; }
+constexpr int attend_waves(bool fp8, int nc, int ht) { return nc <= 2 && ht <= 16 ? 3 : 2; }
+constexpr int attend_depth(bool fp8, int nc, int ht) { return 1; }
 
-// NC: the head's size in 64 columns, rounded up; MT: 16 query heads each; ONE: pages are whole tiles of 16 tokens.
-template <class T, bool FP8, int NC, int MT, bool ONE>
-__global__ __launch_bounds__(256, attend_waves(NC, MT)) void paged_attend_kernel(AttendArgs a)
+// NC: the head's size in 64 columns, rounded up; HT: query heads at a time (4, 8, 16 or 32); EVEN: pages are whole tiles of 16 tokens, and the head's size is NC of 64:
+// a tile's place is then the same for the wavefront, and no lane stays without loads.
+template <class T, bool FP8, int NC, int HT, bool EVEN>
+__global__ __launch_bounds__(256, attend_waves(FP8, NC, HT)) void paged_attend_kernel(AttendArgs a)
 {
     typedef typename T::elem elem;
     typedef typename T::frag frag;
@@ -329,9 +335,12 @@ __global__ __launch_bounds__(256, attend_waves(NC, MT)) void paged_attend_kernel
     constexpr int kLoads = FP8 ? NC : kSteps;        // 16-byte loads of a key's row by a lane
     constexpr int kWide = NC / 2, kNarrow = NC % 2;  // pieces of eight and of four columns of a lane
     constexpr int kCols = NC * 4, kSize = FP8 ? 1 : 2;
-    constexpr int kDepth = attend_depth(FP8, NC, MT);
-    __shared__ float wave_m[4][16 * MT], wave_l[4][16 * MT];
-    __shared__ float parts[4][16 * MT][NC * 64 + 4];
+    constexpr bool kFew = HT <= 8;
+    constexpr int kScores = kFew ? 1 : HT / 16;      // score tiles of 16 heads
+    constexpr int kSums = kFew ? HT / 4 : HT / 16;   // groups of four rows of results in a lane
+    constexpr int kDepth = attend_depth(FP8, NC, HT);
+    __shared__ float wave_m[4][HT], wave_l[4][HT];
+    __shared__ float parts[4][kFew ? 4 * HT : HT][NC * 64 + 4];
     const int lane = threadIdx.x & 63, wave = wave_in_block(), n = lane & 15, g = lane >> 4;
     const PagedView& c = a.c;
     const int D = c.dim;
@@ -354,13 +363,13 @@ __global__ __launch_bounds__(256, attend_waves(NC, MT)) void paged_attend_kernel
         const PagedSpan span = paged_span(c, a.window, s);
         const int rel = (int)(u - before * heads_of_units), hg = rel / span.units, first = rel - hg * span.units;
         const int left = span.units - first, take = left < u_end - u ? left : (int)(u_end - u), last = first + take;
-        const int kvh = hg / a.tiles_of_heads, head0 = (hg - kvh * a.tiles_of_heads) * 16 * MT;
+        const int kvh = hg / a.tiles_of_heads, head0 = (hg - kvh * a.tiles_of_heads) * HT;
 
         // ---- queries ----
-        frag q[MT][kSteps];
+        frag q[kScores][kSteps];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            const int h = head0 + mt * 16 + n;
+        for (int mt = 0; mt < kScores; ++mt) {
+            const int h = head0 + (kFew ? n % HT : mt * 16 + n);
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
                 const int d = FP8 ? i / 2 * 64 + g * 16 + i % 2 * 8 : i * 32 + g * 8;
@@ -373,15 +382,19 @@ __global__ __launch_bounds__(256, attend_waves(NC, MT)) void paged_attend_kernel
         const char* vh = c.v + kvh * c.v_head;
         const int* row = c.table + s * c.ld_table;
 
-        float m[MT], l[MT];
-        float4_t o[MT][kCols];
+        float m[kScores], l[kScores];
+        float4_t o[kSums][kCols];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int mt = 0; mt < kScores; ++mt) {
             m[mt] = -__builtin_inff();
             l[mt] = 0.0f;
+        }
+#pragma unroll
+        for (int mt = 0; mt < kSums; ++mt)
 #pragma unroll
             for (int i = 0; i < kCols; ++i) o[mt][i] = float4_t{0, 0, 0, 0};
-        }
+        // The lane that has the statistics of row r of its results' group mt.
+        auto lane_of = [&](int mt, int r) { return kFew ? (lane & ~7) | (HT == 4 ? (lane & 4) | r : mt * 4 + r) : g * 4 + r; };
 
         // ---- tiles: 16 tokens of each unit ----
         uint4_t k[kDepth][kLoads];
@@ -390,52 +403,62 @@ __global__ __launch_bounds__(256, attend_waves(NC, MT)) void paged_attend_kernel
         unsigned int page_ok[kDepth];  // a bit for each token of a tile
         // This wavefront's first token of a unit; a unit behind the stretch's end has none.
         auto token_of = [&](int unit) { return unit < last ? span.base + unit * kUnit + wave * 16 : span.end; };
-        // Pages: a lane has that of one of the next 64 tiles (ONE), or of a token of one of the next 4; the group after that is on its way.
-        constexpr int kGroup = ONE ? 64 : 4;
+        // Pages: a lane has that of one of the next 64 tiles (EVEN), or of a token of one of the next 4; the group after that is on its way.
+        constexpr int kGroup = EVEN ? 64 : 4;
         auto pages_of = [&](int unit) {
-            const int first_token = token_of(unit + (ONE ? lane : g)), token = first_token + (ONE ? 0 : n);
+            const int first_token = token_of(unit + (EVEN ? lane : g)), token = first_token + (EVEN ? 0 : n);
             return first_token < span.end && token < span.end ? row[c.page_of(token)] : -1;
         };
         int ids = pages_of(first), ids_next = pages_of(first + kGroup);
         // The loads of a unit's tile, in two parts: its place and keys, its values.  A page that is none is read as page 0, and not seen.
         int page = 0, in = 0;
+        const unsigned int k_off = n * c.k_tok + g * 16, v_off = g * 4 * c.v_tok + n * (kWide ? 8 : 4) * kSize;
         auto load_keys = [&](int j, int unit) {
             const int token = token_of(unit), i = (unit - first) & (kGroup - 1);
             if (i == 0 && unit != first) {
                 ids = ids_next;
                 ids_next = pages_of(unit + kGroup);
             }
-            if constexpr (ONE) {
+            if constexpr (EVEN) {
                 const int id = __builtin_amdgcn_readlane(ids, i);
                 const bool ok = id >= 0 && id < c.pages;
                 page_ok[j] = ok ? 0xffffu : 0u;
                 page = ok ? id : 0;
                 in = token - c.page_of(token) * c.page_size;
+                const char* kp = kh + page * c.k_page + in * c.k_tok;
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) k[j][i] = load_global_once<uint4_any_t>(kp + k_off + i * 64);
             } else {
                 const int id = __shfl(ids, i * 16 + n);
                 const bool ok = id >= 0 && id < c.pages;
                 page_ok[j] = (unsigned int)__ballot(ok) & 0xffffu;
                 page = ok ? id : 0;
                 in = token + n - c.page_of(token + n) * c.page_size;
-            }
-            const char* kp = ONE ? kh + page * c.k_page + in * c.k_tok + (unsigned int)(n * c.k_tok + g * 16) : kh + page * c.k_page + in * c.k_tok + g * 16;
+                const char* kp = kh + page * c.k_page + in * c.k_tok + g * 16;
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                k[j][i] = uint4_t{0, 0, 0, 0};
-                if (i * 64 + g * 16 < D * kSize) k[j][i] = load_global<uint4_any_t>(kp + i * 64);
+                for (int i = 0; i < kLoads; ++i) {
+                    k[j][i] = uint4_t{0, 0, 0, 0};
+                    if (i * 64 + g * 16 < D * kSize) k[j][i] = load_global_once<uint4_any_t>(kp + i * 64);
+                }
             }
         };
         auto load_values = [&](int j, int r) {
-            const char* vp = ONE ? vh + page * c.v_page + (in + r) * c.v_tok + (unsigned int)(g * 4 * c.v_tok)
-                                 : vh + __shfl(page, g * 4 + r) * c.v_page + __shfl(in, g * 4 + r) * c.v_tok;
+            if constexpr (EVEN) {
+                const char* vp = vh + page * c.v_page + (in + r) * c.v_tok;
 #pragma unroll
-            for (int i = 0; i < kWide; ++i) {
-                wide[j][r][i].clear();
-                if (i * 128 + n * 8 < D) wide[j][r][i].load(vp + (i * 128 + n * 8) * kSize);
-            }
-            if constexpr (kNarrow) {
-                narrow[j][r][0].clear();
-                if (kWide * 128 + n * 4 < D) narrow[j][r][0].load(vp + (kWide * 128 + n * 4) * kSize);
+                for (int i = 0; i < kWide; ++i) wide[j][r][i].load(vp + v_off + i * 128 * kSize);
+                if constexpr (kNarrow) narrow[j][r][0].load(vp + (kWide ? v_off - n * 4 * kSize + kWide * 128 * kSize : v_off));
+            } else {
+                const char* vp = vh + __shfl(page, g * 4 + r) * c.v_page + __shfl(in, g * 4 + r) * c.v_tok;
+#pragma unroll
+                for (int i = 0; i < kWide; ++i) {
+                    wide[j][r][i].clear();
+                    if (i * 128 + n * 8 < D) wide[j][r][i].load(vp + (i * 128 + n * 8) * kSize);
+                }
+                if constexpr (kNarrow) {
+                    narrow[j][r][0].clear();
+                    if (kWide * 128 + n * 4 < D) narrow[j][r][0].load(vp + (kWide * 128 + n * 4) * kSize);
+                }
             }
         };
 #pragma unroll
@@ -445,17 +468,18 @@ __global__ __launch_bounds__(256, attend_waves(NC, MT)) void paged_attend_kernel
 #pragma unroll
                 for (int r = 0; r < 4; ++r) load_values(j, r);
             }
-        auto tile = [&](int j, int unit) {
+        // A tile; `more`: the loads of the one kDepth behind it are issued as its registers become free.
+        auto tile = [&](auto more, int j, int unit) {
+            constexpr bool kMore = decltype(more)::value;
             const int token = token_of(unit);
-            const bool more = token_of(unit + kDepth) < span.end;
             // Tokens that are not the sequence's, or not in the window, or of no page, are left out, whatever lies there.
             unsigned int seen = page_ok[j];
             if (token < span.first) seen &= 0xffffu << (span.first - token);
             if (token + 16 > span.end) seen &= 0xffffu >> (token + 16 - span.end);
 
-            float4_t sc[MT];
+            float4_t sc[kScores];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) sc[mt] = float4_t{0, 0, 0, 0};
+            for (int mt = 0; mt < kScores; ++mt) sc[mt] = float4_t{0, 0, 0, 0};
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
                 frag kf;
@@ -464,90 +488,115 @@ __global__ __launch_bounds__(256, attend_waves(NC, MT)) void paged_attend_kernel
                 else
                     kf = __builtin_bit_cast(frag, k[j][i]);
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) sc[mt] = T::mfma(kf, q[mt][i], sc[mt]);
+                for (int mt = 0; mt < kScores; ++mt) sc[mt] = T::mfma(kf, q[mt][i], sc[mt]);
             }
-            if (more) load_keys(j, unit + kDepth);
-            bool above = false;
+            if constexpr (kMore) load_keys(j, unit + kDepth);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                sc[mt] *= scale;
-                if (seen != 0xffffu)
+            for (int mt = 0; mt < kScores; ++mt) sc[mt] *= scale;
+            if (seen != 0xffffu) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) sc[mt][r] = seen >> (g * 4 + r) & 1 ? sc[mt][r] : -__builtin_inff();
+                for (int r = 0; r < 4; ++r) {
+                    if (seen >> (g * 4 + r) & 1) continue;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) above |= sc[mt][r] > m[mt] + kLazy;
-            }
-            if (__ballot(above)) {
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    float top = fmaxf(fmaxf(sc[mt][0], sc[mt][1]), fmaxf(sc[mt][2], sc[mt][3]));
-                    top = fmaxf(top, __shfl_xor(top, 16));
-                    top = fmaxf(top, __shfl_xor(top, 32));
-                    const float now = fmaxf(m[mt], top);
-                    const float f = m[mt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m[mt] - now);
-                    m[mt] = now;
-                    l[mt] *= f;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float fr = __shfl(f, g * 4 + r);
-#pragma unroll
-                        for (int i = 0; i < kCols; ++i) o[mt][i][r] *= fr;
-                    }
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float p[MT];
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    p[mt] = sc[mt][r] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(sc[mt][r] - m[mt]);
-                    l[mt] += p[mt];
-                }
-                if (seen != 0xffffu && !(seen >> (g * 4 + r) & 1)) {
+                    for (int mt = 0; mt < kScores; ++mt) sc[mt][r] = -__builtin_inff();
 #pragma unroll
                     for (int i = 0; i < kWide; ++i) wide[j][r][i].clear();
                     if constexpr (kNarrow) narrow[j][r][0].clear();
                 }
-#pragma unroll
-                for (int i = 0; i < kWide; ++i)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float v = wide[j][r][i].value(e);
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) o[mt][i * 8 + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[mt], v, o[mt][i * 8 + e], 0, 0, 0);
-                    }
-                if constexpr (kNarrow)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float v = narrow[j][r][0].value(e);
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt)
-                            o[mt][kWide * 8 + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[mt], v, o[mt][kWide * 8 + e], 0, 0, 0);
-                    }
-                if (more) load_values(j, r);
             }
-        };
-        for (int unit = first; token_of(unit) < span.end; unit += kDepth) {
+            bool above = false;
 #pragma unroll
-            for (int j = 0; j < kDepth; ++j)
-                if (j == 0 || token_of(unit + j) < span.end) tile(j, unit + j);
-        }
-
-        // ---- the four wavefronts' parts, joined by all of the block ----
-        const int rows = a.group - head0 < 16 * MT ? a.group - head0 : 16 * MT;
+            for (int mt = 0; mt < kScores; ++mt) above |= fmaxf(fmaxf(sc[mt][0], sc[mt][1]), fmaxf(sc[mt][2], sc[mt][3])) > m[mt] + kLazy;
+            if (__ballot(above)) {
+                float f[kScores];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            l[mt] += __shfl_xor(l[mt], 16);
-            l[mt] += __shfl_xor(l[mt], 32);
-            if (g == 0) {
-                wave_m[wave][mt * 16 + n] = m[mt];
-                wave_l[wave][mt * 16 + n] = l[mt];
+                for (int mt = 0; mt < kScores; ++mt) {
+                    float top = fmaxf(fmaxf(sc[mt][0], sc[mt][1]), fmaxf(sc[mt][2], sc[mt][3]));
+                    top = fmaxf(top, __shfl_xor(top, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const float now = fmaxf(m[mt], top);
+                    f[mt] = m[mt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m[mt] - now);
+                    m[mt] = now;
+                    l[mt] *= f[mt];
+                }
+#pragma unroll
+                for (int mt = 0; mt < kSums; ++mt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float fr = __shfl(f[kFew ? 0 : mt], lane_of(mt, r));
+#pragma unroll
+                        for (int i = 0; i < kCols; ++i) o[mt][i][r] *= fr;
+                    }
+            }
+            float p[kSums][4];
+#pragma unroll
+            for (int mt = 0; mt < kScores; ++mt) {
+                const float from = m[mt] == -__builtin_inff() ? 0.0f : m[mt];  // (scores are -inf all then)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) p[mt][r] = __builtin_amdgcn_exp2f(sc[mt][r] - from);
+                l[mt] += (p[mt][0] + p[mt][1]) + (p[mt][2] + p[mt][3]);
+            }
+            if constexpr (HT == 8) {  // a lane's operands are those of heads lane % 4 and 4 + lane % 4: the other is four lanes round the row
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float other = dpp_f32<kDppRowRor4>(p[0][r]);
+                    p[1][r] = lane & 4 ? p[0][r] : other;
+                    p[0][r] = lane & 4 ? other : p[0][r];
+                }
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int h = mt * 16 + g * 4 + r;
+                auto add = [&](int i, float v) {
+#pragma unroll
+                    for (int mt = 0; mt < kSums; ++mt)
+                        o[mt][i] = kFew ? __builtin_amdgcn_mfma_f32_4x4x1f32(p[mt][r], v, o[mt][i], 0, 0, 0) : __builtin_amdgcn_mfma_f32_16x16x4f32(p[mt][r], v, o[mt][i], 0, 0, 0);
+                };
+#pragma unroll
+                for (int i = 0; i < kWide; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) add(i * 8 + e, wide[j][r][i].value(e));
+                if constexpr (kNarrow)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) add(kWide * 8 + e, narrow[j][r][0].value(e));
+                if constexpr (kMore) load_values(j, r);
+            }
+        };
+        int unit = first;
+        for (; token_of(unit + 2 * kDepth - 1) < span.end; unit += kDepth) {
+#pragma unroll
+            for (int j = 0; j < kDepth; ++j) tile(std::true_type{}, j, unit + j);
+        }
+        // (2 kDepth - 1 tiles at most are left, the first kDepth of them loaded)
+#pragma unroll
+        for (int j = 0; j < kDepth - 1; ++j)
+            if (token_of(unit + kDepth + j) < span.end) {
+                tile(std::true_type{}, j, unit + j);
+            } else if (token_of(unit + j) < span.end) {
+                tile(std::false_type{}, j, unit + j);
+            }
+        if (token_of(unit + kDepth - 1) < span.end) tile(std::false_type{}, kDepth - 1, unit + kDepth - 1);
+#pragma unroll
+        for (int j = 0; j < kDepth - 1; ++j)
+            if (token_of(unit + kDepth + j) < span.end) tile(std::false_type{}, j, unit + kDepth + j);
+
+        // ---- the four wavefronts' parts, joined by all of the block ----
+        const int rows = a.group - head0 < HT ? a.group - head0 : HT;
+#pragma unroll
+        for (int mt = 0; mt < kScores; ++mt) {
+            l[mt] += __shfl_xor(l[mt], 16);
+            l[mt] += __shfl_xor(l[mt], 32);
+            if (g == 0 && (!kFew || n < HT)) {
+                wave_m[wave][mt * 16 + n] = m[mt];
+                wave_l[wave][mt * 16 + n] = l[mt];
+            }
+        }
+#pragma unroll
+        for (int mt = 0; mt < kSums; ++mt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int h = kFew ? mt * 4 + r : mt * 16 + g * 4 + r;
                 if (h >= rows) continue;
-                float* part = parts[wave][h];
+                float* part = parts[wave][kFew ? g * HT + h : h];
 #pragma unroll
                 for (int i = 0; i < kWide; ++i)
 #pragma unroll
@@ -557,12 +606,11 @@ __global__ __launch_bounds__(256, attend_waves(NC, MT)) void paged_attend_kernel
                     *reinterpret_cast<float4_t*>(part + kWide * 128 + n * 4) =
                         float4_t{o[mt][kWide * 8][r], o[mt][kWide * 8 + 1][r], o[mt][kWide * 8 + 2][r], o[mt][kWide * 8 + 3][r]};
             }
-        }
         __syncthreads();
         const bool complete = first == 0 && last == span.units;
         const float vs = FP8 ? c.v_scale[kvh] : 1.0f;
         const int64_t out0 = (int64_t)s * c.kv_heads * a.group + kvh * a.group + head0;
-        float* piece = a.work + ((int64_t)blockIdx.x * 2 + (first == 0 ? 1 : 0)) * 16 * MT * (D + 4);
+        float* piece = a.work + ((int64_t)blockIdx.x * 2 + (first == 0 ? 1 : 0)) * HT * (D + 4);
         const int each = D / 4;
         for (int i = threadIdx.x; i < rows * each; i += 256) {
             const int h = i / each, d = (i - h * each) * 4;
@@ -573,7 +621,8 @@ __global__ __launch_bounds__(256, attend_waves(NC, MT)) void paged_attend_kernel
             for (int w = 0; w < 4; ++w) {
                 const float f = wave_m[w][h] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(wave_m[w][h] - top);
                 weight += f * wave_l[w][h];
-                sum += f * *reinterpret_cast<const float4_t*>(&parts[w][h][d]);
+#pragma unroll
+                for (int q = 0; q < (kFew ? 4 : 1); ++q) sum += f * *reinterpret_cast<const float4_t*>(&parts[w][q * HT + h][d]);
             }
             if (complete) {
                 store_attended<T>(a, out0 + h, d, sum, weight, top, vs);
