@@ -64,10 +64,10 @@ int cut_of(const PagedView& v, int group, int num_cus, AttendCut* cut)
 {
     const int nc = (v.dim + 63) / 64;
     // (for heads longer than 128 the registers do not hold 32 results' sums)
-    cut->heads = group <= 4 ? 4 : group <= 8 && nc <= 2 ? 8 : group > 16 && nc <= 2 ? 32 : 16;
+    cut->heads = group <= 4 ? 4 : group > 16 && nc <= 2 ? 32 : 16;
     cut->tiles_of_heads = (group + cut->heads - 1) / cut->heads;
     const int64_t heads = (int64_t)v.kv_heads * cut->tiles_of_heads, units = (v.most + 15 + kUnit - 1) / kUnit;
-    if (heads * units > INT32_MAX || (int64_t)v.sequences * v.kv_heads * group > (1 << 23))
+    if (units * v.sequences > INT32_MAX / heads / 2 || (int64_t)v.sequences * v.kv_heads * group > (1 << 23))
         return fail(PIMHIP_ERR_UNSUPPORTED, "%d sequences of up to %d tokens with %d key heads are too many for one launch", v.sequences, v.most, v.kv_heads);
     const int64_t most = (int64_t)v.sequences * heads * units, wanted = attend_waves(v.k_scale != nullptr, nc, cut->heads) * (int64_t)num_cus;
     cut->blocks = (int)(most < wanted ? most : wanted);
@@ -89,7 +89,6 @@ void launch_attend(const AttendArgs& a, const AttendCut& cut, hipStream_t s)
 {
     if (cut.heads == 4) return launch_attend<T, FP8, NC, 4>(a, cut.blocks, s);
     if constexpr (NC <= 2) {
-        if (cut.heads == 8) return launch_attend<T, FP8, NC, 8>(a, cut.blocks, s);
         if (cut.heads == 32) return launch_attend<T, FP8, NC, 32>(a, cut.blocks, s);
     }
     launch_attend<T, FP8, NC, 16>(a, cut.blocks, s);

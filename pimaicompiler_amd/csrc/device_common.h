@@ -73,7 +73,6 @@ static constexpr int kDppQuadXor1 = 0xB1;     // quad_perm:[1,0,3,2]
 static constexpr int kDppQuadXor2 = 0x4E;     // quad_perm:[2,3,0,1]
 static constexpr int kDppRowHalfMirror = 0x141;
 static constexpr int kDppRowMirror = 0x140;
-static constexpr int kDppRowRor4 = 0x124;     // row_ror:4
 static constexpr int kDppRowRor8 = 0x128;     // row_ror:8
 
 template <int CTRL>

@@ -175,9 +175,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
 //             the scores of head l % 16 and tokens 4 (l / 16) + r
 //   values    P [16 heads x 4 tokens] . V [4 tokens x 16 columns] on the 32-bit one, for tokens r, 4 + r, 8 + r, 12 + r: a lane's e_j are its
 //             operand as they are, unrounded, and V is one that 16 lanes read as one row: nothing is turned or exchanged.
-//             Where a key head has up to 8 query heads most of those 16 rows are empty: Q's columns repeat every 4 (8) heads then, and the
-//             matrix instruction of 16 blocks [4 heads x 1 token] . [1 x 4 columns] takes a lane's e_j and its own value of V, a quarter (half) of the
-//             time; the four groups of lanes have sums over tokens of their own, which are added at the end
+//             Where a key head has up to 4 query heads most of those 16 rows are empty: Q's columns repeat every 4 heads then, and the matrix
+//             instruction of 16 blocks [4 heads x 1 token] . [1 x 4 columns] takes a lane's e_j and its own value of V, a quarter of the time; the
+//             four groups of lanes have sums over tokens of their own, which are added at the end.  (Two of them for up to 8 heads need
+//             twice the registers: 1.6 GB in 299 us, with 16 rows 278.)
 // Values lie in registers from memory on; a tile's loads are issued while the one before is worked on.
 static constexpr int kUnit = 64;           // tokens that the four wavefronts of a block take together
 static constexpr float kLazy = 40.0f;      // a running maximum moves on when a score is above it by so many powers of two
@@ -206,10 +207,10 @@ __device__ __forceinline__ void store_attended(const AttendArgs& a, int64_t head
 struct PagedSpan {
     int first, base, end, units;  // tokens first .. end - 1 are seen; tiles begin at base
 };
-__device__ __forceinline__ PagedSpan paged_span(const PagedView& c, int window, int s)
+__device__ __forceinline__ PagedSpan paged_span(int length, int window)
 {
     PagedSpan p;
-    p.end = paged_length(c, s);
+    p.end = length;
     p.first = window > 0 && p.end > window ? p.end - window : 0;
     p.base = p.first & ~15;
     const int n = (p.end - p.base + kUnit - 1) / kUnit;
@@ -217,52 +218,68 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedView& c, int window, 
     return p;
 }
 
-// Where in the row of units (`times` units for each of a sequence's) a sequence begins, and how many units there are in all, by a block
-// of 256.  ask(total) is the unit whose sequence is looked for, or -1 - s for sequence s.
-struct PagedFound {
-    int64_t before, total;
-    int s;
+// The stretch of a block in the row of units (`times` units for each of a sequence's, less than 2^31 in all): units first .. end - 1 of `per` a
+// block, and the sequence it begins in, which begins at unit `before` and is `length` tokens long.
+struct PagedStretch {
+    int first, end, per, s, before, length;
 };
-template <class F>
-__device__ __forceinline__ PagedFound paged_find(const PagedView& c, int window, int64_t times, F ask)
+__device__ __forceinline__ PagedStretch paged_stretch(const PagedView& c, int window, int times)
 {
-    __shared__ int64_t wave_sum_of[4];
-    __shared__ int64_t found_before;
-    __shared__ int found_s;
+    PagedStretch f;
+    if (c.sequences == 1) {
+        f.s = f.before = 0;
+        f.length = paged_length(c, 0);
+        const int total = paged_span(f.length, window).units * times;
+        f.per = (int)((unsigned int)(total + (int)gridDim.x - 1) / gridDim.x);
+        f.first = (int)blockIdx.x * f.per;
+        f.end = f.first + f.per < total ? f.first + f.per : total;
+        return f;
+    }
+    __shared__ int wave_sum_of[4];
+    __shared__ int found[3];
     const int each = (c.sequences + 255) / 256, from = (int)threadIdx.x * each, lo = from < c.sequences ? from : c.sequences;
     const int hi = lo + each < c.sequences ? lo + each : c.sequences;
-    int64_t mine = 0;
-    for (int s = lo; s < hi; ++s) mine += paged_span(c, window, s).units;
-    int64_t incl = mine;
+    int mine = 0, length = 0;
+    for (int s = lo; s < hi; ++s) {
+        length = paged_length(c, s);
+        mine += paged_span(length, window).units * times;
+    }
+    int incl = mine;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
-        const int64_t o = __shfl_up(incl, d);
+        const int o = __shfl_up(incl, d);
         if ((int)(threadIdx.x & 63) >= d) incl += o;
     }
     if ((threadIdx.x & 63) == 63) wave_sum_of[threadIdx.x >> 6] = incl;
     __syncthreads();
-    int64_t before = incl - mine, total = 0;
+    int before = incl - mine, total = 0;
+#pragma unroll
     for (int w = 0; w < 4; ++w) {
         if (w < (int)(threadIdx.x >> 6)) before += wave_sum_of[w];
         total += wave_sum_of[w];
     }
-    PagedFound f;
-    f.total = total * times;
-    const int64_t u = ask(f.total);
-    const int want = u < 0 ? (int)(-1 - u) : -1;
-    if (u < 0 ? lo <= want && want < hi : before * times <= u && u < (before + mine) * times) {
+    f.per = (int)(((unsigned int)total + gridDim.x - 1) / gridDim.x);
+    // (a block behind the last stretch has none, and looks for nothing; blocks times per may pass 2^31)
+    const int64_t first = (int64_t)blockIdx.x * f.per, end = first + f.per;
+    f.first = first < total ? (int)first : total;
+    f.end = end < total ? (int)end : total;
+    if (before <= f.first && f.first < before + mine) {
         int s = lo;
-        for (; s < hi - 1; ++s) {
-            const int n = paged_span(c, window, s).units;
-            if (u < 0 ? s == want : u < (before + n) * times) break;
-            before += n;
-        }
-        found_before = before;
-        found_s = s;
+        if (each > 1)
+            for (; s < hi; ++s) {
+                length = paged_length(c, s);
+                const int n = paged_span(length, window).units * times;
+                if (f.first < before + n) break;
+                before += n;
+            }
+        found[0] = s;
+        found[1] = before;
+        found[2] = length;
     }
     __syncthreads();
-    f.before = found_before;
-    f.s = found_s;
+    f.s = found[0];
+    f.before = found[1];
+    f.length = found[2];
     return f;
 }
 
@@ -324,7 +341,7 @@ struct ValuePiece {
 constexpr int attend_waves(bool fp8, int nc, int ht) { return nc <= 2 && ht <= 16 ? 3 : 2; }
 constexpr int attend_depth(bool fp8, int nc, int ht) { return 1; }
 
-// NC: the head's size in 64 columns, rounded up; HT: query heads at a time (4, 8, 16 or 32); EVEN: pages are whole tiles of 16 tokens, and the head's size is NC of 64:
+// NC: the head's size in 64 columns, rounded up; HT: query heads at a time (4, 16 or 32); EVEN: pages are whole tiles of 16 tokens, and the head's size is NC of 64:
 // a tile's place is then the same for the wavefront, and no lane stays without loads.
 template <class T, bool FP8, int NC, int HT, bool EVEN>
 __global__ __launch_bounds__(256, attend_waves(FP8, NC, HT)) void paged_attend_kernel(AttendArgs a)
@@ -335,34 +352,24 @@ __global__ __launch_bounds__(256, attend_waves(FP8, NC, HT)) void paged_attend_k
     constexpr int kLoads = FP8 ? NC : kSteps;        // 16-byte loads of a key's row by a lane
     constexpr int kWide = NC / 2, kNarrow = NC % 2;  // pieces of eight and of four columns of a lane
     constexpr int kCols = NC * 4, kSize = FP8 ? 1 : 2;
-    constexpr bool kFew = HT <= 8;
-    constexpr int kScores = kFew ? 1 : HT / 16;      // score tiles of 16 heads
-    constexpr int kSums = kFew ? HT / 4 : HT / 16;   // groups of four rows of results in a lane
+    constexpr bool kFew = HT == 4;
+    constexpr int kScores = kFew ? 1 : HT / 16;      // tiles of 16 heads
+    constexpr int kParts = kFew ? 4 : 1;             // sums over tokens that a wavefront leaves of each head
     constexpr int kDepth = attend_depth(FP8, NC, HT);
     __shared__ float wave_m[4][HT], wave_l[4][HT];
-    __shared__ float parts[4][kFew ? 4 * HT : HT][NC * 64 + 4];
+    __shared__ float parts[4][kParts * HT][NC * 64 + 4];
     const int lane = threadIdx.x & 63, wave = wave_in_block(), n = lane & 15, g = lane >> 4;
     const PagedView& c = a.c;
     const int D = c.dim;
-    const int64_t heads_of_units = (int64_t)c.kv_heads * a.tiles_of_heads;
+    const int heads_of_units = c.kv_heads * a.tiles_of_heads;
 
-    // ---- this block's stretch ----
-    int64_t per = 0;
-    const PagedFound at = paged_find(c, a.window, heads_of_units, [&](int64_t total) {
-        per = (total + gridDim.x - 1) / gridDim.x;
-        const int64_t first = blockIdx.x * per;
-        return first < total ? first : total - 1;
-    });
-    int64_t u = blockIdx.x * per;
-    const int64_t u_end = u + per < at.total ? u + per : at.total;
-    if (u >= u_end) return;
-    int s = at.s;
-    int64_t before = at.before;
-
-    while (u < u_end) {
-        const PagedSpan span = paged_span(c, a.window, s);
-        const int rel = (int)(u - before * heads_of_units), hg = rel / span.units, first = rel - hg * span.units;
-        const int left = span.units - first, take = left < u_end - u ? left : (int)(u_end - u), last = first + take;
+    const PagedStretch stretch = paged_stretch(c, a.window, heads_of_units);
+    if (stretch.first >= stretch.end) return;
+    int s = stretch.s, before = stretch.before, length = stretch.length;
+    for (int u = stretch.first; u < stretch.end;) {
+        const PagedSpan span = paged_span(length, a.window);
+        const int rel = u - before, hg = rel / span.units, first = rel - hg * span.units;
+        const int left = span.units - first, take = left < stretch.end - u ? left : stretch.end - u, last = first + take;
         const int kvh = hg / a.tiles_of_heads, head0 = (hg - kvh * a.tiles_of_heads) * HT;
 
         // ---- queries ----
@@ -383,18 +390,18 @@ __global__ __launch_bounds__(256, attend_waves(FP8, NC, HT)) void paged_attend_k
         const int* row = c.table + s * c.ld_table;
 
         float m[kScores], l[kScores];
-        float4_t o[kSums][kCols];
+        float4_t o[kScores][kCols];
 #pragma unroll
         for (int mt = 0; mt < kScores; ++mt) {
             m[mt] = -__builtin_inff();
             l[mt] = 0.0f;
         }
 #pragma unroll
-        for (int mt = 0; mt < kSums; ++mt)
+        for (int mt = 0; mt < kScores; ++mt)
 #pragma unroll
             for (int i = 0; i < kCols; ++i) o[mt][i] = float4_t{0, 0, 0, 0};
-        // The lane that has the statistics of row r of its results' group mt.
-        auto lane_of = [&](int mt, int r) { return kFew ? (lane & ~7) | (HT == 4 ? (lane & 4) | r : mt * 4 + r) : g * 4 + r; };
+        // The lane that has the statistics of row r of a lane's results.
+        auto lane_of = [&](int r) { return kFew ? (lane & ~3) | r : g * 4 + r; };
 
         // ---- tiles: 16 tokens of each unit ----
         uint4_t k[kDepth][kLoads];
@@ -520,15 +527,15 @@ __global__ __launch_bounds__(256, attend_waves(FP8, NC, HT)) void paged_attend_k
                     l[mt] *= f[mt];
                 }
 #pragma unroll
-                for (int mt = 0; mt < kSums; ++mt)
+                for (int mt = 0; mt < kScores; ++mt)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float fr = __shfl(f[kFew ? 0 : mt], lane_of(mt, r));
+                        const float fr = __shfl(f[mt], lane_of(r));
 #pragma unroll
                         for (int i = 0; i < kCols; ++i) o[mt][i][r] *= fr;
                     }
             }
-            float p[kSums][4];
+            float p[kScores][4];
 #pragma unroll
             for (int mt = 0; mt < kScores; ++mt) {
                 const float from = m[mt] == -__builtin_inff() ? 0.0f : m[mt];  // (scores are -inf all then)
@@ -536,19 +543,11 @@ __global__ __launch_bounds__(256, attend_waves(FP8, NC, HT)) void paged_attend_k
                 for (int r = 0; r < 4; ++r) p[mt][r] = __builtin_amdgcn_exp2f(sc[mt][r] - from);
                 l[mt] += (p[mt][0] + p[mt][1]) + (p[mt][2] + p[mt][3]);
             }
-            if constexpr (HT == 8) {  // a lane's operands are those of heads lane % 4 and 4 + lane % 4: the other is four lanes round the row
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float other = dpp_f32<kDppRowRor4>(p[0][r]);
-                    p[1][r] = lane & 4 ? p[0][r] : other;
-                    p[0][r] = lane & 4 ? other : p[0][r];
-                }
-            }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 auto add = [&](int i, float v) {
 #pragma unroll
-                    for (int mt = 0; mt < kSums; ++mt)
+                    for (int mt = 0; mt < kScores; ++mt)
                         o[mt][i] = kFew ? __builtin_amdgcn_mfma_f32_4x4x1f32(p[mt][r], v, o[mt][i], 0, 0, 0) : __builtin_amdgcn_mfma_f32_16x16x4f32(p[mt][r], v, o[mt][i], 0, 0, 0);
                 };
 #pragma unroll
@@ -591,10 +590,10 @@ __global__ __launch_bounds__(256, attend_waves(FP8, NC, HT)) void paged_attend_k
             }
         }
 #pragma unroll
-        for (int mt = 0; mt < kSums; ++mt)
+        for (int mt = 0; mt < kScores; ++mt)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int h = kFew ? mt * 4 + r : mt * 16 + g * 4 + r;
+                const int h = kFew ? r : mt * 16 + g * 4 + r;
                 if (h >= rows) continue;
                 float* part = parts[wave][kFew ? g * HT + h : h];
 #pragma unroll
@@ -622,7 +621,7 @@ __global__ __launch_bounds__(256, attend_waves(FP8, NC, HT)) void paged_attend_k
                 const float f = wave_m[w][h] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(wave_m[w][h] - top);
                 weight += f * wave_l[w][h];
 #pragma unroll
-                for (int q = 0; q < (kFew ? 4 : 1); ++q) sum += f * *reinterpret_cast<const float4_t*>(&parts[w][q * HT + h][d]);
+                for (int q = 0; q < kParts; ++q) sum += f * *reinterpret_cast<const float4_t*>(&parts[w][q * HT + h][d]);
             }
             if (complete) {
                 store_attended<T>(a, out0 + h, d, sum, weight, top, vs);
@@ -631,12 +630,12 @@ __global__ __launch_bounds__(256, attend_waves(FP8, NC, HT)) void paged_attend_k
                 if (d == 0) *reinterpret_cast<float2_t*>(piece + h * (D + 4) + D) = float2_t{top, weight};
             }
         }
-        if (threadIdx.x == 0 && last == span.units) a.pieces[s * heads_of_units + hg] = int2{(int)((u - first) / per), (int)blockIdx.x};
+        if (threadIdx.x == 0 && last == span.units) a.pieces[(int64_t)s * heads_of_units + hg] = int2{(u - first) / stretch.per, (int)blockIdx.x};
         __syncthreads();
         u += take;
         if (rel + take == heads_of_units * span.units) {
-            before += span.units;
-            ++s;
+            before += heads_of_units * span.units;
+            if (++s < c.sequences) length = paged_length(c, s);
         }
     }
 }
