@@ -2,7 +2,15 @@
 #include "api_common.h"
 #include "sample_kernels.h"
 
+#include <type_traits>
+
 using namespace pimhip;
+
+namespace
+{
+constexpr int kCountFrom = 4096;      // (smaller rows are soon looked at again)
+constexpr int kCountMost = 1 << 20;   // (segments' sums beside the counts: larger ones do not fit into LDS)
+}  // namespace
 
 extern "C" int pimhip_sample_tokens(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t vocab, const float* uniform, const PimHipSampleSettings* settings,
                                     int64_t* tokens, float* logp, void* stream)
@@ -14,7 +22,12 @@ extern "C" int pimhip_sample_tokens(const void* logits, int dtype, int64_t ld, i
         return fail(PIMHIP_ERR_INVALID_ARGUMENT, "rows=%lld, vocab=%lld (at most %d)", (long long)rows, (long long)vocab, kSampleMost);
     if (dtype != PIMHIP_F16 && dtype != PIMHIP_BF16 && dtype != PIMHIP_F32) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "dtype=%d", dtype);
     if (!settings) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "settings must be non-null");
-    const int threads = vocab <= 2048 ? 256 : 1024;
+    // 1024 threads for a row where there are CUs for all rows; where not, two blocks share one.  Values are counted where a row may need it (top_p of a
+    // flat distribution, a large top_k), which takes a CU's LDS for one block.
+    const bool count = dtype != PIMHIP_F32 && vocab > kCountFrom && vocab <= kCountMost &&
+                       (settings->top_ks || settings->top_k <= 0 || settings->top_k > kListMost / 2) &&
+                       (settings->top_ks || settings->top_ps || settings->top_p < 1.0f || settings->top_k > 0);
+    const int threads = count ? 1024 : vocab <= 4096 ? 256 : rows > st->num_cus ? 512 : 1024;
     if (rows * threads > UINT32_MAX) return fail(PIMHIP_ERR_UNSUPPORTED, "%lld rows are too many for one launch", (long long)rows);
     if (rows == 0) return PIMHIP_OK;
     if (!logits || (rows > 1 && ld < vocab)) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "logits is null, or ld=%lld is less than vocab=%lld", (long long)ld, (long long)vocab);
@@ -34,10 +47,18 @@ extern "C" int pimhip_sample_tokens(const void* logits, int dtype, int64_t ld, i
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto run = [&](auto type) {
         typedef decltype(type) T;
-        if (threads == 256)
-            sample_kernel<T, 256><<<dim3((unsigned)rows), 256, 0, s>>>(a);
-        else
-            sample_kernel<T, 1024><<<dim3((unsigned)rows), 1024, 0, s>>>(a);
+        auto launch = [&](auto threads, auto counts) {
+            constexpr int kThreads = decltype(threads)::value;
+            constexpr bool kCount = decltype(counts)::value;
+            sample_kernel<T, kThreads, kCount><<<dim3((unsigned)rows), kThreads, sample_shared_bytes<T, kThreads, kCount>(a.V), s>>>(a);
+        };
+        typedef std::integral_constant<int, 256> T256;
+        typedef std::integral_constant<int, 512> T512;
+        typedef std::integral_constant<int, 1024> T1024;
+        if constexpr (!std::is_same<T, F32>::value) {
+            if (count) return launch(T1024{}, std::true_type{});
+        }
+        threads == 256 ? launch(T256{}, std::false_type{}) : threads == 512 ? launch(T512{}, std::false_type{}) : launch(T1024{}, std::false_type{});
     };
     dtype == PIMHIP_F16 ? run(F16{}) : dtype == PIMHIP_BF16 ? run(BF16{}) : run(F32{});
     PIMHIP_HIP_CHECK(hipGetLastError());

@@ -50,26 +50,6 @@ __device__ __forceinline__ void each_four_pieces(const typename T::elem* row, in
     }
 }
 
-// The larger of two keys over the LANES (1, 4 or 16) lanes of a group; every lane returns it.
-template <int LANES>
-__device__ __forceinline__ unsigned long long group_max_u64(unsigned long long k)
-{
-    auto with = [&](unsigned int hi, unsigned int lo) {
-        const unsigned long long o = (unsigned long long)hi << 32 | lo;
-        k = o > k ? o : k;
-    };
-    static_assert(LANES == 1 || LANES == 4 || LANES == 16, "a group is part of a row of 16 lanes");
-    if constexpr (LANES >= 4) {
-        with(dpp_u32<kDppQuadXor1>((unsigned int)(k >> 32)), dpp_u32<kDppQuadXor1>((unsigned int)k));
-        with(dpp_u32<kDppQuadXor2>((unsigned int)(k >> 32)), dpp_u32<kDppQuadXor2>((unsigned int)k));
-    }
-    if constexpr (LANES == 16) {
-        with(dpp_u32<kDppRowHalfMirror>((unsigned int)(k >> 32)), dpp_u32<kDppRowHalfMirror>((unsigned int)k));
-        with(dpp_u32<kDppRowMirror>((unsigned int)(k >> 32)), dpp_u32<kDppRowMirror>((unsigned int)k));
-    }
-    return k;
-}
-
 struct LogProbArgs {
     const void* logits;
     const void* tokens;  // [rows] int64 or int32, or null

@@ -7,24 +7,34 @@
 // One block a row.  The first pass finds the largest value and, where the sum over all tokens is asked for, that too.  What may stay is
 // above a bound that this pass gives (top_k: the k-th largest of the threads' own largest values; top_p: tokens below (1 - top_p) / V of the sum
 // cannot be among those that reach top_p of it, since all of them together do not have the rest; min_p: its own), and goes to a list
-// in LDS in a second pass, out of the caches.  Up to 64 such tokens are put into order by one wavefront.
-// Of more nothing is sorted: top_k and top_p each come down to one value, the smallest that stays, and how many of those equal to it do.  It
-// is found by histograms over the values' order (counts, or sums of w): the bucket in which the target is reached is cut into buckets again
-// until it is one value.  The same goes for the draw, over indices.  Rows whose list would not fit (flat distributions, a large top_k) are read
-// again in place of it.
-// Sums are whole numbers of 64 bits, w in units of 2^-shift of the largest: they are the same in any order.  w itself is worked out in 64 bits (the
-// vector units take as long for an fma of 64 bits as for one of 32): with fp32's 2^-24 a number between two tokens of a large vocabulary would
-// fall on the wrong one in some percent of the rows.
+// in LDS, whose order is worked out there: up to 64 tokens by one wavefront, more of them by buckets.
+// Where it does not fit (flat distributions, a large top_k), nothing is put into order: top_k and top_p each come down to one value, the smallest that
+// stays, and how many of those equal to it do.  It is found by histograms over the values' order (counts, or sums of w): the bucket in which the
+// target is reached is cut into buckets again until it is one value.  16-bit rows of a call that asks for top_p, or a large top_k, are counted value by value
+// instead, all 65536 of them in LDS: the one pass that does so stands for the first, and w is worked out once for each value.
+// Sums that are made in any order are whole numbers of 64 bits, w in units of 2^-shift of the largest.  w itself is worked out in 64 bits (an fma of
+// 64 bits takes a wavefront 5.4 clocks, one of 32 bits 4.4): with fp32's 2^-24 a number between two tokens of a large vocabulary would fall
+// on the wrong one in some percent of the rows.
+// Bound by w: 25 vector instructions a token, 13 us for the 64000 tokens a CU has of 512 rows of 32000 (fp32, nothing cut off: 29 us in all; the
+// bytes take 10).  256 rows of 131072 in bfloat16 whose nucleus holds half of them: 72 us, the counts 20 (LDS atomics), the last pass's w 33.  Reading
+// w out of a table in LDS there takes as long as working it out (30 us for 131072 gathers a CU).  64 rows of 100003 with settings of their own: 34;
+// one row of 32000 with top_k and top_p: 17, code that is run once and the dependent steps.
+// Code is kept short, loops as loops: what one row takes is walked through once and comes cold out of the instruction cache.  (The same steps
+// unrolled, 117 to 177 KB a kernel, took 17 us for one row of 32000 and 69 for 256 of 131072.)
 #pragma once
+
+#include <type_traits>
 
 #include "row_pieces.h"
 
 namespace pimhip
 {
 static constexpr int kSampleMost = 1 << 21;   // tokens of a vocabulary
-static constexpr int kSegment = 512;          // tokens that a wavefront takes at a time, whose sum is kept
-static constexpr int kSegments = kSampleMost / kSegment;
-static constexpr int kListMost = 4096;        // tokens of a row's list
+static constexpr int kSegment = 2048;         // tokens that a wavefront takes at a time, whose sum is kept
+static constexpr int kListMost = 1024;        // tokens of a row's list
+static constexpr int kBins = 2048;            // buckets
+static constexpr int kTopsMost = 1 << 17;     // tokens of a row whose pieces' largest values are kept in LDS
+static constexpr int kCountWords = 32768;     // a count of 16 bits for each 16-bit value, two a word
 static constexpr double kExponents = 900.0;   // largest values up to 2^+-this are summed as they are, in the first pass
 
 struct SampleArgs {
@@ -77,13 +87,6 @@ struct SampleWeight {
     }
 };
 
-__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v)
-{
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-    return v;
-}
-
 // A share of the whole, as whole numbers.  The first pass's sums and those relative to the largest value differ by up to 4.3e-12 of themselves, so shares
 // are moved by 2^-36 of theirs: one that meets a border exactly (equal weights) is on the border's right side whichever it is compared with.
 // The draw falls on the token at which the running sum reaches sample_target(); what reaches nucleus_target() takes no more tokens.
@@ -99,35 +102,50 @@ __device__ __forceinline__ uint64_t nucleus_target(float top_p, uint64_t whole)
     return t < 1 ? 1 : t;
 }
 
-// What stays: values of a key above `key`, the ones equal to it up to index `last`, and none with a weight under `least`.
-struct SampleKept {
-    unsigned int key;
-    int last;
-    double least;
+// Eight values as they lie in memory.
+template <class T>
+struct Piece {
+    static constexpr int kQuads = sizeof(typename T::elem) / 2;
+    uint4_t q[kQuads];
+    __device__ __forceinline__ void load(const typename T::elem* p)
+    {
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) q[i] = reinterpret_cast<const uint4_any_t*>(p)[i];
+    }
+    __device__ __forceinline__ float value(int c) const
+    {
+        typename T::elem e[8];
+        __builtin_memcpy(e, q, sizeof(e));
+        return (float)e[c];
+    }
+    __device__ __forceinline__ void set(int c, float v)
+    {
+        typename T::elem e[8];
+        __builtin_memcpy(e, q, sizeof(e));
+        e[c] = (typename T::elem)v;
+        __builtin_memcpy(q, e, sizeof(e));
+    }
 };
 
 template <class T, int THREADS>
 struct SampleRow {
-    static constexpr int kWaves = THREADS / 64;
-    static constexpr int kBins = 2048;
+    typedef typename T::elem elem;
+    static constexpr int kWaves = THREADS / 64, kAhead = sizeof(elem) == 2 ? 4 : 2;  // (pieces on their way)
     // fp32 words of 16-bit values end in zeros (in their order, in zeros or ones): these bits tell no two of them apart.
     static constexpr int kDrop = __is_same(T, F16) ? 13 : __is_same(T, BF16) ? 16 : 0;
     struct Shared {
-        union {
-            uint64_t bins[kSegments];
-            double segments[kSegments];
-        };
-        unsigned int list_key[kListMost];
-        int list_at[kListMost];
+        unsigned long long list[kListMost];  // keys, and the complements of indices below them
         uint64_t waves[kWaves];
-        double waves_f[kWaves];
         unsigned long long best[kWaves];
+        uint64_t chunk_sums[32], chunk_counts[32];
         uint64_t found_before, found_amount;
-        int found, count, bad;
+        int found, count, named, bad;
     };
-    const typename T::elem* x;
+    const elem* x;
     int V;
     Shared& sh;
+    uint64_t* bins;        // kBins of them, or one for each segment where those are more
+    unsigned int* ties;    // one for each segment, or for each value of one; the counts, or the pieces' largest values, lie there too
 
     static __device__ __forceinline__ unsigned int key_of(float v) { return ordered_bits(v) >> kDrop; }
     static __device__ __forceinline__ float value_of(unsigned int key)
@@ -135,93 +153,101 @@ struct SampleRow {
         const unsigned int o = key << kDrop;  // (a negative value's dropped bits are ones)
         return from_ordered(o & 0x80000000u ? o : o | ((1u << kDrop) - 1u));
     }
+    static __device__ __forceinline__ unsigned long long entry_of(unsigned int key, int at) { return (unsigned long long)key << 32 | (unsigned int)~(unsigned int)at; }
+    static __device__ __forceinline__ float value_in(unsigned long long entry) { return value_of((unsigned int)(entry >> 32)); }
+    static __device__ __forceinline__ int index_in(unsigned long long entry) { return (int)~(unsigned int)entry; }
 
-    __device__ __forceinline__ void piece(int p, float (&v)[8]) const
+    // The piece of values 8 p .. 8 p + 7 and the index of its first; the row's last piece is the last eight values, those of the piece before it -inf.
+    __device__ __forceinline__ int piece(int p, Piece<T>& v) const
     {
-        if (p * 8 + 8 <= V) {
-            load_piece<T>(x, p, v);
-        } else {
-#pragma unroll
-            for (int c = 0; c < 8; ++c) v[c] = p * 8 + c < V ? (float)x[p * 8 + c] : -__builtin_inff();
-        }
-    }
-    // f(number of the segment, index of the first value, eight values) for the pieces of a row, a segment by each wavefront, four at a time;
-    // behind the row's end values are -inf.
-    template <class F>
-    __device__ __forceinline__ void each_segment(F f) const
-    {
-        const int segments = (V + kSegment - 1) / kSegment, lane = threadIdx.x & 63, whole = V / 8;
-        for (int first = wave_in_block(); first < segments; first += 4 * kWaves) {
-            float v[4][8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int p = (first + i * kWaves) * 64 + lane;
-                if (p < whole) {
-                    load_piece<T>(x, p, v[i]);
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) v[i][c] = p * 8 + c < V ? (float)x[p * 8 + c] : -__builtin_inff();
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (first + i * kWaves < segments) f(first + i * kWaves, ((first + i * kWaves) * 64 + lane) * 8, v[i]);
-        }
-    }
-    // f(value, index) for the values of the row, or of its list.
-    template <bool LIST, class F>
-    __device__ __forceinline__ void each(F f) const
-    {
-        if constexpr (LIST) {
-            for (int i = threadIdx.x; i < sh.count; i += THREADS) f(value_of(sh.list_key[i]), sh.list_at[i]);
-        } else {
-            each_segment([&](int, int at, const float(&v)[8]) {
+        const int at = p * 8 + 8 <= V || V < 8 ? p * 8 : V - 8;
+        if (V >= 8) {
+            v.load(x + at);
+            if (at != p * 8)
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
-                    if (at + c < V) f(v[c], at + c);
-            });
+                    if (at + c < p * 8) v.set(c, -__builtin_inff());
+        } else {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v.set(c, c < V ? (float)x[c] : -__builtin_inff());
+        }
+        return at;
+    }
+    // f(number of a piece, index of its first value, the piece) for the pieces of a lane, then after(segment) behind each segment of a wavefront (four
+    // pieces of each lane).
+    template <class F, class G>
+    __device__ __forceinline__ void each_segment(F f, G after) const
+    {
+        const int pieces = (V + 7) / 8, segments = (V + kSegment - 1) / kSegment, lane = threadIdx.x & 63;
+#pragma unroll 1
+        for (int segment = wave_in_block(); segment < segments; segment += kWaves) {
+            Piece<T> v[kAhead];
+            const int p0 = segment * (kSegment / 8) + lane;
+            auto load = [&](int i, int p) {
+                if (p * 8 + 8 <= V) v[i].load(x + p * 8);
+            };
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) load(i, p0 + i * 64);
+#pragma unroll 1
+            for (int p = p0; p < p0 + 256; p += 64) {
+                Piece<T> now = v[0];
+#pragma unroll
+                for (int i = 0; i < kAhead - 1; ++i) v[i] = v[i + 1];
+                if (kAhead < 4 && p + kAhead * 64 < p0 + 256) load(kAhead - 1, p + kAhead * 64);
+                if (p < pieces) {
+                    int at = p * 8;
+                    if (at + 8 > V) at = piece(p, now);
+                    f(p, at, now);
+                }
+            }
+            after(segment);
         }
     }
 
-    __device__ __forceinline__ uint64_t block_sum(uint64_t v) const
+    // The sum of the threads' numbers in front of this one's, and of all.
+    struct Scan {
+        uint64_t before, all;
+    };
+    __device__ __forceinline__ Scan scan(uint64_t mine) const
     {
-        v = wave_sum_u64(v);
+        const uint64_t incl = wave_scan_u64(mine);
         __syncthreads();
-        if ((threadIdx.x & 63) == 0) sh.waves[threadIdx.x >> 6] = v;
+        if ((threadIdx.x & 63) == 63) sh.waves[threadIdx.x >> 6] = incl;
         __syncthreads();
-        uint64_t all = 0;
-        for (int w = 0; w < kWaves; ++w) all += sh.waves[w];
-        return all;
+        const int lane = threadIdx.x & 63, wave = wave_in_block();
+        const uint64_t waves = wave_scan_u64(lane < kWaves ? sh.waves[lane] : 0);
+        return Scan{incl - mine + (wave ? readlane_u64(waves, wave - 1) : 0), readlane_u64(waves, 63)};
+    }
+    // The largest of the threads' numbers.
+    __device__ __forceinline__ unsigned long long largest(unsigned long long mine) const
+    {
+        mine = wave_max_u64(mine);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) sh.best[threadIdx.x >> 6] = mine;
+        __syncthreads();
+        return wave_max_u64(((int)threadIdx.x & 63) < kWaves ? sh.best[threadIdx.x & 63] : 0ull);
     }
 
-    // The first of bins[0 .. n) at whose end base + the running sum reaches `target` (that of all, where it is never reached); the sum before it
-    // in `before` (base included), its own in `amount`.  All of the block call it; some bin is not 0.
-    __device__ __forceinline__ int find_bin(int n, uint64_t base, uint64_t target, uint64_t& before, uint64_t& amount) const
+    // The first of a[0 .. n) at whose end base + the running sum reaches `target` (that of all, where it is never reached); the sum before it
+    // in `before` (base included), its own in `amount`.  All of the block call it; some number is not 0.
+    template <class A>
+    __device__ __forceinline__ int find(const A* a, int n, uint64_t base, uint64_t target, uint64_t& before, uint64_t& amount) const
     {
         __syncthreads();
         const int per = (n + THREADS - 1) / THREADS, lo = threadIdx.x * per < n ? threadIdx.x * per : n, hi = lo + per < n ? lo + per : n;
         uint64_t mine = 0;
-        for (int i = lo; i < hi; ++i) mine += sh.bins[i];
-        uint64_t incl = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const uint64_t o = __shfl_up(incl, d);
-            if ((int)(threadIdx.x & 63) >= d) incl += o;
-        }
-        if ((threadIdx.x & 63) == 63) sh.waves[threadIdx.x >> 6] = incl;
-        __syncthreads();
-        uint64_t at = base + incl - mine, all = base;
-        for (int w = 0; w < kWaves; ++w) {
-            if (w < (int)(threadIdx.x >> 6)) at += sh.waves[w];
-            all += sh.waves[w];
-        }
-        if (target > all) target = all;
+#pragma unroll 1
+        for (int i = lo; i < hi; ++i) mine += a[i];
+        const Scan s = scan(mine);
+        uint64_t at = base + s.before;
+        if (target > base + s.all) target = base + s.all;
         if (at < target && target <= at + mine) {
             int i = lo;
-            while (i < hi - 1 && at + sh.bins[i] < target) at += sh.bins[i++];
+#pragma unroll 1
+            while (i < hi - 1 && at + a[i] < target) at += a[i++];
             sh.found = i;
             sh.found_before = at;
-            sh.found_amount = sh.bins[i];
+            sh.found_amount = a[i];
         }
         __syncthreads();
         before = sh.found_before;
@@ -229,29 +255,37 @@ struct SampleRow {
         return sh.found;
     }
 
-    __device__ __forceinline__ void clear_bins(int n) const
+    __device__ __forceinline__ void clear_bins() const
     {
         __syncthreads();
-        for (int i = threadIdx.x; i < n; i += THREADS) sh.bins[i] = 0;
+#pragma unroll 1
+        for (int i = threadIdx.x; i < kBins; i += THREADS) bins[i] = 0;
         __syncthreads();
     }
-    __device__ __forceinline__ void add(int bin, uint64_t amount) const { atomicAdd((unsigned long long*)&sh.bins[bin], (unsigned long long)amount); }
+    __device__ __forceinline__ void add(int bin, uint64_t amount) const { atomicAdd((unsigned long long*)&bins[bin], (unsigned long long)amount); }
 
-    // The largest key such that the amounts of the keys from it on reach `target` (they do over keys lo .. hi), with the sum above it and its own.
-    template <bool LIST, class F>
-    __device__ __forceinline__ unsigned int select(unsigned int lo, unsigned int hi, uint64_t target, F amount_of, uint64_t& above, uint64_t& amount) const
+    // The largest key such that the amounts (weights in units, or ones) of the keys from it on reach `target` (they do over keys lo .. hi), with the
+    // sum above it and its own.
+    __device__ __forceinline__ unsigned int select(unsigned int lo, unsigned int hi, uint64_t target, const SampleWeight& weight, bool by_weight, uint64_t& above,
+                                                   uint64_t& amount) const
     {
         above = 0;
         while (true) {
             int s = 0;
             while ((hi - lo) >> s >= (unsigned int)kBins) ++s;
-            clear_bins(kBins);
-            each<LIST>([&](float v, int) {
-                const unsigned int key = key_of(v);
-                if (key >= lo && key <= hi) add((hi - key) >> s, amount_of(v));
-            });
+            clear_bins();
+            each_segment([&](int, int at, const Piece<T>& v) {
+                Piece<T> left = v;
+#pragma unroll 1
+                for (int c = 0; c < 8; ++c) {
+                    const float one = left.value(0);
+                    const unsigned int key = key_of(one);
+                    if (key >= lo && key <= hi) add((hi - key) >> s, by_weight ? weight.units(weight(one)) : 1);
+                    left = shifted(left);
+                }
+            }, [](int) {});
             uint64_t before;
-            const int bin = find_bin(kBins, above, target, before, amount);
+            const int bin = find(bins, kBins, above, target, before, amount);
             above = before;
             hi -= (unsigned int)bin << s;
             if (s == 0) return hi;
@@ -259,80 +293,81 @@ struct SampleRow {
             lo = hi - lo > down ? hi - down : lo;
         }
     }
-
-    // What of the row, or of its list, stays.  lo and hi: the smallest and the largest key.
-    template <bool LIST>
-    __device__ __forceinline__ SampleKept keep(const SampleWeight& weight, unsigned int lo, unsigned int hi, int top_k, float top_p, float min_p, bool has_whole,
-                                               uint64_t whole) const
+    static __device__ __forceinline__ Piece<T> shifted(Piece<T> v)  // by one value
     {
-        SampleKept kept{lo, V, 0.0};
-        uint64_t equal_kept = 0;  // how many of the smallest value that stays do, where not all do (0: all)
-        if (top_k > 0 && top_k < V) {
-            uint64_t above, amount;
-            kept.key = select<LIST>(lo, hi, (uint64_t)top_k, [](float) { return (uint64_t)1; }, above, amount);
-            if (above + amount > (uint64_t)top_k) equal_kept = (uint64_t)top_k - above;
-        }
-        if (top_p < 1.0f) {
-            if (!has_whole) {
-                whole = 0;
-                each<LIST>([&](float v, int) {
-                    const unsigned int key = key_of(v);
-                    if (equal_kept ? key > kept.key : key >= kept.key) whole += weight.units(weight(v));
-                });
-                whole = block_sum(whole);
-                if (equal_kept) whole += equal_kept * weight.units(weight(value_of(kept.key)));
-            }
-            const uint64_t target = nucleus_target(top_p, whole);  // a token stays where what is before it is less
-            uint64_t above, amount;
-            const unsigned int key = select<LIST>(kept.key, hi, target, [&](float v) { return weight.units(weight(v)); }, above, amount);
-            const uint64_t one = weight.units(weight(value_of(key)));
-            const uint64_t all = amount / one, wanted = (target - above + one - 1) / one;
-            const uint64_t limit = key == kept.key && equal_kept ? equal_kept : all;
-            kept.key = key;
-            equal_kept = wanted < limit ? wanted : limit;
-            if (equal_kept == all) equal_kept = 0;
-        }
-        if (min_p > 0.0f) {
-            kept.least = fmin((double)min_p, 1.0);
-            if (weight(value_of(kept.key)) < kept.least) equal_kept = 0;
-        }
-        // ---- the index of the last of the equal ones that stay: the segment first, then its place there ----
-        if (equal_kept) {
-            uint64_t before, amount;
-            clear_bins((V + kSegment - 1) / kSegment);
-            each<LIST>([&](float v, int at) {
-                if (key_of(v) == kept.key) add(at / kSegment, 1);
-            });
-            const int segment = find_bin((V + kSegment - 1) / kSegment, 0, equal_kept, before, amount);
-            clear_bins(kSegment);
-            if constexpr (LIST) {
-                each<true>([&](float v, int at) {
-                    if (key_of(v) == kept.key && at / kSegment == segment) add(at % kSegment, 1);
-                });
-            } else {
-                for (int i = threadIdx.x; i < kSegment; i += THREADS)
-                    if (segment * kSegment + i < V && key_of((float)x[segment * kSegment + i]) == kept.key) add(i, 1);
-            }
-            kept.last = segment * kSegment + find_bin(kSegment, before, equal_kept, before, amount);
-        }
-        return kept;
+        elem e[8];
+        __builtin_memcpy(e, v.q, sizeof(e));
+#pragma unroll
+        for (int c = 0; c < 7; ++c) e[c] = e[c + 1];
+        __builtin_memcpy(v.q, e, sizeof(e));
+        return v;
     }
-    static __device__ __forceinline__ bool stays(const SampleKept& kept, float v, int at, double w)
+
+    // ---- counts of 16-bit values ----
+    // A value's place in the order of all, -0 with 0.
+    static __device__ __forceinline__ unsigned int place_of(unsigned int u)
     {
-        const unsigned int key = key_of(v);
-        return (key > kept.key || (key == kept.key && at <= kept.last)) && w >= kept.least;
+        u = u == 0x8000u ? 0u : u;
+        return u & 0x8000u ? ~u & 0xffffu : u | 0x8000u;
+    }
+    static __device__ __forceinline__ float value_at(unsigned int place)
+    {
+        const unsigned short u = (unsigned short)(place & 0x8000u ? place & 0x7fffu : ~place);
+        elem e;
+        __builtin_memcpy(&e, &u, 2);
+        return (float)e;
+    }
+    __device__ __forceinline__ unsigned int count_at(unsigned int place) const { return ties[place >> 1] >> (place & 1u ? 16 : 0) & 0xffffu; }
+    __device__ __forceinline__ void count_all() const
+    {
+        const uint4_t zero = {0, 0, 0, 0};
+#pragma unroll 1
+        for (int i = threadIdx.x; i < kCountWords / 4; i += THREADS) reinterpret_cast<uint4_t*>(ties)[i] = zero;
+        __syncthreads();
+        auto count = [&](unsigned int u) {
+            const unsigned int place = place_of(u);
+            atomicAdd(&ties[place >> 1], place & 1u ? 65536u : 1u);
+        };
+        each_segment([&](int, int at, const Piece<T>& v) {
+            const int from = at % 8 ? 8 - V % 8 : 0;  // (the last piece's first values are not its own)
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                if (c >= from) count(v.q[0][c / 2] >> c % 2 * 16 & 0xffffu);
+        }, [](int) {});
+        __syncthreads();
+    }
+    // The highest place such that the amounts (weights in units, or ones) of the places from it on reach `target`, with the sum above it and its
+    // own; sums: those of chunks of 2048 places.
+    __device__ __forceinline__ unsigned int select_counted(const uint64_t* sums, uint64_t target, const SampleWeight& weight, bool by_weight, uint64_t& above,
+                                                           uint64_t& amount) const
+    {
+        const int lane = threadIdx.x & 63;
+        const uint64_t mine = lane < 32 ? sums[31 - lane] : 0, incl = wave_scan_u64(mine), all = readlane_u64(incl, 63);
+        if (target > all) target = all;
+        const int at = __builtin_ctzll(__ballot(incl >= target)), chunk = 31 - at;  // (lane 31 has reached it)
+        above = readlane_u64(incl - mine, at);
+        __syncthreads();
+#pragma unroll 1
+        for (int i = threadIdx.x; i < kBins; i += THREADS) {
+            const unsigned int place = (unsigned int)(chunk * 2048 + 2047 - i), n = count_at(place);
+            bins[i] = n == 0 ? 0 : by_weight ? n * weight.units(weight(value_at(place))) : n;
+        }
+        const int bin = find(bins, kBins, above, target, above, amount);
+        return (unsigned int)(chunk * 2048 + 2047 - bin);
     }
 };
 
-template <class T, int THREADS>
-__global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a)
+template <class T, int THREADS, bool COUNT>
+__global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
 {
     typedef SampleRow<T, THREADS> Row;
-    constexpr int kWaves = THREADS / 64;
-    __shared__ typename Row::Shared sh;
+    constexpr int kWaves = THREADS / 64, kNamed = kBins * 2;
+    extern __shared__ __align__(16) char shared[];  // sample_shared_bytes()
+    typename Row::Shared& sh = *reinterpret_cast<typename Row::Shared*>(shared);
     const int64_t r = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 63, wave = wave_in_block(), V = a.V;
-    const Row row{(const typename T::elem*)a.logits + r * a.ld, V, sh};
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_in_block(), V = a.V, segments = (V + kSegment - 1) / kSegment;
+    uint64_t* const bins = reinterpret_cast<uint64_t*>(shared + sizeof(typename Row::Shared));
+    const Row row{(const typename T::elem*)a.logits + r * a.ld, V, sh, bins, reinterpret_cast<unsigned int*>(bins + (segments > kBins ? segments : kBins))};
     const float temperature = a.temperatures ? a.temperatures[r] : a.temperature, top_p = a.top_ps ? a.top_ps[r] : a.top_p;
     const float min_p = a.min_ps ? a.min_ps[r] : a.min_p, u = a.uniform[r];
     const int top_k = a.top_ks ? a.top_ks[r] : a.top_k;
@@ -342,276 +377,488 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a)
     };
     const bool unfit = !(temperature >= 0.0f && temperature < __builtin_inff()) || top_p != top_p || min_p != min_p || u != u;
     const bool greedy = unfit || temperature == 0.0f || top_k == 1 || top_p <= 0.0f;  // (the first of the largest is all that stays)
-    const bool cut_k = top_k > 0 && top_k < V, cut_p = top_p < 1.0f, cut_m = min_p > 0.0f;
-    const bool sums = !greedy && !cut_k && (cut_p || !cut_m);
-    const double rate = 1.4426950408889634 / (double)temperature;
-    const int segments = (V + kSegment - 1) / kSegment;
+    const bool cut_k = top_k > 0 && top_k < V, cut_p = top_p < 1.0f, cut_m = min_p > 0.0f, cut = cut_k || cut_p || cut_m;
+    const double rate = 1.4426950408889634 / (double)temperature, unit = ldexp(1.0, a.shift), least_weight = cut_m ? fmin((double)min_p, 1.0) : 0.0;
+    const unsigned int bottom_key = Row::key_of(-__builtin_inff());
+    SampleWeight weight{0.0, rate, unit};
+    // What stays: values above `smallest`, and the first equal_kept of those equal to it (0: all), in the order of indices, up to `last`.
+    float smallest = -__builtin_inff();
+    uint64_t equal_kept = 0;
+    int last = V;
+    uint64_t row_whole = 0, whole = 0, before, amount;
+    unsigned int top_key = 0;
+    bool relative = false;           // a pass's weights are relative to the largest value
+    double to_units = unit;          // and what they come to in units
+    bool settled = false;            // what stays is known before any pass
+    float least = __builtin_inff();  // what is to be listed: values from this on (inf: none)
+    auto log_share = [&](float v) { return (float)(((double)v - weight.top) / (double)temperature - log((double)whole / unit)); };
 
-    // ---- the largest value, the piece that has it first, and the sum of 2^(x rate) ----
-    unsigned long long best = 0;
-    float my_top = -__builtin_inff();
-    bool bad = false;
-    double my_sum = 0.0;
-    if (tid == 0) sh.bad = sh.count = 0;
-    __syncthreads();
-    row.each_segment([&](int segment, int at, const float(&v)[8]) {
-        float top = v[0];
-#pragma unroll
-        for (int c = 1; c < 8; ++c) top = fmaxf(top, v[c]);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) bad |= !(v[c] < __builtin_inff());
-        if (top > my_top || best == 0) {
-            my_top = top;
-            best = (unsigned long long)ordered_bits(top) << 32 | (unsigned int)~(unsigned int)at;
-        }
-        if (sums) {
-            double e[8];
-#pragma unroll
-            for (int c = 0; c < 8; ++c) e[c] = exp2_f64((double)v[c] * rate);
-            const double sum = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-            my_sum += sum;
-            if (!cut_p) {
-                double all = sum;
-#pragma unroll
-                for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
-                if (lane == 0) sh.segments[segment] = all;
-            }
-        }
-    });
-    const unsigned int my_key = best ? Row::key_of(my_top) : 0u;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const unsigned long long o = __shfl_xor(best, d);
-        best = o > best ? o : best;
-        my_sum += __shfl_xor(my_sum, d);
-    }
-    if (lane == 0) {
-        sh.best[wave] = best;
-        sh.waves_f[wave] = my_sum;
-    }
-    if (bad) sh.bad = 1;
-    __syncthreads();
-    double sum = 0.0;
-    for (int w = 0; w < kWaves; ++w) {
-        best = sh.best[w] > best ? sh.best[w] : best;
-        sum += sh.waves_f[w];
-    }
-    const float top = from_ordered((unsigned int)(best >> 32));
-    const unsigned int top_key = Row::key_of(top), bottom_key = Row::key_of(-__builtin_inff());
-    if (sh.bad || unfit) {
-        if (tid == 0) answer(-1, __builtin_nanf(""));
-        return;
-    }
-    if (top == -__builtin_inff()) {
-        if (tid == 0) answer(-1, -__builtin_inff());
-        return;
-    }
-    if (greedy) {
-        if (tid == 0) {
-            const int at = (int)~(unsigned int)best;
-            int c = 0;
-            while (at + c < V - 1 && (float)row.x[at + c] != top) ++c;
-            answer(at + c, 0.0f);
-        }
-        return;
-    }
-    const SampleWeight weight{(double)top, rate, ldexp(1.0, a.shift)};
-    const double exponent = (double)top * rate;
-    const bool summed = sums && fabs(exponent) <= kExponents;
-    const double to_units = summed ? exp2_f64(-exponent) * weight.unit : 0.0;
-    auto log_share = [&](float v, uint64_t whole) { return (float)(((double)v - weight.top) / (double)temperature - log((double)whole / weight.unit)); };
-
-    uint64_t before, amount, whole;
-    SampleKept kept{bottom_key, V, 0.0};
-    int segment;
-    if (summed && !cut_p) {
-        // ---- all tokens stay: the segments' sums are there ----
-        for (int i = tid; i < segments; i += THREADS) sh.bins[i] = (uint64_t)(sh.segments[i] * to_units);
-        __syncthreads();
-        whole = 0;
-        for (int i = tid; i < segments; i += THREADS) whole += sh.bins[i];
-        whole = row.block_sum(whole);
-        segment = row.find_bin(segments, 0, sample_target(u, whole), before, amount);
-    } else {
-        // ---- the list of what may stay ----
-        // Bounds are a little too low: what does not stay of the list is found below.
-        float least = __builtin_inff();
-        if (cut_k) {
-            if (top_k <= THREADS) {
-                // (over the threads' largest values as an order of 2048 steps from the smallest of them)
-                unsigned int low = my_key ? my_key : 0xffffffffu;
-#pragma unroll
-                for (int d = 1; d < 64; d *= 2) {
-                    const unsigned int o = __shfl_xor(low, d);
-                    low = o < low ? o : low;
+    // ---- 16-bit rows, value by value ----
+    if constexpr (COUNT) {
+        if (!greedy && (cut_k ? top_k > kListMost / 2 : cut_p)) {
+            static_assert(THREADS == 1024, "a chunk of places is a word for each thread");
+            row.count_all();
+            unsigned int high = 0, low = 0xffffu, n = 0;
+#pragma unroll 1
+            for (int i = 0; i < 32; ++i) {
+                const unsigned int two = row.ties[i * 1024 + tid], place = (unsigned int)(i * 1024 + tid) * 2;
+                n += (two & 0xffffu) + (two >> 16);
+                if (two != 0) {
+                    high = place + (two >> 16 ? 1 : 0);
+                    low = low != 0xffffu ? low : place + (two & 0xffffu ? 0 : 1);
                 }
-                row.clear_bins(Row::kBins);
-                if (lane == 0) sh.waves[wave] = low;
-                __syncthreads();
-                for (int w = 0; w < kWaves; ++w) low = (unsigned int)sh.waves[w] < low ? (unsigned int)sh.waves[w] : low;
-                __syncthreads();
-                int s = 0;
-                while ((top_key - low) >> s >= (unsigned int)Row::kBins) ++s;
-                if (my_key) row.add((top_key - my_key) >> s, 1);
-                const int bin = row.find_bin(Row::kBins, 0, (uint64_t)top_k, before, amount);
-                // (fewer threads than top_k have values, all of them: no bound then)
-                const unsigned int edge = before + amount < (uint64_t)top_k ? bottom_key : top_key - ((unsigned int)bin << s) - ((1u << s) - 1u);
-                least = Row::value_of(edge > bottom_key ? edge : bottom_key);
-                if (edge > top_key) least = -__builtin_inff();
             }
-        } else if (cut_p ? summed : true) {
-            // w >= share, that is x >= top + T log share; an fp32's rounding and more below that.
-            const double share = cut_p ? (1.0 - (double)top_p) * sum * (to_units / weight.unit) / (double)V : fmin((double)min_p, 1.0);
-            const double at = (double)top + log(share) * (double)temperature;
-            least = (float)(at - (fabs(at) + fabs((double)top)) * 0x1p-20 - 0x1p-100);
+            const uint64_t counted = row.scan(n).all;
+            high = (unsigned int)row.largest(high);
+            low = 0xffffu - (unsigned int)row.largest(0xffffu - low);
+            constexpr unsigned int kInf = __is_same(T, F16) ? 0x7c00u : 0x7f80u;
+            if (counted == (uint64_t)V) {  // (else a count has passed 65535: the row is taken as others are)
+                if (high >= (0x8000u | kInf) || low < (0x7fffu & ~kInf)) {
+                    if (tid == 0) answer(-1, __builtin_nanf(""));
+                    return;
+                }
+                if (high == (0x7fffu & ~kInf)) {
+                    if (tid == 0) answer(-1, -__builtin_inff());
+                    return;
+                }
+                weight.top = (double)Row::value_at(high);
+                top_key = Row::key_of(Row::value_at(high));
+                auto mass = [&](unsigned int place) { return weight.units(weight(Row::value_at(place))); };
+                if (tid < 32) sh.chunk_sums[tid] = sh.chunk_counts[tid] = 0;
+                __syncthreads();
+#pragma unroll 1
+                for (int i = (int)(high >> 11); i >= (int)(low >> 11); --i) {
+                    const unsigned int two = row.ties[i * 1024 + tid];
+                    if (!__ballot(two != 0)) continue;
+                    uint64_t part = 0;
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        const unsigned int count = h ? two >> 16 : two & 0xffffu;
+                        if (count) part += count * mass((unsigned int)(i * 1024 + tid) * 2 + h);
+                    }
+                    part = wave_total_u64(part);
+                    const unsigned int some = wave_total_u32((two & 0xffffu) + (two >> 16));
+                    if (lane == 0) {
+                        atomicAdd((unsigned long long*)&sh.chunk_sums[i], (unsigned long long)part);
+                        atomicAdd((unsigned long long*)&sh.chunk_counts[i], (unsigned long long)some);
+                    }
+                }
+                __syncthreads();
+                // First by counts (top_k), then by weights (top_p); behind each, what the places from the one found on have.
+                unsigned int place = 0;
+                uint64_t above, some = 0;
+#pragma unroll 1
+                for (int by_weight = 0; by_weight < 2; ++by_weight) {
+                    if (by_weight ? !cut_p : !cut_k) continue;
+                    if (by_weight && !cut_k) row_whole = wave_total_u64(lane < 32 ? sh.chunk_sums[lane] : 0);
+                    const uint64_t target = by_weight ? nucleus_target(top_p, row_whole) : (uint64_t)top_k;
+                    const unsigned int found = row.select_counted(by_weight ? sh.chunk_sums : sh.chunk_counts, target, weight, by_weight, above, amount);
+                    const uint64_t one = by_weight ? mass(found) : 1, all = amount / one, wanted = target > above ? (target - above + one - 1) / one : 1;
+                    const uint64_t limit = found == place && equal_kept ? equal_kept : all;
+                    equal_kept = wanted < limit ? wanted : limit;
+                    if (!by_weight) row_whole = equal_kept * mass(found);
+                    if (equal_kept == all) equal_kept = 0;
+                    place = found;
+                    uint64_t sum = tid < 32 && tid > (int)(place >> 11) ? sh.chunk_sums[tid] : 0;
+                    some = tid < 32 && tid > (int)(place >> 11) ? sh.chunk_counts[tid] : 0;
+#pragma unroll 1
+                    for (unsigned int at = (place & ~2047u) + tid; at < (place | 2047u) + 1; at += THREADS) {
+                        const unsigned int count = at >= place ? row.count_at(at) : 0;
+                        some += count;
+                        if (count && !by_weight && at > place) sum += count * mass(at);
+                    }
+                    some = row.scan(some).all;
+                    if (!by_weight) row_whole += row.scan(sum).all;
+                }
+                smallest = Row::value_at(place);
+                const double exponent = weight.top * rate;
+                relative = fabs(exponent) > kExponents;
+                to_units = relative ? unit : exp2_f64(-exponent) * unit;
+                settled = true;
+                if (some <= kListMost) least = smallest;
+            }
+            __syncthreads();
         }
-        const bool bounded = least < __builtin_inff();
-        if (bounded) {
-            row.each_segment([&](int, int at, const float(&v)[8]) {
-                float most = v[0];
+    }
+    if (tid == 0) sh.bad = sh.count = sh.named = 0;
+    __syncthreads();
+
+    // The pieces' largest values, as the upper halves of their keys, where they are looked at again.
+    unsigned short* const tops = reinterpret_cast<unsigned short*>(row.ties);
+    double* const sums_of = reinterpret_cast<double*>(bins);
+    // Passes over the row: the first, one that sums what top_k leaves, the last one with the segments' sums of what stays.
+    enum { kFirst, kSum, kLast };
+    int phase = settled ? kLast : kFirst;
+    bool listed = !settled;  // whether there has been no need of a list, or no room for it
+    while (true) {
+        const bool first = phase == kFirst;
+        if (!(settled && !listed && least < __builtin_inff())) {
+            if (phase == kLast && weight(smallest) < least_weight) {
+                // min_p comes down to a smallest value too: the lowest key of a weight that stays.
+                unsigned int out = Row::key_of(smallest), in = top_key;
+                while (in - out > 1) {
+                    const unsigned int mid = out + (in - out) / 2;
+                    (weight(Row::value_of(mid)) < least_weight ? out : in) = mid;
+                }
+                smallest = Row::value_of(in);
+                equal_kept = 0;
+            }
+            // ---- a pass ----
+            const bool sums = !first || (!greedy && !cut_k && (cut_p || !cut_m)), tops_kept = first && !greedy && cut && V <= kTopsMost;
+            const bool strict = equal_kept != 0;
+            // Values from `limit` on are summed: those above `smallest`, or from it on.  Exponents are those of x rate in the first pass and where that
+            // keeps to 64 bits' range; else relative to the largest value, fp32's differences being exact for what is near it.
+            const float limit = strict ? from_ordered(ordered_bits(smallest) + 1) : smallest, base = relative ? (float)weight.top : 0.0f;
+            unsigned long long best = 0;
+            float my_top = -__builtin_inff();
+            bool bad = false;
+            double sum = 0.0;
+            unsigned int equal = 0;
+            row.each_segment(
+                [&](int p, int at, const Piece<T>& v) {
+                    if (first) {
+                        float top = v.value(0);
 #pragma unroll
-                for (int c = 1; c < 8; ++c) most = fmaxf(most, v[c]);
-                if (most >= least) {
+                        for (int c = 0; c < 8; ++c) {
+                            top = fmaxf(top, v.value(c));
+                            bad |= !(v.value(c) < __builtin_inff());
+                        }
+                        if (tops_kept) tops[p] = (unsigned short)(ordered_bits(top) >> 16);
+                        if (top > my_top || best == 0) {
+                            my_top = top;
+                            best = (unsigned long long)ordered_bits(top) << 32 | (unsigned int)~(unsigned int)at;
+                        }
+                    }
+                    if (sums) {
+                        double e[8];
+                        if (first) {
 #pragma unroll
-                    for (int c = 0; c < 8; ++c)
-                        if (v[c] >= least && at + c < V) {
-                            const int i = atomicAdd(&sh.count, 1);
-                            if (i < kListMost) {
-                                sh.list_key[i] = Row::key_of(v[c]);
-                                sh.list_at[i] = at + c;
+                            for (int c = 0; c < 8; ++c) e[c] = exp2_f64((double)v.value(c) * rate);
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) e[c] = exp2_f64((double)(v.value(c) >= limit ? v.value(c) - base : -__builtin_inff()) * rate);
+                        }
+                        sum += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+                    }
+                    if (strict)
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) equal += v.value(c) == smallest ? 1 : 0;
+                },
+                [&](int segment) {
+                    if (!sums) return;
+                    sum = wave_total_f64(sum);
+                    if (lane == 0) sums_of[segment] = sum;
+                    if (strict) {
+                        equal = wave_total_u32(equal);
+                        if (lane == 0) row.ties[segment] = equal;
+                    }
+                    sum = 0.0;
+                    equal = 0;
+                });
+            __syncthreads();
+            if (first) {
+                const unsigned int my_key = best ? Row::key_of(my_top) : 0u;
+                if (bad) sh.bad = 1;
+                best = row.largest(best);
+                const float top = from_ordered((unsigned int)(best >> 32));
+                if (sh.bad || unfit || top == -__builtin_inff()) {
+                    if (tid == 0) answer(-1, sh.bad || unfit ? __builtin_nanf("") : -__builtin_inff());
+                    return;
+                }
+                if (greedy) {
+                    if (tid == 0) {
+                        const int at = (int)~(unsigned int)best;
+                        int c = 0;
+                        while (at + c < V - 1 && (float)row.x[at + c] != top) ++c;
+                        answer(at + c, 0.0f);
+                    }
+                    return;
+                }
+                top_key = Row::key_of(top);
+                weight.top = (double)top;
+                const double exponent = (double)top * rate;
+                relative = fabs(exponent) > kExponents;
+                const bool summed = sums && !relative;  // (else a pass relative to the largest value is next)
+                to_units = relative ? unit : exp2_f64(-exponent) * unit;
+                if (!cut) {
+                    phase = kLast;
+                    if (!summed) continue;
+                } else if (sums && !summed) {
+                    phase = kSum;
+                }
+                if (cut && phase == kFirst) {
+                    // ---- the bound of what may stay: a little too low each, what does not stay of the list is found there ----
+                    if (cut_k && top_k <= THREADS && top_k <= kListMost / 2) {
+                        // (over the threads' largest values as an order of 2048 steps from the smallest of them)
+                        const unsigned int low = ~(unsigned int)row.largest(my_key ? ~my_key : 0u);
+                        row.clear_bins();
+                        int s = 0;
+                        while ((top_key - low) >> s >= (unsigned int)kBins) ++s;
+                        if (my_key) row.add((top_key - my_key) >> s, 1);
+                        const int bin = row.find(bins, kBins, 0, (uint64_t)top_k, before, amount);
+                        // (fewer threads than top_k have values, all of them: no bound then)
+                        const unsigned int edge = top_key - ((unsigned int)bin << s) - ((1u << s) - 1u);
+                        least = before + amount < (uint64_t)top_k || edge > top_key || edge < bottom_key ? -__builtin_inff() : Row::value_of(edge);
+                    } else if (V <= kListMost) {
+                        least = -__builtin_inff();
+                    }
+                }
+            }
+            if (sums) {
+                // ---- the segments' sums as whole numbers, what is equal to the smallest value as far as it stays ----
+                uint64_t part = 0;
+                const uint64_t equal_units = strict ? weight.units(weight(smallest)) : 0;
+                if (strict && phase == kLast) {
+                    const int edge = row.find(row.ties, segments, 0, equal_kept, before, amount);
+                    // (the index of the last that stays, a value each thread)
+                    const uint64_t in_front = before;
+                    for (int i = tid; i <= edge; i += THREADS) sums_of[i] += (double)((i < edge ? (uint64_t)row.ties[i] : equal_kept - in_front) * equal_units) / to_units;
+                    __syncthreads();
+                    for (int i = tid; i < kSegment; i += THREADS) row.ties[i] = edge * kSegment + i < V && (float)row.x[edge * kSegment + i] == smallest ? 1 : 0;
+                    last = edge * kSegment + row.find(row.ties, kSegment, in_front, equal_kept, before, amount);
+                }
+                for (int i = tid; i < segments; i += THREADS) {
+                    const uint64_t units = (uint64_t)(sums_of[i] * to_units + 0.5);
+                    bins[i] = units;
+                    part += units;
+                }
+                whole = row.scan(part).all;
+                if (phase != kLast) row_whole = whole + (strict ? equal_kept * equal_units : 0);
+            }
+            if (phase == kLast) break;
+            if (first && phase == kFirst && !cut_k && cut && V > kListMost) {
+                // w >= share, that is x >= top + T log share; an fp32's rounding and more below that.
+                const double share = cut_p ? (1.0 - (double)top_p) * ((double)row_whole / unit) / (double)V : least_weight;
+                const double at = weight.top + log(share) * (double)temperature;
+                least = (float)(at - (fabs(at) + fabs(weight.top)) * 0x1p-20 - 0x1p-100);
+            }
+            if (first && phase == kSum) continue;
+        }
+
+        if (least < __builtin_inff()) {
+            // ---- the list: from the pieces whose largest value reaches the bound, or from all ----
+            auto take = [&](int at, const Piece<T>& v) {
+                unsigned int hits = 0;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) hits |= v.value(c) >= least ? 1u << c : 0u;
+                if (V < 8) hits &= (1u << V) - 1u;
+                if (at % 8) hits &= 0xffu << (8 - V % 8);  // (the last piece's first values are not its own)
+#pragma unroll 1
+                while (hits) {
+                    const int at_hit = at + __builtin_ctz(hits), i = atomicAdd(&sh.count, 1);
+                    hits &= hits - 1;
+                    if (i < kListMost) sh.list[i] = Row::entry_of(Row::key_of((float)row.x[at_hit]), at_hit);
+                }
+            };
+            int named = kNamed + 1;
+            if (first && V <= kTopsMost) {
+                unsigned int* names = reinterpret_cast<unsigned int*>(bins);
+                const unsigned short bound = (unsigned short)(ordered_bits(least) >> 16);
+                const int pieces = (V + 7) / 8;
+                __syncthreads();
+#pragma unroll 1
+                for (int p = tid; p < pieces; p += THREADS)
+                    if (tops[p] >= bound) {
+                        const int i = atomicAdd(&sh.named, 1);
+                        if (i < kNamed) names[i] = (unsigned int)p;
+                    }
+                __syncthreads();
+                named = sh.named;
+                if (named <= kNamed)
+#pragma unroll 1
+                    for (int i = tid; i < named; i += THREADS) {
+                        Piece<T> v;
+                        const int at = row.piece((int)names[i], v);
+                        take(at, v);
+                    }
+            }
+            if (named > kNamed)
+                row.each_segment([&](int, int at, const Piece<T>& v) { take(at, v); }, [](int) {});
+            __syncthreads();
+            const int count = sh.count;
+            least = __builtin_inff();
+            listed = true;
+            if (count <= 64) {
+                // ---- one wavefront, a lane each token ----
+                if (wave != 0) return;
+                const unsigned long long entry = lane < count ? sh.list[lane] : 0ull;
+                const float v = Row::value_in(entry);
+                const int at = Row::index_in(entry);
+                const double w = lane < count ? weight(v) : 0.0;
+                const uint64_t mine = weight.units(w);
+                int rank = 0;         // tokens in front of this one
+                uint64_t ahead = 0;   // and their weights
+#pragma unroll 1
+                for (int i = 0; i < count; ++i) {
+                    const uint64_t wi = readlane_u64(mine, i);
+                    if (readlane_u64(entry, i) > entry) {
+                        ++rank;
+                        ahead += wi;
+                    }
+                }
+                bool in = lane < count && !(cut_k && rank >= top_k);
+                const uint64_t all = !settled && (cut_k || V <= kListMost) ? wave_total_u64(in ? mine : 0) : row_whole;
+                in = in && (!cut_p || ahead < nucleus_target(top_p, all) || rank == 0) && w >= least_weight;
+                const uint64_t share = in ? mine : 0;
+                whole = wave_total_u64(share);
+                const uint64_t aim = sample_target(u, whole);
+                ahead = 0;
+#pragma unroll 1
+                for (int i = 0; i < count; ++i) {
+                    const uint64_t wi = readlane_u64(share, i);
+                    if (__builtin_amdgcn_readlane(at, i) < at) ahead += wi;
+                }
+                if (in && ahead < aim && aim <= ahead + share) answer(at, log_share(v));
+                return;
+            }
+            if (count <= kListMost) {
+                // ---- buckets: by keys first, for the order; then by indices, for the draw ----
+                constexpr int kEach = kListMost / THREADS, kPer = kBins / THREADS;
+                unsigned int* const counts = row.ties;                               // [kBins + 1]
+                unsigned short* const members = reinterpret_cast<unsigned short*>(counts + kBins + 1);  // [kListMost]: list entries, bucket by bucket
+                bool in[kEach];
+                unsigned int low = 0xffffffffu;
+                for (int i = tid; i < count; i += THREADS) low = (unsigned int)(sh.list[i] >> 32) < low ? (unsigned int)(sh.list[i] >> 32) : low;
+                low = ~(unsigned int)row.largest(~low);
+                uint64_t aim = 0;
+#pragma unroll 1
+                for (int by_index = 0; by_index < 2; ++by_index) {
+                    int s = 0;
+                    const unsigned int range = by_index ? (unsigned int)V - 1 : top_key - low;
+                    while (range >> s >= (unsigned int)kBins) ++s;
+                    auto bucket = [&](unsigned long long entry) { return (by_index ? (unsigned int)Row::index_in(entry) : top_key - (unsigned int)(entry >> 32)) >> s; };
+                    row.clear_bins();
+                    for (int i = tid; i <= kBins; i += THREADS) counts[i] = 0;
+                    __syncthreads();
+                    unsigned int slot[kEach];
+#pragma unroll
+                    for (int q = 0; q < kEach; ++q) {
+                        const int i = q * THREADS + tid;
+                        if (!by_index) in[q] = i < count;
+                        if (in[q]) {
+                            const unsigned int b = bucket(sh.list[i]);
+                            slot[q] = atomicAdd(&counts[b], 1u);
+                            row.add((int)b, weight.units(weight(Row::value_in(sh.list[i]))));
+                        }
+                    }
+                    __syncthreads();
+                    // Sums in front of each bucket.
+                    uint64_t mine = 0, some = 0;
+#pragma unroll
+                    for (int q = 0; q < kPer; ++q) {
+                        mine += bins[tid * kPer + q];
+                        some += counts[tid * kPer + q];
+                    }
+                    const typename Row::Scan masses = row.scan(mine), numbers = row.scan(some);
+                    mine = masses.before, some = numbers.before;
+#pragma unroll
+                    for (int q = 0; q < kPer; ++q) {
+                        const uint64_t m = bins[tid * kPer + q];
+                        const unsigned int c = counts[tid * kPer + q];
+                        bins[tid * kPer + q] = mine;
+                        counts[tid * kPer + q] = (unsigned int)some;
+                        mine += m;
+                        some += c;
+                    }
+                    if (tid == 0) counts[kBins] = (unsigned int)numbers.all;
+                    __syncthreads();
+#pragma unroll
+                    for (int q = 0; q < kEach; ++q)
+                        if (in[q]) members[counts[bucket(sh.list[q * THREADS + tid])] + slot[q]] = (unsigned short)(q * THREADS + tid);
+                    __syncthreads();
+                    // Each token's place in the order: what is in front of its bucket, and of its bucket what goes before it.
+                    uint64_t kept_sum = 0, ahead[kEach];
+                    int rank[kEach];
+#pragma unroll
+                    for (int q = 0; q < kEach; ++q) {
+                        ahead[q] = 0, rank[q] = 0;
+                        if (!in[q]) continue;
+                        const unsigned long long entry = sh.list[q * THREADS + tid];
+                        const unsigned int b = bucket(entry);
+                        ahead[q] = bins[b];
+                        rank[q] = (int)counts[b];
+#pragma unroll 1
+                        for (unsigned int i = counts[b]; i < counts[b + 1]; ++i) {
+                            const unsigned long long o = sh.list[members[i]];
+                            if (by_index ? (unsigned int)o > (unsigned int)entry : o > entry) {  // (lower halves are the indices' complements)
+                                ++rank[q];
+                                ahead[q] += weight.units(weight(Row::value_in(o)));
                             }
                         }
-                }
-            });
-            __syncthreads();
-        }
-        const int count = bounded ? sh.count : kListMost + 1;
-        const uint64_t row_whole = summed ? (uint64_t)(sum * to_units) : 0;
-        if (count <= 64) {
-            // ---- one wavefront, a lane each token ----
-            if (wave != 0) return;
-            const unsigned int key = lane < count ? sh.list_key[lane] : 0u;
-            const int at = lane < count ? sh.list_at[lane] : 0x7fffffff;
-            const unsigned long long order = (unsigned long long)key << 32 | (unsigned int)~(unsigned int)at;
-            const float v = Row::value_of(key);
-            const double w = lane < count ? weight(v) : 0.0;
-            const uint64_t mine = weight.units(w);
-            int rank = 0;         // tokens in front of this one
-            uint64_t ahead = 0;   // and their weights
-            for (int i = 0; i < count; ++i) {
-                const unsigned long long o = __shfl(order, i);
-                const uint64_t wi = __shfl(mine, i);
-                if (o > order) {
-                    ++rank;
-                    ahead += wi;
-                }
-            }
-            bool in = lane < count && !(cut_k && rank >= top_k);
-            if (cut_p) {
-                const uint64_t all = cut_k ? wave_sum_u64(in ? mine : 0) : row_whole;
-                const uint64_t target = nucleus_target(top_p, all);
-                in = in && (ahead < target || rank == 0);
-            }
-            if (cut_m) in = in && w >= fmin((double)min_p, 1.0);
-            const uint64_t share = in ? mine : 0;
-            whole = wave_sum_u64(share);
-            const uint64_t target = sample_target(u, whole);
-            uint64_t front = 0;  // the weights of what stays at smaller indices
-            for (int i = 0; i < count; ++i) {
-                const int oi = __shfl(at, i);
-                const uint64_t wi = __shfl(share, i);
-                if (oi < at) front += wi;
-            }
-            if (in && front < target && target <= front + share) answer(at, log_share(v, whole));
-            return;
-        }
-        if (count <= kListMost) {
-            unsigned int low = 0xffffffffu;
-            for (int i = tid; i < count; i += THREADS) low = sh.list_key[i] < low ? sh.list_key[i] : low;
+                        if (!by_index && !(cut_k && rank[q] >= top_k)) kept_sum += weight.units(weight(Row::value_in(entry)));
+                    }
+                    if (by_index) {
 #pragma unroll
-            for (int d = 1; d < 64; d *= 2) {
-                const unsigned int o = __shfl_xor(low, d);
-                low = o < low ? o : low;
-            }
-            __syncthreads();
-            if (lane == 0) sh.waves[wave] = low;
-            __syncthreads();
-            for (int w = 0; w < kWaves; ++w) low = (unsigned int)sh.waves[w] < low ? (unsigned int)sh.waves[w] : low;
-            __syncthreads();
-            kept = row.template keep<true>(weight, low, top_key, top_k, top_p, min_p, !cut_k && cut_p, row_whole);
-            // ---- the draw: the segment, then the place in it ----
-            row.clear_bins(segments);
-            uint64_t part = 0;
-            row.template each<true>([&](float v, int at) {
-                const double w = weight(v);
-                if (!Row::stays(kept, v, at, w)) return;
-                row.add(at / kSegment, weight.units(w));
-                part += weight.units(w);
-            });
-            whole = row.block_sum(part);
-            const uint64_t target = sample_target(u, whole);
-            segment = row.find_bin(segments, 0, target, before, amount);
-            row.clear_bins(kSegment);
-            row.template each<true>([&](float v, int at) {
-                if (at / kSegment != segment) return;
-                const double w = weight(v);
-                if (Row::stays(kept, v, at, w)) row.add(at % kSegment, weight.units(w));
-            });
-            const int place = row.find_bin(kSegment, before, target, before, amount);
-            if (tid == 0) answer(segment * kSegment + place, log_share((float)row.x[segment * kSegment + place], whole));
-            return;
-        }
-        // ---- the row in place of the list ----
-        if (cut_k || cut_p || cut_m) kept = row.template keep<false>(weight, bottom_key, top_key, top_k, top_p, min_p, summed && cut_p, row_whole);
-        __syncthreads();
-        row.each_segment([&](int segment, int at, const float(&v)[8]) {
-            uint64_t part = 0;
+                        for (int q = 0; q < kEach; ++q) {
+                            if (!in[q]) continue;
+                            const unsigned long long entry = sh.list[q * THREADS + tid];
+                            const float v = Row::value_in(entry);
+                            if (ahead[q] < aim && aim <= ahead[q] + weight.units(weight(v))) answer(Row::index_in(entry), log_share(v));
+                        }
+                        return;
+                    }
+                    if (!settled && (cut_k || V <= kListMost)) row_whole = row.scan(kept_sum).all;
+                    const uint64_t target = nucleus_target(top_p, row_whole);
+                    uint64_t share = 0;
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                const double w = weight(v[c]);
-                if (at + c < V && Row::stays(kept, v[c], at + c, w)) part += weight.units(w);
+                    for (int q = 0; q < kEach; ++q) {
+                        if (!in[q]) continue;
+                        const double w = weight(Row::value_in(sh.list[q * THREADS + tid]));
+                        in[q] = !(cut_k && rank[q] >= top_k) && (!cut_p || ahead[q] < target || rank[q] == 0) && w >= least_weight;
+                        if (in[q]) share += weight.units(w);
+                    }
+                    whole = row.scan(share).all;
+                    aim = sample_target(u, whole);
+                }
             }
-            part = wave_sum_u64(part);
-            if (lane == 0) sh.bins[segment] = part;
-        });
-        __syncthreads();
-        whole = 0;
-        for (int i = tid; i < segments; i += THREADS) whole += sh.bins[i];
-        whole = row.block_sum(whole);
-        segment = row.find_bin(segments, 0, sample_target(u, whole), before, amount);
+            if (settled) continue;  // (what stays was known to fit: not reached)
+        }
+
+        // ---- the row in place of the list: the smallest value that stays ----
+        const bool by_weight = !(first && cut_k);
+        if (by_weight ? cut_p : true) {
+            const uint64_t target = by_weight ? nucleus_target(top_p, row_whole) : (uint64_t)top_k;
+            const unsigned int from = Row::key_of(smallest);
+            uint64_t above;
+            const unsigned int key = row.select(from, top_key, target, weight, by_weight, above, amount);
+            const uint64_t one = by_weight ? weight.units(weight(Row::value_of(key))) : 1, all = amount / one, wanted = target > above ? (target - above + one - 1) / one : 1;
+            const uint64_t limit = key == from && equal_kept ? equal_kept : all;
+            equal_kept = wanted < limit ? wanted : limit;
+            if (equal_kept == all) equal_kept = 0;
+            smallest = Row::value_of(key);
+        }
+        phase = !by_weight && cut_p ? kSum : kLast;
+
     }
-    // ---- the draw in its segment ----
-    if (wave == 0) {
-        const int at = (segment * 64 + lane) * 8;
-        float v[8];
-        uint64_t w[8], part = 0;
-        row.piece(at < V ? at / 8 : (V - 1) / 8, v);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            const double e = weight(v[c]);
-            w[c] = at + c < V && Row::stays(kept, v[c], at + c, e) ? weight.units(e) : 0;
-            part += w[c];
+
+    // ---- the draw: the segment, then the value in it, one each thread ----
+    const uint64_t aim = sample_target(u, whole);
+    const int segment = row.find(bins, segments, 0, aim, before, amount);
+    const uint64_t in_front = before;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = tid; i < kSegment; i += THREADS) {
+        const int at = segment * kSegment + i;
+        uint64_t units = 0;
+        if (at < V) {
+            const float v = (float)row.x[at];
+            const double w = weight(v);
+            if (v > smallest || (v == smallest && at <= last)) units = weight.units(w);
         }
-        uint64_t incl = part;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const uint64_t o = __shfl_up(incl, d);
-            if (lane >= d) incl += o;
-        }
-        // (the first pass's sum of a segment may be some units more than its tokens': its last token is drawn then)
-        const uint64_t all = __shfl(incl, 63), wanted = sample_target(u, whole) - before, target = wanted < all ? wanted : all;
-        uint64_t front = incl - part;
-        if (front < target && target <= incl) {
-            bool found = false;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                if (!found && front + w[c] >= target) {
-                    found = true;
-                    answer(at + c, log_share(v[c], whole));
-                }
-                front += w[c];
-            }
-        }
+        bins[i] = units;
     }
+    // (a segment's sum may be some units more than its values': its last value is drawn then)
+    const int at = segment * kSegment + row.find(bins, kSegment, in_front, aim, before, amount);
+    if (tid == 0) answer(at, log_share((float)row.x[at]));
+}
+
+// What a block needs of LDS.
+template <class T, int THREADS, bool COUNT>
+inline unsigned int sample_shared_bytes(int V)
+{
+    const int segments = (V + kSegment - 1) / kSegment, bins = segments > kBins ? segments : kBins;
+    const int own = V <= kTopsMost ? segments * (kSegment / 16) : segments > kSegment ? segments : kSegment, buckets = kBins + 1 + kListMost / 2;
+    const int words = COUNT ? kCountWords : own > buckets ? own : buckets;
+    return (unsigned int)(sizeof(typename SampleRow<T, THREADS>::Shared) + bins * sizeof(uint64_t) + words * sizeof(unsigned int));
 }
 }  // namespace pimhip
