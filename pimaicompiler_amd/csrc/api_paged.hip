@@ -139,15 +139,17 @@ extern "C" int pimhip_paged_append(const PimHipPagedCache* cache, const PimHipPa
     if (q) a.q = q->data, a.q_token = q->token_stride, a.q_head = q->head_stride, a.q_out = q_out, a.q_heads = q_heads;
     a.angles = angles, a.ld_angles = ld_angles, a.half = rotary_dim / 2, a.tokens = (int)tokens;
     a.items = (2 * a.c.kv_heads + a.q_heads) * (a.c.dim / 8);
-    const dim3 grid((unsigned)tokens, (unsigned)(a.items + 255) / 256);
+    // Blocks of one group a thread for a step's tokens, of four where there are tokens enough for every CU.
+    const bool many = tokens >= 4 * (int64_t)st->num_cus;
+    const dim3 grid((unsigned)tokens, (unsigned)(a.items + 255) / 256), grid4((unsigned)tokens, (unsigned)(a.items + 1023) / 1024);
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto run = [&](auto type, auto fp8) {
         typedef decltype(type) T;
         constexpr bool kFp8 = decltype(fp8)::value;
         if (interleaved)
-            paged_append_kernel<T, kFp8, true><<<grid, 256, 0, s>>>(a);
+            many ? paged_append_kernel<T, kFp8, true, 4><<<grid4, 256, 0, s>>>(a) : paged_append_kernel<T, kFp8, true, 1><<<grid, 256, 0, s>>>(a);
         else
-            paged_append_kernel<T, kFp8, false><<<grid, 256, 0, s>>>(a);
+            many ? paged_append_kernel<T, kFp8, false, 4><<<grid4, 256, 0, s>>>(a) : paged_append_kernel<T, kFp8, false, 1><<<grid, 256, 0, s>>>(a);
     };
     auto run_type = [&](auto type) { cache->dtype == PIMHIP_F8E4M3 ? run(type, std::true_type{}) : run(type, std::false_type{}); };
     dtype == PIMHIP_F16 ? run_type(F16{}) : run_type(BF16{});

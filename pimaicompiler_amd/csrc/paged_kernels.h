@@ -61,15 +61,41 @@ struct AppendArgs {
     int items;                  // groups of eight of a token
 };
 
-// A block is one token's heads, a thread eight values of one: of a key (query) the eight behind them or half a rotation away are loaded
-// beside them, out of the caches as a rule.  Bound by the bytes where tokens are many, else by four dependent loads: the sequence, its length,
-// the page, the values.
-template <class T, bool FP8, bool INTERLEAVED>
+// A head of a token: those of keys come first, then those of values and of queries.
+template <class E>
+__device__ __forceinline__ const E* row_of(const AppendArgs& a, int t, int head)
+{
+    const int kv = a.c.kv_heads;
+    return head < kv ? (const E*)a.k + t * a.k_token + head * a.k_head
+           : head < 2 * kv ? (const E*)a.v + t * a.v_token + (head - kv) * a.v_head
+                           : (const E*)a.q + t * a.q_token + (head - 2 * kv) * a.q_head;
+}
+
+// A block is heads of one token, a thread ITEMS groups of eight values of one: of a key (query) the eight that a rotation turns them with are loaded
+// beside them, out of the caches as a rule.  Values are asked for before the token's place is known, which takes three dependent loads: the
+// sequence, its length, the page.  Bound by the bytes where tokens are many (8001 of 32 query and 8 key heads of 128 in bfloat16: 8 groups a thread), else
+// by those loads.
+template <class T, bool FP8, bool INTERLEAVED, int ITEMS>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
 {
     typedef typename T::elem elem;
-    const int t = blockIdx.x;
-    const int item = blockIdx.y * 256 + threadIdx.x;
+    typedef typename T::frag frag;
+    const int t = blockIdx.x, groups = a.c.dim / 8;
+    const bool halves = !INTERLEAVED && a.half % 8 == 0;  // a group's partner is another group
+    // ---- the values ----
+    int head[ITEMS], d[ITEMS];  // heads of keys, then of values, then of queries; -1: none
+    frag mine[ITEMS], other[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const int item = ((int)blockIdx.y * ITEMS + i) * 256 + (int)threadIdx.x;
+        head[i] = item < a.items ? item / groups : -1;
+        d[i] = (item - head[i] * groups) * 8;
+        if (head[i] < 0) continue;
+        const elem* x = row_of<elem>(a, t, head[i]);
+        mine[i] = load8_any<T>(x + d[i]);
+        other[i] = frag{};
+        if (halves && d[i] < 2 * a.half) other[i] = load8_any<T>(x + (d[i] < a.half ? d[i] + a.half : d[i] - a.half));
+    }
     // ---- the token's place ----
     int s = t, end = t + 1;
     if (a.starts) {
@@ -91,78 +117,62 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
     int64_t where = -1;
     if (s < a.c.sequences) where = (int64_t)a.c.lengths[s] - ((int64_t)end - t);
     const int pos = where >= 0 && where < a.c.most ? (int)where : -1;
-    int page = -1;
-    if (pos >= 0) page = a.c.table[s * a.c.ld_table + a.c.page_of(pos)];
-    if (item >= a.items) return;
-    const int groups = a.c.dim / 8, head_of_all = item / groups, d = (item - head_of_all * groups) * 8;
-    const bool is_k = head_of_all < a.c.kv_heads, is_v = !is_k && head_of_all < 2 * a.c.kv_heads;
-    const int head = is_k ? head_of_all : is_v ? head_of_all - a.c.kv_heads : head_of_all - 2 * a.c.kv_heads;
+    const int page = pos >= 0 ? a.c.table[s * a.c.ld_table + a.c.page_of(pos)] : -1, at = pos - a.c.page_of(pos) * a.c.page_size;
     const bool stored = page >= 0 && page < a.c.pages;
-    if (!is_k && !is_v && pos < 0) {  // a query of no sequence
-        *reinterpret_cast<uint4_any_t*>((elem*)a.q_out + ((int64_t)t * a.q_heads + head) * a.c.dim + d) = uint4_t{0, 0, 0, 0};
-        return;
-    }
-    if ((is_k || is_v) && !stored) return;
-    const elem* x = is_k   ? (const elem*)a.k + t * a.k_token + head * a.k_head
-                    : is_v ? (const elem*)a.v + t * a.v_token + head * a.v_head
-                           : (const elem*)a.q + t * a.q_token + head * a.q_head;
-    const typename T::frag mine = load8_any<T>(x + d);
-    float y[8];
+    const float* row = a.angles + pos * a.ld_angles;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = (float)mine[i];
-    if (!is_v && d < 2 * a.half) {
-        const float* row = a.angles + pos * a.ld_angles;
-        if constexpr (INTERLEAVED) {
+    for (int i = 0; i < ITEMS; ++i) {
+        const bool is_k = head[i] >= 0 && head[i] < a.c.kv_heads, is_q = head[i] >= 2 * a.c.kv_heads;
+        if (head[i] < 0 || (!is_q && !stored)) continue;
+        float y[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int p = d / 2 + i;
-                if (p < a.half) {
-                    const float c = row[p], w = row[a.half + p], u = y[2 * i], v = y[2 * i + 1];
-                    y[2 * i] = u * c - v * w;
-                    y[2 * i + 1] = u * w + v * c;
+        for (int c = 0; c < 8; ++c) y[c] = (float)mine[i][c];
+        if ((is_k || is_q) && d[i] < 2 * a.half && pos >= 0) {
+            if constexpr (INTERLEAVED) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int p = d[i] / 2 + c;
+                    if (p < a.half) {
+                        const float cosine = row[p], sine = row[a.half + p], u = y[2 * c], v = y[2 * c + 1];
+                        y[2 * c] = u * cosine - v * sine;
+                        y[2 * c + 1] = u * sine + v * cosine;
+                    }
+                }
+            } else {
+                // (a group may hold values of both halves, and values behind them, where a half is no multiple of eight)
+                const elem* x = row_of<elem>(a, t, head[i]);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const int e = d[i] + c;
+                    if (halves || e < 2 * a.half) {
+                        const bool first = e < a.half;
+                        const int p = first ? e : e - a.half;
+                        const float o = halves ? (float)other[i][c] : (float)x[first ? e + a.half : e - a.half];
+                        const float cosine = row[p], sine = row[a.half + p];
+                        y[c] = first ? y[c] * cosine - o * sine : o * sine + y[c] * cosine;
+                    }
                 }
             }
+        }
+        if (is_q) {
+            if (pos < 0)  // a query of no sequence
+#pragma unroll
+                for (int c = 0; c < 8; ++c) y[c] = 0.0f;
+            store8<T>((elem*)a.q_out + ((int64_t)t * a.q_heads + head[i] - 2 * a.c.kv_heads) * a.c.dim + d[i], float4_t{y[0], y[1], y[2], y[3]}, float4_t{y[4], y[5], y[6], y[7]});
+            continue;
+        }
+        const int h = is_k ? head[i] : head[i] - a.c.kv_heads;
+        char* out = is_k ? a.c.k + page * a.c.k_page + h * a.c.k_head + (int64_t)at * a.c.k_tok : a.c.v + page * a.c.v_page + h * a.c.v_head + (int64_t)at * a.c.v_tok;
+        if constexpr (FP8) {
+            const float scale = (is_k ? a.c.k_scale : a.c.v_scale)[h];
+            unsigned int r[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) r[c] = to_e4m3x2(y[4 * c] / scale, y[4 * c + 1] / scale) | to_e4m3x2(y[4 * c + 2] / scale, y[4 * c + 3] / scale) << 16;
+            typedef uint2_t bytes8_t __attribute__((aligned(1)));
+            *reinterpret_cast<bytes8_t*>(out + d[i]) = uint2_t{r[0], r[1]};
         } else {
-            // A group may hold values of both halves, and values behind them, where a half is no multiple of eight.
-            const bool whole = a.half % 8 == 0;
-            typename T::frag other = {};
-            if (whole) other = load8_any<T>(x + (d < a.half ? d + a.half : d - a.half));
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int e = d + i;
-                if (whole || e < 2 * a.half) {
-                    const bool first = e < a.half;
-                    const int p = first ? e : e - a.half;
-                    const float o = whole ? (float)other[i] : (float)x[first ? e + a.half : e - a.half];
-                    const float c = row[p], w = row[a.half + p];
-                    y[i] = first ? y[i] * c - o * w : o * w + y[i] * c;
-                }
-            }
+            store8<T>((elem*)out + d[i], float4_t{y[0], y[1], y[2], y[3]}, float4_t{y[4], y[5], y[6], y[7]});
         }
-    }
-    if (!is_k && !is_v) {
-        elem* out = (elem*)a.q_out + ((int64_t)t * a.q_heads + head) * a.c.dim + d;
-        const elem r[8] = {T::round(y[0]), T::round(y[1]), T::round(y[2]), T::round(y[3]), T::round(y[4]), T::round(y[5]), T::round(y[6]), T::round(y[7])};
-        *reinterpret_cast<uint4_any_t*>(out) = __builtin_bit_cast(uint4_t, r);
-        return;
-    }
-    const int at = pos - a.c.page_of(pos) * a.c.page_size;
-    char* out = is_k ? a.c.k + page * a.c.k_page + head * a.c.k_head + (int64_t)at * a.c.k_tok
-                     : a.c.v + page * a.c.v_page + head * a.c.v_head + (int64_t)at * a.c.v_tok;
-    if constexpr (FP8) {
-        const float scale = (is_k ? a.c.k_scale : a.c.v_scale)[head];
-        unsigned char r[8];
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            const unsigned int two = to_e4m3x2(y[i] / scale, y[i + 1] / scale);
-            r[i] = (unsigned char)two;
-            r[i + 1] = (unsigned char)(two >> 8);
-        }
-        typedef uint2_t bytes8_t __attribute__((aligned(1)));
-        *reinterpret_cast<bytes8_t*>(out + d) = __builtin_bit_cast(uint2_t, r);
-    } else {
-        const elem r[8] = {T::round(y[0]), T::round(y[1]), T::round(y[2]), T::round(y[3]), T::round(y[4]), T::round(y[5]), T::round(y[6]), T::round(y[7])};
-        *reinterpret_cast<uint4_any_t*>(out + 2 * d) = __builtin_bit_cast(uint4_t, r);
     }
 }
 

@@ -270,18 +270,33 @@ struct SampleRow {
                                                    uint64_t& amount) const
     {
         above = 0;
+        const unsigned int top = hi;
         while (true) {
             int s = 0;
             while ((hi - lo) >> s >= (unsigned int)kBins) ++s;
             clear_bins();
+            // (most values are in the first range, few in a bucket of it)
+            const float from = value_of(lo), to = value_of(hi);
             each_segment([&](int, int at, const Piece<T>& v) {
-                Piece<T> left = v;
+                const int begin = at % 8 ? 8 - V % 8 : 0;  // (the last piece's first values are not its own)
+                if (above == 0 && hi == top) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const float one = v.value(c);
+                        const uint64_t amount_of = by_weight ? weight.units(weight(one)) : 1;
+                        if (one >= from && c >= begin) add((hi - key_of(one)) >> s, amount_of);
+                    }
+                    return;
+                }
+                unsigned int hits = 0;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) hits |= v.value(c) >= from && v.value(c) <= to ? 1u << c : 0u;
+                hits &= 0xffu << begin;
 #pragma unroll 1
-                for (int c = 0; c < 8; ++c) {
-                    const float one = left.value(0);
-                    const unsigned int key = key_of(one);
-                    if (key >= lo && key <= hi) add((hi - key) >> s, by_weight ? weight.units(weight(one)) : 1);
-                    left = shifted(left);
+                while (hits) {
+                    const float one = (float)x[at + __builtin_ctz(hits)];
+                    hits &= hits - 1;
+                    add((hi - key_of(one)) >> s, by_weight ? weight.units(weight(one)) : 1);
                 }
             }, [](int) {});
             uint64_t before;
@@ -292,15 +307,6 @@ struct SampleRow {
             const unsigned int down = (1u << s) - 1u;
             lo = hi - lo > down ? hi - down : lo;
         }
-    }
-    static __device__ __forceinline__ Piece<T> shifted(Piece<T> v)  // by one value
-    {
-        elem e[8];
-        __builtin_memcpy(e, v.q, sizeof(e));
-#pragma unroll
-        for (int c = 0; c < 7; ++c) e[c] = e[c + 1];
-        __builtin_memcpy(v.q, e, sizeof(e));
-        return v;
     }
 
     // ---- counts of 16-bit values ----
@@ -391,6 +397,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
     double to_units = unit;          // and what they come to in units
     bool settled = false;            // what stays is known before any pass
     float least = __builtin_inff();  // what is to be listed: values from this on (inf: none)
+    float bound = -__builtin_inff();  // nothing below this stays
     auto log_share = [&](float v) { return (float)(((double)v - weight.top) / (double)temperature - log((double)whole / unit)); };
 
     // ---- 16-bit rows, value by value ----
@@ -599,7 +606,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
                         // (fewer threads than top_k have values, all of them: no bound then)
                         const unsigned int edge = top_key - ((unsigned int)bin << s) - ((1u << s) - 1u);
                         least = before + amount < (uint64_t)top_k || edge > top_key || edge < bottom_key ? -__builtin_inff() : Row::value_of(edge);
-                    } else if (V <= kListMost) {
+                    } else if (cut_k && V <= kListMost) {
                         least = -__builtin_inff();
                     }
                 }
@@ -626,7 +633,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
                 if (phase != kLast) row_whole = whole + (strict ? equal_kept * equal_units : 0);
             }
             if (phase == kLast) break;
-            if (first && phase == kFirst && !cut_k && cut && V > kListMost) {
+            if (first && phase == kFirst && !cut_k && cut) {
                 // w >= share, that is x >= top + T log share; an fp32's rounding and more below that.
                 const double share = cut_p ? (1.0 - (double)top_p) * ((double)row_whole / unit) / (double)V : least_weight;
                 const double at = weight.top + log(share) * (double)temperature;
@@ -653,12 +660,12 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
             int named = kNamed + 1;
             if (first && V <= kTopsMost) {
                 unsigned int* names = reinterpret_cast<unsigned int*>(bins);
-                const unsigned short bound = (unsigned short)(ordered_bits(least) >> 16);
+                const unsigned short from = (unsigned short)(ordered_bits(least) >> 16);
                 const int pieces = (V + 7) / 8;
                 __syncthreads();
 #pragma unroll 1
                 for (int p = tid; p < pieces; p += THREADS)
-                    if (tops[p] >= bound) {
+                    if (tops[p] >= from) {
                         const int i = atomicAdd(&sh.named, 1);
                         if (i < kNamed) names[i] = (unsigned int)p;
                     }
@@ -676,6 +683,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
                 row.each_segment([&](int, int at, const Piece<T>& v) { take(at, v); }, [](int) {});
             __syncthreads();
             const int count = sh.count;
+            bound = least;
             least = __builtin_inff();
             listed = true;
             if (count <= 64) {
@@ -697,7 +705,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
                     }
                 }
                 bool in = lane < count && !(cut_k && rank >= top_k);
-                const uint64_t all = !settled && (cut_k || V <= kListMost) ? wave_total_u64(in ? mine : 0) : row_whole;
+                const uint64_t all = !settled && cut_k ? wave_total_u64(in ? mine : 0) : row_whole;
                 in = in && (!cut_p || ahead < nucleus_target(top_p, all) || rank == 0) && w >= least_weight;
                 const uint64_t share = in ? mine : 0;
                 whole = wave_total_u64(share);
@@ -797,7 +805,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
                         }
                         return;
                     }
-                    if (!settled && (cut_k || V <= kListMost)) row_whole = row.scan(kept_sum).all;
+                    if (!settled && cut_k) row_whole = row.scan(kept_sum).all;
                     const uint64_t target = nucleus_target(top_p, row_whole);
                     uint64_t share = 0;
 #pragma unroll
@@ -818,9 +826,9 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
         const bool by_weight = !(first && cut_k);
         if (by_weight ? cut_p : true) {
             const uint64_t target = by_weight ? nucleus_target(top_p, row_whole) : (uint64_t)top_k;
-            const unsigned int from = Row::key_of(smallest);
+            const unsigned int from = Row::key_of(smallest), lowest = bound > smallest ? Row::key_of(bound) : from;
             uint64_t above;
-            const unsigned int key = row.select(from, top_key, target, weight, by_weight, above, amount);
+            const unsigned int key = row.select(lowest, top_key, target, weight, by_weight, above, amount);
             const uint64_t one = by_weight ? weight.units(weight(Row::value_of(key))) : 1, all = amount / one, wanted = target > above ? (target - above + one - 1) / one : 1;
             const uint64_t limit = key == from && equal_kept ? equal_kept : all;
             equal_kept = wanted < limit ? wanted : limit;
