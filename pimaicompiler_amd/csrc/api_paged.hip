@@ -130,6 +130,7 @@ extern "C" int pimhip_paged_append(const PimHipPagedCache* cache, const PimHipPa
         return fail(PIMHIP_ERR_INVALID_ARGUMENT, "angles must be [%d or more, %d], got %lld rows with a pitch of %lld", a.c.most, rotary_dim, (long long)angle_rows,
                     (long long)ld_angles);
     if (q && (q_heads < 1 || q_heads > 65535 || !q_out || !element_aligned(q_out, 2))) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "q_heads=%d, or q_out is null", q_heads);
+    if (cache->k == cache->v) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "keys and values of the cache are the same memory");
     if (tokens == 0) return PIMHIP_OK;
     if (!k || !v) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "k and v must be non-null");
     if ((rc = check_rows("k", *k)) != PIMHIP_OK || (rc = check_rows("v", *v)) != PIMHIP_OK || (q && (rc = check_rows("q", *q)) != PIMHIP_OK)) return rc;
@@ -183,7 +184,7 @@ extern "C" int pimhip_paged_attend(const PimHipPagedCache* cache, const PimHipPa
     if (dtype != PIMHIP_F16 && dtype != PIMHIP_BF16) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "dtype=%d", dtype);
     if (cache->dtype != dtype && cache->dtype != PIMHIP_F8E4M3) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "a cache of type %d takes no queries of type %d", cache->dtype, dtype);
     if (q_heads < 1 || q_heads % a.c.kv_heads || q_heads > 65535) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "q_heads=%d with %d key heads", q_heads, a.c.kv_heads);
-    if (window < 0) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "window=%d", window);
+    if (window < 0 || !(scale - scale == 0.0f)) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "window=%d, scale=%g", window, (double)scale);
     AttendCut cut;
     if ((rc = cut_of(a.c, q_heads / a.c.kv_heads, st->num_cus, &cut)) != PIMHIP_OK) return rc;
     if (a.c.sequences == 0) return PIMHIP_OK;

@@ -8,8 +8,7 @@ using namespace pimhip;
 
 namespace
 {
-constexpr int kCountFrom = 4096;      // (smaller rows are soon looked at again)
-constexpr int kCountMost = 1 << 20;   // (segments' sums beside the counts: larger ones do not fit into LDS)
+constexpr int kCountFrom = 4096;  // (smaller rows are soon looked at again)
 }  // namespace
 
 extern "C" int pimhip_sample_tokens(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t vocab, const float* uniform, const PimHipSampleSettings* settings,
@@ -24,7 +23,7 @@ extern "C" int pimhip_sample_tokens(const void* logits, int dtype, int64_t ld, i
     if (!settings) return fail(PIMHIP_ERR_INVALID_ARGUMENT, "settings must be non-null");
     // 1024 threads for a row where there are CUs for all rows; where not, two blocks share one.  Values are counted where a row may need it (top_p of a
     // flat distribution, a large top_k), which takes a CU's LDS for one block.
-    const bool count = dtype != PIMHIP_F32 && vocab > kCountFrom && vocab <= kCountMost &&
+    const bool count = dtype != PIMHIP_F32 && vocab > kCountFrom &&
                        (settings->top_ks || settings->top_k <= 0 || settings->top_k > kListMost / 2) &&
                        (settings->top_ks || settings->top_ps || settings->top_p < 1.0f || settings->top_k > 0);
     const int threads = count ? 1024 : vocab <= 4096 ? 256 : rows > st->num_cus ? 512 : 1024;

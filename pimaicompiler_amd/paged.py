@@ -180,8 +180,8 @@ class PagedCache:
         heads = q.size(1)
         if q.size(0) != batch.sequences or heads < 1 or heads % self.kv_heads:
             raise NNRuntimeException(f"q must be [{batch.sequences}, a multiple of {self.kv_heads}, {self.head_dim}], got {tuple(q.shape)}")
-        if not isinstance(window, int) or not 0 <= window <= 2**31 - 1 or not math.isfinite(scale):
-            raise NNRuntimeException(f"window={window!r} must be a whole number from 0 on, scale={scale!r} finite")
+        if not isinstance(window, int) or not 0 <= window <= 2**31 - 1 or not isinstance(scale, (int, float)) or not abs(scale) < 3.4e38:
+            raise NNRuntimeException(f"window={window!r} must be a whole number from 0 on, scale={scale!r} a finite number")
         lib = L.load()
         with _Launch(self.device, stream, q, page_table, lengths, self.k_pages, self.v_pages, self.k_scale, self.v_scale) as handle:
             n = ctypes.c_uint64()

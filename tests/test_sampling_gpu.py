@@ -172,6 +172,38 @@ def test_temperatures_at_the_ends(ops):
         check(ops, x, u, temperature=t, top_p=0.9)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [20000, 5003])
+def test_exponents_out_of_range(ops, dtype, V):
+    """Largest values whose power of two no 64 bits hold: sums are made relative to them."""
+    x, u = logits(3, V, dtype, seed=V)
+    for shift, t in ((0, 1e-3), (0, 0.004), (400, 0.3), (-700, 0.5)):
+        for settings in ({}, {"top_p": 0.9}, {"top_k": 700, "top_p": 0.99}, {"min_p": 1e-3}, {"top_k": 20}):
+            check(ops, (x.float() + shift).to(dtype), u, temperature=t, **settings)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_more_equal_values_than_a_count_holds(ops, dtype):
+    """One value 100000 times in a row of 131072, or all of them: 16-bit counts pass their end."""
+    V = 131072
+    x = torch.full((2, V), 1.25)
+    x[1, ::5] = 2.0
+    x[1, 7::9] = -1.0
+    x = x.to(dtype)
+    for seed in range(2):
+        u = torch.rand(2, generator=torch.Generator().manual_seed(seed))
+        for settings in ({"top_p": 0.5}, {"top_k": 70000, "top_p": 0.75}, {"top_k": 3}, {"top_k": 1000}, {"min_p": 0.9}, {}):
+            check(ops, x, u, **settings)
+
+
+def test_many_rows(ops):
+    """Rows of which two share a CU, and short ones by the thousand."""
+    for rows, V, dtype in ((700, 9000, torch.float32), (3000, 300, torch.bfloat16), (600, 5000, torch.float16)):
+        x, u = logits(rows, V, dtype, seed=rows)
+        for settings in ({}, {"top_k": 30, "top_p": 0.9}, {"top_p": 0.8}):
+            check(ops, x, u, **settings)
+
+
 def test_shares(ops):
     """Evenly spread numbers draw each token as often as its share says, to one."""
     x, n = torch.tensor([0.5, 2.0, -1.0, 0.0, 1.0]), 4096
