@@ -18,7 +18,7 @@
 // Bound by w: 25 vector instructions a token, 13 us for the 64000 tokens a CU has of 512 rows of 32000 (fp32, nothing cut off: 29 us in all; the
 // bytes take 10).  256 rows of 131072 in bfloat16 whose nucleus holds half of them: 72 us, the counts 20 (LDS atomics), the last pass's w 33.  Reading
 // w out of a table in LDS there takes as long as working it out (30 us for 131072 gathers a CU).  64 rows of 100003 with settings of their own: 34;
-// one row of 32000 with top_k and top_p: 17, code that is run once and the dependent steps.
+// one row of 32000 with top_k and top_p: 14.6, code that is run once and the dependent steps.
 // Code is kept short, loops as loops: what one row takes is walked through once and comes cold out of the instruction cache.  (The same steps
 // unrolled, 117 to 177 KB a kernel, took 17 us for one row of 32000 and 69 for 256 of 131072.)
 #pragma once
@@ -76,6 +76,13 @@ __device__ __forceinline__ double exp2_f64(double d)
     return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, q) + n);
 }
 
+// log2 of m >= 1: the hardware's in 32 bits, off by some 1e-7, and what is left of m there.
+__device__ __forceinline__ double log2_f64(double m)
+{
+    const double y = (double)__builtin_amdgcn_logf((float)m);
+    return y + (m * exp2_f64(-y) - 1.0) * 1.4426950408889634;
+}
+
 struct SampleWeight {
     double top, rate, unit;  // largest value, log2(e) / T, 2^shift
     // exp((x - top) / T)
@@ -130,6 +137,7 @@ struct Piece {
 template <class T, int THREADS>
 struct SampleRow {
     typedef typename T::elem elem;
+    static constexpr bool kUnitsKept = THREADS == 1024;
     static constexpr int kWaves = THREADS / 64, kAhead = sizeof(elem) == 2 ? 4 : 2;  // (pieces on their way)
     // fp32 words of 16-bit values end in zeros (in their order, in zeros or ones): these bits tell no two of them apart.
     static constexpr int kDrop = __is_same(T, F16) ? 13 : __is_same(T, BF16) ? 16 : 0;
@@ -384,7 +392,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
     const bool unfit = !(temperature >= 0.0f && temperature < __builtin_inff()) || top_p != top_p || min_p != min_p || u != u;
     const bool greedy = unfit || temperature == 0.0f || top_k == 1 || top_p <= 0.0f;  // (the first of the largest is all that stays)
     const bool cut_k = top_k > 0 && top_k < V, cut_p = top_p < 1.0f, cut_m = min_p > 0.0f, cut = cut_k || cut_p || cut_m;
-    const double rate = 1.4426950408889634 / (double)temperature, unit = ldexp(1.0, a.shift), least_weight = cut_m ? fmin((double)min_p, 1.0) : 0.0;
+    const double rate = 1.4426950408889634 / (double)temperature, unit = ldexp(1.0, a.shift), per_unit = ldexp(1.0, -a.shift), least_weight = cut_m ? fmin((double)min_p, 1.0) : 0.0;
     const unsigned int bottom_key = Row::key_of(-__builtin_inff());
     SampleWeight weight{0.0, rate, unit};
     // What stays: values above `smallest`, and the first equal_kept of those equal to it (0: all), in the order of indices, up to `last`.
@@ -398,7 +406,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
     bool settled = false;            // what stays is known before any pass
     float least = __builtin_inff();  // what is to be listed: values from this on (inf: none)
     float bound = -__builtin_inff();  // nothing below this stays
-    auto log_share = [&](float v) { return (float)(((double)v - weight.top) / (double)temperature - log((double)whole / unit)); };
+    auto log_share = [&](float v) { return (float)((((double)v - weight.top) * rate - log2_f64((double)whole * per_unit)) * 0.6931471805599453); };
 
     // ---- 16-bit rows, value by value ----
     if constexpr (COUNT) {
@@ -712,7 +720,8 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
                 const uint64_t aim = sample_target(u, whole);
                 ahead = 0;
 #pragma unroll 1
-                for (int i = 0; i < count; ++i) {
+                for (unsigned long long left = __ballot(in); left; left &= left - 1) {
+                    const int i = __builtin_ctzll(left);
                     const uint64_t wi = readlane_u64(share, i);
                     if (__builtin_amdgcn_readlane(at, i) < at) ahead += wi;
                 }
@@ -723,7 +732,10 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
                 // ---- buckets: by keys first, for the order; then by indices, for the draw ----
                 constexpr int kEach = kListMost / THREADS, kPer = kBins / THREADS;
                 unsigned int* const counts = row.ties;                               // [kBins + 1]
-                unsigned short* const members = reinterpret_cast<unsigned short*>(counts + kBins + 1);  // [kListMost]: list entries, bucket by bucket
+                unsigned short* const members = reinterpret_cast<unsigned short*>(counts + kBins + 2);  // [kListMost]: list entries, bucket by bucket
+                // The tokens' weights: kept where a CU has one block, worked out again where LDS for them would cost blocks (4096 rows of 500: 98 us, with them 115).
+                uint64_t* const units = reinterpret_cast<uint64_t*>(members + kListMost);
+                auto units_of = [&](int i) { return Row::kUnitsKept ? units[i] : weight.units(weight(Row::value_in(sh.list[i]))); };
                 bool in[kEach];
                 unsigned int low = 0xffffffffu;
                 for (int i = tid; i < count; i += THREADS) low = (unsigned int)(sh.list[i] >> 32) < low ? (unsigned int)(sh.list[i] >> 32) : low;
@@ -742,11 +754,14 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
 #pragma unroll
                     for (int q = 0; q < kEach; ++q) {
                         const int i = q * THREADS + tid;
-                        if (!by_index) in[q] = i < count;
+                        if (!by_index) {
+                            in[q] = i < count;
+                            if (Row::kUnitsKept && in[q]) units[i] = weight.units(weight(Row::value_in(sh.list[i])));
+                        }
                         if (in[q]) {
                             const unsigned int b = bucket(sh.list[i]);
                             slot[q] = atomicAdd(&counts[b], 1u);
-                            row.add((int)b, weight.units(weight(Row::value_in(sh.list[i]))));
+                            row.add((int)b, units_of(i));
                         }
                     }
                     __syncthreads();
@@ -787,13 +802,14 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
                         rank[q] = (int)counts[b];
 #pragma unroll 1
                         for (unsigned int i = counts[b]; i < counts[b + 1]; ++i) {
-                            const unsigned long long o = sh.list[members[i]];
+                            const int member = members[i];
+                            const unsigned long long o = sh.list[member];
                             if (by_index ? (unsigned int)o > (unsigned int)entry : o > entry) {  // (lower halves are the indices' complements)
                                 ++rank[q];
-                                ahead[q] += weight.units(weight(Row::value_in(o)));
+                                ahead[q] += units_of(member);
                             }
                         }
-                        if (!by_index && !(cut_k && rank[q] >= top_k)) kept_sum += weight.units(weight(Row::value_in(entry)));
+                        if (!by_index && !(cut_k && rank[q] >= top_k)) kept_sum += units_of(q * THREADS + tid);
                     }
                     if (by_index) {
 #pragma unroll
@@ -801,7 +817,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
                             if (!in[q]) continue;
                             const unsigned long long entry = sh.list[q * THREADS + tid];
                             const float v = Row::value_in(entry);
-                            if (ahead[q] < aim && aim <= ahead[q] + weight.units(weight(v))) answer(Row::index_in(entry), log_share(v));
+                            if (ahead[q] < aim && aim <= ahead[q] + units_of(q * THREADS + tid)) answer(Row::index_in(entry), log_share(v));
                         }
                         return;
                     }
@@ -811,9 +827,9 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
 #pragma unroll
                     for (int q = 0; q < kEach; ++q) {
                         if (!in[q]) continue;
-                        const double w = weight(Row::value_in(sh.list[q * THREADS + tid]));
-                        in[q] = !(cut_k && rank[q] >= top_k) && (!cut_p || ahead[q] < target || rank[q] == 0) && w >= least_weight;
-                        if (in[q]) share += weight.units(w);
+                        in[q] = !(cut_k && rank[q] >= top_k) && (!cut_p || ahead[q] < target || rank[q] == 0);
+                        if (cut_m) in[q] = in[q] && weight(Row::value_in(sh.list[q * THREADS + tid])) >= least_weight;
+                        if (in[q]) share += units_of(q * THREADS + tid);
                     }
                     whole = row.scan(share).all;
                     aim = sample_target(u, whole);
@@ -865,7 +881,7 @@ template <class T, int THREADS, bool COUNT>
 inline unsigned int sample_shared_bytes(int V)
 {
     const int segments = (V + kSegment - 1) / kSegment, bins = segments > kBins ? segments : kBins;
-    const int own = V <= kTopsMost ? segments * (kSegment / 16) : segments > kSegment ? segments : kSegment, buckets = kBins + 1 + kListMost / 2;
+    const int own = V <= kTopsMost ? segments * (kSegment / 16) : segments > kSegment ? segments : kSegment, buckets = kBins + 2 + kListMost / 2 + (SampleRow<T, THREADS>::kUnitsKept ? kListMost * 2 : 0);
     const int words = COUNT ? kCountWords : own > buckets ? own : buckets;
     return (unsigned int)(sizeof(typename SampleRow<T, THREADS>::Shared) + bins * sizeof(uint64_t) + words * sizeof(unsigned int));
 }
