@@ -23,7 +23,7 @@ struct PagedView {
     const int* table;
     const int* lengths;
     int64_t ld_table;
-    int sequences, width;
+    int sequences;
     int most;  // tokens a row of the table has room for
     unsigned int magic;  // ceil(2^shift / page_size), shift = 31 + ceil(log2 page_size): n / page_size is n magic / 2^shift for n < 2^31
     int shift;
@@ -57,7 +57,7 @@ struct AppendArgs {
     const float* angles;
     int64_t k_token, k_head, v_token, v_head, q_token, q_head;  // elements from one to the next
     int64_t ld_angles;
-    int tokens, q_heads, half;  // half: pairs of a head that are turned
+    int q_heads, half;  // half: pairs of a head that are turned
     int items;                  // groups of eight of a token
 };
 
@@ -71,10 +71,10 @@ __device__ __forceinline__ const E* row_of(const AppendArgs& a, int t, int head)
                            : (const E*)a.q + t * a.q_token + (head - 2 * kv) * a.q_head;
 }
 
-// A block is heads of one token, a thread ITEMS groups of eight values of one: of a key (query) the eight that a rotation turns them with are loaded
-// beside them, out of the caches as a rule.  Values are asked for before the token's place is known, which takes three dependent loads: the
-// sequence, its length, the page.  Bound by the bytes where tokens are many (8001 of 32 query and 8 key heads of 128 in bfloat16: 8 groups a thread), else
-// by those loads.
+// A block is heads of one token, a thread ITEMS groups of eight values of it, all asked for at once: of a key (query) the eight that a rotation turns
+// them with beside them, out of the caches as a rule.  Values are asked for before the token's place is known, which takes three dependent loads: the
+// sequence, its length, the page.  Bound by the bytes where tokens are many (8001 of 32 query and 8 key heads of 128 in bfloat16, 199 MB: 48 us, 4.1 TB/s
+// where a copy has 4.8), else by those loads (one token: 4.2 us, a launch).
 template <class T, bool FP8, bool INTERLEAVED, int ITEMS>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
 {
@@ -187,11 +187,17 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
 //             operand as they are, unrounded, and V is one that 16 lanes read as one row: nothing is turned or exchanged.
 //             Where a key head has up to 4 query heads most of those 16 rows are empty: Q's columns repeat every 4 heads then, and the matrix
 //             instruction of 16 blocks [4 heads x 1 token] . [1 x 4 columns] takes a lane's e_j and its own value of V, a quarter of the time; the
-//             four groups of lanes have sums over tokens of their own, which are added at the end.  (Two of them for up to 8 heads need
-//             twice the registers: 1.6 GB in 299 us, with 16 rows 278.)
-// Values lie in registers from memory on; a tile's loads are issued while the one before is worked on.
+//             four groups of lanes have sums over tokens of their own, which are added at the end (8-bit caches, 160 sequences of 4000 to 8192
+//             tokens: 331 us, with 16 rows 361; 16-bit ones the same either way.  Two of them for up to 8 heads need twice the registers: 1.6 GB in
+//             299 us, with 16 rows 278).  More than 16 query heads of up to 128 values go 32 at a time, so that keys and values are read once (24 heads: 307 us, 16
+//             at a time 530).
+// Values lie in registers from memory on, in loads that pass the caches (1.07 GB: 182 us, through them 208); a tile's are issued while the one
+// before is worked on.  Registers are bounded for three wavefronts a SIMD (two with two tiles each on their way, or four: 1 to 3 % slower).
+// Bound by the bytes: 537 MB of one sequence of 131071 tokens 93 us (5.8 TB/s), 1.07 GB of 64 sequences 180 (6.0), 1.64 GB in 8 bits 273 (6.0), where a kernel that
+// only reads has 6.9.  From 16 query heads a key head on, the 32-bit products of 8-bit caches are as long as the loads (16 heads: 172 us, with 8 159).
+// Short calls take two launches and the dependent loads length, page, keys: 1000 tokens of one sequence 8 us.
 static constexpr int kUnit = 64;           // tokens that the four wavefronts of a block take together
-static constexpr float kLazy = 40.0f;      // a running maximum moves on when a score is above it by so many powers of two
+static constexpr float kLazy = 10.0f;      // a running maximum moves on when a score is above it by so many powers of two
 
 struct AttendArgs {
     PagedView c;
@@ -347,14 +353,13 @@ struct ValuePiece {
     }
 };
 
-// Wavefronts of a SIMD that the registers are bounded for, and tiles whose loads are in flight (below).
-constexpr int attend_waves(bool fp8, int nc, int ht) { return nc <= 2 && ht <= 16 ? 3 : 2; }
-constexpr int attend_depth(bool fp8, int nc, int ht) { return 1; }
+// Wavefronts of a SIMD that the registers are bounded for.
+constexpr int attend_waves(int nc, int ht) { return nc <= 2 && ht <= 16 ? 3 : 2; }
 
 // NC: the head's size in 64 columns, rounded up; HT: query heads at a time (4, 16 or 32); EVEN: pages are whole tiles of 16 tokens, and the head's size is NC of 64:
-// a tile's place is then the same for the wavefront, and no lane stays without loads.
+// a tile's place is then the same for the wavefront, and no lane stays without loads (8-bit caches: 138 us, as others 146; 16-bit ones 258 and 260).
 template <class T, bool FP8, int NC, int HT, bool EVEN>
-__global__ __launch_bounds__(256, attend_waves(FP8, NC, HT)) void paged_attend_kernel(AttendArgs a)
+__global__ __launch_bounds__(256, attend_waves(NC, HT)) void paged_attend_kernel(AttendArgs a)
 {
     typedef typename T::elem elem;
     typedef typename T::frag frag;
@@ -365,7 +370,6 @@ __global__ __launch_bounds__(256, attend_waves(FP8, NC, HT)) void paged_attend_k
     constexpr bool kFew = HT == 4;
     constexpr int kScores = kFew ? 1 : HT / 16;      // tiles of 16 heads
     constexpr int kParts = kFew ? 4 : 1;             // sums over tokens that a wavefront leaves of each head
-    constexpr int kDepth = attend_depth(FP8, NC, HT);
     __shared__ float wave_m[4][HT], wave_l[4][HT];
     __shared__ float parts[4][kParts * HT][NC * 64 + 4];
     const int lane = threadIdx.x & 63, wave = wave_in_block(), n = lane & 15, g = lane >> 4;
@@ -414,10 +418,10 @@ __global__ __launch_bounds__(256, attend_waves(FP8, NC, HT)) void paged_attend_k
         auto lane_of = [&](int r) { return kFew ? (lane & ~3) | r : g * 4 + r; };
 
         // ---- tiles: 16 tokens of each unit ----
-        uint4_t k[kDepth][kLoads];
-        ValuePiece<T, FP8, 8> wide[kDepth][4][kWide ? kWide : 1];
-        ValuePiece<T, FP8, 4> narrow[kDepth][4][kNarrow ? kNarrow : 1];
-        unsigned int page_ok[kDepth];  // a bit for each token of a tile
+        uint4_t k[kLoads];
+        ValuePiece<T, FP8, 8> wide[4][kWide ? kWide : 1];
+        ValuePiece<T, FP8, 4> narrow[4][kNarrow ? kNarrow : 1];
+        unsigned int page_ok = 0;  // a bit for each token of a tile
         // This wavefront's first token of a unit; a unit behind the stretch's end has none.
         auto token_of = [&](int unit) { return unit < last ? span.base + unit * kUnit + wave * 16 : span.end; };
         // Pages: a lane has that of one of the next 64 tiles (EVEN), or of a token of one of the next 4; the group after that is on its way.
@@ -430,7 +434,7 @@ __global__ __launch_bounds__(256, attend_waves(FP8, NC, HT)) void paged_attend_k
         // The loads of a unit's tile, in two parts: its place and keys, its values.  A page that is none is read as page 0, and not seen.
         int page = 0, in = 0;
         const unsigned int k_off = n * c.k_tok + g * 16, v_off = g * 4 * c.v_tok + n * (kWide ? 8 : 4) * kSize;
-        auto load_keys = [&](int j, int unit) {
+        auto load_keys = [&](int unit) {
             const int token = token_of(unit), i = (unit - first) & (kGroup - 1);
             if (i == 0 && unit != first) {
                 ids = ids_next;
@@ -439,58 +443,56 @@ __global__ __launch_bounds__(256, attend_waves(FP8, NC, HT)) void paged_attend_k
             if constexpr (EVEN) {
                 const int id = __builtin_amdgcn_readlane(ids, i);
                 const bool ok = id >= 0 && id < c.pages;
-                page_ok[j] = ok ? 0xffffu : 0u;
+                page_ok = ok ? 0xffffu : 0u;
                 page = ok ? id : 0;
                 in = token - c.page_of(token) * c.page_size;
                 const char* kp = kh + page * c.k_page + in * c.k_tok;
 #pragma unroll
-                for (int i = 0; i < kLoads; ++i) k[j][i] = load_global_once<uint4_any_t>(kp + k_off + i * 64);
+                for (int i = 0; i < kLoads; ++i) k[i] = load_global_once<uint4_any_t>(kp + k_off + i * 64);
             } else {
                 const int id = __shfl(ids, i * 16 + n);
                 const bool ok = id >= 0 && id < c.pages;
-                page_ok[j] = (unsigned int)__ballot(ok) & 0xffffu;
+                page_ok = (unsigned int)__ballot(ok) & 0xffffu;
                 page = ok ? id : 0;
                 in = token + n - c.page_of(token + n) * c.page_size;
                 const char* kp = kh + page * c.k_page + in * c.k_tok + g * 16;
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
-                    k[j][i] = uint4_t{0, 0, 0, 0};
-                    if (i * 64 + g * 16 < D * kSize) k[j][i] = load_global_once<uint4_any_t>(kp + i * 64);
+                    k[i] = uint4_t{0, 0, 0, 0};
+                    if (i * 64 + g * 16 < D * kSize) k[i] = load_global_once<uint4_any_t>(kp + i * 64);
                 }
             }
         };
-        auto load_values = [&](int j, int r) {
+        auto load_values = [&](int r) {
             if constexpr (EVEN) {
                 const char* vp = vh + page * c.v_page + (in + r) * c.v_tok;
 #pragma unroll
-                for (int i = 0; i < kWide; ++i) wide[j][r][i].load(vp + v_off + i * 128 * kSize);
-                if constexpr (kNarrow) narrow[j][r][0].load(vp + (kWide ? v_off - n * 4 * kSize + kWide * 128 * kSize : v_off));
+                for (int i = 0; i < kWide; ++i) wide[r][i].load(vp + v_off + i * 128 * kSize);
+                if constexpr (kNarrow) narrow[r][0].load(vp + (kWide ? v_off - n * 4 * kSize + kWide * 128 * kSize : v_off));
             } else {
                 const char* vp = vh + __shfl(page, g * 4 + r) * c.v_page + __shfl(in, g * 4 + r) * c.v_tok;
 #pragma unroll
                 for (int i = 0; i < kWide; ++i) {
-                    wide[j][r][i].clear();
-                    if (i * 128 + n * 8 < D) wide[j][r][i].load(vp + (i * 128 + n * 8) * kSize);
+                    wide[r][i].clear();
+                    if (i * 128 + n * 8 < D) wide[r][i].load(vp + (i * 128 + n * 8) * kSize);
                 }
                 if constexpr (kNarrow) {
-                    narrow[j][r][0].clear();
-                    if (kWide * 128 + n * 4 < D) narrow[j][r][0].load(vp + (kWide * 128 + n * 4) * kSize);
+                    narrow[r][0].clear();
+                    if (kWide * 128 + n * 4 < D) narrow[r][0].load(vp + (kWide * 128 + n * 4) * kSize);
                 }
             }
         };
+        if (token_of(first) < span.end) {
+            load_keys(first);
 #pragma unroll
-        for (int j = 0; j < kDepth; ++j)
-            if (token_of(first + j) < span.end) {
-                load_keys(j, first + j);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) load_values(j, r);
-            }
-        // A tile; `more`: the loads of the one kDepth behind it are issued as its registers become free.
-        auto tile = [&](auto more, int j, int unit) {
+            for (int r = 0; r < 4; ++r) load_values(r);
+        }
+        // A tile; `more`: the loads of the next one are issued as its registers become free.
+        auto tile = [&](auto more, int unit) {
             constexpr bool kMore = decltype(more)::value;
             const int token = token_of(unit);
             // Tokens that are not the sequence's, or not in the window, or of no page, are left out, whatever lies there.
-            unsigned int seen = page_ok[j];
+            unsigned int seen = page_ok;
             if (token < span.first) seen &= 0xffffu << (span.first - token);
             if (token + 16 > span.end) seen &= 0xffffu >> (token + 16 - span.end);
 
@@ -501,13 +503,13 @@ __global__ __launch_bounds__(256, attend_waves(FP8, NC, HT)) void paged_attend_k
             for (int i = 0; i < kSteps; ++i) {
                 frag kf;
                 if constexpr (FP8)
-                    kf = from_e4m3x8<T>(i % 2 ? uint2_t{k[j][i / 2][2], k[j][i / 2][3]} : uint2_t{k[j][i / 2][0], k[j][i / 2][1]});
+                    kf = from_e4m3x8<T>(i % 2 ? uint2_t{k[i / 2][2], k[i / 2][3]} : uint2_t{k[i / 2][0], k[i / 2][1]});
                 else
-                    kf = __builtin_bit_cast(frag, k[j][i]);
+                    kf = __builtin_bit_cast(frag, k[i]);
 #pragma unroll
                 for (int mt = 0; mt < kScores; ++mt) sc[mt] = T::mfma(kf, q[mt][i], sc[mt]);
             }
-            if constexpr (kMore) load_keys(j, unit + kDepth);
+            if constexpr (kMore) load_keys(unit + 1);
 #pragma unroll
             for (int mt = 0; mt < kScores; ++mt) sc[mt] *= scale;
             if (seen != 0xffffu) {
@@ -517,8 +519,8 @@ __global__ __launch_bounds__(256, attend_waves(FP8, NC, HT)) void paged_attend_k
 #pragma unroll
                     for (int mt = 0; mt < kScores; ++mt) sc[mt][r] = -__builtin_inff();
 #pragma unroll
-                    for (int i = 0; i < kWide; ++i) wide[j][r][i].clear();
-                    if constexpr (kNarrow) narrow[j][r][0].clear();
+                    for (int i = 0; i < kWide; ++i) wide[r][i].clear();
+                    if constexpr (kNarrow) narrow[r][0].clear();
                 }
             }
             bool above = false;
@@ -563,30 +565,16 @@ __global__ __launch_bounds__(256, attend_waves(FP8, NC, HT)) void paged_attend_k
 #pragma unroll
                 for (int i = 0; i < kWide; ++i)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) add(i * 8 + e, wide[j][r][i].value(e));
+                    for (int e = 0; e < 8; ++e) add(i * 8 + e, wide[r][i].value(e));
                 if constexpr (kNarrow)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) add(kWide * 8 + e, narrow[j][r][0].value(e));
-                if constexpr (kMore) load_values(j, r);
+                    for (int e = 0; e < 4; ++e) add(kWide * 8 + e, narrow[r][0].value(e));
+                if constexpr (kMore) load_values(r);
             }
         };
         int unit = first;
-        for (; token_of(unit + 2 * kDepth - 1) < span.end; unit += kDepth) {
-#pragma unroll
-            for (int j = 0; j < kDepth; ++j) tile(std::true_type{}, j, unit + j);
-        }
-        // (2 kDepth - 1 tiles at most are left, the first kDepth of them loaded)
-#pragma unroll
-        for (int j = 0; j < kDepth - 1; ++j)
-            if (token_of(unit + kDepth + j) < span.end) {
-                tile(std::true_type{}, j, unit + j);
-            } else if (token_of(unit + j) < span.end) {
-                tile(std::false_type{}, j, unit + j);
-            }
-        if (token_of(unit + kDepth - 1) < span.end) tile(std::false_type{}, kDepth - 1, unit + kDepth - 1);
-#pragma unroll
-        for (int j = 0; j < kDepth - 1; ++j)
-            if (token_of(unit + kDepth + j) < span.end) tile(std::false_type{}, j, unit + kDepth + j);
+        for (; token_of(unit + 1) < span.end; ++unit) tile(std::true_type{}, unit);
+        if (token_of(unit) < span.end) tile(std::false_type{}, unit);
 
         // ---- the four wavefronts' parts, joined by all of the block ----
         const int rows = a.group - head0 < HT ? a.group - head0 : HT;

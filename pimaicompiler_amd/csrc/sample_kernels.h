@@ -16,9 +16,9 @@
 // 64 bits takes a wavefront 5.4 clocks, one of 32 bits 4.4): with fp32's 2^-24 a number between two tokens of a large vocabulary would fall
 // on the wrong one in some percent of the rows.
 // Bound by w: 25 vector instructions a token, 13 us for the 64000 tokens a CU has of 512 rows of 32000 (fp32, nothing cut off: 29 us in all; the
-// bytes take 10).  256 rows of 131072 in bfloat16 whose nucleus holds half of them: 72 us, the counts 20 (LDS atomics), the last pass's w 33.  Reading
-// w out of a table in LDS there takes as long as working it out (30 us for 131072 gathers a CU).  64 rows of 100003 with settings of their own: 34;
-// one row of 32000 with top_k and top_p: 14.6, code that is run once and the dependent steps.
+// bytes take 10).  256 rows of 131072 in bfloat16 whose nucleus holds half of them: 73 us, the counts 20 (LDS atomics), the last pass's w 33.  Reading
+// w out of a table in LDS there takes as long as working it out (30 us for 131072 gathers a CU).  64 rows of 100003 with settings of their own: 32;
+// one row of 32000 with top_k and top_p: 14.4, code that is run once and the dependent steps.
 // Code is kept short, loops as loops: what one row takes is walked through once and comes cold out of the instruction cache.  (The same steps
 // unrolled, 117 to 177 KB a kernel, took 17 us for one row of 32000 and 69 for 256 of 131072.)
 #pragma once
@@ -375,7 +375,7 @@ template <class T, int THREADS, bool COUNT>
 __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
 {
     typedef SampleRow<T, THREADS> Row;
-    constexpr int kWaves = THREADS / 64, kNamed = kBins * 2;
+    constexpr int kNamed = kBins * 2;
     extern __shared__ __align__(16) char shared[];  // sample_shared_bytes()
     typename Row::Shared& sh = *reinterpret_cast<typename Row::Shared*>(shared);
     const int64_t r = blockIdx.x;
@@ -504,10 +504,9 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
     // Passes over the row: the first, one that sums what top_k leaves, the last one with the segments' sums of what stays.
     enum { kFirst, kSum, kLast };
     int phase = settled ? kLast : kFirst;
-    bool listed = !settled;  // whether there has been no need of a list, or no room for it
     while (true) {
         const bool first = phase == kFirst;
-        if (!(settled && !listed && least < __builtin_inff())) {
+        if (!(settled && least < __builtin_inff())) {
             if (phase == kLast && weight(smallest) < least_weight) {
                 // min_p comes down to a smallest value too: the lowest key of a weight that stays.
                 unsigned int out = Row::key_of(smallest), in = top_key;
@@ -693,7 +692,6 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
             const int count = sh.count;
             bound = least;
             least = __builtin_inff();
-            listed = true;
             if (count <= 64) {
                 // ---- one wavefront, a lane each token ----
                 if (wave != 0) return;
@@ -835,7 +833,6 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
                     aim = sample_target(u, whole);
                 }
             }
-            if (settled) continue;  // (what stays was known to fit: not reached)
         }
 
         // ---- the row in place of the list: the smallest value that stays ----
@@ -852,7 +849,6 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
             smallest = Row::value_of(key);
         }
         phase = !by_weight && cut_p ? kSum : kLast;
-
     }
 
     // ---- the draw: the segment, then the value in it, one each thread ----

@@ -204,6 +204,36 @@ def test_many_rows(ops):
             check(ops, x, u, **settings)
 
 
+@pytest.mark.parametrize("rows, V", [(2, 24576), (2, 24577), (3, 32769), (257, 49152), (257, 49153), (513, 20000), (520, 33000)])
+def test_rows_of_each_length_and_number(ops, rows, V):
+    """What a row is worked out with depends on how long rows are and how many of them there are."""
+    x, u = logits(rows, V, torch.bfloat16, seed=rows)
+    some = torch.arange(0, rows, 1 + rows // 8)
+    for settings in ({}, {"top_k": 40}, {"top_p": 0.9}, {"top_p": 0.6, "temperature": 0.3, "min_p": 0.01}, {"top_k": 2000, "top_p": 0.97}):
+        tokens, logp = ops.sample_tokens(x.to(DEV), u.to(DEV), **settings)
+        got = ops.sample_tokens(x[some].to(DEV), u[some].to(DEV), **settings)   # (few rows: other threads, the same tokens)
+        assert torch.equal(tokens[some], got[0]) and bool(((logp[some] - got[1]).abs() <= logp[some].abs() * 2.0**-23 + 1e-9).all())
+        check(ops, x[some], u[some], **settings)
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2])
+def test_long_rows_at_the_ends(ops, dtype):
+    """Rows that are counted: largest values out of range, no distribution, settings of their own."""
+    V = 30001
+    x, u = logits(8, V, dtype, seed=3)
+    for shift, t in ((0, 1e-3), (400, 0.3), (-700, 0.5)):
+        for settings in ({"top_p": 0.9}, {"top_k": 700, "top_p": 0.99}, {"top_k": 5000, "min_p": 1e-3}):
+            check(ops, (x.float() + shift).to(dtype), u, temperature=t, **settings)
+    x[0, 5], x[1, V - 1] = NAN, INF
+    x[2] = -INF
+    x[3], x[3, 77] = -INF, 2.0
+    x[4, ::2] = -INF
+    u[5], u[6] = NAN, 7.0
+    for settings in ({"top_p": 0.9}, {"top_k": 20000}, {"top_k": 20000, "top_p": 0.5}):
+        check(ops, x, u, **settings)
+    check(ops, x, u, top_k=torch.tensor([0, 900, 40, 0, 29000, 1, 600, 513]).int(), top_p=torch.tensor([0.9, 0.5, 0.9, 0.3, 0.999, 1.0, 1.0, 0.9]), temperature=0.8)
+
+
 def test_shares(ops):
     """Evenly spread numbers draw each token as often as its share says, to one."""
     x, n = torch.tensor([0.5, 2.0, -1.0, 0.0, 1.0]), 4096
