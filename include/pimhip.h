@@ -671,7 +671,11 @@ typedef struct PimHipSampleSettings {
  * A row with a NaN or +inf, of a temperature that is negative, infinite or NaN, or of a NaN elsewhere in its settings or its number: token -1 and
  * logp NaN; a row of -inf alone: -1 and -inf.  A number outside of [0, 1) is taken as the nearest in it. */
 int pimhip_sample_tokens(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t vocab, const float* uniform, const PimHipSampleSettings* settings,
-                         int64_t* tokens, float* logp, void* stream);
+                         int64_t* tokens, float* logp, void* workspace, void* stream);
+
+/* The bytes of device memory (aligned to 16) that pimhip_sample_tokens takes as its workspace for these rows and settings on the current device, 0 for many
+ * calls (workspace may be NULL then): few long rows, whose first pass all CUs share.  Two calls that may run at the same time need one each. */
+int pimhip_sample_workspace_bytes(int dtype, int64_t rows, int64_t vocab, const PimHipSampleSettings* settings, uint64_t* bytes);
 
 #ifdef __cplusplus
 }

@@ -157,7 +157,8 @@ SIGNATURES = {
     "pimhip_paged_attend": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(PagedBatch), ctypes.POINTER(PagedRows), ctypes.c_int, ctypes.c_int, ctypes.c_float,
                                            ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "pimhip_sample_tokens": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
-                                            ctypes.POINTER(SampleSettings), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+                                            ctypes.POINTER(SampleSettings), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "pimhip_sample_workspace_bytes": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.POINTER(SampleSettings), ctypes.POINTER(ctypes.c_uint64)]),
     "pimhip_mx4_matmul": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, c_mx4_p, c_mx4_p, ctypes.c_void_p]),
 }
 

@@ -635,9 +635,7 @@ template <class V>
 bool settingOf(PyObject* o, const at::Tensor& logits, at::ScalarType type, V most, const V*& each, V& one)
 {
     if (THPVariable_Check(o)) {
-        const at::Tensor* t;
-        if (!THPVariable_Check(o)) return false;
-        t = &THPVariable_Unpack(o);
+        const at::Tensor* t = &THPVariable_Unpack(o);
         if (!t->defined() || t->scalar_type() != type || t->device() != logits.device() || t->sizes() != logits.sizes().slice(0, logits.dim() - 1) || !t->is_contiguous() ||
             (t->requires_grad() && at::GradMode::is_enabled()) || (type == at::kFloat && t->_fw_grad(0).defined()))
             return false;
@@ -682,12 +680,15 @@ PyObject* sampleTokens(PyObject*, PyObject* const* args, Py_ssize_t n)
     if (!settingOf<float>(args[2], *x, at::kFloat, largest, s.temperatures, s.temperature) || !settingOf<int>(args[3], *x, at::kInt, INT32_MAX, s.top_ks, s.top_k) ||
         !settingOf<float>(args[4], *x, at::kFloat, 1.0f, s.top_ps, s.top_p) || !settingOf<float>(args[5], *x, at::kFloat, 1.0f, s.min_ps, s.min_p))
         return none();
-    at::Tensor tokens = newTensor(lead, at::kLong, x->device()), logp = newTensor(lead, at::kFloat, x->device());
-    int rc;
+    uint64_t bytes = 0;
+    int rc = pimhip_sample_workspace_bytes(typeCode(x->scalar_type()), rows, cols, &s, &bytes);
+    if (rc != PIMHIP_OK) return status(rc);
+    at::Tensor tokens = newTensor(lead, at::kLong, x->device()), logp = newTensor(lead, at::kFloat, x->device()), workspace;
+    if (bytes) workspace = newTensor({(int64_t)bytes}, at::kByte, x->device());
     void* stream = currentStream();
     Py_BEGIN_ALLOW_THREADS
     rc = pimhip_sample_tokens(x->data_ptr(), typeCode(x->scalar_type()), ld, rows, cols, static_cast<const float*>(u.data_ptr()), &s,
-                              static_cast<int64_t*>(tokens.data_ptr()), static_cast<float*>(logp.data_ptr()), stream);
+                              static_cast<int64_t*>(tokens.data_ptr()), static_cast<float*>(logp.data_ptr()), bytes ? workspace.data_ptr() : nullptr, stream);
     Py_END_ALLOW_THREADS
     if (rc != PIMHIP_OK) return status(rc);
     PyObject* out = PyTuple_New(2);

@@ -4,7 +4,8 @@
 //   less than top_p of their sum has been reached; of them those with w >= min_p.  The token is the first in the order of indices at which
 //   the running sum over what stayed exceeds u times the whole.
 //
-// One block a row.  The first pass finds the largest value and, where the sum over all tokens is asked for, that too.  What may stay is
+// One block a row.  The first pass (few long rows: a launch of its own, by all CUs) finds the largest value and, where the sum over all tokens is asked
+// for, that too.  What may stay is
 // above a bound that this pass gives (top_k: the k-th largest of the threads' own largest values; top_p: tokens below (1 - top_p) / V of the sum
 // cannot be among those that reach top_p of it, since all of them together do not have the rest; min_p: its own), and goes to a list
 // in LDS, whose order is worked out there: up to 64 tokens by one wavefront, more of them by buckets.
@@ -15,10 +16,10 @@
 // Sums that are made in any order are whole numbers of 64 bits, w in units of 2^-shift of the largest.  w itself is worked out in 64 bits (an fma of
 // 64 bits takes a wavefront 5.4 clocks, one of 32 bits 4.4): with fp32's 2^-24 a number between two tokens of a large vocabulary would fall
 // on the wrong one in some percent of the rows.
-// Bound by w: 25 vector instructions a token, 13 us for the 64000 tokens a CU has of 512 rows of 32000 (fp32, nothing cut off: 29 us in all; the
-// bytes take 10).  256 rows of 131072 in bfloat16 whose nucleus holds half of them: 73 us, the counts 20 (LDS atomics), the last pass's w 33.  Reading
-// w out of a table in LDS there takes as long as working it out (30 us for 131072 gathers a CU).  64 rows of 100003 with settings of their own: 32;
-// one row of 32000 with top_k and top_p: 14.4, code that is run once and the dependent steps.
+// Bound by w: 25 vector instructions a token, 13 us for the 64000 tokens a CU has of 512 rows of 32000 (fp32, nothing cut off: 30 us in all; the
+// bytes take 10).  256 rows of 131072 in bfloat16 whose nucleus holds half of them: 76 us, the counts 20 (LDS atomics), the last pass's w 33.  Reading
+// w out of a table in LDS there takes as long as working it out (30 us for 131072 gathers a CU).  64 rows of 100003 with settings of their own: 31;
+// one row of 32000 with top_k and top_p: 14.4, of 131072 with top_k 20.4, code that is run once and the dependent steps.
 // Code is kept short, loops as loops: what one row takes is walked through once and comes cold out of the instruction cache.  (The same steps
 // unrolled, 117 to 177 KB a kernel, took 17 us for one row of 32000 and 69 for 256 of 131072.)
 #pragma once
@@ -47,6 +48,11 @@ struct SampleArgs {
     int64_t* tokens;
     float* logp;
     int64_t ld;
+    // What sample_parts_kernel leaves of each row, or null:
+    unsigned long long* part_best;  // [rows, segments]: the largest value of each, and the complement of its piece's index; all ones: one that has no distribution
+    double* part_sums;              // [rows, segments]: where the row's first pass has sums
+    unsigned short* part_tops;      // [rows, ld_tops]: the upper half of each piece's largest value, in its order
+    int64_t ld_tops;
     int V, shift;  // shift: a weight of 1 is 2^shift, and V of them fit into 62 bits
     float temperature, top_p, min_p;
     int top_k;
@@ -82,6 +88,29 @@ __device__ __forceinline__ double log2_f64(double m)
     const double y = (double)__builtin_amdgcn_logf((float)m);
     return y + (m * exp2_f64(-y) - 1.0) * 1.4426950408889634;
 }
+
+// What is asked of a row.
+struct SampleAsked {
+    float temperature, top_p, min_p, u;
+    int top_k;
+    bool unfit, greedy, cut_k, cut_p, cut_m, sums;  // greedy: the first of the largest is all that stays; sums: the first pass makes them
+    double rate;                                    // log2(e) / T
+    __device__ __forceinline__ SampleAsked(const SampleArgs& a, int64_t r)
+    {
+        temperature = a.temperatures ? a.temperatures[r] : a.temperature;
+        top_p = a.top_ps ? a.top_ps[r] : a.top_p;
+        min_p = a.min_ps ? a.min_ps[r] : a.min_p;
+        u = a.uniform[r];
+        top_k = a.top_ks ? a.top_ks[r] : a.top_k;
+        unfit = !(temperature >= 0.0f && temperature < __builtin_inff()) || top_p != top_p || min_p != min_p || u != u;
+        greedy = unfit || temperature == 0.0f || top_k == 1 || top_p <= 0.0f;
+        cut_k = top_k > 0 && top_k < a.V;
+        cut_p = top_p < 1.0f;
+        cut_m = min_p > 0.0f;
+        sums = !greedy && !cut_k && (cut_p || !cut_m);
+        rate = 1.4426950408889634 / (double)temperature;
+    }
+};
 
 struct SampleWeight {
     double top, rate, unit;  // largest value, log2(e) / T, 2^shift
@@ -135,35 +164,11 @@ struct Piece {
 };
 
 template <class T, int THREADS>
-struct SampleRow {
+struct SampleTokens {
     typedef typename T::elem elem;
-    static constexpr bool kUnitsKept = THREADS == 1024;
     static constexpr int kWaves = THREADS / 64, kAhead = sizeof(elem) == 2 ? 4 : 2;  // (pieces on their way)
-    // fp32 words of 16-bit values end in zeros (in their order, in zeros or ones): these bits tell no two of them apart.
-    static constexpr int kDrop = __is_same(T, F16) ? 13 : __is_same(T, BF16) ? 16 : 0;
-    struct Shared {
-        unsigned long long list[kListMost];  // keys, and the complements of indices below them
-        uint64_t waves[kWaves];
-        unsigned long long best[kWaves];
-        uint64_t chunk_sums[32], chunk_counts[32];
-        uint64_t found_before, found_amount;
-        int found, count, named, bad;
-    };
     const elem* x;
     int V;
-    Shared& sh;
-    uint64_t* bins;        // kBins of them, or one for each segment where those are more
-    unsigned int* ties;    // one for each segment, or for each value of one; the counts, or the pieces' largest values, lie there too
-
-    static __device__ __forceinline__ unsigned int key_of(float v) { return ordered_bits(v) >> kDrop; }
-    static __device__ __forceinline__ float value_of(unsigned int key)
-    {
-        const unsigned int o = key << kDrop;  // (a negative value's dropped bits are ones)
-        return from_ordered(o & 0x80000000u ? o : o | ((1u << kDrop) - 1u));
-    }
-    static __device__ __forceinline__ unsigned long long entry_of(unsigned int key, int at) { return (unsigned long long)key << 32 | (unsigned int)~(unsigned int)at; }
-    static __device__ __forceinline__ float value_in(unsigned long long entry) { return value_of((unsigned int)(entry >> 32)); }
-    static __device__ __forceinline__ int index_in(unsigned long long entry) { return (int)~(unsigned int)entry; }
 
     // The piece of values 8 p .. 8 p + 7 and the index of its first; the row's last piece is the last eight values, those of the piece before it -inf.
     __device__ __forceinline__ int piece(int p, Piece<T>& v) const
@@ -182,13 +187,13 @@ struct SampleRow {
         return at;
     }
     // f(number of a piece, index of its first value, the piece) for the pieces of a lane, then after(segment) behind each segment of a wavefront (four
-    // pieces of each lane).
+    // pieces of each lane), from the wavefront's first on, `step` from one to the next.
     template <class F, class G>
-    __device__ __forceinline__ void each_segment(F f, G after) const
+    __device__ __forceinline__ void each_segment(F f, G after, int from, int step) const
     {
         const int pieces = (V + 7) / 8, segments = (V + kSegment - 1) / kSegment, lane = threadIdx.x & 63;
 #pragma unroll 1
-        for (int segment = wave_in_block(); segment < segments; segment += kWaves) {
+        for (int segment = from; segment < segments; segment += step) {
             Piece<T> v[kAhead];
             const int p0 = segment * (kSegment / 8) + lane;
             auto load = [&](int i, int p) {
@@ -210,6 +215,50 @@ struct SampleRow {
             }
             after(segment);
         }
+    }
+    template <class F, class G>
+    __device__ __forceinline__ void each_segment(F f, G after) const
+    {
+        each_segment(f, after, wave_in_block(), kWaves);
+    }
+};
+
+template <class T, int THREADS>
+struct SampleRow : SampleTokens<T, THREADS> {
+    typedef typename T::elem elem;
+    typedef SampleTokens<T, THREADS> Tokens;
+    using Tokens::kWaves;
+    using Tokens::x;
+    using Tokens::V;
+    using Tokens::each_segment;
+    static constexpr bool kUnitsKept = THREADS == 1024;
+    // fp32 words of 16-bit values end in zeros (in their order, in zeros or ones): these bits tell no two of them apart.
+    static constexpr int kDrop = __is_same(T, F16) ? 13 : __is_same(T, BF16) ? 16 : 0;
+    struct Shared {
+        unsigned long long list[kListMost];  // keys, and the complements of indices below them
+        uint64_t waves[kWaves];
+        unsigned long long best[kWaves];
+        uint64_t chunk_sums[32], chunk_counts[32];
+        uint64_t found_before, found_amount;
+        int found, count, named, bad;
+    };
+    Shared& sh;
+    uint64_t* bins;        // kBins of them, or one for each segment where those are more
+    unsigned int* ties;    // one for each segment, or for each value of one; the counts, or the pieces' largest values, lie there too
+
+    static __device__ __forceinline__ unsigned int key_of(float v) { return ordered_bits(v) >> kDrop; }
+    static __device__ __forceinline__ float value_of(unsigned int key)
+    {
+        const unsigned int o = key << kDrop;  // (a negative value's dropped bits are ones)
+        return from_ordered(o & 0x80000000u ? o : o | ((1u << kDrop) - 1u));
+    }
+    static __device__ __forceinline__ unsigned long long entry_of(unsigned int key, int at) { return (unsigned long long)key << 32 | (unsigned int)~(unsigned int)at; }
+    static __device__ __forceinline__ float value_in(unsigned long long entry) { return value_of((unsigned int)(entry >> 32)); }
+    static __device__ __forceinline__ int index_in(unsigned long long entry) { return (int)~(unsigned int)entry; }
+
+    __device__ __forceinline__ SampleRow(const elem* row, int tokens, Shared& shared, uint64_t* bins_at, unsigned int* ties_at)
+        : Tokens{row, tokens}, sh(shared), bins(bins_at), ties(ties_at)
+    {
     }
 
     // The sum of the threads' numbers in front of this one's, and of all.
@@ -371,28 +420,66 @@ struct SampleRow {
     }
 };
 
-template <class T, int THREADS, bool COUNT>
+// The first pass over rows of which there are fewer than CUs, by all of them: a wavefront a segment.
+template <class T>
+__global__ __launch_bounds__(256) void sample_parts_kernel(SampleArgs a)
+{
+    const int64_t r = blockIdx.y;
+    const int segments = (a.V + kSegment - 1) / kSegment, segment = (int)blockIdx.x * 4 + wave_in_block();
+    const SampleTokens<T, 256> row{(const typename T::elem*)a.logits + r * a.ld, a.V};
+    const SampleAsked asked(a, r);
+    unsigned long long best = 0;
+    bool bad = false;
+    double sum = 0.0;
+    row.each_segment(
+        [&](int p, int at, const Piece<T>& v) {
+            float top = v.value(0);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                top = fmaxf(top, v.value(c));
+                bad |= !(v.value(c) < __builtin_inff());
+            }
+            const unsigned int o = ordered_bits(top);
+            a.part_tops[r * a.ld_tops + p] = (unsigned short)(o >> 16);
+            const unsigned long long entry = (unsigned long long)o << 32 | (unsigned int)~(unsigned int)at;
+            best = entry > best ? entry : best;
+            if (asked.sums) {
+                double e[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) e[c] = exp2_f64((double)v.value(c) * asked.rate);
+                sum += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+            }
+        },
+        [&](int at) {
+            best = __ballot(bad) ? ~0ull : wave_max_u64(best);
+            if (asked.sums) sum = wave_total_f64(sum);
+            if ((threadIdx.x & 63) != 0) return;
+            a.part_best[r * segments + at] = best;
+            if (asked.sums) a.part_sums[r * segments + at] = sum;
+        },
+        segment, segments);
+}
+
+// PARTS: sample_parts_kernel has made the first pass.
+template <class T, int THREADS, bool COUNT, bool PARTS>
 __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
 {
     typedef SampleRow<T, THREADS> Row;
-    constexpr int kNamed = kBins * 2;
     extern __shared__ __align__(16) char shared[];  // sample_shared_bytes()
     typename Row::Shared& sh = *reinterpret_cast<typename Row::Shared*>(shared);
     const int64_t r = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_in_block(), V = a.V, segments = (V + kSegment - 1) / kSegment;
     uint64_t* const bins = reinterpret_cast<uint64_t*>(shared + sizeof(typename Row::Shared));
-    const Row row{(const typename T::elem*)a.logits + r * a.ld, V, sh, bins, reinterpret_cast<unsigned int*>(bins + (segments > kBins ? segments : kBins))};
-    const float temperature = a.temperatures ? a.temperatures[r] : a.temperature, top_p = a.top_ps ? a.top_ps[r] : a.top_p;
-    const float min_p = a.min_ps ? a.min_ps[r] : a.min_p, u = a.uniform[r];
-    const int top_k = a.top_ks ? a.top_ks[r] : a.top_k;
+    const Row row((const typename T::elem*)a.logits + r * a.ld, V, sh, bins, reinterpret_cast<unsigned int*>(bins + (segments > kBins ? segments : kBins)));
+    const SampleAsked asked(a, r);
+    const float temperature = asked.temperature, top_p = asked.top_p, u = asked.u;
+    const int top_k = asked.top_k;
     auto answer = [&](int64_t token, float logp) {
         a.tokens[r] = token;
         a.logp[r] = logp;
     };
-    const bool unfit = !(temperature >= 0.0f && temperature < __builtin_inff()) || top_p != top_p || min_p != min_p || u != u;
-    const bool greedy = unfit || temperature == 0.0f || top_k == 1 || top_p <= 0.0f;  // (the first of the largest is all that stays)
-    const bool cut_k = top_k > 0 && top_k < V, cut_p = top_p < 1.0f, cut_m = min_p > 0.0f, cut = cut_k || cut_p || cut_m;
-    const double rate = 1.4426950408889634 / (double)temperature, unit = ldexp(1.0, a.shift), per_unit = ldexp(1.0, -a.shift), least_weight = cut_m ? fmin((double)min_p, 1.0) : 0.0;
+    const bool unfit = asked.unfit, greedy = asked.greedy, cut_k = asked.cut_k, cut_p = asked.cut_p, cut_m = asked.cut_m, cut = cut_k || cut_p || cut_m;
+    const double rate = asked.rate, unit = ldexp(1.0, a.shift), per_unit = ldexp(1.0, -a.shift), least_weight = cut_m ? fmin((double)asked.min_p, 1.0) : 0.0;
     const unsigned int bottom_key = Row::key_of(-__builtin_inff());
     SampleWeight weight{0.0, rate, unit};
     // What stays: values above `smallest`, and the first equal_kept of those equal to it (0: all), in the order of indices, up to `last`.
@@ -408,103 +495,123 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
     float bound = -__builtin_inff();  // nothing below this stays
     auto log_share = [&](float v) { return (float)((((double)v - weight.top) * rate - log2_f64((double)whole * per_unit)) * 0.6931471805599453); };
 
-    // ---- 16-bit rows, value by value ----
-    if constexpr (COUNT) {
-        if (!greedy && (cut_k ? top_k > kListMost / 2 : cut_p)) {
-            static_assert(THREADS == 1024, "a chunk of places is a word for each thread");
-            row.count_all();
-            unsigned int high = 0, low = 0xffffu, n = 0;
-#pragma unroll 1
-            for (int i = 0; i < 32; ++i) {
-                const unsigned int two = row.ties[i * 1024 + tid], place = (unsigned int)(i * 1024 + tid) * 2;
-                n += (two & 0xffffu) + (two >> 16);
-                if (two != 0) {
-                    high = place + (two >> 16 ? 1 : 0);
-                    low = low != 0xffffu ? low : place + (two & 0xffffu ? 0 : 1);
-                }
-            }
-            const uint64_t counted = row.scan(n).all;
-            high = (unsigned int)row.largest(high);
-            low = 0xffffu - (unsigned int)row.largest(0xffffu - low);
-            constexpr unsigned int kInf = __is_same(T, F16) ? 0x7c00u : 0x7f80u;
-            if (counted == (uint64_t)V) {  // (else a count has passed 65535: the row is taken as others are)
-                if (high >= (0x8000u | kInf) || low < (0x7fffu & ~kInf)) {
-                    if (tid == 0) answer(-1, __builtin_nanf(""));
-                    return;
-                }
-                if (high == (0x7fffu & ~kInf)) {
-                    if (tid == 0) answer(-1, -__builtin_inff());
-                    return;
-                }
-                weight.top = (double)Row::value_at(high);
-                top_key = Row::key_of(Row::value_at(high));
-                auto mass = [&](unsigned int place) { return weight.units(weight(Row::value_at(place))); };
-                if (tid < 32) sh.chunk_sums[tid] = sh.chunk_counts[tid] = 0;
-                __syncthreads();
-#pragma unroll 1
-                for (int i = (int)(high >> 11); i >= (int)(low >> 11); --i) {
-                    const unsigned int two = row.ties[i * 1024 + tid];
-                    if (!__ballot(two != 0)) continue;
-                    uint64_t part = 0;
-#pragma unroll 1
-                    for (int h = 0; h < 2; ++h) {
-                        const unsigned int count = h ? two >> 16 : two & 0xffffu;
-                        if (count) part += count * mass((unsigned int)(i * 1024 + tid) * 2 + h);
-                    }
-                    part = wave_total_u64(part);
-                    const unsigned int some = wave_total_u32((two & 0xffffu) + (two >> 16));
-                    if (lane == 0) {
-                        atomicAdd((unsigned long long*)&sh.chunk_sums[i], (unsigned long long)part);
-                        atomicAdd((unsigned long long*)&sh.chunk_counts[i], (unsigned long long)some);
-                    }
-                }
-                __syncthreads();
-                // First by counts (top_k), then by weights (top_p); behind each, what the places from the one found on have.
-                unsigned int place = 0;
-                uint64_t above, some = 0;
-#pragma unroll 1
-                for (int by_weight = 0; by_weight < 2; ++by_weight) {
-                    if (by_weight ? !cut_p : !cut_k) continue;
-                    if (by_weight && !cut_k) row_whole = wave_total_u64(lane < 32 ? sh.chunk_sums[lane] : 0);
-                    const uint64_t target = by_weight ? nucleus_target(top_p, row_whole) : (uint64_t)top_k;
-                    const unsigned int found = row.select_counted(by_weight ? sh.chunk_sums : sh.chunk_counts, target, weight, by_weight, above, amount);
-                    const uint64_t one = by_weight ? mass(found) : 1, all = amount / one, wanted = target > above ? (target - above + one - 1) / one : 1;
-                    const uint64_t limit = found == place && equal_kept ? equal_kept : all;
-                    equal_kept = wanted < limit ? wanted : limit;
-                    if (!by_weight) row_whole = equal_kept * mass(found);
-                    if (equal_kept == all) equal_kept = 0;
-                    place = found;
-                    uint64_t sum = tid < 32 && tid > (int)(place >> 11) ? sh.chunk_sums[tid] : 0;
-                    some = tid < 32 && tid > (int)(place >> 11) ? sh.chunk_counts[tid] : 0;
-#pragma unroll 1
-                    for (unsigned int at = (place & ~2047u) + tid; at < (place | 2047u) + 1; at += THREADS) {
-                        const unsigned int count = at >= place ? row.count_at(at) : 0;
-                        some += count;
-                        if (count && !by_weight && at > place) sum += count * mass(at);
-                    }
-                    some = row.scan(some).all;
-                    if (!by_weight) row_whole += row.scan(sum).all;
-                }
-                smallest = Row::value_at(place);
-                const double exponent = weight.top * rate;
-                relative = fabs(exponent) > kExponents;
-                to_units = relative ? unit : exp2_f64(-exponent) * unit;
-                settled = true;
-                if (some <= kListMost) least = smallest;
-            }
-            __syncthreads();
-        }
-    }
-    if (tid == 0) sh.bad = sh.count = sh.named = 0;
-    __syncthreads();
-
     // The pieces' largest values, as the upper halves of their keys, where they are looked at again.
     unsigned short* const tops = reinterpret_cast<unsigned short*>(row.ties);
     double* const sums_of = reinterpret_cast<double*>(bins);
+    // f(piece, the upper half of its largest value) of what sample_parts_kernel has left, eight next to each other at a time.
+    auto each_top = [&](auto f) {
+        const int pieces = (V + 7) / 8;
+#pragma unroll 1
+        for (int p = tid * 8; p < pieces; p += THREADS * 8) {
+            const uint4_t q = *reinterpret_cast<const uint4_t*>(a.part_tops + r * a.ld_tops + p);
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                if (p + c < pieces) f(p + c, q[c / 2] >> c % 2 * 16 & 0xffffu);
+        }
+    };
     // Passes over the row: the first, one that sums what top_k leaves, the last one with the segments' sums of what stays.
     enum { kFirst, kSum, kLast };
-    int phase = settled ? kLast : kFirst;
+    int phase = kFirst;
+    // ---- 16-bit rows, value by value: what stays is settled, as long as no count passes its end.  Whether the row has an answer already (no distribution) ----
+    bool counts = COUNT && !greedy && (cut_k ? top_k > kListMost / 2 : cut_p);
+    auto count_row = [&]() -> bool {
+        counts = false;
+        static_assert(!COUNT || THREADS == 1024, "a chunk of places is a word for each thread");
+        row.count_all();
+        unsigned int high = 0, low = 0xffffu, n = 0;
+#pragma unroll 1
+        for (int i = 0; i < 32; ++i) {
+            const unsigned int two = row.ties[i * 1024 + tid], place = (unsigned int)(i * 1024 + tid) * 2;
+            n += (two & 0xffffu) + (two >> 16);
+            if (two != 0) {
+                high = place + (two >> 16 ? 1 : 0);
+                low = low != 0xffffu ? low : place + (two & 0xffffu ? 0 : 1);
+            }
+        }
+        const uint64_t counted = row.scan(n).all;
+        high = (unsigned int)row.largest(high);
+        low = 0xffffu - (unsigned int)row.largest(0xffffu - low);
+        constexpr unsigned int kInf = __is_same(T, F16) ? 0x7c00u : 0x7f80u;
+        if (counted == (uint64_t)V) {  // (else a count has passed 65535: the row is taken as others are)
+            if (high >= (0x8000u | kInf) || low < (0x7fffu & ~kInf)) {
+                if (tid == 0) answer(-1, __builtin_nanf(""));
+                return true;
+            }
+            if (high == (0x7fffu & ~kInf)) {
+                if (tid == 0) answer(-1, -__builtin_inff());
+                return true;
+            }
+            weight.top = (double)Row::value_at(high);
+            top_key = Row::key_of(Row::value_at(high));
+            auto mass = [&](unsigned int place) { return weight.units(weight(Row::value_at(place))); };
+            if (tid < 32) sh.chunk_sums[tid] = sh.chunk_counts[tid] = 0;
+            __syncthreads();
+#pragma unroll 1
+            for (int i = (int)(high >> 11); i >= (int)(low >> 11); --i) {
+                const unsigned int two = row.ties[i * 1024 + tid];
+                if (!__ballot(two != 0)) continue;
+                uint64_t part = 0;
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                    const unsigned int count = h ? two >> 16 : two & 0xffffu;
+                    if (count) part += count * mass((unsigned int)(i * 1024 + tid) * 2 + h);
+                }
+                part = wave_total_u64(part);
+                const unsigned int some = wave_total_u32((two & 0xffffu) + (two >> 16));
+                if (lane == 0) {
+                    atomicAdd((unsigned long long*)&sh.chunk_sums[i], (unsigned long long)part);
+                    atomicAdd((unsigned long long*)&sh.chunk_counts[i], (unsigned long long)some);
+                }
+            }
+            __syncthreads();
+            // First by counts (top_k), then by weights (top_p); behind each, what the places from the one found on have.
+            unsigned int place = 0;
+            uint64_t above, some = 0;
+#pragma unroll 1
+            for (int by_weight = 0; by_weight < 2; ++by_weight) {
+                if (by_weight ? !cut_p : !cut_k) continue;
+                if (by_weight && !cut_k) row_whole = wave_total_u64(lane < 32 ? sh.chunk_sums[lane] : 0);
+                const uint64_t target = by_weight ? nucleus_target(top_p, row_whole) : (uint64_t)top_k;
+                const unsigned int found = row.select_counted(by_weight ? sh.chunk_sums : sh.chunk_counts, target, weight, by_weight, above, amount);
+                const uint64_t one = by_weight ? mass(found) : 1, all = amount / one, wanted = target > above ? (target - above + one - 1) / one : 1;
+                const uint64_t limit = found == place && equal_kept ? equal_kept : all;
+                equal_kept = wanted < limit ? wanted : limit;
+                if (!by_weight) row_whole = equal_kept * mass(found);
+                if (equal_kept == all) equal_kept = 0;
+                place = found;
+                uint64_t sum = tid < 32 && tid > (int)(place >> 11) ? sh.chunk_sums[tid] : 0;
+                some = tid < 32 && tid > (int)(place >> 11) ? sh.chunk_counts[tid] : 0;
+#pragma unroll 1
+                for (unsigned int at = (place & ~2047u) + tid; at < (place | 2047u) + 1; at += THREADS) {
+                    const unsigned int count = at >= place ? row.count_at(at) : 0;
+                    some += count;
+                    if (count && !by_weight && at > place) sum += count * mass(at);
+                }
+                some = row.scan(some).all;
+                if (!by_weight) row_whole += row.scan(sum).all;
+            }
+            smallest = Row::value_at(place);
+            const double exponent = weight.top * rate;
+            relative = fabs(exponent) > kExponents;
+            to_units = relative ? unit : exp2_f64(-exponent) * unit;
+            settled = true;
+            phase = kLast;
+            if (some <= kListMost) least = smallest;
+        }
+        __syncthreads();
+        return false;
+    };
+    if constexpr (COUNT && !PARTS) {
+        if (counts && count_row()) return;
+    }
+    bool count_now = counts && cut_k;  // (PARTS: where the sum over all tokens is there already, a list is tried first)
     while (true) {
+        if constexpr (COUNT && PARTS) {
+            if (count_now && count_row()) return;
+            count_now = false;
+        }
+        if (tid == 0) sh.bad = sh.count = sh.named = 0;
+        __syncthreads();
         const bool first = phase == kFirst;
         if (!(settled && least < __builtin_inff())) {
             if (phase == kLast && weight(smallest) < least_weight) {
@@ -518,7 +625,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
                 equal_kept = 0;
             }
             // ---- a pass ----
-            const bool sums = !first || (!greedy && !cut_k && (cut_p || !cut_m)), tops_kept = first && !greedy && cut && V <= kTopsMost;
+            const bool sums = !first || asked.sums, given = PARTS && first, tops_kept = !greedy && cut && V <= kTopsMost;
             const bool strict = equal_kept != 0;
             // Values from `limit` on are summed: those above `smallest`, or from it on.  Exponents are those of x rate in the first pass and where that
             // keeps to 64 bits' range; else relative to the largest value, fp32's differences being exact for what is near it.
@@ -527,8 +634,17 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
             float my_top = -__builtin_inff();
             bool bad = false;
             double sum = 0.0;
-            unsigned int equal = 0;
-            row.each_segment(
+            unsigned int equal = 0, my_key = 0;
+            if (given) {
+                for (int i = tid; i < segments; i += THREADS) {
+                    const unsigned long long one = a.part_best[r * segments + i];
+                    bad |= one == ~0ull;
+                    best = one > best ? one : best;
+                    if (sums) sums_of[i] = a.part_sums[r * segments + i];
+                }
+                each_top([&](int, unsigned int top) { my_key = top > my_key ? top : my_key; });
+                my_key = (unsigned int)((uint64_t)my_key << 16 >> Row::kDrop);  // (lower than its value's by what the upper half leaves out)
+            } else row.each_segment(
                 [&](int p, int at, const Piece<T>& v) {
                     if (first) {
                         float top = v.value(0);
@@ -571,7 +687,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
                 });
             __syncthreads();
             if (first) {
-                const unsigned int my_key = best ? Row::key_of(my_top) : 0u;
+                if (!given) my_key = best ? Row::key_of(my_top) : 0u;
                 if (bad) sh.bad = 1;
                 best = row.largest(best);
                 const float top = from_ordered((unsigned int)(best >> 32));
@@ -664,30 +780,35 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
                     if (i < kListMost) sh.list[i] = Row::entry_of(Row::key_of((float)row.x[at_hit]), at_hit);
                 }
             };
-            int named = kNamed + 1;
-            if (first && V <= kTopsMost) {
+            if (first && (PARTS || V <= kTopsMost)) {
                 unsigned int* names = reinterpret_cast<unsigned int*>(bins);
-                const unsigned short from = (unsigned short)(ordered_bits(least) >> 16);
+                const unsigned int from = ordered_bits(least) >> 16;
                 const int pieces = (V + 7) / 8;
+                auto name = [&](int p, unsigned int top) {
+                    if (top < from) return;
+                    const int i = atomicAdd(&sh.named, 1);
+                    if (i < kListMost) names[i] = (unsigned int)p;
+                };
                 __syncthreads();
+                if (PARTS)
+                    each_top(name);
+                else
 #pragma unroll 1
-                for (int p = tid; p < pieces; p += THREADS)
-                    if (tops[p] >= from) {
-                        const int i = atomicAdd(&sh.named, 1);
-                        if (i < kNamed) names[i] = (unsigned int)p;
-                    }
+                    for (int p = tid; p < pieces; p += THREADS) name(p, tops[p]);
                 __syncthreads();
-                named = sh.named;
-                if (named <= kNamed)
+                // (of more pieces than the list is long none is looked at: it would not hold what they have)
+                const int named = sh.named;
+                if (named > kListMost && tid == 0) sh.count = named;
+                if (named <= kListMost)
 #pragma unroll 1
                     for (int i = tid; i < named; i += THREADS) {
                         Piece<T> v;
                         const int at = row.piece((int)names[i], v);
                         take(at, v);
                     }
-            }
-            if (named > kNamed)
+            } else {
                 row.each_segment([&](int, int at, const Piece<T>& v) { take(at, v); }, [](int) {});
+            }
             __syncthreads();
             const int count = sh.count;
             bound = least;
@@ -836,6 +957,10 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
         }
 
         // ---- the row in place of the list: the smallest value that stays ----
+        if (PARTS && counts) {
+            count_now = true;
+            continue;
+        }
         const bool by_weight = !(first && cut_k);
         if (by_weight ? cut_p : true) {
             const uint64_t target = by_weight ? nucleus_target(top_p, row_whole) : (uint64_t)top_k;

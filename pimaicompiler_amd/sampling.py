@@ -26,9 +26,9 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     the whole.  temperature 0: the most likely token.
 
     temperature, top_p and min_p are numbers or fp32 tensors [..], top_k a whole number or an int32 tensor [..].  Weights are worked out and summed in
-    64 bits (shares are good to 2^-36, and one that meets a border to within that is taken to meet it), and equal calls give equal results.  A row of -inf alone gives token -1 and logp -inf; one with a NaN or +inf -1 and NaN, and so does a
-    tensor's temperature that is negative, infinite or NaN, or a NaN in its other settings or its number.  Numbers outside of [0, 1) count as the
-    nearest in it."""
+    64 bits (shares are good to 2^-36, and one that meets a border to within that is taken to meet it), and equal calls give equal results.
+    A row of -inf alone gives token -1 and logp -inf; one with a NaN or +inf -1 and NaN, and so does a tensor's temperature that is negative,
+    infinite or NaN, or a NaN in its other settings or its number.  Numbers outside of [0, 1) count as the nearest in it."""
     out = _native().fast_sample_tokens(logits, uniform, temperature, top_k, top_p, min_p) if stream is None else None
     if out is not None:
         return _result(out)
@@ -66,6 +66,9 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
             setattr(settings, name, v.data_ptr())
         tokens = torch.empty(lead, dtype=torch.int64, device=logits.device)
         logp = torch.empty(lead, dtype=torch.float32, device=logits.device)
-        _check(L.load().pimhip_sample_tokens(x.data_ptr(), _CODES[x.dtype], ld, x.size(0), V, uniform.data_ptr(), ctypes.byref(settings), tokens.data_ptr(),
-                                             logp.data_ptr(), handle))
+        lib, n = L.load(), ctypes.c_uint64()
+        _check(lib.pimhip_sample_workspace_bytes(_CODES[x.dtype], x.size(0), V, ctypes.byref(settings), ctypes.byref(n)))
+        workspace = torch.empty(n.value, dtype=torch.uint8, device=logits.device) if n.value else None
+        _check(lib.pimhip_sample_tokens(x.data_ptr(), _CODES[x.dtype], ld, x.size(0), V, uniform.data_ptr(), ctypes.byref(settings), tokens.data_ptr(),
+                                        logp.data_ptr(), workspace.data_ptr() if workspace is not None else None, handle))
     return tokens, logp

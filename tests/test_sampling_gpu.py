@@ -216,10 +216,54 @@ def test_rows_of_each_length_and_number(ops, rows, V):
         check(ops, x[some], u[some], **settings)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, V", [(1, 49152), (1, 49153), (64, 49153), (65, 60000), (3, 131072), (128, 131080), (129, 131073), (2, 300007)])
+def test_few_long_rows(ops, rows, V, dtype):
+    """The first pass by all CUs for few rows: as each row by itself and as more of them."""
+    x, u = logits(rows, V, dtype, seed=rows + V)
+    some = torch.arange(0, rows, 1 + rows // 2)
+    for settings in ({}, {"temperature": 0.0}, {"top_k": 40}, {"top_k": 900, "min_p": 1e-3}, {"top_p": 0.9}, {"top_p": 0.6, "temperature": 0.3}, {"top_k": 3000, "top_p": 0.97}, {"min_p": 0.05}):
+        tokens, logp = ops.sample_tokens(x.to(DEV), u.to(DEV), **settings)
+        got = ops.sample_tokens(x[some].to(DEV).repeat(300, 1), u[some].to(DEV).repeat(300), **settings)
+        got = got[0].view(300, -1), got[1].view(300, -1)
+        assert bool((got[0] == tokens[some]).all()) and bool(((got[1] - logp[some]).abs() <= logp[some].abs() * 2.0**-23 + 1e-9).all())
+        if V < 2**17:
+            check(ops, x[some], u[some], **settings)
+
+
+def test_workspaces(ops):
+    """A call that needs a workspace is refused without one; each call of two has its own."""
+    import ctypes
+
+    from pimaicompiler_amd import _lib as L
+    x, u = torch.randn(2, 60000, device=DEV), torch.rand(2, device=DEV)
+    tokens, logp, n = torch.full((2,), -7, device=DEV), torch.zeros(2, device=DEV), ctypes.c_uint64()
+    settings = L.SampleSettings(temperature=1.0, top_k=5, top_p=1.0)
+    lib = L.load()
+    assert lib.pimhip_sample_workspace_bytes(L.PIMHIP_F32, 2, 60000, ctypes.byref(settings), ctypes.byref(n)) == L.PIMHIP_OK and n.value > 0
+    call = [x.data_ptr(), L.PIMHIP_F32, 60000, 2, 60000, u.data_ptr(), ctypes.byref(settings), tokens.data_ptr(), logp.data_ptr()]
+    workspace = torch.empty(n.value + 16, dtype=torch.uint8, device=DEV)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.pimhip_sample_tokens(*call, None, stream) == L.PIMHIP_ERR_INVALID_ARGUMENT
+    assert lib.pimhip_sample_tokens(*call, workspace.data_ptr() + 8, stream) == L.PIMHIP_ERR_INVALID_ARGUMENT
+    assert tokens.tolist() == [-7, -7]
+    assert lib.pimhip_sample_tokens(*call, workspace.data_ptr(), stream) == L.PIMHIP_OK
+    assert torch.equal(tokens, ops.sample_tokens(x, u, top_k=5)[0])
+    assert lib.pimhip_sample_workspace_bytes(L.PIMHIP_F32, 2, 1000, ctypes.byref(settings), ctypes.byref(n)) == L.PIMHIP_OK and n.value == 0
+    assert lib.pimhip_sample_workspace_bytes(L.PIMHIP_F32, 2, 1000, ctypes.byref(settings), None) == L.PIMHIP_ERR_INVALID_ARGUMENT
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    want = [ops.sample_tokens(v, u, top_p=0.5) for v in (x, -x)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = [ops.sample_tokens(v, u, top_p=0.5, stream=s) for v, s in zip((x, -x), streams)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("V", [30001, 60001])
 @pytest.mark.parametrize("dtype", DTYPES[:2])
-def test_long_rows_at_the_ends(ops, dtype):
+def test_long_rows_at_the_ends(ops, dtype, V):
     """Rows that are counted: largest values out of range, no distribution, settings of their own."""
-    V = 30001
     x, u = logits(8, V, dtype, seed=3)
     for shift, t in ((0, 1e-3), (400, 0.3), (-700, 0.5)):
         for settings in ({"top_p": 0.9}, {"top_k": 700, "top_p": 0.99}, {"top_k": 5000, "min_p": 1e-3}):
