@@ -16,10 +16,10 @@
 // Sums that are made in any order are whole numbers of 64 bits, w in units of 2^-shift of the largest.  w itself is worked out in 64 bits (an fma of
 // 64 bits takes a wavefront 5.4 clocks, one of 32 bits 4.4): with fp32's 2^-24 a number between two tokens of a large vocabulary would fall
 // on the wrong one in some percent of the rows.
-// Bound by w: 25 vector instructions a token, 13 us for the 64000 tokens a CU has of 512 rows of 32000 (fp32, nothing cut off: 30 us in all; the
-// bytes take 10).  256 rows of 131072 in bfloat16 whose nucleus holds half of them: 76 us, the counts 20 (LDS atomics), the last pass's w 33.  Reading
-// w out of a table in LDS there takes as long as working it out (30 us for 131072 gathers a CU).  64 rows of 100003 with settings of their own: 31;
-// one row of 32000 with top_k and top_p: 14.4, of 131072 with top_k 20.4, code that is run once and the dependent steps.
+// Bound by w: 25 vector instructions a token, 13 us for the 64000 tokens a CU has of 512 rows of 32000 (fp32, nothing cut off: 27 us in all; the
+// bytes take 10).  256 rows of 131072 in bfloat16 whose nucleus holds half of them: 73 us, the counts 20 (LDS atomics), the last pass's w 33.  Reading
+// w out of a table in LDS there takes as long as working it out (30 us for 131072 gathers a CU).  64 rows of 100003 with settings of their own: 29;
+// one row of 32000 with top_k and top_p: 13.4, of 131072 with top_k 19, code that is run once and the dependent steps.
 // Code is kept short, loops as loops: what one row takes is walked through once and comes cold out of the instruction cache.  (The same steps
 // unrolled, 117 to 177 KB a kernel, took 17 us for one row of 32000 and 69 for 256 of 131072.)
 #pragma once
@@ -138,6 +138,15 @@ __device__ __forceinline__ uint64_t nucleus_target(float top_p, uint64_t whole)
     return t < 1 ? 1 : t;
 }
 
+// The thread's number, asked for anew: what is made of it is made where it is used, not at the kernel's start and kept in registers (24 to 53 of them spilled
+// so, 25 to 87 MB written by a call: 512 rows of 32000 30.4 us, now 26.7).
+__device__ __forceinline__ int this_thread()
+{
+    int t = (int)threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+
 // Eight values as they lie in memory.
 template <class T>
 struct Piece {
@@ -191,7 +200,7 @@ struct SampleTokens {
     template <class F, class G>
     __device__ __forceinline__ void each_segment(F f, G after, int from, int step) const
     {
-        const int pieces = (V + 7) / 8, segments = (V + kSegment - 1) / kSegment, lane = threadIdx.x & 63;
+        const int pieces = (V + 7) / 8, segments = (V + kSegment - 1) / kSegment, lane = this_thread() & 63;
 #pragma unroll 1
         for (int segment = from; segment < segments; segment += step) {
             Piece<T> v[kAhead];
@@ -268,21 +277,22 @@ struct SampleRow : SampleTokens<T, THREADS> {
     __device__ __forceinline__ Scan scan(uint64_t mine) const
     {
         const uint64_t incl = wave_scan_u64(mine);
+        const int lane = this_thread() & 63, wave = wave_in_block();
         __syncthreads();
-        if ((threadIdx.x & 63) == 63) sh.waves[threadIdx.x >> 6] = incl;
+        if (lane == 63) sh.waves[wave] = incl;
         __syncthreads();
-        const int lane = threadIdx.x & 63, wave = wave_in_block();
         const uint64_t waves = wave_scan_u64(lane < kWaves ? sh.waves[lane] : 0);
         return Scan{incl - mine + (wave ? readlane_u64(waves, wave - 1) : 0), readlane_u64(waves, 63)};
     }
     // The largest of the threads' numbers.
     __device__ __forceinline__ unsigned long long largest(unsigned long long mine) const
     {
+        const int lane = this_thread() & 63;
         mine = wave_max_u64(mine);
         __syncthreads();
-        if ((threadIdx.x & 63) == 0) sh.best[threadIdx.x >> 6] = mine;
+        if (lane == 0) sh.best[wave_in_block()] = mine;
         __syncthreads();
-        return wave_max_u64(((int)threadIdx.x & 63) < kWaves ? sh.best[threadIdx.x & 63] : 0ull);
+        return wave_max_u64(lane < kWaves ? sh.best[lane] : 0ull);
     }
 
     // The first of a[0 .. n) at whose end base + the running sum reaches `target` (that of all, where it is never reached); the sum before it
@@ -291,7 +301,7 @@ struct SampleRow : SampleTokens<T, THREADS> {
     __device__ __forceinline__ int find(const A* a, int n, uint64_t base, uint64_t target, uint64_t& before, uint64_t& amount) const
     {
         __syncthreads();
-        const int per = (n + THREADS - 1) / THREADS, lo = threadIdx.x * per < n ? threadIdx.x * per : n, hi = lo + per < n ? lo + per : n;
+        const int tid = this_thread(), per = (n + THREADS - 1) / THREADS, lo = tid * per < n ? tid * per : n, hi = lo + per < n ? lo + per : n;
         uint64_t mine = 0;
 #pragma unroll 1
         for (int i = lo; i < hi; ++i) mine += a[i];
@@ -316,7 +326,7 @@ struct SampleRow : SampleTokens<T, THREADS> {
     {
         __syncthreads();
 #pragma unroll 1
-        for (int i = threadIdx.x; i < kBins; i += THREADS) bins[i] = 0;
+        for (int i = this_thread(); i < kBins; i += THREADS) bins[i] = 0;
         __syncthreads();
     }
     __device__ __forceinline__ void add(int bin, uint64_t amount) const { atomicAdd((unsigned long long*)&bins[bin], (unsigned long long)amount); }
@@ -385,7 +395,7 @@ struct SampleRow : SampleTokens<T, THREADS> {
     {
         const uint4_t zero = {0, 0, 0, 0};
 #pragma unroll 1
-        for (int i = threadIdx.x; i < kCountWords / 4; i += THREADS) reinterpret_cast<uint4_t*>(ties)[i] = zero;
+        for (int i = this_thread(); i < kCountWords / 4; i += THREADS) reinterpret_cast<uint4_t*>(ties)[i] = zero;
         __syncthreads();
         auto count = [&](unsigned int u) {
             const unsigned int place = place_of(u);
@@ -404,14 +414,14 @@ struct SampleRow : SampleTokens<T, THREADS> {
     __device__ __forceinline__ unsigned int select_counted(const uint64_t* sums, uint64_t target, const SampleWeight& weight, bool by_weight, uint64_t& above,
                                                            uint64_t& amount) const
     {
-        const int lane = threadIdx.x & 63;
+        const int lane = this_thread() & 63;
         const uint64_t mine = lane < 32 ? sums[31 - lane] : 0, incl = wave_scan_u64(mine), all = readlane_u64(incl, 63);
         if (target > all) target = all;
         const int at = __builtin_ctzll(__ballot(incl >= target)), chunk = 31 - at;  // (lane 31 has reached it)
         above = readlane_u64(incl - mine, at);
         __syncthreads();
 #pragma unroll 1
-        for (int i = threadIdx.x; i < kBins; i += THREADS) {
+        for (int i = this_thread(); i < kBins; i += THREADS) {
             const unsigned int place = (unsigned int)(chunk * 2048 + 2047 - i), n = count_at(place);
             bins[i] = n == 0 ? 0 : by_weight ? n * weight.units(weight(value_at(place))) : n;
         }
@@ -468,7 +478,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
     extern __shared__ __align__(16) char shared[];  // sample_shared_bytes()
     typename Row::Shared& sh = *reinterpret_cast<typename Row::Shared*>(shared);
     const int64_t r = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 63, wave = wave_in_block(), V = a.V, segments = (V + kSegment - 1) / kSegment;
+    const int tid = threadIdx.x, lane = tid & 63, V = a.V, segments = (V + kSegment - 1) / kSegment;
     uint64_t* const bins = reinterpret_cast<uint64_t*>(shared + sizeof(typename Row::Shared));
     const Row row((const typename T::elem*)a.logits + r * a.ld, V, sh, bins, reinterpret_cast<unsigned int*>(bins + (segments > kBins ? segments : kBins)));
     const SampleAsked asked(a, r);
@@ -500,7 +510,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
     double* const sums_of = reinterpret_cast<double*>(bins);
     // f(piece, the upper half of its largest value) of what sample_parts_kernel has left, eight next to each other at a time.
     auto each_top = [&](auto f) {
-        const int pieces = (V + 7) / 8;
+        const int tid = this_thread(), pieces = (V + 7) / 8;
 #pragma unroll 1
         for (int p = tid * 8; p < pieces; p += THREADS * 8) {
             const uint4_t q = *reinterpret_cast<const uint4_t*>(a.part_tops + r * a.ld_tops + p);
@@ -515,6 +525,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
     // ---- 16-bit rows, value by value: what stays is settled, as long as no count passes its end.  Whether the row has an answer already (no distribution) ----
     bool counts = COUNT && !greedy && (cut_k ? top_k > kListMost / 2 : cut_p);
     auto count_row = [&]() -> bool {
+        const int tid = this_thread();
         counts = false;
         static_assert(!COUNT || THREADS == 1024, "a chunk of places is a word for each thread");
         row.count_all();
@@ -625,6 +636,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
                 equal_kept = 0;
             }
             // ---- a pass ----
+            const int tid = this_thread(), lane = tid & 63;
             const bool sums = !first || asked.sums, given = PARTS && first, tops_kept = !greedy && cut && V <= kTopsMost;
             const bool strict = equal_kept != 0;
             // Values from `limit` on are summed: those above `smallest`, or from it on.  Exponents are those of x rate in the first pass and where that
@@ -767,6 +779,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
 
         if (least < __builtin_inff()) {
             // ---- the list: from the pieces whose largest value reaches the bound, or from all ----
+            const int tid = this_thread();
             auto take = [&](int at, const Piece<T>& v) {
                 unsigned int hits = 0;
 #pragma unroll
@@ -815,7 +828,8 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
             least = __builtin_inff();
             if (count <= 64) {
                 // ---- one wavefront, a lane each token ----
-                if (wave != 0) return;
+                if (wave_in_block() != 0) return;
+                const int lane = this_thread() & 63;
                 const unsigned long long entry = lane < count ? sh.list[lane] : 0ull;
                 const float v = Row::value_in(entry);
                 const int at = Row::index_in(entry);
@@ -862,6 +876,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
                 uint64_t aim = 0;
 #pragma unroll 1
                 for (int by_index = 0; by_index < 2; ++by_index) {
+                    const int tid = this_thread();
                     int s = 0;
                     const unsigned int range = by_index ? (unsigned int)V - 1 : top_key - low;
                     while (range >> s >= (unsigned int)kBins) ++s;
@@ -982,7 +997,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
     const uint64_t in_front = before;
     __syncthreads();
 #pragma unroll 1
-    for (int i = tid; i < kSegment; i += THREADS) {
+    for (int i = this_thread(); i < kSegment; i += THREADS) {
         const int at = segment * kSegment + i;
         uint64_t units = 0;
         if (at < V) {
