@@ -606,7 +606,8 @@ typedef struct PimHipPagedCache {
 } PimHipPagedCache;
 
 /* page_table [sequences, table_width] (pitch ld_table) and lengths [sequences]: tokens of each sequence, those of this call among them.  A row's
- * entries behind its sequence's last page may be anything; a page outside of the cache is none: its tokens are not stored and not seen. */
+ * entries behind its sequence's last page may be anything; a page outside of the cache is none: its tokens are not stored and not seen,
+ * nor are those of a sequence from table_width * page_size on. */
 typedef struct PimHipPagedBatch {
     const int* page_table;
     const int* lengths;
@@ -639,7 +640,8 @@ int pimhip_paged_attend_workspace_bytes(const PimHipPagedCache* cache, const Pim
 /* out[s, h] = softmax over the tokens j of sequence s of (scale * q[s, h] . k[j, h'])  times  v[j, h'], h' = h / (q_heads / kv_heads): attention of one new
  * token of each sequence, q and out [sequences, q_heads, head_dim] (out dense).  window > 0: the last `window` tokens only.  lse [sequences, q_heads] or
  * NULL: the logarithm of the sum of the softmax's exponentials.  Sums, statistics and the weights of the values are fp32, out is rounded once.  A
- * sequence without tokens: zeros, lse -inf.  What lies in places that are not seen, NaN included, has no influence.
+ * sequence without tokens: zeros, lse -inf.  What lies in places that are not seen, NaN included, has no influence.  Weights are up to 2^10 before their
+ * sum divides them: values above 2^118 / tokens may overflow.
  * Allocates and synchronises nothing.  The workspace is the call's until it has run: calls that may overlap, and captured graphs that are replayed
  * at the same time, need one each. */
 int pimhip_paged_attend(const PimHipPagedCache* cache, const PimHipPagedBatch* batch, const PimHipPagedRows* q, int q_heads, int dtype, float scale,

@@ -48,7 +48,7 @@ class PagedCache:
 
     Common to both calls: page_table [sequences, width] int32, a sequence's pages in order, and lengths [sequences] int32, its tokens, those of the
     current step among them.  Entries of the table behind a sequence's last page may be anything; a page outside of the cache is none: its
-    tokens are not stored and not seen."""
+    tokens are not stored and not seen, nor are those of a sequence that its row of the table has no room for."""
 
     def __init__(self, k_pages, v_pages, k_scale=None, v_scale=None):
         for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
@@ -120,7 +120,7 @@ class PagedCache:
         None: one token for each sequence.  A sequence of length 0, or shorter than its tokens, has none at the positions below 0.
         rotary [width * page_size or more, n] fp32 (rotary_table): the first n values of each key are turned in pairs by the token's
         position, in fp32, values i and n / 2 + i, or 2 i and 2 i + 1 if interleaved; so are those of q [tokens, heads, head_dim], the queries
-        of the same tokens, which are returned (zeros for a token that is nobody's).  Without q the result is None.
+        of the same tokens, which are returned (zeros for a token that is nobody's, or at no position of the table).  Without q the result is None.
 
         Values are rounded once; in 8 bits x / scale is, saturating at 448.  Two tokens of a call that are given the same place (a page that two
         sequences write) leave either's values there."""
@@ -170,7 +170,8 @@ class PagedCache:
         default.  With lse also [sequences, heads] fp32, the logarithm of the sum of exp(scale q . k).
 
         Statistics, sums and the weights of the values are fp32, out is rounded once.  A sequence without tokens: zeros, and -inf.  What lies in places
-        that are not seen has no influence, NaN included."""
+        that are not seen has no influence, NaN included.  Weights are up to 2^10 before their sum divides them: values above 2^118 / tokens may
+        overflow."""
         scale = 1.0 / math.sqrt(self.head_dim) if scale is None else scale
         native = _native().fast_paged_attend(self._at, self._device_index, q, page_table, lengths, scale, window, lse) if stream is None else None
         if native is not None:
