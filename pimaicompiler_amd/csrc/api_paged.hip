@@ -64,7 +64,7 @@ int cut_of(const PagedView& v, int group, int num_cus, AttendCut* cut)
 {
     const int nc = (v.dim + 63) / 64;
     // (for heads longer than 128 the registers do not hold the sums of 32 query heads)
-    cut->heads = group <= 4 ? 4 : group > 16 && nc <= 2 ? 32 : 16;
+    cut->heads = group > 16 && nc <= 2 ? 32 : 16;
     cut->tiles_of_heads = (group + cut->heads - 1) / cut->heads;
     const int64_t heads = (int64_t)v.kv_heads * cut->tiles_of_heads, units = (v.most + 15 + kUnit - 1) / kUnit;
     if (units * v.sequences > INT32_MAX / heads / 2 || (int64_t)v.sequences * v.kv_heads * group > (1 << 23))
@@ -87,7 +87,6 @@ void launch_attend(const AttendArgs& a, int blocks, hipStream_t s)
 template <class T, bool FP8, int NC>
 void launch_attend(const AttendArgs& a, const AttendCut& cut, hipStream_t s)
 {
-    if (cut.heads == 4) return launch_attend<T, FP8, NC, 4>(a, cut.blocks, s);
     if constexpr (NC <= 2) {
         if (cut.heads == 32) return launch_attend<T, FP8, NC, 32>(a, cut.blocks, s);
     }

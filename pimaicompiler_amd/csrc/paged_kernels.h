@@ -183,18 +183,17 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
 // kernel joins such pieces.  A wavefront takes 16 tokens of a unit at a time:
 //   scores    K [16 tokens x dim] . Q^T [dim x 16 heads] on the 16-bit matrix instruction (8-bit keys become Q's type, exactly): a lane has
 //             the scores of head l % 16 and tokens 4 (l / 16) + r
-//   values    P [16 heads x 4 tokens] . V [4 tokens x 16 columns] on the 32-bit one, for tokens r, 4 + r, 8 + r, 12 + r: a lane's e_j are its
-//             operand as they are, unrounded, and V is one that 16 lanes read as one row: nothing is turned or exchanged.
-//             Where a key head has up to 4 query heads most of those 16 rows are empty: Q's columns repeat every 4 heads then, and the matrix
-//             instruction of 16 blocks [4 heads x 1 token] . [1 x 4 columns] takes a lane's e_j and its own value of V, a quarter of the time; the
-//             four groups of lanes have sums over tokens of their own, which are added at the end (8-bit caches, 160 sequences of 4000 to 8192
-//             tokens: 331 us, with 16 rows 361; 16-bit ones the same either way.  Two of them for up to 8 heads need twice the registers: 1.6 GB in
-//             299 us, with 16 rows 278).  More than 16 query heads of up to 128 values go 32 at a time, so that keys and values are read once (24 heads: 307 us, 16
-//             at a time 530).
+//   values    P [16 heads x 16 tokens] . V [16 tokens x 16 columns]: a lane's four e_j are its operand as they are, and V's is four tokens of a column that
+//             16 lanes read as rows: nothing is exchanged.  Values of bfloat16 and of 8 bits, which bfloat16 has exactly, go through its matrix
+//             instruction, with e_j in three pieces of it, which are all of its 24 bits; fp16 ones through the 32-bit one, four tokens at a time, e_j
+//             as it is.  (The 32-bit one takes 2.7 times as long: 8-bit caches with 8 query heads a key head 159 us, in pieces 143; with 32, 16-bit
+//             ones 319 and 299.)
+// More than 16 query heads of up to 128 values go 32 at a time, so that keys and values are read once (24 heads: 287 us, 16 at a time some 530).  Fewer
+// leave rows of the instructions empty (a form with the instruction of 16 blocks of 4 rows for up to 4 heads took 0 to 3 % longer).
 // Values lie in registers from memory on, in loads that pass the caches (1.07 GB: 182 us, through them 208); a tile's are issued while the one
 // before is worked on.  Registers are bounded for three wavefronts a SIMD (two with two tiles each on their way, or four: 1 to 3 % slower).
 // Bound by the bytes: 537 MB of one sequence of 131071 tokens 93 us (5.8 TB/s), 1.07 GB of 64 sequences 180 (6.0), 1.64 GB in 8 bits 273 (6.0), where a kernel that
-// only reads has 6.9.  From 16 query heads a key head on, the 32-bit products of 8-bit caches are as long as the loads (16 heads: 172 us, with 8 159).
+// only reads has 6.9.  From 16 query heads a key head on, products are as long as the loads (8-bit caches: 155 us with 16, 143 with 8, 138 with 4).
 // Short calls take two launches and the dependent loads length, page, keys: 1000 tokens of one sequence 8 us.
 static constexpr int kUnit = 64;           // tokens that the four wavefronts of a block take together
 static constexpr float kLazy = 10.0f;      // a running maximum moves on when a score is above it by so many powers of two
@@ -351,12 +350,20 @@ struct ValuePiece {
             return (float)__builtin_bit_cast(half2_t, w[i / 2])[i % 2];
         }
     }
+    // Values 2 i and 2 i + 1 in bfloat16, where that has them exactly.
+    __device__ __forceinline__ unsigned int pair(int i) const
+    {
+        if constexpr (FP8)
+            return __builtin_bit_cast(unsigned int, i % 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i / 2], 1.0f, 1) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i / 2], 1.0f, 0));
+        else
+            return w[i];
+    }
 };
 
 // Wavefronts of a SIMD that the registers are bounded for.
 constexpr int attend_waves(int nc, int ht) { return nc <= 2 && ht <= 16 ? 3 : 2; }
 
-// NC: the head's size in 64 columns, rounded up; HT: query heads at a time (4, 16 or 32); EVEN: pages are whole tiles of 16 tokens, and the head's size is NC of 64:
+// NC: the head's size in 64 columns, rounded up; HT: query heads at a time (16 or 32); EVEN: pages are whole tiles of 16 tokens, and the head's size is NC of 64:
 // a tile's place is then the same for the wavefront, and no lane stays without loads (8-bit caches: 138 us, as others 146; 16-bit ones 258 and 260).
 template <class T, bool FP8, int NC, int HT, bool EVEN>
 __global__ __launch_bounds__(256, attend_waves(NC, HT)) void paged_attend_kernel(AttendArgs a)
@@ -367,11 +374,10 @@ __global__ __launch_bounds__(256, attend_waves(NC, HT)) void paged_attend_kernel
     constexpr int kLoads = FP8 ? NC : kSteps;        // 16-byte loads of a key's row by a lane
     constexpr int kWide = NC / 2, kNarrow = NC % 2;  // pieces of eight and of four columns of a lane
     constexpr int kCols = NC * 4, kSize = FP8 ? 1 : 2;
-    constexpr bool kFew = HT == 4;
-    constexpr int kScores = kFew ? 1 : HT / 16;      // tiles of 16 heads
-    constexpr int kParts = kFew ? 4 : 1;             // sums over tokens that a wavefront leaves of each head
+    constexpr int kScores = HT / 16;                 // tiles of 16 heads
+    constexpr bool kThree = FP8 || __is_same(T, BF16);  // weights in three pieces of bfloat16
     __shared__ float wave_m[4][HT], wave_l[4][HT];
-    __shared__ float parts[4][kParts * HT][NC * 64 + 4];
+    __shared__ float parts[4][HT][NC * 64 + 4];
     const int lane = threadIdx.x & 63, wave = wave_in_block(), n = lane & 15, g = lane >> 4;
     const PagedView& c = a.c;
     const int D = c.dim;
@@ -390,7 +396,7 @@ __global__ __launch_bounds__(256, attend_waves(NC, HT)) void paged_attend_kernel
         frag q[kScores][kSteps];
 #pragma unroll
         for (int mt = 0; mt < kScores; ++mt) {
-            const int h = head0 + (kFew ? n % HT : mt * 16 + n);
+            const int h = head0 + mt * 16 + n;
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
                 const int d = FP8 ? i / 2 * 64 + g * 16 + i % 2 * 8 : i * 32 + g * 8;
@@ -414,8 +420,6 @@ __global__ __launch_bounds__(256, attend_waves(NC, HT)) void paged_attend_kernel
         for (int mt = 0; mt < kScores; ++mt)
 #pragma unroll
             for (int i = 0; i < kCols; ++i) o[mt][i] = float4_t{0, 0, 0, 0};
-        // The lane that has the statistics of row r of a lane's results.
-        auto lane_of = [&](int r) { return kFew ? (lane & ~3) | r : g * 4 + r; };
 
         // ---- tiles: 16 tokens of each unit ----
         uint4_t k[kLoads];
@@ -542,7 +546,7 @@ __global__ __launch_bounds__(256, attend_waves(NC, HT)) void paged_attend_kernel
                 for (int mt = 0; mt < kScores; ++mt)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float fr = __shfl(f[mt], lane_of(r));
+                        const float fr = __shfl(f[mt], g * 4 + r);
 #pragma unroll
                         for (int i = 0; i < kCols; ++i) o[mt][i][r] *= fr;
                     }
@@ -555,12 +559,53 @@ __global__ __launch_bounds__(256, attend_waves(NC, HT)) void paged_attend_kernel
                 for (int r = 0; r < 4; ++r) p[mt][r] = __builtin_amdgcn_exp2f(sc[mt][r] - from);
                 l[mt] += (p[mt][0] + p[mt][1]) + (p[mt][2] + p[mt][3]);
             }
+            if constexpr (kThree) {
+                typedef short short4v_t __attribute__((ext_vector_type(4)));
+                auto operand = [](unsigned int w0, unsigned int w1) { return __builtin_bit_cast(short4v_t, uint2_t{w0, w1}); };
+                auto halves = [](unsigned int w0, unsigned int w1, bool upper) { return __builtin_amdgcn_perm(w1, w0, upper ? 0x07060302u : 0x05040100u); };
+                short4v_t part[3][kScores];
+#pragma unroll
+                for (int mt = 0; mt < kScores; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) {
+                        unsigned int b[4];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            b[r] = __builtin_bit_cast(unsigned int, p[mt][r]);
+                            // (what is left, never 0: an infinite value times it stays one)
+                            p[mt][r] = fmaxf(p[mt][r] - __builtin_bit_cast(float, b[r] & 0xffff0000u), 0x1p-126f);
+                        }
+                        part[i][mt] = operand(halves(b[0], b[1], true), halves(b[2], b[3], true));
+                    }
+                // Columns i and i + 1 of a lane, of its four tokens.
+                auto add = [&](int i, const unsigned int(&w)[4]) {
+                    const short4v_t v[2] = {operand(halves(w[0], w[1], false), halves(w[2], w[3], false)), operand(halves(w[0], w[1], true), halves(w[2], w[3], true))};
+#pragma unroll
+                    for (int k = 0; k < 3; ++k)
+#pragma unroll
+                        for (int mt = 0; mt < kScores; ++mt)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) o[mt][i + c] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(part[k][mt], v[c], o[mt][i + c], 0, 0, 0);
+                };
+#pragma unroll
+                for (int i = 0; i < kWide; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) add(i * 8 + e * 2, {wide[0][i].pair(e), wide[1][i].pair(e), wide[2][i].pair(e), wide[3][i].pair(e)});
+                if constexpr (kNarrow)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) add(kWide * 8 + e * 2, {narrow[0][0].pair(e), narrow[1][0].pair(e), narrow[2][0].pair(e), narrow[3][0].pair(e)});
+                if constexpr (kMore) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) load_values(r);
+                }
+                return;
+            }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 auto add = [&](int i, float v) {
 #pragma unroll
                     for (int mt = 0; mt < kScores; ++mt)
-                        o[mt][i] = kFew ? __builtin_amdgcn_mfma_f32_4x4x1f32(p[mt][r], v, o[mt][i], 0, 0, 0) : __builtin_amdgcn_mfma_f32_16x16x4f32(p[mt][r], v, o[mt][i], 0, 0, 0);
+                        o[mt][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[mt][r], v, o[mt][i], 0, 0, 0);
                 };
 #pragma unroll
                 for (int i = 0; i < kWide; ++i)
@@ -582,7 +627,7 @@ __global__ __launch_bounds__(256, attend_waves(NC, HT)) void paged_attend_kernel
         for (int mt = 0; mt < kScores; ++mt) {
             l[mt] += __shfl_xor(l[mt], 16);
             l[mt] += __shfl_xor(l[mt], 32);
-            if (g == 0 && (!kFew || n < HT)) {
+            if (g == 0) {
                 wave_m[wave][mt * 16 + n] = m[mt];
                 wave_l[wave][mt * 16 + n] = l[mt];
             }
@@ -591,9 +636,9 @@ __global__ __launch_bounds__(256, attend_waves(NC, HT)) void paged_attend_kernel
         for (int mt = 0; mt < kScores; ++mt)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int h = kFew ? r : mt * 16 + g * 4 + r;
+                const int h = mt * 16 + g * 4 + r;
                 if (h >= rows) continue;
-                float* part = parts[wave][kFew ? g * HT + h : h];
+                float* part = parts[wave][h];
 #pragma unroll
                 for (int i = 0; i < kWide; ++i)
 #pragma unroll
@@ -618,8 +663,7 @@ __global__ __launch_bounds__(256, attend_waves(NC, HT)) void paged_attend_kernel
             for (int w = 0; w < 4; ++w) {
                 const float f = wave_m[w][h] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(wave_m[w][h] - top);
                 weight += f * wave_l[w][h];
-#pragma unroll
-                for (int q = 0; q < kParts; ++q) sum += f * *reinterpret_cast<const float4_t*>(&parts[w][q * HT + h][d]);
+                sum += f * *reinterpret_cast<const float4_t*>(&parts[w][h][d]);
             }
             if (complete) {
                 store_attended<T>(a, out0 + h, d, sum, weight, top, vs);

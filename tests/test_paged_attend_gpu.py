@@ -52,6 +52,35 @@ def test_query_heads_of_a_key_head(ops, heads, kv, dim, held):
     run(ops, [1, 33, 100], heads, kv, dim, 32, torch.float16, held, seed=heads)
 
 
+@pytest.mark.parametrize("heads,kv", [(2, 2), (5, 1), (8, 1), (17, 1), (32, 1), (48, 2), (71, 1)])
+@pytest.mark.parametrize("dim,page", [(64, 32), (128, 16), (192, 16), (72, 24)])
+def test_query_heads_of_a_key_head_in_bfloat16(ops, heads, kv, dim, page):
+    run(ops, [1, 33, 100, 400], heads, kv, dim, page, torch.bfloat16, torch.bfloat16, seed=heads)
+    if dim % 16 == 0:
+        run(ops, [1, 33, 100], heads, kv, dim, page, torch.bfloat16, FP8, seed=heads)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads", [1, 20])
+def test_infinite_and_large_values(ops, dtype, heads):
+    """A value that is infinite makes its columns so, also with a weight of exactly one, and large ones stay finite."""
+    cache = Cache([1, 40, 200, 90], 1, 16, 64, dtype, seed=heads)
+    for s, j, column, value in ((0, 0, 3, INF), (0, 0, 40, -INF), (1, 39, 63, INF), (2, 100, 0, -INF), (2, 150, 17, INF)):
+        cache.v[int(cache.table[s, j // 16]), 0, j % 16, column] = value
+    large = 2.0**100 if dtype == torch.bfloat16 else 2.0**14
+    for page in cache.table[3][cache.table[3] >= 0].tolist():
+        cache.v[page] *= large
+    q = 0.05 * torch.randn(4, heads, 64, generator=torch.Generator().manual_seed(7))   # (weights that no type loses: an infinite value times 0 is NaN)
+    table, n = cache.tensors(DEV)
+    out = cache.on(ops, DEV).attend(q.to(dtype).to(DEV), table, n).cpu()
+    want, _, bound, _ = attend(cache, q.to(dtype), 1 / 8)
+    fixed = want.isfinite()
+    assert torch.equal(out.double()[~fixed], want[~fixed]) and bool(out[fixed].isfinite().all())
+    rest = fixed & bound.isfinite()
+    assert bool(((out.double() - want).abs() <= bound)[rest].all())
+    assert bool(out[3].isfinite().all()) and int((~fixed).sum()) == 5 * heads
+
+
 @pytest.mark.parametrize("page", [1, 2, 15, 16, 17, 32, 48, 100, 128, 1000])
 @pytest.mark.parametrize("held", [torch.bfloat16, FP8])
 def test_page_sizes(ops, page, held):

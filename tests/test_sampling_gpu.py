@@ -260,6 +260,36 @@ def test_workspaces(ops):
         assert all(torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) for a, b in zip(got, want))
 
 
+def test_two_captured_calls(ops):
+    """Two graphs of calls that have workspaces, replayed in turn and at the same time with eager calls between, read logits, numbers and settings anew."""
+    n, V = 3, 60000
+    g = torch.Generator().manual_seed(1)
+    xs = [torch.empty(n, V, dtype=t, device=DEV) for t in (torch.bfloat16, torch.float32)]
+    us, ks = [torch.empty(n, device=DEV) for _ in xs], [torch.zeros(n, dtype=torch.int32, device=DEV) for _ in xs]
+    streams, graphs, outs = [torch.cuda.Stream() for _ in xs], [torch.cuda.CUDAGraph() for _ in xs], []
+    fill = lambda: [t.copy_(v) for x, u, k in zip(xs, us, ks) for t, v in ((x, 2.5 * torch.randn(n, V, generator=g)), (u, torch.rand(n, generator=g)),  # noqa: E731
+                                                                          (k, torch.randint(0, 900, (n,), generator=g)))]
+    fill()
+    call = lambda i: ops.sample_tokens(xs[i], us[i], temperature=0.7, top_k=ks[i], top_p=0.9)  # noqa: E731
+    for i in range(2):
+        call(i)
+    torch.cuda.synchronize()
+    for graph, i in zip(graphs, range(2)):
+        with torch.cuda.graph(graph):
+            outs.append(call(i))
+    for _ in range(4):
+        fill()
+        want = [call(i) for i in range(2)]
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        call(0)
+        torch.cuda.synchronize()
+        for out, w in zip(outs, want):
+            assert torch.equal(out[0], w[0]) and torch.equal(out[1], w[1])
+
+
 @pytest.mark.parametrize("V", [30001, 60001])
 @pytest.mark.parametrize("dtype", DTYPES[:2])
 def test_long_rows_at_the_ends(ops, dtype, V):
