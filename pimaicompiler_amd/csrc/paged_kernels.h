@@ -192,7 +192,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
 // leave rows of the instructions empty (a form with the instruction of 16 blocks of 4 rows for up to 4 heads took 0 to 3 % longer).
 // Values lie in registers from memory on, in loads that pass the caches (1.07 GB: 182 us, through them 208); a tile's are issued while the one
 // before is worked on.  Registers are bounded for three wavefronts a SIMD (two with two tiles each on their way, or four: 1 to 3 % slower).
-// Bound by the bytes: 537 MB of one sequence of 131071 tokens 93 us (5.8 TB/s), 1.07 GB of 64 sequences 180 (6.0), 1.64 GB in 8 bits 273 (6.0), where a kernel that
+// Bound by the bytes: 537 MB of one sequence of 131071 tokens 93 us (5.8 TB/s), 1.07 GB of 64 sequences 179 (6.0), 1.64 GB in 8 bits 272 (6.0), where a kernel that
 // only reads has 6.9.  From 16 query heads a key head on, products are as long as the loads (8-bit caches: 155 us with 16, 143 with 8, 138 with 4).
 // Short calls take two launches and the dependent loads length, page, keys: 1000 tokens of one sequence 8 us.
 static constexpr int kUnit = 64;           // tokens that the four wavefronts of a block take together
@@ -682,28 +682,28 @@ __global__ __launch_bounds__(256, attend_waves(NC, HT)) void paged_attend_kernel
     }
 }
 
-// The pieces of each (sequence, key head) that more than one block worked on: a block a head, its wavefronts a quarter of the pieces each.
-template <class T>
-__global__ __launch_bounds__(256) void paged_join_kernel(AttendArgs a, int rows)
+// The pieces of each (sequence, key head) that more than one block worked on: a block a head, its wavefronts an equal share of the pieces each.
+template <class T, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void paged_join_kernel(AttendArgs a, int rows)
 {
     const PagedView& c = a.c;
     const int D = c.dim, heads = c.kv_heads * a.group;
     const int s = blockIdx.x / heads, h_all = blockIdx.x - s * heads, kvh = h_all / a.group, h_in = h_all - kvh * a.group, tile = h_in / rows, h = h_in - tile * rows;
     const int2 blocks = a.pieces[((int64_t)s * c.kv_heads + kvh) * a.tiles_of_heads + tile];
     if (blocks.x == blocks.y) return;
-    __shared__ float wave_m[4], wave_l[4];
-    __shared__ float parts[4][256];
+    __shared__ float wave_m[WAVES], wave_l[WAVES];
+    __shared__ float parts[WAVES][256];
     const int lane = threadIdx.x & 63, wave = wave_in_block(), d = lane * 4;
     // (a piece's place: the block's second where the sequence begins in it, else its first)
     auto part = [&](int b) { return a.work + (((int64_t)b * 2 + (b == blocks.x ? 1 : 0)) * rows + h) * (D + 4); };
     float top = -__builtin_inff(), l = 0.0f;
     float4_t sum = {0, 0, 0, 0};
-    for (int b = blocks.x + wave; b <= blocks.y; b += 16) {
+    for (int b = blocks.x + wave; b <= blocks.y; b += 4 * WAVES) {
         float2_t ml[4];
         float4_t v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float* p = part(b + 4 * i <= blocks.y ? b + 4 * i : b);
+            const float* p = part(b + WAVES * i <= blocks.y ? b + WAVES * i : b);
             ml[i] = *reinterpret_cast<const float2_t*>(p + D);
             v[i] = d < D ? *reinterpret_cast<const float4_t*>(p + d) : float4_t{0, 0, 0, 0};
         }
@@ -715,7 +715,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttendArgs a, int rows)
         sum *= f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (b + 4 * i > blocks.y) continue;
+            if (b + WAVES * i > blocks.y) continue;
             const float fi = ml[i][0] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ml[i][0] - now);
             l += fi * ml[i][1];
             sum += fi * v[i];
@@ -729,11 +729,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttendArgs a, int rows)
     *reinterpret_cast<float4_t*>(&parts[wave][d]) = sum;
     __syncthreads();
     if (wave != 0 || d >= D) return;
-    const float all = fmaxf(fmaxf(wave_m[0], wave_m[1]), fmaxf(wave_m[2], wave_m[3]));
+    float all = wave_m[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) all = fmaxf(all, wave_m[w]);
     float weight = 0.0f;
     sum = float4_t{0, 0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
         const float f = wave_m[w] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(wave_m[w] - all);
         weight += f * wave_l[w];
         sum += f * *reinterpret_cast<const float4_t*>(&parts[w][d]);
