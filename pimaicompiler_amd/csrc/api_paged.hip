@@ -105,6 +105,7 @@ template <class T>
 void launch_attend(const AttendArgs& a, const AttendCut& cut, hipStream_t s)
 {
     a.c.k_scale ? launch_attend<T, true>(a, cut, s) : launch_attend<T, false>(a, cut, s);
+    if (a.whole) return;
     // Sixteen wavefronts where a head may have more than 32 parts (one sequence of 131071 tokens, 96 of them: 92.9 us, with four 94.8; of 8000 15.7 and 17.0; of
     // 1000 in 16 heads, 16 parts: 9.4 and 8.6).
     const dim3 heads(a.c.sequences * a.c.kv_heads * a.group);
@@ -200,6 +201,13 @@ extern "C" int pimhip_paged_attend(const PimHipPagedCache* cache, const PimHipPa
     a.out = out, a.lse = lse, a.work = static_cast<float*>(workspace);
     a.pieces = reinterpret_cast<int2*>(static_cast<char*>(workspace) + part_bytes(cut, a.c.dim));
     a.group = q_heads / a.c.kv_heads, a.tiles_of_heads = cut.tiles_of_heads, a.window = window;
+    // Sequences of a few units, by the room they have or by the window, are not cut, and nothing is joined.
+    const int64_t seen = window > 0 && window < a.c.most ? (int64_t)window + 15 : a.c.most;
+    const int64_t heads = (int64_t)a.c.sequences * a.c.kv_heads * cut.tiles_of_heads;
+    if (seen <= paged_whole_units(heads, true) * (int64_t)kUnit) {
+        a.whole = 1;
+        cut.blocks = (int)heads;
+    }
     hipStream_t s = static_cast<hipStream_t>(stream);
     dtype == PIMHIP_F16 ? launch_attend<F16>(a, cut, s) : launch_attend<BF16>(a, cut, s);
     PIMHIP_HIP_CHECK(hipGetLastError());

@@ -179,7 +179,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
 // ---- attend ---------------------------------------------------------------------------------------
 //
 // The tokens of all sequences and key heads lie in a row of units of 64; each block takes an equal stretch of them, so that lengths may differ
-// as they like.  A piece of a (sequence, key head) that does not fill it goes to the workspace with its own maximum and sum, and a second
+// as they like (short sequences: a block takes a key head of one from end to end).  A piece of a (sequence, key head) that does not fill it goes to the workspace with its own maximum and sum, and a second
 // kernel joins such pieces.  A wavefront takes 16 tokens of a unit at a time:
 //   scores    K [16 tokens x dim] . Q^T [dim x 16 heads] on the 16-bit matrix instruction (8-bit keys become Q's type, exactly): a lane has
 //             the scores of head l % 16 and tokens 4 (l / 16) + r
@@ -207,6 +207,7 @@ struct AttendArgs {
     int2* pieces; // [sequences * kv_heads * tiles_of_heads]: the first and the last block that worked on each
     int64_t q_seq, q_head;  // elements
     int group, tiles_of_heads, window;
+    int whole;  // a block takes one (sequence, key head) from end to end, and nothing is joined
     float scale_log2;
 };
 
@@ -233,31 +234,65 @@ __device__ __forceinline__ PagedSpan paged_span(int length, int window)
     return p;
 }
 
+// Units up to which sequences are not cut, with `heads` (sequence, key head)s: each of these is then a block's from end to end.  Where the room that sequences
+// have, or the window, says so (first), nothing is joined either; where lengths do, the launch that joins finds nothing.  In us, cut, whole and whole by
+// lengths (8 key heads of 128, bfloat16): 1 sequence of 200 tokens 8.6, 5.7 and -, of 2000 10.1 and 14.9; 16 of 500 15.6, 13.3 and 16.3; 64 of 300 22.4, 15.2 and 18.5, of
+// 1000 44.0, 38.1 and 41.4, of 4000 132 and 137; 256 of 500 83.8, 72.7 and 77.7, of 1 to 1000 114, 99 and 112.
+__host__ __device__ constexpr int paged_whole_units(int64_t heads, bool first) { return first ? (heads >= 256 ? 16 : heads >= 64 ? 8 : 4) : heads >= 512 ? 16 : heads >= 256 ? 8 : 0; }
+
 // The stretch of a block in the row of units (`times` units for each of a sequence's, less than 2^31 in all): units first .. end - 1 of `per` a
 // block, and the sequence it begins in, which begins at unit `before` and is `length` tokens long.
 struct PagedStretch {
     int first, end, per, s, before, length;
+    bool whole;  // this and every grid's size-th (sequence, key head) behind it instead, as long as there are any
 };
-__device__ __forceinline__ PagedStretch paged_stretch(const PagedView& c, int window, int times)
+// The block's first (sequence, key head), as a stretch of its own.
+__device__ __forceinline__ void paged_whole(const PagedView& c, int window, int times, int at, PagedStretch& f)
+{
+    f.whole = true;
+    f.s = at / times;
+    f.before = 0;
+    f.first = f.end = 0;
+    if (f.s >= c.sequences) return;
+    f.length = paged_length(c, f.s);
+    f.per = paged_span(f.length, window).units;
+    f.first = (at - f.s * times) * f.per;
+    f.end = f.first + f.per;
+}
+__device__ __forceinline__ PagedStretch paged_stretch(const PagedView& c, int window, int times, bool whole)
 {
     PagedStretch f;
+    if (whole) {
+        paged_whole(c, window, times, (int)blockIdx.x, f);
+        return f;
+    }
+    f.whole = false;
+    const int most = paged_whole_units((int64_t)c.sequences * times, false);
     if (c.sequences == 1) {
         f.s = f.before = 0;
         f.length = paged_length(c, 0);
-        const int total = paged_span(f.length, window).units * times;
+        const int units = paged_span(f.length, window).units, total = units * times;
+        if (units <= most) {
+            paged_whole(c, window, times, (int)blockIdx.x, f);
+            return f;
+        }
         f.per = (int)((unsigned int)(total + (int)gridDim.x - 1) / gridDim.x);
         f.first = (int)blockIdx.x * f.per;
         f.end = f.first + f.per < total ? f.first + f.per : total;
         return f;
     }
     __shared__ int wave_sum_of[4];
+    __shared__ bool wave_long[4];
     __shared__ int found[3];
     const int each = (c.sequences + 255) / 256, from = (int)threadIdx.x * each, lo = from < c.sequences ? from : c.sequences;
     const int hi = lo + each < c.sequences ? lo + each : c.sequences;
     int mine = 0, length = 0;
+    bool is_long = false;
     for (int s = lo; s < hi; ++s) {
         length = paged_length(c, s);
-        mine += paged_span(length, window).units * times;
+        const int units = paged_span(length, window).units;
+        is_long |= units > most;
+        mine += units * times;
     }
     int incl = mine;
 #pragma unroll
@@ -265,8 +300,16 @@ __device__ __forceinline__ PagedStretch paged_stretch(const PagedView& c, int wi
         const int o = __shfl_up(incl, d);
         if ((int)(threadIdx.x & 63) >= d) incl += o;
     }
-    if ((threadIdx.x & 63) == 63) wave_sum_of[threadIdx.x >> 6] = incl;
+    const bool some_long = __ballot(is_long) != 0;
+    if ((threadIdx.x & 63) == 63) {
+        wave_sum_of[threadIdx.x >> 6] = incl;
+        wave_long[threadIdx.x >> 6] = some_long;
+    }
     __syncthreads();
+    if (!(wave_long[0] || wave_long[1] || wave_long[2] || wave_long[3])) {
+        paged_whole(c, window, times, (int)blockIdx.x, f);
+        return f;
+    }
     int before = incl - mine, total = 0;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -383,13 +426,13 @@ __global__ __launch_bounds__(256, attend_waves(NC, HT)) void paged_attend_kernel
     const int D = c.dim;
     const int heads_of_units = c.kv_heads * a.tiles_of_heads;
 
-    const PagedStretch stretch = paged_stretch(c, a.window, heads_of_units);
+    PagedStretch stretch = paged_stretch(c, a.window, heads_of_units, a.whole != 0);
     if (stretch.first >= stretch.end) return;
-    int s = stretch.s, before = stretch.before, length = stretch.length;
-    for (int u = stretch.first; u < stretch.end;) {
+    int s = stretch.s, before = stretch.before, length = stretch.length, end = stretch.end, at = (int)blockIdx.x;
+    for (int u = stretch.first; u < end;) {
         const PagedSpan span = paged_span(length, a.window);
         const int rel = u - before, hg = rel / span.units, first = rel - hg * span.units;
-        const int left = span.units - first, take = left < stretch.end - u ? left : stretch.end - u, last = first + take;
+        const int left = span.units - first, take = left < end - u ? left : end - u, last = first + take;
         const int kvh = hg / a.tiles_of_heads, head0 = (hg - kvh * a.tiles_of_heads) * HT;
 
         // ---- queries ----
@@ -672,8 +715,14 @@ __global__ __launch_bounds__(256, attend_waves(NC, HT)) void paged_attend_kernel
                 if (d == 0) *reinterpret_cast<float2_t*>(piece + h * (D + 4) + D) = float2_t{top, weight};
             }
         }
-        if (threadIdx.x == 0 && last == span.units) a.pieces[(int64_t)s * heads_of_units + hg] = int2{(u - first) / stretch.per, (int)blockIdx.x};
+        if (threadIdx.x == 0 && last == span.units) a.pieces[(int64_t)s * heads_of_units + hg] = int2{stretch.whole ? (int)blockIdx.x : (u - first) / stretch.per, (int)blockIdx.x};
         __syncthreads();
+        if (stretch.whole) {
+            at += (int)gridDim.x;
+            paged_whole(c, a.window, heads_of_units, at, stretch);
+            s = stretch.s, length = stretch.length, u = stretch.first, end = stretch.end;
+            continue;
+        }
         u += take;
         if (rel + take == heads_of_units * span.units) {
             before += heads_of_units * span.units;

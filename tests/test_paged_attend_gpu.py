@@ -81,6 +81,18 @@ def test_infinite_and_large_values(ops, dtype, heads):
     assert bool(out[3].isfinite().all()) and int((~fixed).sum()) == 5 * heads
 
 
+@pytest.mark.parametrize("sequences,kv,longest", [(1, 1, 256), (1, 1, 257), (8, 8, 512), (8, 8, 513), (32, 8, 700), (128, 4, 512), (129, 4, 300), (70, 16, 100)])
+@pytest.mark.parametrize("extra", [0, 60])
+def test_sequences_that_are_not_cut(ops, sequences, kv, longest, extra):
+    """Up to some length, which goes by the table's room and by the lengths, sequences are taken from end to end; windows are too."""
+    g = torch.Generator().manual_seed(longest)
+    lengths = torch.randint(0, longest + 1, (sequences,), generator=g).tolist()
+    lengths[sequences // 2] = longest
+    cache = Cache(lengths, kv, 64, 16, torch.bfloat16, seed=sequences, rest=float("nan"), extra_width=extra)
+    run(ops, lengths, 2 * kv, kv, 16, 64, torch.bfloat16, torch.bfloat16, cache=cache)
+    run(ops, lengths, 2 * kv, kv, 16, 64, torch.bfloat16, torch.bfloat16, cache=cache, window=100)
+
+
 @pytest.mark.parametrize("page", [1, 2, 15, 16, 17, 32, 48, 100, 128, 1000])
 @pytest.mark.parametrize("held", [torch.bfloat16, FP8])
 def test_page_sizes(ops, page, held):
