@@ -102,14 +102,19 @@ void launch_attend(const AttendArgs& a, const AttendCut& cut, hipStream_t s)
               : launch_attend<T, FP8, 4>(a, cut, s);
 }
 template <class T>
-void launch_attend(const AttendArgs& a, const AttendCut& cut, hipStream_t s)
+void launch_attend(const AttendArgs& a, const AttendCut& cut, int num_cus, hipStream_t s)
 {
     a.c.k_scale ? launch_attend<T, true>(a, cut, s) : launch_attend<T, false>(a, cut, s);
     if (a.whole) return;
-    // Sixteen wavefronts where a head may have more than 32 parts (one sequence of 131071 tokens, 96 of them: 92.9 us, with four 94.8; of 8000 15.7 and 17.0; of
-    // 1000 in 16 heads, 16 parts: 9.4 and 8.6).
-    const dim3 heads(a.c.sequences * a.c.kv_heads * a.group);
-    cut.blocks > 32 * (int64_t)a.c.sequences * a.c.kv_heads * a.tiles_of_heads ? paged_join_kernel<T, 16><<<heads, 1024, 0, s>>>(a, cut.heads) : paged_join_kernel<T, 4><<<heads, 256, 0, s>>>(a, cut.heads);
+    // One wavefront a head where heads are many (64 sequences, 192 heads each: 276 us, with four 286), sixteen where they are few and may have more
+    // than 32 parts (one sequence of 131071 tokens, 96 of them: 92.9 us, with four 94.8), else four (32 heads of 16 parts: 9.9 us, with one 10.8).
+    const int heads = a.c.sequences * a.c.kv_heads * a.group;
+    if (heads > 2 * num_cus)
+        paged_join_kernel<T, 1><<<dim3((heads + 3) / 4), 256, 0, s>>>(a, cut.heads);
+    else if (cut.blocks > 32 * (int64_t)a.c.sequences * a.c.kv_heads * a.tiles_of_heads)
+        paged_join_kernel<T, 16><<<dim3(heads), 1024, 0, s>>>(a, cut.heads);
+    else
+        paged_join_kernel<T, 4><<<dim3(heads), 256, 0, s>>>(a, cut.heads);
 }
 }  // namespace
 
@@ -209,7 +214,7 @@ extern "C" int pimhip_paged_attend(const PimHipPagedCache* cache, const PimHipPa
         cut.blocks = (int)heads;
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
-    dtype == PIMHIP_F16 ? launch_attend<F16>(a, cut, s) : launch_attend<BF16>(a, cut, s);
+    dtype == PIMHIP_F16 ? launch_attend<F16>(a, cut, st->num_cus, s) : launch_attend<BF16>(a, cut, st->num_cus, s);
     PIMHIP_HIP_CHECK(hipGetLastError());
     return PIMHIP_OK;
 }

@@ -731,64 +731,76 @@ __global__ __launch_bounds__(256, attend_waves(NC, HT)) void paged_attend_kernel
     }
 }
 
-// The pieces of each (sequence, key head) that more than one block worked on: a block a head, its wavefronts an equal share of the pieces each.
+// The pieces of each (sequence, key head) that more than one block worked on, of a head by WAVES wavefronts, an equal share of the pieces each: by one (four heads
+// a block), four or sixteen.  A wavefront asks for four pieces at a time, one that is alone for sixteen where there are more, a lane for four columns of each.
 template <class T, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void paged_join_kernel(AttendArgs a, int rows)
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void paged_join_kernel(AttendArgs a, int rows)
 {
     const PagedView& c = a.c;
-    const int D = c.dim, heads = c.kv_heads * a.group;
-    const int s = blockIdx.x / heads, h_all = blockIdx.x - s * heads, kvh = h_all / a.group, h_in = h_all - kvh * a.group, tile = h_in / rows, h = h_in - tile * rows;
+    const int D = c.dim, heads = c.kv_heads * a.group, lane = threadIdx.x & 63, wave = WAVES == 1 ? 0 : wave_in_block(), d = lane * 4;
+    const int at = WAVES == 1 ? (int)blockIdx.x * 4 + wave_in_block() : (int)blockIdx.x;
+    if (WAVES == 1 && at >= c.sequences * heads) return;
+    const int s = at / heads, h_all = at - s * heads, kvh = h_all / a.group, h_in = h_all - kvh * a.group, tile = h_in / rows, h = h_in - tile * rows;
     const int2 blocks = a.pieces[((int64_t)s * c.kv_heads + kvh) * a.tiles_of_heads + tile];
     if (blocks.x == blocks.y) return;
-    __shared__ float wave_m[WAVES], wave_l[WAVES];
-    __shared__ float parts[WAVES][256];
-    const int lane = threadIdx.x & 63, wave = wave_in_block(), d = lane * 4;
     // (a piece's place: the block's second where the sequence begins in it, else its first)
     auto part = [&](int b) { return a.work + (((int64_t)b * 2 + (b == blocks.x ? 1 : 0)) * rows + h) * (D + 4); };
     float top = -__builtin_inff(), l = 0.0f;
     float4_t sum = {0, 0, 0, 0};
-    for (int b = blocks.x + wave; b <= blocks.y; b += 4 * WAVES) {
-        float2_t ml[4];
-        float4_t v[4];
+    auto add = [&](auto count, int b) {
+        constexpr int kCount = decltype(count)::value;
+        float2_t ml[kCount];
+        float4_t v[kCount];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kCount; ++i) {
             const float* p = part(b + WAVES * i <= blocks.y ? b + WAVES * i : b);
             ml[i] = *reinterpret_cast<const float2_t*>(p + D);
             v[i] = d < D ? *reinterpret_cast<const float4_t*>(p + d) : float4_t{0, 0, 0, 0};
         }
         float now = top;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) now = fmaxf(now, ml[i][0]);
+        for (int i = 0; i < kCount; ++i) now = fmaxf(now, ml[i][0]);
         const float f = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(top - now);
         l *= f;
         sum *= f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kCount; ++i) {
             if (b + WAVES * i > blocks.y) continue;
             const float fi = ml[i][0] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ml[i][0] - now);
             l += fi * ml[i][1];
             sum += fi * v[i];
         }
         top = now;
-    }
-    if (lane == 0) {
-        wave_m[wave] = top;
-        wave_l[wave] = l;
-    }
-    *reinterpret_cast<float4_t*>(&parts[wave][d]) = sum;
-    __syncthreads();
-    if (wave != 0 || d >= D) return;
-    float all = wave_m[0];
+    };
+    int b = blocks.x + wave;
+    if constexpr (WAVES == 1)
+        for (; b + 4 <= blocks.y; b += 16) add(std::integral_constant<int, 16>{}, b);
+    for (; b <= blocks.y; b += 4 * WAVES) add(std::integral_constant<int, 4>{}, b);
+    const float scale = c.v_scale ? c.v_scale[kvh] : 1.0f;
+    if constexpr (WAVES == 1) {
+        if (d < D) store_attended<T>(a, at, d, sum, l, top, scale);
+    } else {
+        __shared__ float wave_m[WAVES], wave_l[WAVES];
+        __shared__ float parts[WAVES][256];
+        if (lane == 0) {
+            wave_m[wave] = top;
+            wave_l[wave] = l;
+        }
+        *reinterpret_cast<float4_t*>(&parts[wave][d]) = sum;
+        __syncthreads();
+        if (wave != 0 || d >= D) return;
+        float all = wave_m[0];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) all = fmaxf(all, wave_m[w]);
-    float weight = 0.0f;
-    sum = float4_t{0, 0, 0, 0};
+        for (int w = 1; w < WAVES; ++w) all = fmaxf(all, wave_m[w]);
+        float weight = 0.0f;
+        sum = float4_t{0, 0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        const float f = wave_m[w] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(wave_m[w] - all);
-        weight += f * wave_l[w];
-        sum += f * *reinterpret_cast<const float4_t*>(&parts[w][d]);
+        for (int w = 0; w < WAVES; ++w) {
+            const float f = wave_m[w] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(wave_m[w] - all);
+            weight += f * wave_l[w];
+            sum += f * *reinterpret_cast<const float4_t*>(&parts[w][d]);
+        }
+        store_attended<T>(a, at, d, sum, weight, all, scale);
     }
-    store_attended<T>(a, blockIdx.x, d, sum, weight, all, c.v_scale ? c.v_scale[kvh] : 1.0f);
 }
 }  // namespace pimhip
