@@ -188,12 +188,12 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
 //             instruction, with e_j in three pieces of it, which are all of its 24 bits; fp16 ones through the 32-bit one, four tokens at a time, e_j
 //             as it is.  (The 32-bit one takes 2.7 times as long: 8-bit caches with 8 query heads a key head 159 us, in pieces 143; with 32, 16-bit
 //             ones 319 and 299.)
-// More than 16 query heads of up to 128 values go 32 at a time, so that keys and values are read once (24 heads: 287 us, 16 at a time some 530).  Fewer
+// More than 16 query heads of up to 128 values go 32 at a time, so that keys and values are read once (24 heads: 278 us, 16 at a time some 530).  Fewer
 // leave rows of the instructions empty (a form with the instruction of 16 blocks of 4 rows for up to 4 heads took 0 to 3 % longer).
 // Values lie in registers from memory on, in loads that pass the caches (1.07 GB: 182 us, through them 208); a tile's are issued while the one
 // before is worked on.  Registers are bounded for three wavefronts a SIMD (two with two tiles each on their way, or four: 1 to 3 % slower).
-// Bound by the bytes: 537 MB of one sequence of 131071 tokens 93 us (5.8 TB/s), 1.07 GB of 64 sequences 179 (6.0), 1.64 GB in 8 bits 272 (6.0), where a kernel that
-// only reads has 6.9.  From 16 query heads a key head on, products are as long as the loads (8-bit caches: 155 us with 16, 143 with 8, 138 with 4).
+// Bound by the bytes: 537 MB of one sequence of 131071 tokens 93 us (5.8 TB/s), 1.07 GB of 64 sequences 177 (6.1), 1.64 GB in 8 bits 270 (6.1), where a kernel that
+// only reads has 6.9.  From 16 query heads a key head on, products are as long as the loads (8-bit caches: 149 us with 16, 140 with 8, 136 with 4).
 // Short calls take two launches and the dependent loads length, page, keys: 1000 tokens of one sequence 8 us.
 static constexpr int kUnit = 64;           // tokens that the four wavefronts of a block take together
 static constexpr float kLazy = 10.0f;      // a running maximum moves on when a score is above it by so many powers of two
