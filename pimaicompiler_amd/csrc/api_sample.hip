@@ -9,20 +9,20 @@ using namespace pimhip;
 namespace
 {
 // Values are counted (16-bit rows) where a row may need it, with a top_p or a top_k above the list's: it takes a CU for one row and some 15 us, whatever
-// the row's length.  A nucleus of half of 32000 tokens, in us, counted and not: 64 rows 40 and 53, of 16000 38 and 35; a peaked one of 32000
-// 27 and 27.  Where CUs have several rows each: 512 rows of 32000 82 and 80, of 64000 99 and 135, peaked ones 72 and 54.
+// the row's length.  A nucleus of half of 32000 tokens, in us, counted and not: 64 rows 40 and 44, of 16000 38 and 30; a peaked one of 32000
+// 27 and 25.  Where CUs have several rows each: 512 rows of 32000 80 and 73, of 64000 98 and 121, peaked ones 68 and 53.
 constexpr int kCountFrom = 24576, kCountFromMany = 49152;
 
-// The first pass by all CUs, in a launch of its own, where rows are few and long.  In us, without and with it: one row of 131072 with nothing cut off 38 and 16,
-// with top_k 40 26.7 and 20.4, with a peaked nucleus 44 and 22, a flat one 58 and 72 (it is counted after all; in fp32 131 and 111); one of 32000 with top_k
-// 40 17.0 and 19.1; 64 rows of 100003 34.5 and 23.5, with top_k 40 26.2 and 24.7; 128 of them with top_k 40 27 and 28.7, of 200000, whose pieces' largest
-// values do not fit into LDS, 45 and 35.
+// The first pass by all CUs, in a launch of its own, where rows are few and long.  In us, without and with it: one row of 131072 with nothing cut off 36 and 15,
+// with top_k 40 24.5 and 19.4, with a peaked nucleus 43 and 19, a flat one 57 and 68 (it is counted after all; in fp32 128 and 107); one of 32000 with top_k
+// 40 15.8 and 17.8; 64 rows of 100003 33 and 22, with top_k 40 23.7 and 22.7; 128 of them with top_k 40 24 and 26, of 200000, whose pieces' largest
+// values do not fit into LDS, 43 and 33.
 constexpr int kPartsFrom = 49152;
 
-// Threads of a block.  One row a CU: 256 while that is enough (4000 tokens: 13.7 us with any number), 512, and 1024 for long ones (64 rows
-// with top_k 40, of 16000: 15.8 and 16.5 us with 512 and 1024; of 100003: 27.9 and 25.5).  Two rows of 512 threads share a CU (512 rows of 32000: 26.0 with 512,
-// 26.7 with 256, 38 with 1024), four of 256 as long as their largest values leave LDS for that (2000 rows of 8000: 41.7 with 256, 64.8 with 512; 1024 of
-// 32000 38.3 and 44.0, of 64000 69.7 and 62.4).
+// Threads of a block.  One row a CU: 256 while that is enough (4000 tokens: 13.3 us, with 512 13.0, with 1024 14.5), 512, and 1024 for long ones (64 rows
+// with top_k 40, of 16000: 14.4 and 15.6 us with 512 and 1024; of 100003: 26.7 and 23.9).  Two rows of 512 threads share a CU (512 rows of 32000: 22.4 with 512,
+// 24.6 with 256, 34 with 1024), four of 256 as long as their largest values leave LDS for that (2000 rows of 8000: 36 with 256, 58 with 512; 1024 of
+// 32000 32 and 39, of 64000 65 and 57).
 int threads_of(int64_t rows, int64_t vocab, int num_cus)
 {
     constexpr int kMiddle = 32768;
