@@ -969,6 +969,8 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
                     aim = sample_target(u, whole);
                 }
             }
+            // The list has no room: all of the block have read how many there are before the next pass begins to count.
+            __syncthreads();
         }
 
         // ---- the row in place of the list: the smallest value that stays ----

@@ -1,0 +1,84 @@
+"""What a draw may be, asked of every row, near an edge or not: a token that stays, has a weight, and whose share holds the number."""
+import math
+
+import pytest
+import torch
+
+from test_sampling_gpu import DTYPES, f32
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+INF = math.inf
+
+
+def kept_of(x, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(the tokens that stay in the order of indices, their weights) of one row, in 64 bits, and how near top_p is to the edge of what stays."""
+    x = x.double()
+    order = torch.sort(x, descending=True, stable=True).indices
+    w, near = torch.exp((x - x.max()) / f32(temperature)), 1.0
+    kept = order[:top_k] if top_k > 0 else order
+    if top_p < 1:
+        whole = w[kept].sum()
+        before = torch.cumsum(w[kept], 0) - w[kept]
+        near = float(((before - f32(top_p) * whole).abs() / whole).min())
+        kept = kept[:max(1, int((before < f32(top_p) * whole).sum()))]
+    if min_p > 0:
+        kept = kept[w[kept] >= f32(min_p)]
+    kept = torch.sort(kept).values
+    return kept, w[kept], near
+
+
+def unit_of(V):
+    """What weights are rounded to, of the largest: V of them fit into 62 bits."""
+    shift = 45
+    while V > 1 << (62 - shift):
+        shift -= 1
+    return 2.0**-shift
+
+
+def drawn(ops, x, u, **settings):
+    """tokens and logp of a call, each looked at.  A running sum is off by 2^-36 of the whole (borders are moved by that), by 2^-38 of itself (weights) and by half a unit for
+    each token; so is the whole.  Returns how many rows were compared (top_p may be as near as that to an edge of what stays)."""
+    tokens, logp = ops.sample_tokens(x.to(DEV), u.to(DEV), **settings)
+    compared, cache = 0, {}
+    for r in range(x.size(0)):
+        same = x[r].numpy().tobytes() if x.dtype != torch.bfloat16 else x[r].view(torch.int16).numpy().tobytes()
+        if same not in cache:
+            cache[same] = kept_of(x[r], **settings)
+        kept, w, near = cache[same]
+        whole = float(w.sum())
+        off = 2.0**-36 + 2 * 2.0**-38 + x.size(1) * unit_of(x.size(1)) / 2 / whole
+        token, lp = int(tokens[r]), float(logp[r])
+        assert 0 <= token < x.size(1), (r, token)
+        if near <= 2 * off:
+            continue
+        at = int(torch.searchsorted(kept, token))
+        assert at < len(kept) and int(kept[at]) == token, (r, token, "does not stay")
+        assert float(w[at]) > 0, (r, token, "has no weight")
+        edge = float(w[:at + 1].sum())
+        number = min(max(float(u[r]), 0.0), 1 - 2.0**-24)
+        assert edge - float(w[at]) <= (number + 2 * off) * whole and edge >= (number - 2 * off) * whole, (r, token, number, edge / whole)
+        want = math.log(float(w[at]) / whole)
+        assert abs(lp - want) <= abs(want) * 2.0**-24 + 2 * off + 1e-9, (r, lp, want)
+        compared += 1
+    return compared
+
+
+# (rows, V): 256, 512 and 1024 threads a row, many rows, 16-bit rows that may be counted, the first pass by all CUs, the largest
+SIZES = [(6, 6147), (6, 3001), (6, 8196), (6, 32000), (2000, 8000), (300, 50000), (6, 60000), (6, 131072), (2, 300007)]
+
+
+@pytest.mark.parametrize("rows, V", SIZES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_more_tokens_than_a_list_with_min_p_alone(ops, rows, V, dtype):
+    """Nothing but min_p, which thousands of tokens pass: the list is given up and the row walked, with every wavefront's segments in the sum."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.stack([torch.full((V,), 2.0), torch.randn(V, generator=g), torch.arange(V) * (3.0 / V), torch.where(torch.rand(V, generator=g) < 0.3, 1.0, -INF)]).to(dtype)
+    x = x.repeat(-(-rows // 4), 1)[:rows]
+    u = torch.rand(rows, generator=g)
+    assert drawn(ops, x, u, min_p=1e-3) == rows
+    on = x.to(DEV), u.to(DEV)
+    first = ops.sample_tokens(*on, min_p=1e-3)
+    for _ in range(20):
+        again = ops.sample_tokens(*on, min_p=1e-3)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
