@@ -296,7 +296,8 @@ struct SampleRow : SampleTokens<T, THREADS> {
     }
 
     // The first of a[0 .. n) at whose end base + the running sum reaches `target` (that of all, where it is never reached); the sum before it
-    // in `before` (base included), its own in `amount`.  All of the block call it; some number is not 0.
+    // in `before` (base included), its own in `amount`.  All of the block call it; where all numbers are 0 nothing is found,
+    // and it returns what was found before.
     template <class A>
     __device__ __forceinline__ int find(const A* a, int n, uint64_t base, uint64_t target, uint64_t& before, uint64_t& amount) const
     {
@@ -996,21 +997,32 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
     // ---- the draw: the segment, then the value in it, one each thread ----
     const uint64_t aim = sample_target(u, whole);
     const int segment = row.find(bins, segments, 0, aim, before, amount);
-    const uint64_t in_front = before;
-    __syncthreads();
+    // A segment's sum is rounded as one, its values one by one.  Where they come to less the last of them that has a unit is drawn.  Where each is below half a unit none
+    // has any, and they are looked at again in 2^-40 of a unit (they are below 2^39 of these then, and one of them above 2^27: 2048 come to half a unit at
+    // least), of which the target's place in the segment is as many for each unit.
+    uint64_t in_front = before, target = aim;
+    int in = -1;
 #pragma unroll 1
-    for (int i = this_thread(); i < kSegment; i += THREADS) {
-        const int at = segment * kSegment + i;
-        uint64_t units = 0;
-        if (at < V) {
-            const float v = (float)row.x[at];
-            const double w = weight(v);
-            if (v > smallest || (v == smallest && at <= last)) units = weight.units(w);
+    for (int pass = 0; pass < 2 && in < 0; ++pass) {
+        __syncthreads();
+#pragma unroll 1
+        for (int i = this_thread(); i < kSegment; i += THREADS) {
+            const int at = segment * kSegment + i;
+            uint64_t units = 0;
+            if (at < V) {
+                const float v = (float)row.x[at];
+                const double w = weight(v);
+                if (v > smallest || (v == smallest && at <= last)) units = weight.units(w);
+            }
+            bins[i] = units;
         }
-        bins[i] = units;
+        if (tid == 0) sh.found = -1;
+        in = row.find(bins, kSegment, in_front, target, before, amount);
+        target = ((aim - in_front - 1) << 40) + 1;
+        in_front = 0;
+        weight.unit *= 0x1p40;
     }
-    // (a segment's sum may be some units more than its values': its last value is drawn then)
-    const int at = segment * kSegment + row.find(bins, kSegment, in_front, aim, before, amount);
+    const int at = segment * kSegment + in;
     if (tid == 0) answer(at, log_share((float)row.x[at]));
 }
 

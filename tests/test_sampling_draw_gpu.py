@@ -64,6 +64,14 @@ def drawn(ops, x, u, **settings):
     return compared
 
 
+def low(V, at, gap, dtype, masked=()):
+    """One token of weight 1 at `at`, the others `gap` below it, those of `masked` out."""
+    x = torch.full((V,), -gap)
+    x[list(masked)] = -INF
+    x[at] = 0.0
+    return x.to(dtype)
+
+
 # (rows, V): 256, 512 and 1024 threads a row, many rows, 16-bit rows that may be counted, the first pass by all CUs, the largest
 SIZES = [(6, 6147), (6, 3001), (6, 8196), (6, 32000), (2000, 8000), (300, 50000), (6, 60000), (6, 131072), (2, 300007)]
 
@@ -82,3 +90,19 @@ def test_more_tokens_than_a_list_with_min_p_alone(ops, rows, V, dtype):
     for _ in range(20):
         again = ops.sample_tokens(*on, min_p=1e-3)
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.parametrize("rows, V", SIZES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_segments_whose_values_are_less_than_half_a_unit_each(ops, rows, V, dtype):
+    """Tokens of 2^-47 to 2^-56 of the largest: one by one nothing, together some units.  A number that falls there draws one of them, never one that is out,
+    nor one behind the row."""
+    kinds = [low(V, V // 2 + 900, 32.5, dtype, masked=[0]), low(V, 0, 32.5, dtype), low(V, V - 1, 36.0, dtype, masked=range(3)), low(V, 2500, 38.0, dtype, masked=[0, 1, V - 1]),
+             low(V, V // 2 + 900, 33.0, dtype, masked=range(1, min(V // 2, 5000), 2)), low(V, 2000, 32.0, dtype, masked=range(V - 3, V))]
+    numbers = [0.0, 1.0 - 2.0**-24, 2.0**-60, 0.5, 2.0**-24, -1.0]
+    for i, u in enumerate(numbers):
+        x = torch.stack([kinds[(r + i) % 6] for r in range(min(rows, 12))])
+        x = x.repeat(-(-rows // x.size(0)), 1)[:rows]
+        for settings in ({}, {"top_k": V - 2}, {"min_p": 1e-17}, {"temperature": 0.5}, {"top_k": V - 5, "min_p": 1e-18}):
+            scaled = (x.float() * settings.get("temperature", 1.0)).to(dtype)
+            assert drawn(ops, scaled, torch.full((rows,), u), **settings) == rows
