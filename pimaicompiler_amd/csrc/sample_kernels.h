@@ -103,6 +103,7 @@ struct SampleAsked {
         u = a.uniform[r];
         top_k = a.top_ks ? a.top_ks[r] : a.top_k;
         unfit = !(temperature >= 0.0f && temperature < __builtin_inff()) || top_p != top_p || min_p != min_p || u != u;
+        u = fminf(fmaxf(u, 0.0f), 0x1.fffffep-1f);  // (the nearest in [0, 1))
         greedy = unfit || temperature == 0.0f || top_k == 1 || top_p <= 0.0f;
         cut_k = top_k > 0 && top_k < a.V;
         cut_p = top_p < 1.0f;
@@ -129,7 +130,7 @@ struct SampleWeight {
 static constexpr double kBorder = 0x1p-36;
 __device__ __forceinline__ uint64_t sample_target(float u, uint64_t whole)
 {
-    const uint64_t t = (uint64_t)((double)(u < 0.0f ? 0.0f : u) * (1.0 + kBorder) * (double)whole);
+    const uint64_t t = (uint64_t)((double)u * (1.0 + kBorder) * (double)whole);
     return (t < whole ? t : whole - 1) + 1;
 }
 __device__ __forceinline__ uint64_t nucleus_target(float top_p, uint64_t whole)

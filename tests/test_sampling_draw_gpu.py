@@ -106,3 +106,26 @@ def test_segments_whose_values_are_less_than_half_a_unit_each(ops, rows, V, dtyp
         for settings in ({}, {"top_k": V - 2}, {"min_p": 1e-17}, {"temperature": 0.5}, {"top_k": V - 5, "min_p": 1e-18}):
             scaled = (x.float() * settings.get("temperature", 1.0)).to(dtype)
             assert drawn(ops, scaled, torch.full((rows,), u), **settings) == rows
+
+
+@pytest.mark.parametrize("rows, V", SIZES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_numbers_outside_of_their_range(ops, rows, V, dtype):
+    """They count as the nearest in it, 0 and 1 - 2^-24: the last tokens, which together have less than 2^-24 of the whole, are not drawn by 1."""
+    kinds = [low(V, V // 3, 20.0 + math.log(V), dtype, masked=[0]), low(V, 0, 20.0 + math.log(V), dtype), low(V, 5, 40.0, dtype, masked=range(V // 2, V)),
+             2 * torch.randn(V, generator=torch.Generator().manual_seed(V)).to(dtype)]
+    x = torch.stack([kinds[r % 4] for r in range(min(rows, 8))])
+    for settings in ({}, {"top_k": 30}, {"top_k": 400}, {"top_k": V - 2}, {"min_p": 1e-13}, {"top_p": 0.97}):
+        ends = [drawn_at(ops, x, u, settings) for u in (0.0, 1.0 - 2.0**-24)]
+        for u in (1.0, 1.0 + 2.0**-23, 7.0, 1e30, INF):
+            got = drawn_at(ops, x, u, settings)
+            assert torch.equal(got[0], ends[1][0]) and torch.equal(got[1], ends[1][1])
+        for u in (-0.0, -1e-30, -5.0, -INF):
+            got = drawn_at(ops, x, u, settings)
+            assert torch.equal(got[0], ends[0][0]) and torch.equal(got[1], ends[0][1])
+        if settings.get("top_p", 1.0) == 1.0:
+            assert drawn(ops, x, torch.full((x.size(0),), 1.0), **settings) == x.size(0)
+
+
+def drawn_at(ops, x, u, settings):
+    return ops.sample_tokens(x.to(DEV), torch.full((x.size(0),), u, device=DEV), **settings)
