@@ -86,32 +86,36 @@ class PagedCache:
         """A deep copy, or one read from a file, is made of its own tensors: what the native calls read it through holds addresses."""
         return PagedCache, (self.k_pages, self.v_pages, self.k_scale, self.v_scale)
 
-    def _tokens(self, name, t, heads=None):
-        """[tokens, heads, head_dim] of one of the types that go with the cache, the values of a head next to each other."""
+    def _require_tokens(self, name, t, heads=None):
+        """[tokens, heads, head_dim] of one of the types that go with the cache."""
         _require(name, t, (torch.float16, torch.bfloat16))
         if self.dtype != torch.float8_e4m3fn and t.dtype != self.dtype:
             raise NNRuntimeException(f"{name} is {t.dtype}, the cache {self.dtype}")
         if t.dim() != 3 or t.size(2) != self.head_dim or heads is not None and t.size(1) != heads or t.device != self.device:
             raise NNRuntimeException(f"{name} must be [tokens, {'heads' if heads is None else heads}, {self.head_dim}] on {self.device}, got {tuple(t.shape)} on {t.device}")
         _require_no_gradient(t)
-        return t if t.stride(2) == 1 else t.contiguous()
 
-    def _batch(self, page_table, lengths):
+    def _require_batch(self, page_table, lengths):
         for name, t, dims in (("page_table", page_table, 2), ("lengths", lengths, 1)):
             _require(name, t, (torch.int32,))
             if t.dim() != dims or t.device != self.device:
                 raise NNRuntimeException(f"{name} must have {dims} dimension{'s' if dims > 1 else ''} on {self.device}, got {tuple(t.shape)} on {t.device}")
         if page_table.size(0) != lengths.size(0) or page_table.size(1) < 1:
             raise NNRuntimeException(f"page_table must be [{lengths.size(0)}, 1 or more] for {lengths.size(0)} lengths, got {tuple(page_table.shape)}")
+
+    # What the native calls take of tensors that were looked at, and the tensors it points into.  Copies are made here, so it is called inside _Launch: on the
+    # stream that reads them.
+    @staticmethod
+    def _batch(page_table, lengths):
         if page_table.stride(1) != 1 and page_table.size(1) > 1 or page_table.size(0) > 1 and page_table.stride(0) < page_table.size(1):
             page_table = page_table.contiguous()
         lengths = lengths.contiguous()
-        batch = L.PagedBatch(page_table.data_ptr(), lengths.data_ptr(), page_table.stride(0), lengths.size(0), page_table.size(1))
-        return batch, page_table, lengths
+        return L.PagedBatch(page_table.data_ptr(), lengths.data_ptr(), page_table.stride(0), lengths.size(0), page_table.size(1)), (page_table, lengths)
 
     @staticmethod
     def _rows(t):
-        return L.PagedRows(t.data_ptr(), t.stride(0), t.stride(1))
+        t = t if t.stride(2) == 1 else t.contiguous()   # (the values of a head next to each other)
+        return L.PagedRows(t.data_ptr(), t.stride(0), t.stride(1)), t
 
     def append(self, k, v, page_table, lengths, starts=None, q=None, rotary=None, interleaved=False, stream=None):
         """Stores k and v [tokens, kv_heads, head_dim] (fp16 or bf16, the cache's type where that is not in 8 bits).
@@ -127,25 +131,25 @@ class PagedCache:
         native = _native().fast_paged_append(self._at, self._device_index, k, v, page_table, lengths, starts, q, rotary, interleaved) if stream is None else None
         if native is not None:
             return _result(native) if type(native) is int else native[0]
-        k, v = self._tokens("k", k, self.kv_heads), self._tokens("v", v, self.kv_heads)
+        self._require_tokens("k", k, self.kv_heads)
+        self._require_tokens("v", v, self.kv_heads)
         if v.shape != k.shape or v.dtype != k.dtype:
             raise NNRuntimeException(f"k and v differ: {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype}")
         tokens = k.size(0)
         if q is not None:
             if rotary is None:
                 raise NNRuntimeException("q is only turned: it goes with rotary")
-            q = self._tokens("q", q)
+            self._require_tokens("q", q)
             if q.size(0) != tokens or q.dtype != k.dtype or q.size(1) < 1:
                 raise NNRuntimeException(f"q must be [{tokens}, 1 or more, {self.head_dim}] in {k.dtype}, got {tuple(q.shape)} in {q.dtype}")
-        batch, page_table, lengths = self._batch(page_table, lengths)
+        self._require_batch(page_table, lengths)
+        sequences = lengths.size(0)
         if starts is not None:
             _require("starts", starts, (torch.int32,))
-            if tuple(starts.shape) != (batch.sequences + 1,) or starts.device != self.device:
-                raise NNRuntimeException(f"starts must be [{batch.sequences + 1}] on {self.device}, got {tuple(starts.shape)} on {starts.device}")
-            starts = starts.contiguous()
-        elif tokens != batch.sequences:
-            raise NNRuntimeException(f"{tokens} tokens for {batch.sequences} sequences need starts")
-        dim = rows = pitch = 0
+            if tuple(starts.shape) != (sequences + 1,) or starts.device != self.device:
+                raise NNRuntimeException(f"starts must be [{sequences + 1}] on {self.device}, got {tuple(starts.shape)} on {starts.device}")
+        elif tokens != sequences:
+            raise NNRuntimeException(f"{tokens} tokens for {sequences} sequences need starts")
         if rotary is not None:
             _require("rotary", rotary, (torch.float32,))
             _require_no_gradient(rotary)
@@ -153,14 +157,23 @@ class PagedCache:
                 raise NNRuntimeException(f"rotary must be [positions, an even number up to {self.head_dim}] on {self.device}, got {tuple(rotary.shape)} on {rotary.device}")
             if rotary.size(0) < page_table.size(1) * self.page_size:
                 raise NNRuntimeException(f"rotary has {rotary.size(0)} positions, the page table room for {page_table.size(1) * self.page_size}")
-            if rotary.stride(1) != 1 or rotary.stride(0) < rotary.size(1):
-                rotary = rotary.contiguous()
-            rows, dim, pitch = rotary.size(0), rotary.size(1), rotary.stride(0)
         ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
         with _Launch(self.device, stream, k, v, q, page_table, lengths, starts, rotary, self.k_pages, self.v_pages, self.k_scale, self.v_scale) as handle:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device) if q is not None else None
-            _check(L.load().pimhip_paged_append(self._at, ctypes.byref(batch), ptr(starts), tokens, ctypes.byref(self._rows(k)), ctypes.byref(self._rows(v)),
-                                                ctypes.byref(self._rows(q)) if q is not None else None, q.size(1) if q is not None else 0, ptr(out),
+            batch, batch_tensors = self._batch(page_table, lengths)
+            (k_rows, k), (v_rows, v) = self._rows(k), self._rows(v)
+            q_rows, out = None, None
+            if q is not None:
+                q_rows, q = self._rows(q)
+                out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            if starts is not None:
+                starts = starts.contiguous()
+            dim = rows = pitch = 0
+            if rotary is not None:
+                if rotary.stride(1) != 1 or rotary.stride(0) < rotary.size(1):
+                    rotary = rotary.contiguous()
+                rows, dim, pitch = rotary.size(0), rotary.size(1), rotary.stride(0)
+            _check(L.load().pimhip_paged_append(self._at, ctypes.byref(batch), ptr(starts), tokens, ctypes.byref(k_rows), ctypes.byref(v_rows),
+                                                ctypes.byref(q_rows) if q is not None else None, q.size(1) if q is not None else 0, ptr(out),
                                                 _CACHE_CODES[k.dtype], ptr(rotary), rows, pitch, dim, int(bool(interleaved)), handle))
         return out
 
@@ -176,20 +189,21 @@ class PagedCache:
         native = _native().fast_paged_attend(self._at, self._device_index, q, page_table, lengths, scale, window, lse) if stream is None else None
         if native is not None:
             return _result(native)
-        q = self._tokens("q", q)
-        batch, page_table, lengths = self._batch(page_table, lengths)
+        self._require_tokens("q", q)
+        self._require_batch(page_table, lengths)
         heads = q.size(1)
-        if q.size(0) != batch.sequences or heads < 1 or heads % self.kv_heads:
-            raise NNRuntimeException(f"q must be [{batch.sequences}, a multiple of {self.kv_heads}, {self.head_dim}], got {tuple(q.shape)}")
+        if q.size(0) != lengths.size(0) or heads < 1 or heads % self.kv_heads:
+            raise NNRuntimeException(f"q must be [{lengths.size(0)}, a multiple of {self.kv_heads}, {self.head_dim}], got {tuple(q.shape)}")
         if not isinstance(window, int) or not 0 <= window <= 2**31 - 1 or not isinstance(scale, (int, float)) or not abs(scale) < 3.4e38:
             raise NNRuntimeException(f"window={window!r} must be a whole number from 0 on, scale={scale!r} a finite number")
         lib = L.load()
         with _Launch(self.device, stream, q, page_table, lengths, self.k_pages, self.v_pages, self.k_scale, self.v_scale) as handle:
+            (batch, batch_tensors), (rows, q) = self._batch(page_table, lengths), self._rows(q)
             n = ctypes.c_uint64()
             _check(lib.pimhip_paged_attend_workspace_bytes(self._at, ctypes.byref(batch), heads, ctypes.byref(n)))
             out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
             sums = torch.empty(q.shape[:2], dtype=torch.float32, device=self.device) if lse else None
             workspace = torch.empty(n.value, dtype=torch.uint8, device=self.device)
-            _check(lib.pimhip_paged_attend(self._at, ctypes.byref(batch), ctypes.byref(self._rows(q)), heads, _CACHE_CODES[q.dtype], scale, window,
+            _check(lib.pimhip_paged_attend(self._at, ctypes.byref(batch), ctypes.byref(rows), heads, _CACHE_CODES[q.dtype], scale, window,
                                            out.data_ptr(), sums.data_ptr() if lse else None, workspace.data_ptr(), handle))
         return (out, sums) if lse else out
