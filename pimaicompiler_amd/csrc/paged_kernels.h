@@ -615,8 +615,8 @@ __global__ __launch_bounds__(256, attend_waves(NC, HT)) void paged_attend_kernel
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             b[r] = __builtin_bit_cast(unsigned int, p[mt][r]);
-                            // (what is left, never 0: an infinite value times it stays one)
-                            p[mt][r] = fmaxf(p[mt][r] - __builtin_bit_cast(float, b[r] & 0xffff0000u), 0x1p-126f);
+                            // (what is left, 2^-126 at least: an infinite value times it stays one.  But nothing of a weight that is 0: its value has no part)
+                            p[mt][r] = __builtin_amdgcn_fmed3f(p[mt][r] - __builtin_bit_cast(float, b[r] & 0xffff0000u), 0x1p-126f, p[mt][r]);
                         }
                         part[i][mt] = operand(halves(b[0], b[1], true), halves(b[2], b[3], true));
                     }
