@@ -53,7 +53,6 @@ __device__ __forceinline__ unsigned long long group_max_u64(unsigned long long k
 }
 
 // ---- 64-bit numbers over the lanes of a wavefront, on DPP (a generic shuffle of 64 bits takes two trips through the LDS crossbar) ----
-static constexpr int kDppQuadReverse = 0x1B;    // quad_perm:[3,2,1,0]
 static constexpr int kDppRowShr1 = 0x111;       // row_shr:1 (and on: 2, 4, 8)
 static constexpr int kDppRowBcast15 = 0x142;    // lane 15 of each row to the row behind it
 static constexpr int kDppRowBcast31 = 0x143;    // lane 31 to the two rows behind it
@@ -113,16 +112,5 @@ __device__ __forceinline__ unsigned long long wave_max_u64(unsigned long long v)
         best = o > best ? o : best;
     }
     return best;
-}
-// The value of lane l ^ j, j a power of two that all lanes have in common.
-__device__ __forceinline__ uint64_t lane_xor_u64(uint64_t v, int j)
-{
-    switch (j) {
-    case 1: return dpp_u64<kDppQuadXor1>(v);
-    case 2: return dpp_u64<kDppQuadXor2>(v);
-    case 4: return dpp_u64<kDppQuadReverse>(dpp_u64<kDppRowHalfMirror>(v));
-    case 8: return dpp_u64<kDppRowRor8>(v);
-    default: return __shfl_xor(v, j);
-    }
 }
 }  // namespace pimhip
