@@ -169,9 +169,10 @@ class PagedCache:
                 starts = starts.contiguous()
             dim = rows = pitch = 0
             if rotary is not None:
-                if rotary.stride(1) != 1 or rotary.stride(0) < rotary.size(1):
+                if rotary.stride(1) != 1 or rotary.size(0) > 1 and rotary.stride(0) < rotary.size(1):
                     rotary = rotary.contiguous()
-                rows, dim, pitch = rotary.size(0), rotary.size(1), rotary.stride(0)
+                rows, dim = rotary.shape
+                pitch = rotary.stride(0) if rows > 1 else dim   # (one row may have any stride)
             _check(L.load().pimhip_paged_append(self._at, ctypes.byref(batch), ptr(starts), tokens, ctypes.byref(k_rows), ctypes.byref(v_rows),
                                                 ctypes.byref(q_rows) if q is not None else None, q.size(1) if q is not None else 0, ptr(out),
                                                 _CACHE_CODES[k.dtype], ptr(rotary), rows, pitch, dim, int(bool(interleaved)), handle))

@@ -1,4 +1,5 @@
-"""A paged cache's calls on a stream that is asked for, with inputs that have to be copied: the copies are that stream's work, whatever the current one is busy with."""
+"""A paged cache's calls on a stream that is asked for, with inputs that have to be copied: the copies are that stream's work, whatever the current one is busy with.  And
+angles of one position, whose stride may be any."""
 import pytest
 import torch
 
@@ -69,3 +70,19 @@ def test_append(ops, held, as_handle):
     assert torch.equal(got, want.cpu())
     assert all(torch.equal(x, y.view(raw).cpu()) for x, y in zip(pages, (a.k_pages, a.v_pages)))
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("stride", [1, 3, 16, 40])
+def test_angles_of_one_position(ops, stride):
+    """A cache with room for one token: its angles are one row."""
+    k = torch.randn(2, 1, 16).half().to(DEV)
+    table, n = torch.tensor([[1], [0]], dtype=torch.int32, device=DEV), torch.ones(2, dtype=torch.int32, device=DEV)
+    c, d = (ops.PagedCache(*(torch.zeros(2, 1, 1, 16, dtype=torch.float16, device=DEV) for _ in range(2))) for _ in range(2))
+    angles = torch.rand(16, device=DEV)
+    want = c.append(k, k, table, n, q=k, rotary=angles.view(1, 16))
+    one = torch.cat([angles, torch.zeros(40, device=DEV)]).as_strided((1, 16), (stride, 1))
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    got = d.append(k, k, table, n, q=k, rotary=one, stream=s)
+    s.synchronize()
+    assert torch.equal(got, want) and torch.equal(c.k_pages, d.k_pages)
