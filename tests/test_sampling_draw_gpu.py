@@ -36,15 +36,16 @@ def unit_of(V):
     return 2.0**-shift
 
 
-def drawn(ops, x, u, **settings):
+def drawn(ops, x, u, some=None, **settings):
     """tokens and logp of a call, each looked at.  A running sum is off by 2^-36 of the whole (borders are moved by that), by 2^-38 of itself (weights) and by half a unit for
-    each token; so is the whole.  Returns how many rows were compared (top_p may be as near as that to an edge of what stays)."""
-    tokens, logp = ops.sample_tokens(x.to(DEV), u.to(DEV), **settings)
+    each token; so is the whole.  Returns how many rows (all, or those of `some`) were compared: top_p may be as near as that to an edge of what stays."""
+    tokens, logp = ops.sample_tokens(x.to(DEV), u.to(DEV), **{k: v.to(DEV) if isinstance(v, torch.Tensor) else v for k, v in settings.items()})
     compared, cache = 0, {}
-    for r in range(x.size(0)):
-        same = x[r].numpy().tobytes() if x.dtype != torch.bfloat16 else x[r].view(torch.int16).numpy().tobytes()
+    for r in range(x.size(0)) if some is None else some:
+        one = {k: v[r].item() if isinstance(v, torch.Tensor) else v for k, v in settings.items()}
+        same = (x[r].numpy().tobytes() if x.dtype != torch.bfloat16 else x[r].view(torch.int16).numpy().tobytes()), tuple(one.values())
         if same not in cache:
-            cache[same] = kept_of(x[r], **settings)
+            cache[same] = kept_of(x[r], **one)
         kept, w, near = cache[same]
         whole = float(w.sum())
         off = 2.0**-36 + 2 * 2.0**-38 + x.size(1) * unit_of(x.size(1)) / 2 / whole
@@ -129,3 +130,25 @@ def test_numbers_outside_of_their_range(ops, rows, V, dtype):
 
 def drawn_at(ops, x, u, settings):
     return ops.sample_tokens(x.to(DEV), torch.full((x.size(0),), u, device=DEV), **settings)
+
+
+# (rows, V): around 2^17 tokens, up to which weights are whole numbers of 2^-45, and far above it; with the first pass by all CUs, and without
+LONG = [(3, 131072), (3, 131073), (128, 131080), (129, 131073), (4, 300007), (3, 1 << 20), (3, (1 << 21) - 1), (3, 1 << 21)]
+
+
+@pytest.mark.parametrize("rows, V", LONG)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_long_rows_against_the_definition(ops, rows, V, dtype):
+    g = torch.Generator().manual_seed(V + rows)
+    x = 2.5 * torch.randn(rows, V, generator=g)
+    x = torch.where(torch.rand(rows, V, generator=g) < 0.001, x + 8, x)
+    x[torch.rand(rows, V, generator=g) < 0.05] = -INF
+    x, u = x.to(dtype), torch.rand(rows, generator=g)
+    u[0] = 0.0
+    some = [0, rows // 2, rows - 1]
+    each = dict(temperature=0.3 + torch.rand(rows, generator=g), top_k=torch.randint(0, 2000, (rows,), generator=g).int(), top_p=0.5 + 0.5 * torch.rand(rows, generator=g),
+                min_p=0.01 * torch.rand(rows, generator=g))
+    whole, near = ({}, {"top_k": 40}, {"top_k": V // 2}, {"min_p": 0.03}, {"min_p": 1e-4, "top_k": 900}), ({"top_p": 0.9}, {"top_k": 3000, "top_p": 0.97}, {"top_p": 0.7, "temperature": 0.4}, each)
+    for settings in whole:
+        assert drawn(ops, x, u, some, **settings) == 3
+    assert sum(drawn(ops, x, u, some, **settings) for settings in near) >= 10
