@@ -627,7 +627,8 @@ typedef struct PimHipPagedRows {
  * rotary_dim > 0: the first rotary_dim values of each key, and of each query q [tokens, q_heads, head_dim] (q may be NULL), are turned in pairs by
  * the token's position, in fp32: values i and rotary_dim / 2 + i, or 2 i and 2 i + 1 if interleaved, by angles[position, i] (cosines) and
  * angles[position, rotary_dim / 2 + i] (sines); angles has table_width * page_size rows at least.  Queries go to q_out [tokens, q_heads, head_dim],
- * zeros for a token that is nobody's or at no position.  k and v of the cache are different memory.
+ * zeros for a token that is nobody's or at no position.  k and v of the cache are different memory,
+ * and the rows of k, v and q are none of it.
  * 16-bit values are rounded once; 8-bit ones are x / scale, rounded once, saturating at 448.  Two tokens of a call that are given the same place
  * leave either's values there, each of eight by itself. */
 int pimhip_paged_append(const PimHipPagedCache* cache, const PimHipPagedBatch* batch, const int* starts, int64_t tokens, const PimHipPagedRows* k,
@@ -667,11 +668,12 @@ typedef struct PimHipSampleSettings {
  *   top_p < 1      of them those before which less than top_p of their sum has been reached, the first always;
  *   min_p > 0      of them those with w >= min_p.
  * tokens[row] (int64) is the first in the order of indices at which the running sum of w over what stayed exceeds uniform[row] times the whole,
- * logp[row] the logarithm of its share of it.  temperature 0: the first of the largest.  Weights are worked out to 2^-38 of themselves (2^-46 of the
- * largest for up to 2^17 tokens), sums are good to 2^-36, and a share that meets a border to within that is taken to meet it; equal calls give equal
- * results.
+ * logp[row] the logarithm of its share of it.  temperature 0: the first of the largest.  Weights are worked out to 2^-38 of themselves and rounded to whole
+ * numbers of 2^-45 of the largest for up to 2^17 tokens, of 2^-41 for 2^21; sums are good to 2^-36 and half such a number for each token, and a share that
+ * meets a border to within 2^-36 is taken to meet it.  Equal calls give equal results.
  * A row with a NaN or +inf, of a temperature that is negative, infinite or NaN, or of a NaN elsewhere in its settings or its number: token -1 and
- * logp NaN; a row of -inf alone: -1 and -inf.  A number outside of [0, 1) is taken as the nearest in it. */
+ * logp NaN; a row of -inf alone: -1 and -inf.  A number outside of [0, 1) is taken as the nearest in it, 0 or
+ * 1 - 2^-24. */
 int pimhip_sample_tokens(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t vocab, const float* uniform, const PimHipSampleSettings* settings,
                          int64_t* tokens, float* logp, void* workspace, void* stream);
 

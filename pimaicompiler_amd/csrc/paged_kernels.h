@@ -73,8 +73,10 @@ __device__ __forceinline__ const E* row_of(const AppendArgs& a, int t, int head)
 
 // A block is heads of one token, a thread ITEMS groups of eight values of it, all asked for at once: of a key (query) the eight that a rotation turns
 // them with beside them, out of the caches as a rule.  Values are asked for before the token's place is known, which takes three dependent loads: the
-// sequence, its length, the page.  Bound by the bytes where tokens are many (8001 of 32 query and 8 key heads of 128 in bfloat16, 199 MB: 48 us, 4.1 TB/s
-// where a copy has 4.8), else by those loads (one token: 4.2 us, a launch).
+// sequence, its length, the page.  Bound by the bytes where tokens are many (8001 of 32 query and 8 key heads of 128 in bfloat16, neighbouring pairs of half of a
+// head, 199 MB: 48 us, 4.1 TB/s where a copy has 4.8; into 8 bits 45), but by the angles and partners
+// read beside them where more is turned (neighbouring pairs of all of a head 56 us; halves of half a head 66, of all of it 90, into 8 bits 89), else by those loads
+// (one token: 4.2 us, a launch).
 template <class T, bool FP8, bool INTERLEAVED, int ITEMS>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
 {

@@ -19,7 +19,7 @@
 // Bound by w: 25 vector instructions a token, 13 us for the 64000 tokens a CU has of 512 rows of 32000 (fp32, nothing cut off: 27 us in all; the
 // bytes take 10).  256 rows of 131072 in bfloat16 whose nucleus holds half of them: 73 us, the counts 20 (LDS atomics), the last pass's w 33.  Reading
 // w out of a table in LDS there takes as long as working it out (30 us for 131072 gathers a CU).  64 rows of 100003 with settings of their own: 29;
-// one row of 32000 with top_k and top_p: 13.4, of 131072 with top_k 19, code that is run once and the dependent steps.
+// one row of 32000 with top_k and top_p: 13.6, of 131072 with top_k 18.5, code that is run once and the dependent steps.
 // Code is kept short, loops as loops: what one row takes is walked through once and comes cold out of the instruction cache.  (The same steps
 // unrolled, 117 to 177 KB a kernel, took 17 us for one row of 32000 and 69 for 256 of 131072.)
 #pragma once
@@ -140,7 +140,7 @@ __device__ __forceinline__ uint64_t nucleus_target(float top_p, uint64_t whole)
 }
 
 // The thread's number, asked for anew: what is made of it is made where it is used, not at the kernel's start and kept in registers (24 to 53 of them spilled
-// so, 25 to 87 MB written by a call: 512 rows of 32000 30.4 us, now 26.7).
+// so, 25 to 87 MB written by a call; now 0 to 14, 10 MB for 512 rows of 32000, 30.4 us then and 27 now, and 19 for 2000 of 8000).
 __device__ __forceinline__ int this_thread()
 {
     int t = (int)threadIdx.x;
@@ -868,7 +868,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleArgs a)
                 constexpr int kEach = kListMost / THREADS, kPer = kBins / THREADS;
                 unsigned int* const counts = row.ties;                               // [kBins + 1]
                 unsigned short* const members = reinterpret_cast<unsigned short*>(counts + kBins + 2);  // [kListMost]: list entries, bucket by bucket
-                // The tokens' weights: kept where a CU has one block, worked out again where LDS for them would cost blocks (4096 rows of 500: 98 us, with them 115).
+                // The tokens' weights: kept where a CU has one block, worked out again where LDS for them would cost blocks (4096 rows of 500: 87 us, with them 96.5; 2000 of 8000 34.5 and 43).
                 uint64_t* const units = reinterpret_cast<uint64_t*>(members + kListMost);
                 auto units_of = [&](int i) { return Row::kUnitsKept ? units[i] : weight.units(weight(Row::value_in(sh.list[i]))); };
                 bool in[kEach];

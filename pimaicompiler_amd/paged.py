@@ -126,6 +126,7 @@ class PagedCache:
         position, in fp32, values i and n / 2 + i, or 2 i and 2 i + 1 if interleaved; so are those of q [tokens, heads, head_dim], the queries
         of the same tokens, which are returned (zeros for a token that is nobody's, or at no position of the table).  Without q the result is None.
 
+        k, v and q lie in other memory than the cache, whose keys and values lie in memory of their own (a cache of one tensor for both is refused).
         Values are rounded once; in 8 bits x / scale is, saturating at 448.  Two tokens of a call that are given the same place (a page that two
         sequences write) leave either's values there."""
         native = _native().fast_paged_append(self._at, self._device_index, k, v, page_table, lengths, starts, q, rotary, interleaved) if stream is None else None

@@ -26,9 +26,10 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     the whole.  temperature 0: the most likely token.
 
     temperature, top_p and min_p are numbers or fp32 tensors [..], top_k a whole number or an int32 tensor [..].  Weights are worked out and summed in
-    64 bits (shares are good to 2^-36, and one that meets a border to within that is taken to meet it), and equal calls give equal results.
+    64 bits, as whole numbers of 2^-45 of the largest for up to 2^17 tokens, of 2^-41 for 2^21: shares are good to 2^-36 and half such a number for each token,
+    and one that meets a border to within 2^-36 is taken to meet it.  Equal calls give equal results.
     A row of -inf alone gives token -1 and logp -inf; one with a NaN or +inf -1 and NaN, and so does a tensor's temperature that is negative,
-    infinite or NaN, or a NaN in its other settings or its number.  Numbers outside of [0, 1) count as the nearest in it."""
+    infinite or NaN, or a NaN in its other settings or its number.  Numbers outside of [0, 1) count as the nearest in it, 0 or 1 - 2^-24."""
     out = _native().fast_sample_tokens(logits, uniform, temperature, top_k, top_p, min_p) if stream is None else None
     if out is not None:
         return _result(out)
